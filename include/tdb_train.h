@@ -1,0 +1,58 @@
+/*
+ * tdb_train.h -- C ABI of the operators that training a DeBERTa-v2/v3 encoder needs beside tdb_attn.h's forward ones: dropout,
+ * LayerNorm (with dropout and residual in front of it) and attention with its gradient.
+ *
+ * Conventions are those of tdb_attn.h: plain pointers and sizes, element strides, buffers (workspaces too) of the caller, TDB_OK or a
+ * negative TDB_ERR_* code, nothing allocated, freed or synchronised, launches on the stream passed in.
+ *
+ * Random numbers.  `seed` is a device pointer to one 64-bit number.  A counter of four 32-bit words gives eight 16-bit numbers, the halves (low
+ * first) of the words that Philox-4x32 with seven rounds makes of it under the seed as its key (low word first).  A value is dropped where its
+ * number is below `threshold` (0 .. 65536, the probability in units of 2^-16; 0: nothing is dropped and `seed` is not read); the
+ * others are multiplied by 65536 / (65536 - threshold).  No mask is stored: whoever needs it again computes it again.
+ * A dropped value is 0 whatever it was, infinities and NaN included.
+ */
+#ifndef TDB_TRAIN_H
+#define TDB_TRAIN_H
+
+#include <stdint.h>
+
+#include "tdb_attn.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+/*
+ * y = dropout(x), n values back to back; also its backward pass (x: the gradient of y).  Value i has number i mod 8 of counter
+ * (i / 8, low word and high word, 0, 0).  x and y may be the same memory.
+ */
+int tdb_dropout(const void* x, void* y, int64_t n, int32_t dtype, int32_t threshold, const int64_t* seed, void* stream);
+
+/*
+ * LayerNorm over rows of `hidden` (1 .. 32768) values, z = dropout(x) + residual, y = (z - mean) / sqrt(var + eps) * weight + bias, var without
+ * Bessel's correction.  residual NULL: z = dropout(x).  The random numbers of row r, column c are those of value r * hidden + c in
+ * tdb_dropout.  weight and bias (both or neither NULL) have weight_dtype: that of x, or TDB_F32.  Strides are those of rows.
+ * Backward: dx, dresidual (NULL: not wanted, or no residual) from x, residual, dy; dweight and dbias (NULL: not wanted; both or neither) of weight_dtype.
+ * The statistics are computed again from x and residual.  workspace: tdb_norm_workspace() floats, where dweight is wanted.
+ */
+typedef struct tdb_norm_args {
+    int32_t dtype, weight_dtype, hidden, threshold;
+    int64_t rows;
+    float   eps;
+    int32_t reserved;
+    const void *x, *residual, *weight, *bias, *dy;
+    void *y, *dx, *dresidual, *dweight, *dbias;
+    float* workspace;
+    const int64_t* seed;
+    int64_t x_stride, residual_stride, dy_stride, y_stride, dx_stride, dresidual_stride;
+} tdb_norm_args;
+
+int tdb_norm_fwd(const tdb_norm_args* args, void* stream);
+int tdb_norm_bwd(const tdb_norm_args* args, void* stream);
+/* floats of workspace for a backward call of these sizes (host only; at most 2^31) */
+int64_t tdb_norm_workspace(int64_t rows, int32_t hidden);
+
+#ifdef __cplusplus
+}
+#endif
+#endif /* TDB_TRAIN_H */

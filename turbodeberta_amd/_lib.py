@@ -29,6 +29,7 @@ _VALUE_ERRORS = {-1, -2, -3, -4, -5, -6, -7, -8, -9}
 
 EXPORTS = ("tdb_version", "tdb_last_error", "tdb_attn_fwd_fixed", "tdb_attn_fwd_varlen", "tdb_bucket_table",
            "tdb_delta_table", "tdb_check_cu_seqlens", "tdb_set_workgroup_limit")
+TRAIN_EXPORTS = ("tdb_dropout", "tdb_norm_fwd", "tdb_norm_bwd", "tdb_norm_workspace")       # declared in include/tdb_train.h
 
 
 class PosArgs(C.Structure):
@@ -72,6 +73,18 @@ class VarlenArgs(C.Structure):
     ]
 
 
+class NormArgs(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("weight_dtype", C.c_int32), ("hidden", C.c_int32), ("threshold", C.c_int32),
+        ("rows", C.c_int64), ("eps", C.c_float), ("reserved", C.c_int32),
+        ("x", C.c_void_p), ("residual", C.c_void_p), ("weight", C.c_void_p), ("bias", C.c_void_p), ("dy", C.c_void_p),
+        ("y", C.c_void_p), ("dx", C.c_void_p), ("dresidual", C.c_void_p), ("dweight", C.c_void_p), ("dbias", C.c_void_p),
+        ("workspace", C.c_void_p), ("seed", C.c_void_p),
+        ("x_stride", C.c_int64), ("residual_stride", C.c_int64), ("dy_stride", C.c_int64), ("y_stride", C.c_int64),
+        ("dx_stride", C.c_int64), ("dresidual_stride", C.c_int64),
+    ]
+
+
 _lock = threading.Lock()
 _lib = None
 _host = None
@@ -104,6 +117,11 @@ def load() -> C.CDLL:
         lib.tdb_check_cu_seqlens.restype = C.c_int
         lib.tdb_set_workgroup_limit.argtypes = [C.c_int]
         lib.tdb_set_workgroup_limit.restype = C.c_int
+        lib.tdb_dropout.argtypes = [C.c_void_p, C.c_void_p, C.c_int64, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p]
+        for name in ("tdb_norm_fwd", "tdb_norm_bwd"):
+            getattr(lib, name).argtypes = [C.POINTER(NormArgs), C.c_void_p]
+        lib.tdb_norm_workspace.argtypes = [C.c_int64, C.c_int32]
+        lib.tdb_norm_workspace.restype = C.c_int64
         if lib.tdb_version() != ABI_VERSION:
             raise RuntimeError(f"libtdb_attn.so has ABI {lib.tdb_version()}, this package expects {ABI_VERSION}")
         _lib = lib

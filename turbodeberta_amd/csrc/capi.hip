@@ -12,13 +12,17 @@ namespace {
 
 thread_local char g_err[512] = "";
 
-int fail(int code, const char* fmt, ...) {
+}  // namespace
+
+int tdb_fail(int code, const char* fmt, ...) {
     va_list ap;
     va_start(ap, fmt);
     vsnprintf(g_err, sizeof(g_err), fmt, ap);
     va_end(ap);
     return code;
 }
+
+namespace {
 
 size_t elem_size(int dtype) { return dtype == TDB_F32 ? 4 : 2; }
 
@@ -35,13 +39,13 @@ constexpr double kMargin = 3e-5;
 
 int check_common(int dtype, int batch, int heads, int head_dim, int len, int causal, const void* q, const void* k,
                  const void* v, const void* o) {
-    if (dtype != TDB_F32 && dtype != TDB_BF16 && dtype != TDB_F16) return fail(TDB_ERR_DTYPE, "unknown dtype %d", dtype);
-    if (batch < 0 || heads < 1 || heads > 65535) return fail(TDB_ERR_SHAPE, "bad batch %d / heads %d", batch, heads);
-    if (head_dim < 8 || head_dim > 256 || head_dim % 8) return fail(TDB_ERR_SHAPE, "head_dim %d: need a multiple of 8 in [8, 256]", head_dim);
-    if (len < 1 || len > kMaxLen) return fail(TDB_ERR_SHAPE, "sequence length %d out of range [1, %d]", len, kMaxLen);
-    if (causal) return fail(TDB_ERR_CAUSAL, "causal attention is not supported");
-    if (!q || !k || !v || !o) return fail(TDB_ERR_NULL, "q, k, v and o must be non-NULL");
-    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o)) return fail(TDB_ERR_ALIGN, "q, k, v, o must be 16-byte aligned");
+    if (dtype != TDB_F32 && dtype != TDB_BF16 && dtype != TDB_F16) return tdb_fail(TDB_ERR_DTYPE, "unknown dtype %d", dtype);
+    if (batch < 0 || heads < 1 || heads > 65535) return tdb_fail(TDB_ERR_SHAPE, "bad batch %d / heads %d", batch, heads);
+    if (head_dim < 8 || head_dim > 256 || head_dim % 8) return tdb_fail(TDB_ERR_SHAPE, "head_dim %d: need a multiple of 8 in [8, 256]", head_dim);
+    if (len < 1 || len > kMaxLen) return tdb_fail(TDB_ERR_SHAPE, "sequence length %d out of range [1, %d]", len, kMaxLen);
+    if (causal) return tdb_fail(TDB_ERR_CAUSAL, "causal attention is not supported");
+    if (!q || !k || !v || !o) return tdb_fail(TDB_ERR_NULL, "q, k, v and o must be non-NULL");
+    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o)) return tdb_fail(TDB_ERR_ALIGN, "q, k, v, o must be 16-byte aligned");
     return TDB_OK;
 }
 
@@ -49,21 +53,21 @@ int check_pos(const tdb_pos_args& ps, int dtype, int len, bool varlen) {
     const bool any = ps.pos_key || ps.pos_query || ps.c2p_strip || ps.p2c_strip;
     if (!any) return TDB_OK;
     if ((ps.pos_key && ps.c2p_strip) || (ps.pos_query && ps.p2c_strip))
-        return fail(TDB_ERR_POSITION, "a term takes either a fused table or a strip, not both");
-    if (ps.span < 1 || ps.span > (1 << 20)) return fail(TDB_ERR_POSITION, "span %d out of range", ps.span);
-    if (!ps.delta_lut) return fail(TDB_ERR_POSITION, "delta_lut is required when a position term is on");
-    if (ps.lut_half < len - 1) return fail(TDB_ERR_POSITION, "delta_lut covers |r| <= %d but sequences reach %d", ps.lut_half, len - 1);
+        return tdb_fail(TDB_ERR_POSITION, "a term takes either a fused table or a strip, not both");
+    if (ps.span < 1 || ps.span > (1 << 20)) return tdb_fail(TDB_ERR_POSITION, "span %d out of range", ps.span);
+    if (!ps.delta_lut) return tdb_fail(TDB_ERR_POSITION, "delta_lut is required when a position term is on");
+    if (ps.lut_half < len - 1) return tdb_fail(TDB_ERR_POSITION, "delta_lut covers |r| <= %d but sequences reach %d", ps.lut_half, len - 1);
     const void* ptrs[4] = {ps.pos_key, ps.pos_query, ps.c2p_strip, ps.p2c_strip};
     for (const void* p : ptrs)
-        if (p && !aligned16(p)) return fail(TDB_ERR_ALIGN, "position inputs must be 16-byte aligned");
+        if (p && !aligned16(p)) return tdb_fail(TDB_ERR_ALIGN, "position inputs must be 16-byte aligned");
     if (ps.pos_key && !(stride_ok(ps.pos_key_stride_h, dtype) && stride_ok(ps.pos_key_stride_r, dtype)))
-        return fail(TDB_ERR_STRIDE, "pos_key strides must be non-negative multiples of 16 bytes");
+        return tdb_fail(TDB_ERR_STRIDE, "pos_key strides must be non-negative multiples of 16 bytes");
     if (ps.pos_query && !(stride_ok(ps.pos_query_stride_h, dtype) && stride_ok(ps.pos_query_stride_r, dtype)))
-        return fail(TDB_ERR_STRIDE, "pos_query strides must be non-negative multiples of 16 bytes");
+        return tdb_fail(TDB_ERR_STRIDE, "pos_query strides must be non-negative multiples of 16 bytes");
     if (ps.c2p_strip && (ps.c2p_stride_h < 0 || ps.c2p_stride_l < 0 || (!varlen && ps.c2p_stride_b < 0)))
-        return fail(TDB_ERR_STRIDE, "negative c2p strip stride");
+        return tdb_fail(TDB_ERR_STRIDE, "negative c2p strip stride");
     if (ps.p2c_strip && (ps.p2c_stride_h < 0 || ps.p2c_stride_l < 0 || (!varlen && ps.p2c_stride_b < 0)))
-        return fail(TDB_ERR_STRIDE, "negative p2c strip stride");
+        return tdb_fail(TDB_ERR_STRIDE, "negative p2c strip stride");
     return TDB_OK;
 }
 
@@ -105,7 +109,7 @@ int dispatch(const TdbKernelParams& kp, int dtype, int flags, void* stream) {
         if (kp.gap_cu) e = tdb_zero_gaps(kp, dtype, s);     // (the other kernels do this themselves)
         if (e == hipSuccess) e = tdb_launch_generic(kp, dtype, s);
     }
-    if (e != hipSuccess) return fail(TDB_ERR_LAUNCH, "kernel launch failed: %s", hipGetErrorString(e));
+    if (e != hipSuccess) return tdb_fail(TDB_ERR_LAUNCH, "kernel launch failed: %s", hipGetErrorString(e));
     return TDB_OK;
 }
 
@@ -161,19 +165,19 @@ int tdb_version(void) { return TDB_ABI_VERSION; }
 const char* tdb_last_error(void) { return g_err; }
 
 int tdb_bucket_table(int32_t* out, int32_t max_len, int32_t position_buckets, int32_t max_position) {
-    if (!out) return fail(TDB_ERR_NULL, "out is NULL");
-    if (max_len < 1 || max_len > kMaxLen) return fail(TDB_ERR_SHAPE, "max_len %d out of range", max_len);
+    if (!out) return tdb_fail(TDB_ERR_NULL, "out is NULL");
+    if (max_len < 1 || max_len > kMaxLen) return tdb_fail(TDB_ERR_SHAPE, "max_len %d out of range", max_len);
     bool exact = true;
     for (int32_t r = -(max_len - 1); r <= max_len - 1; ++r) out[r + max_len - 1] = bucket_one(r, position_buckets, max_position, exact);
     if (!exact)
-        return fail(TDB_ERR_BUCKET_MARGIN, "bucket(%d, %d): a ceil() argument is within 3e-5 of an integer; table withheld",
+        return tdb_fail(TDB_ERR_BUCKET_MARGIN, "bucket(%d, %d): a ceil() argument is within 3e-5 of an integer; table withheld",
                     position_buckets, max_position);
     return TDB_OK;
 }
 
 int tdb_delta_table(int32_t* out, int32_t max_len, int32_t position_buckets, int32_t max_position) {
     const int32_t span = position_buckets > 0 ? position_buckets : max_position;
-    if (span < 1) return fail(TDB_ERR_POSITION, "span %d: need position_buckets > 0 or max_position > 0", span);
+    if (span < 1) return tdb_fail(TDB_ERR_POSITION, "span %d: need position_buckets > 0 or max_position > 0", span);
     const int rc = tdb_bucket_table(out, max_len, position_buckets, max_position);
     if (rc != TDB_OK) return rc;
     for (int32_t i = 0; i < 2 * max_len - 1; ++i) {
@@ -184,28 +188,28 @@ int tdb_delta_table(int32_t* out, int32_t max_len, int32_t position_buckets, int
 }
 
 int tdb_check_cu_seqlens(const int32_t* cu, int32_t batch, int32_t total_tokens, int32_t max_seqlen) {
-    if (!cu) return fail(TDB_ERR_NULL, "cu_seqlens is NULL");
-    if (batch < 0) return fail(TDB_ERR_SHAPE, "negative batch");
-    if (cu[0] != 0) return fail(TDB_ERR_CU_SEQLENS, "cu_seqlens[0] = %d, expected 0", cu[0]);
+    if (!cu) return tdb_fail(TDB_ERR_NULL, "cu_seqlens is NULL");
+    if (batch < 0) return tdb_fail(TDB_ERR_SHAPE, "negative batch");
+    if (cu[0] != 0) return tdb_fail(TDB_ERR_CU_SEQLENS, "cu_seqlens[0] = %d, expected 0", cu[0]);
     for (int32_t b = 0; b < batch; ++b) {
         const int64_t n = int64_t(cu[b + 1]) - cu[b];
-        if (n < 0) return fail(TDB_ERR_CU_SEQLENS, "cu_seqlens decreases at %d", b + 1);
-        if (n > max_seqlen) return fail(TDB_ERR_CU_SEQLENS, "sequence %d has %lld tokens > max_seqlen %d", b, (long long)n, max_seqlen);
+        if (n < 0) return tdb_fail(TDB_ERR_CU_SEQLENS, "cu_seqlens decreases at %d", b + 1);
+        if (n > max_seqlen) return tdb_fail(TDB_ERR_CU_SEQLENS, "sequence %d has %lld tokens > max_seqlen %d", b, (long long)n, max_seqlen);
     }
-    if (cu[batch] != total_tokens) return fail(TDB_ERR_CU_SEQLENS, "cu_seqlens[%d] = %d, expected total_tokens %d", batch, cu[batch], total_tokens);
+    if (cu[batch] != total_tokens) return tdb_fail(TDB_ERR_CU_SEQLENS, "cu_seqlens[%d] = %d, expected total_tokens %d", batch, cu[batch], total_tokens);
     return TDB_OK;
 }
 
 int tdb_set_workgroup_limit(int workgroups) { return tdb_mfma_set_workgroup_limit(workgroups); }
 
 int tdb_attn_fwd_fixed(const tdb_fixed_args* a, void* stream) {
-    if (!a) return fail(TDB_ERR_NULL, "args is NULL");
+    if (!a) return tdb_fail(TDB_ERR_NULL, "args is NULL");
     int rc = check_common(a->dtype, a->batch, a->heads, a->head_dim, a->seqlen, a->causal, a->q, a->k, a->v, a->o);
     if (rc != TDB_OK) return rc;
     const int64_t* st[4] = {&a->q_stride_b, &a->k_stride_b, &a->v_stride_b, &a->o_stride_b};
     for (auto s : st)
         if (!stride_ok(s[0], a->dtype) || !stride_ok(s[1], a->dtype) || !stride_ok(s[2], a->dtype) || s[2] < a->head_dim)
-            return fail(TDB_ERR_STRIDE, "q/k/v/o strides must be multiples of 16 bytes with row stride >= head_dim");
+            return tdb_fail(TDB_ERR_STRIDE, "q/k/v/o strides must be multiples of 16 bytes with row stride >= head_dim");
     rc = check_pos(a->pos, a->dtype, a->seqlen, false);
     if (rc != TDB_OK) return rc;
     if (a->batch == 0) return TDB_OK;
@@ -225,15 +229,15 @@ int tdb_attn_fwd_fixed(const tdb_fixed_args* a, void* stream) {
 }
 
 int tdb_attn_fwd_varlen(const tdb_varlen_args* a, void* stream) {
-    if (!a) return fail(TDB_ERR_NULL, "args is NULL");
-    if (a->total_tokens < 0) return fail(TDB_ERR_SHAPE, "negative total_tokens");
+    if (!a) return tdb_fail(TDB_ERR_NULL, "args is NULL");
+    if (a->total_tokens < 0) return tdb_fail(TDB_ERR_SHAPE, "negative total_tokens");
     int rc = check_common(a->dtype, a->batch, a->heads, a->head_dim, a->max_seqlen, a->causal, a->q, a->k, a->v, a->o);
     if (rc != TDB_OK) return rc;
-    if (!a->cu_seqlens) return fail(TDB_ERR_NULL, "cu_seqlens is NULL");
+    if (!a->cu_seqlens) return tdb_fail(TDB_ERR_NULL, "cu_seqlens is NULL");
     const int64_t* st[4] = {&a->q_stride_t, &a->k_stride_t, &a->v_stride_t, &a->o_stride_t};
     for (auto s : st)
         if (!stride_ok(s[0], a->dtype) || !stride_ok(s[1], a->dtype) || s[0] < a->head_dim)
-            return fail(TDB_ERR_STRIDE, "q/k/v/o strides must be multiples of 16 bytes with token stride >= head_dim");
+            return tdb_fail(TDB_ERR_STRIDE, "q/k/v/o strides must be multiples of 16 bytes with token stride >= head_dim");
     rc = check_pos(a->pos, a->dtype, a->max_seqlen, true);
     if (rc != TDB_OK) return rc;
     if (a->batch == 0 || a->total_tokens == 0) return TDB_OK;

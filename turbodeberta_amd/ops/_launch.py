@@ -145,3 +145,27 @@ class PreparedLaunch:
 
 
 BACKWARD_MESSAGE = "Backward pass is not implemented for FlashAttentionDisentangled"
+
+
+def drop_threshold(p: float) -> int:
+    """A dropout probability in units of 2^-16."""
+    p = float(p)
+    if not 0 <= p <= 1:
+        raise ValueError(f"dropout probability {p}: need a value in [0, 1]")
+    return round(65536 * p)
+
+
+def one_seed(seed: torch.Tensor) -> torch.Tensor:
+    if not torch.is_tensor(seed) or seed.dtype != torch.int64 or seed.numel() != 1:
+        raise ValueError("seed must be an int64 tensor with one element")
+    return seed
+
+
+def call(fn, dev: torch.device, *args) -> None:
+    """``fn(*args, stream)`` on the current stream of the device, whichever device is the current one."""
+    if torch.cuda.current_device() != dev.index:                # HIP launches on the current device
+        with torch.cuda.device(dev):
+            return call(fn, dev, *args)
+    rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    if rc:
+        _lib.check(rc)
