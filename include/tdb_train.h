@@ -52,6 +52,47 @@ int tdb_norm_bwd(const tdb_norm_args* args, void* stream);
 /* floats of workspace for a backward call of these sizes (host only; at most 2^31) */
 int64_t tdb_norm_workspace(int64_t rows, int32_t hidden);
 
+/*
+ * Attention as in tdb_attn.h (fixed layout [batch, heads, max_seqlen, head_dim] with optional lengths, or packed where cu_seqlens is there:
+ * [total_tokens, heads, head_dim], stride_b unused), position terms as tables, with dropout on the probabilities; head_dim a multiple of 8 up to 64.
+ * The probability of key j for query i of head h in sequence b has number 4 (j / 16 mod 2) + j mod 4 of counter (4 (j / 32) + j / 4 mod 4, i, b * heads + h, 1).
+ * Forward writes o and lse, float32 [heads, rows], rows = batch * max_seqlen or total_tokens: the logarithm (base 2) of the sum of each row's exponentials, for the backward
+ * call, which also reads o.  Backward writes dq, dk, dv and the gradients of the tables, [heads, 2 span, head_dim] with rows back to back.  Rows beyond a sequence's
+ * length, and packed rows of no sequence, are zeros in every result; what the inputs hold there does not matter.  workspace: tdb_attn_train_workspace() bytes for the
+ * same arguments, 16-byte aligned.  Besides a few bytes for each row and table it holds the scores' gradients of as many heads at a time as fit 512 MiB, at least one:
+ * element size * sum of (length * max_seqlen), lengths rounded up to 64.
+ * The gradient of rows whose sequence has one token is zero in q, k and the tables.
+ */
+typedef struct tdb_train_attn_args {
+    int32_t dtype, batch, heads, head_dim, max_seqlen, total_tokens, threshold, span, lut_half;
+    float   sm_scale;               /* positive */
+    const void *q, *k, *v;
+    void*   o;
+    const void* dout;
+    void *dq, *dk, *dv;
+    int64_t q_stride_b, q_stride_h, q_stride_l;
+    int64_t k_stride_b, k_stride_h, k_stride_l;
+    int64_t v_stride_b, v_stride_h, v_stride_l;
+    int64_t o_stride_b, o_stride_h, o_stride_l;
+    int64_t dout_stride_b, dout_stride_h, dout_stride_l;
+    int64_t dq_stride_b, dq_stride_h, dq_stride_l;
+    int64_t dk_stride_b, dk_stride_h, dk_stride_l;
+    int64_t dv_stride_b, dv_stride_h, dv_stride_l;
+    const int32_t *seqlens_k, *cu_seqlens, *delta_lut;
+    const void *pos_key, *pos_query;
+    int64_t pos_key_stride_h, pos_key_stride_r, pos_query_stride_h, pos_query_stride_r;
+    void *dpos_key, *dpos_query;
+    int64_t dpos_key_stride_h, dpos_query_stride_h;
+    float*  lse;
+    void*   workspace;
+    int64_t workspace_bytes;
+    const int64_t* seed;
+} tdb_train_attn_args;
+
+int tdb_attn_train_fwd(const tdb_train_attn_args* args, void* stream);
+int tdb_attn_train_bwd(const tdb_train_attn_args* args, void* stream);
+int64_t tdb_attn_train_workspace(const tdb_train_attn_args* args);
+
 #ifdef __cplusplus
 }
 #endif

@@ -30,7 +30,7 @@ def test_header_and_binding_agree():
     header = _declared("tdb_train.h")
     assert set(re.findall(r"^(?:int|int64_t)\s+(tdb_\w+)\s*\(", header, re.M)) == set(_lib.TRAIN_EXPORTS)
     assert all(hasattr(_lib.load(), n) for n in _lib.TRAIN_EXPORTS)
-    for cname, cls in (("tdb_norm_args", _lib.NormArgs),):
+    for cname, cls in (("tdb_norm_args", _lib.NormArgs), ("tdb_train_attn_args", _lib.TrainAttnArgs)):
         body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (cname, cname), header, re.S).group(1)
         names = []
         for decl in re.sub(r"/\*.*?\*/", "", body, flags=re.S).split(";"):

@@ -89,3 +89,52 @@ def check(name, got, ref, off):
     far = (got.detach().cpu().double() - ref).abs()
     bad = ~(far <= bound)
     assert not bad.any(), f"{name}: {int(bad.sum())} of {bad.numel()} values, by up to {(far / bound).max().item():.3g} of the bound"
+
+
+def attention(q, k, v, pk, pq, dout, rows, scale, keep, factor, dtype, most):
+    """One sequence and head in 64 bits: {name: (value, bound)} of o, dq, dk, dv and, where there are tables, dpk, dpq.  q, k, v, dout [l, D]; rows: table row of
+    (query, key); keep: what the probabilities are multiplied by (factor or 0); most: the largest |dout| |v| of the whole call (float16).
+
+    Bounds, u half a step of the type, U of float32.  A score is a sum of 64 products for each of three terms: off by 70 U of its terms' sizes A.  A probability is
+    off by that, by its exponent's rounding and by its sum's, relative: rho = 100 U (1 + A + max A).  Rounded to the type where it enters a product: u, or in float16, for
+    small ones, half the smallest step: 2^-25 of a row's largest forward, 2^-25 / 2^floor(log2 l) backward.  D comes from the rounded result.  A gradient of a score is off by what
+    its factors are, and rounded to the type (float16: or half the smallest step after a scaling that brings 2 most factor below 2^15, to 2^14 at least).  The
+    sums that follow have `steps` terms one after another."""
+    u, half = torch.finfo(dtype).eps / 2, dtype == torch.float16
+    if dtype == torch.float32:
+        u = 0.0
+    l = q.shape[0]
+    steps = 100 + l / 8
+    K, Q = (k[None] + pk[rows] if pk is not None else k[None].expand(l, -1, -1)), (q[:, None] + pq[rows] if pq is not None else q[:, None].expand(-1, l, -1))
+    size = lambda *t: sum(x.abs() for x in t if x is not None)
+    sizeK, sizeQ = size(k[None], None if pk is None else pk[rows]), size(q[:, None], None if pq is None else pq[rows])
+    s, A = q @ k.t(), q.abs() @ k.abs().t()
+    if pk is not None:
+        s, A = s + torch.einsum("id,ijd->ij", q, pk[rows]), A + torch.einsum("id,ijd->ij", q.abs(), pk[rows].abs())
+    if pq is not None:
+        s, A = s + torch.einsum("jd,ijd->ij", k, pq[rows]), A + torch.einsum("jd,ijd->ij", k.abs(), pq[rows].abs())
+    p, A = torch.softmax(s * scale, -1), A * scale
+    rho = 100 * U * (1 + A + A.amax(-1, keepdim=True))
+    kept = p * keep
+    o = kept @ v
+    low = p.amax(-1, keepdim=True) * 2.0 ** -25 * (keep != 0) * factor if half else 0
+    o_off = ((u + rho + steps * U) * kept + low) @ v.abs()
+    dv = kept.t() @ dout
+    low = 2.0 ** -25 / 2 ** int(np.log2(l)) * factor if half else 0
+    dv_off = ((u + rho + steps * U) * kept + low).t() @ dout.abs()
+    dp = dout @ v.t() * keep
+    D = (p * dp).sum(-1, keepdim=True)
+    D_off = (dout.abs() * (u * o.abs() + o_off + 70 * U * o.abs())).sum(-1, keepdim=True)
+    ds = p * (dp - D) * (l > 1)
+    ds_off = (rho + u) * ds.abs() + p * (72 * U * (dout.abs() @ v.abs().t()) * keep + D_off + 4 * U * (dp.abs() + D.abs())) * (1 + u)
+    if half:
+        ds_off = ds_off + 2.0 ** -25 / 2 ** 14 * 2 * 2 * most * factor
+    ds_off = ds_off * (l > 1) + steps * U * ds.abs()
+    got = {"o": (o, o_off), "dv": (dv, dv_off),
+           "dq": tuple(scale * torch.einsum("ij,ijd->id", x, y) for x, y in ((ds, K), (ds_off, sizeK))),
+           "dk": tuple(scale * torch.einsum("ij,ijd->jd", x, y) for x, y in ((ds, Q), (ds_off, sizeQ)))}
+    for name, table, rows_of in (("dpk", pk, q[:, None].expand(l, l, -1)), ("dpq", pq, k[None].expand(l, l, -1))):
+        if table is not None:
+            got[name] = tuple(scale * torch.zeros_like(table).index_add_(0, rows.flatten(), (x[..., None] * y).flatten(0, 1))
+                              for x, y in ((ds, rows_of), (ds_off, rows_of.abs())))
+    return got

@@ -29,7 +29,8 @@ _VALUE_ERRORS = {-1, -2, -3, -4, -5, -6, -7, -8, -9}
 
 EXPORTS = ("tdb_version", "tdb_last_error", "tdb_attn_fwd_fixed", "tdb_attn_fwd_varlen", "tdb_bucket_table",
            "tdb_delta_table", "tdb_check_cu_seqlens", "tdb_set_workgroup_limit")
-TRAIN_EXPORTS = ("tdb_dropout", "tdb_norm_fwd", "tdb_norm_bwd", "tdb_norm_workspace")       # declared in include/tdb_train.h
+TRAIN_EXPORTS = ("tdb_dropout", "tdb_norm_fwd", "tdb_norm_bwd", "tdb_norm_workspace", "tdb_attn_train_fwd", "tdb_attn_train_bwd",
+                 "tdb_attn_train_workspace")       # declared in include/tdb_train.h
 
 
 class PosArgs(C.Structure):
@@ -85,6 +86,20 @@ class NormArgs(C.Structure):
     ]
 
 
+class TrainAttnArgs(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("batch", C.c_int32), ("heads", C.c_int32), ("head_dim", C.c_int32), ("max_seqlen", C.c_int32),
+        ("total_tokens", C.c_int32), ("threshold", C.c_int32), ("span", C.c_int32), ("lut_half", C.c_int32), ("sm_scale", C.c_float),
+        ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("o", C.c_void_p), ("dout", C.c_void_p),
+        ("dq", C.c_void_p), ("dk", C.c_void_p), ("dv", C.c_void_p),
+        *((f"{t}_stride_{n}", C.c_int64) for t in ("q", "k", "v", "o", "dout", "dq", "dk", "dv") for n in "bhl"),
+        ("seqlens_k", C.c_void_p), ("cu_seqlens", C.c_void_p), ("delta_lut", C.c_void_p), ("pos_key", C.c_void_p), ("pos_query", C.c_void_p),
+        ("pos_key_stride_h", C.c_int64), ("pos_key_stride_r", C.c_int64), ("pos_query_stride_h", C.c_int64), ("pos_query_stride_r", C.c_int64),
+        ("dpos_key", C.c_void_p), ("dpos_query", C.c_void_p), ("dpos_key_stride_h", C.c_int64), ("dpos_query_stride_h", C.c_int64),
+        ("lse", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64), ("seed", C.c_void_p),
+    ]
+
+
 _lock = threading.Lock()
 _lib = None
 _host = None
@@ -120,6 +135,10 @@ def load() -> C.CDLL:
         lib.tdb_dropout.argtypes = [C.c_void_p, C.c_void_p, C.c_int64, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p]
         for name in ("tdb_norm_fwd", "tdb_norm_bwd"):
             getattr(lib, name).argtypes = [C.POINTER(NormArgs), C.c_void_p]
+        for name in ("tdb_attn_train_fwd", "tdb_attn_train_bwd"):
+            getattr(lib, name).argtypes = [C.POINTER(TrainAttnArgs), C.c_void_p]
+        lib.tdb_attn_train_workspace.argtypes = [C.POINTER(TrainAttnArgs)]
+        lib.tdb_attn_train_workspace.restype = C.c_int64
         lib.tdb_norm_workspace.argtypes = [C.c_int64, C.c_int32]
         lib.tdb_norm_workspace.restype = C.c_int64
         if lib.tdb_version() != ABI_VERSION:
