@@ -4,15 +4,15 @@
 // 8 g .. 8 g + 7, g = lane >> 4.  In 16 bits that is one matrix instruction (16x16x32), in float32 eight (16x16x4: step s contracts column
 // 8 g + s of lane group g; the order of a sum is free as long as both operands have it).  A result has row 4 g + e (e = 0..3), column c in a lane.
 //
-// Layout of scores.  A wave owns 16 NX rows x (a lane has one of each 16) and runs over the other side's rows y, 64 a step: S[y][x], y in the
+// Layout of scores.  A wave owns 16 rows x (a lane has one) and runs over the other side's rows y, 64 a step: S[y][x], y in the
 // result's rows.  Forward x are queries and y keys, so a softmax row is in a lane and the three others of its column, and the probabilities are an operand
 // of the next product as they stand.  Backward x are keys and y queries: the same for the gradients of keys and values.
 //
 // Position terms.  Both are functions of x - y (r = x - y + 63 in a tile), with the table of x's side ("own") and of y's ("other"):
 //   own:   x . T_own[r]    computed for the 80 r that 16 x and 64 y have, result columns x: stored to LDS as rows x, index y + 16 - x, a row of
-//          81 floats: x * 81 + 16 - x + y is a multiple of 4 for every y that is one, so four y at once are one read of 16 bytes.
-//   other: y . T_other[r]  for the 16 (NX + 1) r of 16 y and the wave's x, result columns y: stored as rows y, read back value by value, lanes
-//          along x, without conflicts.
+//          85 floats: x * 85 + 16 - x + y is a multiple of 4 for every y that is one, so four y at once are one read of 16 bytes, and 84 x for
+//          16 x are on distinct banks.
+//   other: y . T_other[r]  for the 32 r of 16 y and 16 x, result columns y: stored as rows y, read back value by value, lanes along x.
 // They are held in float32.  The tables' rows lie in LDS as rings in the order of r; 64 rows are new in each step.
 #pragma once
 
@@ -64,17 +64,11 @@ struct Elem<TDB_F32> {
 
 constexpr int TILE = 64;                        // rows y of a step, and of a tile of score gradients
 constexpr int TILE_VALUES = TILE * TILE;
-constexpr int THREADS = 256;
 constexpr float LOG2E = 1.44269504088896340736f;
 
 // Rows of 64 values in LDS, 16 bytes apart: 16 rows at the same column are on distinct banks.
 template <int DT>
 constexpr int ROW = DT == TDB_F32 ? 68 : 72;
-// 16-byte pieces of a row of 64 values, and of a tile for each thread
-template <int DT>
-constexpr int PIECES = DT == TDB_F32 ? 16 : 8;
-template <int DT>
-constexpr int LOADS = TILE * PIECES<DT> / THREADS;
 
 __device__ __forceinline__ int lane_c() { return threadIdx.x & 15; }
 __device__ __forceinline__ int lane_g() { return threadIdx.x >> 4 & 3; }
@@ -220,43 +214,122 @@ __device__ __forceinline__ const typename Elem<DT>::T* rows_of(const Tensor& t, 
     return static_cast<const typename Elem<DT>::T*>(t.p) + (a.cu ? w.first * t.l : w.b * t.b) + h * t.h;
 }
 
-// A tile of 64 rows of 64 values on its way from global memory to LDS.
-template <int DT>
+// Loads go through buffer resources: what lies beyond the resource's end reads as zeros, so rows past a sequence and columns past D need no code of their own.
+constexpr uint32_t NOWHERE = 0x80000000u;       // an offset past every end
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void* p, int64_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, int(min(max(bytes, int64_t(0)), int64_t(0x7fffffff))), 0x00020000);
+}
+
+// A tile of 64 rows of 64 values on its way from global memory to LDS, 16 bytes a lane at a time, by `threads` threads.
+template <int DT, int threads>
 struct Stage {
     using T = typename Elem<DT>::T;
-    static constexpr int EACH = 64 / PIECES<DT>, STEP = THREADS / PIECES<DT>;      // values of a piece, rows of a pass
-    u32x4 x[LOADS<DT>];
-    static __device__ __forceinline__ int row(int n) { return threadIdx.x / PIECES<DT> + n * STEP; }
-    static __device__ __forceinline__ int col() { return threadIdx.x % PIECES<DT> * EACH; }
-    // rows row0 .., zeros from `len` on and past D columns
-    __device__ __forceinline__ void load(const T* rows, int64_t stride, int row0, int len, int D) {
+    static constexpr int PIECES = DT == TDB_F32 ? 16 : 8, EACH = 64 / PIECES, STEP = threads / PIECES, LOADS = TILE * PIECES / threads;
+    u32x4 x[LOADS];
+    static __device__ __forceinline__ int row(int n) { return threadIdx.x / PIECES + n * STEP; }
+    static __device__ __forceinline__ int col() { return threadIdx.x % PIECES * EACH; }
+    // of a lane's pieces, in bytes, where rows are `stride` bytes apart
+    static __device__ __forceinline__ void offsets(uint32_t (&at)[LOADS], uint32_t stride, int D) {
 #pragma unroll
-        for (int n = 0; n < LOADS<DT>; ++n) {
-            const int r = row0 + row(n);
-            x[n] = r < len && col() < D ? *reinterpret_cast<const u32x4*>(rows + r * stride + col()) : u32x4{0, 0, 0, 0};
-        }
+        for (int n = 0; n < LOADS; ++n) at[n] = col() < D ? row(n) * stride + col() * sizeof(T) : NOWHERE;
     }
-    // rows of a table, given for each pass
-    __device__ __forceinline__ void load(const T* rows, int64_t stride, const int (&which)[LOADS<DT>], int D) {
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t from, const uint32_t (&at)[LOADS]) {
 #pragma unroll
-        for (int n = 0; n < LOADS<DT>; ++n)
-            x[n] = col() < D ? *reinterpret_cast<const u32x4*>(rows + which[n] * stride + col()) : u32x4{0, 0, 0, 0};
+        for (int n = 0; n < LOADS; ++n) x[n] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(from, int(at[n]), 0, 0));
     }
     __device__ __forceinline__ void store(T* rows) const {
 #pragma unroll
-        for (int n = 0; n < LOADS<DT>; ++n) *reinterpret_cast<u32x4*>(rows + row(n) * ROW<DT> + col()) = x[n];
+        for (int n = 0; n < LOADS; ++n) *reinterpret_cast<u32x4*>(rows + row(n) * ROW<DT> + col()) = x[n];
     }
 };
 
-// The table rows of 64 neighbouring r: r = r0 + (row of the stage) of a tile whose x start at x0 and whose y start at y0.  SIGN: 1 where x are
-// queries (relative position x - y), -1 where they are keys.
-template <int DT, int SIGN>
-__device__ __forceinline__ void table_rows(const Args& a, int r0, int x0, int y0, int (&which)[LOADS<DT>]) {
-#pragma unroll
-    for (int n = 0; n < LOADS<DT>; ++n) {
-        const int at = SIGN * (r0 + Stage<DT>::row(n) - 63 + x0 - y0);
-        which[n] = a.lut[min(max(at, -a.lut_half), a.lut_half) + a.lut_half];
+// Rows of one head of one sequence, 64 at a time in order.
+template <int DT, int threads>
+struct Source {
+    using S = Stage<DT, threads>;
+    const char* next;
+    uint32_t stride;                    // bytes, at most 2^24
+    int left;                           // rows
+    uint32_t at[S::LOADS];
+    __device__ __forceinline__ Source(const Tensor& t, const Args& a, const Where& w, int h, int row = 0) {
+        stride = uint32_t(t.l) * sizeof(typename S::T), left = w.len - row;
+        next = reinterpret_cast<const char*>(rows_of<DT>(t, a, w, h)) + int64_t(row) * stride;
+        S::offsets(at, stride, a.D);
     }
+    __device__ __forceinline__ void load(S& s) {
+        s.load(__builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(next), 0, int(min(left, TILE) * stride), 0x00020000), at);
+        next += int64_t(TILE) * stride, left -= TILE;
+    }
+};
+
+// Both tables' rows for 64 neighbouring r of a tile.  SIGN: 1 where x are queries (the relative position is x - y), -1 where they are keys.
+template <int DT, int SIGN, int threads, bool PK, bool PQ>
+struct Tables {
+    using S = Stage<DT, threads>;
+    using T = typename S::T;
+    __amdgpu_buffer_rsrc_t lut, pk, pq;
+    uint32_t pk_stride, pq_stride, lane;        // bytes; of the lane's column (past every end where there is none: what is added is below 2^31)
+    int at, last;                               // the lane's place in the lookup table for x0 = y0 and r0 = 0, and its last one, in bytes
+    S k, q;
+    int which[S::LOADS];
+    __device__ __forceinline__ Tables(const Args& a, int h) {
+        lut = buffer(a.lut, (2 * int64_t(a.lut_half) + 1) * 4);
+        if constexpr (PK) pk = buffer(static_cast<const T*>(a.pk.p) + h * a.pk.h, 2 * int64_t(a.span) * a.pk.l * sizeof(T));
+        if constexpr (PQ) pq = buffer(static_cast<const T*>(a.pq.p) + h * a.pq.h, 2 * int64_t(a.span) * a.pq.l * sizeof(T));
+        pk_stride = uint32_t(a.pk.l) * sizeof(T), pq_stride = uint32_t(a.pq.l) * sizeof(T);
+        lane = S::col() < a.D ? S::col() * sizeof(T) : NOWHERE;
+        at = (SIGN * (S::row(0) - 63) + a.lut_half) * 4, last = 8 * a.lut_half;
+    }
+    // looks up the rows of r0 .. r0 + 63; `from`: x0 - y0 of the tile
+    __device__ __forceinline__ void look(int r0, int from) {
+        if constexpr (PK || PQ) {
+#pragma unroll
+            for (int n = 0; n < S::LOADS; ++n)
+                which[n] = int(__builtin_amdgcn_raw_buffer_load_b32(lut, min(max(at + 4 * SIGN * (r0 + from + n * S::STEP), 0), last), 0, 0));
+        }
+    }
+    // and fetches those looked up last
+    __device__ __forceinline__ void load() {
+        auto one = [&](S& s, __amdgpu_buffer_rsrc_t from, uint32_t stride) {
+            uint32_t to[S::LOADS];
+#pragma unroll
+            for (int n = 0; n < S::LOADS; ++n) to[n] = uint32_t(which[n]) * stride + lane;
+            s.load(from, to);
+        };
+        if constexpr (PK) one(k, pk, pk_stride);
+        if constexpr (PQ) one(q, pq, pq_stride);
+    }
+    __device__ __forceinline__ void store(T* pk_ring, T* pq_ring, int to) const {
+        if constexpr (PK) k.store(pk_ring + to * ROW<DT>);
+        if constexpr (PQ) q.store(pq_ring + to * ROW<DT>);
+    }
+    // the rows of a ring from r = 64 on, for a first step at x0 = from, all looked up before the first is fetched; those of r = 0 .. 63 are looked up last
+    template <int ring>
+    __device__ __forceinline__ void fill(T* pk_ring, T* pq_ring, int from) {
+        if constexpr (!PK && !PQ) return;
+        constexpr int N = ring / 64;
+        int rows[N][S::LOADS];
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            look(64 * n, from);
+#pragma unroll
+            for (int i = 0; i < S::LOADS; ++i) rows[n][i] = which[i];
+        }
+#pragma unroll
+        for (int n = N - 1; n >= 0; --n) {
+#pragma unroll
+            for (int i = 0; i < S::LOADS; ++i) which[i] = rows[n][i];
+            if (n == 0) return;
+            load();
+            store(pk_ring, pq_ring, 64 * n);
+        }
+    }
+};
+
+// Whether all relative positions first .. last that occur have one table row.
+__device__ __forceinline__ bool one_row(const Args& a, int first, int last) {
+    const int lo = min(max(first, 1 - a.L), a.L - 1), hi = min(max(last, 1 - a.L), a.L - 1);
+    return a.lut[lo + a.lut_half] == a.lut[hi + a.lut_half];
 }
 
 // Sum, and maximum, over the four lanes of a column.
@@ -275,12 +348,10 @@ __device__ __forceinline__ float column_max(float x) {
     return fmaxf(__builtin_bit_cast(float, uint32_t(s[0])), __builtin_bit_cast(float, uint32_t(s[1])));
 }
 
-constexpr int OWN_ROW = 81;                     // floats of a row of x's term, see above
-template <int NX>
-constexpr int OTHER_ROW = 16 * (NX + 1) + 4;    // and of y's term: 16 rows at the same column are on distinct banks
-// floats of a wave's scratch for the two
-template <int NX>
-constexpr int TERMS = NX * 16 * OWN_ROW + 16 * OTHER_ROW<NX>;
+constexpr int OWN_ROW = 85;             // floats of a row of x's term, see above
+constexpr int OTHER_ROW = 36;           // and of y's term: 16 rows at the same column are on distinct banks
+// floats of a wave's scratch for the two, the second twice: one is written while the other is read
+constexpr int OWN_TERM = 16 * OWN_ROW, OTHER_TERM = 16 * OTHER_ROW, TERMS = OWN_TERM + 2 * OTHER_TERM;
 
 // Place of a ring's row; at is below twice its size.
 template <int ring>
@@ -288,65 +359,94 @@ __device__ __forceinline__ int wrapped(int at) {
     return at >= ring ? at - ring : at;
 }
 
-// Scores of the wave's 16 NX rows x (x blocks first .. first + NX - 1 of 16 rows) with a step's 64 rows y, without the scale.  own[a][k]: frags of x.  Rings of
-// `ring` rows whose row for r is (r + base) mod ring.  scratch: the wave's own, TERMS<NX> floats.
-template <int DT, int NX, int ring>
-__device__ __forceinline__ void scores(f32x4 (&s)[NX][4], const typename Elem<DT>::X8 (&own)[NX][2], const typename Elem<DT>::T* y_rows,
-                                       const typename Elem<DT>::T* own_ring, const typename Elem<DT>::T* other_ring, bool has_own, bool has_other, int base,
-                                       int first, float* scratch) {
+// A row of a ring as both operands' frags: the same for every row or column.
+template <int DT>
+__device__ __forceinline__ typename Elem<DT>::X8 same_frag(const typename Elem<DT>::T* row, int k0) {
+    return read8<DT>(row + k0 + 8 * lane_g());
+}
+// And as an operand whose row is column col + c and which is the same all along the contraction.
+template <int DT>
+__device__ __forceinline__ typename Elem<DT>::X8 level_frag(const typename Elem<DT>::T* row, int col) {
+    const typename Elem<DT>::T v = row[col + lane_c()];
+    typename Elem<DT>::X8 x;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = v;
+    return x;
+}
+
+// Scores of the wave's 16 rows x (x block `first`) with a step's 64 rows y, without the scale.  own[k]: frags of x.  Rings of `ring` rows whose row for r is
+// (r + base) mod ring.  scratch: the wave's own, TERMS floats.  far: the step's relative positions have one table row, so the terms are one number for each x and one for
+// each y.
+template <int DT, int ring, bool OWN, bool OTHER>
+__device__ __forceinline__ void scores(f32x4 (&s)[4], const typename Elem<DT>::X8 (&own)[2], const typename Elem<DT>::T* y_rows, const typename Elem<DT>::T* own_ring,
+                                       const typename Elem<DT>::T* other_ring, int base, int first, float* scratch, bool far) {
     using E = Elem<DT>;
     using X8 = typename E::X8;
     const int c = lane_c(), g = lane_g();
     const f32x4 none = {0.f, 0.f, 0.f, 0.f};
-    if (has_own) {
+    const int mid = wrapped<ring>(63 + base) * ROW<DT>;
+    if ((OWN || OTHER) && far) {
+        f32x4 w = none;
+        if constexpr (OWN) w = E::mma(same_frag<DT>(own_ring + mid, 32), own[1], E::mma(same_frag<DT>(own_ring + mid, 0), own[0], none));
+        X8 t0, t1;
+        if constexpr (OTHER) t0 = same_frag<DT>(other_ring + mid, 0), t1 = same_frag<DT>(other_ring + mid, 32);
 #pragma unroll
-        for (int n = 0; n < NX + 4; ++n) {      // r = 16 (first + n) + 15 - row of the frag
-            const int at = wrapped<ring>(16 * (first + n) + base);
-            const X8 t0 = read8<DT>(own_ring + (at + 15 - c) * ROW<DT> + 8 * g), t1 = read8<DT>(own_ring + (at + 15 - c) * ROW<DT> + 32 + 8 * g);
-#pragma unroll
-            for (int a = 0; a < NX; ++a) {
-                const int b = n - a;
-                if (b < 0 || b > 4) continue;
-                const f32x4 w = E::mma(t1, own[a][1], E::mma(t0, own[a][0], none));
-                float* const to = scratch + a * 16 * OWN_ROW + c * OWN_ROW + 64 - 16 * b + 4 * g;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) to[e] = w[e];
-            }
+        for (int m = 0; m < 4; ++m) {
+            const X8 y0 = row_frag<DT>(y_rows, 16 * m, 0), y1 = row_frag<DT>(y_rows, 16 * m, 32);
+            s[m] = E::mma(y1, own[1], E::mma(y0, own[0], w));
+            if constexpr (OTHER) s[m] = E::mma(y1, t1, E::mma(y0, t0, s[m]));
         }
-        wave_fence();
-#pragma unroll
-        for (int a = 0; a < NX; ++a)
-#pragma unroll
-            for (int m = 0; m < 4; ++m) s[a][m] = *reinterpret_cast<const f32x4*>(scratch + a * 16 * OWN_ROW + c * (OWN_ROW - 1) + 16 + 16 * m + 4 * g);
-        wave_fence();
-    } else {
-#pragma unroll
-        for (int a = 0; a < NX; ++a)
-#pragma unroll
-            for (int m = 0; m < 4; ++m) s[a][m] = none;
+        return;
     }
-    float* const other = scratch + NX * 16 * OWN_ROW;
+    if constexpr (OWN) {
+        f32x4 w[5];
+#pragma unroll
+        for (int n = 0; n < 5; ++n) {           // r = 16 (first + n) + 15 - row of the frag
+            const int at = wrapped<ring>(16 * (first + n) + base) + 15 - c;
+            w[n] = E::mma(read8<DT>(own_ring + at * ROW<DT> + 8 * g), own[0], none);
+            w[n] = E::mma(read8<DT>(own_ring + at * ROW<DT> + 32 + 8 * g), own[1], w[n]);
+        }
+#pragma unroll
+        for (int n = 0; n < 5; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) scratch[c * OWN_ROW + 64 - 16 * n + 4 * g + e] = w[n][e];
+    }
+    X8 y[4][2];
+#pragma unroll
+    for (int m = 0; m < 4; ++m)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) y[m][k] = row_frag<DT>(y_rows, 16 * m, 32 * k);
+    f32x4 w[OTHER ? 4 : 1][2];
+    if constexpr (OTHER) {
+#pragma unroll
+        for (int n = 0; n < 5; ++n) {           // r = 16 (first + n) + row: of y blocks 3 - n and 4 - n
+            const int at = wrapped<ring>(16 * (first + n) + base);
+            const X8 t0 = row_frag<DT>(other_ring, at, 0), t1 = row_frag<DT>(other_ring, at, 32);
+#pragma unroll
+            for (int m = 3 - n; m <= 4 - n; ++m)
+                if (m >= 0 && m < 4) w[m][n - 3 + m] = E::mma(t1, y[m][1], E::mma(t0, y[m][0], none));
+        }
+    }
+    wave_fence();
 #pragma unroll
     for (int m = 0; m < 4; ++m) {
-        const X8 y0 = row_frag<DT>(y_rows, 16 * m, 0), y1 = row_frag<DT>(y_rows, 16 * m, 32);
+        if constexpr (OWN) s[m] = *reinterpret_cast<const f32x4*>(scratch + c * (OWN_ROW - 1) + 16 + 16 * m + 4 * g);
+        else s[m] = none;
+    }
 #pragma unroll
-        for (int a = 0; a < NX; ++a) s[a][m] = E::mma(y1, own[a][1], E::mma(y0, own[a][0], s[a][m]));
-        if (has_other) {
+    for (int m = 0; m < 4; ++m) s[m] = E::mma(y[m][1], own[1], E::mma(y[m][0], own[0], s[m]));
+    if constexpr (OTHER) {
 #pragma unroll
-            for (int n = 0; n <= NX; ++n) {     // r = 16 (first - m + 3 + n) + row
-                const int at = wrapped<ring>(16 * (first - m + 3 + n) + base);
-                const X8 t0 = row_frag<DT>(other_ring, at, 0), t1 = row_frag<DT>(other_ring, at, 32);
-                const f32x4 w = E::mma(t1, y1, E::mma(t0, y0, none));
-                *reinterpret_cast<f32x4*>(other + c * OTHER_ROW<NX> + 16 * n + 4 * g) = w;
-            }
+        for (int m = 0; m < 4; ++m) {
+            float* const other = scratch + OWN_TERM + (m & 1) * OTHER_TERM;
+#pragma unroll
+            for (int n = 0; n < 2; ++n) *reinterpret_cast<f32x4*>(other + c * OTHER_ROW + 16 * n + 4 * g) = w[m][n];
             wave_fence();
 #pragma unroll
-            for (int a = 0; a < NX; ++a)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s[a][m][e] += other[(4 * g + e) * OTHER_ROW<NX> + 16 * a + c + 15 - 4 * g - e];
-            wave_fence();
+            for (int e = 0; e < 4; ++e) s[m][e] += other[(4 * g + e) * OTHER_ROW + c + 15 - 4 * g - e];
         }
     }
+    wave_fence();
 }
 
 // Four neighbouring values of a result's row, rounded to the type.
@@ -373,16 +473,14 @@ __device__ __forceinline__ void store_rows(const Tensor& t, const Args& a, const
 }
 
 // The wave's own rows as frags; zeros past the sequence and past D columns.
-template <int DT, int NX>
-__device__ __forceinline__ void load_own(typename Elem<DT>::X8 (&own)[NX][2], const Tensor& t, const Args& a, const Where& w, int h, int row) {
+template <int DT>
+__device__ __forceinline__ void load_own(typename Elem<DT>::X8 (&own)[2], const Tensor& t, const Args& a, const Where& w, int h, int row) {
     const typename Elem<DT>::T* const from = rows_of<DT>(t, a, w, h);
 #pragma unroll
-    for (int n = 0; n < NX; ++n)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const int r = row + 16 * n + lane_c(), d = 32 * k + 8 * lane_g();
-            own[n][k] = r < w.len && d < a.D ? read8<DT>(from + r * t.l + d) : zero8<DT>();
-        }
+    for (int k = 0; k < 2; ++k) {
+        const int r = row + lane_c(), d = 32 * k + 8 * lane_g();
+        own[k] = r < w.len && d < a.D ? read8<DT>(from + r * t.l + d) : zero8<DT>();
+    }
 }
 
 // float16: a power of two that brings the gradients of scores near the top of the type's range: they are at most 2 |dout| |v| times dropout's factor.  Other types

@@ -19,159 +19,137 @@ namespace tdb_train {
 
 // ---------------------------------------------------------------------------------------------------------------- forward
 
-template <int DT, int NX>
-constexpr int RING = 64 * NX + 64;
-
-template <int DT, int NX>
-struct FwdLds {
-    using T = typename Elem<DT>::T;
-    alignas(16) T k[TILE * ROW<DT>], v[TILE * ROW<DT>], pk[RING<DT, NX> * ROW<DT>], pq[RING<DT, NX> * ROW<DT>];
-    alignas(16) float scratch[4][TERMS<NX>];
+// A workgroup has 128 rows x in 16 bits, 64 in float32, where the tables' rows for more would not fit LDS; a wave 16.
+template <int DT>
+struct Shape {
+    static constexpr int WAVES = DT == TDB_F32 ? 4 : 8, ROWS = 16 * WAVES, RING = ROWS + 64, THREADS = 64 * WAVES;
 };
 
-template <int DT, int NX>
-__global__ __launch_bounds__(THREADS, 1) void attn_fwd_kernel(Args a) {
+template <int DT>
+struct FwdLds {
+    using T = typename Elem<DT>::T;
+    using S = Shape<DT>;
+    alignas(16) T k[TILE * ROW<DT>], v[TILE * ROW<DT>], pk[S::RING * ROW<DT>], pq[S::RING * ROW<DT>];
+    alignas(16) float scratch[S::WAVES][TERMS];
+};
+
+template <int DT, bool PK, bool PQ>
+__global__ __launch_bounds__(Shape<DT>::THREADS, 1) void attn_fwd_kernel(Args a) {
     using E = Elem<DT>;
     using T = typename E::T;
     using X8 = typename E::X8;
-    constexpr int ring = RING<DT, NX>;
+    using S = Shape<DT>;
+    constexpr int ring = S::RING;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    FwdLds<DT, NX>& sm = *reinterpret_cast<FwdLds<DT, NX>*>(smem);
+    FwdLds<DT>& sm = *reinterpret_cast<FwdLds<DT>*>(smem);
     if (a.cu && threadIdx.x < 64)
         tdb_fill_gaps(a.cu, a.B, a.L, a.total, static_cast<char*>(a.o.p), a.o.l * sizeof(T), a.o.h * sizeof(T), a.H, a.D * sizeof(T), blockIdx.x, gridDim.x);
     int h;
     Where w;
-    if (!locate<64 * NX>(a, h, w)) return;
+    if (!locate<S::ROWS>(a, h, w)) return;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane_c(), g = lane_g();
-    const int row = w.row0 + 16 * NX * wave;        // the wave's first query
-    f32x4 o[NX][4];
+    const int row = w.row0 + 16 * wave;             // the wave's first query
+    f32x4 o[4];
 #pragma unroll
-    for (int x = 0; x < NX; ++x)
-#pragma unroll
-        for (int d = 0; d < 4; ++d) o[x][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int d = 0; d < 4; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
     if (w.row0 >= w.len) {
-#pragma unroll
-        for (int x = 0; x < NX; ++x) store_rows<DT>(a.o, a, w, h, row + 16 * x, o[x], 0.f);
+        store_rows<DT>(a.o, a, w, h, row, o, 0.f);
         return;
     }
-    const T *const kp = rows_of<DT>(a.k, a, w, h), *const vp = rows_of<DT>(a.v, a, w, h);
-    const T *const pk = static_cast<const T*>(a.pk.p) + h * a.pk.h, *const pq = static_cast<const T*>(a.pq.p) + h * a.pq.h;
-    const bool has_pk = a.pk.p, has_pq = a.pq.p;
     const TdbKey key = a.threshold ? tdb_key(a.seed) : TdbKey{0, 0};
-    X8 q[NX][2];
-    load_own<DT, NX>(q, a.q, a, w, h, row);
-
-    Stage<DT> k_next, v_next, pk_next, pq_next;
-    int which[LOADS<DT>];
-    auto tables = [&](Stage<DT>& s1, Stage<DT>& s2) {
-        if (has_pk) s1.load(pk, a.pk.l, which, a.D);
-        if (has_pq) s2.load(pq, a.pq.l, which, a.D);
-    };
-    if (has_pk || has_pq) {
-#pragma unroll
-        for (int n = 1; n <= NX; ++n) {
-            table_rows<DT, 1>(a, 64 * n, w.row0, 0, which);
-            tables(pk_next, pq_next);
-            if (has_pk) pk_next.store(sm.pk + 64 * n * ROW<DT>);
-            if (has_pq) pq_next.store(sm.pq + 64 * n * ROW<DT>);
-        }
-        table_rows<DT, 1>(a, 0, w.row0, 0, which);
-    }
+    Source<DT, S::THREADS> keys(a.k, a, w, h), values(a.v, a, w, h);
+    Stage<DT, S::THREADS> k_next, v_next;
+    Tables<DT, 1, S::THREADS, PK, PQ> tables(a, h);
+    X8 q[2];
+    load_own<DT>(q, a.q, a, w, h, row);
+    tables.template fill<ring>(sm.pk, sm.pq, w.row0);
+    bool far = false, far_next = false;
     auto fetch = [&](int y0) {
-        k_next.load(kp, a.k.l, y0, w.len, a.D);
-        v_next.load(vp, a.v.l, y0, w.len, a.D);
-        if (has_pk || has_pq) {
-            tables(pk_next, pq_next);
-            table_rows<DT, 1>(a, 0, w.row0, y0 + TILE, which);
-        }
+        keys.load(k_next);
+        values.load(v_next);
+        tables.load();
+        tables.look(0, w.row0 - y0 - TILE);
+        if constexpr (PK || PQ) far_next = one_row(a, w.row0 - y0 - 63, w.row0 - y0 + S::ROWS - 1);
     };
     fetch(0);
 
     const float c1 = a.scale * LOG2E;
-    float most[NX], sum[NX];
-#pragma unroll
-    for (int x = 0; x < NX; ++x) most[x] = -__builtin_inff(), sum[x] = 0.f;
+    float most = -__builtin_inff(), sum = 0.f;
     int base = 0;
     for (int y0 = 0; y0 < w.len; y0 += TILE, base = base == 0 ? ring - 64 : base - 64) {
         __syncthreads();
         k_next.store(sm.k);
         v_next.store(sm.v);
-        if (has_pk) pk_next.store(sm.pk + base * ROW<DT>);
-        if (has_pq) pq_next.store(sm.pq + base * ROW<DT>);
+        tables.store(sm.pk, sm.pq, base);
+        far = far_next;
         __syncthreads();
         if (y0 + TILE < w.len) fetch(y0 + TILE);
 
-        f32x4 s[NX][4];
-        scores<DT, NX, ring>(s, q, sm.k, sm.pk, sm.pq, has_pk, has_pq, base, NX * wave, sm.scratch[wave]);
+        f32x4 s[4];
+        scores<DT, ring, PK, PQ>(s, q, sm.k, sm.pk, sm.pq, base, wave, sm.scratch[wave], far);
         if (y0 + TILE > w.len) {
-#pragma unroll
-            for (int x = 0; x < NX; ++x)
-#pragma unroll
-                for (int m = 0; m < 4; ++m)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (y0 + 16 * m + 4 * g + e >= w.len) s[x][m][e] = -__builtin_inff();
-        }
-        X8 p[NX][2];
-#pragma unroll
-        for (int x = 0; x < NX; ++x) {
-            float mx = s[x][0][0];
 #pragma unroll
             for (int m = 0; m < 4; ++m)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) mx = fmaxf(mx, s[x][m][e]);
-            mx = fmaxf(most[x], column_max(mx) * c1);
-            const float from = mx == -__builtin_inff() ? 0.f : mx;       // (a row of nothing but -inf)
-            const float again = __builtin_amdgcn_exp2f(most[x] - from);
-            most[x] = mx;
-            sum[x] *= again;
+                for (int e = 0; e < 4; ++e)
+                    if (y0 + 16 * m + 4 * g + e >= w.len) s[m][e] = -__builtin_inff();
+        }
+        float mx = s[0][0];
 #pragma unroll
-            for (int d = 0; d < 4; ++d) o[x][d] *= again;
-            float part = 0.f;
+        for (int m = 0; m < 4; ++m)
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                uint32_t kept = 0xff;
-                if (a.threshold) kept = tdb_kept(tdb_philox(4 * ((y0 >> 5) + u) + g, row + 16 * x + c, w.b * a.H + h, 1, key), a.threshold);
+            for (int e = 0; e < 4; ++e) mx = fmaxf(mx, s[m][e]);
+        mx = fmaxf(most, column_max(mx) * c1);
+        const float from = mx == -__builtin_inff() ? 0.f : mx;       // (a row of nothing but -inf)
+        const float again = __builtin_amdgcn_exp2f(most - from);
+        most = mx;
+        sum *= again;
 #pragma unroll
-                for (int n = 0; n < 8; ++n) {
-                    const float v = __builtin_amdgcn_exp2f(fmaf(s[x][2 * u + (n >> 2)][n & 3], c1, -from));
-                    part += v;
-                    p[x][u][n] = T((kept >> n & 1) ? v : 0.f);
-                }
+        for (int d = 0; d < 4; ++d) o[d] *= again;
+        X8 p[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            float v[8];
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+                v[n] = __builtin_amdgcn_exp2f(fmaf(s[2 * u + (n >> 2)][n & 3], c1, -from));
+                sum += v[n];
             }
-            sum[x] += part;
+            if (a.threshold) {
+                const uint4 r = tdb_philox(4 * ((y0 >> 5) + u) + g, row + c, w.b * a.H + h, 1, key);
+#pragma unroll
+                for (int n = 0; n < 8; ++n) v[n] = tdb_number(r, n) >= a.threshold ? v[n] : 0.f;
+            }
+#pragma unroll
+            for (int n = 0; n < 8; ++n) p[u][n] = T(v[n]);
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int d = 0; d < 4; ++d) {
-                const X8 v = pair_frag<DT>(sm.v, ROW<DT>, 32 * u, 16 * d);
-#pragma unroll
-                for (int x = 0; x < NX; ++x) o[x][d] = E::mma(v, p[x][u], o[x][d]);
-            }
+            for (int d = 0; d < 4; ++d) o[d] = E::mma(pair_frag<DT>(sm.v, ROW<DT>, 32 * u, 16 * d), p[u], o[d]);
     }
-#pragma unroll
-    for (int x = 0; x < NX; ++x) {
-        const float all = column_sum(sum[x]);
-        store_rows<DT>(a.o, a, w, h, row + 16 * x, o[x], all > 0.f ? a.factor / all : all == 0.f ? 0.f : all);      // (NaN stays)
-        const int r = row + 16 * x + c;
-        if (g == 0 && r < w.len) a.lse[h * a.lines + w.line + r] = all == 0.f ? __builtin_inff() : most[x] + __builtin_amdgcn_logf(all);
-    }
+    const float all = column_sum(sum);
+    store_rows<DT>(a.o, a, w, h, row, o, all > 0.f ? a.factor / all : all == 0.f ? 0.f : all);      // (NaN stays)
+    if (g == 0 && row + c < w.len) a.lse[h * a.lines + w.line + row + c] = all == 0.f ? __builtin_inff() : most + __builtin_amdgcn_logf(all);
 }
 
 // --------------------------------------------------------------------------------------------------------------- backward
 
 // D_i = dO_i . O_i for every row and head: 8 lanes each.  float16: the largest squares of the norms of rows of dO and V as well.
+constexpr int THREADS = 256;
+
 template <int DT>
 __global__ __launch_bounds__(THREADS) void attn_delta_kernel(Args a, uint32_t* largest) {
-    const int64_t unit = (int64_t(blockIdx.x) * THREADS + threadIdx.x) >> 3;
-    const int64_t row = unit / a.H;
-    const int h = int(unit - row * a.H), d = 8 * (threadIdx.x & 7);
-    bool mine = row < a.lines;
-    if (mine) {
+    using T = typename Elem<DT>::T;
+    const int d = 8 * (threadIdx.x & 7);
+    float most_do = 0.f, most_v = 0.f;
+    for (int64_t unit = (int64_t(blockIdx.x) * THREADS + threadIdx.x) >> 3; unit < a.lines * a.H; unit += int64_t(gridDim.x) * (THREADS / 8)) {
+        const int64_t row = unit / a.H;
+        const int h = int(unit - row * a.H);
+        const int64_t b = a.cu ? 0 : row / a.L, r = row - b * a.L * (a.cu ? 0 : 1);
+        bool mine = true;
         if (!a.cu) {
-            const int b = int(row / a.L);
-            mine = !a.seqlens || row - int64_t(b) * a.L < a.seqlens[b];
+            mine = !a.seqlens || r < a.seqlens[b];
         } else if (DT == TDB_F16) {         // rows of no sequence may hold anything
             int lo = 0, hi = a.B;
             while (hi - lo > 1) {
@@ -183,212 +161,219 @@ __global__ __launch_bounds__(THREADS) void attn_delta_kernel(Args a, uint32_t* l
             const int len = valid_rows(a, lo, first);
             mine = row >= first && row < first + len;
         }
-    }
-    float dot = 0.f, sq = 0.f, sv = 0.f;
-    if (mine && d < a.D) {
-        using T = typename Elem<DT>::T;
-        const int64_t b = a.cu ? 0 : row / a.L, r = a.cu ? row : row - b * a.L;
-        const auto o = read8<DT>(static_cast<const T*>(a.o.p) + b * a.o.b + h * a.o.h + r * a.o.l + d);
-        const auto x = read8<DT>(static_cast<const T*>(a.dout.p) + b * a.dout.b + h * a.dout.h + r * a.dout.l + d);
+        float dot = 0.f, sq = 0.f, sv = 0.f;
+        if (mine && d < a.D) {
+            const auto o = read8<DT>(static_cast<const T*>(a.o.p) + b * a.o.b + h * a.o.h + r * a.o.l + d);
+            const auto x = read8<DT>(static_cast<const T*>(a.dout.p) + b * a.dout.b + h * a.dout.h + r * a.dout.l + d);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) dot += float(o[i]) * float(x[i]), sq += float(x[i]) * float(x[i]);
-        if constexpr (DT == TDB_F16) {
-            const auto v = read8<DT>(static_cast<const T*>(a.v.p) + b * a.v.b + h * a.v.h + r * a.v.l + d);
+            for (int i = 0; i < 8; ++i) dot += float(o[i]) * float(x[i]), sq += float(x[i]) * float(x[i]);
+            if constexpr (DT == TDB_F16) {
+                const auto v = read8<DT>(static_cast<const T*>(a.v.p) + b * a.v.b + h * a.v.h + r * a.v.l + d);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sv += float(v[i]) * float(v[i]);
+                for (int i = 0; i < 8; ++i) sv += float(v[i]) * float(v[i]);
+            }
         }
+#pragma unroll
+        for (int n = 1; n < 8; n <<= 1) dot += __shfl_xor(dot, n), sq += __shfl_xor(sq, n), sv += __shfl_xor(sv, n);
+        if (mine && (threadIdx.x & 7) == 0) a.delta[h * a.lines + row] = dot;
+        most_do = fmaxf(most_do, sq), most_v = fmaxf(most_v, sv);
     }
-#pragma unroll
-    for (int n = 1; n < 8; n <<= 1) dot += __shfl_xor(dot, n), sq += __shfl_xor(sq, n), sv += __shfl_xor(sv, n);
-    if (mine && (threadIdx.x & 7) == 0) a.delta[h * a.lines + row] = dot;
     if constexpr (DT == TDB_F16) {
+        __shared__ float s_most[2][THREADS / 64];
 #pragma unroll
-        for (int n = 8; n < 64; n <<= 1) sq = fmaxf(sq, __shfl_xor(sq, n)), sv = fmaxf(sv, __shfl_xor(sv, n));
-        if ((threadIdx.x & 63) == 0) {      // (squares: their bits are in their order; the largest does not depend on theirs)
-            atomicMax(largest, __builtin_bit_cast(uint32_t, sq));
-            atomicMax(largest + 1, __builtin_bit_cast(uint32_t, sv));
+        for (int n = 8; n < 64; n <<= 1) most_do = fmaxf(most_do, __shfl_xor(most_do, n)), most_v = fmaxf(most_v, __shfl_xor(most_v, n));
+        if ((threadIdx.x & 63) == 0) s_most[0][threadIdx.x >> 6] = most_do, s_most[1][threadIdx.x >> 6] = most_v;
+        __syncthreads();
+        if (threadIdx.x < 2) {              // (squares: their bits are in their order; the largest does not depend on it)
+            const float* const m = s_most[threadIdx.x];
+            atomicMax(largest + threadIdx.x, __builtin_bit_cast(uint32_t, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]))));
         }
     }
 }
 
 __global__ void clear_kernel(uint32_t* x) { x[threadIdx.x] = 0; }
 
-// A skewed tile: row x has the values of y at index 79 - y, zeros on both sides.  A row is 97 values apart from the next, so that
-// index 16 + r - x of row x, r = x - y + 63, lies at 96 x + 16 + r: eight neighbouring r at a multiple of 8.
-constexpr int SKEW = 97, SKEWED = 16 * SKEW + 32;
+// A skewed tile: row x has the values of y at index 79 - y.  A row is 105 values apart from the next, so that index 16 + r - x of row x, r = x - y + 63, lies at
+// 104 x + 16 + r: eight neighbouring r at a multiple of 8, and 16 x on distinct banks.  r runs to 95: what lies outside of 0 <= y < 64 is not the row's.
+constexpr int SKEW = 105, SKEWED = 16 * SKEW;
 
-template <int DT, int NX>
+// The eight r = 32 n + 8 g .. of the lane's row, zeros outside.
+template <int DT>
+__device__ __forceinline__ typename Elem<DT>::X8 skew_frag(const typename Elem<DT>::T* skewed, int n) {
+    const int c = lane_c(), r = 32 * n + 8 * lane_g();
+    typename Elem<DT>::X8 x = read8<DT>(skewed + c * (SKEW - 1) + 16 + r);
+    if (n == 1) return x;               // (c <= r <= c + 63)
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (n == 0 ? r + i < c : r + i > c + 63) x[i] = typename Elem<DT>::T(0.f);
+    return x;
+}
+
+template <int DT>
 struct KvLds {
     using T = typename Elem<DT>::T;
-    alignas(16) T q[TILE * ROW<DT>], dout[TILE * ROW<DT>], pk[RING<DT, NX> * ROW<DT>], pq[RING<DT, NX> * ROW<DT>];
-    alignas(16) T skewed[4][NX * SKEWED];
+    using S = Shape<DT>;
+    alignas(16) T q[TILE * ROW<DT>], dout[TILE * ROW<DT>], pk[S::RING * ROW<DT>], pq[S::RING * ROW<DT>];
     alignas(16) float lse[TILE], delta[TILE];
-    alignas(16) uint32_t kept[4][TILE];
-    alignas(16) float scratch[4][TERMS<NX>];
+    alignas(16) uint32_t kept[2][S::WAVES / 2][TILE];       // a bit for each of 32 keys
+    alignas(16) float scratch[S::WAVES][TERMS];             // of the scores; then the skewed gradients of scores
+    static_assert(SKEWED * sizeof(T) <= TERMS * sizeof(float), "");
 };
 
-template <int DT, int NX>
-__global__ __launch_bounds__(THREADS, 1) void attn_bwd_kv_kernel(Args a) {
+template <int DT, bool PK, bool PQ>
+__global__ __launch_bounds__(Shape<DT>::THREADS, 1) void attn_bwd_kv_kernel(Args a) {
     using E = Elem<DT>;
     using T = typename E::T;
     using X8 = typename E::X8;
-    constexpr int ring = RING<DT, NX>;
+    using S = Shape<DT>;
+    constexpr int ring = S::RING;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    KvLds<DT, NX>& sm = *reinterpret_cast<KvLds<DT, NX>*>(smem);
+    KvLds<DT>& sm = *reinterpret_cast<KvLds<DT>*>(smem);
     int h;
     Where w;
-    if (!locate<64 * NX>(a, h, w)) return;
+    if (!locate<S::ROWS>(a, h, w)) return;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane_c(), g = lane_g();
-    const int row = w.row0 + 16 * NX * wave;        // the wave's first key
-    f32x4 dk[NX][4], dv[NX][4];
+    const int row = w.row0 + 16 * wave;             // the wave's first key
+    f32x4 dk[4], dv[4];
 #pragma unroll
-    for (int x = 0; x < NX; ++x)
-#pragma unroll
-        for (int d = 0; d < 4; ++d) dk[x][d] = dv[x][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int d = 0; d < 4; ++d) dk[d] = dv[d] = f32x4{0.f, 0.f, 0.f, 0.f};
     if (w.row0 >= w.len) {
-#pragma unroll
-        for (int x = 0; x < NX; ++x) store_rows<DT>(a.dk, a, w, h, row + 16 * x, dk[x], 0.f), store_rows<DT>(a.dv, a, w, h, row + 16 * x, dv[x], 0.f);
+        store_rows<DT>(a.dk, a, w, h, row, dk, 0.f);
+        store_rows<DT>(a.dv, a, w, h, row, dv, 0.f);
         return;
     }
-    const T *const qp = rows_of<DT>(a.q, a, w, h), *const dop = rows_of<DT>(a.dout, a, w, h);
-    const T *const pk = static_cast<const T*>(a.pk.p) + h * a.pk.h, *const pq = static_cast<const T*>(a.pq.p) + h * a.pq.h;
-    const bool has_pk = a.pk.p, has_pq = a.pq.p;
+    Source<DT, S::THREADS> queries(a.q, a, w, h), douts(a.dout, a, w, h);
+    Stage<DT, S::THREADS> q_next, do_next;
+    Tables<DT, -1, S::THREADS, PK, PQ> tables(a, h);
+    X8 k[2], v[2];
+    load_own<DT>(k, a.k, a, w, h, row);
+    load_own<DT>(v, a.v, a, w, h, row);
+    tables.template fill<ring>(sm.pk, sm.pq, w.row0);
     const TdbKey key = a.threshold ? tdb_key(a.seed) : TdbKey{0, 0};
     const float power = score_power<DT>(a), rounded = w.len > 1 ? power : 0.f;      // (the softmax of one key is a constant)
-    X8 k[NX][2], v[NX][2];
-    load_own<DT, NX>(k, a.k, a, w, h, row);
-    load_own<DT, NX>(v, a.v, a, w, h, row);
-    T* const skewed = sm.skewed[wave];
-    for (int n = lane; n < NX * SKEWED; n += 64) skewed[n] = T(0.f);
-
-    Stage<DT> q_next, do_next, pk_next, pq_next;
+    const __amdgpu_buffer_rsrc_t lines = buffer((wave == 0 ? a.lse : a.delta) + h * a.lines + w.line, int64_t(w.len) * 4);      // of the waves that load them
     float line_next = 0.f;
-    int which[LOADS<DT>];
-    auto tables = [&](Stage<DT>& s1, Stage<DT>& s2) {
-        if (has_pk) s1.load(pk, a.pk.l, which, a.D);
-        if (has_pq) s2.load(pq, a.pq.l, which, a.D);
-    };
-    if (has_pk || has_pq) {
-#pragma unroll
-        for (int n = 1; n <= NX; ++n) {
-            table_rows<DT, -1>(a, 64 * n, w.row0, 0, which);
-            tables(pk_next, pq_next);
-            if (has_pk) pk_next.store(sm.pk + 64 * n * ROW<DT>);
-            if (has_pq) pq_next.store(sm.pq + 64 * n * ROW<DT>);
-        }
-        table_rows<DT, -1>(a, 0, w.row0, 0, which);
-    }
-    const float* const lines = (threadIdx.x < TILE ? a.lse : a.delta) + h * a.lines + w.line;
+    bool far = false, far_next = false;
     auto fetch = [&](int y0) {
-        q_next.load(qp, a.q.l, y0, w.len, a.D);
-        do_next.load(dop, a.dout.l, y0, w.len, a.D);
-        if (threadIdx.x < 2 * TILE) {
-            const int r = y0 + (threadIdx.x & (TILE - 1));
-            line_next = r < w.len ? lines[r] : threadIdx.x < TILE ? __builtin_inff() : 0.f;
-        }
-        if (has_pk || has_pq) {
-            tables(pk_next, pq_next);
-            table_rows<DT, -1>(a, 0, w.row0, y0 + TILE, which);
-        }
+        queries.load(q_next);
+        douts.load(do_next);
+        if (wave < 2) line_next = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(lines, lane * 4, y0 * 4, 0));
+        tables.load();
+        tables.look(0, w.row0 - y0 - TILE);
+        if constexpr (PK || PQ) far_next = one_row(a, y0 - w.row0 - S::ROWS + 1, y0 - w.row0 + 63);
     };
     fetch(0);
+    // Which of 32 keys are kept for the queries of a step: the two waves that have the keys share the work, a step ahead.  A lane has a query and two of the four counters
+    // whose numbers are those of the keys: 4 neighbouring ones of each half.
+    auto draw = [&](int y0, int to) {
+        const int query = 32 * (wave & 1) + (lane & 31), n = lane >> 5;
+        uint32_t low = 0, high = 0;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t kept = tdb_kept(tdb_philox(4 * (row >> 5) + 2 * n + i, y0 + query, w.b * a.H + h, 1, key), a.threshold);
+            low |= (kept & 15) << (4 * i), high |= (kept >> 4) << (4 * i);
+        }
+        uint8_t* const bytes = reinterpret_cast<uint8_t*>(&sm.kept[to][wave >> 1][query]);
+        bytes[n] = uint8_t(low), bytes[2 + n] = uint8_t(high);
+    };
+    if (a.threshold) draw(0, 0);
 
     const float c1 = a.scale * LOG2E, shift = DT == TDB_F16 ? float(a.p_shift) : 0.f, unshift = DT == TDB_F16 ? ldexpf(1.f, -a.p_shift) : 1.f;
-    const bool edge = w.row0 + 64 * NX > w.len;
-    const int tile_col = row / TILE, block = row / 16 % 4;
-    T* const ds = static_cast<T*>(a.ds) + ((int64_t(h - a.head0) * a.row_tiles + w.row_tile) * a.tiles + tile_col) * TILE_VALUES + (block * 128 + lane) * 8;
-    int base = 0;
-    for (int y0 = 0; y0 < w.len; y0 += TILE, base = base == 0 ? ring - 64 : base - 64) {
+    const float down = unshift * rounded;
+    const bool edge = w.row0 + S::ROWS > w.len;
+    const int tile_col = row / TILE, bit = (row & 16) + c;
+    T* ds = static_cast<T*>(a.ds) + ((int64_t(h - a.head0) * a.row_tiles + w.row_tile) * a.tiles + tile_col) * TILE_VALUES + (row / 16 % 4 * 128 + lane) * 8;
+    T* const skewed = reinterpret_cast<T*>(sm.scratch[wave]);
+    int base = 0, odd = 0;
+    for (int y0 = 0; y0 < w.len; y0 += TILE, base = base == 0 ? ring - 64 : base - 64, ds += int64_t(a.tiles) * TILE_VALUES, odd ^= 1) {
         __syncthreads();
         q_next.store(sm.q);
         do_next.store(sm.dout);
-        if (has_pk) pk_next.store(sm.pk + base * ROW<DT>);
-        if (has_pq) pq_next.store(sm.pq + base * ROW<DT>);
-        if (threadIdx.x < 2 * TILE) (threadIdx.x < TILE ? sm.lse : sm.delta)[threadIdx.x & (TILE - 1)] = line_next;
+        tables.store(sm.pk, sm.pq, base);
+        if (wave < 2) (wave == 0 ? sm.lse : sm.delta)[lane] = line_next;
+        far = far_next;
         __syncthreads();
-        if (y0 + TILE < w.len) fetch(y0 + TILE);
-
-        if (a.threshold) {      // a lane has a query: whether each of the wave's keys is kept
-            uint32_t bits = 0;
-#pragma unroll
-            for (int n = 0; n < 4; ++n) {
-                const uint32_t kept = tdb_kept(tdb_philox(4 * (row >> 5) + n, y0 + lane, w.b * a.H + h, 1, key), a.threshold);
-                if constexpr (NX == 2) bits |= (kept & 15) << (4 * n) | (kept >> 4) << (16 + 4 * n);
-                else bits |= (kept >> (row & 16 ? 4 : 0) & 15) << (4 * n);
-            }
-            sm.kept[wave][lane] = bits;
-            wave_fence();
+        if (y0 + TILE < w.len) {
+            fetch(y0 + TILE);
+            if (a.threshold) draw(y0 + TILE, odd ^ 1);
         }
-        f32x4 s[NX][4], dp[NX][4];
-        scores<DT, NX, ring>(s, k, sm.q, sm.pq, sm.pk, has_pq, has_pk, base, NX * wave, sm.scratch[wave]);
+        f32x4 s[4], dp[4];
+        scores<DT, ring, PQ, PK>(s, k, sm.q, sm.pq, sm.pk, base, wave, sm.scratch[wave], far);
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+            dp[m] = E::mma(row_frag<DT>(sm.dout, 16 * m, 32), v[1], E::mma(row_frag<DT>(sm.dout, 16 * m, 0), v[0], f32x4{0.f, 0.f, 0.f, 0.f}));
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
-            const X8 d0 = row_frag<DT>(sm.dout, 16 * m, 0), d1 = row_frag<DT>(sm.dout, 16 * m, 32);
+            const f32x4 lse = *reinterpret_cast<const f32x4*>(sm.lse + 16 * m + 4 * g);
 #pragma unroll
-            for (int x = 0; x < NX; ++x) dp[x][m] = E::mma(d1, v[x][1], E::mma(d0, v[x][0], f32x4{0.f, 0.f, 0.f, 0.f}));
+            for (int e = 0; e < 4; ++e) s[m][e] = __builtin_amdgcn_exp2f(fmaf(s[m][e], c1, shift - lse[e]));
         }
-        const bool some = edge || y0 + TILE > w.len;
-        X8 p[NX][2], dsx[NX][2];
+        if (edge || y0 + TILE > w.len) {        // rows and keys behind the sequence, whatever they have given
+#pragma unroll
+            for (int m = 0; m < 4; ++m)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (y0 + 16 * m + 4 * g + e >= w.len || row + c >= w.len) s[m][e] = 0.f, dp[m][e] = 0.f;
+        }
+        X8 p[2], dsx[2];
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
-            const f32x4 lse = *reinterpret_cast<const f32x4*>(sm.lse + 16 * m + 4 * g), delta = *reinterpret_cast<const f32x4*>(sm.delta + 16 * m + 4 * g);
-            uint32_t kept[4] = {~0u, ~0u, ~0u, ~0u};
+            const f32x4 delta = *reinterpret_cast<const f32x4*>(sm.delta + 16 * m + 4 * g);
+            f32x4 pr = s[m], grad = dp[m];
             if (a.threshold) {
-                const u32x4 words = *reinterpret_cast<const u32x4*>(sm.kept[wave] + 16 * m + 4 * g);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) kept[e] = words[e];
-            }
-#pragma unroll
-            for (int x = 0; x < NX; ++x)
+                const u32x4 words = *reinterpret_cast<const u32x4*>(sm.kept[odd][wave >> 1] + 16 * m + 4 * g);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    float pr = __builtin_amdgcn_exp2f(fmaf(s[x][m][e], c1, shift - lse[e]));
-                    float grad = dp[x][m][e];
-                    if (some && (y0 + 16 * m + 4 * g + e >= w.len || row + 16 * x + c >= w.len)) pr = 0.f, grad = 0.f;
-                    const bool in = kept[e] >> (16 * x + c) & 1;
-                    p[x][m >> 1][4 * (m & 1) + e] = T(in ? pr : 0.f);
-                    dsx[x][m >> 1][4 * (m & 1) + e] = T(pr * unshift * ((in ? grad * a.factor : 0.f) - delta[e]) * rounded);
+                    const bool in = words[e] >> bit & 1;
+                    pr[e] = in ? pr[e] : 0.f;
+                    grad[e] = in ? grad[e] * a.factor : 0.f;
                 }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                p[m >> 1][4 * (m & 1) + e] = T(pr[e]);
+                dsx[m >> 1][4 * (m & 1) + e] = T(s[m][e] * ((grad[e] - delta[e]) * down));
+            }
         }
         if (tile_col * TILE < w.len) {
-            T* const to = ds + int64_t(y0 / TILE) * a.tiles * TILE_VALUES;
 #pragma unroll
-            for (int x = 0; x < NX; ++x)
+            for (int u = 0; u < 2; ++u) *reinterpret_cast<X8*>(ds + u * 64 * 8) = dsx[u];
+        }
+        if (PQ && !far) {
 #pragma unroll
-                for (int u = 0; u < 2; ++u) *reinterpret_cast<X8*>(to + (x * 128 + u * 64) * 8) = dsx[x][u];
+            for (int n = 0; n < 16; ++n) skewed[c * SKEW + 79 - 16 * (n >> 2) - 4 * g - (n & 3)] = dsx[n >> 3][n & 7];
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int d = 0; d < 4; ++d) {
-                const X8 o = pair_frag<DT>(sm.dout, ROW<DT>, 32 * u, 16 * d), q = pair_frag<DT>(sm.q, ROW<DT>, 32 * u, 16 * d);
-#pragma unroll
-                for (int x = 0; x < NX; ++x) dv[x][d] = E::mma(o, p[x][u], dv[x][d]), dk[x][d] = E::mma(q, dsx[x][u], dk[x][d]);
+                dv[d] = E::mma(pair_frag<DT>(sm.dout, ROW<DT>, 32 * u, 16 * d), p[u], dv[d]);
+                dk[d] = E::mma(pair_frag<DT>(sm.q, ROW<DT>, 32 * u, 16 * d), dsx[u], dk[d]);
             }
-        if (has_pq) {
-            wave_fence();
+        if constexpr (PQ) {
+            if (far) {
+                const T* const same = sm.pq + wrapped<ring>(63 + base) * ROW<DT>;
 #pragma unroll
-            for (int x = 0; x < NX; ++x)
+                for (int d = 0; d < 4; ++d) {
+                    const X8 t = level_frag<DT>(same, 16 * d);
 #pragma unroll
-                for (int n = 0; n < 16; ++n) skewed[x * SKEWED + c * SKEW + 79 - 16 * (n >> 2) - 4 * g - (n & 3)] = dsx[x][n >> 3][n & 7];
-            wave_fence();
-#pragma unroll
-            for (int x = 0; x < NX; ++x)
+                    for (int u = 0; u < 2; ++u) dk[d] = E::mma(t, dsx[u], dk[d]);
+                }
+            } else {
+                wave_fence();
 #pragma unroll
                 for (int n = 0; n < 3; ++n) {
-                    const X8 b = read8<DT>(skewed + x * SKEWED + c * (SKEW - 1) + 16 + 32 * n + 8 * g);
-                    const int at = wrapped<ring>(16 * (NX * wave + x) + 32 * n + 8 * g + base);
+                    const X8 b = skew_frag<DT>(skewed, n);
+                    const int at = wrapped<ring>(16 * wave + 32 * n + 8 * g + base);
 #pragma unroll
-                    for (int d = 0; d < 4; ++d) dk[x][d] = E::mma(turned_frag<DT>(sm.pq, ROW<DT>, at, at + 4, 16 * d), b, dk[x][d]);
+                    for (int d = 0; d < 4; ++d) dk[d] = E::mma(turned_frag<DT>(sm.pq, ROW<DT>, at, at + 4, 16 * d), b, dk[d]);
                 }
-            wave_fence();
+                wave_fence();
+            }
         }
     }
-#pragma unroll
-    for (int x = 0; x < NX; ++x) {
-        store_rows<DT>(a.dk, a, w, h, row + 16 * x, dk[x], a.scale / power);
-        store_rows<DT>(a.dv, a, w, h, row + 16 * x, dv[x], a.factor * unshift);
-    }
+    store_rows<DT>(a.dk, a, w, h, row, dk, a.scale / power);
+    store_rows<DT>(a.dv, a, w, h, row, dv, a.factor * unshift);
 }
 
 // A tile of dS as bwd_kv leaves it: 8 values each of 512 lanes: key 16 blk + c, queries 32 u + 4 g + e and 32 u + 16 + 4 g + e.
@@ -399,6 +384,16 @@ struct Scores {
     __device__ __forceinline__ void load(const typename Elem<DT>::T* tile) {
 #pragma unroll
         for (int n = 0; n < 2; ++n) x[n] = read8<DT>(tile + (n * THREADS + threadIdx.x) * 8);
+    }
+    // as rows of keys, columns of queries
+    __device__ __forceinline__ void store(typename Elem<DT>::T* rows) const {
+        typedef __attribute__((ext_vector_type(4))) typename Elem<DT>::T T4;
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            typename Elem<DT>::T* const to = rows + key(n) * ROW<DT> + query(0);
+            *reinterpret_cast<T4*>(to) = __builtin_shufflevector(x[n], x[n], 0, 1, 2, 3);
+            *reinterpret_cast<T4*>(to + 16) = __builtin_shufflevector(x[n], x[n], 4, 5, 6, 7);
+        }
     }
     static __device__ __forceinline__ int key(int n) { return 16 * ((n * THREADS + threadIdx.x) >> 7) + lane_c(); }
     static __device__ __forceinline__ int query(int i) { return 32 * (threadIdx.x >> 6 & 1) + 16 * (i >> 2) + 4 * lane_g() + (i & 3); }
@@ -411,23 +406,22 @@ struct QLds {
 };
 
 // dq: a workgroup has 64 queries, a wave 16.
-template <int DT>
+template <int DT, bool PK>
 __global__ __launch_bounds__(THREADS, DT == TDB_F32 ? 1 : 2) void attn_bwd_q_kernel(Args a) {
     using E = Elem<DT>;
     using T = typename E::T;
     using X8 = typename E::X8;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     QLds<DT>& sm = *reinterpret_cast<QLds<DT>*>(smem);
-    if (a.cu && threadIdx.x < 64) {
+    if (a.cu && threadIdx.x < 64 && a.head0 == 0) {
         const Tensor* const all[] = {&a.dq, &a.dk, &a.dv};
-        if (a.head0 == 0)
-            for (const Tensor* t : all)
-                tdb_fill_gaps(a.cu, a.B, a.L, a.total, static_cast<char*>(t->p), t->l * sizeof(T), t->h * sizeof(T), a.H, a.D * sizeof(T), blockIdx.x, gridDim.x);
+        for (const Tensor* t : all)
+            tdb_fill_gaps(a.cu, a.B, a.L, a.total, static_cast<char*>(t->p), t->l * sizeof(T), t->h * sizeof(T), a.H, a.D * sizeof(T), blockIdx.x, gridDim.x);
     }
     int h;
     Where w;
     if (!locate<TILE>(a, h, w)) return;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane_c(), g = lane_g();
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane_g();
     f32x4 dq[4];
 #pragma unroll
     for (int d = 0; d < 4; ++d) dq[d] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -435,47 +429,37 @@ __global__ __launch_bounds__(THREADS, DT == TDB_F32 ? 1 : 2) void attn_bwd_q_ker
         store_rows<DT>(a.dq, a, w, h, w.row0 + 16 * wave, dq, 0.f);
         return;
     }
-    const T* const kp = rows_of<DT>(a.k, a, w, h);
-    const T* const pk = static_cast<const T*>(a.pk.p) + h * a.pk.h;
-    const bool has_pk = a.pk.p;
-    const T* const tiles = static_cast<const T*>(a.ds) + (int64_t(h - a.head0) * a.row_tiles + w.row_tile + w.row0 / TILE) * a.tiles * TILE_VALUES;
-    for (int n = threadIdx.x; n < 4 * SKEWED; n += THREADS) sm.skewed[0][n] = T(0.f);
-    Stage<DT> k_next, pk_next;
+    const T* tile = static_cast<const T*>(a.ds) + (int64_t(h - a.head0) * a.row_tiles + w.row_tile + w.row0 / TILE) * a.tiles * TILE_VALUES;
+    Source<DT, THREADS> keys(a.k, a, w, h);
+    Stage<DT, THREADS> k_next;
     Scores<DT> ds_next;
-    int which[LOADS<DT>];
-    if (has_pk) {
-        table_rows<DT, 1>(a, 64, w.row0, 0, which);
-        pk_next.load(pk, a.pk.l, which, a.D);
-        pk_next.store(sm.pk + 64 * ROW<DT>);
-        table_rows<DT, 1>(a, 0, w.row0, 0, which);
-    }
+    Tables<DT, 1, THREADS, PK, false> tables(a, h);
+    tables.template fill<128>(sm.pk, nullptr, w.row0);
+    bool far = false, far_next = false;
     auto fetch = [&](int y0) {
-        k_next.load(kp, a.k.l, y0, w.len, a.D);
-        ds_next.load(tiles + int64_t(y0 / TILE) * TILE_VALUES);
-        if (has_pk) {
-            pk_next.load(pk, a.pk.l, which, a.D);
-            table_rows<DT, 1>(a, 0, w.row0, y0 + TILE, which);
-        }
+        keys.load(k_next);
+        ds_next.load(tile);
+        tile += TILE_VALUES;
+        tables.load();
+        tables.look(0, w.row0 - y0 - TILE);
+        if constexpr (PK) far_next = one_row(a, w.row0 - y0 - 63, w.row0 - y0 + 63);
     };
     fetch(0);
     int base = 0;
     for (int y0 = 0; y0 < w.len; y0 += TILE, base ^= 64) {
         __syncthreads();
         k_next.store(sm.k);
-        if (has_pk) pk_next.store(sm.pk + base * ROW<DT>);
+        tables.store(sm.pk, nullptr, base);
+        far = far_next;
+        ds_next.store(sm.ds);
+        if (PK && !far) {
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            const int j = Scores<DT>::key(n), i = Scores<DT>::query(0);
-            typedef __attribute__((ext_vector_type(4))) T T4;
-            *reinterpret_cast<T4*>(sm.ds + j * ROW<DT> + i) = __builtin_shufflevector(ds_next.x[n], ds_next.x[n], 0, 1, 2, 3);
-            *reinterpret_cast<T4*>(sm.ds + j * ROW<DT> + i + 16) = __builtin_shufflevector(ds_next.x[n], ds_next.x[n], 4, 5, 6, 7);
-            if (has_pk) {
+            for (int n = 0; n < 2; ++n)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const int q = Scores<DT>::query(e);
-                    sm.skewed[q >> 4][(q & 15) * SKEW + 79 - j] = ds_next.x[n][e];
+                    sm.skewed[q >> 4][(q & 15) * SKEW + 79 - Scores<DT>::key(n)] = ds_next.x[n][e];
                 }
-            }
         }
         __syncthreads();
         if (y0 + TILE < w.len) fetch(y0 + TILE);
@@ -483,12 +467,15 @@ __global__ __launch_bounds__(THREADS, DT == TDB_F32 ? 1 : 2) void attn_bwd_q_ker
         for (int n = 0; n < 2; ++n) {
             const X8 b = line_frag<DT>(sm.ds, ROW<DT>, 32 * n, 16 * wave);
 #pragma unroll
-            for (int d = 0; d < 4; ++d) dq[d] = E::mma(line_frag<DT>(sm.k, ROW<DT>, 32 * n, 16 * d), b, dq[d]);
+            for (int d = 0; d < 4; ++d) {
+                dq[d] = E::mma(line_frag<DT>(sm.k, ROW<DT>, 32 * n, 16 * d), b, dq[d]);
+                if (PK && far) dq[d] = E::mma(level_frag<DT>(sm.pk + ((63 + base) & 127) * ROW<DT>, 16 * d), b, dq[d]);
+            }
         }
-        if (has_pk) {
+        if (PK && !far) {
 #pragma unroll
             for (int n = 0; n < 3; ++n) {
-                const X8 b = read8<DT>(sm.skewed[wave] + c * (SKEW - 1) + 16 + 32 * n + 8 * g);
+                const X8 b = skew_frag<DT>(sm.skewed[wave], n);
                 const int at = (16 * wave + 32 * n + 8 * g + base) & 127;
 #pragma unroll
                 for (int d = 0; d < 4; ++d) dq[d] = E::mma(turned_frag<DT>(sm.pk, ROW<DT>, at, at + 4, 16 * d), b, dq[d]);
@@ -498,7 +485,11 @@ __global__ __launch_bounds__(THREADS, DT == TDB_F32 ? 1 : 2) void attn_bwd_q_ker
     store_rows<DT>(a.dq, a, w, h, w.row0 + 16 * wave, dq, a.scale / score_power<DT>(a));
 }
 
-// Tables: a workgroup has a diagonal of tiles (query tile - key tile = t) of every `splits`-th sequence, a wave 32 of its 128 offsets r = i - j + 63.
+// Parts that the sequences of a diagonal are dealt to: as many as it has tiles, next to the longest one.
+__device__ __forceinline__ int splits_of(const Args& a, int t) { return max(1, a.splits * (a.tiles - abs(t)) / a.tiles); }
+
+// Tables: a workgroup has a diagonal of tiles (query tile - key tile = t) of every `splits`-th sequence, a wave 32 of its 128 offsets r = i - j + 63.  Where all offsets
+// of a diagonal have one table row ("far") their sum is all that is wanted: Q^T dS and K^T dS^T, whose columns are added up at the end, one row for each wave.
 constexpr int BY_OFFSET = 128;
 template <int DT>
 constexpr int OFFSET_ROW = DT == TDB_F32 ? BY_OFFSET + 4 : BY_OFFSET + 8;
@@ -509,7 +500,19 @@ struct TablesLds {
     alignas(16) T q[TILE * ROW<DT>], k[TILE * ROW<DT>], by_query[TILE * OFFSET_ROW<DT>], by_key[TILE * OFFSET_ROW<DT>];
 };
 
-template <int DT>
+// Sum over the 16 lanes of a row of a result.
+__device__ __forceinline__ float row_sum(float x) {
+    auto turn = [](float v, auto ctrl) {
+        return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), decltype(ctrl)::value, 0xf, 0xf, true));
+    };
+    x += turn(x, std::integral_constant<int, 0x128>{});
+    x += turn(x, std::integral_constant<int, 0x124>{});
+    x += turn(x, std::integral_constant<int, 0x122>{});
+    x += turn(x, std::integral_constant<int, 0x121>{});
+    return x;
+}
+
+template <int DT, bool PK, bool PQ>
 __global__ __launch_bounds__(THREADS, DT == TDB_F32 ? 1 : 2) void attn_bwd_tables_kernel(Args a) {
     using E = Elem<DT>;
     using T = typename E::T;
@@ -518,22 +521,25 @@ __global__ __launch_bounds__(THREADS, DT == TDB_F32 ? 1 : 2) void attn_bwd_table
     TablesLds<DT>& sm = *reinterpret_cast<TablesLds<DT>*>(smem);
     const int diagonals = 2 * a.tiles - 1, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane_c(), g = lane_g();
     const int split = blockIdx.x % a.splits, at = blockIdx.x / a.splits, t = at % diagonals - (a.tiles - 1), h = a.head0 + at / diagonals;
-    const bool has_pk = a.pk.p, has_pq = a.pq.p;
+    const int splits = splits_of(a, t);
+    if (split >= splits) return;
+    const bool far = one_row(a, TILE * t - 63, TILE * t + 63);
     f32x4 dpk[2][4], dpq[2][4];
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int d = 0; d < 4; ++d) dpk[n][d] = dpq[n][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int n = threadIdx.x; n < TILE * OFFSET_ROW<DT>; n += THREADS) sm.by_query[n] = sm.by_key[n] = T(0.f);
+    if (!far)
+        for (int n = threadIdx.x; n < TILE * OFFSET_ROW<DT>; n += THREADS) sm.by_query[n] = sm.by_key[n] = T(0.f);
 
-    Stage<DT> q_next, k_next;
+    Stage<DT, THREADS> q_next, k_next;
     Scores<DT> ds_next;
     Where w;
     int it = 0, end = 0;
-    w.b = split - a.splits;
+    w.b = split - splits;
     auto advance = [&]() {              // to the next tile; false: none is left
         for (++it; it >= end;) {
-            w.b += a.splits;
+            w.b += splits;
             if (w.b >= a.B) return false;
             w.len = valid_rows(a, w.b, w.first);
             w.row_tile = a.cu ? w.first / TILE + w.b : int64_t(w.b) * a.tiles;
@@ -543,29 +549,44 @@ __global__ __launch_bounds__(THREADS, DT == TDB_F32 ? 1 : 2) void attn_bwd_table
         return true;
     };
     auto fetch = [&]() {
-        q_next.load(rows_of<DT>(a.q, a, w, h), a.q.l, it * TILE, w.len, a.D);
-        k_next.load(rows_of<DT>(a.k, a, w, h), a.k.l, (it - t) * TILE, w.len, a.D);
+        if constexpr (PK) Source<DT, THREADS>(a.q, a, w, h, it * TILE).load(q_next);
+        if constexpr (PQ) Source<DT, THREADS>(a.k, a, w, h, (it - t) * TILE).load(k_next);
         ds_next.load(static_cast<const T*>(a.ds) + ((int64_t(h - a.head0) * a.row_tiles + w.row_tile + it) * a.tiles + it - t) * TILE_VALUES);
     };
     bool more = advance();
     if (more) fetch();
     while (more) {
         __syncthreads();
-        q_next.store(sm.q);
-        k_next.store(sm.k);
+        if constexpr (PK) q_next.store(sm.q);
+        if constexpr (PQ) k_next.store(sm.k);
+        if (far) {
+            if constexpr (PQ) ds_next.store(sm.by_key);
+        } else {
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            const int j = Scores<DT>::key(n);
+            for (int n = 0; n < 2; ++n) {
+                const int j = Scores<DT>::key(n);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int i = Scores<DT>::query(e);
-                if (has_pk) sm.by_query[i * OFFSET_ROW<DT> + i - j + 63] = ds_next.x[n][e];
-                if (has_pq) sm.by_key[j * OFFSET_ROW<DT> + i - j + 63] = ds_next.x[n][e];
+                for (int e = 0; e < 8; ++e) {
+                    const int i = Scores<DT>::query(e);
+                    if constexpr (PK) sm.by_query[i * OFFSET_ROW<DT> + i - j + 63] = ds_next.x[n][e];
+                    if constexpr (PQ) sm.by_key[j * OFFSET_ROW<DT> + i - j + 63] = ds_next.x[n][e];
+                }
             }
         }
+        const Scores<DT> ds = ds_next;
         __syncthreads();
         more = advance();
         if (more) fetch();
+        if (far) {                      // the wave's two pieces of dS, queries in pairs; 16 queries of dS as rows of keys
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                    if constexpr (PK) dpk[n][d] = E::mma(pair_frag<DT>(sm.q, ROW<DT>, 32 * (wave & 1), 16 * d), ds.x[n], dpk[n][d]);
+                    if constexpr (PQ) dpq[n][d] = E::mma(line_frag<DT>(sm.k, ROW<DT>, 32 * n, 16 * d), line_frag<DT>(sm.by_key, ROW<DT>, 32 * n, 16 * wave), dpq[n][d]);
+                }
+            continue;
+        }
         auto add = [&](f32x4 (&acc)[2][4], const T* rows, const T* by) {
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
@@ -580,21 +601,33 @@ __global__ __launch_bounds__(THREADS, DT == TDB_F32 ? 1 : 2) void attn_bwd_table
                 }
             }
         };
-        if (has_pk) add(dpk, sm.q, sm.by_query);
-        if (has_pq) add(dpq, sm.k, sm.by_key);
+        if constexpr (PK) add(dpk, sm.q, sm.by_query);
+        if constexpr (PQ) add(dpq, sm.k, sm.by_key);
     }
     float* const part = a.partial + int64_t(blockIdx.x) * 2 * BY_OFFSET * 64;
+    if (far) {
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            f32x4 x = dpk[0][d] + dpk[1][d], y = dpq[0][d] + dpq[1][d];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = row_sum(x[e]), y[e] = row_sum(y[e]);
+            const int to = wave * 64 + 16 * d + 4 * g;
+            if (PK && c == 0) *reinterpret_cast<f32x4*>(part + to) = x;
+            if (PQ && c == 0) *reinterpret_cast<f32x4*>(part + BY_OFFSET * 64 + to) = y;
+        }
+        return;
+    }
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
             const int to = (32 * wave + 16 * n + c) * 64 + 16 * d + 4 * g;
-            if (has_pk) *reinterpret_cast<f32x4*>(part + to) = dpk[n][d];
-            if (has_pq) *reinterpret_cast<f32x4*>(part + BY_OFFSET * 64 + to) = dpq[n][d];
+            if constexpr (PK) *reinterpret_cast<f32x4*>(part + to) = dpk[n][d];
+            if constexpr (PQ) *reinterpret_cast<f32x4*>(part + BY_OFFSET * 64 + to) = dpq[n][d];
         }
 }
 
-// The first offset in [-(L - 1), L) whose table row is `row` or a later one (the lookup table does not decrease): 64 places at a time.
+// The first offset in [1 - L, L) whose table row is `row` or a later one (the lookup table does not decrease), L if there is none: 64 places at a time.
 __device__ __forceinline__ int first_offset(const Args& a, int row) {
     int lo = 1 - a.L, hi = a.L;             // the answer lies in [lo, hi]
     while (lo < hi) {
@@ -608,28 +641,48 @@ __device__ __forceinline__ int first_offset(const Args& a, int row) {
     return lo;
 }
 
-// A table row's gradient: the offsets that share it, each in the one or two diagonals whose tiles have it, and their splits.  Four waves share the offsets.
+// A table row's gradient, offsets lo .. hi - 1: those of far diagonals come as four rows of each diagonal; the others, fewer than 128 at either end, from the one or two
+// diagonals whose tiles have them.  A wave for each row.
 template <int DT>
 __global__ __launch_bounds__(THREADS) void tables_sum_kernel(Args a) {
-    __shared__ float s_sum[4][64];
-    const int which = blockIdx.z, h = a.head0 + blockIdx.y, row = blockIdx.x, wave = threadIdx.x >> 6, d = threadIdx.x & 63, diagonals = 2 * a.tiles - 1;
-    if (!(which ? a.pq.p : a.pk.p)) return;
+    const int which = blockIdx.z, h = a.head0 + blockIdx.y, row = blockIdx.x * (THREADS / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), d = threadIdx.x & 63;
+    const int diagonals = 2 * a.tiles - 1;
+    if (!(which ? a.pq.p : a.pk.p) || row >= 2 * a.span) return;
     const int lo = first_offset(a, row), hi = first_offset(a, row + 1);
+    auto is_far = [&](int t) { return max(TILE * t - 63, 1 - a.L) >= lo && min(TILE * t + 63, a.L - 1) < hi; };
+    const float* const parts = a.partial + (int64_t(blockIdx.y) * diagonals * a.splits * 2 + which) * BY_OFFSET * 64 + d;
+    constexpr int64_t EACH = 2 * BY_OFFSET * 64;
     float sum = 0.f;
-    for (int off = lo + ((wave - lo) & 3); off < hi; off += 4) {        // (a wave's offsets do not depend on the longest length)
-        const int n0 = off + 63 + 64 * a.tiles, last = n0 / 64 - a.tiles, r = off + 63 - 64 * last;         // (rounded down: 64 last <= off + 63)
-        for (int n = 0; n < 2; ++n) {
-            const int t = last - n, at = r + 64 * n;        // offset `at` of diagonal t
-            if (at > 126 || t <= -a.tiles || t >= a.tiles) continue;
-            const float* p = a.partial + (((int64_t(blockIdx.y) * diagonals + t + a.tiles - 1) * a.splits * 2 + which) * BY_OFFSET + at) * 64 + d;
-            for (int s = 0; s < a.splits; ++s) sum += p[int64_t(s) * 2 * BY_OFFSET * 64];
+    auto add = [&](int t, int at) {             // row `at` of diagonal t, all its parts
+        const float* p = parts + int64_t(t + a.tiles - 1) * a.splits * EACH + at * 64;
+        const int n = splits_of(a, t);
+        int s = 0;
+        for (; s + 4 <= n; s += 4) {
+            const float x0 = p[s * EACH], x1 = p[(s + 1) * EACH], x2 = p[(s + 2) * EACH], x3 = p[(s + 3) * EACH];
+            sum += x0 + x1 + x2 + x3;
         }
+        for (; s < n; ++s) sum += p[s * EACH];
+    };
+    auto offsets = [&](int from, int to) {
+        for (int off = from; off < to; ++off) {
+            const int last = (off + 63 + TILE * a.tiles) / TILE - a.tiles, r = off + 63 - TILE * last;      // (rounded down)
+            for (int n = 0; n < 2; ++n) {
+                const int t = last - n, at = r + TILE * n;          // offset `at` of diagonal t
+                if (at <= 126 && t > -a.tiles && t < a.tiles && !is_far(t)) add(t, at);
+            }
+        }
+    };
+    const int middle = hi - lo > 256 ? 128 : (hi - lo + 1) / 2;
+    offsets(lo, lo + middle);
+    offsets(max(lo + middle, hi - 128), hi);
+    if (hi > lo) {
+        const int t0 = lo == 1 - a.L ? 1 - a.tiles : (lo + 63 + TILE * a.tiles) / TILE - a.tiles, t1 = hi == a.L ? a.tiles - 1 : (hi + TILE * a.tiles) / TILE - a.tiles;
+        for (int t = t0; t <= t1; ++t)
+            if (is_far(t))
+                for (int n = 0; n < 4; ++n) add(t, n);
     }
-    s_sum[wave][d] = sum;
-    __syncthreads();
-    if (wave == 0 && d < a.D) {
+    if (d < a.D) {
         using T = typename Elem<DT>::T;
-        for (int n = 1; n < 4; ++n) sum += s_sum[n][d];
         T* const to = static_cast<T*>(which ? a.dpq : a.dpk) + h * (which ? a.dpq_h : a.dpk_h) + int64_t(row) * a.D + d;
         *to = T(sum * a.scale / score_power<DT>(a));
     }
@@ -640,6 +693,7 @@ __global__ __launch_bounds__(THREADS) void tables_sum_kernel(Args a) {
 size_t elem(int dtype) { return dtype == TDB_F32 ? 4 : 2; }
 int64_t up(int64_t x) { return (x + 255) / 256 * 256; }
 
+constexpr int64_t MOST_STRIDE = int64_t(1) << 24;        // bytes: 64 rows' offsets fit 31 bits
 constexpr int64_t MOST_SCORES = int64_t(512) << 20;      // bytes of dS at a time, unless one head has more
 
 // What a backward call needs, and how many heads it takes at a time.
@@ -655,7 +709,7 @@ Plan plan_of(const tdb_train_attn_args& a) {
     const int64_t each = int64_t(p.row_tiles) * p.tiles * TILE_VALUES * int64_t(elem(a.dtype));
     p.heads = int(std::max<int64_t>(1, std::min<int64_t>(a.heads, MOST_SCORES / std::max<int64_t>(each, 1))));
     const int diagonals = 2 * p.tiles - 1;
-    p.splits = int(std::max<int64_t>(1, std::min<int64_t>(a.batch, 1024 / (int64_t(p.heads) * diagonals))));
+    p.splits = int(std::max<int64_t>(1, std::min<int64_t>(a.batch, 768 / (int64_t(p.heads) * p.tiles))));     // three workgroups for each of 256 CUs
     p.delta = 256;                                  // in front: the two maxima
     p.partial = p.delta + up(p.lines * a.heads * 4);
     p.ds = p.partial + ((a.pos_key || a.pos_query) ? int64_t(p.heads) * diagonals * p.splits * 2 * BY_OFFSET * 64 * 4 : 0);
@@ -688,14 +742,17 @@ int check(const tdb_train_attn_args* a, bool backward) {
         const int64_t s = (&a->q_stride_b)[n];
         if (s < 0 || s * int64_t(elem(a->dtype)) % 16) return tdb_fail(TDB_ERR_STRIDE, "strides must be non-negative multiples of 16 bytes");
     }
-    const int64_t rows[] = {a->o_stride_l, a->dq_stride_l, a->dk_stride_l, a->dv_stride_l};
-    for (int n = 0; n < (backward ? 4 : 1); ++n)
-        if (rows[n] < a->head_dim) return tdb_fail(TDB_ERR_STRIDE, "rows of a result overlap");
+    const int64_t rows[] = {a->q_stride_l, a->k_stride_l, a->v_stride_l, a->o_stride_l, a->dout_stride_l, a->dq_stride_l, a->dk_stride_l, a->dv_stride_l};
+    for (int n = 0; n < (backward ? 8 : 4); ++n)
+        if (rows[n] < a->head_dim || rows[n] * int64_t(elem(a->dtype)) > MOST_STRIDE)
+            return tdb_fail(TDB_ERR_STRIDE, "rows must lie head_dim values to 16 MiB apart");
     const int64_t table[] = {a->pos_key_stride_h, a->pos_key_stride_r, a->pos_query_stride_h, a->pos_query_stride_r};
     for (int64_t s : table)
         if (s < 0 || s * int64_t(elem(a->dtype)) % 16) return tdb_fail(TDB_ERR_STRIDE, "strides of the tables must be non-negative multiples of 16 bytes");
     if (a->pos_key || a->pos_query) {
         if (a->span < 1 || a->span > (1 << 20)) return tdb_fail(TDB_ERR_POSITION, "span %d out of range", a->span);
+        if (2 * int64_t(a->span) * std::max(a->pos_key ? a->pos_key_stride_r : 0, a->pos_query ? a->pos_query_stride_r : 0) * int64_t(elem(a->dtype)) > INT32_MAX)
+            return tdb_fail(TDB_ERR_STRIDE, "a head's table must lie within 2 GiB");
         if (!a->delta_lut || a->lut_half < a->max_seqlen - 1) return tdb_fail(TDB_ERR_POSITION, "delta_lut is missing or shorter than the sequences");
         if (backward && ((a->pos_key && !a->dpos_key) || (a->pos_query && !a->dpos_query))) return tdb_fail(TDB_ERR_NULL, "a table's gradient has no place");
     }
@@ -739,7 +796,7 @@ int blocks_of(const Args& k, int rows) { return k.cu ? k.total / rows + k.B : k.
 
 // The kernels' LDS lies above what a launch has without asking, once per device and kernel.
 template <auto kernel>
-hipError_t launch(size_t lds, int64_t grid, hipStream_t s, const Args& k) {
+hipError_t launch(size_t lds, int64_t grid, int threads, hipStream_t s, const Args& k) {
     static std::mutex mutex;
     static bool raised[64];
     int device = 0;
@@ -754,37 +811,60 @@ hipError_t launch(size_t lds, int64_t grid, hipStream_t s, const Args& k) {
             raised[device] = true;
         }
     }
-    kernel<<<unsigned(grid), THREADS, lds, s>>>(k);
+    kernel<<<unsigned(grid), threads, lds, s>>>(k);
     return hipGetLastError();
 }
 
-template <int DT, int NX>
-hipError_t forward(Args k, hipStream_t s) {
-    static_assert(sizeof(FwdLds<DT, NX>) <= 163840 && sizeof(KvLds<DT, NX>) <= 163840, "LDS of a CU");
-    k.blocks = blocks_of(k, 64 * NX);
-    return launch<attn_fwd_kernel<DT, NX>>(sizeof(FwdLds<DT, NX>), int64_t(k.blocks) * k.heads, s, k);
+// The kernel's instance for the terms that a call has.
+template <template <bool, bool> class F>
+hipError_t by_terms(const Args& k, hipStream_t s) {
+    if (k.pk.p && k.pq.p) return F<true, true>::run(k, s);
+    if (k.pk.p) return F<true, false>::run(k, s);
+    if (k.pq.p) return F<false, true>::run(k, s);
+    return F<false, false>::run(k, s);
 }
 
-template <int DT, int NX>
-hipError_t backward(Args k, int heads, hipStream_t s) {
-    if (DT == TDB_F16) clear_kernel<<<1, 2, 0, s>>>(const_cast<uint32_t*>(k.largest));
-    attn_delta_kernel<DT><<<unsigned((k.lines * k.H * 8 + THREADS - 1) / THREADS), THREADS, 0, s>>>(k, const_cast<uint32_t*>(k.largest));
-    hipError_t e = hipGetLastError();
-    for (k.head0 = 0; e == hipSuccess && k.head0 < k.H; k.head0 += heads) {
-        k.heads = std::min(heads, k.H - k.head0);
-        k.blocks = blocks_of(k, 64 * NX);
-        e = launch<attn_bwd_kv_kernel<DT, NX>>(sizeof(KvLds<DT, NX>), int64_t(k.blocks) * k.heads, s, k);
-        if (e != hipSuccess) break;
-        k.blocks = blocks_of(k, TILE);
-        e = launch<attn_bwd_q_kernel<DT>>(sizeof(QLds<DT>), int64_t(k.blocks) * k.heads, s, k);
-        if (e != hipSuccess || (!k.pk.p && !k.pq.p)) continue;
-        e = launch<attn_bwd_tables_kernel<DT>>(sizeof(TablesLds<DT>), int64_t(k.heads) * (2 * k.tiles - 1) * k.splits, s, k);
-        if (e != hipSuccess) break;
-        tables_sum_kernel<DT><<<dim3(2 * k.span, k.heads, 2), THREADS, 0, s>>>(k);
-        e = hipGetLastError();
+template <int DT>
+struct Launch {
+    using S = Shape<DT>;
+    static_assert(sizeof(FwdLds<DT>) <= 163840 && sizeof(KvLds<DT>) <= 163840, "LDS of a CU");
+    template <bool PK, bool PQ>
+    struct Fwd {
+        static hipError_t run(Args k, hipStream_t s) {
+            k.blocks = blocks_of(k, S::ROWS);
+            return launch<attn_fwd_kernel<DT, PK, PQ>>(sizeof(FwdLds<DT>), int64_t(k.blocks) * k.heads, S::THREADS, s, k);
+        }
+    };
+    template <bool PK, bool PQ>
+    struct Heads {                      // the backward pass of a number of heads
+        static hipError_t run(Args k, hipStream_t s) {
+            k.blocks = blocks_of(k, S::ROWS);
+            hipError_t e = launch<attn_bwd_kv_kernel<DT, PK, PQ>>(sizeof(KvLds<DT>), int64_t(k.blocks) * k.heads, S::THREADS, s, k);
+            if (e != hipSuccess) return e;
+            k.blocks = blocks_of(k, TILE);
+            e = launch<attn_bwd_q_kernel<DT, PK>>(sizeof(QLds<DT>), int64_t(k.blocks) * k.heads, THREADS, s, k);
+            if constexpr (PK || PQ) {
+                if (e != hipSuccess) return e;
+                e = launch<attn_bwd_tables_kernel<DT, PK, PQ>>(sizeof(TablesLds<DT>), int64_t(k.heads) * (2 * k.tiles - 1) * k.splits, THREADS, s, k);
+                if (e != hipSuccess) return e;
+                tables_sum_kernel<DT><<<dim3((2 * k.span + 3) / 4, k.heads, 2), THREADS, 0, s>>>(k);
+                e = hipGetLastError();
+            }
+            return e;
+        }
+    };
+    static hipError_t forward(const Args& k, hipStream_t s) { return by_terms<Fwd>(k, s); }
+    static hipError_t backward(Args k, int heads, hipStream_t s) {
+        if (DT == TDB_F16) clear_kernel<<<1, 2, 0, s>>>(const_cast<uint32_t*>(k.largest));
+        attn_delta_kernel<DT><<<unsigned(std::min<int64_t>((k.lines * k.H * 8 + THREADS - 1) / THREADS, DT == TDB_F16 ? 1024 : 1 << 22)), THREADS, 0, s>>>(k, const_cast<uint32_t*>(k.largest));
+        hipError_t e = hipGetLastError();
+        for (k.head0 = 0; e == hipSuccess && k.head0 < k.H; k.head0 += heads) {
+            k.heads = std::min(heads, k.H - k.head0);
+            e = by_terms<Heads>(k, s);
+        }
+        return e;
     }
-    return e;
-}
+};
 
 int run(const tdb_train_attn_args* a, bool back, void* stream) {
     if (const int rc = check(a, back); rc != TDB_OK) return rc;
@@ -793,9 +873,9 @@ int run(const tdb_train_attn_args* a, bool back, void* stream) {
     const Args k = args_of(*a, p);
     const hipStream_t s = static_cast<hipStream_t>(stream);
     hipError_t e;
-    if (a->dtype == TDB_F32) e = back ? backward<TDB_F32, 1>(k, p.heads, s) : forward<TDB_F32, 1>(k, s);
-    else if (a->dtype == TDB_BF16) e = back ? backward<TDB_BF16, 2>(k, p.heads, s) : forward<TDB_BF16, 2>(k, s);
-    else e = back ? backward<TDB_F16, 2>(k, p.heads, s) : forward<TDB_F16, 2>(k, s);
+    if (a->dtype == TDB_F32) e = back ? Launch<TDB_F32>::backward(k, p.heads, s) : Launch<TDB_F32>::forward(k, s);
+    else if (a->dtype == TDB_BF16) e = back ? Launch<TDB_BF16>::backward(k, p.heads, s) : Launch<TDB_BF16>::forward(k, s);
+    else e = back ? Launch<TDB_F16>::backward(k, p.heads, s) : Launch<TDB_F16>::forward(k, s);
     if (e != hipSuccess) return tdb_fail(TDB_ERR_LAUNCH, "kernel launch failed: %s", hipGetErrorString(e));
     return TDB_OK;
 }

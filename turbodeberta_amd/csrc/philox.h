@@ -27,6 +27,12 @@ __device__ __forceinline__ uint4 tdb_philox(uint32_t a, uint32_t b, uint32_t c, 
     return uint4{a, b, c, d};
 }
 
+// Number n of the eight, n a constant.
+__device__ __forceinline__ uint32_t tdb_number(uint4 w, int n) {
+    const uint32_t x = n < 2 ? w.x : n < 4 ? w.y : n < 6 ? w.z : w.w;
+    return n & 1 ? x >> 16 : x & 0xffffu;
+}
+
 // Bit k: whether value k of the counter is kept.
 __device__ __forceinline__ uint32_t tdb_kept(uint4 w, uint32_t threshold) {
     const uint32_t x[4] = {w.x, w.y, w.z, w.w};

@@ -21,10 +21,16 @@ def _strides(t):
     return (t.stride(0), t.stride(1), t.stride(2)) if t.dim() == 4 else (0, t.stride(1), t.stride(0))
 
 
+def _apart(t):
+    """t where the kernels can address it: aligned rows that do not share memory, not too far apart for 32-bit offsets."""
+    stride = t.stride(-2) if t.dim() == 4 else t.stride(0)
+    return t if L.rows_ok(t) and t.shape[-1] <= stride <= (1 << 24) // t.element_size() else t.contiguous()
+
+
 def _like(t):
     """A tensor for results of t's shape: t's strides where the kernels can address them, else contiguous."""
     o = torch.empty_like(t)
-    return o if L.rows_ok(o) else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    return o if _apart(o) is o else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
 def _args(q, k, v, o, lse, pk, pq, lens, cu, longest, scale, buckets, max_rel, threshold, seed):
@@ -61,7 +67,7 @@ def _fill(a, **tensors):
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, pk, pq, lens, cu, seed, *plain):
-        q, k, v = L.as_rows(q), L.as_rows(k), L.as_rows(v)
+        q, k, v = _apart(q), _apart(k), _apart(v)
         pk, pq = (None if t is None else L.as_rows(t) for t in (pk, pq))
         o = _like(q)
         ctx.plain, ctx.nothing = plain, q.numel() == 0 or (cu is not None and cu.numel() < 2)
@@ -80,7 +86,7 @@ class _Attention(torch.autograd.Function):
         if ctx.nothing:
             return tuple(None if t is None else torch.zeros_like(t) for t in ctx.saved_tensors) + (None,) * (3 + len(ctx.plain))
         q, k, v, o, lse, pk, pq, lens, cu, seed = ctx.saved_tensors
-        dout = L.as_rows(dout)
+        dout = _apart(dout)
         dq, dk, dv = _like(q), _like(k), _like(v)
         a = _args(q, k, v, o, lse, pk, pq, lens, cu, *ctx.plain, seed)
         _fill(a, dout=dout, dq=dq, dk=dk, dv=dv)
