@@ -66,9 +66,15 @@ constexpr int TILE = 64;                        // rows y of a step, and of a ti
 constexpr int TILE_VALUES = TILE * TILE;
 constexpr float LOG2E = 1.44269504088896340736f;
 
-// Rows of 64 values in LDS, 16 bytes apart: 16 rows at the same column are on distinct banks.
+// Rows of 64 values in LDS.  float32: 16 bytes apart.  16 bits: side by side, so that two workgroups fit a CU, their 16-byte chunks permuted: 16 rows at the same chunk
+// are on distinct banks, and so are the 32 bytes that a transposing read takes of each of 8 rows.
 template <int DT>
-constexpr int ROW = DT == TDB_F32 ? 68 : 72;
+constexpr int ROW = DT == TDB_F32 ? 68 : 64;
+template <int DT>
+__device__ __forceinline__ int place(int row, int col) {
+    if constexpr (DT == TDB_F32) return row * ROW<DT> + col;
+    return row * ROW<DT> + (col ^ (((row & 6) | (row >> 3 & 1)) << 3));
+}
 
 __device__ __forceinline__ int lane_c() { return threadIdx.x & 15; }
 __device__ __forceinline__ int lane_g() { return threadIdx.x >> 4 & 3; }
@@ -98,37 +104,37 @@ __device__ __forceinline__ typename Elem<DT>::X8 read8(const typename Elem<DT>::
     }
 }
 
-// Frag of rows `row` + c, columns k0 + 8 g ..
+// Frag of rows `row` + c, columns k0 + 8 g ..; row a multiple of 16
 template <int DT>
 __device__ __forceinline__ typename Elem<DT>::X8 row_frag(const typename Elem<DT>::T* rows, int row, int k0) {
-    return read8<DT>(rows + (row + lane_c()) * ROW<DT> + k0 + 8 * lane_g());
+    return read8<DT>(rows + row * ROW<DT> + place<DT>(lane_c(), k0 + 8 * lane_g()));
 }
 
 // Transposed frags: the lane's row of the operand is column col + c in LDS, the contraction runs over rows in LDS.  Each lane gives the address of four columns of
-// one row; the hardware hands the lanes of a group their columns.  `lo` and `hi`: first of the four rows of the lane group's two halves.
-template <int DT>
-__device__ __forceinline__ typename Elem<DT>::X8 turned_frag(const typename Elem<DT>::T* rows, int stride, int lo, int hi, int col) {
+// one row; the hardware hands the lanes of a group their columns.  `lo` and `hi`: first of the four rows of the lane group's two halves, multiples of 4.  AT: where a value lies.
+template <int DT, typename AT>
+__device__ __forceinline__ typename Elem<DT>::X8 turned_frag(const typename Elem<DT>::T* rows, int lo, int hi, int col, AT at) {
     if constexpr (DT == TDB_F32) {
         f32x8 x;
 #pragma unroll
-        for (int s = 0; s < 4; ++s) x[s] = rows[(lo + s) * stride + col + lane_c()], x[4 + s] = rows[(hi + s) * stride + col + lane_c()];
+        for (int s = 0; s < 4; ++s) x[s] = rows[at(lo + s, col + lane_c())], x[4 + s] = rows[at(hi + s, col + lane_c())];
         return x;
     } else {
-        const int at = (lane_c() >> 2) * stride + col + 4 * (lane_c() & 3);
-        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(TDB_SHARED(s16x4, rows + lo * stride + at));
-        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(TDB_SHARED(s16x4, rows + hi * stride + at));
+        const int r = lane_c() >> 2, c = col + 4 * (lane_c() & 3);
+        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(TDB_SHARED(s16x4, rows + at(lo + r, c)));
+        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(TDB_SHARED(s16x4, rows + at(hi + r, c)));
         return __builtin_bit_cast(typename Elem<DT>::X8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
     }
 }
 // Over rows k0 + 8 g + s
 template <int DT>
-__device__ __forceinline__ typename Elem<DT>::X8 line_frag(const typename Elem<DT>::T* rows, int stride, int k0, int col) {
-    return turned_frag<DT>(rows, stride, k0 + 8 * lane_g(), k0 + 8 * lane_g() + 4, col);
+__device__ __forceinline__ typename Elem<DT>::X8 line_frag(const typename Elem<DT>::T* rows, int k0, int col) {
+    return turned_frag<DT>(rows + k0 * ROW<DT>, 8 * lane_g(), 8 * lane_g() + 4, col, place<DT>);
 }
 // Over rows k0 + 4 g + s and k0 + 16 + 4 g + s, the order in which two results of 16 rows are an operand
 template <int DT>
-__device__ __forceinline__ typename Elem<DT>::X8 pair_frag(const typename Elem<DT>::T* rows, int stride, int k0, int col) {
-    return turned_frag<DT>(rows, stride, k0 + 4 * lane_g(), k0 + 16 + 4 * lane_g(), col);
+__device__ __forceinline__ typename Elem<DT>::X8 pair_frag(const typename Elem<DT>::T* rows, int k0, int col) {
+    return turned_frag<DT>(rows + k0 * ROW<DT>, 4 * lane_g(), 16 + 4 * lane_g(), col, place<DT>);
 }
 
 // Strides in elements; the last dimension is contiguous, every row starts at a multiple of 16 bytes.
@@ -239,7 +245,7 @@ struct Stage {
     }
     __device__ __forceinline__ void store(T* rows) const {
 #pragma unroll
-        for (int n = 0; n < LOADS; ++n) *reinterpret_cast<u32x4*>(rows + row(n) * ROW<DT> + col()) = x[n];
+        for (int n = 0; n < LOADS; ++n) *reinterpret_cast<u32x4*>(rows + place<DT>(row(n), col())) = x[n];
     }
 };
 
@@ -271,8 +277,10 @@ struct Tables {
     uint32_t pk_stride, pq_stride, lane;        // bytes; of the lane's column (past every end where there is none: what is added is below 2^31)
     int at, last;                               // the lane's place in the lookup table for x0 = y0 and r0 = 0, and its last one, in bytes
     S k, q;
-    int which[S::LOADS];
+    int which[S::LOADS], ends[2];
+    int most, half;                             // the largest relative position, and its place
     __device__ __forceinline__ Tables(const Args& a, int h) {
+        most = a.L - 1, half = a.lut_half, ends[0] = 0, ends[1] = 1;
         lut = buffer(a.lut, (2 * int64_t(a.lut_half) + 1) * 4);
         if constexpr (PK) pk = buffer(static_cast<const T*>(a.pk.p) + h * a.pk.h, 2 * int64_t(a.span) * a.pk.l * sizeof(T));
         if constexpr (PQ) pq = buffer(static_cast<const T*>(a.pq.p) + h * a.pq.h, 2 * int64_t(a.span) * a.pq.l * sizeof(T));
@@ -288,7 +296,17 @@ struct Tables {
                 which[n] = int(__builtin_amdgcn_raw_buffer_load_b32(lut, min(max(at + 4 * SIGN * (r0 + from + n * S::STEP), 0), last), 0, 0));
         }
     }
-    // and fetches those looked up last
+    // looks up the rows of the first and the last relative position of a tile of 64 x 64
+    __device__ __forceinline__ void look_at_ends(int from) {
+        if constexpr (PK || PQ) {
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+                ends[n] = int(__builtin_amdgcn_raw_buffer_load_b32(lut, (min(max(SIGN * from + (n ? 63 : -63), -most), most) + half) * 4, 0, 0));
+        }
+    }
+    // whether they are one row
+    __device__ __forceinline__ bool far() const { return (PK || PQ) && __builtin_amdgcn_readfirstlane(ends[0]) == __builtin_amdgcn_readfirstlane(ends[1]); }
+    // fetches the rows looked up last
     __device__ __forceinline__ void load() {
         auto one = [&](S& s, __amdgpu_buffer_rsrc_t from, uint32_t stride) {
             uint32_t to[S::LOADS];
@@ -303,25 +321,19 @@ struct Tables {
         if constexpr (PK) k.store(pk_ring + to * ROW<DT>);
         if constexpr (PQ) q.store(pq_ring + to * ROW<DT>);
     }
-    // the rows of a ring from r = 64 on, for a first step at x0 = from, all looked up before the first is fetched; those of r = 0 .. 63 are looked up last
-    template <int ring>
+    // fills the second half of the rings for a first step with x0 - y0 = from; the rows of r = 0 .. 63 are those looked up last
     __device__ __forceinline__ void fill(T* pk_ring, T* pq_ring, int from) {
-        if constexpr (!PK && !PQ) return;
-        constexpr int N = ring / 64;
-        int rows[N][S::LOADS];
+        if constexpr (PK || PQ) {
+            look_at_ends(from);
+            look(0, from);
+            int first[S::LOADS];
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
-            look(64 * n, from);
-#pragma unroll
-            for (int i = 0; i < S::LOADS; ++i) rows[n][i] = which[i];
-        }
-#pragma unroll
-        for (int n = N - 1; n >= 0; --n) {
-#pragma unroll
-            for (int i = 0; i < S::LOADS; ++i) which[i] = rows[n][i];
-            if (n == 0) return;
+            for (int i = 0; i < S::LOADS; ++i) first[i] = which[i];
+            look(64, from);
             load();
-            store(pk_ring, pq_ring, 64 * n);
+            store(pk_ring, pq_ring, 64);
+#pragma unroll
+            for (int i = 0; i < S::LOADS; ++i) which[i] = first[i];
         }
     }
 };
@@ -350,46 +362,49 @@ __device__ __forceinline__ float column_max(float x) {
 
 constexpr int OWN_ROW = 85;             // floats of a row of x's term, see above
 constexpr int OTHER_ROW = 36;           // and of y's term: 16 rows at the same column are on distinct banks
-// floats of a wave's scratch for the two, the second twice: one is written while the other is read
-constexpr int OWN_TERM = 16 * OWN_ROW, OTHER_TERM = 16 * OTHER_ROW, TERMS = OWN_TERM + 2 * OTHER_TERM;
+constexpr int OWN_TERM = 16 * OWN_ROW, TERMS = OWN_TERM + 16 * OTHER_ROW;      // floats of a wave's scratch for the two
 
-// Place of a ring's row; at is below twice its size.
-template <int ring>
-__device__ __forceinline__ int wrapped(int at) {
-    return at >= ring ? at - ring : at;
-}
+// A table's rows r = 0 .. 126 of a tile of 64 x and 64 y, and one more.
+constexpr int RING = 128;
+__device__ __forceinline__ int wrapped(int at) { return at & (RING - 1); }
 
-// A row of a ring as both operands' frags: the same for every row or column.
+// A row as both operands' frags: the same for every row or column.
 template <int DT>
-__device__ __forceinline__ typename Elem<DT>::X8 same_frag(const typename Elem<DT>::T* row, int k0) {
-    return read8<DT>(row + k0 + 8 * lane_g());
+__device__ __forceinline__ typename Elem<DT>::X8 same_frag(const typename Elem<DT>::T* rows, int row, int k0) {
+    return read8<DT>(rows + place<DT>(row, k0 + 8 * lane_g()));
 }
 // And as an operand whose row is column col + c and which is the same all along the contraction.
 template <int DT>
-__device__ __forceinline__ typename Elem<DT>::X8 level_frag(const typename Elem<DT>::T* row, int col) {
-    const typename Elem<DT>::T v = row[col + lane_c()];
+__device__ __forceinline__ typename Elem<DT>::X8 level_frag(const typename Elem<DT>::T* rows, int row, int col) {
+    const typename Elem<DT>::T v = rows[place<DT>(row, col + lane_c())];
     typename Elem<DT>::X8 x;
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = v;
     return x;
 }
+// Over the ring's rows r0 + 8 g + s
+template <int DT>
+__device__ __forceinline__ typename Elem<DT>::X8 ring_frag(const typename Elem<DT>::T* rows, int r0, int col) {
+    const int at = wrapped(r0 + 8 * lane_g());
+    return turned_frag<DT>(rows, at, at + 4, col, place<DT>);
+}
 
-// Scores of the wave's 16 rows x (x block `first`) with a step's 64 rows y, without the scale.  own[k]: frags of x.  Rings of `ring` rows whose row for r is
-// (r + base) mod ring.  scratch: the wave's own, TERMS floats.  far: the step's relative positions have one table row, so the terms are one number for each x and one for
+// Scores of the wave's 16 rows x (x block `first`) with a step's 64 rows y, without the scale.  own[k]: frags of x.  Rings whose row for r is (r + base) mod RING, base a
+// multiple of 64.  scratch: the wave's own, TERMS floats.  far: the step's relative positions have one table row, so the terms are one number for each x and one for
 // each y.
-template <int DT, int ring, bool OWN, bool OTHER>
+template <int DT, bool OWN, bool OTHER>
 __device__ __forceinline__ void scores(f32x4 (&s)[4], const typename Elem<DT>::X8 (&own)[2], const typename Elem<DT>::T* y_rows, const typename Elem<DT>::T* own_ring,
                                        const typename Elem<DT>::T* other_ring, int base, int first, float* scratch, bool far) {
     using E = Elem<DT>;
     using X8 = typename E::X8;
     const int c = lane_c(), g = lane_g();
     const f32x4 none = {0.f, 0.f, 0.f, 0.f};
-    const int mid = wrapped<ring>(63 + base) * ROW<DT>;
+    const int mid = wrapped(63 + base);
     if ((OWN || OTHER) && far) {
         f32x4 w = none;
-        if constexpr (OWN) w = E::mma(same_frag<DT>(own_ring + mid, 32), own[1], E::mma(same_frag<DT>(own_ring + mid, 0), own[0], none));
+        if constexpr (OWN) w = E::mma(same_frag<DT>(own_ring, mid, 32), own[1], E::mma(same_frag<DT>(own_ring, mid, 0), own[0], none));
         X8 t0, t1;
-        if constexpr (OTHER) t0 = same_frag<DT>(other_ring + mid, 0), t1 = same_frag<DT>(other_ring + mid, 32);
+        if constexpr (OTHER) t0 = same_frag<DT>(other_ring, mid, 0), t1 = same_frag<DT>(other_ring, mid, 32);
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
             const X8 y0 = row_frag<DT>(y_rows, 16 * m, 0), y1 = row_frag<DT>(y_rows, 16 * m, 32);
@@ -402,9 +417,9 @@ __device__ __forceinline__ void scores(f32x4 (&s)[4], const typename Elem<DT>::X
         f32x4 w[5];
 #pragma unroll
         for (int n = 0; n < 5; ++n) {           // r = 16 (first + n) + 15 - row of the frag
-            const int at = wrapped<ring>(16 * (first + n) + base) + 15 - c;
-            w[n] = E::mma(read8<DT>(own_ring + at * ROW<DT> + 8 * g), own[0], none);
-            w[n] = E::mma(read8<DT>(own_ring + at * ROW<DT> + 32 + 8 * g), own[1], w[n]);
+            const typename E::T* const at = own_ring + wrapped(16 * (first + n) + base) * ROW<DT>;
+            w[n] = E::mma(read8<DT>(at + place<DT>(15 - c, 8 * g)), own[0], none);
+            w[n] = E::mma(read8<DT>(at + place<DT>(15 - c, 32 + 8 * g)), own[1], w[n]);
         }
 #pragma unroll
         for (int n = 0; n < 5; ++n)
@@ -420,7 +435,7 @@ __device__ __forceinline__ void scores(f32x4 (&s)[4], const typename Elem<DT>::X
     if constexpr (OTHER) {
 #pragma unroll
         for (int n = 0; n < 5; ++n) {           // r = 16 (first + n) + row: of y blocks 3 - n and 4 - n
-            const int at = wrapped<ring>(16 * (first + n) + base);
+            const int at = wrapped(16 * (first + n) + base);
             const X8 t0 = row_frag<DT>(other_ring, at, 0), t1 = row_frag<DT>(other_ring, at, 32);
 #pragma unroll
             for (int m = 3 - n; m <= 4 - n; ++m)
@@ -438,12 +453,13 @@ __device__ __forceinline__ void scores(f32x4 (&s)[4], const typename Elem<DT>::X
     if constexpr (OTHER) {
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
-            float* const other = scratch + OWN_TERM + (m & 1) * OTHER_TERM;
+            float* const other = scratch + OWN_TERM;
 #pragma unroll
             for (int n = 0; n < 2; ++n) *reinterpret_cast<f32x4*>(other + c * OTHER_ROW + 16 * n + 4 * g) = w[m][n];
             wave_fence();
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[m][e] += other[(4 * g + e) * OTHER_ROW + c + 15 - 4 * g - e];
+            wave_fence();
         }
     }
     wave_fence();

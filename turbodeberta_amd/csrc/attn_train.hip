@@ -19,34 +19,30 @@ namespace tdb_train {
 
 // ---------------------------------------------------------------------------------------------------------------- forward
 
-// A workgroup has 128 rows x in 16 bits, 64 in float32, where the tables' rows for more would not fit LDS; a wave 16.
+// Workgroups of four waves, 64 rows x; in 16 bits two of them fit a CU's LDS.
+constexpr int THREADS = 256, WAVES = THREADS / 64;
 template <int DT>
-struct Shape {
-    static constexpr int WAVES = DT == TDB_F32 ? 4 : 8, ROWS = 16 * WAVES, RING = ROWS + 64, THREADS = 64 * WAVES;
-};
+constexpr int PER_CU = DT == TDB_F32 ? 1 : 2;
 
 template <int DT>
 struct FwdLds {
     using T = typename Elem<DT>::T;
-    using S = Shape<DT>;
-    alignas(16) T k[TILE * ROW<DT>], v[TILE * ROW<DT>], pk[S::RING * ROW<DT>], pq[S::RING * ROW<DT>];
-    alignas(16) float scratch[S::WAVES][TERMS];
+    alignas(16) T k[TILE * ROW<DT>], v[TILE * ROW<DT>], pk[RING * ROW<DT>], pq[RING * ROW<DT>];
+    alignas(16) float scratch[WAVES][TERMS];
 };
 
 template <int DT, bool PK, bool PQ>
-__global__ __launch_bounds__(Shape<DT>::THREADS, 1) void attn_fwd_kernel(Args a) {
+__global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_fwd_kernel(Args a) {
     using E = Elem<DT>;
     using T = typename E::T;
     using X8 = typename E::X8;
-    using S = Shape<DT>;
-    constexpr int ring = S::RING;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     FwdLds<DT>& sm = *reinterpret_cast<FwdLds<DT>*>(smem);
     if (a.cu && threadIdx.x < 64)
         tdb_fill_gaps(a.cu, a.B, a.L, a.total, static_cast<char*>(a.o.p), a.o.l * sizeof(T), a.o.h * sizeof(T), a.H, a.D * sizeof(T), blockIdx.x, gridDim.x);
     int h;
     Where w;
-    if (!locate<S::ROWS>(a, h, w)) return;
+    if (!locate<TILE>(a, h, w)) return;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane_c(), g = lane_g();
     const int row = w.row0 + 16 * wave;             // the wave's first query
     f32x4 o[4];
@@ -57,36 +53,36 @@ __global__ __launch_bounds__(Shape<DT>::THREADS, 1) void attn_fwd_kernel(Args a)
         return;
     }
     const TdbKey key = a.threshold ? tdb_key(a.seed) : TdbKey{0, 0};
-    Source<DT, S::THREADS> keys(a.k, a, w, h), values(a.v, a, w, h);
-    Stage<DT, S::THREADS> k_next, v_next;
-    Tables<DT, 1, S::THREADS, PK, PQ> tables(a, h);
+    Source<DT, THREADS> keys(a.k, a, w, h), values(a.v, a, w, h);
+    Stage<DT, THREADS> k_next, v_next;
+    Tables<DT, 1, THREADS, PK, PQ> tables(a, h);
     X8 q[2];
     load_own<DT>(q, a.q, a, w, h, row);
-    tables.template fill<ring>(sm.pk, sm.pq, w.row0);
-    bool far = false, far_next = false;
+    tables.fill(sm.pk, sm.pq, w.row0);
+    bool far = false;
     auto fetch = [&](int y0) {
         keys.load(k_next);
         values.load(v_next);
         tables.load();
         tables.look(0, w.row0 - y0 - TILE);
-        if constexpr (PK || PQ) far_next = one_row(a, w.row0 - y0 - 63, w.row0 - y0 + S::ROWS - 1);
+        tables.look_at_ends(w.row0 - y0);
     };
     fetch(0);
 
     const float c1 = a.scale * LOG2E;
     float most = -__builtin_inff(), sum = 0.f;
     int base = 0;
-    for (int y0 = 0; y0 < w.len; y0 += TILE, base = base == 0 ? ring - 64 : base - 64) {
+    for (int y0 = 0; y0 < w.len; y0 += TILE, base ^= 64) {
         __syncthreads();
         k_next.store(sm.k);
         v_next.store(sm.v);
         tables.store(sm.pk, sm.pq, base);
-        far = far_next;
+        far = tables.far();
         __syncthreads();
         if (y0 + TILE < w.len) fetch(y0 + TILE);
 
         f32x4 s[4];
-        scores<DT, ring, PK, PQ>(s, q, sm.k, sm.pk, sm.pq, base, wave, sm.scratch[wave], far);
+        scores<DT, PK, PQ>(s, q, sm.k, sm.pk, sm.pq, base, wave, sm.scratch[wave], far);
         if (y0 + TILE > w.len) {
 #pragma unroll
             for (int m = 0; m < 4; ++m)
@@ -126,7 +122,7 @@ __global__ __launch_bounds__(Shape<DT>::THREADS, 1) void attn_fwd_kernel(Args a)
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int d = 0; d < 4; ++d) o[d] = E::mma(pair_frag<DT>(sm.v, ROW<DT>, 32 * u, 16 * d), p[u], o[d]);
+            for (int d = 0; d < 4; ++d) o[d] = E::mma(pair_frag<DT>(sm.v, 32 * u, 16 * d), p[u], o[d]);
     }
     const float all = column_sum(sum);
     store_rows<DT>(a.o, a, w, h, row, o, all > 0.f ? a.factor / all : all == 0.f ? 0.f : all);      // (NaN stays)
@@ -136,8 +132,6 @@ __global__ __launch_bounds__(Shape<DT>::THREADS, 1) void attn_fwd_kernel(Args a)
 // --------------------------------------------------------------------------------------------------------------- backward
 
 // D_i = dO_i . O_i for every row and head: 8 lanes each.  float16: the largest squares of the norms of rows of dO and V as well.
-constexpr int THREADS = 256;
-
 template <int DT>
 __global__ __launch_bounds__(THREADS) void attn_delta_kernel(Args a, uint32_t* largest) {
     using T = typename Elem<DT>::T;
@@ -212,26 +206,23 @@ __device__ __forceinline__ typename Elem<DT>::X8 skew_frag(const typename Elem<D
 template <int DT>
 struct KvLds {
     using T = typename Elem<DT>::T;
-    using S = Shape<DT>;
-    alignas(16) T q[TILE * ROW<DT>], dout[TILE * ROW<DT>], pk[S::RING * ROW<DT>], pq[S::RING * ROW<DT>];
+    alignas(16) T q[TILE * ROW<DT>], dout[TILE * ROW<DT>], pk[RING * ROW<DT>], pq[RING * ROW<DT>];
     alignas(16) float lse[TILE], delta[TILE];
-    alignas(16) uint32_t kept[2][S::WAVES / 2][TILE];       // a bit for each of 32 keys
-    alignas(16) float scratch[S::WAVES][TERMS];             // of the scores; then the skewed gradients of scores
+    alignas(16) uint32_t kept[2][WAVES / 2][TILE];       // a bit for each of 32 keys
+    alignas(16) float scratch[WAVES][TERMS];             // of the scores; then the skewed gradients of scores
     static_assert(SKEWED * sizeof(T) <= TERMS * sizeof(float), "");
 };
 
 template <int DT, bool PK, bool PQ>
-__global__ __launch_bounds__(Shape<DT>::THREADS, 1) void attn_bwd_kv_kernel(Args a) {
+__global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_bwd_kv_kernel(Args a) {
     using E = Elem<DT>;
     using T = typename E::T;
     using X8 = typename E::X8;
-    using S = Shape<DT>;
-    constexpr int ring = S::RING;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     KvLds<DT>& sm = *reinterpret_cast<KvLds<DT>*>(smem);
     int h;
     Where w;
-    if (!locate<S::ROWS>(a, h, w)) return;
+    if (!locate<TILE>(a, h, w)) return;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane_c(), g = lane_g();
     const int row = w.row0 + 16 * wave;             // the wave's first key
     f32x4 dk[4], dv[4];
@@ -242,25 +233,25 @@ __global__ __launch_bounds__(Shape<DT>::THREADS, 1) void attn_bwd_kv_kernel(Args
         store_rows<DT>(a.dv, a, w, h, row, dv, 0.f);
         return;
     }
-    Source<DT, S::THREADS> queries(a.q, a, w, h), douts(a.dout, a, w, h);
-    Stage<DT, S::THREADS> q_next, do_next;
-    Tables<DT, -1, S::THREADS, PK, PQ> tables(a, h);
+    Source<DT, THREADS> queries(a.q, a, w, h), douts(a.dout, a, w, h);
+    Stage<DT, THREADS> q_next, do_next;
+    Tables<DT, -1, THREADS, PK, PQ> tables(a, h);
     X8 k[2], v[2];
     load_own<DT>(k, a.k, a, w, h, row);
     load_own<DT>(v, a.v, a, w, h, row);
-    tables.template fill<ring>(sm.pk, sm.pq, w.row0);
+    tables.fill(sm.pk, sm.pq, w.row0);
     const TdbKey key = a.threshold ? tdb_key(a.seed) : TdbKey{0, 0};
     const float power = score_power<DT>(a), rounded = w.len > 1 ? power : 0.f;      // (the softmax of one key is a constant)
     const __amdgpu_buffer_rsrc_t lines = buffer((wave == 0 ? a.lse : a.delta) + h * a.lines + w.line, int64_t(w.len) * 4);      // of the waves that load them
     float line_next = 0.f;
-    bool far = false, far_next = false;
+    bool far = false;
     auto fetch = [&](int y0) {
         queries.load(q_next);
         douts.load(do_next);
         if (wave < 2) line_next = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(lines, lane * 4, y0 * 4, 0));
         tables.load();
         tables.look(0, w.row0 - y0 - TILE);
-        if constexpr (PK || PQ) far_next = one_row(a, y0 - w.row0 - S::ROWS + 1, y0 - w.row0 + 63);
+        tables.look_at_ends(w.row0 - y0);
     };
     fetch(0);
     // Which of 32 keys are kept for the queries of a step: the two waves that have the keys share the work, a step ahead.  A lane has a query and two of the four counters
@@ -280,25 +271,25 @@ __global__ __launch_bounds__(Shape<DT>::THREADS, 1) void attn_bwd_kv_kernel(Args
 
     const float c1 = a.scale * LOG2E, shift = DT == TDB_F16 ? float(a.p_shift) : 0.f, unshift = DT == TDB_F16 ? ldexpf(1.f, -a.p_shift) : 1.f;
     const float down = unshift * rounded;
-    const bool edge = w.row0 + S::ROWS > w.len;
+    const bool edge = w.row0 + TILE > w.len;
     const int tile_col = row / TILE, bit = (row & 16) + c;
     T* ds = static_cast<T*>(a.ds) + ((int64_t(h - a.head0) * a.row_tiles + w.row_tile) * a.tiles + tile_col) * TILE_VALUES + (row / 16 % 4 * 128 + lane) * 8;
     T* const skewed = reinterpret_cast<T*>(sm.scratch[wave]);
     int base = 0, odd = 0;
-    for (int y0 = 0; y0 < w.len; y0 += TILE, base = base == 0 ? ring - 64 : base - 64, ds += int64_t(a.tiles) * TILE_VALUES, odd ^= 1) {
+    for (int y0 = 0; y0 < w.len; y0 += TILE, base ^= 64, ds += int64_t(a.tiles) * TILE_VALUES, odd ^= 1) {
         __syncthreads();
         q_next.store(sm.q);
         do_next.store(sm.dout);
         tables.store(sm.pk, sm.pq, base);
         if (wave < 2) (wave == 0 ? sm.lse : sm.delta)[lane] = line_next;
-        far = far_next;
+        far = tables.far();
         __syncthreads();
         if (y0 + TILE < w.len) {
             fetch(y0 + TILE);
             if (a.threshold) draw(y0 + TILE, odd ^ 1);
         }
         f32x4 s[4], dp[4];
-        scores<DT, ring, PQ, PK>(s, k, sm.q, sm.pq, sm.pk, base, wave, sm.scratch[wave], far);
+        scores<DT, PQ, PK>(s, k, sm.q, sm.pq, sm.pk, base, wave, sm.scratch[wave], far);
 #pragma unroll
         for (int m = 0; m < 4; ++m)
             dp[m] = E::mma(row_frag<DT>(sm.dout, 16 * m, 32), v[1], E::mma(row_frag<DT>(sm.dout, 16 * m, 0), v[0], f32x4{0.f, 0.f, 0.f, 0.f}));
@@ -347,15 +338,14 @@ __global__ __launch_bounds__(Shape<DT>::THREADS, 1) void attn_bwd_kv_kernel(Args
         for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int d = 0; d < 4; ++d) {
-                dv[d] = E::mma(pair_frag<DT>(sm.dout, ROW<DT>, 32 * u, 16 * d), p[u], dv[d]);
-                dk[d] = E::mma(pair_frag<DT>(sm.q, ROW<DT>, 32 * u, 16 * d), dsx[u], dk[d]);
+                dv[d] = E::mma(pair_frag<DT>(sm.dout, 32 * u, 16 * d), p[u], dv[d]);
+                dk[d] = E::mma(pair_frag<DT>(sm.q, 32 * u, 16 * d), dsx[u], dk[d]);
             }
         if constexpr (PQ) {
             if (far) {
-                const T* const same = sm.pq + wrapped<ring>(63 + base) * ROW<DT>;
 #pragma unroll
                 for (int d = 0; d < 4; ++d) {
-                    const X8 t = level_frag<DT>(same, 16 * d);
+                    const X8 t = level_frag<DT>(sm.pq, wrapped(63 + base), 16 * d);
 #pragma unroll
                     for (int u = 0; u < 2; ++u) dk[d] = E::mma(t, dsx[u], dk[d]);
                 }
@@ -364,9 +354,8 @@ __global__ __launch_bounds__(Shape<DT>::THREADS, 1) void attn_bwd_kv_kernel(Args
 #pragma unroll
                 for (int n = 0; n < 3; ++n) {
                     const X8 b = skew_frag<DT>(skewed, n);
-                    const int at = wrapped<ring>(16 * wave + 32 * n + 8 * g + base);
 #pragma unroll
-                    for (int d = 0; d < 4; ++d) dk[d] = E::mma(turned_frag<DT>(sm.pq, ROW<DT>, at, at + 4, 16 * d), b, dk[d]);
+                    for (int d = 0; d < 4; ++d) dk[d] = E::mma(ring_frag<DT>(sm.pq, 16 * wave + 32 * n + base, 16 * d), b, dk[d]);
                 }
                 wave_fence();
             }
@@ -390,9 +379,8 @@ struct Scores {
         typedef __attribute__((ext_vector_type(4))) typename Elem<DT>::T T4;
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-            typename Elem<DT>::T* const to = rows + key(n) * ROW<DT> + query(0);
-            *reinterpret_cast<T4*>(to) = __builtin_shufflevector(x[n], x[n], 0, 1, 2, 3);
-            *reinterpret_cast<T4*>(to + 16) = __builtin_shufflevector(x[n], x[n], 4, 5, 6, 7);
+            *reinterpret_cast<T4*>(rows + place<DT>(key(n), query(0))) = __builtin_shufflevector(x[n], x[n], 0, 1, 2, 3);
+            *reinterpret_cast<T4*>(rows + place<DT>(key(n), query(4))) = __builtin_shufflevector(x[n], x[n], 4, 5, 6, 7);
         }
     }
     static __device__ __forceinline__ int key(int n) { return 16 * ((n * THREADS + threadIdx.x) >> 7) + lane_c(); }
@@ -402,7 +390,7 @@ struct Scores {
 template <int DT>
 struct QLds {
     using T = typename Elem<DT>::T;
-    alignas(16) T k[TILE * ROW<DT>], pk[128 * ROW<DT>], ds[TILE * ROW<DT>], skewed[4][SKEWED];
+    alignas(16) T k[TILE * ROW<DT>], pk[RING * ROW<DT>], ds[TILE * ROW<DT>], skewed[4][SKEWED];
 };
 
 // dq: a workgroup has 64 queries, a wave 16.
@@ -434,15 +422,15 @@ __global__ __launch_bounds__(THREADS, DT == TDB_F32 ? 1 : 2) void attn_bwd_q_ker
     Stage<DT, THREADS> k_next;
     Scores<DT> ds_next;
     Tables<DT, 1, THREADS, PK, false> tables(a, h);
-    tables.template fill<128>(sm.pk, nullptr, w.row0);
-    bool far = false, far_next = false;
+    tables.fill(sm.pk, nullptr, w.row0);
+    bool far = false;
     auto fetch = [&](int y0) {
         keys.load(k_next);
         ds_next.load(tile);
         tile += TILE_VALUES;
         tables.load();
         tables.look(0, w.row0 - y0 - TILE);
-        if constexpr (PK) far_next = one_row(a, w.row0 - y0 - 63, w.row0 - y0 + 63);
+        tables.look_at_ends(w.row0 - y0);
     };
     fetch(0);
     int base = 0;
@@ -450,7 +438,7 @@ __global__ __launch_bounds__(THREADS, DT == TDB_F32 ? 1 : 2) void attn_bwd_q_ker
         __syncthreads();
         k_next.store(sm.k);
         tables.store(sm.pk, nullptr, base);
-        far = far_next;
+        far = tables.far();
         ds_next.store(sm.ds);
         if (PK && !far) {
 #pragma unroll
@@ -465,20 +453,19 @@ __global__ __launch_bounds__(THREADS, DT == TDB_F32 ? 1 : 2) void attn_bwd_q_ker
         if (y0 + TILE < w.len) fetch(y0 + TILE);
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-            const X8 b = line_frag<DT>(sm.ds, ROW<DT>, 32 * n, 16 * wave);
+            const X8 b = line_frag<DT>(sm.ds, 32 * n, 16 * wave);
 #pragma unroll
             for (int d = 0; d < 4; ++d) {
-                dq[d] = E::mma(line_frag<DT>(sm.k, ROW<DT>, 32 * n, 16 * d), b, dq[d]);
-                if (PK && far) dq[d] = E::mma(level_frag<DT>(sm.pk + ((63 + base) & 127) * ROW<DT>, 16 * d), b, dq[d]);
+                dq[d] = E::mma(line_frag<DT>(sm.k, 32 * n, 16 * d), b, dq[d]);
+                if (PK && far) dq[d] = E::mma(level_frag<DT>(sm.pk, wrapped(63 + base), 16 * d), b, dq[d]);
             }
         }
         if (PK && !far) {
 #pragma unroll
             for (int n = 0; n < 3; ++n) {
                 const X8 b = skew_frag<DT>(sm.skewed[wave], n);
-                const int at = (16 * wave + 32 * n + 8 * g + base) & 127;
 #pragma unroll
-                for (int d = 0; d < 4; ++d) dq[d] = E::mma(turned_frag<DT>(sm.pk, ROW<DT>, at, at + 4, 16 * d), b, dq[d]);
+                for (int d = 0; d < 4; ++d) dq[d] = E::mma(ring_frag<DT>(sm.pk, 16 * wave + 32 * n + base, 16 * d), b, dq[d]);
             }
         }
     }
@@ -493,6 +480,11 @@ __device__ __forceinline__ int splits_of(const Args& a, int t) { return max(1, a
 constexpr int BY_OFFSET = 128;
 template <int DT>
 constexpr int OFFSET_ROW = DT == TDB_F32 ? BY_OFFSET + 4 : BY_OFFSET + 8;
+
+template <int DT>
+__device__ __forceinline__ typename Elem<DT>::X8 offset_frag(const typename Elem<DT>::T* rows, int k0, int col) {
+    return turned_frag<DT>(rows, k0 + 8 * lane_g(), k0 + 8 * lane_g() + 4, col, [](int r, int c) { return r * OFFSET_ROW<DT> + c; });
+}
 
 template <int DT>
 struct TablesLds {
@@ -582,8 +574,8 @@ __global__ __launch_bounds__(THREADS, DT == TDB_F32 ? 1 : 2) void attn_bwd_table
             for (int n = 0; n < 2; ++n)
 #pragma unroll
                 for (int d = 0; d < 4; ++d) {
-                    if constexpr (PK) dpk[n][d] = E::mma(pair_frag<DT>(sm.q, ROW<DT>, 32 * (wave & 1), 16 * d), ds.x[n], dpk[n][d]);
-                    if constexpr (PQ) dpq[n][d] = E::mma(line_frag<DT>(sm.k, ROW<DT>, 32 * n, 16 * d), line_frag<DT>(sm.by_key, ROW<DT>, 32 * n, 16 * wave), dpq[n][d]);
+                    if constexpr (PK) dpk[n][d] = E::mma(pair_frag<DT>(sm.q, 32 * (wave & 1), 16 * d), ds.x[n], dpk[n][d]);
+                    if constexpr (PQ) dpq[n][d] = E::mma(line_frag<DT>(sm.k, 32 * n, 16 * d), line_frag<DT>(sm.by_key, 32 * n, 16 * wave), dpq[n][d]);
                 }
             continue;
         }
@@ -592,10 +584,10 @@ __global__ __launch_bounds__(THREADS, DT == TDB_F32 ? 1 : 2) void attn_bwd_table
             for (int u = 0; u < 2; ++u) {
                 X8 b[2];
 #pragma unroll
-                for (int n = 0; n < 2; ++n) b[n] = line_frag<DT>(by, OFFSET_ROW<DT>, 32 * u, 32 * wave + 16 * n);
+                for (int n = 0; n < 2; ++n) b[n] = offset_frag<DT>(by, 32 * u, 32 * wave + 16 * n);
 #pragma unroll
                 for (int d = 0; d < 4; ++d) {
-                    const X8 x = line_frag<DT>(rows, ROW<DT>, 32 * u, 16 * d);
+                    const X8 x = line_frag<DT>(rows, 32 * u, 16 * d);
 #pragma unroll
                     for (int n = 0; n < 2; ++n) acc[n][d] = E::mma(x, b[n], acc[n][d]);
                 }
@@ -826,20 +818,19 @@ hipError_t by_terms(const Args& k, hipStream_t s) {
 
 template <int DT>
 struct Launch {
-    using S = Shape<DT>;
-    static_assert(sizeof(FwdLds<DT>) <= 163840 && sizeof(KvLds<DT>) <= 163840, "LDS of a CU");
+    static_assert(sizeof(FwdLds<DT>) * PER_CU<DT> <= 163840 && sizeof(KvLds<DT>) * PER_CU<DT> <= 163840, "LDS of a CU");
     template <bool PK, bool PQ>
     struct Fwd {
         static hipError_t run(Args k, hipStream_t s) {
-            k.blocks = blocks_of(k, S::ROWS);
-            return launch<attn_fwd_kernel<DT, PK, PQ>>(sizeof(FwdLds<DT>), int64_t(k.blocks) * k.heads, S::THREADS, s, k);
+            k.blocks = blocks_of(k, TILE);
+            return launch<attn_fwd_kernel<DT, PK, PQ>>(sizeof(FwdLds<DT>), int64_t(k.blocks) * k.heads, THREADS, s, k);
         }
     };
     template <bool PK, bool PQ>
     struct Heads {                      // the backward pass of a number of heads
         static hipError_t run(Args k, hipStream_t s) {
-            k.blocks = blocks_of(k, S::ROWS);
-            hipError_t e = launch<attn_bwd_kv_kernel<DT, PK, PQ>>(sizeof(KvLds<DT>), int64_t(k.blocks) * k.heads, S::THREADS, s, k);
+            k.blocks = blocks_of(k, TILE);
+            hipError_t e = launch<attn_bwd_kv_kernel<DT, PK, PQ>>(sizeof(KvLds<DT>), int64_t(k.blocks) * k.heads, THREADS, s, k);
             if (e != hipSuccess) return e;
             k.blocks = blocks_of(k, TILE);
             e = launch<attn_bwd_q_kernel<DT, PK>>(sizeof(QLds<DT>), int64_t(k.blocks) * k.heads, THREADS, s, k);
