@@ -395,7 +395,7 @@ struct QLds {
 
 // dq: a workgroup has 64 queries, a wave 16.
 template <int DT, bool PK>
-__global__ __launch_bounds__(THREADS, DT == TDB_F32 ? 1 : 2) void attn_bwd_q_kernel(Args a) {
+__global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_bwd_q_kernel(Args a) {
     using E = Elem<DT>;
     using T = typename E::T;
     using X8 = typename E::X8;
@@ -409,7 +409,7 @@ __global__ __launch_bounds__(THREADS, DT == TDB_F32 ? 1 : 2) void attn_bwd_q_ker
     int h;
     Where w;
     if (!locate<TILE>(a, h, w)) return;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane_g();
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     f32x4 dq[4];
 #pragma unroll
     for (int d = 0; d < 4; ++d) dq[d] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -419,38 +419,43 @@ __global__ __launch_bounds__(THREADS, DT == TDB_F32 ? 1 : 2) void attn_bwd_q_ker
     }
     const T* tile = static_cast<const T*>(a.ds) + (int64_t(h - a.head0) * a.row_tiles + w.row_tile + w.row0 / TILE) * a.tiles * TILE_VALUES;
     Source<DT, THREADS> keys(a.k, a, w, h);
-    Stage<DT, THREADS> k_next;
-    Scores<DT> ds_next;
+    struct Next {                       // a step's rows on their way
+        Stage<DT, THREADS> k, pk;
+        Scores<DT> ds;
+        int ends[2];
+    };
     Tables<DT, 1, THREADS, PK, false> tables(a, h);
     tables.fill(sm.pk, nullptr, w.row0);
-    bool far = false;
-    auto fetch = [&](int y0) {
-        keys.load(k_next);
-        ds_next.load(tile);
+    int y_next = 0;
+    auto fetch = [&](Next& n) {
+        keys.load(n.k);
+        n.ds.load(tile);
         tile += TILE_VALUES;
         tables.load();
-        tables.look(0, w.row0 - y0 - TILE);
-        tables.look_at_ends(w.row0 - y0);
+        n.pk = tables.k;
+        tables.look_at_ends(w.row0 - y_next);
+        n.ends[0] = tables.ends[0], n.ends[1] = tables.ends[1];
+        y_next += TILE;
+        tables.look(0, w.row0 - y_next);
     };
-    fetch(0);
     int base = 0;
-    for (int y0 = 0; y0 < w.len; y0 += TILE, base ^= 64) {
+    auto step = [&](Next& next) {
         __syncthreads();
-        k_next.store(sm.k);
-        tables.store(sm.pk, nullptr, base);
-        far = tables.far();
-        ds_next.store(sm.ds);
+        next.k.store(sm.k);
+        if constexpr (PK) next.pk.store(sm.pk + base * ROW<DT>);
+        next.ds.store(sm.ds);
+        const bool far = PK && __builtin_amdgcn_readfirstlane(next.ends[0]) == __builtin_amdgcn_readfirstlane(next.ends[1]);
         if (PK && !far) {
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
+            for (int n = 0; n < 2; ++n) {
+                const int q = Scores<DT>::query(0);
+                T* const to = sm.skewed[q >> 4] + (q & 15) * SKEW + 79 - Scores<DT>::key(n);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int q = Scores<DT>::query(e);
-                    sm.skewed[q >> 4][(q & 15) * SKEW + 79 - Scores<DT>::key(n)] = ds_next.x[n][e];
-                }
+                for (int e = 0; e < 8; ++e) to[(e >> 2) * SKEWED + (e & 3) * SKEW] = next.ds.x[n][e];
+            }
         }
         __syncthreads();
-        if (y0 + TILE < w.len) fetch(y0 + TILE);
+        if (y_next < w.len) fetch(next);
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
             const X8 b = line_frag<DT>(sm.ds, 32 * n, 16 * wave);
@@ -468,6 +473,14 @@ __global__ __launch_bounds__(THREADS, DT == TDB_F32 ? 1 : 2) void attn_bwd_q_ker
                 for (int d = 0; d < 4; ++d) dq[d] = E::mma(ring_frag<DT>(sm.pk, 16 * wave + 32 * n + base, 16 * d), b, dq[d]);
             }
         }
+        base ^= 64;
+    };
+    Next one, two;
+    fetch(one);
+    if (y_next < w.len) fetch(two);
+    for (int y0 = 0; y0 < w.len; y0 += 2 * TILE) {
+        step(one);
+        if (y0 + TILE < w.len) step(two);
     }
     store_rows<DT>(a.dq, a, w, h, w.row0 + 16 * wave, dq, a.scale / score_power<DT>(a));
 }
@@ -475,12 +488,12 @@ __global__ __launch_bounds__(THREADS, DT == TDB_F32 ? 1 : 2) void attn_bwd_q_ker
 // Parts that the sequences of a diagonal are dealt to: as many as it has tiles, next to the longest one.
 __device__ __forceinline__ int splits_of(const Args& a, int t) { return max(1, a.splits * (a.tiles - abs(t)) / a.tiles); }
 
-// Tables: a workgroup has a diagonal of tiles (query tile - key tile = t) of every `splits`-th sequence, a wave 32 of its 128 offsets r = i - j + 63.  Where all offsets
-// of a diagonal have one table row ("far") their sum is all that is wanted: Q^T dS and K^T dS^T, whose columns are added up at the end, one row for each wave.
+// Tables: a workgroup has a diagonal of tiles (query tile - key tile = t) of every `splits`-th sequence.  Its waves share the two tables and the 128 offsets r = i - j + 63 of
+// a tile: in blocks of 16, dealt in turn, so that each has as many of those that 32 queries (or keys) reach.  Where all offsets of a diagonal have one table row ("far")
+// their sum is all that is wanted: Q^T dS and K^T dS^T, whose columns are added up at the end.
 constexpr int BY_OFFSET = 128;
 template <int DT>
 constexpr int OFFSET_ROW = DT == TDB_F32 ? BY_OFFSET + 4 : BY_OFFSET + 8;
-
 template <int DT>
 __device__ __forceinline__ typename Elem<DT>::X8 offset_frag(const typename Elem<DT>::T* rows, int k0, int col) {
     return turned_frag<DT>(rows, k0 + 8 * lane_g(), k0 + 8 * lane_g() + 4, col, [](int r, int c) { return r * OFFSET_ROW<DT> + c; });
@@ -504,119 +517,147 @@ __device__ __forceinline__ float row_sum(float x) {
     return x;
 }
 
-template <int DT, bool PK, bool PQ>
-__global__ __launch_bounds__(THREADS, DT == TDB_F32 ? 1 : 2) void attn_bwd_tables_kernel(Args a) {
-    using E = Elem<DT>;
-    using T = typename E::T;
-    using X8 = typename E::X8;
-    extern __shared__ __attribute__((aligned(16))) char smem[];
-    TablesLds<DT>& sm = *reinterpret_cast<TablesLds<DT>*>(smem);
-    const int diagonals = 2 * a.tiles - 1, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane_c(), g = lane_g();
-    const int split = blockIdx.x % a.splits, at = blockIdx.x / a.splits, t = at % diagonals - (a.tiles - 1), h = a.head0 + at / diagonals;
-    const int splits = splits_of(a, t);
-    if (split >= splits) return;
-    const bool far = one_row(a, TILE * t - 63, TILE * t + 63);
-    f32x4 dpk[2][4], dpq[2][4];
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int d = 0; d < 4; ++d) dpk[n][d] = dpq[n][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (!far)
-        for (int n = threadIdx.x; n < TILE * OFFSET_ROW<DT>; n += THREADS) sm.by_query[n] = sm.by_key[n] = T(0.f);
-
-    Stage<DT, THREADS> q_next, k_next;
-    Scores<DT> ds_next;
-    Where w;
-    int it = 0, end = 0;
-    w.b = split - splits;
-    auto advance = [&]() {              // to the next tile; false: none is left
-        for (++it; it >= end;) {
-            w.b += splits;
-            if (w.b >= a.B) return false;
-            w.len = valid_rows(a, w.b, w.first);
-            w.row_tile = a.cu ? w.first / TILE + w.b : int64_t(w.b) * a.tiles;
-            const int n = (w.len + TILE - 1) / TILE;
+// The tiles of a diagonal in the sequences first, first + step, ...; a sequence's length is read while the one before it is walked through.
+struct Diagonal {
+    int t, step, it, end, b_next;
+    int b, first, len;                  // of the sequence
+    int from, to;                       // of the one to come, as they stand in memory
+    __device__ __forceinline__ void start(const Args& a, int diagonal, int sequence, int splits) {
+        t = diagonal, step = splits, b_next = sequence, it = end = 0;
+        peek(a);
+    }
+    __device__ __forceinline__ void peek(const Args& a) {
+        const int n = min(b_next, a.B - 1);
+        const int32_t* const ends = a.cu ? a.cu + 1 : a.seqlens;
+        from = 0, to = a.L;
+        if (a.cu) from = a.cu[n];
+        if (ends) to = ends[n];
+    }
+    __device__ __forceinline__ bool advance(const Args& a) {             // to the next tile; false: none is left
+        ++it;
+        while (it >= end) {
+            if (b_next >= a.B) return false;
+            b = b_next, first = __builtin_amdgcn_readfirstlane(from);
+            const int last = __builtin_amdgcn_readfirstlane(to);
+            len = first < 0 || last < first || (a.cu && last > a.total) ? 0 : min(last - first, a.L);
+            b_next += step;
+            peek(a);
+            const int n = (len + TILE - 1) / TILE;
             it = max(0, t), end = min(n, n + t);
         }
         return true;
-    };
-    auto fetch = [&]() {
-        if constexpr (PK) Source<DT, THREADS>(a.q, a, w, h, it * TILE).load(q_next);
-        if constexpr (PQ) Source<DT, THREADS>(a.k, a, w, h, (it - t) * TILE).load(k_next);
-        ds_next.load(static_cast<const T*>(a.ds) + ((int64_t(h - a.head0) * a.row_tiles + w.row_tile + it) * a.tiles + it - t) * TILE_VALUES);
-    };
-    bool more = advance();
-    if (more) fetch();
+    }
+};
+
+template <int DT, bool PK, bool PQ>
+struct TablesNext {
+    Stage<DT, THREADS> q, k;
+    Scores<DT> ds;
+    __device__ __forceinline__ void load(const Diagonal& d, const Args& a, int h) {
+        Where w;
+        w.b = d.b, w.first = d.first, w.len = d.len;
+        const int64_t row_tile = a.cu ? d.first / TILE + d.b : int64_t(d.b) * a.tiles;
+        if constexpr (PK) Source<DT, THREADS>(a.q, a, w, h, d.it * TILE).load(q);
+        if constexpr (PQ) Source<DT, THREADS>(a.k, a, w, h, (d.it - d.t) * TILE).load(k);
+        ds.load(static_cast<const typename Elem<DT>::T*>(a.ds) + ((int64_t(h - a.head0) * a.row_tiles + row_tile + d.it) * a.tiles + d.it - d.t) * TILE_VALUES);
+    }
+};
+
+// What a wave does, for each of the roles that waves have: every one of them passes the same barriers.  KEYS: it sums up for the table of queries (from keys).
+template <int DT, bool PK, bool PQ, bool KEYS, bool FAR>
+__device__ __forceinline__ void sum_tables(const Args& a, TablesLds<DT>& sm, Diagonal diagonal, int h, int wave) {
+    using E = Elem<DT>;
+    using T = typename E::T;
+    using X8 = typename E::X8;
+    constexpr int SHARE = PK && PQ ? 2 : 4, BLOCKS = 8 / SHARE, SOME = BLOCKS == 4 ? 3 : 2;         // waves of a table, blocks of a wave, those that 32 rows reach
+    const int share = wave % SHARE, c = lane_c(), g = lane_g();
+    f32x4 acc[FAR ? 1 : BLOCKS][4];
+#pragma unroll
+    for (int n = 0; n < (FAR ? 1 : BLOCKS); ++n)
+#pragma unroll
+        for (int d = 0; d < 4; ++d) acc[n][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const T* const rows = KEYS ? sm.k : sm.q;
+    TablesNext<DT, PK, PQ> next;
+    bool more = diagonal.advance(a);
+    if (more) next.load(diagonal, a, h);
     while (more) {
         __syncthreads();
-        if constexpr (PK) q_next.store(sm.q);
-        if constexpr (PQ) k_next.store(sm.k);
-        if (far) {
-            if constexpr (PQ) ds_next.store(sm.by_key);
+        if constexpr (PK) next.q.store(sm.q);
+        if constexpr (PQ) next.k.store(sm.k);
+        if constexpr (FAR) {
+            next.ds.store(sm.by_key);
         } else {
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
-                const int j = Scores<DT>::key(n);
+                const int j = Scores<DT>::key(n), i0 = Scores<DT>::query(0);
+                T* const by_query = sm.by_query + i0 * (OFFSET_ROW<DT> + 1) - j + 63;
+                T* const by_key = sm.by_key + j * (OFFSET_ROW<DT> - 1) + i0 + 63;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const int i = Scores<DT>::query(e);
-                    if constexpr (PK) sm.by_query[i * OFFSET_ROW<DT> + i - j + 63] = ds_next.x[n][e];
-                    if constexpr (PQ) sm.by_key[j * OFFSET_ROW<DT> + i - j + 63] = ds_next.x[n][e];
+                    const int i = 16 * (e >> 2) + (e & 3);
+                    if constexpr (PK) by_query[i * (OFFSET_ROW<DT> + 1)] = next.ds.x[n][e];
+                    if constexpr (PQ) by_key[i] = next.ds.x[n][e];
                 }
             }
         }
-        const Scores<DT> ds = ds_next;
         __syncthreads();
-        more = advance();
-        if (more) fetch();
-        if (far) {                      // the wave's two pieces of dS, queries in pairs; 16 queries of dS as rows of keys
+        more = diagonal.advance(a);
+        if (more) next.load(diagonal, a, h);
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
+        for (int u = 0; u < 2; ++u) {
+            // far: 16 keys of the queries' sum, or 16 queries of the keys'; twice as many for half as many waves.  Else: 32 queries reach the blocks 2 u .. 2 u + 5, 32 keys
+            // 2 - 2 u .. 7 - 2 u: of a wave's four all but the first or the last.
+            constexpr int N = FAR ? 4 / SHARE : SOME;
+            const int late = BLOCKS == 4 && (KEYS ? u == 0 : u == 1);
+            X8 b[N];
 #pragma unroll
-                for (int d = 0; d < 4; ++d) {
-                    if constexpr (PK) dpk[n][d] = E::mma(pair_frag<DT>(sm.q, 32 * (wave & 1), 16 * d), ds.x[n], dpk[n][d]);
-                    if constexpr (PQ) dpq[n][d] = E::mma(line_frag<DT>(sm.k, 32 * n, 16 * d), line_frag<DT>(sm.by_key, 32 * n, 16 * wave), dpq[n][d]);
-                }
-            continue;
-        }
-        auto add = [&](f32x4 (&acc)[2][4], const T* rows, const T* by) {
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                X8 b[2];
-#pragma unroll
-                for (int n = 0; n < 2; ++n) b[n] = offset_frag<DT>(by, 32 * u, 32 * wave + 16 * n);
-#pragma unroll
-                for (int d = 0; d < 4; ++d) {
-                    const X8 x = line_frag<DT>(rows, 32 * u, 16 * d);
-#pragma unroll
-                    for (int n = 0; n < 2; ++n) acc[n][d] = E::mma(x, b[n], acc[n][d]);
-                }
+            for (int n = 0; n < N; ++n) {
+                if constexpr (!FAR) b[n] = offset_frag<DT>(KEYS ? sm.by_key : sm.by_query, 32 * u, 16 * (share + SHARE * (n + late)));
+                else if constexpr (KEYS) b[n] = line_frag<DT>(sm.by_key, 32 * u, 16 * (share + SHARE * n));
+                else b[n] = row_frag<DT>(sm.by_key, 16 * (share + SHARE * n), 32 * u);
             }
-        };
-        if constexpr (PK) add(dpk, sm.q, sm.by_query);
-        if constexpr (PQ) add(dpq, sm.k, sm.by_key);
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+                const X8 x = line_frag<DT>(rows, 32 * u, 16 * d);
+#pragma unroll
+                for (int n = 0; n < N; ++n) acc[FAR ? 0 : n + late][d] = E::mma(x, b[n], acc[FAR ? 0 : n + late][d]);
+            }
+        }
     }
-    float* const part = a.partial + int64_t(blockIdx.x) * 2 * BY_OFFSET * 64;
-    if (far) {
+    float* const part = a.partial + int64_t(blockIdx.x) * 2 * BY_OFFSET * 64 + (KEYS ? BY_OFFSET * 64 : 0);
+#pragma unroll
+    for (int n = 0; n < (FAR ? 1 : BLOCKS); ++n)
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
-            f32x4 x = dpk[0][d] + dpk[1][d], y = dpq[0][d] + dpq[1][d];
+            if constexpr (FAR) {            // a row for each wave of a table
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = row_sum(x[e]), y[e] = row_sum(y[e]);
-            const int to = wave * 64 + 16 * d + 4 * g;
-            if (PK && c == 0) *reinterpret_cast<f32x4*>(part + to) = x;
-            if (PQ && c == 0) *reinterpret_cast<f32x4*>(part + BY_OFFSET * 64 + to) = y;
+                for (int e = 0; e < 4; ++e) acc[n][d][e] = row_sum(acc[n][d][e]);
+                if (c == 0) *reinterpret_cast<f32x4*>(part + share * 64 + 16 * d + 4 * g) = acc[n][d];
+            } else {
+                *reinterpret_cast<f32x4*>(part + (16 * (share + SHARE * n) + c) * 64 + 16 * d + 4 * g) = acc[n][d];
+            }
         }
+}
+
+template <int DT, bool PK, bool PQ>
+__global__ __launch_bounds__(THREADS, DT == TDB_F32 ? 1 : 3) void attn_bwd_tables_kernel(Args a) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    TablesLds<DT>& sm = *reinterpret_cast<TablesLds<DT>*>(smem);
+    const int diagonals = 2 * a.tiles - 1, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int split = blockIdx.x % a.splits, at = blockIdx.x / a.splits, t = at % diagonals - (a.tiles - 1), h = a.head0 + at / diagonals;
+    const int splits = splits_of(a, t);
+    if (split >= splits) return;
+    Diagonal diagonal;
+    diagonal.start(a, t, split, splits);
+    const bool keys = PQ && (!PK || wave >= 2);
+    if (one_row(a, TILE * t - 63, TILE * t + 63)) {
+        if (keys) sum_tables<DT, PK, PQ, PQ, true>(a, sm, diagonal, h, wave);
+        else sum_tables<DT, PK, PQ, !PK, true>(a, sm, diagonal, h, wave);
         return;
     }
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int d = 0; d < 4; ++d) {
-            const int to = (32 * wave + 16 * n + c) * 64 + 16 * d + 4 * g;
-            if constexpr (PK) *reinterpret_cast<f32x4*>(part + to) = dpk[n][d];
-            if constexpr (PQ) *reinterpret_cast<f32x4*>(part + BY_OFFSET * 64 + to) = dpq[n][d];
-        }
+    for (int n = threadIdx.x; n < TILE * OFFSET_ROW<DT>; n += THREADS) sm.by_query[n] = sm.by_key[n] = typename Elem<DT>::T(0.f);
+    if (keys) sum_tables<DT, PK, PQ, PQ, false>(a, sm, diagonal, h, wave);
+    else sum_tables<DT, PK, PQ, !PK, false>(a, sm, diagonal, h, wave);
 }
 
 // The first offset in [1 - L, L) whose table row is `row` or a later one (the lookup table does not decrease), L if there is none: 64 places at a time.
@@ -633,19 +674,22 @@ __device__ __forceinline__ int first_offset(const Args& a, int row) {
     return lo;
 }
 
-// A table row's gradient, offsets lo .. hi - 1: those of far diagonals come as four rows of each diagonal; the others, fewer than 128 at either end, from the one or two
-// diagonals whose tiles have them.  A wave for each row.
+// A table row's gradient, offsets lo .. hi - 1: those of far diagonals come as one row for each wave of a table; the others, fewer than 128 at either end, from the one or
+// two diagonals whose tiles have them.  A wave for each row; the far diagonals of a workgroup's rows are shared out among its waves.
 template <int DT>
 __global__ __launch_bounds__(THREADS) void tables_sum_kernel(Args a) {
-    const int which = blockIdx.z, h = a.head0 + blockIdx.y, row = blockIdx.x * (THREADS / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), d = threadIdx.x & 63;
-    const int diagonals = 2 * a.tiles - 1;
-    if (!(which ? a.pq.p : a.pk.p) || row >= 2 * a.span) return;
+    __shared__ float s_far[WAVES][WAVES][64];
+    __shared__ int s_range[WAVES][2];
+    const int which = blockIdx.z, h = a.head0 + blockIdx.y, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = blockIdx.x * WAVES + wave, d = threadIdx.x & 63;
+    const int diagonals = 2 * a.tiles - 1, share = a.pk.p && a.pq.p ? 2 : 4;
+    if (!(which ? a.pq.p : a.pk.p)) return;
     const int lo = first_offset(a, row), hi = first_offset(a, row + 1);
-    auto is_far = [&](int t) { return max(TILE * t - 63, 1 - a.L) >= lo && min(TILE * t + 63, a.L - 1) < hi; };
+    // diagonals whose offsets all lie in the row's
+    const int t0 = lo == 1 - a.L ? 1 - a.tiles : (lo + 63 + TILE * a.tiles + TILE - 1) / TILE - a.tiles, t1 = hi == a.L ? a.tiles - 1 : (hi - 64 + TILE * a.tiles) / TILE - a.tiles;
+    if (d == 0) s_range[wave][0] = t0, s_range[wave][1] = hi > lo ? t1 : t0 - 1;
     const float* const parts = a.partial + (int64_t(blockIdx.y) * diagonals * a.splits * 2 + which) * BY_OFFSET * 64 + d;
     constexpr int64_t EACH = 2 * BY_OFFSET * 64;
-    float sum = 0.f;
-    auto add = [&](int t, int at) {             // row `at` of diagonal t, all its parts
+    auto add = [&](float& sum, int t, int at) {             // row `at` of diagonal t, all its parts
         const float* p = parts + int64_t(t + a.tiles - 1) * a.splits * EACH + at * 64;
         const int n = splits_of(a, t);
         int s = 0;
@@ -655,25 +699,36 @@ __global__ __launch_bounds__(THREADS) void tables_sum_kernel(Args a) {
         }
         for (; s < n; ++s) sum += p[s * EACH];
     };
+    float sum = 0.f;
     auto offsets = [&](int from, int to) {
         for (int off = from; off < to; ++off) {
             const int last = (off + 63 + TILE * a.tiles) / TILE - a.tiles, r = off + 63 - TILE * last;      // (rounded down)
             for (int n = 0; n < 2; ++n) {
                 const int t = last - n, at = r + TILE * n;          // offset `at` of diagonal t
-                if (at <= 126 && t > -a.tiles && t < a.tiles && !is_far(t)) add(t, at);
+                if (at <= 126 && t > -a.tiles && t < a.tiles && !(t0 <= t && t <= t1)) add(sum, t, at);
             }
         }
     };
     const int middle = hi - lo > 256 ? 128 : (hi - lo + 1) / 2;
     offsets(lo, lo + middle);
     offsets(max(lo + middle, hi - 128), hi);
-    if (hi > lo) {
-        const int t0 = lo == 1 - a.L ? 1 - a.tiles : (lo + 63 + TILE * a.tiles) / TILE - a.tiles, t1 = hi == a.L ? a.tiles - 1 : (hi + TILE * a.tiles) / TILE - a.tiles;
-        for (int t = t0; t <= t1; ++t)
-            if (is_far(t))
-                for (int n = 0; n < 4; ++n) add(t, n);
+    __syncthreads();
+    bool any = false;
+#pragma unroll
+    for (int n = 0; n < WAVES; ++n) {
+        const int from = s_range[n][0], to = s_range[n][1];
+        any = any || from <= to;
+        float far = 0.f;
+        for (int t = from + ((wave - from) & (WAVES - 1)); t <= to; t += WAVES)
+            for (int i = 0; i < share; ++i) add(far, t, i);
+        s_far[n][wave][d] = far;
     }
-    if (d < a.D) {
+    if (any) {
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < WAVES; ++n) sum += s_far[wave][n][d];
+    }
+    if (d < a.D && row < 2 * a.span) {
         using T = typename Elem<DT>::T;
         T* const to = static_cast<T*>(which ? a.dpq : a.dpk) + h * (which ? a.dpq_h : a.dpk_h) + int64_t(row) * a.D + d;
         *to = T(sum * a.scale / score_power<DT>(a));
