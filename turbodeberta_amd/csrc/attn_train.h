@@ -85,14 +85,6 @@ __device__ __forceinline__ void wave_fence() {
     __builtin_amdgcn_wave_barrier();
 }
 
-template <int DT>
-__device__ __forceinline__ typename Elem<DT>::X8 zero8() {
-    typename Elem<DT>::X8 x;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = typename Elem<DT>::T(0.f);
-    return x;
-}
-
 // Eight neighbouring values at a 16-byte boundary of LDS or global memory.
 template <int DT>
 __device__ __forceinline__ typename Elem<DT>::X8 read8(const typename Elem<DT>::T* p) {
@@ -102,6 +94,13 @@ __device__ __forceinline__ typename Elem<DT>::X8 read8(const typename Elem<DT>::
     } else {
         return *reinterpret_cast<const typename Elem<DT>::X8*>(p);
     }
+}
+
+// What is written ahead of it stays ahead.  16 bits: operands are asked for well ahead of their products (left alone, the compiler fetches them two by two, and every
+// product waits for LDS).  float32 has no registers for that.
+template <int DT>
+__device__ __forceinline__ void ahead() {
+    if constexpr (DT != TDB_F32) __builtin_amdgcn_sched_barrier(0);
 }
 
 // Frag of rows `row` + c, columns k0 + 8 g ..; row a multiple of 16
@@ -362,6 +361,7 @@ __device__ __forceinline__ float column_max(float x) {
 
 constexpr int OWN_ROW = 85;             // floats of a row of x's term, see above
 constexpr int OTHER_ROW = 36;           // and of y's term: 16 rows at the same column are on distinct banks
+static_assert(2 * OTHER_ROW <= OWN_ROW, "");
 constexpr int OWN_TERM = 16 * OWN_ROW, TERMS = OWN_TERM + 16 * OTHER_ROW;      // floats of a wave's scratch for the two
 
 // A table's rows r = 0 .. 126 of a tile of 64 x and 64 y, and one more.
@@ -389,6 +389,9 @@ __device__ __forceinline__ typename Elem<DT>::X8 ring_frag(const typename Elem<D
     return turned_frag<DT>(rows, at, at + 4, col, place<DT>);
 }
 
+// Four results behind the wait states of their products, on every path (see tdb_settled).
+__device__ __forceinline__ void settle(f32x4 (&s)[4]) { asm volatile("s_nop 7\n\ts_nop 7" : "+v"(s[0]), "+v"(s[1]), "+v"(s[2]), "+v"(s[3])); }
+
 // Scores of the wave's 16 rows x (x block `first`) with a step's 64 rows y, without the scale.  own[k]: frags of x.  Rings whose row for r is (r + base) mod RING, base a
 // multiple of 64.  scratch: the wave's own, TERMS floats.  far: the step's relative positions have one table row, so the terms are one number for each x and one for
 // each y.
@@ -411,36 +414,38 @@ __device__ __forceinline__ void scores(f32x4 (&s)[4], const typename Elem<DT>::X
             s[m] = E::mma(y1, own[1], E::mma(y0, own[0], w));
             if constexpr (OTHER) s[m] = E::mma(y1, t1, E::mma(y0, t0, s[m]));
         }
+        settle(s);
         return;
     }
+    X8 t[5][2], y[4][2];
     if constexpr (OWN) {
-        f32x4 w[5];
 #pragma unroll
-        for (int n = 0; n < 5; ++n) {           // r = 16 (first + n) + 15 - row of the frag
-            const typename E::T* const at = own_ring + wrapped(16 * (first + n) + base) * ROW<DT>;
-            w[n] = E::mma(read8<DT>(at + place<DT>(15 - c, 8 * g)), own[0], none);
-            w[n] = E::mma(read8<DT>(at + place<DT>(15 - c, 32 + 8 * g)), own[1], w[n]);
-        }
+        for (int n = 0; n < 5; ++n)             // r = 16 (first + n) + 15 - row of the frag
 #pragma unroll
-        for (int n = 0; n < 5; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) scratch[c * OWN_ROW + 64 - 16 * n + 4 * g + e] = w[n][e];
+            for (int k = 0; k < 2; ++k) t[n][k] = read8<DT>(own_ring + wrapped(16 * (first + n) + base) * ROW<DT> + place<DT>(15 - c, 32 * k + 8 * g));
     }
-    X8 y[4][2];
 #pragma unroll
     for (int m = 0; m < 4; ++m)
 #pragma unroll
         for (int k = 0; k < 2; ++k) y[m][k] = row_frag<DT>(y_rows, 16 * m, 32 * k);
+    ahead<DT>();
     f32x4 w[OTHER ? 4 : 1][2];
+    if constexpr (OWN) {
+        f32x4 x[5];
+#pragma unroll
+        for (int n = 0; n < 5; ++n) x[n] = E::mma(t[n][0], own[0], none);
+#pragma unroll
+        for (int n = 0; n < 5; ++n) x[n] = E::mma(t[n][1], own[1], x[n]);
+#pragma unroll
+        for (int n = 0; n < 5; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) scratch[c * OWN_ROW + 64 - 16 * n + 4 * g + e] = x[n][e];
+    }
     if constexpr (OTHER) {
 #pragma unroll
-        for (int n = 0; n < 5; ++n) {           // r = 16 (first + n) + row: of y blocks 3 - n and 4 - n
-            const int at = wrapped(16 * (first + n) + base);
-            const X8 t0 = row_frag<DT>(other_ring, at, 0), t1 = row_frag<DT>(other_ring, at, 32);
+        for (int n = 0; n < 5; ++n)             // r = 16 (first + n) + row: of y blocks 3 - n and 4 - n
 #pragma unroll
-            for (int m = 3 - n; m <= 4 - n; ++m)
-                if (m >= 0 && m < 4) w[m][n - 3 + m] = E::mma(t1, y[m][1], E::mma(t0, y[m][0], none));
-        }
+            for (int k = 0; k < 2; ++k) t[n][k] = row_frag<DT>(other_ring, wrapped(16 * (first + n) + base), 32 * k);
     }
     wave_fence();
 #pragma unroll
@@ -448,54 +453,87 @@ __device__ __forceinline__ void scores(f32x4 (&s)[4], const typename Elem<DT>::X
         if constexpr (OWN) s[m] = *reinterpret_cast<const f32x4*>(scratch + c * (OWN_ROW - 1) + 16 + 16 * m + 4 * g);
         else s[m] = none;
     }
-#pragma unroll
-    for (int m = 0; m < 4; ++m) s[m] = E::mma(y[m][1], own[1], E::mma(y[m][0], own[0], s[m]));
+    ahead<DT>();
     if constexpr (OTHER) {
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
-            float* const other = scratch + OWN_TERM;
+        for (int k = 0; k < 2; ++k)
 #pragma unroll
-            for (int n = 0; n < 2; ++n) *reinterpret_cast<f32x4*>(other + c * OTHER_ROW + 16 * n + 4 * g) = w[m][n];
-            wave_fence();
+            for (int m = 0; m < 4; ++m)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[m][e] += other[(4 * g + e) * OTHER_ROW + c + 15 - 4 * g - e];
-            wave_fence();
-        }
+                for (int n = 0; n < 2; ++n) w[m][n] = E::mma(t[3 - m + n][k], y[m][k], k == 0 ? none : w[m][n]);
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int m = 0; m < 4; ++m) s[m] = E::mma(y[m][k], own[k], s[m]);
+    if constexpr (OTHER) {                      // three y blocks at once: x's term, which has been read, makes room for two
+        auto at = [&](int m) { return scratch + (m == 1 ? 0 : m == 2 ? 16 * OTHER_ROW : OWN_TERM); };
+        auto put = [&](int m) {
+#pragma unroll
+            for (int n = 0; n < 2; ++n) *reinterpret_cast<f32x4*>(at(m) + c * OTHER_ROW + 16 * n + 4 * g) = w[m][n];
+        };
+        auto get = [&](int m) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[m][e] += at(m)[(4 * g + e) * OTHER_ROW + c + 15 - 4 * g - e];
+        };
+        put(0), put(1), put(2);
+        wave_fence();
+        get(0);
+        wave_fence();
+        put(3);
+        get(1), get(2);
+        wave_fence();
+        get(3);
+    } else {
+        settle(s);
     }
     wave_fence();
 }
 
-// Four neighbouring values of a result's row, rounded to the type.
+// 16 rows of a tensor from `row` on, of which `rows` are there; offsets of a lane's row c and column d.
 template <int DT>
-__device__ __forceinline__ void store4(typename Elem<DT>::T* p, f32x4 v) {
-    using T = typename Elem<DT>::T;
-    typedef __attribute__((ext_vector_type(4))) T T4;
-    T4 x;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] = T(v[e]);
-    *reinterpret_cast<T4*>(p) = x;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows16(const Tensor& t, const Args& a, const Where& w, int h, int row, int rows) {
+    const int stride = int(t.l) * int(sizeof(typename Elem<DT>::T));
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<typename Elem<DT>::T*>(rows_of<DT>(t, a, w, h)) + row * t.l, 0, min(max(rows - row, 0), 16) * stride, 0x00020000);
+}
+template <int DT>
+__device__ __forceinline__ uint32_t offset16(const Tensor& t, const Args& a, int d) {
+    return d < a.D ? (uint32_t(lane_c()) * uint32_t(t.l) + d) * sizeof(typename Elem<DT>::T) : NOWHERE;
 }
 
 // A result with columns x (16 of them from row `row` on) and rows d, as rows of a tensor: rows of the sequence as they are, the padding behind them as zeros.
 template <int DT>
 __device__ __forceinline__ void store_rows(const Tensor& t, const Args& a, const Where& w, int h, int row, const f32x4 (&acc)[4], float factor) {
     using T = typename Elem<DT>::T;
-    T* const to = const_cast<T*>(rows_of<DT>(t, a, w, h));
-    const int r = row + lane_c();
-    if (r >= (a.cu ? w.len : a.L)) return;
+    typedef __attribute__((ext_vector_type(4))) T T4;
+    typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
+    const __amdgpu_buffer_rsrc_t to = rows16<DT>(t, a, w, h, row, a.cu ? w.len : a.L);
+    const bool there = row + lane_c() < w.len;
 #pragma unroll
-    for (int d = 0; d < 4; ++d)
-        if (16 * d + 4 * lane_g() < a.D) store4<DT>(to + r * t.l + 16 * d + 4 * lane_g(), r < w.len ? acc[d] * factor : f32x4{0.f, 0.f, 0.f, 0.f});
+    for (int d = 0; d < 4; ++d) {
+        T4 x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = T(there ? acc[d][e] * factor : 0.f);
+        const int at = int(offset16<DT>(t, a, 16 * d + 4 * lane_g()));
+        if constexpr (DT == TDB_F32) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), to, at, 0, 0);
+        else __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, x), to, at, 0, 0);
+    }
 }
 
 // The wave's own rows as frags; zeros past the sequence and past D columns.
 template <int DT>
 __device__ __forceinline__ void load_own(typename Elem<DT>::X8 (&own)[2], const Tensor& t, const Args& a, const Where& w, int h, int row) {
-    const typename Elem<DT>::T* const from = rows_of<DT>(t, a, w, h);
+    const __amdgpu_buffer_rsrc_t from = rows16<DT>(t, a, w, h, row, w.len);
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-        const int r = row + lane_c(), d = 32 * k + 8 * lane_g();
-        own[k] = r < w.len && d < a.D ? read8<DT>(from + r * t.l + d) : zero8<DT>();
+        const int at = int(offset16<DT>(t, a, 32 * k + 8 * lane_g()));
+        const u32x4 lo = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(from, at, 0, 0));
+        if constexpr (DT == TDB_F32) {
+            const u32x4 hi = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(from, at, 16, 0));
+            own[k] = __builtin_bit_cast(f32x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        } else {
+            own[k] = __builtin_bit_cast(typename Elem<DT>::X8, lo);
+        }
     }
 }
 

@@ -83,6 +83,12 @@ __global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_fwd_kernel(Args a) {
 
         f32x4 s[4];
         scores<DT, PK, PQ>(s, q, sm.k, sm.pk, sm.pq, base, wave, sm.scratch[wave], far);
+        X8 v[2][4];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int d = 0; d < 4; ++d) v[u][d] = pair_frag<DT>(sm.v, 32 * u, 16 * d);
+        ahead<DT>();
         if (y0 + TILE > w.len) {
 #pragma unroll
             for (int m = 0; m < 4; ++m)
@@ -105,28 +111,29 @@ __global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_fwd_kernel(Args a) {
         X8 p[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            float v[8];
+            float z[8];
 #pragma unroll
             for (int n = 0; n < 8; ++n) {
-                v[n] = __builtin_amdgcn_exp2f(fmaf(s[2 * u + (n >> 2)][n & 3], c1, -from));
-                sum += v[n];
+                z[n] = __builtin_amdgcn_exp2f(fmaf(s[2 * u + (n >> 2)][n & 3], c1, -from));
+                sum += z[n];
             }
             if (a.threshold) {
                 const uint4 r = tdb_philox(4 * ((y0 >> 5) + u) + g, row + c, w.b * a.H + h, 1, key);
 #pragma unroll
-                for (int n = 0; n < 8; ++n) v[n] = tdb_number(r, n) >= a.threshold ? v[n] : 0.f;
+                for (int n = 0; n < 8; ++n) z[n] = tdb_number(r, n) >= a.threshold ? z[n] : 0.f;
             }
 #pragma unroll
-            for (int n = 0; n < 8; ++n) p[u][n] = T(v[n]);
+            for (int n = 0; n < 8; ++n) p[u][n] = T(z[n]);
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int d = 0; d < 4; ++d) o[d] = E::mma(pair_frag<DT>(sm.v, 32 * u, 16 * d), p[u], o[d]);
+            for (int d = 0; d < 4; ++d) o[d] = E::mma(v[u][d], p[u], o[d]);
     }
     const float all = column_sum(sum);
     store_rows<DT>(a.o, a, w, h, row, o, all > 0.f ? a.factor / all : all == 0.f ? 0.f : all);      // (NaN stays)
-    if (g == 0 && row + c < w.len) a.lse[h * a.lines + w.line + row + c] = all == 0.f ? __builtin_inff() : most + __builtin_amdgcn_logf(all);
+    const float lse = all == 0.f ? __builtin_inff() : most + __builtin_amdgcn_logf(all);
+    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, lse), buffer(a.lse + h * a.lines + w.line, int64_t(w.len) * 4), g == 0 ? (row + c) * 4 : int(NOWHERE), 0, 0);
 }
 
 // --------------------------------------------------------------------------------------------------------------- backward
@@ -290,9 +297,24 @@ __global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_bwd_kv_kernel(Args a
         }
         f32x4 s[4], dp[4];
         scores<DT, PQ, PK>(s, k, sm.q, sm.pq, sm.pk, base, wave, sm.scratch[wave], far);
+        {
+            X8 y[4][2];
 #pragma unroll
-        for (int m = 0; m < 4; ++m)
-            dp[m] = E::mma(row_frag<DT>(sm.dout, 16 * m, 32), v[1], E::mma(row_frag<DT>(sm.dout, 16 * m, 0), v[0], f32x4{0.f, 0.f, 0.f, 0.f}));
+            for (int m = 0; m < 4; ++m)
+#pragma unroll
+                for (int n = 0; n < 2; ++n) y[m][n] = row_frag<DT>(sm.dout, 16 * m, 32 * n);
+            ahead<DT>();
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int m = 0; m < 4; ++m) dp[m] = E::mma(y[m][n], v[n], n == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : dp[m]);
+        }
+        X8 turned[2][4];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int d = 0; d < 4; ++d) turned[u][d] = pair_frag<DT>(sm.dout, 32 * u, 16 * d);
+        ahead<DT>();
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
             const f32x4 lse = *reinterpret_cast<const f32x4*>(sm.lse + 16 * m + 4 * g);
@@ -334,13 +356,20 @@ __global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_bwd_kv_kernel(Args a
 #pragma unroll
             for (int n = 0; n < 16; ++n) skewed[c * SKEW + 79 - 16 * (n >> 2) - 4 * g - (n & 3)] = dsx[n >> 3][n & 7];
         }
+        X8 q[2][4];
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int d = 0; d < 4; ++d) {
-                dv[d] = E::mma(pair_frag<DT>(sm.dout, 32 * u, 16 * d), p[u], dv[d]);
-                dk[d] = E::mma(pair_frag<DT>(sm.q, 32 * u, 16 * d), dsx[u], dk[d]);
-            }
+            for (int d = 0; d < 4; ++d) q[u][d] = pair_frag<DT>(sm.q, 32 * u, 16 * d);
+        ahead<DT>();
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int d = 0; d < 4; ++d) dv[d] = E::mma(turned[u][d], p[u], dv[d]);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int d = 0; d < 4; ++d) dk[d] = E::mma(q[u][d], dsx[u], dk[d]);
         if constexpr (PQ) {
             if (far) {
 #pragma unroll
@@ -351,12 +380,18 @@ __global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_bwd_kv_kernel(Args a
                 }
             } else {
                 wave_fence();
+                X8 t[3][4], b[3];
 #pragma unroll
                 for (int n = 0; n < 3; ++n) {
-                    const X8 b = skew_frag<DT>(skewed, n);
+                    b[n] = skew_frag<DT>(skewed, n);
 #pragma unroll
-                    for (int d = 0; d < 4; ++d) dk[d] = E::mma(ring_frag<DT>(sm.pq, 16 * wave + 32 * n + base, 16 * d), b, dk[d]);
+                    for (int d = 0; d < 4; ++d) t[n][d] = ring_frag<DT>(sm.pq, 16 * wave + 32 * n + base, 16 * d);
                 }
+                ahead<DT>();
+#pragma unroll
+                for (int n = 0; n < 3; ++n)
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) dk[d] = E::mma(t[n][d], b[n], dk[d]);
                 wave_fence();
             }
         }
@@ -456,23 +491,38 @@ __global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_bwd_q_kernel(Args a)
         }
         __syncthreads();
         if (y_next < w.len) fetch(next);
+        X8 b[2], k[2][4];
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-            const X8 b = line_frag<DT>(sm.ds, 32 * n, 16 * wave);
+            b[n] = line_frag<DT>(sm.ds, 32 * n, 16 * wave);
 #pragma unroll
-            for (int d = 0; d < 4; ++d) {
-                dq[d] = E::mma(line_frag<DT>(sm.k, 32 * n, 16 * d), b, dq[d]);
-                if (PK && far) dq[d] = E::mma(level_frag<DT>(sm.pk, wrapped(63 + base), 16 * d), b, dq[d]);
-            }
+            for (int d = 0; d < 4; ++d) k[n][d] = line_frag<DT>(sm.k, 32 * n, 16 * d);
         }
         if (PK && !far) {
+            X8 by[3], t[3][4];
 #pragma unroll
             for (int n = 0; n < 3; ++n) {
-                const X8 b = skew_frag<DT>(sm.skewed[wave], n);
+                by[n] = skew_frag<DT>(sm.skewed[wave], n);
 #pragma unroll
-                for (int d = 0; d < 4; ++d) dq[d] = E::mma(ring_frag<DT>(sm.pk, 16 * wave + 32 * n + base, 16 * d), b, dq[d]);
+                for (int d = 0; d < 4; ++d) t[n][d] = ring_frag<DT>(sm.pk, 16 * wave + 32 * n + base, 16 * d);
+            }
+            ahead<DT>();
+#pragma unroll
+            for (int n = 0; n < 3; ++n)
+#pragma unroll
+                for (int d = 0; d < 4; ++d) dq[d] = E::mma(t[n][d], by[n], dq[d]);
+        } else if (PK) {
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+                const X8 t = level_frag<DT>(sm.pk, wrapped(63 + base), 16 * d);
+#pragma unroll
+                for (int n = 0; n < 2; ++n) dq[d] = E::mma(t, b[n], dq[d]);
             }
         }
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int d = 0; d < 4; ++d) dq[d] = E::mma(k[n][d], b[n], dq[d]);
         base ^= 64;
     };
     Next one, two;
