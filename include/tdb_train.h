@@ -57,10 +57,11 @@ int64_t tdb_norm_workspace(int64_t rows, int32_t hidden);
  * [total_tokens, heads, head_dim], stride_b unused), position terms as tables, with dropout on the probabilities; head_dim a multiple of 8 up to 64.
  * The probability of key j for query i of head h in sequence b has number 4 (j / 16 mod 2) + j mod 4 of counter (4 (j / 32) + j / 4 mod 4, i, b * heads + h, 1).
  * Forward writes o and lse, float32 [heads, rows], rows = batch * max_seqlen or total_tokens: the logarithm (base 2) of the sum of each row's exponentials, for the backward
- * call, which also reads o.  Backward writes dq, dk, dv and the gradients of the tables, [heads, 2 span, head_dim] with rows back to back.  Rows beyond a sequence's
+ * call, which also reads o.  In 16 bits o_rest, [heads, rows, head_dim] back to back, takes what rounding took from o and goes to the backward call with it; NULL in both calls:
+ * the gradients are made from o as it is rounded, and are the less exact the longer the rows.  Backward writes dq, dk, dv and the gradients of the tables, [heads, 2 span, head_dim] with rows back to back.  Rows beyond a sequence's
  * length, and packed rows of no sequence, are zeros in every result; what the inputs hold there does not matter.  workspace: tdb_attn_train_workspace() bytes for the
- * same arguments, 16-byte aligned.  Besides a few bytes for each row and table it holds the scores' gradients of as many heads at a time as fit 512 MiB, at least one:
- * element size * sum of (length * max_seqlen), lengths rounded up to 64.
+ * same arguments, 16-byte aligned.  Besides a few bytes for each row and table it holds the scores' gradients of as many heads at a time as fit 2 GiB, at least one:
+ * element size * sum of (length * max_seqlen), lengths rounded up to 64.  Where there are tables, also a part for each table row and for each 64 x 64 of these scores 1 KiB.
  * The gradient of rows whose sequence has one token is zero in q, k and the tables.
  */
 typedef struct tdb_train_attn_args {
@@ -87,6 +88,7 @@ typedef struct tdb_train_attn_args {
     void*   workspace;
     int64_t workspace_bytes;
     const int64_t* seed;
+    void*   o_rest;
 } tdb_train_attn_args;
 
 int tdb_attn_train_fwd(const tdb_train_attn_args* args, void* stream);

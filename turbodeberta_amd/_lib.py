@@ -96,7 +96,7 @@ class TrainAttnArgs(C.Structure):
         ("seqlens_k", C.c_void_p), ("cu_seqlens", C.c_void_p), ("delta_lut", C.c_void_p), ("pos_key", C.c_void_p), ("pos_query", C.c_void_p),
         ("pos_key_stride_h", C.c_int64), ("pos_key_stride_r", C.c_int64), ("pos_query_stride_h", C.c_int64), ("pos_query_stride_r", C.c_int64),
         ("dpos_key", C.c_void_p), ("dpos_query", C.c_void_p), ("dpos_key_stride_h", C.c_int64), ("dpos_query_stride_h", C.c_int64),
-        ("lse", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64), ("seed", C.c_void_p),
+        ("lse", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64), ("seed", C.c_void_p), ("o_rest", C.c_void_p),
     ]
 
 

@@ -153,9 +153,14 @@ struct Args {
     int32_t blocks;                     // per head
     int64_t lines;                      // rows of lse and delta for each head
     float *lse, *delta;
+    void* rest;                         // 16 bits: what rounding took from o
+    int32_t* starts;                    // of table rows: the first offset whose row is this one or a later one
     void* ds;                           // [heads][tiles of rows][tiles][64 x 64]
-    float* partial;
-    int32_t tiles, row_tiles, splits;   // tiles: of the longest sequence; row_tiles: of all sequences
+    float *partial, *level_parts, *row_sums;
+    int32_t* level;                     // the first and the last diagonal of tiles whose offsets all have the last, the first row
+    int32_t tiles, row_tiles;           // of the longest sequence; of all sequences
+    int32_t split_bits, seg_bits;       // parts of the longest diagonal: of the sequences, of each sequence
+    int32_t per_tile;                   // 65536 / tiles, rounded up
     void *dpk, *dpq;                    // [H, table rows, D]
     int64_t dpk_h, dpq_h;
     const int64_t* seed;
@@ -170,6 +175,7 @@ struct Where {
     int64_t first;          // row of the packed tensors (else 0)
     int64_t line;           // of lse and delta
     int64_t row_tile;       // number of the sequence's first row tile among all sequences'
+    int block;              // number of this tile, in the workspace too
 };
 
 __device__ __forceinline__ int valid_rows(const Args& a, int b, int64_t& first) {
@@ -190,6 +196,7 @@ __device__ __forceinline__ bool locate(const Args& a, int& h, Where& w) {
     const uint32_t n = xcd * part + min(xcd, more) + (id >> 3);
     h = __builtin_amdgcn_readfirstlane(int(n / uint32_t(a.blocks)));
     const int block = int(n) - h * a.blocks;
+    w.block = block;
     h += a.head0;
     if (!a.cu) {
         const int tiles = (a.L + rows - 1) / rows;
@@ -517,6 +524,25 @@ __device__ __forceinline__ void store_rows(const Tensor& t, const Args& a, const
         const int at = int(offset16<DT>(t, a, 16 * d + 4 * lane_g()));
         if constexpr (DT == TDB_F32) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), to, at, 0, 0);
         else __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, x), to, at, 0, 0);
+    }
+}
+
+// What rounding takes from those results, [heads, rows, D] of the type, back to back.  The sum D = dO . O of a row stands against every score's gradient of the row, the same
+// error in all of them: with O as it is stored the gradients of long rows lose more to it than to their own roundings.
+template <int DT>
+__device__ __forceinline__ void store_rest(void* rest, const Args& a, const Where& w, int h, int row, const f32x4 (&acc)[4], float factor) {
+    using T = typename Elem<DT>::T;
+    typedef __attribute__((ext_vector_type(4))) T T4;
+    typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
+    const int stride = a.D * int(sizeof(T));
+    const __amdgpu_buffer_rsrc_t to = buffer(static_cast<char*>(rest) + (h * a.lines + w.line + row) * stride, rest ? min(w.len - row, 16) * stride : 0);
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+        T4 x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = T(acc[d][e] * factor - float(T(acc[d][e] * factor)));
+        const int col = 16 * d + 4 * lane_g();
+        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, x), to, col < a.D ? lane_c() * stride + col * int(sizeof(T)) : int(NOWHERE), 0, 0);
     }
 }
 

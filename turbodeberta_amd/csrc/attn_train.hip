@@ -131,18 +131,33 @@ __global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_fwd_kernel(Args a) {
             for (int d = 0; d < 4; ++d) o[d] = E::mma(v[u][d], p[u], o[d]);
     }
     const float all = column_sum(sum);
-    store_rows<DT>(a.o, a, w, h, row, o, all > 0.f ? a.factor / all : all == 0.f ? 0.f : all);      // (NaN stays)
+    const float whole = all > 0.f ? a.factor / all : all == 0.f ? 0.f : all;                       // (NaN stays)
+    store_rows<DT>(a.o, a, w, h, row, o, whole);
+    if constexpr (DT != TDB_F32) store_rest<DT>(a.rest, a, w, h, row, o, whole);
     const float lse = all == 0.f ? __builtin_inff() : most + __builtin_amdgcn_logf(all);
     __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, lse), buffer(a.lse + h * a.lines + w.line, int64_t(w.len) * 4), g == 0 ? (row + c) * 4 : int(NOWHERE), 0, 0);
 }
 
 // --------------------------------------------------------------------------------------------------------------- backward
 
-// D_i = dO_i . O_i for every row and head: 8 lanes each.  float16: the largest squares of the norms of rows of dO and V as well.
+// Rounded to a tile, up and down: |x| < 64 tiles.
+__device__ __forceinline__ int tile_up(const Args& a, int x) { return (x + TILE * a.tiles + TILE - 1) / TILE - a.tiles; }
+__device__ __forceinline__ int tile_down(const Args& a, int x) { return (x + TILE * a.tiles) / TILE - a.tiles; }
+
+// D_i = dO_i . O_i for every row and head: 8 lanes each.  float16: the largest squares of the norms of rows of dO and V as well.  And the offsets at which the rows of the
+// tables start, and the diagonals of tiles that lie in the last or in the first of these rows altogether.
 template <int DT>
 __global__ __launch_bounds__(THREADS) void attn_delta_kernel(Args a, uint32_t* largest) {
     using T = typename Elem<DT>::T;
     const int d = 8 * (threadIdx.x & 7);
+    if (a.lut)
+        for (int n = blockIdx.x * THREADS + threadIdx.x; n < 2 * a.L; n += gridDim.x * THREADS) {
+            const int off = n + 1 - a.L, before = n ? a.lut[off - 1 + a.lut_half] : -1, row = off < a.L ? a.lut[off + a.lut_half] : 2 * a.span;
+            for (int r = max(before, -1) + 1; r <= min(row, 2 * a.span); ++r) a.starts[r] = off;
+            const int last = a.lut[a.L - 1 + a.lut_half], first = a.lut[1 - a.L + a.lut_half];
+            if (off < a.L && row == last && (n == 0 || before != last)) a.level[0] = n == 0 ? 1 - a.tiles : tile_up(a, off + 63);
+            if (off == a.L ? n && first == last : n && before == first && row != first) a.level[1] = off == a.L ? -a.tiles : tile_down(a, off - 64);
+        }
     float most_do = 0.f, most_v = 0.f;
     for (int64_t unit = (int64_t(blockIdx.x) * THREADS + threadIdx.x) >> 3; unit < a.lines * a.H; unit += int64_t(gridDim.x) * (THREADS / 8)) {
         const int64_t row = unit / a.H;
@@ -168,6 +183,11 @@ __global__ __launch_bounds__(THREADS) void attn_delta_kernel(Args a, uint32_t* l
             const auto x = read8<DT>(static_cast<const T*>(a.dout.p) + b * a.dout.b + h * a.dout.h + r * a.dout.l + d);
 #pragma unroll
             for (int i = 0; i < 8; ++i) dot += float(o[i]) * float(x[i]), sq += float(x[i]) * float(x[i]);
+            if (DT != TDB_F32 && a.rest) {
+                const auto o = read8<DT>(static_cast<const T*>(a.rest) + (h * a.lines + row) * a.D + d);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) dot += float(o[i]) * float(x[i]);
+            }
             if constexpr (DT == TDB_F16) {
                 const auto v = read8<DT>(static_cast<const T*>(a.v.p) + b * a.v.b + h * a.v.h + r * a.v.l + d);
 #pragma unroll
@@ -193,6 +213,84 @@ __global__ __launch_bounds__(THREADS) void attn_delta_kernel(Args a, uint32_t* l
 }
 
 __global__ void clear_kernel(uint32_t* x) { x[threadIdx.x] = 0; }
+
+// Level tiles: those of the diagonals from hi on and up to lo, whose offsets all have the last or the first row of the tables.  They come in runs, and all that the
+// positions add to a gradient there is a row of a table times a sum of scores' gradients: kept in float32, from before they are rounded, for the owner's row of keys or
+// queries, and multiplied when its walk has ended.  4 x 4096, 256 buckets: of 127 diagonals 112.
+struct Level {
+    int hi, lo;
+    __device__ __forceinline__ Level(const Args& a) {
+        hi = 1 << 24, lo = -(1 << 24);
+        if (a.lut) hi = a.level[0], lo = a.level[1];
+    }
+    __device__ __forceinline__ void ready() { hi = __builtin_amdgcn_readfirstlane(hi), lo = __builtin_amdgcn_readfirstlane(lo); }
+    __device__ __forceinline__ bool has(int t) const { return t >= hi || t <= lo; }
+    __device__ __forceinline__ bool any(int first, int last) const { return last >= hi || first <= lo; }        // of first .. last
+};
+constexpr int ROW_SUMS = WAVES * TILE;          // of a tile: each query's over 16 keys at a time
+
+// Sums over the 16 lanes of a row of a result, for 16 values at once: lane c has that of value c.  (In each step a lane gives half of its values away and keeps the others;
+// the partners are c ^ 8, c ^ 7, c ^ 2, c ^ 1.)
+__device__ __forceinline__ float sums_of_16(float (&x)[16]) {
+    const int c = lane_c();
+    auto turn = [](float v, auto ctrl) { return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), decltype(ctrl)::value, 0xf, 0xf, true)); };
+    auto step = [&](auto half, auto ctrl) {
+        constexpr int N = decltype(half)::value;
+        const bool upper = c & N;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const float keep = upper ? x[n + N] : x[n], give = upper ? x[n] : x[n + N];
+            x[n] = keep + turn(give, ctrl);
+        }
+    };
+    step(std::integral_constant<int, 8>{}, std::integral_constant<int, 0x128>{});      // rotated by 8
+    step(std::integral_constant<int, 4>{}, std::integral_constant<int, 0x141>{});      // eight lanes mirrored
+    step(std::integral_constant<int, 2>{}, std::integral_constant<int, 0x4e>{});       // quads: 2 3 0 1
+    step(std::integral_constant<int, 1>{}, std::integral_constant<int, 0xb1>{});       // 1 0 3 2
+    return x[0];
+}
+
+__device__ __forceinline__ float* level_part(const Args& a, int which, int h, int block) { return a.level_parts + (int64_t(which * a.heads + h - a.head0) * a.blocks + block) * 2 * 64; }
+__device__ __forceinline__ void level_none(const Args& a, int which, int h, int block) {
+    if (threadIdx.x < 128) level_part(a, which, h, block)[threadIdx.x] = 0.f;
+}
+
+// An owner's share of level tiles.  sum[0], sum[1]: over the tiles of hi and lo, for row c.  Adds the two table rows times the sums to acc, and leaves the workgroup's two
+// sums of own rows times the sums for the table's gradient.  lds: 2 KiB.
+template <int DT>
+__device__ __forceinline__ void level_end(const Args& a, const Tensor& table, int which, int h, int block, const typename Elem<DT>::X8 (&own)[2], const float (&sum)[2], f32x4 (&acc)[4],
+                                          void* lds, int wave) {
+    using T = typename Elem<DT>::T;
+    const int c = lane_c(), g = lane_g();
+    float(*const part)[2][64] = static_cast<float(*)[2][64]>(lds);
+    __syncthreads();                    // (what was in it has been read)
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+        const int row = a.lut[(n ? 1 - a.L : a.L - 1) + a.lut_half];
+        const __amdgpu_buffer_rsrc_t from = buffer(static_cast<const T*>(table.p) + h * table.h + int64_t(row) * table.l, a.D * sizeof(T));
+        typedef __attribute__((ext_vector_type(4))) T T4;
+        typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            const int at = (16 * d + 4 * g) * int(sizeof(T));
+            T4 t;
+            if constexpr (DT == TDB_F32) t = __builtin_bit_cast(T4, __builtin_amdgcn_raw_buffer_load_b128(from, at, 0, 0));
+            else t = __builtin_bit_cast(T4, __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(from, at, 0, 0)));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[d][e] += float(t[e]) * sum[n];
+        }
+        float x[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] = float(own[e >> 3][e & 7]) * sum[n];
+        const float total = sums_of_16(x);
+        part[wave][n][32 * (c >> 3) + 8 * g + (c & 7)] = total;
+    }
+    __syncthreads();
+    if (threadIdx.x < 128) {
+        const int n = threadIdx.x >> 6, d = threadIdx.x & 63;
+        level_part(a, which, h, block)[threadIdx.x] = (part[0][n][d] + part[1][n][d]) + (part[2][n][d] + part[3][n][d]);
+    }
+}
 
 // A skewed tile: row x has the values of y at index 79 - y.  A row is 105 values apart from the next, so that index 16 + r - x of row x, r = x - y + 63, lies at
 // 104 x + 16 + r: eight neighbouring r at a multiple of 8, and 16 x on distinct banks.  r runs to 95: what lies outside of 0 <= y < 64 is not the row's.
@@ -230,6 +328,7 @@ __global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_bwd_kv_kernel(Args a
     int h;
     Where w;
     if (!locate<TILE>(a, h, w)) return;
+    Level level(a);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane_c(), g = lane_g();
     const int row = w.row0 + 16 * wave;             // the wave's first key
     f32x4 dk[4], dv[4];
@@ -280,10 +379,14 @@ __global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_bwd_kv_kernel(Args a
     const float down = unshift * rounded;
     const bool edge = w.row0 + TILE > w.len;
     const int tile_col = row / TILE, bit = (row & 16) + c;
-    T* ds = static_cast<T*>(a.ds) + ((int64_t(h - a.head0) * a.row_tiles + w.row_tile) * a.tiles + tile_col) * TILE_VALUES + (row / 16 % 4 * 128 + lane) * 8;
+    T* ds = static_cast<T*>(a.ds) + ((int64_t(h - a.head0) * a.row_tiles + w.row_tile) * a.tiles + tile_col) * TILE_VALUES + row / 16 % 4 * 1024;
     T* const skewed = reinterpret_cast<T*>(sm.scratch[wave]);
     int base = 0, odd = 0;
-    for (int y0 = 0; y0 < w.len; y0 += TILE, base ^= 64, ds += int64_t(a.tiles) * TILE_VALUES, odd ^= 1) {
+    float by_key[2] = {0.f, 0.f};
+    float* row_sums = a.row_sums + ((int64_t(h - a.head0) * a.row_tiles + w.row_tile) * a.tiles + tile_col) * ROW_SUMS;
+    level.ready();
+    for (int y0 = 0; y0 < w.len; y0 += TILE, base ^= 64, ds += int64_t(a.tiles) * TILE_VALUES, row_sums += int64_t(a.tiles) * ROW_SUMS, odd ^= 1) {
+        const bool is_level = (PK || PQ) && level.has((y0 - w.row0) / TILE);
         __syncthreads();
         q_next.store(sm.q);
         do_next.store(sm.dout);
@@ -329,6 +432,7 @@ __global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_bwd_kv_kernel(Args a
                     if (y0 + 16 * m + 4 * g + e >= w.len || row + c >= w.len) s[m][e] = 0.f, dp[m][e] = 0.f;
         }
         X8 p[2], dsx[2];
+        float grads[16];
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
             const f32x4 delta = *reinterpret_cast<const f32x4*>(sm.delta + 16 * m + 4 * g);
@@ -345,14 +449,34 @@ __global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_bwd_kv_kernel(Args a
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 p[m >> 1][4 * (m & 1) + e] = T(pr[e]);
-                dsx[m >> 1][4 * (m & 1) + e] = T(s[m][e] * ((grad[e] - delta[e]) * down));
+                grads[4 * m + e] = s[m][e] * ((grad[e] - delta[e]) * down);
+                dsx[m >> 1][4 * (m & 1) + e] = T(grads[4 * m + e]);
             }
         }
-        if (tile_col * TILE < w.len) {
+        if (is_level) {
+            if constexpr (PQ) {
+                float all = 0.f;
 #pragma unroll
-            for (int u = 0; u < 2; ++u) *reinterpret_cast<X8*>(ds + u * 64 * 8) = dsx[u];
+                for (int n = 0; n < 16; ++n) all += grads[n];
+                by_key[y0 - w.row0 >= TILE * level.hi ? 0 : 1] += all;
+            }
+            if constexpr (PK) {
+                const float of_query = sums_of_16(grads);
+                __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, of_query), buffer(row_sums, ROW_SUMS * 4), (16 * (c >> 2) + 4 * g + (c & 3)) * 16, wave * 4, 0);
+            }
         }
-        if (PQ && !far) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const __amdgpu_buffer_rsrc_t to = buffer(ds, 1024 * sizeof(T));
+            if constexpr (DT == TDB_F32) {
+                const f32x8 x = __builtin_bit_cast(f32x8, dsx[u]);
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, __builtin_shufflevector(x, x, 0, 1, 2, 3)), to, lane * 32, u * 2048, 0);
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, __builtin_shufflevector(x, x, 4, 5, 6, 7)), to, lane * 32 + 16, u * 2048, 0);
+            } else {
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, dsx[u]), to, lane * 16, u * 1024, 0);
+            }
+        }
+        if (PQ && !far && !is_level) {
 #pragma unroll
             for (int n = 0; n < 16; ++n) skewed[c * SKEW + 79 - 16 * (n >> 2) - 4 * g - (n & 3)] = dsx[n >> 3][n & 7];
         }
@@ -370,7 +494,7 @@ __global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_bwd_kv_kernel(Args a
         for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int d = 0; d < 4; ++d) dk[d] = E::mma(q[u][d], dsx[u], dk[d]);
-        if constexpr (PQ) {
+        if (PQ && !is_level) {
             if (far) {
 #pragma unroll
                 for (int d = 0; d < 4; ++d) {
@@ -395,6 +519,12 @@ __global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_bwd_kv_kernel(Args a
                 wave_fence();
             }
         }
+    }
+    if (PQ && level.any(-w.row0 / TILE, (w.len - 1) / TILE - w.row0 / TILE)) {
+        by_key[0] = column_sum(by_key[0]), by_key[1] = column_sum(by_key[1]);
+        level_end<DT>(a, a.pq, 1, h, w.block, k, by_key, dk, sm.pq, wave);
+    } else if (PQ) {
+        level_none(a, 1, h, w.block);
     }
     store_rows<DT>(a.dk, a, w, h, row, dk, a.scale / power);
     store_rows<DT>(a.dv, a, w, h, row, dv, a.factor * unshift);
@@ -444,12 +574,13 @@ __global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_bwd_q_kernel(Args a)
     int h;
     Where w;
     if (!locate<TILE>(a, h, w)) return;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    Level level(a);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = w.row0 + 16 * wave;
     f32x4 dq[4];
 #pragma unroll
     for (int d = 0; d < 4; ++d) dq[d] = f32x4{0.f, 0.f, 0.f, 0.f};
     if (w.row0 >= w.len) {
-        store_rows<DT>(a.dq, a, w, h, w.row0 + 16 * wave, dq, 0.f);
+        store_rows<DT>(a.dq, a, w, h, row, dq, 0.f);
         return;
     }
     const T* tile = static_cast<const T*>(a.ds) + (int64_t(h - a.head0) * a.row_tiles + w.row_tile + w.row0 / TILE) * a.tiles * TILE_VALUES;
@@ -458,11 +589,20 @@ __global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_bwd_q_kernel(Args a)
         Stage<DT, THREADS> k, pk;
         Scores<DT> ds;
         int ends[2];
+        u32x4 sums;
     };
     Tables<DT, 1, THREADS, PK, false> tables(a, h);
     tables.fill(sm.pk, nullptr, w.row0);
     int y_next = 0;
+    const float* row_sums = a.row_sums + (int64_t(h - a.head0) * a.row_tiles + w.row_tile + w.row0 / TILE) * a.tiles * ROW_SUMS;
+    float by_query[2] = {0.f, 0.f};
+    level.ready();
     auto fetch = [&](Next& n) {
+        if constexpr (PK) {             // (zeros for other tiles)
+            const __amdgpu_buffer_rsrc_t from = buffer(row_sums, level.has((w.row0 - y_next) / TILE) ? ROW_SUMS * 4 : 0);
+            n.sums = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(from, (16 * wave + lane_c()) * 16, 0, 0));
+            row_sums += ROW_SUMS;
+        }
         keys.load(n.k);
         n.ds.load(tile);
         tile += TILE_VALUES;
@@ -474,13 +614,20 @@ __global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_bwd_q_kernel(Args a)
         tables.look(0, w.row0 - y_next);
     };
     int base = 0;
-    auto step = [&](Next& next) {
+    auto step = [&](Next& next, int y0) {
+        const int t = (w.row0 - y0) / TILE;
+        const bool is_level = PK && level.has(t);
         __syncthreads();
         next.k.store(sm.k);
+        if constexpr (PK) {
+            const f32x4 x = __builtin_bit_cast(f32x4, next.sums);
+            const float all = (x[0] + x[1]) + (x[2] + x[3]);
+            by_query[0] += t >= level.hi ? all : 0.f, by_query[1] += t >= level.hi ? 0.f : all;
+        }
         if constexpr (PK) next.pk.store(sm.pk + base * ROW<DT>);
         next.ds.store(sm.ds);
         const bool far = PK && __builtin_amdgcn_readfirstlane(next.ends[0]) == __builtin_amdgcn_readfirstlane(next.ends[1]);
-        if (PK && !far) {
+        if (PK && !far && !is_level) {
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
                 const int q = Scores<DT>::query(0);
@@ -492,13 +639,15 @@ __global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_bwd_q_kernel(Args a)
         __syncthreads();
         if (y_next < w.len) fetch(next);
         X8 b[2], k[2][4];
+        auto own = [&]() {
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            b[n] = line_frag<DT>(sm.ds, 32 * n, 16 * wave);
+            for (int n = 0; n < 2; ++n) {
+                b[n] = line_frag<DT>(sm.ds, 32 * n, 16 * wave);
 #pragma unroll
-            for (int d = 0; d < 4; ++d) k[n][d] = line_frag<DT>(sm.k, 32 * n, 16 * d);
-        }
-        if (PK && !far) {
+                for (int d = 0; d < 4; ++d) k[n][d] = line_frag<DT>(sm.k, 32 * n, 16 * d);
+            }
+        };
+        if (PK && !far && !is_level) {
             X8 by[3], t[3][4];
 #pragma unroll
             for (int n = 0; n < 3; ++n) {
@@ -507,11 +656,15 @@ __global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_bwd_q_kernel(Args a)
                 for (int d = 0; d < 4; ++d) t[n][d] = ring_frag<DT>(sm.pk, 16 * wave + 32 * n + base, 16 * d);
             }
             ahead<DT>();
+            own();
 #pragma unroll
             for (int n = 0; n < 3; ++n)
 #pragma unroll
                 for (int d = 0; d < 4; ++d) dq[d] = E::mma(t[n][d], by[n], dq[d]);
-        } else if (PK) {
+        } else {
+            own();
+        }
+        if (PK && far && !is_level) {
 #pragma unroll
             for (int d = 0; d < 4; ++d) {
                 const X8 t = level_frag<DT>(sm.pk, wrapped(63 + base), 16 * d);
@@ -529,14 +682,21 @@ __global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_bwd_q_kernel(Args a)
     fetch(one);
     if (y_next < w.len) fetch(two);
     for (int y0 = 0; y0 < w.len; y0 += 2 * TILE) {
-        step(one);
-        if (y0 + TILE < w.len) step(two);
+        step(one, y0);
+        if (y0 + TILE < w.len) step(two, y0 + TILE);
     }
-    store_rows<DT>(a.dq, a, w, h, w.row0 + 16 * wave, dq, a.scale / score_power<DT>(a));
+    if (PK && level.any(w.row0 / TILE - (w.len - 1) / TILE, w.row0 / TILE)) {
+        X8 q[2];
+        load_own<DT>(q, a.q, a, w, h, row);
+        level_end<DT>(a, a.pk, 0, h, w.block, q, by_query, dq, sm.pk, wave);
+    } else if (PK) {
+        level_none(a, 0, h, w.block);
+    }
+    store_rows<DT>(a.dq, a, w, h, row, dq, a.scale / score_power<DT>(a));
 }
 
-// Parts that the sequences of a diagonal are dealt to: as many as it has tiles, next to the longest one.
-__device__ __forceinline__ int splits_of(const Args& a, int t) { return max(1, a.splits * (a.tiles - abs(t)) / a.tiles); }
+// Parts that the sequences of a diagonal are dealt to, as many as it has tiles, next to the longest one; each is 2^seg_bits, to which a sequence's tiles are dealt in turn.
+__device__ __forceinline__ int splits_of(const Args& a, int t) { return min(max(1, (((a.tiles - abs(t)) << a.split_bits) * a.per_tile) >> 16), 1 << a.split_bits); }
 
 // Tables: a workgroup has a diagonal of tiles (query tile - key tile = t) of every `splits`-th sequence.  Its waves share the two tables and the 128 offsets r = i - j + 63 of
 // a tile: in blocks of 16, dealt in turn, so that each has as many of those that 32 queries (or keys) reach.  Where all offsets of a diagonal have one table row ("far")
@@ -569,11 +729,12 @@ __device__ __forceinline__ float row_sum(float x) {
 
 // The tiles of a diagonal in the sequences first, first + step, ...; a sequence's length is read while the one before it is walked through.
 struct Diagonal {
-    int t, step, it, end, b_next;
+    int t, step, it, end, b_next, seg, segs;
     int b, first, len;                  // of the sequence
     int from, to;                       // of the one to come, as they stand in memory
-    __device__ __forceinline__ void start(const Args& a, int diagonal, int sequence, int splits) {
-        t = diagonal, step = splits, b_next = sequence, it = end = 0;
+    __device__ __forceinline__ void start(const Args& a, int diagonal, int sequence, int seg, int splits) {
+        this->seg = seg;
+        t = diagonal, step = splits, b_next = sequence, segs = 1 << a.seg_bits, it = end = 0;
         peek(a);
     }
     __device__ __forceinline__ void peek(const Args& a) {
@@ -584,7 +745,7 @@ struct Diagonal {
         if (ends) to = ends[n];
     }
     __device__ __forceinline__ bool advance(const Args& a) {             // to the next tile; false: none is left
-        ++it;
+        it += segs;
         while (it >= end) {
             if (b_next >= a.B) return false;
             b = b_next, first = __builtin_amdgcn_readfirstlane(from);
@@ -593,7 +754,7 @@ struct Diagonal {
             b_next += step;
             peek(a);
             const int n = (len + TILE - 1) / TILE;
-            it = max(0, t), end = min(n, n + t);
+            it = max(0, t) + seg, end = min(n, n + t);
         }
         return true;
     }
@@ -615,7 +776,7 @@ struct TablesNext {
 
 // What a wave does, for each of the roles that waves have: every one of them passes the same barriers.  KEYS: it sums up for the table of queries (from keys).
 template <int DT, bool PK, bool PQ, bool KEYS, bool FAR>
-__device__ __forceinline__ void sum_tables(const Args& a, TablesLds<DT>& sm, Diagonal diagonal, int h, int wave) {
+__device__ __forceinline__ void sum_tables(const Args& a, TablesLds<DT>& sm, Diagonal diagonal, int h, int split, int wave) {
     using E = Elem<DT>;
     using T = typename E::T;
     using X8 = typename E::X8;
@@ -674,7 +835,7 @@ __device__ __forceinline__ void sum_tables(const Args& a, TablesLds<DT>& sm, Dia
             }
         }
     }
-    float* const part = a.partial + int64_t(blockIdx.x) * 2 * BY_OFFSET * 64 + (KEYS ? BY_OFFSET * 64 : 0);
+    float* const part = a.partial + ((((int64_t(h - a.head0) * (2 * a.tiles - 1) + diagonal.t + a.tiles - 1) << (a.split_bits + a.seg_bits)) + split) * 2 + (KEYS ? 1 : 0)) * (BY_OFFSET * 64);
 #pragma unroll
     for (int n = 0; n < (FAR ? 1 : BLOCKS); ++n)
 #pragma unroll
@@ -693,95 +854,138 @@ template <int DT, bool PK, bool PQ>
 __global__ __launch_bounds__(THREADS, DT == TDB_F32 ? 1 : 3) void attn_bwd_tables_kernel(Args a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     TablesLds<DT>& sm = *reinterpret_cast<TablesLds<DT>*>(smem);
-    const int diagonals = 2 * a.tiles - 1, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int split = blockIdx.x % a.splits, at = blockIdx.x / a.splits, t = at % diagonals - (a.tiles - 1), h = a.head0 + at / diagonals;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // Long diagonals first.  A short one has no use for its last parts: which of eight neighbours, one for each XCD, these are changes from diagonal to diagonal.
+    const int bits = a.split_bits + a.seg_bits, at = blockIdx.x >> bits, split = (blockIdx.x + at) & ((1 << bits) - 1), n = at / a.heads, t = n & 1 ? (n + 1) / 2 : -(n / 2);
+    const int h = a.head0 + at - n * a.heads;
     const int splits = splits_of(a, t);
-    if (split >= splits) return;
+    Level level(a);
+    level.ready();
+    if ((split >> a.seg_bits) >= splits || level.has(t)) return;
     Diagonal diagonal;
-    diagonal.start(a, t, split, splits);
+    diagonal.start(a, t, split >> a.seg_bits, split & ((1 << a.seg_bits) - 1), splits);
     const bool keys = PQ && (!PK || wave >= 2);
     if (one_row(a, TILE * t - 63, TILE * t + 63)) {
-        if (keys) sum_tables<DT, PK, PQ, PQ, true>(a, sm, diagonal, h, wave);
-        else sum_tables<DT, PK, PQ, !PK, true>(a, sm, diagonal, h, wave);
+        if (keys) sum_tables<DT, PK, PQ, PQ, true>(a, sm, diagonal, h, split, wave);
+        else sum_tables<DT, PK, PQ, !PK, true>(a, sm, diagonal, h, split, wave);
         return;
     }
     for (int n = threadIdx.x; n < TILE * OFFSET_ROW<DT>; n += THREADS) sm.by_query[n] = sm.by_key[n] = typename Elem<DT>::T(0.f);
-    if (keys) sum_tables<DT, PK, PQ, PQ, false>(a, sm, diagonal, h, wave);
-    else sum_tables<DT, PK, PQ, !PK, false>(a, sm, diagonal, h, wave);
-}
-
-// The first offset in [1 - L, L) whose table row is `row` or a later one (the lookup table does not decrease), L if there is none: 64 places at a time.
-__device__ __forceinline__ int first_offset(const Args& a, int row) {
-    int lo = 1 - a.L, hi = a.L;             // the answer lies in [lo, hi]
-    while (lo < hi) {
-        const int step = (hi - lo + 63) / 64, at = lo + (threadIdx.x & 63) * step;
-        const uint64_t less = __builtin_amdgcn_ballot_w64(at < hi && a.lut[at + a.lut_half] < row);
-        const int n = __builtin_popcountll(less);
-        if (n == 0) return lo;
-        hi = min(hi, lo + n * step);
-        lo = lo + (n - 1) * step + 1;
-    }
-    return lo;
+    if (keys) sum_tables<DT, PK, PQ, PQ, false>(a, sm, diagonal, h, split, wave);
+    else sum_tables<DT, PK, PQ, !PK, false>(a, sm, diagonal, h, split, wave);
 }
 
 // A table row's gradient, offsets lo .. hi - 1: those of far diagonals come as one row for each wave of a table; the others, fewer than 128 at either end, from the one or
-// two diagonals whose tiles have them.  A wave for each row; the far diagonals of a workgroup's rows are shared out among its waves.
+// two diagonals whose tiles have them.  A wave for each row, parts dealt to its four groups of 16 lanes and asked for four at a time; the outermost rows, which have
+// hundreds of offsets, take the workgroup's waves together.  (A wave for each row, one part after the other: 290 us at 4 x 4096.)  Which group has a part does not depend on
+// the longest length, and a sum's bits do not either.
 template <int DT>
 __global__ __launch_bounds__(THREADS) void tables_sum_kernel(Args a) {
-    __shared__ float s_far[WAVES][WAVES][64];
-    __shared__ int s_range[WAVES][2];
-    const int which = blockIdx.z, h = a.head0 + blockIdx.y, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = blockIdx.x * WAVES + wave, d = threadIdx.x & 63;
-    const int diagonals = 2 * a.tiles - 1, share = a.pk.p && a.pq.p ? 2 : 4;
+    constexpr int MANY = 32, MOST_GROUPS = THREADS / 16;
+    __shared__ f32x4 s_sum[MOST_GROUPS][16];
+    const int which = blockIdx.z, h = a.head0 + blockIdx.y, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), d = threadIdx.x & 15;
+    const int diagonals = 2 * a.tiles - 1, share_bits = a.pk.p && a.pq.p ? 1 : 2, split_bits = a.split_bits + a.seg_bits;
     if (!(which ? a.pq.p : a.pk.p)) return;
-    const int lo = first_offset(a, row), hi = first_offset(a, row + 1);
-    // diagonals whose offsets all lie in the row's
-    const int t0 = lo == 1 - a.L ? 1 - a.tiles : (lo + 63 + TILE * a.tiles + TILE - 1) / TILE - a.tiles, t1 = hi == a.L ? a.tiles - 1 : (hi - 64 + TILE * a.tiles) / TILE - a.tiles;
-    if (d == 0) s_range[wave][0] = t0, s_range[wave][1] = hi > lo ? t1 : t0 - 1;
-    const float* const parts = a.partial + (int64_t(blockIdx.y) * diagonals * a.splits * 2 + which) * BY_OFFSET * 64 + d;
-    constexpr int64_t EACH = 2 * BY_OFFSET * 64;
-    auto add = [&](float& sum, int t, int at) {             // row `at` of diagonal t, all its parts
-        const float* p = parts + int64_t(t + a.tiles - 1) * a.splits * EACH + at * 64;
-        const int n = splits_of(a, t);
-        int s = 0;
-        for (; s + 4 <= n; s += 4) {
-            const float x0 = p[s * EACH], x1 = p[(s + 1) * EACH], x2 = p[(s + 2) * EACH], x3 = p[(s + 3) * EACH];
-            sum += x0 + x1 + x2 + x3;
-        }
-        for (; s < n; ++s) sum += p[s * EACH];
+    const float* const parts = a.partial + (((int64_t(blockIdx.y) * diagonals) << (split_bits + 1)) + which) * (BY_OFFSET * 64) + 4 * d;
+    auto range = [&](int row, int& lo, int& hi) {
+        lo = hi = a.L;
+        if (row >= 2 * a.span) return;
+        lo = min(max(a.starts[row], 1 - a.L), a.L), hi = min(max(a.starts[row + 1], lo), a.L);
     };
-    float sum = 0.f;
-    auto offsets = [&](int from, int to) {
-        for (int off = from; off < to; ++off) {
-            const int last = (off + 63 + TILE * a.tiles) / TILE - a.tiles, r = off + 63 - TILE * last;      // (rounded down)
-            for (int n = 0; n < 2; ++n) {
-                const int t = last - n, at = r + TILE * n;          // offset `at` of diagonal t
-                if (at <= 126 && t > -a.tiles && t < a.tiles && !(t0 <= t && t <= t1)) add(sum, t, at);
+    // the sum of the row's parts that group `group` of `groups` (a power of two) has
+    auto sum_of = [&](int lo, int hi, int group, int groups) {
+        // diagonals whose offsets all lie in the row's
+        const int t0 = lo == 1 - a.L ? 1 - a.tiles : tile_up(a, lo + 63), t1 = hi == a.L ? a.tiles - 1 : tile_down(a, hi - 64);
+        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+        // where(n, t, at, s): part n is row `at` of part s of diagonal t; false: there is none
+        auto add = [&](int from, int to, auto where) {
+            constexpr int AHEAD = 4;
+            for (int n = from + ((group - from) & (groups - 1)); n < to; n += AHEAD * groups) {
+                f32x4 x[AHEAD];
+#pragma unroll
+                for (int u = 0; u < AHEAD; ++u) {
+                    int t = 0, at = 0, s = 0;
+                    const bool any = n + u * groups < to && where(n + u * groups, t, at, s) && (s >> a.seg_bits) < splits_of(a, t);
+                    const int64_t tile = ((int64_t(t + a.tiles - 1) << split_bits) + s) * (2 * BY_OFFSET * 64);
+                    const f32x4 y = *reinterpret_cast<const f32x4*>(parts + (any ? tile + at * 64 : 0));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[u][e] = any ? y[e] : 0.f;
+                }
+#pragma unroll
+                for (int u = 0; u < AHEAD; ++u) sum += x[u];
             }
+        };
+        const int zero = (a.L + MOST_GROUPS - 1) / MOST_GROUPS * MOST_GROUPS;           // offset `off` has the numbers (off + zero) << (split_bits + 1) ...
+        auto offsets = [&](int from, int to) {
+            add((from + zero) << (split_bits + 1), (to + zero) << (split_bits + 1), [&](int n, int& t, int& at, int& s) {
+                const int off = (n >> (split_bits + 1)) - zero;
+                t = ((off + 63) >> 6) - ((n >> split_bits) & 1), at = off + 63 - TILE * t, s = n & ((1 << split_bits) - 1);
+                return at <= 126 && t > -a.tiles && t < a.tiles && !(t0 <= t && t <= t1);
+            });
+        };
+        if (hi - lo > 256) {
+            offsets(lo, lo + 128);
+            offsets(hi - 128, hi);
+        } else {
+            offsets(lo, hi);
         }
+        if (t0 <= t1 && (lo == 1 - a.L || hi == a.L)) {      // level tiles: a sum of each workgroup that has met one, which stands for them all
+            const float* const from = a.level_parts + (int64_t(which * a.heads + blockIdx.y) * a.blocks * 2 + (hi == a.L ? 0 : 1)) * 64 + 4 * d;
+            const int share = min(groups, 4), mine = group & (share - 1);           // groups that share a sequence
+            for (int b = group / share; b < a.B; b += groups / share) {
+                int64_t first;
+                const int len = valid_rows(a, b, first), tiles = (len + TILE - 1) / TILE;
+                const int64_t at = a.cu ? first / TILE + b : int64_t(b) * a.tiles;
+                for (int n = mine; n < tiles; n += 4 * share) {
+                    f32x4 x[4];
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const bool any = n + u * share < tiles;
+                        const f32x4 y = *reinterpret_cast<const f32x4*>(from + (at + (any ? n + u * share : 0)) * 128);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[u][e] = any ? y[e] : 0.f;
+                    }
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) sum += x[u];
+                }
+            }
+        } else if (t0 <= t1) {
+            const int first = (a.tiles + MOST_GROUPS - 1) / MOST_GROUPS * MOST_GROUPS, bits = share_bits + split_bits;
+            add((t0 + first) << bits, (t1 + 1 + first) << bits, [&](int n, int& t, int& at, int& s) {
+                t = (n >> bits) - first, at = (n >> split_bits) & ((1 << share_bits) - 1), s = n & ((1 << split_bits) - 1);
+                return true;
+            });
+        }
+        return sum;
     };
-    const int middle = hi - lo > 256 ? 128 : (hi - lo + 1) / 2;
-    offsets(lo, lo + middle);
-    offsets(max(lo + middle, hi - 128), hi);
-    __syncthreads();
-    bool any = false;
-#pragma unroll
-    for (int n = 0; n < WAVES; ++n) {
-        const int from = s_range[n][0], to = s_range[n][1];
-        any = any || from <= to;
-        float far = 0.f;
-        for (int t = from + ((wave - from) & (WAVES - 1)); t <= to; t += WAVES)
-            for (int i = 0; i < share; ++i) add(far, t, i);
-        s_far[n][wave][d] = far;
-    }
-    if (any) {
-        __syncthreads();
-#pragma unroll
-        for (int n = 0; n < WAVES; ++n) sum += s_far[wave][n][d];
-    }
-    if (d < a.D && row < 2 * a.span) {
+    auto store = [&](int row, float all) {
+        if (row >= 2 * a.span || int(threadIdx.x & 63) >= a.D) return;
         using T = typename Elem<DT>::T;
-        T* const to = static_cast<T*>(which ? a.dpq : a.dpk) + h * (which ? a.dpq_h : a.dpk_h) + int64_t(row) * a.D + d;
-        *to = T(sum * a.scale / score_power<DT>(a));
+        T* const to = static_cast<T*>(which ? a.dpq : a.dpk) + h * (which ? a.dpq_h : a.dpk_h) + int64_t(row) * a.D + (threadIdx.x & 63);
+        *to = T(all * a.scale / score_power<DT>(a));
+    };
+    // what lane 4 d + e of a wave adds up: value e of lane d of each group
+    auto total = [&](int first, int groups) {
+        float all = 0.f;
+        for (int n = 0; n < groups; ++n) all += s_sum[first + n][(threadIdx.x & 63) >> 2][threadIdx.x & 3];
+        return all;
+    };
+    const int row0 = blockIdx.x * WAVES;
+    int lo, hi;
+    range(row0 + wave, lo, hi);
+    const bool many = hi - lo > MANY;
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    if (!many && hi > lo) sum = sum_of(lo, hi, (threadIdx.x >> 4) & 3, 4);
+    s_sum[threadIdx.x >> 4][d] = sum;
+    __syncthreads();
+    if (!many) store(row0 + wave, total(4 * wave, 4));
+    for (int n = 0; n < WAVES; ++n) {           // (the same for every wave)
+        range(row0 + n, lo, hi);
+        if (hi - lo <= MANY) continue;
+        __syncthreads();
+        s_sum[threadIdx.x >> 4][d] = sum_of(lo, hi, threadIdx.x >> 4, MOST_GROUPS);
+        __syncthreads();
+        if (wave == n) store(row0 + n, total(0, MOST_GROUPS));
     }
 }
 
@@ -791,12 +995,12 @@ size_t elem(int dtype) { return dtype == TDB_F32 ? 4 : 2; }
 int64_t up(int64_t x) { return (x + 255) / 256 * 256; }
 
 constexpr int64_t MOST_STRIDE = int64_t(1) << 24;        // bytes: 64 rows' offsets fit 31 bits
-constexpr int64_t MOST_SCORES = int64_t(512) << 20;      // bytes of dS at a time, unless one head has more
+constexpr int64_t MOST_SCORES = int64_t(2) << 30;        // bytes of dS at a time, unless one head has more (4 x 4096, 12 heads: 3.1 ms with 512 MiB, 2.8)
 
 // What a backward call needs, and how many heads it takes at a time.
 struct Plan {
-    int tiles, row_tiles, splits, heads;
-    int64_t lines, delta, partial, ds, bytes;       // offsets of the parts, and the sum
+    int tiles, row_tiles, split_bits, seg_bits, heads;
+    int64_t lines, starts, delta, level, partial, sums, ds, bytes;       // offsets of the parts, and the sum
 };
 Plan plan_of(const tdb_train_attn_args& a) {
     Plan p;
@@ -806,17 +1010,27 @@ Plan plan_of(const tdb_train_attn_args& a) {
     const int64_t each = int64_t(p.row_tiles) * p.tiles * TILE_VALUES * int64_t(elem(a.dtype));
     p.heads = int(std::max<int64_t>(1, std::min<int64_t>(a.heads, MOST_SCORES / std::max<int64_t>(each, 1))));
     const int diagonals = 2 * p.tiles - 1;
-    p.splits = int(std::max<int64_t>(1, std::min<int64_t>(a.batch, 768 / (int64_t(p.heads) * p.tiles))));     // three workgroups for each of 256 CUs
-    p.delta = 256;                                  // in front: the two maxima
-    p.partial = p.delta + up(p.lines * a.heads * 4);
-    p.ds = p.partial + ((a.pos_key || a.pos_query) ? int64_t(p.heads) * diagonals * p.splits * 2 * BY_OFFSET * 64 * 4 : 0);
+    // A diagonal's parts, a power of two: three workgroups for each of 256 CUs where every diagonal has its own sums, and 64 tiles for a workgroup where most are level.
+    int bits = 0;
+    while ((int64_t(2) << bits) * p.heads * p.tiles <= 768 && (2 << bits) <= a.batch) ++bits;
+    while (bits < 12 && (int64_t(a.batch) * p.tiles) >> bits > 64) ++bits;
+    p.split_bits = 0;
+    while (p.split_bits < bits && (2 << p.split_bits) <= a.batch) ++p.split_bits;
+    p.seg_bits = bits - p.split_bits;
+    p.starts = 256;                                 // in front: the two maxima and the diagonals of level tiles
+    p.delta = p.starts + up((2 * int64_t(a.span) + 1) * 4);
+    p.level = p.delta + up(p.lines * a.heads * 4);
+    const bool terms = a.pos_key || a.pos_query;
+    p.partial = p.level + (terms ? int64_t(2) * p.heads * p.row_tiles * 2 * 64 * 4 : 0);
+    p.sums = p.partial + (terms ? ((int64_t(p.heads) * diagonals) << (bits + 1)) * BY_OFFSET * 64 * 4 : 0);
+    p.ds = p.sums + (terms ? int64_t(p.heads) * p.row_tiles * p.tiles * ROW_SUMS * 4 : 0);
     p.bytes = p.ds + p.heads * each;
     return p;
 }
 
 bool aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
-int check(const tdb_train_attn_args* a, bool backward) {
+int check(const tdb_train_attn_args* a, bool backward, bool sizes_only = false) {
     if (!a) return tdb_fail(TDB_ERR_NULL, "args is NULL");
     if (a->dtype != TDB_F32 && a->dtype != TDB_BF16 && a->dtype != TDB_F16) return tdb_fail(TDB_ERR_DTYPE, "unknown dtype %d", a->dtype);
     if (a->batch < 0 || a->heads < 1 || a->heads > 65535) return tdb_fail(TDB_ERR_SHAPE, "bad batch %d / heads %d", a->batch, a->heads);
@@ -828,11 +1042,11 @@ int check(const tdb_train_attn_args* a, bool backward) {
     const int64_t lines = a->cu_seqlens ? a->total_tokens : int64_t(a->batch) * a->max_seqlen;
     if (lines * a->heads > (1 << 28) || (lines / TILE + a->batch) * a->heads >= (1 << 24))       // (of the launches' sizes)
         return tdb_fail(TDB_ERR_SHAPE, "%lld rows of %d heads: need 2^28 at most", (long long)lines, a->heads);
-    if (a->batch == 0 || lines == 0) return TDB_OK;
+    if (sizes_only || a->batch == 0 || lines == 0) return TDB_OK;
     if (!a->q || !a->k || !a->v || !a->o || !a->lse || (backward && (!a->dout || !a->dq || !a->dk || !a->dv || !a->workspace)))
         return tdb_fail(TDB_ERR_NULL, "a required pointer is NULL");
     if (a->threshold && !a->seed) return tdb_fail(TDB_ERR_NULL, "dropout needs a seed");
-    const void* ptrs[] = {a->q, a->k, a->v, a->o, a->dout, a->dq, a->dk, a->dv, a->pos_key, a->pos_query, a->workspace};
+    const void* ptrs[] = {a->q, a->k, a->v, a->o, a->dout, a->dq, a->dk, a->dv, a->pos_key, a->pos_query, a->workspace, a->o_rest};
     for (const void* p : ptrs)
         if (!aligned(p)) return tdb_fail(TDB_ERR_ALIGN, "tensors must be 16-byte aligned");
     for (int n = 0; n < 24; ++n) {
@@ -874,14 +1088,16 @@ Args args_of(const tdb_train_attn_args& a, const Plan& p) {
     k.seqlens = a.seqlens_k, k.cu = a.cu_seqlens;
     k.B = a.batch, k.H = a.heads, k.D = a.head_dim, k.L = a.max_seqlen, k.total = a.total_tokens;
     k.head0 = 0, k.heads = a.heads;
-    k.lines = p.lines, k.lse = a.lse;
-    k.tiles = p.tiles, k.row_tiles = p.row_tiles, k.splits = p.splits;
+    k.lines = p.lines, k.lse = a.lse, k.rest = a.dtype == TDB_F32 ? nullptr : a.o_rest;
+    k.tiles = p.tiles, k.row_tiles = p.row_tiles, k.split_bits = p.split_bits, k.seg_bits = p.seg_bits, k.per_tile = 65536 / p.tiles + 1;
     k.dpk = a.dpos_key, k.dpq = a.dpos_query, k.dpk_h = a.dpos_key_stride_h, k.dpq_h = a.dpos_query_stride_h;
     k.seed = a.seed, k.threshold = uint32_t(a.threshold), k.factor = tdb_kept_factor(a.threshold), k.scale = a.sm_scale;
     while (k.p_shift < 15 && (2 << k.p_shift) <= a.max_seqlen) ++k.p_shift;
     if (a.workspace) {
         char* const at = static_cast<char*>(a.workspace);
         k.largest = reinterpret_cast<const uint32_t*>(at);
+        k.starts = reinterpret_cast<int32_t*>(at + p.starts), k.level = reinterpret_cast<int32_t*>(at) + 2;
+        k.level_parts = reinterpret_cast<float*>(at + p.level), k.row_sums = reinterpret_cast<float*>(at + p.sums);
         k.delta = reinterpret_cast<float*>(at + p.delta);
         k.partial = reinterpret_cast<float*>(at + p.partial);
         k.ds = at + p.ds;
@@ -941,9 +1157,9 @@ struct Launch {
             e = launch<attn_bwd_q_kernel<DT, PK>>(sizeof(QLds<DT>), int64_t(k.blocks) * k.heads, THREADS, s, k);
             if constexpr (PK || PQ) {
                 if (e != hipSuccess) return e;
-                e = launch<attn_bwd_tables_kernel<DT, PK, PQ>>(sizeof(TablesLds<DT>), int64_t(k.heads) * (2 * k.tiles - 1) * k.splits, THREADS, s, k);
+                e = launch<attn_bwd_tables_kernel<DT, PK, PQ>>(sizeof(TablesLds<DT>), (int64_t(k.heads) * (2 * k.tiles - 1)) << (k.split_bits + k.seg_bits), THREADS, s, k);
                 if (e != hipSuccess) return e;
-                tables_sum_kernel<DT><<<dim3((2 * k.span + 3) / 4, k.heads, 2), THREADS, 0, s>>>(k);
+                tables_sum_kernel<DT><<<dim3((2 * k.span + WAVES - 1) / WAVES, k.heads, 2), THREADS, 0, s>>>(k);
                 e = hipGetLastError();
             }
             return e;
@@ -982,6 +1198,6 @@ extern "C" {
 
 int tdb_attn_train_fwd(const tdb_train_attn_args* args, void* stream) { return tdb_train::run(args, false, stream); }
 int tdb_attn_train_bwd(const tdb_train_attn_args* args, void* stream) { return tdb_train::run(args, true, stream); }
-int64_t tdb_attn_train_workspace(const tdb_train_attn_args* args) { return args ? tdb_train::plan_of(*args).bytes : 0; }
+int64_t tdb_attn_train_workspace(const tdb_train_attn_args* args) { return tdb_train::check(args, false, true) == TDB_OK ? tdb_train::plan_of(*args).bytes : 0; }
 
 }  // extern "C"

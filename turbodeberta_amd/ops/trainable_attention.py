@@ -2,7 +2,7 @@
 
 What ``ops.flash_attention`` and ``ops.flash_attention_varlen`` compute forward only, with dropout on the probabilities and gradients of q, k, v and
 of both position tables.  No ``[L, L]`` array and no mask outlives a call: the forward pass keeps its inputs, its result and one number for each row; the
-backward pass holds the scores' gradients of a few heads at a time (512 MiB, or one head if that has more: element size x sum of length x longest).
+backward pass holds the scores' gradients of a few heads at a time (2 GiB, or one head if that has more: element size x sum of length x longest).
 The device work goes through ``tdb_attn_train_fwd`` and ``tdb_attn_train_bwd`` (include/tdb_train.h)."""
 from __future__ import annotations
 
@@ -33,13 +33,15 @@ def _like(t):
     return o if _apart(o) is o else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
-def _args(q, k, v, o, lse, pk, pq, lens, cu, longest, scale, buckets, max_rel, threshold, seed):
+def _args(q, k, v, o, rest, lse, pk, pq, lens, cu, longest, scale, buckets, max_rel, threshold, seed):
     a = _lib.TrainAttnArgs()
     packed = cu is not None
     a.dtype, a.heads, a.head_dim, a.max_seqlen, a.threshold, a.sm_scale = L.dtype_code(q), q.shape[1], q.shape[-1], longest, threshold, scale
     a.batch, a.total_tokens = (cu.numel() - 1, q.shape[0]) if packed else (q.shape[0], 0)
     _fill(a, q=q, k=k, v=v, o=o)
     a.lse = lse.data_ptr()
+    if rest is not None:
+        a.o_rest = rest.data_ptr()
     if packed:
         a.cu_seqlens = cu.data_ptr()
     elif lens is not None:
@@ -75,9 +77,10 @@ class _Attention(torch.autograd.Function):
             ctx.save_for_backward(q, k, v, pk, pq)
             return o.zero_()
         lse = torch.empty(q.shape[1], q.numel() // max(q.shape[1] * q.shape[-1], 1), dtype=torch.float32, device=q.device)
-        a = _args(q, k, v, o, lse, pk, pq, lens, cu, *plain, seed)
+        rest = None if q.dtype == torch.float32 else torch.empty(*lse.shape, q.shape[-1], dtype=q.dtype, device=q.device)
+        a = _args(q, k, v, o, rest, lse, pk, pq, lens, cu, *plain, seed)
         L.call(_lib.load().tdb_attn_train_fwd, q.device, C.byref(a))
-        ctx.save_for_backward(q, k, v, o, lse, pk, pq, lens, cu, seed)
+        ctx.save_for_backward(q, k, v, o, rest, lse, pk, pq, lens, cu, seed)
         return o
 
     @staticmethod
@@ -85,10 +88,10 @@ class _Attention(torch.autograd.Function):
     def backward(ctx, dout):
         if ctx.nothing:
             return tuple(None if t is None else torch.zeros_like(t) for t in ctx.saved_tensors) + (None,) * (3 + len(ctx.plain))
-        q, k, v, o, lse, pk, pq, lens, cu, seed = ctx.saved_tensors
+        q, k, v, o, rest, lse, pk, pq, lens, cu, seed = ctx.saved_tensors
         dout = _apart(dout)
         dq, dk, dv = _like(q), _like(k), _like(v)
-        a = _args(q, k, v, o, lse, pk, pq, lens, cu, *ctx.plain, seed)
+        a = _args(q, k, v, o, rest, lse, pk, pq, lens, cu, *ctx.plain, seed)
         _fill(a, dout=dout, dq=dq, dk=dk, dv=dv)
         tables = []
         for name, t in (("dpos_key", pk), ("dpos_query", pq)):
