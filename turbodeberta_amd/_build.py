@@ -51,7 +51,7 @@ def _compile_host() -> str:
            "-D__HIP_PLATFORM_AMD__=1", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            *(f for d in include_paths() + [sysconfig.get_paths()["include"]] for f in ("-isystem", d)),
            "-isystem", os.path.join(rocm, "include"), "-I", os.path.join(ROOT, "include"), "-I", CSRC,
-           *(os.path.join(CSRC, f) for f in ("host.cpp", "host_encoder.cpp")), "-o", tmp, "-L", os.path.join(os.path.dirname(torch.__file__), "lib"),
+           *(os.path.join(CSRC, f) for f in ("host.cpp", "host_encoder.cpp", "host_train.cpp")), "-o", tmp, "-L", os.path.join(os.path.dirname(torch.__file__), "lib"),
            "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:

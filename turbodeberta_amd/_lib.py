@@ -162,6 +162,8 @@ def host():
         address = lambda n: C.cast(getattr(lib, n), C.c_void_p).value
         module.bind_encoder(*(address("tdb_enc_" + n) for n in ("scan_mask", "embed", "add_norm", "small_gemm", "small_tiles", "small_splits", "unpack", "gemm", "gemm_splits",
                                                                                 "rows_fused", "embed_rows", "norm_gemm", "gemm_add", "norm_rows")))
+        module.bind_train(*(address(n) for n in ("tdb_dropout", "tdb_norm_fwd", "tdb_norm_bwd", "tdb_norm_workspace", "tdb_attn_train_fwd", "tdb_attn_train_bwd",
+                                                 "tdb_attn_train_workspace", "tdb_last_error")))
         module.bind(address("tdb_attn_fwd_fixed"), address("tdb_attn_fwd_varlen"))
         _host = module
     return _host

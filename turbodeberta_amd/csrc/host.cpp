@@ -122,20 +122,24 @@ bool inputs_ok(const Common& c, int dims) {
     return true;
 }
 
+const Lut* find_lut(int64_t buckets, int64_t max_rel, int64_t max_len, int device) {
+    int64_t size = 512;
+    while (size < max_len) size *= 2;
+    for (const Lut& l : luts())
+        if (l.device == device && l.size == size && l.buckets == buckets && l.max_rel == max_rel) return &l;
+    return nullptr;
+}
+
 // span and delta table of sequences up to max_len; false where no such table has been handed over
 bool fill_delta(tdb_pos_args& pos, int64_t buckets, int64_t max_rel, int64_t max_len, int device) {
     const int64_t span = buckets > 0 ? buckets : max_rel;
     if (span < 1) return false;
-    int64_t size = 512;
-    while (size < max_len) size *= 2;
-    for (const Lut& l : luts())
-        if (l.device == device && l.size == size && l.buckets == buckets && l.max_rel == max_rel) {
-            pos.span = int32_t(span);
-            pos.lut_half = int32_t(size - 1);
-            pos.delta_lut = static_cast<const int32_t*>(l.table.data_ptr());
-            return true;
-        }
-    return false;
+    const Lut* l = find_lut(buckets, max_rel, max_len, device);
+    if (!l) return false;
+    pos.span = int32_t(span);
+    pos.lut_half = int32_t(l->size - 1);
+    pos.delta_lut = static_cast<const int32_t*>(l->table.data_ptr());
+    return true;
 }
 
 bool fill_pos(tdb_pos_args& pos, const Common& c, int64_t heads, int64_t head_dim, int64_t max_len) {
@@ -328,6 +332,15 @@ bool tdb_host_plain(const at::Tensor& t, const at::Tensor& q, bool grad) {
     return t.device() == q.device() && t.layout() == at::kStrided && !(grad && t.requires_grad()) && !t.is_neg() && !t.is_conj();
 }
 
+bool tdb_host_rows_ok(const at::Tensor& t) { return rows_ok(t); }
+
+bool tdb_host_output_like(const at::Tensor& q, at::Tensor& o) { return output_like(q, o); }
+
+const at::Tensor* tdb_host_lut(int64_t buckets, int64_t max_rel, int64_t max_len, int device) {
+    const Lut* l = find_lut(buckets, max_rel, max_len, device);
+    return l ? &l->table : nullptr;
+}
+
 bool tdb_host_observed() { return c10::impl::dispatch_mode_enabled() || at::tracer::impl::is_dispatch_enabled(); }
 
 bool tdb_host_fill_tables(tdb_pos_args& pos, const at::Tensor* pk, const at::Tensor* pq, int64_t buckets, int64_t max_rel, int64_t max_len, int device) {
@@ -340,7 +353,7 @@ bool tdb_host_fill_tables(tdb_pos_args& pos, const at::Tensor* pk, const at::Ten
 
 PyMODINIT_FUNC PyInit__host(void) {
     PyObject* m = PyModule_Create(&kModule);
-    if (m && !tdb_host_add_encoder(m)) {
+    if (m && !(tdb_host_add_encoder(m) && tdb_host_add_train(m))) {
         Py_DECREF(m);
         return nullptr;
     }

@@ -1,4 +1,4 @@
-// What the two files of the native host module share.
+// What the files of the native host module share.
 #pragma once
 #include <Python.h>
 
@@ -22,4 +22,14 @@ bool tdb_host_observed();
 // around it.
 bool tdb_host_plain(const at::Tensor& t, const at::Tensor& q, bool grad);
 
+// Rows the kernels can address: last dim contiguous, base and every outer stride 16-byte aligned.
+bool tdb_host_rows_ok(const at::Tensor& t);
+
+// A tensor like q: q's strides where q is dense, the dense strides of the same dimension order otherwise; false where its rows are none of those.
+bool tdb_host_output_like(const at::Tensor& q, at::Tensor& o);
+
+// The device's delta table of sequences up to max_len, null where none is at hand.
+const at::Tensor* tdb_host_lut(int64_t buckets, int64_t max_rel, int64_t max_len, int device);
+
 bool tdb_host_add_encoder(PyObject* module);
+bool tdb_host_add_train(PyObject* module);

@@ -39,6 +39,9 @@ def dropout(x: torch.Tensor, p: float, seed: torch.Tensor) -> torch.Tensor:
         backward pass (autograd raises).  Draw a new one for every call, e.g. with ``new_seed``.
 
     A dropped value is 0 whatever it was, infinities and NaN included.  Differentiable once."""
+    y = _lib.host().train_dropout(x, p, seed)
+    if y is not None:
+        return y
     threshold = L.drop_threshold(p)
     L.require_gpu(x, L.one_seed(seed))
     L.dtype_code(x)

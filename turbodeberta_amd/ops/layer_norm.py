@@ -89,7 +89,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     weight, bias : ``[hidden]``, both or neither, in x's dtype or float32.
 
     Statistics, sums and the gradient of weight and bias are held in float32; the latter is added up in a fixed order.  Differentiable once."""
-    return _norm(x, None, weight, bias, 0, None, eps)
+    y = _lib.host().train_norm(x, None, weight, bias, 0, None, eps)
+    return _norm(x, None, weight, bias, 0, None, eps) if y is None else y
 
 
 def dropout_add_layer_norm(x: torch.Tensor, residual: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
@@ -97,7 +98,10 @@ def dropout_add_layer_norm(x: torch.Tensor, residual: torch.Tensor, weight: Opti
     """``layer_norm(dropout(x, p, seed) + residual, weight, bias, eps)`` in one pass over x and residual, which the backward pass reads again
     instead of what lies between (modeling_deberta_v2.py:42-53, :400-411).  x and residual have one shape and dtype; the
     rest as in ``layer_norm`` and ``ops.dropout.dropout``, whose mask for x this is."""
-    threshold = L.drop_threshold(p)
     if residual is None:
         raise ValueError("residual is required: layer_norm takes rows without one")
+    y = _lib.host().train_norm(x, residual, weight, bias, p, seed, eps)
+    if y is not None:
+        return y
+    threshold = L.drop_threshold(p)
     return _norm(x, residual, weight, bias, threshold, L.one_seed(seed) if threshold else None, eps)

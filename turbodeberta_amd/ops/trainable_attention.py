@@ -155,6 +155,9 @@ def trainable_attention_with_disentangled(q, k, v, pos_key_layer: Optional[torch
         packed batch of the same sequences drop the same.
 
     Scores, sums and the gradients' sums are held in float32; probabilities and the scores' gradients are rounded to the type where they enter a product."""
+    o = _lib.host().train_attention(q, k, v, pos_key_layer, pos_query_layer, sm_scale, position_buckets, max_relative_distance, seqlens_k, None, 0, dropout_p, seed)
+    if o is not None:
+        return o
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
         raise ValueError("q, k, v must be [B, H, L, D]")
     scale, (pk, pq), threshold, seed = _checked(q, k, v, pos_key_layer, pos_query_layer, q.shape[1], sm_scale, position_buckets, max_relative_distance,
@@ -173,6 +176,9 @@ def trainable_attention_with_disentangled_varlen(q, k, v, pos_key_layer: Optiona
     """``trainable_attention_with_disentangled`` of packed sequences: q, k, v ``[total_tokens, H, D]``, cu_seqlens int32 ``[B+1]`` running sums of the lengths with a
     leading 0, max_seqlen the longest (an upper bound is fine; what it cuts off, and tokens of no sequence, are zeros in the result and in the
     gradients).  No host synchronisation."""
+    o = _lib.host().train_attention(q, k, v, pos_key_layer, pos_query_layer, sm_scale, position_buckets, max_relative_distance, None, cu_seqlens, max_seqlen, dropout_p, seed)
+    if o is not None:
+        return o
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
         raise ValueError("q, k, v must be [total_tokens, H, D]")
     if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
