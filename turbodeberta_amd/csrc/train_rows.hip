@@ -128,34 +128,46 @@ struct Norm {
 template <int CH>
 using Row = float[CH][8];
 
-// z of row t
-template <int DT, int CH, bool RES>
-__device__ __forceinline__ void load_z(const Norm& p, int64_t t, TdbKey key, Row<CH>& z, uint32_t (&kept)[CH]) {
-    const int l = threadIdx.x & 63, chunks = p.hidden / 8;
-    float r[CH][8];
+// A row as it lies in memory, on its way: x, the residual, dy.
+template <int DT, int CH, bool RES, bool DY>
+struct Raw {
+    using T = typename Elem<DT>::T;
+    typedef __attribute__((ext_vector_type(8))) T T8;
+    T8 x[CH], r[RES ? CH : 1], dy[DY ? CH : 1];
+    __device__ __forceinline__ void load(const Norm& p, int64_t t) {
+        const int l = threadIdx.x & 63, chunks = p.hidden / 8;
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-        const int at = l + 64 * c;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) z[c][i] = r[c][i] = 0.f;
-        if (at < chunks) {
-            load8<DT>(p.x, t * p.xs + 8 * at, z[c]);
-            if constexpr (RES) load8<DT>(p.residual, t * p.rs + 8 * at, r[c]);
+        for (int c = 0; c < CH; ++c) {
+            const int at = 8 * min(l + 64 * c, chunks - 1);         // (past the row: read, not used)
+            x[c] = *reinterpret_cast<const T8*>(static_cast<const T*>(p.x) + t * p.xs + at);
+            if constexpr (RES) r[c] = *reinterpret_cast<const T8*>(static_cast<const T*>(p.residual) + t * p.rs + at);
+            if constexpr (DY) dy[c] = *reinterpret_cast<const T8*>(static_cast<const T*>(p.dy) + t * p.dys + at);
         }
     }
+    // z of row t, zeros past the row
+    __device__ __forceinline__ void z_of(const Norm& p, int64_t t, TdbKey key, Row<CH>& z, uint32_t (&kept)[CH]) const {
+        const int l = threadIdx.x & 63, chunks = p.hidden / 8;
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-        kept[c] = 0xff;
-        if (p.threshold) {
-            kept[c] = kept8(uint64_t(t) * chunks + l + 64 * c, p.threshold, key);
-            drop8(z[c], kept[c], p.factor);
-        }
-        if constexpr (RES) {
+        for (int c = 0; c < CH; ++c) {
+            kept[c] = 0xff;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) z[c][i] += r[c][i];
+            for (int i = 0; i < 8; ++i) z[c][i] = float(x[c][i]);
+            if (p.threshold) {
+                kept[c] = kept8(uint64_t(t) * chunks + l + 64 * c, p.threshold, key);
+                drop8(z[c], kept[c], p.factor);
+            }
+            if constexpr (RES) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) z[c][i] += float(r[c][i]);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) z[c][i] = l + 64 * c < chunks ? z[c][i] : 0.f;
         }
     }
-}
+};
+// Whether a wave has registers for the next row while it works on one.
+template <int DT, int CH>
+constexpr bool AHEAD = CH <= 2;
 
 // z -> z - mean, zeros past the row; returns 1 / standard deviation
 template <int CH>
@@ -190,8 +202,13 @@ __global__ __launch_bounds__(256) void norm_fwd_kernel(Norm p) {
         for (int i = 0; i < 8; ++i) w[c][i] = 1.f, b[c][i] = 0.f;
         if (p.weight) load_weight8<DT>(p.weight, p.wide, at, w[c]), load_weight8<DT>(p.bias, p.wide, at, b[c]);
     }
-    for (int64_t t = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6); t < p.rows; t += int64_t(gridDim.x) * 4) {
-        load_z<DT, CH, RES>(p, t, key, z, kept);
+    Raw<DT, CH, RES, false> row;
+    int64_t t = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    const int64_t step = int64_t(gridDim.x) * 4;
+    if (t < p.rows) row.load(p, t);
+    for (; t < p.rows; t += step) {
+        row.z_of(p, t, key, z, kept);
+        if (t + step < p.rows) row.load(p, t + step);
         const float rstd = centre<CH>(z, p.hidden, p.eps);
 #pragma unroll
         for (int c = 0; c < CH; ++c)
@@ -219,16 +236,20 @@ __global__ __launch_bounds__(64 * BWD_WAVES) void norm_bwd_kernel(Norm p) {
         for (int i = 0; i < 8; ++i) w[c][i] = 1.f, dw[c][i] = db[c][i] = 0.f;
         if (p.weight) load_weight8<DT>(p.weight, p.wide, 8 * min(l + 64 * c, chunks - 1), w[c]);
     }
-    for (int64_t t = int64_t(blockIdx.x) * BWD_WAVES + wave; t < p.rows; t += int64_t(gridDim.x) * BWD_WAVES) {
+    Raw<DT, CH, RES, true> row;
+    int64_t t = int64_t(blockIdx.x) * BWD_WAVES + wave;
+    const int64_t step = int64_t(gridDim.x) * BWD_WAVES;
+    if (AHEAD<DT, CH> && t < p.rows) row.load(p, t);
+    for (; t < p.rows; t += step) {
         float z[CH][8], g[CH][8];
         uint32_t kept[CH];
+        if (!AHEAD<DT, CH>) row.load(p, t);
 #pragma unroll
-        for (int c = 0; c < CH; ++c) {
+        for (int c = 0; c < CH; ++c)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) g[c][i] = 0.f;
-            if (l + 64 * c < chunks) load8<DT>(p.dy, t * p.dys + 8 * (l + 64 * c), g[c]);
-        }
-        load_z<DT, CH, RES>(p, t, key, z, kept);
+            for (int i = 0; i < 8; ++i) g[c][i] = l + 64 * c < chunks ? float(row.dy[c][i]) : 0.f;
+        row.z_of(p, t, key, z, kept);
+        if (AHEAD<DT, CH> && t + step < p.rows) row.load(p, t + step);
         const float rstd = centre<CH>(z, p.hidden, p.eps);
         float sum = 0.f, dot = 0.f;
 #pragma unroll
@@ -360,27 +381,34 @@ __global__ __launch_bounds__(256) void norm_bwd_any_kernel(Norm p) {
     }
 }
 
-// dweight, dbias: column sums of the workgroups' parts.  A workgroup has 64 columns, its waves share out the parts.
+// dweight, dbias: column sums of the workgroups' parts.  A workgroup has 16 columns; its 32 groups of 16 lanes share out the parts and ask for eight at a time.
 template <int DT>
 __global__ __launch_bounds__(512) void norm_sum_kernel(const float* partial, int parts, int hidden, void* dweight, void* dbias) {
-    __shared__ float s_sum[8][64];
-    const int wave = threadIdx.x >> 6, l = threadIdx.x & 63, c = blockIdx.x * 64 + l;
+    __shared__ float s_sum[32][17];
+    const int group = threadIdx.x >> 4, l = threadIdx.x & 15, c = blockIdx.x * 16 + l;
     const float* at = partial + int64_t(blockIdx.y) * hidden + min(c, hidden - 1);
     float sum = 0.f;
-    for (int g = wave; g < parts; g += 8) sum += at[int64_t(g) * 2 * hidden];
-    s_sum[wave][l] = sum;
-    __syncthreads();
-    if (wave == 0 && c < hidden) {
+    for (int g = group; g < parts; g += 32 * 8) {
+        float x[8];
 #pragma unroll
-        for (int v = 1; v < 8; ++v) sum += s_sum[v][l];
+        for (int u = 0; u < 8; ++u) x[u] = at[int64_t(min(g + 32 * u, parts - 1)) * 2 * hidden];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) sum += g + 32 * u < parts ? x[u] : 0.f;
+    }
+    s_sum[group][l] = sum;
+    __syncthreads();
+    if (threadIdx.x < 16 && c < hidden) {
+#pragma unroll
+        for (int v = 1; v < 32; ++v) sum += s_sum[v][l];
         store1<DT>(blockIdx.y ? dbias : dweight, c, sum);
     }
 }
 
-constexpr int MAX_PARTS = 512, MAX_GRID = 1 << 20;
-
-// Workgroups of a backward launch whose workgroups take `at_once` rows each.
-int parts_of(int64_t rows, int at_once) { return int(std::min<int64_t>(MAX_PARTS, std::max<int64_t>(1, (rows + at_once - 1) / at_once))); }
+// Workgroups of a launch, at most.  Waves with a row each walk on and ask for the next row ahead: forward 4 workgroups of 4 waves to a CU (16384 x 768 with residual: 17.7 us, with a
+// wave for each row 19.5), backward one of 8 waves (31 us; two 37, four 48: each ends by adding up its waves).  Workgroups with a row each, backward: two to a CU
+// (1013 x 771: 13 us, one 19).
+constexpr int MAX_GRID = 1 << 20, FWD_GRID = 1024, BWD_PARTS = 256, BWD_ANY_PARTS = 512;
+int parts_of(int64_t rows, int at_once) { return int(std::min<int64_t>(at_once > 1 ? BWD_PARTS : BWD_ANY_PARTS, std::max<int64_t>(1, (rows + at_once - 1) / at_once))); }
 
 bool aligned(const void* p, int64_t stride, int size) { return !p || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * size % 16 == 0); }
 
@@ -411,7 +439,7 @@ int check_norm(const tdb_norm_args* a, bool backward) {
 template <int DT, int CH, bool RES>
 void launch_rows(const Norm& n, int parts, hipStream_t s) {
     if (parts) norm_bwd_kernel<DT, CH, RES><<<parts, 64 * BWD_WAVES, 0, s>>>(n);
-    else norm_fwd_kernel<DT, CH, RES><<<unsigned(std::min<int64_t>((n.rows + 3) / 4, MAX_GRID)), 256, 0, s>>>(n);
+    else norm_fwd_kernel<DT, CH, RES><<<unsigned(std::min<int64_t>((n.rows + 3) / 4, FWD_GRID)), 256, 0, s>>>(n);
 }
 
 template <int DT>
@@ -452,7 +480,7 @@ hipError_t launch_norm(const tdb_norm_args& a, bool backward, hipStream_t s) {
         norm_fwd_any_kernel<DT><<<unsigned(std::min<int64_t>(a.rows, MAX_GRID)), 256, lds, s>>>(n);
     }
     if (n.partial) {
-        const dim3 grid((a.hidden + 63) / 64, 2);
+        const dim3 grid((a.hidden + 15) / 16, 2);
         if (n.wide) norm_sum_kernel<TDB_F32><<<grid, 512, 0, s>>>(n.partial, parts, a.hidden, a.dweight, a.dbias);
         else norm_sum_kernel<DT><<<grid, 512, 0, s>>>(n.partial, parts, a.hidden, a.dweight, a.dbias);
     }
