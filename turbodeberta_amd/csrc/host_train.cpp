@@ -9,6 +9,7 @@
 #include <c10/core/GradMode.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -310,16 +311,15 @@ Tensor as_seed(PyObject* o, int64_t threshold, const Tensor& x, bool& ok) {
 template <class F>
 PyObject* native(F call) {
     if (!g.dropout || tdb_host_observed()) Py_RETURN_NONE;
+    HANDLE_TH_ERRORS                    // (what hooks of saved tensors raise passes through as it is)
     try {
         Tensor out = call();
         if (!out.defined()) Py_RETURN_NONE;
         return THPVariable_Wrap(std::move(out));
     } catch (const Refused&) {
         Py_RETURN_NONE;
-    } catch (const std::exception& e) {
-        PyErr_SetString(PyExc_RuntimeError, e.what());
-        return nullptr;
     }
+    END_HANDLE_TH_ERRORS
 }
 
 // train_dropout(x, p, seed)

@@ -59,7 +59,10 @@ from . import _lib
 from .ops._launch import delta_lut
 from .ops.flash_attention import flash_attention_with_disentangled
 from .ops.flash_attention_varlen import flash_attention_with_disentangled_varlen
+from .ops.trainable_attention import trainable_attention_with_disentangled
 from .padding import index_first_axis, key_padding_mask, pad_input
+from . import training as _training
+from .training import FlashDebertaV2Output, FlashDebertaV2SelfOutput, FlashDropout, FlashLayerNorm
 
 
 def _versions(*tensors):
@@ -198,7 +201,11 @@ class FlashDisentangledSelfAttention(DisentangledSelfAttention):
     are returned as zeros (the eager module gives them a meaningless uniform average,
     modeling_deberta_v2.py:256-259); downstream layers mask them anyway.
     ``output_attentions=True`` needs the probability matrix, which the fused kernel never forms: that
-    call is served by the eager parent class."""
+    call is served by the eager parent class.
+    ``trainable = True`` (``patch_model(model, training=True)``): a call that autograd records goes to ``ops.trainable_attention``, which has the
+    gradient and, in training mode, the dropout of the probabilities (modeling_deberta_v2.py:262); without it such a call has no gradient and drops nothing."""
+
+    trainable = False
 
     def forward(self, hidden_states, attention_mask, output_attentions=False, query_states=None,
                 relative_pos=None, rel_embeddings=None):
@@ -227,9 +234,14 @@ class FlashDisentangledSelfAttention(DisentangledSelfAttention):
         pos_key, pos_query, sm_scale, buckets, max_rel = self._position_terms(rel_embeddings, hidden_states.dtype,
                                                                               frozen)
         seqlens = _mask_info(attention_mask).lengths if attention_mask is not None else None
-        out = flash_attention_with_disentangled(q, k, v, None, None, False, sm_scale, buckets, max_rel,
-                                                pos_key_layer=pos_key, pos_query_layer=pos_query,
-                                                seqlens_k=seqlens)
+        if self.trainable and _training.recorded(q, k, v):
+            p = _training.rate_of(self, self.dropout)
+            out = trainable_attention_with_disentangled(q, k, v, pos_key, pos_query, sm_scale, buckets, max_rel, seqlens_k=seqlens, dropout_p=p,
+                                                        seed=_training.draw_seed(self, q.device) if p else None)
+        else:
+            out = flash_attention_with_disentangled(q, k, v, None, None, False, sm_scale, buckets, max_rel,
+                                                    pos_key_layer=pos_key, pos_query_layer=pos_query,
+                                                    seqlens_k=seqlens)
         # out has q's strides: [B, H, L, D] view of token-major storage
         return (out.permute(0, 2, 1, 3).reshape(B, L, H * D), None)
 
@@ -462,9 +474,9 @@ def _known_structure(model):
     attention, exact GELU, no convolution, embeddings that are a table and a LayerNorm, and in the places of the dropouts
     dropouts, which the loop leaves out."""
     emb, enc = model.embeddings, model.encoder
-    dropout = lambda m: type(m._modules.get("dropout")) is nn.Dropout
+    dropout = lambda m: type(m._modules.get("dropout")) in (nn.Dropout, FlashDropout)
     plain = lambda m, *names: all(type(getattr(m, n)) is nn.Linear and getattr(m, n).bias is not None for n in names)
-    norm = lambda m: type(m) is nn.LayerNorm and m.weight is not None and m.bias is not None
+    norm = lambda m: type(m) in (nn.LayerNorm, FlashLayerNorm) and m.weight is not None and m.bias is not None
     if not (type(emb) is DebertaV2Embeddings and type(emb.word_embeddings) is nn.Embedding and emb.word_embeddings.max_norm is None
             and not emb.position_biased_input and emb.token_type_embeddings is None and emb.embed_proj is None and norm(emb.LayerNorm) and dropout(emb)
             and type(enc) is FlashDebertaV2Encoder and enc.conv is None and len(enc.layer) > 0):
@@ -478,10 +490,10 @@ def _known_structure(model):
             return False
         att, so, mid, out = layer.attention.self, layer.attention.output, layer.intermediate, layer.output
         first = first or (att, mid)
-        if not (type(att) is FlashDisentangledSelfAttention and type(so) is DebertaV2SelfOutput and type(mid) is DebertaV2Intermediate
-                and type(out) is DebertaV2Output and type(mid.intermediate_act_fn) is GELUActivation
+        if not (type(att) is FlashDisentangledSelfAttention and type(so) in (DebertaV2SelfOutput, FlashDebertaV2SelfOutput) and type(mid) is DebertaV2Intermediate
+                and type(out) in (DebertaV2Output, FlashDebertaV2Output) and type(mid.intermediate_act_fn) is GELUActivation
                 and mid.intermediate_act_fn.act is nn.functional.gelu
-                and dropout(att) and dropout(so) and dropout(out) and type(att._modules.get("pos_dropout")) in (nn.Dropout, type(None))):
+                and dropout(att) and dropout(so) and dropout(out) and type(att._modules.get("pos_dropout")) in (nn.Dropout, FlashDropout, type(None))):
             return False
         if not (plain(att, "query_proj", "key_proj", "value_proj") and plain(so, "dense") and plain(out, "dense") and plain(mid, "dense")
                 and norm(so.LayerNorm) and norm(out.LayerNorm) and att.num_attention_heads * att.attention_head_size == hidden == out.dense.out_features
@@ -495,7 +507,7 @@ def _known_structure(model):
 # its class the modules are run.  (What happens to them later, or on an instance, the snapshot of a plan sees.)
 _LOOP_TYPES = (nn.Linear, nn.LayerNorm, nn.Embedding, nn.Dropout, GELUActivation, DebertaV2Embeddings, DebertaV2Attention, DebertaV2SelfOutput,
                DebertaV2Intermediate, DebertaV2Output, DebertaV2Layer, FlashDebertaV2Attention, FlashDebertaV2Layer,
-               FlashDisentangledSelfAttention, FlashDebertaV2Encoder)
+               FlashDisentangledSelfAttention, FlashDebertaV2Encoder, FlashDropout, FlashLayerNorm, FlashDebertaV2SelfOutput, FlashDebertaV2Output)
 
 
 def _own(cls, name):
@@ -629,12 +641,33 @@ class FlashDebertaV2ForMultipleChoice(_FusedHead, DebertaV2ForMultipleChoice):
     pass
 
 
-def patch_model(model: nn.Module) -> nn.Module:
+def patch_model(model: nn.Module, training: bool = False) -> nn.Module:
     """Switch every ``DisentangledSelfAttention`` inside ``model`` (any DeBERTa-v2/v3 model or task head,
-    e.g. one loaded with ``from_pretrained``) to the fused kernel, in place.  Parameters are untouched."""
+    e.g. one loaded with ``from_pretrained``) to the fused kernel, in place.  Parameters are untouched.
+
+    ``training=True``: the model can be trained as well.  Attention, LayerNorms and dropouts of the DeBERTa modules run the training operators
+    (``turbodeberta_amd.training``) wherever autograd records; evaluation under ``torch.no_grad`` is not changed by it.  Head dimensions: multiples of 8
+    up to 64; no ``pos_att_type`` where ``relative_attention`` is off.  Masks come from PyTorch's generator but are not those that ``nn.Dropout`` would draw."""
     swaps = {DisentangledSelfAttention: FlashDisentangledSelfAttention, DebertaV2Encoder: FlashDebertaV2Encoder,
              DebertaV2Model: FlashDebertaV2Model}        # none of them adds parameters or constructor state
+    if training:
+        for module in model.modules():
+            if not isinstance(module, DisentangledSelfAttention):
+                continue
+            if module.attention_head_size % 8 or not 8 <= module.attention_head_size <= 64:
+                raise ValueError(f"head dimension {module.attention_head_size}: training needs a multiple of 8 up to 64")
+            if module.pos_att_type and not module.relative_attention:        # Hugging Face counts them in the scale all the same (modeling_deberta_v2.py:237-243)
+                raise ValueError("pos_att_type names position terms and relative_attention is off: training needs one without the other")
+    inner = set()                       # of the DeBERTa modules: a task head's own dropout and norm stay as they are
     for module in model.modules():
         if type(module) in swaps:
             module.__class__ = swaps[type(module)]
+        if training and isinstance(module, (DebertaV2Embeddings, DebertaV2Encoder)):
+            inner.update(module.modules())
+    blocks = {DebertaV2SelfOutput: FlashDebertaV2SelfOutput, DebertaV2Output: FlashDebertaV2Output, nn.Dropout: FlashDropout, nn.LayerNorm: FlashLayerNorm}
+    for module in inner:
+        if type(module) in blocks:
+            module.__class__ = blocks[type(module)]
+        if isinstance(module, FlashDisentangledSelfAttention):
+            module.trainable = True
     return model

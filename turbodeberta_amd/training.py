@@ -1,0 +1,85 @@
+"""Modules of a DeBERTa-v2/v3 model that is trained with this package's operators.
+
+``patch_model(model, training=True)`` (``turbodeberta_amd.model``) switches a model's dropouts, LayerNorms and output blocks to the classes below and
+its attention to ``ops.trainable_attention``.  They add no parameters and no state.  Where autograd records (``torch.enable_grad``, tensors on the GPU
+in float32, bfloat16 or float16) they call the operators, which store no masks, no probabilities and nothing between dropout, residual and
+LayerNorm; everything else -- evaluation, ``torch.no_grad``, the CPU -- runs the parent class's code."""
+from __future__ import annotations
+
+import torch
+from torch import nn
+from transformers.models.deberta_v2.modeling_deberta_v2 import DebertaV2Output, DebertaV2SelfOutput
+
+from .ops.dropout import dropout, new_seed
+from .ops.layer_norm import dropout_add_layer_norm, layer_norm
+
+_TYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def recorded(*tensors) -> bool:
+    """Whether a call of these tensors is one for the training operators."""
+    return torch.is_grad_enabled() and all(t.is_cuda and t.dtype in _TYPES for t in tensors)
+
+
+def draw_seed(module: nn.Module, device) -> torch.Tensor:
+    """The seed of a module's next dropout, from PyTorch's generator of the device: ``torch.manual_seed`` decides, and gradient checkpointing, which
+    puts the generator's state back, finds the same masks."""
+    return new_seed(device)
+
+
+def rate_of(module: nn.Module, drop: nn.Module) -> float:
+    """The probability that ``drop``, a dropout of ``module``, drops a value with in the next call."""
+    return float(drop.p) if drop.training else 0.0
+
+
+class FlashDropout(nn.Dropout):
+    """``nn.Dropout`` by ``ops.dropout.dropout``."""
+
+    def forward(self, x):
+        if not (self.training and self.p > 0 and not self.inplace and recorded(x)):
+            return super().forward(x)
+        return dropout(x, self.p, draw_seed(self, x.device))
+
+
+def _norm_arguments(norm: nn.LayerNorm, x):
+    """``(x, weight, bias)`` of a call of the norm's operators; None where they do not take it.  Autocast has LayerNorm computed in float32."""
+    if torch.is_autocast_enabled("cuda"):
+        x = x.float()
+    w, b = norm.weight, norm.bias
+    if len(norm.normalized_shape) != 1 or (w is None) != (b is None) or x.shape[-1] > 32768:
+        return None
+    if w is not None and (w.dtype != b.dtype or w.dtype not in (x.dtype, torch.float32)):
+        return None
+    return x, w, b
+
+
+class FlashLayerNorm(nn.LayerNorm):
+    """``nn.LayerNorm`` by ``ops.layer_norm.layer_norm``."""
+
+    def forward(self, x):
+        a = _norm_arguments(self, x) if recorded(x) else None
+        return super().forward(x) if a is None else layer_norm(*a, self.eps)
+
+
+class _Output:
+    """``LayerNorm(dropout(dense(x)) + input)`` (modeling_deberta_v2.py:42-53, :400-411) by ``ops.layer_norm.dropout_add_layer_norm``."""
+
+    def forward(self, hidden_states, input_tensor):
+        if not recorded(hidden_states, input_tensor):
+            return super().forward(hidden_states, input_tensor)
+        x = self.dense(hidden_states)
+        wide = torch.promote_types(x.dtype, input_tensor.dtype)
+        a = _norm_arguments(self.LayerNorm, x.to(wide))
+        if a is None:
+            return self.LayerNorm(self.dropout(x) + input_tensor)
+        x, weight, bias = a
+        p = rate_of(self, self.dropout)
+        return dropout_add_layer_norm(x, input_tensor.to(x.dtype), weight, bias, p, draw_seed(self, x.device) if p else None, self.LayerNorm.eps)
+
+
+class FlashDebertaV2SelfOutput(_Output, DebertaV2SelfOutput):
+    pass
+
+
+class FlashDebertaV2Output(_Output, DebertaV2Output):
+    pass
