@@ -66,14 +66,15 @@ constexpr int TILE = 64;                        // rows y of a step, and of a ti
 constexpr int TILE_VALUES = TILE * TILE;
 constexpr float LOG2E = 1.44269504088896340736f;
 
-// Rows of 64 values in LDS.  float32: 16 bytes apart.  16 bits: side by side, so that two workgroups fit a CU, their 16-byte chunks permuted: 16 rows at the same chunk
-// are on distinct banks, and so are the 32 bytes that a transposing read takes of each of 8 rows.
+// Rows of 64 values in LDS.  float32: 16 bytes apart.  16 bits: side by side, so that two workgroups fit a CU, their 16-byte chunks permuted.  LDS serves a read of 16 bytes a
+// lane in 4 clocks if each time these 16 lanes are on distinct banks, in 8 if not (measured): rows 0 .. 3 and 12 .. 15 at one chunk with rows 4 .. 11 at the next.  A
+// transposing read has 32 bytes of rows 0 .. 7, or of 0 .. 3 and 8 .. 11.  This permutation serves all of them.
 template <int DT>
 constexpr int ROW = DT == TDB_F32 ? 68 : 64;
 template <int DT>
 __device__ __forceinline__ int place(int row, int col) {
     if constexpr (DT == TDB_F32) return row * ROW<DT> + col;
-    return row * ROW<DT> + (col ^ (((row & 6) | (row >> 3 & 1)) << 3));
+    return row * ROW<DT> + (col ^ (((row & 6) ^ (row & 8 ? 5 : 0)) << 3));
 }
 
 __device__ __forceinline__ int lane_c() { return threadIdx.x & 15; }
@@ -366,10 +367,12 @@ __device__ __forceinline__ float column_max(float x) {
     return fmaxf(__builtin_bit_cast(float, uint32_t(s[0])), __builtin_bit_cast(float, uint32_t(s[1])));
 }
 
-constexpr int OWN_ROW = 85;             // floats of a row of x's term, see above
-constexpr int OTHER_ROW = 36;           // and of y's term: 16 rows at the same column are on distinct banks
+// Floats of a row of x's term, of which 88 (22 chunks of 16 bytes) are next to the one before in what is read: reads of 16 bytes a lane, and writes of one value a lane, are on
+// distinct banks.  And of y's term, two blocks of 16 rows in the same place: 43 apart in what is read, four times that is 44 banks on.
+constexpr int OWN_ROW = 89, OTHER_ROW = 44;
 static_assert(2 * OTHER_ROW <= OWN_ROW, "");
-constexpr int OWN_TERM = 16 * OWN_ROW, TERMS = OWN_TERM + 16 * OTHER_ROW;      // floats of a wave's scratch for the two
+template <int DT>
+constexpr int TERMS = DT == TDB_F32 ? 1552 : 16 * OWN_ROW;      // floats of a wave's scratch for the two, in turn, and for a skewed tile
 
 // A table's rows r = 0 .. 126 of a tile of 64 x and 64 y, and one more.
 constexpr int RING = 128;
@@ -473,24 +476,21 @@ __device__ __forceinline__ void scores(f32x4 (&s)[4], const typename Elem<DT>::X
     for (int k = 0; k < 2; ++k)
 #pragma unroll
         for (int m = 0; m < 4; ++m) s[m] = E::mma(y[m][k], own[k], s[m]);
-    if constexpr (OTHER) {                      // three y blocks at once: x's term, which has been read, makes room for two
-        auto at = [&](int m) { return scratch + (m == 1 ? 0 : m == 2 ? 16 * OTHER_ROW : OWN_TERM); };
-        auto put = [&](int m) {
+    if constexpr (OTHER) {                      // two y blocks at once, where x's term was, which has been read
+        wave_fence();
 #pragma unroll
-            for (int n = 0; n < 2; ++n) *reinterpret_cast<f32x4*>(at(m) + c * OTHER_ROW + 16 * n + 4 * g) = w[m][n];
-        };
-        auto get = [&](int m) {
+        for (int two = 0; two < 4; two += 2) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[m][e] += at(m)[(4 * g + e) * OTHER_ROW + c + 15 - 4 * g - e];
-        };
-        put(0), put(1), put(2);
-        wave_fence();
-        get(0);
-        wave_fence();
-        put(3);
-        get(1), get(2);
-        wave_fence();
-        get(3);
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int n = 0; n < 2; ++n) *reinterpret_cast<f32x4*>(scratch + (16 * m + c) * OTHER_ROW + 16 * n + 4 * g) = w[two + m][n];
+            wave_fence();
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[two + m][e] += scratch[(16 * m + 4 * g + e) * OTHER_ROW + c + 15 - 4 * g - e];
+            wave_fence();
+        }
     } else {
         settle(s);
     }

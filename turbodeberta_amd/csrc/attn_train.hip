@@ -28,7 +28,7 @@ template <int DT>
 struct FwdLds {
     using T = typename Elem<DT>::T;
     alignas(16) T k[TILE * ROW<DT>], v[TILE * ROW<DT>], pk[RING * ROW<DT>], pq[RING * ROW<DT>];
-    alignas(16) float scratch[WAVES][TERMS];
+    alignas(16) float scratch[WAVES][TERMS<DT>];
 };
 
 template <int DT, bool PK, bool PQ>
@@ -292,15 +292,22 @@ __device__ __forceinline__ void level_end(const Args& a, const Tensor& table, in
     }
 }
 
-// A skewed tile: row x has the values of y at index 79 - y.  A row is 105 values apart from the next, so that index 16 + r - x of row x, r = x - y + 63, lies at
-// 104 x + 16 + r: eight neighbouring r at a multiple of 8, and 16 x on distinct banks.  r runs to 95: what lies outside of 0 <= y < 64 is not the row's.
-constexpr int SKEW = 105, SKEWED = 16 * SKEW;
+// A skewed tile: row x has the values of y at index 79 - y.  A row is 113 values apart from the next, so that index 16 + r - x of row x, r = x - y + 63, lies at
+// 112 x + 16 + r: eight neighbouring r at a multiple of 8, and 16 x on distinct banks (14 chunks of 16 bytes).  r runs to 95: what lies outside of 0 <= y < 64 is not the
+// row's.
+template <int DT>
+constexpr int SKEW = DT == TDB_F32 ? 97 : 113;
+template <int DT>
+constexpr int SKEWED = 16 * SKEW<DT>;
+// A value of LDS by itself.  (Left alone, the compiler writes neighbours together, eight bytes at odd addresses: 60 clocks for each of four.)
+template <class T>
+__device__ __forceinline__ void put(T* to, T x) { *TDB_SHARED(volatile T, to) = x; }
 
 // The eight r = 32 n + 8 g .. of the lane's row, zeros outside.
 template <int DT>
 __device__ __forceinline__ typename Elem<DT>::X8 skew_frag(const typename Elem<DT>::T* skewed, int n) {
     const int c = lane_c(), r = 32 * n + 8 * lane_g();
-    typename Elem<DT>::X8 x = read8<DT>(skewed + c * (SKEW - 1) + 16 + r);
+    typename Elem<DT>::X8 x = read8<DT>(skewed + c * (SKEW<DT> - 1) + 16 + r);
     if (n == 1) return x;               // (c <= r <= c + 63)
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -314,8 +321,8 @@ struct KvLds {
     alignas(16) T q[TILE * ROW<DT>], dout[TILE * ROW<DT>], pk[RING * ROW<DT>], pq[RING * ROW<DT>];
     alignas(16) float lse[TILE], delta[TILE];
     alignas(16) uint32_t kept[2][WAVES / 2][TILE];       // a bit for each of 32 keys
-    alignas(16) float scratch[WAVES][TERMS];             // of the scores; then the skewed gradients of scores
-    static_assert(SKEWED * sizeof(T) <= TERMS * sizeof(float), "");
+    alignas(16) float scratch[WAVES][TERMS<DT>];             // of the scores; then the skewed gradients of scores
+    static_assert(SKEWED<DT> * sizeof(T) <= TERMS<DT> * sizeof(float), "");
 };
 
 template <int DT, bool PK, bool PQ>
@@ -478,7 +485,7 @@ __global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_bwd_kv_kernel(Args a
         }
         if (PQ && !far && !is_level) {
 #pragma unroll
-            for (int n = 0; n < 16; ++n) skewed[c * SKEW + 79 - 16 * (n >> 2) - 4 * g - (n & 3)] = dsx[n >> 3][n & 7];
+            for (int n = 0; n < 16; ++n) put(skewed + c * SKEW<DT> + 79 - 16 * (n >> 2) - 4 * g - (n & 3), T(dsx[n >> 3][n & 7]));
         }
         X8 q[2][4];
 #pragma unroll
@@ -555,7 +562,7 @@ struct Scores {
 template <int DT>
 struct QLds {
     using T = typename Elem<DT>::T;
-    alignas(16) T k[TILE * ROW<DT>], pk[RING * ROW<DT>], ds[TILE * ROW<DT>], skewed[4][SKEWED];
+    alignas(16) T k[TILE * ROW<DT>], pk[RING * ROW<DT>], ds[TILE * ROW<DT>], skewed[4][SKEWED<DT>];
 };
 
 // dq: a workgroup has 64 queries, a wave 16.
@@ -631,9 +638,9 @@ __global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_bwd_q_kernel(Args a)
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
                 const int q = Scores<DT>::query(0);
-                T* const to = sm.skewed[q >> 4] + (q & 15) * SKEW + 79 - Scores<DT>::key(n);
+                T* const to = sm.skewed[q >> 4] + (q & 15) * SKEW<DT> + 79 - Scores<DT>::key(n);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) to[(e >> 2) * SKEWED + (e & 3) * SKEW] = next.ds.x[n][e];
+                for (int e = 0; e < 8; ++e) to[(e >> 2) * SKEWED<DT> + (e & 3) * SKEW<DT>] = next.ds.x[n][e];
             }
         }
         __syncthreads();
