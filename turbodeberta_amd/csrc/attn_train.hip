@@ -108,7 +108,7 @@ __global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_fwd_kernel(Args a) {
         sum *= again;
 #pragma unroll
         for (int d = 0; d < 4; ++d) o[d] *= again;
-        X8 p[2];
+        X8 p[2], rest[2];                   // 16 bits: a probability is the sum of two values, as D (see store_rest) takes the result for exact
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             float z[8];
@@ -123,12 +123,18 @@ __global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_fwd_kernel(Args a) {
                 for (int n = 0; n < 8; ++n) z[n] = tdb_number(r, n) >= a.threshold ? z[n] : 0.f;
             }
 #pragma unroll
-            for (int n = 0; n < 8; ++n) p[u][n] = T(z[n]);
+            for (int n = 0; n < 8; ++n) {
+                p[u][n] = T(z[n]);
+                if constexpr (DT != TDB_F32) rest[u][n] = T(z[n] - float(p[u][n]));
+            }
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int d = 0; d < 4; ++d) o[d] = E::mma(v[u][d], p[u], o[d]);
+            for (int d = 0; d < 4; ++d) {
+                o[d] = E::mma(v[u][d], p[u], o[d]);
+                if constexpr (DT != TDB_F32) o[d] = E::mma(v[u][d], rest[u], o[d]);
+            }
     }
     const float all = column_sum(sum);
     const float whole = all > 0.f ? a.factor / all : all == 0.f ? 0.f : all;                       // (NaN stays)
