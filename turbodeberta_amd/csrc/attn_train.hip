@@ -5,6 +5,9 @@
 //   dq_i = scale sum_j dS_ij (k_j + K_r[d(i-j)]),  dk_j = scale sum_i dS_ij (q_i + Q_r[d(i-j)])
 //   dK_r[x] = scale sum_{d(i-j) = x} dS_ij q_i,  dQ_r[x] = scale sum_{d(i-j) = x} dS_ij k_j
 //
+// Roundings to the type, each where a matrix instruction of it takes its operand: P' (in 16 bits as the sum of two values in the forward pass), dS, and what is stored.  A
+// gradient's error is that of dS's rounding and its own, 1.4 times its own (bfloat16 2.3e-3 of its norm, 1.7e-3 for its own alone); sums are float32.  float16: P' and dS are
+// scaled by powers of two to the top of its range.
 // Backward in four launches for a number of heads at a time.  The costly part, scores, exponentials, random numbers, is done once: attn_bwd_kv_kernel owns keys, sums up
 // their gradients and writes dS, rounded to the type, tile by tile to a workspace; attn_bwd_q_kernel owns queries and reads dS; attn_bwd_tables_kernel owns relative
 // positions (a diagonal of tiles) and reads dS; tables_sum_kernel adds its parts up by table row.  No atomics: every sum has one owner and one order.
@@ -31,6 +34,12 @@ struct FwdLds {
     alignas(16) float scratch[WAVES][TERMS<DT>];
 };
 
+// Forward: one pass over the keys with the running maximum and sum of each row.  A wave has 16 queries, a lane one of them, so the transposed scores S^T come out of the products
+// with a query's keys in a lane's registers, and the probabilities go into the next product as they are.  A step's keys, values and the 64 table rows that the ring
+// of the tables lacks are on their way while the step before is worked on.
+// Batch 32 x 512, lengths 384 .. 512, 12 heads, bfloat16: 170 us for 42 GFLOP.  Bound by the waits of one wave's chain (scores, their turn
+// through LDS, maximum, exponentials, product), of which two waves of a SIMD hide a part: vector instructions take 49 % of the time, LDS 45, products 20.  Two workgroups to a CU
+// are what LDS holds; one takes 240 us.
 template <int DT, bool PK, bool PQ>
 __global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_fwd_kernel(Args a) {
     using E = Elem<DT>;
@@ -331,6 +340,9 @@ struct KvLds {
     static_assert(SKEWED<DT> * sizeof(T) <= TERMS<DT> * sizeof(float), "");
 };
 
+// dk, dv: a workgroup has 64 keys, a wave 16, a lane one of them; it walks over the queries.  Here scores, exponentials and random numbers are made again, once for the whole
+// backward pass.  (Each owner making its own scores, without a workspace, needs them three times.)  Which keys are dropped is drawn a step ahead, a bit each.
+// The batch above: 262 us, bound like the forward pass (vector instructions 50 % of the time, LDS 44, products 18).  Registers are full: 256, two waves to a SIMD.
 template <int DT, bool PK, bool PQ>
 __global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_bwd_kv_kernel(Args a) {
     using E = Elem<DT>;
@@ -571,7 +583,8 @@ struct QLds {
     alignas(16) T k[TILE * ROW<DT>], pk[RING * ROW<DT>], ds[TILE * ROW<DT>], skewed[4][SKEWED<DT>];
 };
 
-// dq: a workgroup has 64 queries, a wave 16.
+// dq: a workgroup has 64 queries, a wave 16.  Two steps' rows and tiles of dS on their way.  The batch above: 106 us, of which the tiles, 154 MB, need 31; 4 x 4096: 540 for
+// 1.6 GB, 320 at the rate of a large copy.
 template <int DT, bool PK>
 __global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_bwd_q_kernel(Args a) {
     using E = Elem<DT>;
@@ -863,6 +876,8 @@ __device__ __forceinline__ void sum_tables(const Args& a, TablesLds<DT>& sm, Dia
         }
 }
 
+// The batch above: 104 us.  Bound by what it reads, a tile of dS, of Q and of K for each step, 450 MB at 4.3 TB/s; 4 x 4096, where 15 of 127 diagonals are its: 280 us.
+// (Each head's workgroups on one XCD, for its cache: equal, and 107 and 380 us in packed and long batches, whose diagonals are less alike.)
 template <int DT, bool PK, bool PQ>
 __global__ __launch_bounds__(THREADS, DT == TDB_F32 ? 1 : 3) void attn_bwd_tables_kernel(Args a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -890,7 +905,7 @@ __global__ __launch_bounds__(THREADS, DT == TDB_F32 ? 1 : 3) void attn_bwd_table
 
 // A table row's gradient, offsets lo .. hi - 1: those of far diagonals come as one row for each wave of a table; the others, fewer than 128 at either end, from the one or
 // two diagonals whose tiles have them.  A wave for each row, parts dealt to its four groups of 16 lanes and asked for four at a time; the outermost rows, which have
-// hundreds of offsets, take the workgroup's waves together.  (A wave for each row, one part after the other: 290 us at 4 x 4096.)  Which group has a part does not depend on
+// hundreds of offsets, take the workgroup's waves together.  (A wave for each row, one part after the other, took 290 us at 4 x 4096, this 70; batch 32 x 512 18.)  Which group has a part does not depend on
 // the longest length, and a sum's bits do not either.
 template <int DT>
 __global__ __launch_bounds__(THREADS) void tables_sum_kernel(Args a) {
