@@ -147,6 +147,22 @@ def test_evaluation_is_as_before(dtype):
     assert all(torch.equal(a, b) for a, b in zip(*out))
 
 
+def test_a_model_that_has_been_evaluated_before():
+    torch.manual_seed(11)
+    model = patch_model(DebertaV2Model(config(0.25))).cuda().eval()
+    ids, mask, dout = (t.cuda() for t in inputs())
+    evaluate = lambda: [model(input_ids=ids, attention_mask=m).last_hidden_state for m in (mask, torch.ones_like(mask))]
+    with torch.no_grad():
+        before = evaluate()
+    patch_model(model, training=True)
+    with torch.no_grad():
+        assert all(torch.equal(a, b) for a, b in zip(before, evaluate()))
+    gradients(model.train(), ids, mask, dout)
+    model.eval()
+    with torch.no_grad():
+        assert all(torch.equal(a, b) for a, b in zip(before, evaluate()))
+
+
 def test_gradients_reach_the_embeddings_of_a_model_in_eval_mode():
     """Without dropout, whatever the mode: the gradient of inputs."""
     torch.manual_seed(11)

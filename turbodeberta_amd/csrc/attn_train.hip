@@ -1041,7 +1041,7 @@ Plan plan_of(const tdb_train_attn_args& a) {
     // A diagonal's parts, a power of two: three workgroups for each of 256 CUs where every diagonal has its own sums, and 64 tiles for a workgroup where most are level.
     int bits = 0;
     while ((int64_t(2) << bits) * p.heads * p.tiles <= 768 && (2 << bits) <= a.batch) ++bits;
-    while (bits < 12 && (int64_t(a.batch) * p.tiles) >> bits > 64) ++bits;
+    while (bits < 12 && p.row_tiles >> bits > 64) ++bits;
     p.split_bits = 0;
     while (p.split_bits < bits && (2 << p.split_bits) <= a.batch) ++p.split_bits;
     p.seg_bits = bits - p.split_bits;
@@ -1085,6 +1085,9 @@ int check(const tdb_train_attn_args* a, bool backward, bool sizes_only = false) 
     for (int n = 0; n < (backward ? 8 : 4); ++n)
         if (rows[n] < a->head_dim || rows[n] * int64_t(elem(a->dtype)) > MOST_STRIDE)
             return tdb_fail(TDB_ERR_STRIDE, "rows must lie head_dim values to 16 MiB apart");
+    const int64_t written[][2] = {{a->o_stride_h, a->o_stride_b}, {a->dq_stride_h, a->dq_stride_b}, {a->dk_stride_h, a->dk_stride_b}, {a->dv_stride_h, a->dv_stride_b}};
+    for (int n = backward ? 1 : 0; n < (backward ? 4 : 1); ++n)
+        if ((a->heads > 1 && written[n][0] < a->head_dim) || (!a->cu_seqlens && a->batch > 1 && written[n][1] < a->head_dim)) return tdb_fail(TDB_ERR_STRIDE, "rows of a result overlap");
     const int64_t table[] = {a->pos_key_stride_h, a->pos_key_stride_r, a->pos_query_stride_h, a->pos_query_stride_r};
     for (int64_t s : table)
         if (s < 0 || s * int64_t(elem(a->dtype)) % 16) return tdb_fail(TDB_ERR_STRIDE, "strides of the tables must be non-negative multiples of 16 bytes");
@@ -1094,6 +1097,9 @@ int check(const tdb_train_attn_args* a, bool backward, bool sizes_only = false) 
             return tdb_fail(TDB_ERR_STRIDE, "a head's table must lie within 2 GiB");
         if (!a->delta_lut || a->lut_half < a->max_seqlen - 1) return tdb_fail(TDB_ERR_POSITION, "delta_lut is missing or shorter than the sequences");
         if (backward && ((a->pos_key && !a->dpos_key) || (a->pos_query && !a->dpos_query))) return tdb_fail(TDB_ERR_NULL, "a table's gradient has no place");
+        const int64_t least = a->heads > 1 ? 2 * int64_t(a->span) * a->head_dim : 0;
+        if (backward && ((a->pos_key && a->dpos_key_stride_h < least) || (a->pos_query && a->dpos_query_stride_h < least)))
+            return tdb_fail(TDB_ERR_STRIDE, "gradients of the heads' tables overlap");
     }
     if (backward && a->workspace_bytes < plan_of(*a).bytes) return tdb_fail(TDB_ERR_SHAPE, "the workspace is too small");
     return TDB_OK;
