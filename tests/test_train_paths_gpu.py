@@ -40,6 +40,7 @@ def random(*shape, dtype=torch.float32, n=0):
 
 def calls(dtype):
     """name -> (function, inputs)"""
+    s = seed()
     x, r, w, b = random(37, 96, dtype=dtype), random(37, 96, dtype=dtype, n=1), random(96, dtype=dtype, n=2), random(96, dtype=dtype, n=3)
     q, k, v = (random(2, 3, 90, 24, dtype=dtype, n=n) for n in (4, 5, 6))
     pk, pq = (random(3, 16, 24, dtype=dtype, n=n) for n in (7, 8))
@@ -47,12 +48,12 @@ def calls(dtype):
     cu = torch.tensor([0, 50, 50, 180], dtype=torch.int32).cuda()
     tokens = lambda t: t.transpose(1, 2).reshape(180, 3, 24)
     return {
-        "dropout": (lambda x: dropout(x, 0.3, seed()), [x]),
+        "dropout": (lambda x: dropout(x, 0.3, s), [x]),
         "layer_norm": (layer_norm, [x, w, b]),
         "plain_layer_norm": (layer_norm, [x]),
-        "add_norm": (lambda *a: dropout_add_layer_norm(*a, p=0.3, seed=seed()), [x, r, w, b]),
-        "attention": (lambda *a: fixed(*a, 0.2, 8, 32, seqlens_k=lens, dropout_p=0.2, seed=seed()), [q, k, v, pk, pq]),
-        "packed_attention": (lambda *a: varlen(*a, cu, 130, 0.2, 8, 32, dropout_p=0.2, seed=seed()), [*map(tokens, (q, k, v)), pk, pq]),
+        "add_norm": (lambda *a: dropout_add_layer_norm(*a, p=0.3, seed=s), [x, r, w, b]),
+        "attention": (lambda *a: fixed(*a, 0.2, 8, 32, seqlens_k=lens, dropout_p=0.2, seed=s), [q, k, v, pk, pq]),
+        "packed_attention": (lambda *a: varlen(*a, cu, 130, 0.2, 8, 32, dropout_p=0.2, seed=s), [*map(tokens, (q, k, v)), pk, pq]),
     }
 
 
@@ -182,3 +183,58 @@ def test_tiles_of_one_table_row(lens, buckets, max_rel, dtype):
     c = Case(lens, H=1 if lens[0] > 900 else 2, dtype=dtype, buckets=buckets, max_rel=max_rel, p=0.1, seed=21)
     c.check(c.packed())
     c.check(c.unpad(c.padded(max(lens)), max(lens)))
+
+
+class Look(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, seen):
+        ctx.seen = seen
+        return x.clone()
+
+    @staticmethod
+    def backward(ctx, dy):
+        ctx.seen.append(_lib.host().backward_begins())
+        return dy, None
+
+
+def test_a_leaf_that_belongs_to_another_stream_is_seen():
+    side = torch.cuda.Stream()
+    for alive in (False, True):
+        x = random(8, 64).requires_grad_()
+        earlier = x * 2 if alive else None
+        side.wait_stream(torch.cuda.current_stream())
+        seen = []
+        with torch.cuda.stream(side):
+            Look.apply(x, seen).sum().backward()
+        torch.cuda.synchronize()
+        assert seen == [alive] and (earlier is not None) == alive
+
+
+@pytest.mark.parametrize("path", ["native", "python"])
+@pytest.mark.parametrize("name", ["dropout", "layer_norm", "attention"])
+def test_capture_while_an_eager_graph_of_the_same_leaves_lives(name, path, python_path):
+    """Refused before autograd's engine meets the other stream; possible once that graph is gone, also by the same leaves."""
+    if path == "python":
+        python_path()
+    want = run(name, torch.float32)
+    fn, inputs = calls(torch.float32)[name]
+    inputs = [t.requires_grad_() for t in inputs]
+    earlier = fn(*inputs)
+    dy = random(*earlier.shape, n=9)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = fn(*inputs)
+        with pytest.raises(RuntimeError, match="holds the same leaves"):
+            torch.autograd.grad(y, inputs, dy)
+    del y, earlier
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = fn(*inputs)
+        grads = torch.autograd.grad(y, inputs, dy)
+    for _ in range(3):
+        for t in (y, *grads):
+            t.detach().zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert same((y.detach(), list(grads)), want)

@@ -8,9 +8,11 @@
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/core/GradMode.h>
 #include <c10/hip/HIPFunctions.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -57,9 +59,27 @@ Optional optional(const Tensor& t) { return t.defined() ? Optional(t) : std::nul
 Tensor plain(const Optional& t) { return t.value_or(Tensor()); }
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
+// Whether the node whose backward pass runs hands a gradient to a leaf whose accumulation belongs to another stream: that of the first graph of the leaf that still lives.
+bool tied_to_another_stream() {
+    const auto node = torch::autograd::get_current_node();
+    if (!node) return false;
+    for (const auto& edge : node->next_edges()) {
+        if (!dynamic_cast<torch::autograd::AccumulateGrad*>(edge.function.get())) continue;
+        const auto stream = edge.function->stream();
+        if (stream && stream->id() != c10::hip::getCurrentHIPStream(stream->device_index()).id()) return true;
+    }
+    return false;
+}
+// Under capture autograd's engine would wait across the two streams, and the process ends.
+void capturable() {
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    TORCH_CHECK(!tied_to_another_stream(), "a backward pass cannot be captured while a graph of autograd's that was recorded on another stream holds the same leaves: drop its results first");
+}
+
 // The gradient that arrives has to be a tensor of the device's memory, with no transform around it.
 void arrived(const Tensor& dy, const Tensor& x) {
     TORCH_CHECK(tdb_host_plain(dy, x, false), "the gradient must be an ordinary tensor on ", x.device());
+    capturable();
 }
 
 // Results of a backward pass, which is not differentiable itself: asked for a second gradient they raise.
@@ -407,7 +427,16 @@ PyObject* py_bind_train(PyObject*, PyObject* args) {
     Py_RETURN_NONE;
 }
 
+// backward_begins(): what the Python path's backward passes ask first, see capturable; returns what it looks at
+PyObject* py_backward_begins(PyObject*, PyObject*) {
+    HANDLE_TH_ERRORS
+    capturable();
+    return PyBool_FromLong(tied_to_another_stream());
+    END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef kTrain[] = {
+    {"backward_begins", py_backward_begins, METH_NOARGS, nullptr},
     {"bind_train", py_bind_train, METH_VARARGS, nullptr},
     {"train_dropout", reinterpret_cast<PyCFunction>(py_dropout), METH_FASTCALL, nullptr},
     {"train_norm", reinterpret_cast<PyCFunction>(py_norm), METH_FASTCALL, nullptr},

@@ -27,6 +27,7 @@ class _Dropout(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
+        _lib.host().backward_begins()
         return _launch(dy, ctx.threshold, *ctx.saved_tensors), None, None
 
 

@@ -42,6 +42,7 @@ class _Norm(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
+        _lib.host().backward_begins()
         x, residual, weight, bias, seed = ctx.saved_tensors
         want_x, want_res, want_w, want_b = ctx.needs_input_grad[:4]
         hidden = x.shape[-1]

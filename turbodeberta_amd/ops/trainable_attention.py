@@ -86,6 +86,7 @@ class _Attention(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
+        _lib.host().backward_begins()
         if ctx.nothing:
             return tuple(None if t is None else torch.zeros_like(t) for t in ctx.saved_tensors) + (None,) * (3 + len(ctx.plain))
         q, k, v, o, rest, lse, pk, pq, lens, cu, seed = ctx.saved_tensors
