@@ -563,12 +563,12 @@ __device__ __forceinline__ void load_own(typename Elem<DT>::X8 (&own)[2], const 
     }
 }
 
-// float16: a power of two that brings the gradients of scores near the top of the type's range: they are at most 2 |dout| |v| times dropout's factor.  Other types
+// float16: a power of two that brings the gradients of scores, which are kept without dropout's factor, near the top of the type's range: they are at most 2 |dout| |v|.  Other types
 // hold any size: 1.
 template <int DT>
 __device__ __forceinline__ float score_power(const Args& a) {
     if constexpr (DT != TDB_F16) return 1.f;
-    const float most = 2.f * a.factor * sqrtf(__builtin_bit_cast(float, a.largest[0])) * sqrtf(__builtin_bit_cast(float, a.largest[1]));
+    const float most = 2.f * sqrtf(__builtin_bit_cast(float, a.largest[0])) * sqrtf(__builtin_bit_cast(float, a.largest[1]));
     if (!(most > 0.f) || !(most < __builtin_inff())) return 1.f;
     int e;
     (void)frexpf(most, &e);             // most < 2^e

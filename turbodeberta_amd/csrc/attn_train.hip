@@ -159,7 +159,7 @@ __global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_fwd_kernel(Args a) {
 __device__ __forceinline__ int tile_up(const Args& a, int x) { return (x + TILE * a.tiles + TILE - 1) / TILE - a.tiles; }
 __device__ __forceinline__ int tile_down(const Args& a, int x) { return (x + TILE * a.tiles) / TILE - a.tiles; }
 
-// D_i = dO_i . O_i for every row and head: 8 lanes each.  float16: the largest squares of the norms of rows of dO and V as well.  And the offsets at which the rows of the
+// D_i = dO_i . O_i for every row and head, without dropout's factor: 8 lanes each.  float16: the largest squares of the norms of rows of dO and V as well.  And the offsets at which the rows of the
 // tables start, and the diagonals of tiles that lie in the last or in the first of these rows altogether.
 template <int DT>
 __global__ __launch_bounds__(THREADS) void attn_delta_kernel(Args a, uint32_t* largest) {
@@ -211,7 +211,7 @@ __global__ __launch_bounds__(THREADS) void attn_delta_kernel(Args a, uint32_t* l
         }
 #pragma unroll
         for (int n = 1; n < 8; n <<= 1) dot += __shfl_xor(dot, n), sq += __shfl_xor(sq, n), sv += __shfl_xor(sv, n);
-        if (mine && (threadIdx.x & 7) == 0) a.delta[h * a.lines + row] = dot;
+        if (mine && (threadIdx.x & 7) == 0) a.delta[h * a.lines + row] = a.factor > 0.f ? dot / a.factor : 0.f;
         most_do = fmaxf(most_do, sq), most_v = fmaxf(most_v, sv);
     }
     if constexpr (DT == TDB_F16) {
@@ -318,12 +318,12 @@ constexpr int SKEWED = 16 * SKEW<DT>;
 template <class T>
 __device__ __forceinline__ void put(T* to, T x) { *TDB_SHARED(volatile T, to) = x; }
 
-// The eight r = 32 n + 8 g .. of the lane's row, zeros outside.
-template <int DT>
+// The eight r = 32 n + 8 g .. of the lane's row, zeros outside (ZEROS: these are in LDS already).
+template <int DT, bool ZEROS>
 __device__ __forceinline__ typename Elem<DT>::X8 skew_frag(const typename Elem<DT>::T* skewed, int n) {
     const int c = lane_c(), r = 32 * n + 8 * lane_g();
     typename Elem<DT>::X8 x = read8<DT>(skewed + c * (SKEW<DT> - 1) + 16 + r);
-    if (n == 1) return x;               // (c <= r <= c + 63)
+    if (ZEROS || n == 1) return x;      // (c <= r <= c + 63)
 #pragma unroll
     for (int i = 0; i < 8; ++i)
         if (n == 0 ? r + i < c : r + i > c + 63) x[i] = typename Elem<DT>::T(0.f);
@@ -372,7 +372,7 @@ __global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_bwd_kv_kernel(Args a
     load_own<DT>(v, a.v, a, w, h, row);
     tables.fill(sm.pk, sm.pq, w.row0);
     const TdbKey key = a.threshold ? tdb_key(a.seed) : TdbKey{0, 0};
-    const float power = score_power<DT>(a), rounded = w.len > 1 ? power : 0.f;      // (the softmax of one key is a constant)
+    const float power = score_power<DT>(a);
     const __amdgpu_buffer_rsrc_t lines = buffer((wave == 0 ? a.lse : a.delta) + h * a.lines + w.line, int64_t(w.len) * 4);      // of the waves that load them
     float line_next = 0.f;
     bool far = false;
@@ -401,7 +401,7 @@ __global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_bwd_kv_kernel(Args a
     if (a.threshold) draw(0, 0);
 
     const float c1 = a.scale * LOG2E, shift = DT == TDB_F16 ? float(a.p_shift) : 0.f, unshift = DT == TDB_F16 ? ldexpf(1.f, -a.p_shift) : 1.f;
-    const float down = unshift * rounded;
+    const float down = unshift * power;         // (1 but in float16)
     const bool edge = w.row0 + TILE > w.len;
     const int tile_col = row / TILE, bit = (row & 16) + c;
     T* ds = static_cast<T*>(a.ds) + ((int64_t(h - a.head0) * a.row_tiles + w.row_tile) * a.tiles + tile_col) * TILE_VALUES + row / 16 % 4 * 1024;
@@ -468,15 +468,19 @@ __global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_bwd_kv_kernel(Args a
                 for (int e = 0; e < 4; ++e) {
                     const bool in = words[e] >> bit & 1;
                     pr[e] = in ? pr[e] : 0.f;
-                    grad[e] = in ? grad[e] * a.factor : 0.f;
+                    grad[e] = in ? grad[e] : 0.f;
                 }
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 p[m >> 1][4 * (m & 1) + e] = T(pr[e]);
-                grads[4 * m + e] = s[m][e] * ((grad[e] - delta[e]) * down);
+                grads[4 * m + e] = DT == TDB_F16 ? s[m][e] * ((grad[e] - delta[e]) * down) : s[m][e] * (grad[e] - delta[e]);
                 dsx[m >> 1][4 * (m & 1) + e] = T(grads[4 * m + e]);
             }
+        }
+        if (w.len == 1) {               // the softmax of one key is a constant
+#pragma unroll
+            for (int n = 0; n < 16; ++n) grads[n] = 0.f, dsx[n >> 3][n & 7] = T(0.f);
         }
         if (is_level) {
             if constexpr (PQ) {
@@ -532,7 +536,7 @@ __global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_bwd_kv_kernel(Args a
                 X8 t[3][4], b[3];
 #pragma unroll
                 for (int n = 0; n < 3; ++n) {
-                    b[n] = skew_frag<DT>(skewed, n);
+                    b[n] = skew_frag<DT, false>(skewed, n);
 #pragma unroll
                     for (int d = 0; d < 4; ++d) t[n][d] = ring_frag<DT>(sm.pq, 16 * wave + 32 * n + base, 16 * d);
                 }
@@ -551,7 +555,7 @@ __global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_bwd_kv_kernel(Args a
     } else if (PQ) {
         level_none(a, 1, h, w.block);
     }
-    store_rows<DT>(a.dk, a, w, h, row, dk, a.scale / power);
+    store_rows<DT>(a.dk, a, w, h, row, dk, a.scale * a.factor / power);
     store_rows<DT>(a.dv, a, w, h, row, dv, a.factor * unshift);
 }
 
@@ -619,6 +623,9 @@ __global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_bwd_q_kernel(Args a)
     };
     Tables<DT, 1, THREADS, PK, false> tables(a, h);
     tables.fill(sm.pk, nullptr, w.row0);
+    if constexpr (PK) {                 // what no step writes: an index below 16 or above 79 of a row
+        for (int n = threadIdx.x; n < 4 * SKEWED<DT>; n += THREADS) (&sm.skewed[0][0])[n] = T(0.f);
+    }
     int y_next = 0;
     const float* row_sums = a.row_sums + (int64_t(h - a.head0) * a.row_tiles + w.row_tile + w.row0 / TILE) * a.tiles * ROW_SUMS;
     float by_query[2] = {0.f, 0.f};
@@ -677,7 +684,7 @@ __global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_bwd_q_kernel(Args a)
             X8 by[3], t[3][4];
 #pragma unroll
             for (int n = 0; n < 3; ++n) {
-                by[n] = skew_frag<DT>(sm.skewed[wave], n);
+                by[n] = skew_frag<DT, true>(sm.skewed[wave], n);
 #pragma unroll
                 for (int d = 0; d < 4; ++d) t[n][d] = ring_frag<DT>(sm.pk, 16 * wave + 32 * n + base, 16 * d);
             }
@@ -718,7 +725,7 @@ __global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_bwd_q_kernel(Args a)
     } else if (PK) {
         level_none(a, 0, h, w.block);
     }
-    store_rows<DT>(a.dq, a, w, h, row, dq, a.scale / score_power<DT>(a));
+    store_rows<DT>(a.dq, a, w, h, row, dq, a.scale * a.factor / score_power<DT>(a));
 }
 
 // Parts that the sequences of a diagonal are dealt to, as many as it has tiles, next to the longest one; each is 2^seg_bits, to which a sequence's tiles are dealt in turn.
@@ -990,7 +997,7 @@ __global__ __launch_bounds__(THREADS) void tables_sum_kernel(Args a) {
         if (row >= 2 * a.span || int(threadIdx.x & 63) >= a.D) return;
         using T = typename Elem<DT>::T;
         T* const to = static_cast<T*>(which ? a.dpq : a.dpk) + h * (which ? a.dpq_h : a.dpk_h) + int64_t(row) * a.D + (threadIdx.x & 63);
-        *to = T(all * a.scale / score_power<DT>(a));
+        *to = T(all * (a.scale * a.factor / score_power<DT>(a)));
     };
     // what lane 4 d + e of a wave adds up: value e of lane d of each group
     auto total = [&](int first, int groups) {
