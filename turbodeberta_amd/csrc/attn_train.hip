@@ -587,8 +587,8 @@ struct QLds {
     alignas(16) T k[TILE * ROW<DT>], pk[RING * ROW<DT>], ds[TILE * ROW<DT>], skewed[4][SKEWED<DT>];
 };
 
-// dq: a workgroup has 64 queries, a wave 16.  Two steps' rows and tiles of dS on their way.  The batch above: 106 us, of which the tiles, 154 MB, need 31; 4 x 4096: 540 for
-// 1.6 GB, 320 at the rate of a large copy.
+// dq: a workgroup has 64 queries, a wave 16; the next step's rows and tile of dS are on their way.  The batch above: 86 us, of which the tiles, 154 MB, need 31; 4 x 4096: 490
+// for 1.6 GB, 320 at the rate of a large copy.  (Two steps ahead took 104 and 540: registers for two waves to a SIMD, not three.)
 template <int DT, bool PK>
 __global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_bwd_q_kernel(Args a) {
     using E = Elem<DT>;
@@ -620,7 +620,7 @@ __global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_bwd_q_kernel(Args a)
         Scores<DT> ds;
         int ends[2];
         u32x4 sums;
-    };
+    } next;
     Tables<DT, 1, THREADS, PK, false> tables(a, h);
     tables.fill(sm.pk, nullptr, w.row0);
     if constexpr (PK) {                 // what no step writes: an index below 16 or above 79 of a row
@@ -630,24 +630,24 @@ __global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_bwd_q_kernel(Args a)
     const float* row_sums = a.row_sums + (int64_t(h - a.head0) * a.row_tiles + w.row_tile + w.row0 / TILE) * a.tiles * ROW_SUMS;
     float by_query[2] = {0.f, 0.f};
     level.ready();
-    auto fetch = [&](Next& n) {
+    auto fetch = [&]() {
         if constexpr (PK) {             // (zeros for other tiles)
             const __amdgpu_buffer_rsrc_t from = buffer(row_sums, level.has((w.row0 - y_next) / TILE) ? ROW_SUMS * 4 : 0);
-            n.sums = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(from, (16 * wave + lane_c()) * 16, 0, 0));
+            next.sums = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(from, (16 * wave + lane_c()) * 16, 0, 0));
             row_sums += ROW_SUMS;
         }
-        keys.load(n.k);
-        n.ds.load(tile);
+        keys.load(next.k);
+        next.ds.load(tile);
         tile += TILE_VALUES;
         tables.load();
-        n.pk = tables.k;
+        next.pk = tables.k;
         tables.look_at_ends(w.row0 - y_next);
-        n.ends[0] = tables.ends[0], n.ends[1] = tables.ends[1];
+        next.ends[0] = tables.ends[0], next.ends[1] = tables.ends[1];
         y_next += TILE;
         tables.look(0, w.row0 - y_next);
     };
     int base = 0;
-    auto step = [&](Next& next, int y0) {
+    auto step = [&](int y0) {
         const int t = (w.row0 - y0) / TILE;
         const bool is_level = PK && level.has(t);
         __syncthreads();
@@ -670,7 +670,7 @@ __global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_bwd_q_kernel(Args a)
             }
         }
         __syncthreads();
-        if (y_next < w.len) fetch(next);
+        if (y_next < w.len) fetch();
         X8 b[2], k[2][4];
         auto own = [&]() {
 #pragma unroll
@@ -711,13 +711,8 @@ __global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_bwd_q_kernel(Args a)
             for (int d = 0; d < 4; ++d) dq[d] = E::mma(k[n][d], b[n], dq[d]);
         base ^= 64;
     };
-    Next one, two;
-    fetch(one);
-    if (y_next < w.len) fetch(two);
-    for (int y0 = 0; y0 < w.len; y0 += 2 * TILE) {
-        step(one, y0);
-        if (y0 + TILE < w.len) step(two, y0 + TILE);
-    }
+    fetch();
+    for (int y0 = 0; y0 < w.len; y0 += TILE) step(y0);
     if (PK && level.any(w.row0 / TILE - (w.len - 1) / TILE, w.row0 / TILE)) {
         X8 q[2];
         load_own<DT>(q, a.q, a, w, h, row);
