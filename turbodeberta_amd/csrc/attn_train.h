@@ -22,6 +22,7 @@
 #include <type_traits>
 
 #include "philox.h"
+#include "tdb_error.h"
 #include "tdb_internal.h"
 #include "tdb_train.h"
 

@@ -6,6 +6,7 @@
 #include <cstdio>
 #include <cstring>
 
+#include "tdb_error.h"
 #include "tdb_internal.h"
 
 namespace {

@@ -6,9 +6,6 @@
 
 #include "tdb_attn.h"
 
-// Leaves the message that tdb_last_error() returns to this thread; returns the code.
-int tdb_fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
-
 // One flattened description of a launch; fixed-length and packed calls both reduce to it.
 // A sequence b starts at element offset  b*stride_b  (fixed)  or  cu_seqlens[b]*stride_l  (packed)
 // and its row l, head h lives at  + l*stride_l + h*stride_h.

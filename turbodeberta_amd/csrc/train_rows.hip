@@ -12,6 +12,7 @@
 #include <algorithm>
 
 #include "philox.h"
+#include "tdb_error.h"
 #include "tdb_internal.h"
 #include "tdb_train.h"
 
