@@ -347,7 +347,7 @@ struct KvLds {
 
 // dk, dv: a workgroup has 64 keys, a wave 16, a lane one of them; it walks over the queries.  Here scores, exponentials and random numbers are made again, once for the whole
 // backward pass.  (Each owner making its own scores, without a workspace, needs them three times.)  Which keys are dropped is drawn a step ahead, a bit each.
-// The batch above: 262 us, bound like the forward pass (vector instructions 50 % of the time, LDS 44, products 18).  Registers are full: 256, two waves to a SIMD.
+// The batch above: 260 us, bound like the forward pass (vector instructions 48 % of the time, LDS 45, products 19).  Registers are full: 256, two waves to a SIMD.
 template <int DT, bool PK, bool PQ>
 __global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_bwd_kv_kernel(Args a) {
     using E = Elem<DT>;
@@ -592,7 +592,7 @@ struct QLds {
     alignas(16) T k[TILE * ROW<DT>], pk[RING * ROW<DT>], ds[TILE * ROW<DT>], skewed[4][SKEWED<DT>];
 };
 
-// dq: a workgroup has 64 queries, a wave 16; the next step's rows and tile of dS are on their way.  The batch above: 86 us, of which the tiles, 154 MB, need 31; 4 x 4096: 490
+// dq: a workgroup has 64 queries, a wave 16; the next step's rows and tile of dS are on their way.  The batch above: 88 us, of which the tiles, 154 MB, need 31; 4 x 4096: 490
 // for 1.6 GB, 320 at the rate of a large copy.  (Two steps ahead took 104 and 540: registers for two waves to a SIMD, not three.)
 template <int DT, bool PK>
 __global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_bwd_q_kernel(Args a) {
