@@ -202,8 +202,9 @@ class FlashDisentangledSelfAttention(DisentangledSelfAttention):
     modeling_deberta_v2.py:256-259); downstream layers mask them anyway.
     ``output_attentions=True`` needs the probability matrix, which the fused kernel never forms: that
     call is served by the eager parent class.
-    ``trainable = True`` (``patch_model(model, training=True)``): a call that autograd records goes to ``ops.trainable_attention``, which has the
-    gradient and, in training mode, the dropout of the probabilities (modeling_deberta_v2.py:262); without it such a call has no gradient and drops nothing."""
+    ``trainable = True`` (``patch_model(model, training=True)``): a call in training mode, or one that autograd records, goes to
+    ``ops.trainable_attention``, which has the gradient and, in training mode, the dropout of the probabilities
+    (modeling_deberta_v2.py:262); without it such a call has no gradient and drops nothing."""
 
     trainable = False
 
@@ -234,7 +235,7 @@ class FlashDisentangledSelfAttention(DisentangledSelfAttention):
         pos_key, pos_query, sm_scale, buckets, max_rel = self._position_terms(rel_embeddings, hidden_states.dtype,
                                                                               frozen)
         seqlens = _mask_info(attention_mask).lengths if attention_mask is not None else None
-        if self.trainable and _training.recorded(q, k, v):
+        if self.trainable and _training.operators_take(self, q, k, v):
             p = _training.rate_of(self, self.dropout)
             out = trainable_attention_with_disentangled(q, k, v, pos_key, pos_query, sm_scale, buckets, max_rel, seqlens_k=seqlens, dropout_p=p,
                                                         seed=_training.draw_seed(self, q.device) if p else None)
@@ -646,7 +647,7 @@ def patch_model(model: nn.Module, training: bool = False) -> nn.Module:
     e.g. one loaded with ``from_pretrained``) to the fused kernel, in place.  Parameters are untouched.
 
     ``training=True``: the model can be trained as well.  Attention, LayerNorms and dropouts of the DeBERTa modules run the training operators
-    (``turbodeberta_amd.training``) wherever autograd records; evaluation under ``torch.no_grad`` is not changed by it.  Head dimensions: multiples of 8
+    (``turbodeberta_amd.training``) in training mode and wherever autograd records; evaluation under ``torch.no_grad`` is not changed by it.  Head dimensions: multiples of 8
     up to 64; no ``pos_att_type`` where ``relative_attention`` is off.  Masks come from PyTorch's generator but are not those that ``nn.Dropout`` would draw."""
     swaps = {DisentangledSelfAttention: FlashDisentangledSelfAttention, DebertaV2Encoder: FlashDebertaV2Encoder,
              DebertaV2Model: FlashDebertaV2Model}        # none of them adds parameters or constructor state

@@ -1,9 +1,12 @@
 """Modules of a DeBERTa-v2/v3 model that is trained with this package's operators.
 
 ``patch_model(model, training=True)`` (``turbodeberta_amd.model``) switches a model's dropouts, LayerNorms and output blocks to the classes below and
-its attention to ``ops.trainable_attention``.  They add no parameters and no state.  Where autograd records (``torch.enable_grad``, tensors on the GPU
-in float32, bfloat16 or float16) they call the operators, which store no masks, no probabilities and nothing between dropout, residual and
-LayerNorm; everything else -- evaluation, ``torch.no_grad``, the CPU -- runs the parent class's code."""
+its attention to ``ops.trainable_attention``.  They add no parameters and no state.  In training mode, and in evaluation where autograd records, they
+call the operators for tensors on the GPU in float32, bfloat16 or float16, which store no masks, no probabilities and nothing between
+dropout, residual and LayerNorm; everything else -- evaluation under ``torch.no_grad``, the CPU -- runs the parent class's code.
+
+Training mode under ``torch.no_grad`` counts as well: checkpointing of the reentrant kind runs a layer that way first and again with gradients, and
+both runs have to draw the same masks."""
 from __future__ import annotations
 
 import torch
@@ -16,9 +19,9 @@ from .ops.layer_norm import dropout_add_layer_norm, layer_norm
 _TYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 
-def recorded(*tensors) -> bool:
-    """Whether a call of these tensors is one for the training operators."""
-    return torch.is_grad_enabled() and all(t.is_cuda and t.dtype in _TYPES for t in tensors)
+def operators_take(module: nn.Module, *tensors) -> bool:
+    """Whether a module's call with these tensors is one for the training operators."""
+    return (module.training or torch.is_grad_enabled()) and all(t.is_cuda and t.dtype in _TYPES for t in tensors)
 
 
 def draw_seed(module: nn.Module, device) -> torch.Tensor:
@@ -36,7 +39,7 @@ class FlashDropout(nn.Dropout):
     """``nn.Dropout`` by ``ops.dropout.dropout``."""
 
     def forward(self, x):
-        if not (self.training and self.p > 0 and not self.inplace and recorded(x)):
+        if not (self.training and self.p > 0 and not self.inplace and operators_take(self, x)):
             return super().forward(x)
         return dropout(x, self.p, draw_seed(self, x.device))
 
@@ -57,7 +60,7 @@ class FlashLayerNorm(nn.LayerNorm):
     """``nn.LayerNorm`` by ``ops.layer_norm.layer_norm``."""
 
     def forward(self, x):
-        a = _norm_arguments(self, x) if recorded(x) else None
+        a = _norm_arguments(self, x) if operators_take(self, x) else None
         return super().forward(x) if a is None else layer_norm(*a, self.eps)
 
 
@@ -65,7 +68,7 @@ class _Output:
     """``LayerNorm(dropout(dense(x)) + input)`` (modeling_deberta_v2.py:42-53, :400-411) by ``ops.layer_norm.dropout_add_layer_norm``."""
 
     def forward(self, hidden_states, input_tensor):
-        if not recorded(hidden_states, input_tensor):
+        if not operators_take(self, hidden_states, input_tensor):
             return super().forward(hidden_states, input_tensor)
         x = self.dense(hidden_states)
         wide = torch.promote_types(x.dtype, input_tensor.dtype)
