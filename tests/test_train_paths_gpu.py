@@ -238,3 +238,50 @@ def test_capture_while_an_eager_graph_of_the_same_leaves_lives(name, path, pytho
         graph.replay()
         torch.cuda.synchronize()
         assert same((y.detach(), list(grads)), want)
+
+
+def test_offsets_past_32_bits():
+    """Tensors of more than 2^32 bytes and 2^31 values; what is not looked at is not written first."""
+    n = (1 << 31) + 72
+    x = torch.empty(n, dtype=torch.float16, device="cuda")
+    y = torch.empty_like(x)
+    ends = [slice(0, 64), slice((1 << 31) - 64, n)]
+    for e in ends:
+        x[e] = 1.0
+    _lib.check(_lib.load().tdb_dropout(x.data_ptr(), y.data_ptr(), n, _lib.TDB_F16, 1 << 15, seed().data_ptr(), torch.cuda.current_stream().cuda_stream))
+    import numpy as np
+    import train_reference as R
+    for e in ends:
+        at = np.arange(e.start, e.stop)
+        u = R.numbers(((at // 8 & 0xffffffff).astype(np.uint64), (at // 8 >> 32).astype(np.uint64), np.zeros(len(at), np.uint64), np.zeros(len(at), np.uint64)), SEED)
+        assert torch.equal(y[e].cpu().double(), R.factors(u[np.arange(len(at)), at % 8], 0.5))
+    del x, y
+    rows, hidden = (1 << 31) // 2048 + 5, 2048
+    x = torch.empty(rows, hidden, dtype=torch.float16, device="cuda")
+    x[-7:] = random(7, hidden, dtype=torch.float16)
+    assert torch.equal(layer_norm(x)[-7:], layer_norm(x[-7:].clone()))
+    del x
+    torch.cuda.empty_cache()
+
+
+def test_attention_offsets_past_32_bits():
+    """A batch of 2100 whose first and last sequence have tokens: 4.4 GB for q alone; the last one's results are those it has by itself."""
+    B, H, L, D = 2100, 8, 2048, 64
+    lens = torch.zeros(B, dtype=torch.int32, device="cuda")
+    lens[0], lens[-1] = 100, 130
+    big = [torch.empty(B, H, L, D, dtype=torch.bfloat16, device="cuda") for _ in range(4)]
+    small = [random(1, H, 130, D, dtype=torch.bfloat16, n=n) for n in range(4)]
+    for t, s in zip(big, small):
+        t[0, :, :100], t[-1, :, :130] = s[0, :, :100], s[0]
+    tables = [random(H, 32, D, dtype=torch.bfloat16, n=n) for n in (5, 6)]
+
+    def grads(q, k, v, dout, n):
+        q, k, v = (t.requires_grad_() for t in (q, k, v))
+        o = fixed(q, k, v, *tables, 0.1, 16, 64, seqlens_k=n)
+        return [o, *torch.autograd.grad(o, (q, k, v), dout)]
+
+    got = [t[-1, :, :130].clone() for t in grads(*big, lens)]
+    want = grads(*(s.clone() for s in small), lens[-1:].clone())
+    assert all(torch.equal(a, b[0]) for a, b in zip(got, want))
+    del big
+    torch.cuda.empty_cache()
