@@ -912,7 +912,7 @@ __global__ __launch_bounds__(THREADS, DT == TDB_F32 ? 1 : 3) void attn_bwd_table
 
 // A table row's gradient, offsets lo .. hi - 1: those of far diagonals come as one row for each wave of a table; the others, fewer than 128 at either end, from the one or
 // two diagonals whose tiles have them.  A wave for each row, parts dealt to its four groups of 16 lanes and asked for four at a time; the outermost rows, which have
-// hundreds of offsets, take the workgroup's waves together.  (A wave for each row, one part after the other, took 290 us at 4 x 4096, this 70; batch 32 x 512 18.)  Which group has a part does not depend on
+// hundreds of offsets, take the workgroup's waves together.  (A wave for each row, one part after the other, took 290 us at 4 x 4096, this 32; batch 32 x 512 18.)  Which group has a part does not depend on
 // the longest length, and a sum's bits do not either.
 template <int DT>
 __global__ __launch_bounds__(THREADS) void tables_sum_kernel(Args a) {
@@ -922,10 +922,9 @@ __global__ __launch_bounds__(THREADS) void tables_sum_kernel(Args a) {
     const int diagonals = 2 * a.tiles - 1, share_bits = a.pk.p && a.pq.p ? 1 : 2, split_bits = a.split_bits + a.seg_bits;
     if (!(which ? a.pq.p : a.pk.p)) return;
     const float* const parts = a.partial + (((int64_t(blockIdx.y) * diagonals) << (split_bits + 1)) + which) * (BY_OFFSET * 64) + 4 * d;
-    auto range = [&](int row, int& lo, int& hi) {
-        lo = hi = a.L;
-        if (row >= 2 * a.span) return;
-        lo = min(max(a.starts[row], 1 - a.L), a.L), hi = min(max(a.starts[row + 1], lo), a.L);
+    const int row0 = blockIdx.x * WAVES, mine = a.starts[min(row0 + min(int(threadIdx.x & 63), WAVES), 2 * a.span)];       // lane n: where row row0 + n starts
+    auto range = [&](int n, int& lo, int& hi) {         // (no offsets past the last row)
+        lo = min(max(__builtin_amdgcn_readlane(mine, n), 1 - a.L), a.L), hi = min(max(__builtin_amdgcn_readlane(mine, n + 1), lo), a.L);
     };
     // the sum of the row's parts that group `group` of `groups` (a power of two) has
     auto sum_of = [&](int lo, int hi, int group, int groups) {
@@ -958,11 +957,11 @@ __global__ __launch_bounds__(THREADS) void tables_sum_kernel(Args a) {
                 return at <= 126 && t > -a.tiles && t < a.tiles && !(t0 <= t && t <= t1);
             });
         };
-        if (hi - lo > 256) {
-            offsets(lo, lo + 128);
-            offsets(hi - 128, hi);
-        } else {
+        if (t0 > t1) {
             offsets(lo, hi);
+        } else {                        // what diagonals t0 - 1 and t1 + 1 have, where there are such
+            if (t0 > 1 - a.tiles) offsets(lo, min(TILE * t0, hi));
+            if (t1 < a.tiles - 1) offsets(max(TILE * t1 + 1, lo), hi);
         }
         if (t0 <= t1 && (lo == 1 - a.L || hi == a.L)) {      // level tiles: a sum of each workgroup that has met one, which stands for them all
             const float* const from = a.level_parts + (int64_t(which * a.heads + blockIdx.y) * a.blocks * 2 + (hi == a.L ? 0 : 1)) * 64 + 4 * d;
@@ -1005,9 +1004,8 @@ __global__ __launch_bounds__(THREADS) void tables_sum_kernel(Args a) {
         for (int n = 0; n < groups; ++n) all += s_sum[first + n][(threadIdx.x & 63) >> 2][threadIdx.x & 3];
         return all;
     };
-    const int row0 = blockIdx.x * WAVES;
     int lo, hi;
-    range(row0 + wave, lo, hi);
+    range(wave, lo, hi);
     const bool many = hi - lo > MANY;
     f32x4 sum = {0.f, 0.f, 0.f, 0.f};
     if (!many && hi > lo) sum = sum_of(lo, hi, (threadIdx.x >> 4) & 3, 4);
@@ -1015,7 +1013,7 @@ __global__ __launch_bounds__(THREADS) void tables_sum_kernel(Args a) {
     __syncthreads();
     if (!many) store(row0 + wave, total(4 * wave, 4));
     for (int n = 0; n < WAVES; ++n) {           // (the same for every wave)
-        range(row0 + n, lo, hi);
+        range(n, lo, hi);
         if (hi - lo <= MANY) continue;
         __syncthreads();
         s_sum[threadIdx.x >> 4][d] = sum_of(lo, hi, threadIdx.x >> 4, MOST_GROUPS);
