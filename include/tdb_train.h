@@ -58,10 +58,11 @@ int64_t tdb_norm_workspace(int64_t rows, int32_t hidden);
  * The probability of key j for query i of head h in sequence b has number 4 (j / 16 mod 2) + j mod 4 of counter (4 (j / 32) + j / 4 mod 4, i, b * heads + h, 1).
  * Forward writes o and lse, float32 [heads, rows], rows = batch * max_seqlen or total_tokens: the logarithm (base 2) of the sum of each row's exponentials, for the backward
  * call, which also reads o.  In 16 bits o_rest, [heads, rows, head_dim] back to back, takes what rounding took from o and goes to the backward call with it; NULL in both calls:
- * the gradients are made from o as it is rounded, and are the less exact the longer the rows.  Backward writes dq, dk, dv and the gradients of the tables, [heads, 2 span, head_dim] with rows back to back.  Rows beyond a sequence's
- * length, and packed rows of no sequence, are zeros in every result; what the inputs hold there does not matter.  workspace: tdb_attn_train_workspace() bytes for the
- * same arguments, 16-byte aligned.  Besides a few bytes for each row and table it holds the scores' gradients of as many heads at a time as fit 2 GiB, at least one:
- * element size * sum of (length * max_seqlen), lengths rounded up to 64.  Where there are tables, also a part for each table row and for each 64 x 64 of these scores 1 KiB.
+ * the gradients are made from o as it is rounded, and are the less exact the longer the rows.
+ * Backward writes dq, dk, dv and the gradients of the tables, [heads, 2 span, head_dim] with rows back to back.  Rows beyond a sequence's length, and packed rows of no
+ * sequence, are zeros in every result; what the inputs hold there does not matter.  workspace: tdb_attn_train_workspace() bytes for the same arguments, 16-byte aligned.  Besides a few bytes for each row and table it holds the scores' gradients of as many heads at a time as fit 2 GiB, at least one:
+ * element size * sum of (length * max_seqlen), lengths rounded up to 64.  Where there are tables, also for each 64 x 64 of these scores 1 KiB, and sums by
+ * relative position, up to 96 MiB or half as much as the scores' gradients in 16 bits.
  * The gradient of rows whose sequence has one token is zero in q, k and the tables.  Results must not overlap each other or an input.
  */
 typedef struct tdb_train_attn_args {

@@ -1043,7 +1043,8 @@ Plan plan_of(const tdb_train_attn_args& a) {
     const int64_t each = int64_t(p.row_tiles) * p.tiles * TILE_VALUES * int64_t(elem(a.dtype));
     p.heads = int(std::max<int64_t>(1, std::min<int64_t>(a.heads, MOST_SCORES / std::max<int64_t>(each, 1))));
     const int diagonals = 2 * p.tiles - 1;
-    // A diagonal's parts, a power of two: three workgroups for each of 256 CUs where every diagonal has its own sums, and 64 tiles for a workgroup where most are level.
+    // A diagonal's parts, a power of two: three workgroups for each of 256 CUs where every diagonal has its own sums, and 64 tiles for a workgroup where most are level
+    // (4 x 4096: 281 us and 32 for the sums; with 32 tiles 230 and 54, for sums of half of dS's size).
     int bits = 0;
     while ((int64_t(2) << bits) * p.heads * p.tiles <= 768 && (2 << bits) <= a.batch) ++bits;
     while (bits < 12 && p.row_tiles >> bits > 64) ++bits;

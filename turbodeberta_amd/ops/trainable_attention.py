@@ -2,7 +2,8 @@
 
 What ``ops.flash_attention`` and ``ops.flash_attention_varlen`` compute forward only, with dropout on the probabilities and gradients of q, k, v and
 of both position tables.  No ``[L, L]`` array and no mask outlives a call: the forward pass keeps its inputs, its result and one number for each row; the
-backward pass holds the scores' gradients of a few heads at a time (2 GiB, or one head if that has more: element size x sum of length x longest).
+backward pass holds the scores' gradients of a few heads at a time (2 GiB, or one head if that has more: element size x sum of length x longest), and
+with tables sums of up to half that size, or 96 MiB.
 The device work goes through ``tdb_attn_train_fwd`` and ``tdb_attn_train_bwd`` (include/tdb_train.h)."""
 from __future__ import annotations
 
