@@ -285,3 +285,27 @@ def test_attention_offsets_past_32_bits():
     assert all(torch.equal(a, b[0]) for a, b in zip(got, want))
     del big
     torch.cuda.empty_cache()
+
+
+def test_threads_with_streams_of_their_own():
+    """Two calls of every operator at once."""
+    import threading
+    want = {name: run(name, torch.bfloat16) for name in NAMES}
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(names):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for name in names:
+                got = run(name, torch.bfloat16)
+                stream.synchronize()
+                if not same(got, want[name]):
+                    wrong.append(name)
+
+    threads = [threading.Thread(target=work, args=(names,)) for names in (NAMES * 5, NAMES[::-1] * 5)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
