@@ -204,13 +204,19 @@ class FlashDisentangledSelfAttention(DisentangledSelfAttention):
     call is served by the eager parent class.
     ``trainable = True`` (``patch_model(model, training=True)``): a call in training mode, or one that autograd records, goes to
     ``ops.trainable_attention``, which has the gradient and, in training mode, the dropout of the probabilities
-    (modeling_deberta_v2.py:262); without it such a call has no gradient and drops nothing."""
+    (modeling_deberta_v2.py:262); without it such a call has no gradient and drops nothing.  Where ``dropout`` is no stock one, or has hooks, it has to be
+    run on the probabilities: the eager parent class serves such a call as well."""
 
     trainable = False
 
     def forward(self, hidden_states, attention_mask, output_attentions=False, query_states=None,
                 relative_pos=None, rel_embeddings=None):
-        if output_attentions:
+        watched = self.trainable and _training.operators_take(self, hidden_states) and not _training.is_dropout(self.dropout)
+        if output_attentions or watched:
+            if relative_pos is not None and not relative_pos.numel():        # (the encoder's stand-in for what fused layers do not read)
+                relative_pos = None
+            if watched and attention_mask is None:
+                attention_mask = hidden_states.new_ones(hidden_states.shape[0], 1, 1, hidden_states.shape[1])
             return super().forward(hidden_states, attention_mask, output_attentions, query_states,
                                    relative_pos, rel_embeddings)
         if query_states is None:

@@ -5,6 +5,9 @@ its attention to ``ops.trainable_attention``.  They add no parameters and no sta
 call the operators for tensors on the GPU in float32, bfloat16 or float16, which store no masks, no probabilities and nothing between
 dropout, residual and LayerNorm; everything else -- evaluation under ``torch.no_grad``, the CPU -- runs the parent class's code.
 
+An operator that takes the place of several modules runs none of them, so it does so only where they are what their classes say: a dropout or LayerNorm
+that has been replaced by another class's, or that has hooks or a ``forward`` of its own, is called (``stands_for``).
+
 Training mode under ``torch.no_grad`` counts as well: checkpointing of the reentrant kind runs a layer that way first and again with gradients, and
 both runs have to draw the same masks."""
 from __future__ import annotations
@@ -30,9 +33,22 @@ def draw_seed(module: nn.Module, device) -> torch.Tensor:
     return new_seed(device)
 
 
+def stands_for(module: nn.Module, *classes) -> bool:
+    """Whether an operator may stand for a call of ``module``: it is one of these classes and no subclass, with the ``forward`` that the class had when this
+    file was imported, and nobody watches the call."""
+    return (type(module) in classes and type(module).forward is _FORWARDS[type(module)] and "forward" not in module.__dict__ and module._compiled_call_impl is None
+            and not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks)
+            and not torch.nn.modules.module._has_any_global_hook())
+
+
+def is_dropout(drop: nn.Module) -> bool:
+    """Whether ``rate_of`` says all about a dropout: a stock one, or none (``nn.Identity``)."""
+    return stands_for(drop, nn.Dropout, FlashDropout, nn.Identity)
+
+
 def rate_of(module: nn.Module, drop: nn.Module) -> float:
     """The probability that ``drop``, a dropout of ``module``, drops a value with in the next call."""
-    return float(drop.p) if drop.training else 0.0
+    return float(drop.p) if isinstance(drop, nn.Dropout) and drop.training else 0.0
 
 
 class FlashDropout(nn.Dropout):
@@ -64,11 +80,14 @@ class FlashLayerNorm(nn.LayerNorm):
         return super().forward(x) if a is None else layer_norm(*a, self.eps)
 
 
+_FORWARDS = {c: c.forward for c in (nn.Dropout, nn.Identity, nn.LayerNorm, FlashDropout, FlashLayerNorm)}
+
+
 class _Output:
     """``LayerNorm(dropout(dense(x)) + input)`` (modeling_deberta_v2.py:42-53, :400-411) by ``ops.layer_norm.dropout_add_layer_norm``."""
 
     def forward(self, hidden_states, input_tensor):
-        if not operators_take(self, hidden_states, input_tensor):
+        if not (operators_take(self, hidden_states, input_tensor) and is_dropout(self.dropout) and stands_for(self.LayerNorm, nn.LayerNorm, FlashLayerNorm)):
             return super().forward(hidden_states, input_tensor)
         x = self.dense(hidden_states)
         wide = torch.promote_types(x.dtype, input_tensor.dtype)
