@@ -63,6 +63,7 @@ int64_t tdb_norm_workspace(int64_t rows, int32_t hidden);
  * sequence, are zeros in every result; what the inputs hold there does not matter.  workspace: tdb_attn_train_workspace() bytes for the same arguments, 16-byte aligned.  Besides a few bytes for each row and table it holds the scores' gradients of as many heads at a time as fit 2 GiB, at least one:
  * element size * sum of (length * max_seqlen), lengths rounded up to 64.  Where there are tables, also for each 64 x 64 of these scores 1 KiB, and sums by
  * relative position, up to 96 MiB or half as much as the scores' gradients in 16 bits.
+ * delta_lut, lut_half and span belong to the tables: without pos_key and pos_query they are not looked at.
  * The gradient of rows whose sequence has one token is zero in q, k and the tables.  Results must not overlap each other or an input.
  */
 typedef struct tdb_train_attn_args {

@@ -1,0 +1,40 @@
+"""Calls of the training operators' C side that the Python one does not make."""
+import ctypes as C
+
+import pytest
+import torch
+
+import turbodeberta_amd.ops.trainable_attention as T
+from turbodeberta_amd import _lib
+
+pytestmark = pytest.mark.gpu
+
+
+def random(*shape, dtype=torch.float32, n=0):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(n)).to(dtype).cuda()
+
+
+def attention(fields, dtype):
+    """Results and gradients of one call without tables, with these fields set."""
+    q, k, v, dout = (random(2, 3, 150, 32, dtype=dtype, n=n) for n in range(4))
+    o, dq, dk, dv = (torch.empty_like(q) for _ in range(4))
+    lse = torch.empty(3, 300, device="cuda")
+    a = T._args(q, k, v, o, None, lse, None, None, None, None, 150, 0.2, 0, 0, 0, None)
+    T._fill(a, dout=dout, dq=dq, dk=dk, dv=dv)
+    for name, x in fields.items():
+        setattr(a, name, x)
+    a.workspace_bytes = _lib.load().tdb_attn_train_workspace(C.byref(a))
+    work = torch.empty(a.workspace_bytes, dtype=torch.uint8, device="cuda")
+    a.workspace = work.data_ptr()
+    stream = torch.cuda.current_stream().cuda_stream
+    _lib.check(_lib.load().tdb_attn_train_fwd(C.byref(a), stream))
+    _lib.check(_lib.load().tdb_attn_train_bwd(C.byref(a), stream))
+    return o, lse, dq, dk, dv
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_a_tables_fields_without_tables_change_nothing(dtype):
+    lut = torch.arange(4096, dtype=torch.int32, device="cuda")
+    want = attention({}, dtype)
+    for fields in ({"delta_lut": lut.data_ptr(), "lut_half": 2047}, {"delta_lut": lut.data_ptr(), "lut_half": 0, "span": -5}):
+        assert all(torch.equal(a, b) for a, b in zip(attention(fields, dtype), want))

@@ -1030,6 +1030,9 @@ int64_t up(int64_t x) { return (x + 255) / 256 * 256; }
 constexpr int64_t MOST_STRIDE = int64_t(1) << 24;        // bytes: 64 rows' offsets fit 31 bits
 constexpr int64_t MOST_SCORES = int64_t(2) << 30;        // bytes of dS at a time, unless one head has more (4 x 4096, 12 heads: 3.1 ms with 512 MiB, 2.8)
 
+// Whether there are position terms; without them the table's fields mean nothing and are not looked at.
+bool has_terms(const tdb_train_attn_args& a) { return a.pos_key || a.pos_query; }
+
 // What a backward call needs, and how many heads it takes at a time.
 struct Plan {
     int tiles, row_tiles, split_bits, seg_bits, heads;
@@ -1052,9 +1055,9 @@ Plan plan_of(const tdb_train_attn_args& a) {
     while (p.split_bits < bits && (2 << p.split_bits) <= a.batch) ++p.split_bits;
     p.seg_bits = bits - p.split_bits;
     p.starts = 256;                                 // in front: the two maxima and the diagonals of level tiles
-    p.delta = p.starts + up((2 * int64_t(a.span) + 1) * 4);
+    const bool terms = has_terms(a);
+    p.delta = p.starts + (terms ? up((2 * int64_t(a.span) + 1) * 4) : 0);
     p.level = p.delta + up(p.lines * a.heads * 4);
-    const bool terms = a.pos_key || a.pos_query;
     p.partial = p.level + (terms ? int64_t(2) * p.heads * p.row_tiles * 2 * 64 * 4 : 0);
     p.sums = p.partial + (terms ? ((int64_t(p.heads) * diagonals) << (bits + 1)) * BY_OFFSET * 64 * 4 : 0);
     p.ds = p.sums + (terms ? int64_t(p.heads) * p.row_tiles * p.tiles * ROW_SUMS * 4 : 0);
@@ -1076,6 +1079,7 @@ int check(const tdb_train_attn_args* a, bool backward, bool sizes_only = false) 
     const int64_t lines = a->cu_seqlens ? a->total_tokens : int64_t(a->batch) * a->max_seqlen;
     if (lines * a->heads > (1 << 28) || (lines / TILE + a->batch) * a->heads >= (1 << 24))       // (of the launches' sizes)
         return tdb_fail(TDB_ERR_SHAPE, "%lld rows of %d heads: need 2^28 at most", (long long)lines, a->heads);
+    if (has_terms(*a) && (a->span < 1 || a->span > (1 << 20))) return tdb_fail(TDB_ERR_POSITION, "span %d out of range", a->span);
     if (sizes_only || a->batch == 0 || lines == 0) return TDB_OK;
     if (!a->q || !a->k || !a->v || !a->o || !a->lse || (backward && (!a->dout || !a->dq || !a->dk || !a->dv || !a->workspace)))
         return tdb_fail(TDB_ERR_NULL, "a required pointer is NULL");
@@ -1097,8 +1101,7 @@ int check(const tdb_train_attn_args* a, bool backward, bool sizes_only = false) 
     const int64_t table[] = {a->pos_key_stride_h, a->pos_key_stride_r, a->pos_query_stride_h, a->pos_query_stride_r};
     for (int64_t s : table)
         if (s < 0 || s * int64_t(elem(a->dtype)) % 16) return tdb_fail(TDB_ERR_STRIDE, "strides of the tables must be non-negative multiples of 16 bytes");
-    if (a->pos_key || a->pos_query) {
-        if (a->span < 1 || a->span > (1 << 20)) return tdb_fail(TDB_ERR_POSITION, "span %d out of range", a->span);
+    if (has_terms(*a)) {
         if (2 * int64_t(a->span) * std::max(a->pos_key ? a->pos_key_stride_r : 0, a->pos_query ? a->pos_query_stride_r : 0) * int64_t(elem(a->dtype)) > INT32_MAX)
             return tdb_fail(TDB_ERR_STRIDE, "a head's table must lie within 2 GiB");
         if (!a->delta_lut || a->lut_half < a->max_seqlen - 1) return tdb_fail(TDB_ERR_POSITION, "delta_lut is missing or shorter than the sequences");
@@ -1124,7 +1127,7 @@ Args args_of(const tdb_train_attn_args& a, const Plan& p) {
     k.dv = {a.dv, a.dv_stride_b, a.dv_stride_h, a.dv_stride_l};
     k.pk = {const_cast<void*>(a.pos_key), 0, a.pos_key_stride_h, a.pos_key_stride_r};
     k.pq = {const_cast<void*>(a.pos_query), 0, a.pos_query_stride_h, a.pos_query_stride_r};
-    k.lut = a.delta_lut, k.lut_half = a.lut_half, k.span = a.span;
+    if (has_terms(a)) k.lut = a.delta_lut, k.lut_half = a.lut_half, k.span = a.span;
     k.seqlens = a.seqlens_k, k.cu = a.cu_seqlens;
     k.B = a.batch, k.H = a.heads, k.D = a.head_dim, k.L = a.max_seqlen, k.total = a.total_tokens;
     k.head0 = 0, k.heads = a.heads;
