@@ -24,3 +24,12 @@ def test_a_bad_span_needs_no_workspace():
     assert workspace() > 0
     for span in (0, -1, (1 << 20) + 1):
         assert workspace(span=span) == workspace(span=span, pos_key=None) == 0
+
+
+@pytest.mark.parametrize("total", [1, 63, 200, 5000])
+def test_a_loose_bound_of_packed_lengths_costs_no_workspace(total):
+    tight = workspace(cu_seqlens=4096, total_tokens=total, max_seqlen=total, lut_half=1 << 20)
+    for loose in (total + 1, 32768, 1 << 20):
+        assert workspace(cu_seqlens=4096, total_tokens=total, max_seqlen=loose, lut_half=1 << 20) == tight > 0
+    if total > 64:
+        assert workspace(cu_seqlens=4096, total_tokens=total, max_seqlen=64, lut_half=1 << 20) < tight

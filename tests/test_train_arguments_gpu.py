@@ -4,6 +4,7 @@ import ctypes as C
 import pytest
 import torch
 
+from test_train_attention_gpu import TYPES, Case
 import turbodeberta_amd.ops.trainable_attention as T
 from turbodeberta_amd import _lib
 
@@ -32,9 +33,19 @@ def attention(fields, dtype):
     return o, lse, dq, dk, dv
 
 
-@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dtype", TYPES)
 def test_a_tables_fields_without_tables_change_nothing(dtype):
     lut = torch.arange(4096, dtype=torch.int32, device="cuda")
     want = attention({}, dtype)
     for fields in ({"delta_lut": lut.data_ptr(), "lut_half": 2047}, {"delta_lut": lut.data_ptr(), "lut_half": 0, "span": -5}):
         assert all(torch.equal(a, b) for a, b in zip(attention(fields, dtype), want))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_loose_bound_of_packed_lengths_changes_nothing(dtype):
+    c = Case([100, 0, 70], dtype=dtype, p=0.1, seed=31)
+    tight = c.packed(170)
+    for loose in (171, 5000, 1 << 17):
+        got = c.packed(loose)
+        assert all(torch.equal(got[n], tight[n]) for n in tight)
+    c.check(tight)

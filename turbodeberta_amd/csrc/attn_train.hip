@@ -1033,6 +1033,9 @@ constexpr int64_t MOST_SCORES = int64_t(2) << 30;        // bytes of dS at a tim
 // Whether there are position terms; without them the table's fields mean nothing and are not looked at.
 bool has_terms(const tdb_train_attn_args& a) { return a.pos_key || a.pos_query; }
 
+// No sequence of a packing is longer than all its tokens, whatever bound the caller gives.
+int longest_of(const tdb_train_attn_args& a) { return a.cu_seqlens ? std::max(1, std::min(a.max_seqlen, a.total_tokens)) : a.max_seqlen; }
+
 // What a backward call needs, and how many heads it takes at a time.
 struct Plan {
     int tiles, row_tiles, split_bits, seg_bits, heads;
@@ -1040,7 +1043,7 @@ struct Plan {
 };
 Plan plan_of(const tdb_train_attn_args& a) {
     Plan p;
-    p.tiles = (a.max_seqlen + TILE - 1) / TILE;
+    p.tiles = (longest_of(a) + TILE - 1) / TILE;
     p.row_tiles = a.cu_seqlens ? a.total_tokens / TILE + a.batch : a.batch * p.tiles;
     p.lines = a.cu_seqlens ? a.total_tokens : int64_t(a.batch) * a.max_seqlen;
     const int64_t each = int64_t(p.row_tiles) * p.tiles * TILE_VALUES * int64_t(elem(a.dtype));
@@ -1129,13 +1132,13 @@ Args args_of(const tdb_train_attn_args& a, const Plan& p) {
     k.pq = {const_cast<void*>(a.pos_query), 0, a.pos_query_stride_h, a.pos_query_stride_r};
     if (has_terms(a)) k.lut = a.delta_lut, k.lut_half = a.lut_half, k.span = a.span;
     k.seqlens = a.seqlens_k, k.cu = a.cu_seqlens;
-    k.B = a.batch, k.H = a.heads, k.D = a.head_dim, k.L = a.max_seqlen, k.total = a.total_tokens;
+    k.B = a.batch, k.H = a.heads, k.D = a.head_dim, k.L = longest_of(a), k.total = a.total_tokens;
     k.head0 = 0, k.heads = a.heads;
     k.lines = p.lines, k.lse = a.lse, k.rest = a.dtype == TDB_F32 ? nullptr : a.o_rest;
     k.tiles = p.tiles, k.row_tiles = p.row_tiles, k.split_bits = p.split_bits, k.seg_bits = p.seg_bits, k.per_tile = 65536 / p.tiles + 1;
     k.dpk = a.dpos_key, k.dpq = a.dpos_query, k.dpk_h = a.dpos_key_stride_h, k.dpq_h = a.dpos_query_stride_h;
     k.seed = a.seed, k.threshold = uint32_t(a.threshold), k.factor = tdb_kept_factor(a.threshold), k.scale = a.sm_scale;
-    while (k.p_shift < 15 && (2 << k.p_shift) <= a.max_seqlen) ++k.p_shift;
+    while (k.p_shift < 15 && (2 << k.p_shift) <= k.L) ++k.p_shift;
     if (a.workspace) {
         char* const at = static_cast<char*>(a.workspace);
         k.largest = reinterpret_cast<const uint32_t*>(at);
