@@ -60,9 +60,10 @@ int64_t tdb_norm_workspace(int64_t rows, int32_t hidden);
  * call, which also reads o.  In 16 bits o_rest, [heads, rows, head_dim] back to back, takes what rounding took from o and goes to the backward call with it; NULL in both calls:
  * the gradients are made from o as it is rounded, and are the less exact the longer the rows.
  * Backward writes dq, dk, dv and the gradients of the tables, [heads, 2 span, head_dim] with rows back to back.  Rows beyond a sequence's length, and packed rows of no
- * sequence, are zeros in every result; what the inputs hold there does not matter.  workspace: tdb_attn_train_workspace() bytes for the same arguments, 16-byte aligned.  Besides a few bytes for each row and table it holds the scores' gradients of as many heads at a time as fit 2 GiB, at least one:
- * element size * sum of (length * max_seqlen), lengths rounded up to 64 and max_seqlen at most total_tokens where packed.  Where there are tables, also for each 64 x 64 of these scores 1 KiB, and sums by
- * relative position, up to 96 MiB or half as much as the scores' gradients in 16 bits.
+ * sequence, are zeros in every result; what the inputs hold there does not matter.  workspace: tdb_attn_train_workspace() bytes for the same arguments, 16-byte aligned.  Besides a few bytes for each row and table
+ * it holds, for as many heads at a time as fit (at least one), the scores' gradients in 2 GiB: element size * sum of (length * max_seqlen), lengths rounded up to 64 and max_seqlen
+ * at most total_tokens where packed; and where there are tables, in 2 GiB as well, 1 KiB for each 64 x 64 of these scores and sums by relative position: at most the largest of half
+ * the scores' gradients in 16 bits, 96 MiB, and 128 KiB for each of these heads and 64 tokens of max_seqlen.
  * delta_lut, lut_half and span belong to the tables: without pos_key and pos_query they are not looked at.
  * The gradient of rows whose sequence has one token is zero in q, k and the tables.  Results must not overlap each other or an input.
  */

@@ -33,3 +33,30 @@ def test_a_loose_bound_of_packed_lengths_costs_no_workspace(total):
         assert workspace(cu_seqlens=4096, total_tokens=total, max_seqlen=loose, lut_half=1 << 20) == tight > 0
     if total > 64:
         assert workspace(cu_seqlens=4096, total_tokens=total, max_seqlen=64, lut_half=1 << 20) < tight
+
+
+def documented(batch, heads, max_seqlen, dtype):
+    """The largest workspace that tdb_train.h speaks of for a padded batch, `few` bytes for each row and table included."""
+    size, tiles = 4 if dtype == _lib.TDB_F32 else 2, -(-max_seqlen // 64)
+    each = batch * tiles * tiles * 64 * 64
+    gib2, kib = 2 << 30, 1 << 10
+    at_once = max(1, min(heads, gib2 // (each * size)))
+    scores = at_once * each * size
+    sums = max(at_once * each, 96 * kib * kib, at_once * tiles * 128 * kib)
+    one = max(each, tiles * 128 * kib) + each // 4
+    few = 32 * batch * tiles * 64 * heads + 17 * 8 + 4 * kib
+    return scores + min(sums + at_once * each // 4, max(gib2, one)) + few
+
+
+@pytest.mark.parametrize("dtype", [_lib.TDB_F32, _lib.TDB_BF16])
+@pytest.mark.parametrize("batch,heads,max_seqlen", [(1, 64, 1024), (1, 12, 29), (32, 12, 512), (4, 12, 4096), (1, 65535, 64), (1, 4096, 700), (300, 40, 64), (1, 16, 1 << 15), (1000, 1, 1000),
+                                                    (3, 2, 4096), (1, 1, 4160), (2, 1000, 1), (70, 300, 130)])
+def test_the_documented_bounds(batch, heads, max_seqlen, dtype):
+    need = workspace(batch=batch, heads=heads, max_seqlen=max_seqlen, lut_half=1 << 20, dtype=dtype)
+    assert 0 < need <= documented(batch, heads, max_seqlen, dtype)
+
+
+def test_many_heads_sums_come_in_rounds():
+    """One tile for each of 65535 heads: 8 KiB of scores, 64 KiB of sums by relative position."""
+    need = workspace(batch=1, heads=65535, max_seqlen=64, lut_half=1 << 20)
+    assert need < 2.4 * 2 ** 30

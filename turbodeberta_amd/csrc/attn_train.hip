@@ -1028,7 +1028,7 @@ size_t elem(int dtype) { return dtype == TDB_F32 ? 4 : 2; }
 int64_t up(int64_t x) { return (x + 255) / 256 * 256; }
 
 constexpr int64_t MOST_STRIDE = int64_t(1) << 24;        // bytes: 64 rows' offsets fit 31 bits
-constexpr int64_t MOST_SCORES = int64_t(2) << 30;        // bytes of dS at a time, unless one head has more (4 x 4096, 12 heads: 3.1 ms with 512 MiB, 2.8)
+constexpr int64_t MOST_SCORES = int64_t(2) << 30;        // bytes of dS, and of the positions' sums, at a time, unless one head has more (4 x 4096, 12 heads: 3.1 ms with 512 MiB, 2.8)
 
 // Whether there are position terms; without them the table's fields mean nothing and are not looked at.
 bool has_terms(const tdb_train_attn_args& a) { return a.pos_key || a.pos_query; }
@@ -1047,22 +1047,25 @@ Plan plan_of(const tdb_train_attn_args& a) {
     p.row_tiles = a.cu_seqlens ? a.total_tokens / TILE + a.batch : a.batch * p.tiles;
     p.lines = a.cu_seqlens ? a.total_tokens : int64_t(a.batch) * a.max_seqlen;
     const int64_t each = int64_t(p.row_tiles) * p.tiles * TILE_VALUES * int64_t(elem(a.dtype));
-    p.heads = int(std::max<int64_t>(1, std::min<int64_t>(a.heads, MOST_SCORES / std::max<int64_t>(each, 1))));
+    const bool terms = has_terms(a);
     const int diagonals = 2 * p.tiles - 1;
+    int least = 0;                                  // parts of a long diagonal, see below
+    while (least < 12 && p.row_tiles >> least > 64) ++least;
+    const int64_t part = BY_OFFSET * 64 * 4, sums = terms ? ((int64_t(diagonals) << (least + 1)) * part) + int64_t(p.row_tiles) * (p.tiles * ROW_SUMS * 4 + 1024) : 0;
+    p.heads = int(std::max<int64_t>(1, std::min<int64_t>(a.heads, MOST_SCORES / std::max<int64_t>({each, sums, 1}))));
     // A diagonal's parts, a power of two: three workgroups for each of 256 CUs where every diagonal has its own sums, and 64 tiles for a workgroup where most are level
     // (4 x 4096: 281 us and 32 for the sums; with 32 tiles 230 and 54, for sums of half of dS's size).
     int bits = 0;
     while ((int64_t(2) << bits) * p.heads * p.tiles <= 768 && (2 << bits) <= a.batch) ++bits;
-    while (bits < 12 && p.row_tiles >> bits > 64) ++bits;
+    bits = std::max(bits, least);
     p.split_bits = 0;
     while (p.split_bits < bits && (2 << p.split_bits) <= a.batch) ++p.split_bits;
     p.seg_bits = bits - p.split_bits;
     p.starts = 256;                                 // in front: the two maxima and the diagonals of level tiles
-    const bool terms = has_terms(a);
     p.delta = p.starts + (terms ? up((2 * int64_t(a.span) + 1) * 4) : 0);
     p.level = p.delta + up(p.lines * a.heads * 4);
     p.partial = p.level + (terms ? int64_t(2) * p.heads * p.row_tiles * 2 * 64 * 4 : 0);
-    p.sums = p.partial + (terms ? ((int64_t(p.heads) * diagonals) << (bits + 1)) * BY_OFFSET * 64 * 4 : 0);
+    p.sums = p.partial + (terms ? ((int64_t(p.heads) * diagonals) << (bits + 1)) * part : 0);
     p.ds = p.sums + (terms ? int64_t(p.heads) * p.row_tiles * p.tiles * ROW_SUMS * 4 : 0);
     p.bytes = p.ds + p.heads * each;
     return p;

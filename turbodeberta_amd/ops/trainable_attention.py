@@ -1,9 +1,10 @@
 """Disentangled attention with its gradient, for training: padded batches and packed sequences.
 
 What ``ops.flash_attention`` and ``ops.flash_attention_varlen`` compute forward only, with dropout on the probabilities and gradients of q, k, v and
-of both position tables.  No ``[L, L]`` array and no mask outlives a call: the forward pass keeps its inputs, its result and one number for each row; the
-backward pass holds the scores' gradients of a few heads at a time (2 GiB, or one head if that has more: element size x sum of length x longest), and
-with tables sums of up to half that size, or 96 MiB.
+of both position tables.  No ``[L, L]`` array and no mask outlives a call: the forward pass keeps its inputs, its result, one number for each row and, in 16
+bits, what rounding took from the result, as much again; the backward pass holds the scores' gradients of a few heads at a time (2 GiB, or one head
+if that has more: element size x sum of length x longest), and with tables sums by relative position: up to half that size, 96 MiB, or 128 KiB for each of the
+heads and 64 tokens of the longest sequence, and no more than 2 GiB unless one head has.
 The device work goes through ``tdb_attn_train_fwd`` and ``tdb_attn_train_bwd`` (include/tdb_train.h)."""
 from __future__ import annotations
 
