@@ -64,6 +64,8 @@ int64_t tdb_norm_workspace(int64_t rows, int32_t hidden);
  * it holds, for as many heads at a time as fit (at least one), the scores' gradients in 2 GiB: element size * sum of (length * max_seqlen), lengths rounded up to 64 and max_seqlen
  * at most total_tokens where packed; and where there are tables, in 2 GiB as well, 1 KiB for each 64 x 64 of these scores and sums by relative position: at most the largest of half
  * the scores' gradients in 16 bits, 96 MiB, and 128 KiB for each of these heads and 64 tokens of max_seqlen.
+ * delta_lut must not fall as the relative position rises, from 1 - max_seqlen to max_seqlen - 1 (max_seqlen: at most total_tokens where packed): the gradients' sums are made by runs
+ * of positions that share a row.  tdb_delta_table's rows fall where max_position - 1 <= position_buckets / 2, beyond position_buckets / 2 + 1 tokens.
  * delta_lut, lut_half and span belong to the tables: without pos_key and pos_query they are not looked at.
  * The gradient of rows whose sequence has one token is zero in q, k and the tables.  Results must not overlap each other or an input.
  */

@@ -1,10 +1,13 @@
 """Arguments of the training operators' C side, and what it asks for as workspace."""
 import ctypes as C
 
+import numpy as np
 import pytest
+import torch
 
 from test_train_cpu import _attention
 from turbodeberta_amd import _lib
+from turbodeberta_amd.ops import _launch
 
 
 def workspace(**kw):
@@ -60,3 +63,18 @@ def test_many_heads_sums_come_in_rounds():
     """One tile for each of 65535 heads: 8 KiB of scores, 64 KiB of sums by relative position."""
     need = workspace(batch=1, heads=65535, max_seqlen=64, lut_half=1 << 20)
     assert need < 2.4 * 2 ** 30
+
+
+@pytest.mark.parametrize("buckets,max_rel,longest", [(256, 512, None), (0, 64, None), (256, 130, None), (8, 6, None), (256, 129, 129), (256, 64, 129), (32, 16, 17), (32, 17, 17), (4, 3, 3)])
+def test_buckets_that_run_backwards_are_refused(buckets, max_rel, longest):
+    """Where max_rel - 1 <= buckets / 2 the logarithm's sign turns: rows are met again, and no run of positions has them."""
+    table = _lib.delta_table(512, buckets, max_rel).astype(int)
+    falls = lambda l: (np.diff(table[511 - (l - 1):511 + l]) < 0).any()
+    device = torch.device("cpu")
+    _launch.require_rising(device, 512, longest or 512, buckets, max_rel)
+    assert not falls(longest or 512)
+    if longest:
+        assert falls(longest + 1)
+        for reach in (longest + 1, 300):
+            with pytest.raises(ValueError, match=f"run backwards.* up to {longest} tokens"):
+                _launch.require_rising(device, 512, reach, buckets, max_rel)

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from test_train_attention_gpu import TYPES, Case
+from test_train_paths_gpu import python_path  # noqa: F401
 import turbodeberta_amd.ops.trainable_attention as T
 from turbodeberta_amd import _lib
 
@@ -49,3 +50,18 @@ def test_a_loose_bound_of_packed_lengths_changes_nothing(dtype):
         got = c.packed(loose)
         assert all(torch.equal(got[n], tight[n]) for n in tight)
     c.check(tight)
+
+
+@pytest.mark.parametrize("path", ["native", "python"])
+def test_buckets_that_run_backwards(path, python_path):  # noqa: F811
+    """Taken where no sequence is long enough to meet them, refused else."""
+    if path == "python":
+        python_path()
+    c = Case([129, 40], dtype=torch.float32, buckets=256, max_rel=129, p=0.1, seed=32)
+    c.check(c.packed(129))
+    c.check(c.unpad(c.padded(129), 129))
+    short = Case([40, 60], buckets=256, max_rel=129, seed=33)
+    short.check(short.packed(1000))                     # 100 tokens in all
+    for refused in (lambda: c.packed(130), lambda: c.padded(130), lambda: c.packed(5000)):
+        with pytest.raises(ValueError, match="up to 129 tokens"):
+            refused()

@@ -35,7 +35,7 @@ int (*g_varlen)(const tdb_varlen_args*, void*) = nullptr;
 // as many as the Python cache holds).
 struct Lut {
     int device;
-    int64_t size, buckets, max_rel;
+    int64_t size, buckets, max_rel, rising;     // rising: the longest length whose rows do not fall
     at::Tensor table;
 };
 std::vector<Lut>& luts() {
@@ -292,17 +292,17 @@ PyObject* py_bind(PyObject*, PyObject* args) {
     Py_RETURN_NONE;
 }
 
-// add_lut(table, size, position_buckets, max_relative_distance): a device table to be found by later calls
+// add_lut(table, size, position_buckets, max_relative_distance, rising length): a device table to be found by later calls
 PyObject* py_add_lut(PyObject*, PyObject* args) {
     PyObject* t;
-    long long size, buckets, max_rel;
-    if (!PyArg_ParseTuple(args, "OLLL", &t, &size, &buckets, &max_rel)) return nullptr;
+    long long size, buckets, max_rel, rising;
+    if (!PyArg_ParseTuple(args, "OLLLL", &t, &size, &buckets, &max_rel, &rising)) return nullptr;
     if (!THPVariable_Check(t)) {
         PyErr_SetString(PyExc_TypeError, "add_lut: a tensor is expected");
         return nullptr;
     }
     const at::Tensor& table = THPVariable_Unpack(t);
-    luts().push_back(Lut{table.device().index(), size, buckets, max_rel, table});
+    luts().push_back(Lut{table.device().index(), size, buckets, max_rel, rising, table});
     Py_RETURN_NONE;
 }
 
@@ -336,9 +336,9 @@ bool tdb_host_rows_ok(const at::Tensor& t) { return rows_ok(t); }
 
 bool tdb_host_output_like(const at::Tensor& q, at::Tensor& o) { return output_like(q, o); }
 
-const at::Tensor* tdb_host_lut(int64_t buckets, int64_t max_rel, int64_t max_len, int device) {
+const at::Tensor* tdb_host_lut(int64_t buckets, int64_t max_rel, int64_t max_len, int64_t reach, int device) {
     const Lut* l = find_lut(buckets, max_rel, max_len, device);
-    return l ? &l->table : nullptr;
+    return l && reach <= l->rising ? &l->table : nullptr;
 }
 
 bool tdb_host_observed() { return c10::impl::dispatch_mode_enabled() || at::tracer::impl::is_dispatch_enabled(); }

@@ -28,8 +28,8 @@ bool tdb_host_rows_ok(const at::Tensor& t);
 // A tensor like q: q's strides where q is dense, the dense strides of the same dimension order otherwise; false where its rows are none of those.
 bool tdb_host_output_like(const at::Tensor& q, at::Tensor& o);
 
-// The device's delta table of sequences up to max_len, null where none is at hand.
-const at::Tensor* tdb_host_lut(int64_t buckets, int64_t max_rel, int64_t max_len, int device);
+// The device's delta table of sequences up to max_len, null where none is at hand or where rows of relative positions below `reach` fall.
+const at::Tensor* tdb_host_lut(int64_t buckets, int64_t max_rel, int64_t max_len, int64_t reach, int device);
 
 bool tdb_host_add_encoder(PyObject* module);
 bool tdb_host_add_train(PyObject* module);

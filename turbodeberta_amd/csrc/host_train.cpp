@@ -405,7 +405,7 @@ PyObject* py_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         Tensor lut;
         const int64_t span = buckets > 0 ? buckets : max_rel;
         if (pk.defined() || pq.defined()) {
-            const Tensor* table = span < 1 ? nullptr : tdb_host_lut(buckets, max_rel, longest, q.device().index());
+            const Tensor* table = span < 1 ? nullptr : tdb_host_lut(buckets, max_rel, longest, cu.defined() ? std::min(longest, q.size(0)) : longest, q.device().index());
             if (!table) return Tensor();
             lut = *table;
         }

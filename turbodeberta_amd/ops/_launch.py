@@ -15,6 +15,7 @@ _DTYPES = {torch.float32: _lib.TDB_F32, torch.bfloat16: _lib.TDB_BF16, torch.flo
 
 _lut_lock = threading.Lock()
 _lut_cache: dict = {}
+_rising: dict = {}
 
 
 def dtype_code(t: torch.Tensor) -> int:
@@ -30,13 +31,18 @@ def att_span(position_buckets: int, max_relative_distance: int) -> int:
     return position_buckets if position_buckets > 0 else max_relative_distance
 
 
-def delta_lut(device: torch.device, max_len: int, position_buckets: int, max_relative_distance: int):
-    """Device int32 table of delta(r) for |r| < half+1, and its half-width.  Built on the host by
-    tdb_delta_table once per (device, size class, bucket configuration) and then reused."""
+def _lut_key(device: torch.device, max_len: int, position_buckets: int, max_relative_distance: int):
     size = 512
     while size < max_len:
         size *= 2
-    key = (device.type, device.index, size, int(position_buckets), int(max_relative_distance))
+    return (device.type, device.index, size, int(position_buckets), int(max_relative_distance))
+
+
+def delta_lut(device: torch.device, max_len: int, position_buckets: int, max_relative_distance: int):
+    """Device int32 table of delta(r) for |r| < half+1, and its half-width.  Built on the host by
+    tdb_delta_table once per (device, size class, bucket configuration) and then reused."""
+    key = _lut_key(device, max_len, position_buckets, max_relative_distance)
+    size = key[2]
     hit = _lut_cache.get(key)
     if hit is not None:
         return hit
@@ -44,11 +50,29 @@ def delta_lut(device: torch.device, max_len: int, position_buckets: int, max_rel
         hit = _lut_cache.get(key)
         if hit is None:
             table = torch.from_numpy(_lib.delta_table(size, int(position_buckets), int(max_relative_distance)))
+            _rising[key] = rising = rising_length(table)
             hit = (table.to(device), size - 1)
             _lut_cache[key] = hit
             if device.type == "cuda":
-                _lib.host().add_lut(hit[0], size, int(position_buckets), int(max_relative_distance))
+                _lib.host().add_lut(hit[0], size, int(position_buckets), int(max_relative_distance), rising)
     return hit
+
+
+def rising_length(table: torch.Tensor) -> int:
+    """The longest length whose relative positions' table rows do not fall as the positions rise.  All of the table's, but for logarithmic buckets that
+    run backwards: where max_relative_distance - 1 <= position_buckets / 2, beyond position_buckets / 2 + 1 tokens."""
+    half = table.numel() // 2
+    falls = (table[1:] < table[:-1]).nonzero().flatten() - half             # from relative position r to r + 1
+    return min([half + 1] + [max(abs(r), abs(r + 1)) for r in falls.tolist()])
+
+
+def require_rising(device: torch.device, max_len: int, reach: int, position_buckets: int, max_relative_distance: int) -> None:
+    """Raises where table rows of relative positions below ``reach`` fall: the gradients' sums are made by runs of positions that share a row."""
+    delta_lut(device, max_len, position_buckets, max_relative_distance)
+    most = _rising[_lut_key(device, max_len, position_buckets, max_relative_distance)]
+    if reach > most:
+        raise ValueError(f"position_buckets={position_buckets} with max_relative_distance={max_relative_distance}: the buckets run backwards; the training operators take sequences of up "
+                         f"to {most} tokens, got {reach}")
 
 
 def require_gpu(*tensors) -> torch.device:

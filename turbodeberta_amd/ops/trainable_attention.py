@@ -112,8 +112,8 @@ class _Attention(torch.autograd.Function):
         return (dq, dk, dv, *tables) + (None,) * (3 + len(ctx.plain))
 
 
-def _checked(q, k, v, pos_key_layer, pos_query_layer, heads, sm_scale, buckets, max_rel, p, seed, others):
-    """(sm_scale, tables, threshold, seed) of a call whose q, k, v have been looked at by themselves."""
+def _checked(q, k, v, pos_key_layer, pos_query_layer, heads, sm_scale, buckets, max_rel, p, seed, longest, reach, others):
+    """(sm_scale, tables, threshold, seed) of a call whose q, k, v have been looked at by themselves.  reach: what no sequence is longer than."""
     threshold = L.drop_threshold(p)
     seed = L.one_seed(seed) if threshold else None
     L.require_gpu(q, k, v, pos_key_layer, pos_query_layer, seed, *others)
@@ -139,6 +139,8 @@ def _checked(q, k, v, pos_key_layer, pos_query_layer, heads, sm_scale, buckets, 
             if t.dim() != 3 or t.shape[0] != heads or t.shape[2] != D or t.shape[1] < 2 * span:
                 raise ValueError(f"{name}: expected [H={heads}, >=2*span={2 * span}, D={D}], got {tuple(t.shape)}")
         tables.append(t)
+    if longest <= 1 << 20 and not all(t is None for t in tables):        # (the C side refuses longer ones)
+        L.require_rising(q.device, longest, reach, buckets, max_rel)
     return scale, tables, threshold, seed
 
 
@@ -150,7 +152,8 @@ def trainable_attention_with_disentangled(q, k, v, pos_key_layer: Optional[torch
     q, k, v : ``[B, H, L, D]``, float32, bfloat16 or float16, D a multiple of 8 up to 64; any strides with a contiguous last dimension and rows at
         multiples of 16 bytes (others are copied).  The result has q's shape and strides.
     pos_key_layer, pos_query_layer : ``[H, >= 2*span, D]`` (or with a leading 1) projections of the relative embeddings, or None; indexed as in
-        ``ops.flash_attention.flash_attention_with_disentangled``, as are position_buckets and max_relative_distance.
+        ``ops.flash_attention.flash_attention_with_disentangled``, as are position_buckets and max_relative_distance.  (Buckets that run backwards, max_relative_distance - 1 <=
+        position_buckets / 2, are refused beyond position_buckets / 2 + 1 tokens.)
     sm_scale : positive; None means ``1/sqrt(D)``.
     seqlens_k : int32 ``[B]`` valid lengths of right-padded sequences.  Rows beyond are zeros in the result and in every gradient; what the inputs and
         the result's gradient hold there is not read.
@@ -163,13 +166,14 @@ def trainable_attention_with_disentangled(q, k, v, pos_key_layer: Optional[torch
         return o
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
         raise ValueError("q, k, v must be [B, H, L, D]")
+    longest = max(q.shape[2], 1)
     scale, (pk, pq), threshold, seed = _checked(q, k, v, pos_key_layer, pos_query_layer, q.shape[1], sm_scale, position_buckets, max_relative_distance,
-                                                dropout_p, seed, (seqlens_k,))
+                                                dropout_p, seed, longest, longest, (seqlens_k,))
     if seqlens_k is not None:
         if seqlens_k.shape != q.shape[:1]:
             raise ValueError(f"seqlens_k must be [B={q.shape[0]}], got {tuple(seqlens_k.shape)}")
         seqlens_k = seqlens_k.to(torch.int32).contiguous()
-    return _Attention.apply(q, k, v, pk, pq, seqlens_k, None, seed, max(q.shape[2], 1), scale, int(position_buckets), int(max_relative_distance), threshold)
+    return _Attention.apply(q, k, v, pk, pq, seqlens_k, None, seed, longest, scale, int(position_buckets), int(max_relative_distance), threshold)
 
 
 def trainable_attention_with_disentangled_varlen(q, k, v, pos_key_layer: Optional[torch.Tensor], pos_query_layer: Optional[torch.Tensor],
@@ -186,7 +190,8 @@ def trainable_attention_with_disentangled_varlen(q, k, v, pos_key_layer: Optiona
         raise ValueError("q, k, v must be [total_tokens, H, D]")
     if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
         raise ValueError("cu_seqlens must be a 1-D tensor of B+1 offsets")
+    longest = max(int(max_seqlen), 1)
     scale, (pk, pq), threshold, seed = _checked(q, k, v, pos_key_layer, pos_query_layer, q.shape[1], sm_scale, position_buckets, max_relative_distance,
-                                                dropout_p, seed, (cu_seqlens,))
-    return _Attention.apply(q, k, v, pk, pq, None, cu_seqlens.to(torch.int32).contiguous(), seed, max(int(max_seqlen), 1), scale, int(position_buckets),
+                                                dropout_p, seed, longest, min(longest, q.shape[0]), (cu_seqlens,))
+    return _Attention.apply(q, k, v, pk, pq, None, cu_seqlens.to(torch.int32).contiguous(), seed, longest, scale, int(position_buckets),
                             int(max_relative_distance), threshold)
