@@ -7,7 +7,7 @@ import torch
 
 from test_train_cpu import _attention
 from turbodeberta_amd import _lib
-from turbodeberta_amd.ops import _launch
+from turbodeberta_amd.ops import _launch, trainable_attention
 
 
 def workspace(**kw):
@@ -78,3 +78,27 @@ def test_buckets_that_run_backwards_are_refused(buckets, max_rel, longest):
         for reach in (longest + 1, 300):
             with pytest.raises(ValueError, match=f"run backwards.* up to {longest} tokens"):
                 _launch.require_rising(device, 512, reach, buckets, max_rel)
+
+
+def odd_tensors():
+    """Contiguous, and nothing that the kernels can address: at an odd address; single rows with strides of no size."""
+    yield torch.randn(2 * 3 * 5 * 8 + 1)[1:].view(2, 3, 5, 8)
+    yield torch.randn(64).as_strided((2, 3, 1, 8), (24, 8, 0, 1))
+    yield torch.randn(64).as_strided((2, 3, 1, 8), (24, 8, 3, 1))
+    yield torch.randn(64).as_strided((2, 3, 1, 8), (24, 8, 1 << 30, 1))
+    yield torch.randn(8).as_strided((1, 1, 1, 8), (1, 5, 0, 1))
+    yield torch.randn(41)[1:].view(5, 1, 8)
+    yield torch.randn(24).as_strided((1, 3, 8), (0, 8, 1))
+
+
+@pytest.mark.parametrize("t", odd_tensors(), ids=lambda t: f"{tuple(t.shape)}-{t.stride()}")
+def test_contiguous_tensors_that_cannot_be_addressed_are_copied(t):
+    assert t.is_contiguous()
+    got = trainable_attention._apart(t)
+    assert torch.equal(got, t) and _launch.rows_ok(got) and got.shape[-1] <= got.stride(-2 if t.dim() == 4 else 0) <= 64
+
+
+def test_tables_at_an_odd_address_are_copied():
+    t = torch.randn(3 * 16 * 8 + 1)[1:].view(3, 16, 8)
+    got = _launch.as_rows(t)
+    assert torch.equal(got, t) and _launch.rows_ok(got)

@@ -65,3 +65,23 @@ def test_buckets_that_run_backwards(path, python_path):  # noqa: F811
     for refused in (lambda: c.packed(130), lambda: c.padded(130), lambda: c.packed(5000)):
         with pytest.raises(ValueError, match="up to 129 tokens"):
             refused()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_contiguous_tensors_that_cannot_be_addressed(dtype):
+    """Inputs, tables and the gradient at odd addresses, and rows of one token with strides of no size: as their copies."""
+    def odd(t):
+        room = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)[1:].view(t.shape)
+        return room.copy_(t)
+
+    def grads(*t):
+        leaves = [x.detach().requires_grad_() for x in t[:5]]
+        o = T.trainable_attention_with_disentangled(*leaves, 0.2, 8, 32)
+        return [o.detach(), *torch.autograd.grad(o, leaves, t[5])]
+
+    for length, change in ((33, odd), (1, odd), (1, lambda t: t.as_strided(t.shape, (*t.stride()[:2], 0, 1)) if t.dim() == 4 else t)):
+        t = [random(2, 3, length, 16, dtype=dtype, n=n) for n in range(3)] + [random(3, 16, 16, dtype=dtype, n=n) for n in (3, 4)] + [random(2, 3, length, 16, dtype=dtype, n=5)]
+        want = grads(*t)
+        for some in ([0], [1], [2], [3], [4], [5], range(6)):
+            got = grads(*(change(x) if n in some else x for n, x in enumerate(t)))
+            assert all(torch.equal(a, b) for a, b in zip(got, want)), (length, some)

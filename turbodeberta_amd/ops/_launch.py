@@ -93,8 +93,14 @@ def rows_ok(t: torch.Tensor) -> bool:
             and all(s >= 0 and (s * es) % 16 == 0 for s in t.stride()[:-1]))
 
 
+def copied(t: torch.Tensor) -> torch.Tensor:
+    """A copy with dense rows at an aligned address.  (``contiguous`` hands back what is contiguous already: tensors at odd addresses, and dimensions of
+    size 1 with any stride.)"""
+    return t.clone(memory_format=torch.contiguous_format)
+
+
 def as_rows(t: torch.Tensor) -> torch.Tensor:
-    return t if rows_ok(t) else t.contiguous()
+    return t if rows_ok(t) else copied(t)
 
 
 def fused_table(t: Optional[torch.Tensor], heads: int, span: int, head_dim: int, name: str):

@@ -26,7 +26,7 @@ def _strides(t):
 def _apart(t):
     """t where the kernels can address it: aligned rows that do not share memory, not too far apart for 32-bit offsets."""
     stride = t.stride(-2) if t.dim() == 4 else t.stride(0)
-    return t if L.rows_ok(t) and t.shape[-1] <= stride <= (1 << 24) // t.element_size() else t.contiguous()
+    return t if L.rows_ok(t) and t.shape[-1] <= stride <= (1 << 24) // t.element_size() else L.copied(t)
 
 
 def _like(t):
