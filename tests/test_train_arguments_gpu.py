@@ -85,3 +85,50 @@ def test_contiguous_tensors_that_cannot_be_addressed(dtype):
         for some in ([0], [1], [2], [3], [4], [5], range(6)):
             got = grads(*(change(x) if n in some else x for n, x in enumerate(t)))
             assert all(torch.equal(a, b) for a, b in zip(got, want)), (length, some)
+
+
+@pytest.mark.parametrize("path", ["native", "python"])
+def test_tables_with_a_leading_1_are_the_operators_own_leaves(path, python_path):  # noqa: F811
+    """Nothing stands between such a leaf and the operator's node, which looks at the streams of its leaves; gradients have the leaf's shape."""
+    if path == "python":
+        python_path()
+    q = random(2, 3, 40, 16)
+    tables = [random(1, 3, rows, 16, n=rows).requires_grad_() for rows in (16, 19)]
+    plain = [t.detach()[0].requires_grad_() for t in tables]
+    call = lambda pk, pq: T.trainable_attention_with_disentangled(q, q, q, pk, pq, 0.2, 8, 32)
+    o = call(*tables)
+    leaves = [f.variable for f, _ in o.grad_fn.next_functions if f is not None]
+    assert len(leaves) == 2 and all(a is b for a, b in zip(leaves, tables))
+    want = torch.autograd.grad(call(*plain), plain, random(2, 3, 40, 16, n=9))
+    got = torch.autograd.grad(o, tables, random(2, 3, 40, 16, n=9))
+    assert all(a.shape == t.shape and torch.equal(a[0], b) for a, b, t in zip(got, want, tables))
+    none = T.trainable_attention_with_disentangled(q[:0], q[:0], q[:0], *tables, 0.2, 8, 32)
+    assert all(g.shape == t.shape and not g.any() for g, t in zip(torch.autograd.grad(none.sum(), tables), tables))
+
+
+@pytest.mark.parametrize("path", ["native", "python"])
+def test_capture_while_an_eager_graph_of_a_table_with_a_leading_1_lives(path, python_path):  # noqa: F811
+    """Refused, as for any other leaf, before autograd's engine meets the other stream."""
+    if path == "python":
+        python_path()
+    q, dy = random(2, 3, 40, 16), random(2, 3, 40, 16, n=9)
+    table = random(1, 3, 16, 16, n=1).requires_grad_()
+    call = lambda: T.trainable_attention_with_disentangled(q, q, q, table, None, 0.2, 8, 32)
+    earlier = call()
+    want, = torch.autograd.grad(call(), table, dy)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o = call()
+        with pytest.raises(RuntimeError, match="holds the same leaves"):
+            torch.autograd.grad(o, table, dy)
+    del o, earlier
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o = call()
+        got, = torch.autograd.grad(o, table, dy)
+    for _ in range(3):
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)

@@ -210,6 +210,10 @@ Tensor result_like(const Tensor& t) {
     return tdb_host_output_like(t, o) && apart(o) ? o : empty(t.sizes(), t);
 }
 
+// A table [H, rows, D]: as it is handed in, or without a leading 1.  (Taken off within a node, so that a leaf's accumulation is that node's own edge, which tied_to_another_stream
+// looks at.)
+Tensor table_of(const Tensor& t) { return t.defined() && t.dim() == 4 ? t.select(0, 0) : t; }
+
 // (batch, head, row) strides of [B, H, L, D], or of packed [T, H, D]
 void strides(const Tensor& t, int64_t* to) { to[0] = t.dim() == 4 ? t.stride(0) : 0, to[1] = t.stride(1), to[2] = t.stride(t.dim() == 4 ? 2 : 0); }
 
@@ -230,7 +234,7 @@ struct Attention : torch::autograd::Function<Attention> {
     }
     static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Optional& of_pk, const Optional& of_pq, const Optional& of_lens, const Optional& of_cu,
                           const Optional& of_seed, const Optional& of_lut, int64_t longest, double scale, int64_t span, int64_t threshold) {
-        const Tensor pk = plain(of_pk), pq = plain(of_pq), lens = plain(of_lens), cu = plain(of_cu), seed = plain(of_seed), lut = plain(of_lut);
+        const Tensor pk = table_of(plain(of_pk)), pq = table_of(plain(of_pq)), lens = plain(of_lens), cu = plain(of_cu), seed = plain(of_seed), lut = plain(of_lut);
         tdb_train_attn_args a = args(q, k, v, pk, pq, lens, cu, seed, lut, longest, scale, span, threshold);
         Tensor o = result_like(q), rest;
         const int64_t rows = q.numel() / (q.size(1) * q.size(-1));
@@ -239,17 +243,18 @@ struct Attention : torch::autograd::Function<Attention> {
         a.o = o.data_ptr(), a.lse = static_cast<float*>(lse.data_ptr()), a.o_rest = ptr(rest);
         strides(o, &a.o_stride_b);
         forward_ok(g.attn_fwd(&a, stream_of(q)));
-        ctx->save_for_backward({q, k, v, o, rest, lse, pk, pq, lens, cu, seed, lut});
+        ctx->save_for_backward({q, k, v, o, rest, lse, plain(of_pk), plain(of_pq), lens, cu, seed, lut});
         ctx->saved_data["longest"] = longest, ctx->saved_data["scale"] = scale, ctx->saved_data["span"] = span, ctx->saved_data["threshold"] = threshold;
         return o;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const variable_list saved = ctx->get_saved_variables();
-        const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &o = saved[3], &rest = saved[4], &lse = saved[5], &pk = saved[6], &pq = saved[7];
+        const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &o = saved[3], &rest = saved[4], &lse = saved[5];
         arrived(grads[0], q);
         variable_list out(13);
         {
             const at::NoGradGuard off;
+            const Tensor pk = table_of(saved[6]), pq = table_of(saved[7]);
             const Tensor dout = apart(grads[0]) ? grads[0] : grads[0].clone(at::MemoryFormat::Contiguous);
             const int64_t span = ctx->saved_data["span"].toInt();
             tdb_train_attn_args a = args(q, k, v, pk, pq, saved[8], saved[9], saved[10], saved[11], ctx->saved_data["longest"].toInt(), ctx->saved_data["scale"].toDouble(), span,
@@ -262,10 +267,10 @@ struct Attention : torch::autograd::Function<Attention> {
                 const Tensor& t = n ? pq : pk;
                 if (!t.defined()) continue;
                 Tensor& d = out[3 + n];
-                d = empty(t.sizes(), t);
+                d = empty(saved[6 + n].sizes(), t);
                 if (t.size(1) != 2 * span) d.zero_();       // (rows that no offset has)
                 (n ? a.dpos_query : a.dpos_key) = d.data_ptr();
-                (n ? a.dpos_query_stride_h : a.dpos_key_stride_h) = d.stride(0);
+                (n ? a.dpos_query_stride_h : a.dpos_key_stride_h) = t.size(1) * t.size(2);
             }
             a.workspace_bytes = g.attn_workspace(&a);
             const Tensor work = empty({a.workspace_bytes}, at::kByte, q);
@@ -383,7 +388,7 @@ PyObject* py_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         const Tensor q = first(args[0], ok);
         if (!ok || !as_int(args[6], buckets) || !as_int(args[7], max_rel) || !as_threshold(args[11], threshold)) return Tensor();
         const Tensor k = take(args[1], &q, ok), v = take(args[2], &q, ok), lens = take(args[8], &q, ok), cu = take(args[9], &q, ok), seed = as_seed(args[12], threshold, q, ok);
-        Tensor pk = take(args[3], &q, ok), pq = take(args[4], &q, ok);
+        const Tensor pk = take(args[3], &q, ok), pq = take(args[4], &q, ok);
         const int64_t dims = cu.defined() ? 3 : 4;
         if (!ok || !k.defined() || !v.defined() || q.dim() != dims || k.sizes() != q.sizes() || v.sizes() != q.sizes() || k.scalar_type() != q.scalar_type() ||
             v.scalar_type() != q.scalar_type() || !apart(q) || !apart(k) || !apart(v))
@@ -409,10 +414,12 @@ PyObject* py_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
             if (!table) return Tensor();
             lut = *table;
         }
-        for (Tensor* t : {&pk, &pq}) {
+        for (const Tensor* t : {&pk, &pq}) {
             if (!t->defined()) continue;
-            if (t->dim() == 4 && t->size(0) == 1) *t = t->select(0, 0);
-            if (t->dim() != 3 || t->size(0) != heads || t->size(1) < 2 * span || t->size(2) != D || t->scalar_type() != q.scalar_type() || !tdb_host_rows_ok(*t)) return Tensor();
+            const int64_t at = t->dim() - 3;
+            if (!(at == 0 || (at == 1 && t->size(0) == 1)) || t->size(at) != heads || t->size(at + 1) < 2 * span || t->size(at + 2) != D || t->scalar_type() != q.scalar_type() ||
+                !tdb_host_rows_ok(*t))
+                return Tensor();
         }
         return Attention::apply(q, k, v, optional(pk), optional(pq), optional(lens), optional(cu), optional(seed), optional(lut), longest, scale, span, threshold);
     });

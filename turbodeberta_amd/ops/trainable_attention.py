@@ -68,11 +68,17 @@ def _fill(a, **tensors):
             setattr(a, f"{name}_stride_{axis}", s)
 
 
+def _shaped(t, shape):
+    return None if t is None else t.view(shape)
+
+
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, pk, pq, lens, cu, seed, *plain):
         q, k, v = _apart(q), _apart(k), _apart(v)
-        pk, pq = (None if t is None else L.as_rows(t) for t in (pk, pq))
+        ctx.shapes = [None if t is None else t.shape for t in (pk, pq)]
+        # (A leading 1 is taken off in here, so that a leaf's accumulation is this node's own edge, which backward_begins looks at.)
+        pk, pq = (None if t is None else L.as_rows(t[0] if t.dim() == 4 else t) for t in (pk, pq))
         o = _like(q)
         ctx.plain, ctx.nothing = plain, q.numel() == 0 or (cu is not None and cu.numel() < 2)
         if ctx.nothing:                     # no sequences, or none with a token: nothing is launched
@@ -90,7 +96,8 @@ class _Attention(torch.autograd.Function):
     def backward(ctx, dout):
         _lib.host().backward_begins()
         if ctx.nothing:
-            return tuple(None if t is None else torch.zeros_like(t) for t in ctx.saved_tensors) + (None,) * (3 + len(ctx.plain))
+            grads = [None if t is None else torch.zeros_like(t) for t in ctx.saved_tensors]
+            return (*grads[:3], *map(_shaped, grads[3:], ctx.shapes)) + (None,) * (3 + len(ctx.plain))
         q, k, v, o, rest, lse, pk, pq, lens, cu, seed = ctx.saved_tensors
         dout = _apart(dout)
         dq, dk, dv = _like(q), _like(k), _like(v)
@@ -109,7 +116,7 @@ class _Attention(torch.autograd.Function):
         work = torch.empty(a.workspace_bytes, dtype=torch.uint8, device=q.device)
         a.workspace = work.data_ptr()
         L.call(lib.tdb_attn_train_bwd, q.device, C.byref(a))
-        return (dq, dk, dv, *tables) + (None,) * (3 + len(ctx.plain))
+        return (dq, dk, dv, *map(_shaped, tables, ctx.shapes)) + (None,) * (3 + len(ctx.plain))
 
 
 def _checked(q, k, v, pos_key_layer, pos_query_layer, heads, sm_scale, buckets, max_rel, p, seed, longest, reach, others):
@@ -134,9 +141,8 @@ def _checked(q, k, v, pos_key_layer, pos_query_layer, heads, sm_scale, buckets, 
         if t is not None:
             if t.dtype != q.dtype:
                 raise ValueError("position tables must have the dtype of q")
-            if t.dim() == 4 and t.shape[0] == 1:
-                t = t[0]
-            if t.dim() != 3 or t.shape[0] != heads or t.shape[2] != D or t.shape[1] < 2 * span:
+            shape = t.shape[1:] if t.dim() == 4 and t.shape[0] == 1 else t.shape
+            if len(shape) != 3 or shape[0] != heads or shape[2] != D or shape[1] < 2 * span:
                 raise ValueError(f"{name}: expected [H={heads}, >=2*span={2 * span}, D={D}], got {tuple(t.shape)}")
         tables.append(t)
     if longest <= 1 << 20 and not all(t is None for t in tables):        # (the C side refuses longer ones)
