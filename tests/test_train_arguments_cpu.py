@@ -102,3 +102,11 @@ def test_tables_at_an_odd_address_are_copied():
     t = torch.randn(3 * 16 * 8 + 1)[1:].view(3, 16, 8)
     got = _launch.as_rows(t)
     assert torch.equal(got, t) and _launch.rows_ok(got)
+
+
+def test_dropout_of_nothing_needs_no_seed():
+    """(Without a GPU the launch fails.)"""
+    f, name = _lib.load().tdb_dropout, lambda rc: _lib.ERROR_NAMES.get(rc)
+    assert name(f(4096, 4096, 5, _lib.TDB_F32, 1, None, None)) == "TDB_ERR_NULL"
+    if not torch.cuda.is_available():
+        assert name(f(4096, 4096, 5, _lib.TDB_F32, 0, None, None)) not in ("TDB_ERR_NULL", "TDB_OK")

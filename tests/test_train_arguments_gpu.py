@@ -132,3 +132,12 @@ def test_capture_while_an_eager_graph_of_a_table_with_a_leading_1_lives(path, py
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_dropout_of_nothing_reads_no_seed(dtype):
+    x = random(1003, dtype=dtype)
+    y = torch.empty_like(x)
+    code = {torch.float32: _lib.TDB_F32, torch.bfloat16: _lib.TDB_BF16, torch.float16: _lib.TDB_F16}[dtype]
+    _lib.check(_lib.load().tdb_dropout(x.data_ptr(), y.data_ptr(), x.numel(), code, 0, None, torch.cuda.current_stream().cuda_stream))
+    assert torch.equal(x, y)

@@ -100,7 +100,7 @@ __device__ __forceinline__ void drop8(float (&v)[8], uint32_t kept, float factor
 
 template <int DT, bool ALIGNED>
 __global__ __launch_bounds__(256) void dropout_kernel(const void* x, void* y, int64_t n, uint32_t threshold, float factor, const int64_t* seed) {
-    const TdbKey key = tdb_key(seed);
+    const TdbKey key = threshold ? tdb_key(seed) : TdbKey{0, 0};
     const int64_t chunks = (n + 7) / 8, step = int64_t(gridDim.x) * 256;
     for (int64_t c = int64_t(blockIdx.x) * 256 + threadIdx.x; c < chunks; c += step) {
         if (ALIGNED && 8 * c + 8 <= n) {
@@ -517,7 +517,8 @@ int tdb_dropout(const void* x, void* y, int64_t n, int32_t dtype, int32_t thresh
     if (n < 0) return tdb_fail(TDB_ERR_SHAPE, "negative number of values");
     if (threshold < 0 || threshold > 65536) return tdb_fail(TDB_ERR_SHAPE, "threshold %d: need 0 to 65536", threshold);
     if (n == 0) return TDB_OK;
-    if (!x || !y || !seed) return tdb_fail(TDB_ERR_NULL, "x, y and seed must be non-NULL");
+    if (!x || !y) return tdb_fail(TDB_ERR_NULL, "x and y must be non-NULL");
+    if (threshold && !seed) return tdb_fail(TDB_ERR_NULL, "dropout needs a seed");
     const hipStream_t s = static_cast<hipStream_t>(stream);
     if (dtype == TDB_F32) launch_dropout<TDB_F32>(x, y, n, threshold, seed, s);
     else if (dtype == TDB_BF16) launch_dropout<TDB_BF16>(x, y, n, threshold, seed, s);
