@@ -169,7 +169,7 @@ struct Args {
     uint32_t threshold;
     float factor, scale;
     int32_t p_shift;                    // float16: probabilities are multiplied by 2^p_shift where they are rounded
-    const uint32_t* largest;            // float16: squares of the largest norms of a row of dout and of v
+    uint32_t* largest;                  // float16, [heads, sequences, 2]: squares of the largest norms of a row of dout and of v
 };
 
 struct Where {
@@ -564,16 +564,17 @@ __device__ __forceinline__ void load_own(typename Elem<DT>::X8 (&own)[2], const 
     }
 }
 
-// float16: a power of two that brings the gradients of scores, which are kept without dropout's factor, near the top of the type's range: they are at most 2 |dout| |v|.  Other types
-// hold any size: 1.
+// float16: a power of two that brings the gradients of a sequence's and head's scores, which are kept without dropout's factor, near the top of the type's range: they are at most
+// 2 |dout| |v|.  2^40 at most (from 2^-24 for the type's largest rows on): sums of several sequences are scaled from one's power to the next one's.  Other types hold any size: 1.
 template <int DT>
-__device__ __forceinline__ float score_power(const Args& a) {
+__device__ __forceinline__ float score_power(const Args& a, int h, int b) {
     if constexpr (DT != TDB_F16) return 1.f;
-    const float most = 2.f * sqrtf(__builtin_bit_cast(float, a.largest[0])) * sqrtf(__builtin_bit_cast(float, a.largest[1]));
+    const uint32_t* const of = a.largest + (int64_t(h) * a.B + b) * 2;
+    const float most = 2.f * sqrtf(__builtin_bit_cast(float, of[0])) * sqrtf(__builtin_bit_cast(float, of[1]));
     if (!(most > 0.f) || !(most < __builtin_inff())) return 1.f;
     int e;
     (void)frexpf(most, &e);             // most < 2^e
-    return ldexpf(1.f, min(max(15 - e, -100), 100));
+    return ldexpf(1.f, min(15 - e, 40));
 }
 
 }  // namespace tdb_train

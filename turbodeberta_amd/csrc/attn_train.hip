@@ -7,7 +7,7 @@
 //
 // Roundings to the type, each where a matrix instruction of it takes its operand: P' (in 16 bits as the sum of two values in the forward pass), dS, and what is stored.  A
 // gradient's error is that of dS's rounding and its own, 1.4 times its own (bfloat16 2.3e-3 of its norm, 1.7e-3 for its own alone); sums are float32.  float16: P' and dS are
-// scaled by powers of two to the top of its range.
+// scaled by powers of two to the top of its range, dS by one for each sequence and head, so that no sequence's gradients depend on the others'.
 // Backward in four launches for a number of heads at a time.  The costly part, scores, exponentials, random numbers, is done once: attn_bwd_kv_kernel owns keys, sums up
 // their gradients and writes dS, rounded to the type, tile by tile to a workspace; attn_bwd_q_kernel owns queries and reads dS; attn_bwd_tables_kernel owns relative
 // positions (a diagonal of tiles) and reads dS; tables_sum_kernel adds its parts up by table row.  No atomics: every sum has one owner and one order.
@@ -159,10 +159,10 @@ __global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_fwd_kernel(Args a) {
 __device__ __forceinline__ int tile_up(const Args& a, int x) { return (x + TILE * a.tiles + TILE - 1) / TILE - a.tiles; }
 __device__ __forceinline__ int tile_down(const Args& a, int x) { return (x + TILE * a.tiles) / TILE - a.tiles; }
 
-// D_i = dO_i . O_i for every row and head, without dropout's factor: 8 lanes each.  float16: the largest squares of the norms of rows of dO and V as well.  And the offsets at which the rows of the
-// tables start, and the diagonals of tiles that lie in the last or in the first of these rows altogether.
+// D_i = dO_i . O_i for every row and head, without dropout's factor: 8 lanes each, a workgroup for 64 rows.  float16: the largest squares of the norms of the sequence's rows of dO
+// and V as well.  And the offsets at which the rows of the tables start, and the diagonals of tiles that lie in the last or in the first of these rows altogether.
 template <int DT>
-__global__ __launch_bounds__(THREADS) void attn_delta_kernel(Args a, uint32_t* largest) {
+__global__ __launch_bounds__(THREADS) void attn_delta_kernel(Args a) {
     using T = typename Elem<DT>::T;
     const int d = 8 * (threadIdx.x & 7);
     if (a.lut) {
@@ -178,61 +178,54 @@ __global__ __launch_bounds__(THREADS) void attn_delta_kernel(Args a, uint32_t* l
             if (row != before && before == first) a.level[1] = tile_down(a, off - 64);
         }
     }
+    int h;
+    Where w;
+    if (!locate<TILE>(a, h, w)) return;
+    const T *const o = rows_of<DT>(a.o, a, w, h), *const dout = rows_of<DT>(a.dout, a, w, h), *const v = rows_of<DT>(a.v, a, w, h);
+    const T* const rest = static_cast<const T*>(a.rest) + (h * a.lines + w.line) * a.D;
     float most_do = 0.f, most_v = 0.f;
-    for (int64_t unit = (int64_t(blockIdx.x) * THREADS + threadIdx.x) >> 3; unit < a.lines * a.H; unit += int64_t(gridDim.x) * (THREADS / 8)) {
-        const int64_t row = unit / a.H;
-        const int h = int(unit - row * a.H);
-        const int64_t b = a.cu ? 0 : row / a.L, r = row - b * a.L * (a.cu ? 0 : 1);
-        bool mine = true;
-        if (!a.cu) {
-            mine = !a.seqlens || r < a.seqlens[b];
-        } else if (DT == TDB_F16) {         // rows of no sequence may hold anything
-            int lo = 0, hi = a.B;
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (a.cu[mid] <= row) lo = mid;
-                else hi = mid;
-            }
-            int64_t first;
-            const int len = valid_rows(a, lo, first);
-            mine = row >= first && row < first + len;
-        }
+#pragma unroll
+    for (int n = 0; n < 8 * TILE / THREADS; ++n) {
+        const int row = w.row0 + n * (THREADS / 8) + (threadIdx.x >> 3);
+        const bool mine = row < w.len;
         float dot = 0.f, sq = 0.f, sv = 0.f;
         if (mine && d < a.D) {
-            const auto o = read8<DT>(static_cast<const T*>(a.o.p) + b * a.o.b + h * a.o.h + r * a.o.l + d);
-            const auto x = read8<DT>(static_cast<const T*>(a.dout.p) + b * a.dout.b + h * a.dout.h + r * a.dout.l + d);
+            const auto y = read8<DT>(o + row * a.o.l + d);
+            const auto x = read8<DT>(dout + row * a.dout.l + d);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) dot += float(o[i]) * float(x[i]), sq += float(x[i]) * float(x[i]);
+            for (int i = 0; i < 8; ++i) dot += float(y[i]) * float(x[i]), sq += float(x[i]) * float(x[i]);
             if (DT != TDB_F32 && a.rest) {
-                const auto o = read8<DT>(static_cast<const T*>(a.rest) + (h * a.lines + row) * a.D + d);
+                const auto y = read8<DT>(rest + int64_t(row) * a.D + d);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) dot += float(o[i]) * float(x[i]);
+                for (int i = 0; i < 8; ++i) dot += float(y[i]) * float(x[i]);
             }
             if constexpr (DT == TDB_F16) {
-                const auto v = read8<DT>(static_cast<const T*>(a.v.p) + b * a.v.b + h * a.v.h + r * a.v.l + d);
+                const auto z = read8<DT>(v + row * a.v.l + d);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) sv += float(v[i]) * float(v[i]);
+                for (int i = 0; i < 8; ++i) sv += float(z[i]) * float(z[i]);
             }
         }
 #pragma unroll
         for (int n = 1; n < 8; n <<= 1) dot += __shfl_xor(dot, n), sq += __shfl_xor(sq, n), sv += __shfl_xor(sv, n);
-        if (mine && (threadIdx.x & 7) == 0) a.delta[h * a.lines + row] = a.factor > 0.f ? dot / a.factor : 0.f;
+        if (mine && (threadIdx.x & 7) == 0) a.delta[h * a.lines + w.line + row] = a.factor > 0.f ? dot / a.factor : 0.f;
         most_do = fmaxf(most_do, sq), most_v = fmaxf(most_v, sv);
     }
     if constexpr (DT == TDB_F16) {
-        __shared__ float s_most[2][THREADS / 64];
+        __shared__ float s_most[2][WAVES];
 #pragma unroll
         for (int n = 8; n < 64; n <<= 1) most_do = fmaxf(most_do, __shfl_xor(most_do, n)), most_v = fmaxf(most_v, __shfl_xor(most_v, n));
         if ((threadIdx.x & 63) == 0) s_most[0][threadIdx.x >> 6] = most_do, s_most[1][threadIdx.x >> 6] = most_v;
         __syncthreads();
         if (threadIdx.x < 2) {              // (squares: their bits are in their order; the largest does not depend on it)
             const float* const m = s_most[threadIdx.x];
-            atomicMax(largest + threadIdx.x, __builtin_bit_cast(uint32_t, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]))));
+            atomicMax(a.largest + (int64_t(h) * a.B + w.b) * 2 + threadIdx.x, __builtin_bit_cast(uint32_t, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]))));
         }
     }
 }
 
-__global__ void clear_kernel(uint32_t* x) { x[threadIdx.x] = 0; }
+__global__ __launch_bounds__(THREADS) void clear_kernel(uint32_t* x, int64_t n) {
+    for (int64_t i = int64_t(blockIdx.x) * THREADS + threadIdx.x; i < n; i += int64_t(gridDim.x) * THREADS) x[i] = 0;
+}
 
 // Level tiles: those of the diagonals from hi on and up to lo, whose offsets all have the last or the first row of the tables.  They come in runs, and all that the
 // positions add to a gradient there is a row of a table times a sum of scores' gradients: kept in float32, from before they are rounded, for the owner's row of keys or
@@ -276,10 +269,10 @@ __device__ __forceinline__ void level_none(const Args& a, int which, int h, int 
 }
 
 // An owner's share of level tiles.  sum[0], sum[1]: over the tiles of hi and lo, for row c.  Adds the two table rows times the sums to acc, and leaves the workgroup's two
-// sums of own rows times the sums for the table's gradient.  lds: 2 KiB.
+// sums of own rows times the sums, without the sequence's power, for the table's gradient.  lds: 2 KiB.
 template <int DT>
 __device__ __forceinline__ void level_end(const Args& a, const Tensor& table, int which, int h, int block, const typename Elem<DT>::X8 (&own)[2], const float (&sum)[2], f32x4 (&acc)[4],
-                                          void* lds, int wave) {
+                                          void* lds, int wave, float power) {
     using T = typename Elem<DT>::T;
     const int c = lane_c(), g = lane_g();
     float(*const part)[2][64] = static_cast<float(*)[2][64]>(lds);
@@ -301,7 +294,7 @@ __device__ __forceinline__ void level_end(const Args& a, const Tensor& table, in
         }
         float x[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x[e] = float(own[e >> 3][e & 7]) * sum[n];
+        for (int e = 0; e < 16; ++e) x[e] = float(own[e >> 3][e & 7]) * (sum[n] / power);
         const float total = sums_of_16(x);
         part[wave][n][32 * (c >> 3) + 8 * g + (c & 7)] = total;
     }
@@ -377,7 +370,7 @@ __global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_bwd_kv_kernel(Args a
     load_own<DT>(v, a.v, a, w, h, row);
     tables.fill(sm.pk, sm.pq, w.row0);
     const TdbKey key = a.threshold ? tdb_key(a.seed) : TdbKey{0, 0};
-    const float power = score_power<DT>(a);
+    const float power = score_power<DT>(a, h, w.b);
     const __amdgpu_buffer_rsrc_t lines = buffer((wave == 0 ? a.lse : a.delta) + h * a.lines + w.line, int64_t(w.len) * 4);      // of the waves that load them
     float line_next = 0.f;
     bool far = false;
@@ -556,7 +549,7 @@ __global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_bwd_kv_kernel(Args a
     }
     if (PQ && level.any(-w.row0 / TILE, (w.len - 1) / TILE - w.row0 / TILE)) {
         by_key[0] = column_sum(by_key[0]), by_key[1] = column_sum(by_key[1]);
-        level_end<DT>(a, a.pq, 1, h, w.block, k, by_key, dk, sm.pq, wave);
+        level_end<DT>(a, a.pq, 1, h, w.block, k, by_key, dk, sm.pq, wave, power);
     } else if (PQ) {
         level_none(a, 1, h, w.block);
     }
@@ -718,14 +711,15 @@ __global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_bwd_q_kernel(Args a)
     };
     fetch();
     for (int y0 = 0; y0 < w.len; y0 += TILE) step(y0);
+    const float power = score_power<DT>(a, h, w.b);
     if (PK && level.any(w.row0 / TILE - (w.len - 1) / TILE, w.row0 / TILE)) {
         X8 q[2];
         load_own<DT>(q, a.q, a, w, h, row);
-        level_end<DT>(a, a.pk, 0, h, w.block, q, by_query, dq, sm.pk, wave);
+        level_end<DT>(a, a.pk, 0, h, w.block, q, by_query, dq, sm.pk, wave, power);
     } else if (PK) {
         level_none(a, 0, h, w.block);
     }
-    store_rows<DT>(a.dq, a, w, h, row, dq, a.scale * a.factor / score_power<DT>(a));
+    store_rows<DT>(a.dq, a, w, h, row, dq, a.scale * a.factor / power);
 }
 
 // Parts that the sequences of a diagonal are dealt to, as many as it has tiles, next to the longest one; each is 2^seg_bits, to which a sequence's tiles are dealt in turn.
@@ -822,9 +816,22 @@ __device__ __forceinline__ void sum_tables(const Args& a, TablesLds<DT>& sm, Dia
         for (int d = 0; d < 4; ++d) acc[n][d] = f32x4{0.f, 0.f, 0.f, 0.f};
     const T* const rows = KEYS ? sm.k : sm.q;
     TablesNext<DT, PK, PQ> next;
+    float power = 1.f, coming = 1.f;            // float16: of the sums, and of the next tile's sequence
+    int of = -1;
+    auto fetch = [&]() {
+        next.load(diagonal, a, h);
+        if (DT == TDB_F16 && diagonal.b != of) coming = score_power<DT>(a, h, diagonal.b), of = diagonal.b;
+    };
     bool more = diagonal.advance(a);
-    if (more) next.load(diagonal, a, h);
+    if (more) fetch();
     while (more) {
+        if (DT == TDB_F16 && coming != power) {
+#pragma unroll
+            for (int n = 0; n < (FAR ? 1 : BLOCKS); ++n)
+#pragma unroll
+                for (int d = 0; d < 4; ++d) acc[n][d] *= coming / power;
+            power = coming;
+        }
         __syncthreads();
         if constexpr (PK) next.q.store(sm.q);
         if constexpr (PQ) next.k.store(sm.k);
@@ -846,7 +853,7 @@ __device__ __forceinline__ void sum_tables(const Args& a, TablesLds<DT>& sm, Dia
         }
         __syncthreads();
         more = diagonal.advance(a);
-        if (more) next.load(diagonal, a, h);
+        if (more) fetch();
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             // far: 16 keys of the queries' sum, or 16 queries of the keys'; twice as many for half as many waves.  Else: 32 queries reach the blocks 2 u .. 2 u + 5, 32 keys
@@ -873,6 +880,7 @@ __device__ __forceinline__ void sum_tables(const Args& a, TablesLds<DT>& sm, Dia
     for (int n = 0; n < (FAR ? 1 : BLOCKS); ++n)
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
+            if constexpr (DT == TDB_F16) acc[n][d] *= 1.f / power;
             if constexpr (FAR) {            // a row for each wave of a table
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[n][d][e] = row_sum(acc[n][d][e]);
@@ -996,7 +1004,7 @@ __global__ __launch_bounds__(THREADS) void tables_sum_kernel(Args a) {
         if (row >= 2 * a.span || int(threadIdx.x & 63) >= a.D) return;
         using T = typename Elem<DT>::T;
         T* const to = static_cast<T*>(which ? a.dpq : a.dpk) + h * (which ? a.dpq_h : a.dpk_h) + int64_t(row) * a.D + (threadIdx.x & 63);
-        *to = T(all * (a.scale * a.factor / score_power<DT>(a)));
+        *to = T(all * (a.scale * a.factor));
     };
     // what lane 4 d + e of a wave adds up: value e of lane d of each group
     auto total = [&](int first, int groups) {
@@ -1039,7 +1047,7 @@ int longest_of(const tdb_train_attn_args& a) { return a.cu_seqlens ? std::max(1,
 // What a backward call needs, and how many heads it takes at a time.
 struct Plan {
     int tiles, row_tiles, split_bits, seg_bits, heads;
-    int64_t lines, starts, delta, level, partial, sums, ds, bytes;       // offsets of the parts, and the sum
+    int64_t lines, largest, starts, delta, level, partial, sums, ds, bytes;       // offsets of the parts, and the sum
 };
 Plan plan_of(const tdb_train_attn_args& a) {
     Plan p;
@@ -1061,7 +1069,8 @@ Plan plan_of(const tdb_train_attn_args& a) {
     p.split_bits = 0;
     while (p.split_bits < bits && (2 << p.split_bits) <= a.batch) ++p.split_bits;
     p.seg_bits = bits - p.split_bits;
-    p.starts = 256;                                 // in front: the two maxima and the diagonals of level tiles
+    p.largest = 256;                                // in front: the diagonals of level tiles
+    p.starts = p.largest + (a.dtype == TDB_F16 ? up(int64_t(a.heads) * a.batch * 8) : 0);
     p.delta = p.starts + (terms ? up((2 * int64_t(a.span) + 1) * 4) : 0);
     p.level = p.delta + up(p.lines * a.heads * 4);
     p.partial = p.level + (terms ? int64_t(2) * p.heads * p.row_tiles * 2 * 64 * 4 : 0);
@@ -1144,8 +1153,8 @@ Args args_of(const tdb_train_attn_args& a, const Plan& p) {
     while (k.p_shift < 15 && (2 << k.p_shift) <= k.L) ++k.p_shift;
     if (a.workspace) {
         char* const at = static_cast<char*>(a.workspace);
-        k.largest = reinterpret_cast<const uint32_t*>(at);
-        k.starts = reinterpret_cast<int32_t*>(at + p.starts), k.level = reinterpret_cast<int32_t*>(at) + 2;
+        k.level = reinterpret_cast<int32_t*>(at), k.largest = reinterpret_cast<uint32_t*>(at + p.largest);
+        k.starts = reinterpret_cast<int32_t*>(at + p.starts);
         k.level_parts = reinterpret_cast<float*>(at + p.level), k.row_sums = reinterpret_cast<float*>(at + p.sums);
         k.delta = reinterpret_cast<float*>(at + p.delta);
         k.partial = reinterpret_cast<float*>(at + p.partial);
@@ -1216,9 +1225,12 @@ struct Launch {
     };
     static hipError_t forward(const Args& k, hipStream_t s) { return by_terms<Fwd>(k, s); }
     static hipError_t backward(Args k, int heads, hipStream_t s) {
-        if (DT == TDB_F16) clear_kernel<<<1, 2, 0, s>>>(const_cast<uint32_t*>(k.largest));
-        // (float16: two workgroups to a CU, as each ends with two atomics on the same words: 8 of 96 .. 384 tokens 10 us, with four 15)
-        attn_delta_kernel<DT><<<unsigned(std::min<int64_t>((k.lines * k.H * 8 + THREADS - 1) / THREADS, DT == TDB_F16 ? 512 : 1 << 22)), THREADS, 0, s>>>(k, const_cast<uint32_t*>(k.largest));
+        if (DT == TDB_F16) {
+            const int64_t n = int64_t(k.H) * k.B * 2;
+            clear_kernel<<<unsigned(std::min<int64_t>((n + THREADS - 1) / THREADS, 1024)), THREADS, 0, s>>>(k.largest, n);
+        }
+        k.blocks = blocks_of(k, TILE);
+        attn_delta_kernel<DT><<<unsigned(int64_t(k.blocks) * k.H), THREADS, 0, s>>>(k);
         hipError_t e = hipGetLastError();
         for (k.head0 = 0; e == hipSuccess && k.head0 < k.H; k.head0 += heads) {
             k.heads = std::min(heads, k.H - k.head0);
