@@ -146,3 +146,12 @@ def test_attentions_dropout_of_another_class_or_with_a_hook_is_called(calls):
     m.dropout.register_forward_hook(lambda module, args, out: shapes.append(tuple(out.shape)))
     run()
     assert shapes == [(2, 4, 6, 6)] and not calls
+
+
+def test_a_norm_without_weights_takes_rows_of_its_width():
+    """Other rows go to the parent's code, which raises."""
+    norm = FlashLayerNorm(8, elementwise_affine=False)
+    assert training._norm_arguments(norm, torch.zeros(2, 8)) is not None
+    assert all(training._norm_arguments(norm, torch.zeros(shape)) is None for shape in ((2, 6), (8, 1), ()))
+    with pytest.raises(RuntimeError):
+        norm(torch.zeros(2, 6))

@@ -65,7 +65,7 @@ def _norm_arguments(norm: nn.LayerNorm, x):
     if torch.is_autocast_enabled("cuda"):
         x = x.float()
     w, b = norm.weight, norm.bias
-    if len(norm.normalized_shape) != 1 or (w is None) != (b is None) or x.shape[-1] > 32768:
+    if tuple(norm.normalized_shape) != tuple(x.shape[-1:]) or (w is None) != (b is None) or x.shape[-1] > 32768:
         return None
     if w is not None and (w.dtype != b.dtype or w.dtype not in (x.dtype, torch.float32)):
         return None
