@@ -155,3 +155,12 @@ def test_a_norm_without_weights_takes_rows_of_its_width():
     assert all(training._norm_arguments(norm, torch.zeros(shape)) is None for shape in ((2, 6), (8, 1), ()))
     with pytest.raises(RuntimeError):
         norm(torch.zeros(2, 6))
+
+
+@pytest.mark.parametrize("cls", BLOCKS)
+def test_inputs_that_broadcast(cls, calls):
+    """The parent's sum takes them, the operator does not."""
+    m, x, r = block(cls, nn.Identity())
+    torch.testing.assert_close(m(x, r[:1]), m.LayerNorm(m.dense(x) + r[:1]))
+    torch.testing.assert_close(m(x[:1], r), m.LayerNorm(m.dense(x[:1]) + r))
+    assert not calls

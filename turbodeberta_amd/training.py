@@ -92,7 +92,7 @@ class _Output:
         x = self.dense(hidden_states)
         wide = torch.promote_types(x.dtype, input_tensor.dtype)
         a = _norm_arguments(self.LayerNorm, x.to(wide))
-        if a is None:
+        if a is None or x.shape != input_tensor.shape:
             return self.LayerNorm(self.dropout(x) + input_tensor)
         x, weight, bias = a
         p = rate_of(self, self.dropout)
