@@ -340,7 +340,7 @@ struct KvLds {
 
 // dk, dv: a workgroup has 64 keys, a wave 16, a lane one of them; it walks over the queries.  Here scores, exponentials and random numbers are made again, once for the whole
 // backward pass.  (Each owner making its own scores, without a workspace, needs them three times.)  Which keys are dropped is drawn a step ahead, a bit each.
-// The batch above: 260 us, bound like the forward pass (vector instructions 48 % of the time, LDS 45, products 19).  Registers are full: 256, two waves to a SIMD.
+// The batch above: 260 us, bound like the forward pass (vector instructions 48 % of the time, LDS 45, products 19).  Registers are full: 256, two waves to a SIMD; with both tables 128 scalar and 2 vector registers are spilled (float16 132 and 6).
 template <int DT, bool PK, bool PQ>
 __global__ __launch_bounds__(THREADS, PER_CU<DT>) void attn_bwd_kv_kernel(Args a) {
     using E = Elem<DT>;
@@ -891,7 +891,9 @@ __device__ __forceinline__ void sum_tables(const Args& a, TablesLds<DT>& sm, Dia
         }
 }
 
-// The batch above: 104 us.  Bound by what it reads, a tile of dS, of Q and of K for each step, 450 MB at 4.3 TB/s; 4 x 4096, where 15 of 127 diagonals are its: 280 us.
+// The batch above: 104 us.  A step asks for a tile of dS, of Q and of K, 450 MB in all, of which 225 come from beyond the XCDs' caches; 50 are written: 2.6 TB/s, half of what a
+// large copy makes.  LDS is busy 45 % of the time, products 20, vector instructions 10: no unit is its bound, a step's chain of loads, LDS and two barriers is.  4 x 4096, where
+// 15 of 127 diagonals are its: 280 us.
 // (Each head's workgroups on one XCD, for its cache: equal, and 107 and 380 us in packed and long batches, whose diagonals are less alike.)
 template <int DT, bool PK, bool PQ>
 __global__ __launch_bounds__(THREADS, DT == TDB_F32 ? 1 : 3) void attn_bwd_tables_kernel(Args a) {

@@ -6,9 +6,9 @@
 //   * Backward: the workgroups share the rows out among themselves, each wave keeps its rows' part of the weight's and bias's gradient in registers;
 //     the waves of a workgroup are added up in LDS, the workgroups by a second launch in a fixed order: no atomics, the same bits every time.
 //   * Rows of other widths than multiples of 8, wider than 2048 or not aligned to 16 bytes: a workgroup per row, a column a lane at a time, the row in LDS.
-// Measured, with what a pass reads and writes: dropout of 16384 x 1024 float32 22 us (134 MB, 6.0 TB/s); LayerNorm of 16384 x 768 bfloat16 forward 10.6 us (50 MB), backward
-// 20.4 (76 MB, 3.7 TB/s); with dropout and residual, 16384 x 1024 forward 17.4 (101 MB), backward 31.2 (168 MB, 5.4 TB/s), the sum of the parts 4.2. A large copy makes
-// 5.0 TB/s; what was written just before is still in the last cache.
+// Measured, with what a pass reads and writes: dropout of 16384 x 1024 float32 22 us (134 MB, 6.0 TB/s); LayerNorm of 16384 x 768 bfloat16 forward 11.5 us (50 MB, 4.4 TB/s),
+// backward 20.1 (76 MB, 3.8 TB/s) and the sum of the parts 3.8; with dropout and residual, 16384 x 1024 forward 18.1 (101 MB, 5.6 TB/s), backward 31.6 (168 MB, 5.3 TB/s) and 4.1. A
+// large copy makes 5.0 TB/s; what was written just before is still in the last cache.
 #include <algorithm>
 
 #include "philox.h"
