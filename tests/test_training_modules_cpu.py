@@ -1,4 +1,6 @@
 """Modules that an operator of the training mode stands for, replaced or watched: they are called then.  The check of the device and the operators are stood in for."""
+import copy
+
 import pytest
 import torch
 from torch import nn
@@ -163,4 +165,29 @@ def test_inputs_that_broadcast(cls, calls):
     m, x, r = block(cls, nn.Identity())
     torch.testing.assert_close(m(x, r[:1]), m.LayerNorm(m.dense(x) + r[:1]))
     torch.testing.assert_close(m(x[:1], r), m.LayerNorm(m.dense(x[:1]) + r))
+    assert not calls
+
+
+@pytest.mark.parametrize("lengths", [(6, 6), (6, 2), (0, 5)])
+@pytest.mark.parametrize("terms", [["c2p", "p2c"], ["c2p"], ["p2c"], []])
+def test_attention_by_its_probabilities(terms, lengths, calls):
+    """Hugging Face's module where tokens are valid, zeros behind them; gradients too."""
+    config = copy.deepcopy(CONFIG)
+    config.pos_att_type, config.relative_attention = terms, bool(terms)
+    m = FlashDisentangledSelfAttention(config).double().train()
+    m.trainable, m.pos_dropout, m.dropout = True, nn.Identity(), Halved(0.25)
+    valid = torch.arange(6) < torch.tensor(lengths)[:, None]
+    mask = (valid[:, None, :, None] & valid[:, None, None, :]).long()
+    dy = torch.randn(2, 6, 32, dtype=torch.float64) * valid[..., None]
+    out = []
+    for forward in (m, super(FlashDisentangledSelfAttention, m).forward):
+        m.zero_grad()
+        h = x.double().requires_grad_()
+        y = forward(h, mask, rel_embeddings=rel.double())[0]
+        y.backward(dy)
+        out.append([y[valid], h.grad] + [p.grad for p in m.parameters() if p.grad is not None])
+        if forward is m:
+            assert not y[~valid].any()
+    # float32 products of 8 and 6 terms, their roundings' sum and a softmax between them: 50 steps of 2^-24
+    assert len(out[0]) == len(out[1]) and all((a - b).norm() <= 50 * 2.0 ** -24 * max(b.norm(), 1) for a, b in zip(*out))
     assert not calls

@@ -6,7 +6,7 @@ import torch
 from torch import nn
 from transformers.models.deberta_v2.modeling_deberta_v2 import DebertaV2Model
 
-from test_training_gpu import FLOAT32, compare, config, gradients, inputs
+from test_training_gpu import BFLOAT16, FLOAT32, compare, config, gradients, inputs
 from turbodeberta_amd.model import patch_model
 
 pytestmark = pytest.mark.gpu
@@ -48,3 +48,18 @@ def test_a_models_gradients(change, p):
     ids, mask, dout = inputs()
     out = gradients(model, ids.cuda(), mask.cuda(), dout.cuda())
     compare(model, exact, out, gradients(exact, ids, mask, dout), mask, FLOAT32)
+
+
+@pytest.mark.parametrize("change", [classes, hooks])
+@pytest.mark.parametrize("autocast", [False, True])
+def test_in_bfloat16_and_under_autocast(change, autocast):
+    torch.manual_seed(11)
+    stock = DebertaV2Model(config(0.0)).to(torch.float32 if autocast else torch.bfloat16)
+    exact = copy.deepcopy(stock).double().train()
+    model = patch_model(copy.deepcopy(stock), training=True).cuda().train()
+    for m in (exact, model):
+        change(m)
+    ids, mask, dout = inputs()
+    with torch.autocast("cuda", torch.bfloat16, enabled=autocast):
+        out = gradients(model, ids.cuda(), mask.cuda(), dout.cuda())
+    compare(model, exact, out, gradients(exact, ids, mask, dout), mask, BFLOAT16)

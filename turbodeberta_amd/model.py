@@ -204,19 +204,14 @@ class FlashDisentangledSelfAttention(DisentangledSelfAttention):
     call is served by the eager parent class.
     ``trainable = True`` (``patch_model(model, training=True)``): a call in training mode, or one that autograd records, goes to
     ``ops.trainable_attention``, which has the gradient and, in training mode, the dropout of the probabilities
-    (modeling_deberta_v2.py:262); without it such a call has no gradient and drops nothing.  Where ``dropout`` is no stock one, or has hooks, it has to be
-    run on the probabilities: the eager parent class serves such a call as well."""
+    (modeling_deberta_v2.py:262); without it such a call has no gradient and drops nothing.  Where ``dropout`` is no stock one, or has hooks, such a call
+    forms the probabilities and runs it on them."""
 
     trainable = False
 
     def forward(self, hidden_states, attention_mask, output_attentions=False, query_states=None,
                 relative_pos=None, rel_embeddings=None):
-        watched = self.trainable and _training.operators_take(self, hidden_states) and not _training.is_dropout(self.dropout)
-        if output_attentions or watched:
-            if relative_pos is not None and not relative_pos.numel():        # (the encoder's stand-in for what fused layers do not read)
-                relative_pos = None
-            if watched and attention_mask is None:
-                attention_mask = hidden_states.new_ones(hidden_states.shape[0], 1, 1, hidden_states.shape[1])
+        if output_attentions:
             return super().forward(hidden_states, attention_mask, output_attentions, query_states,
                                    relative_pos, rel_embeddings)
         if query_states is None:
@@ -241,7 +236,9 @@ class FlashDisentangledSelfAttention(DisentangledSelfAttention):
         pos_key, pos_query, sm_scale, buckets, max_rel = self._position_terms(rel_embeddings, hidden_states.dtype,
                                                                               frozen)
         seqlens = _mask_info(attention_mask).lengths if attention_mask is not None else None
-        if self.trainable and _training.operators_take(self, q, k, v):
+        if self.trainable and _training.operators_take(self, q, k, v) and not _training.is_dropout(self.dropout):
+            out = self._by_probabilities(q, k, v, pos_key, pos_query, sm_scale, buckets, max_rel, seqlens)
+        elif self.trainable and _training.operators_take(self, q, k, v):
             p = _training.rate_of(self, self.dropout)
             out = trainable_attention_with_disentangled(q, k, v, pos_key, pos_query, sm_scale, buckets, max_rel, seqlens_k=seqlens, dropout_p=p,
                                                         seed=_training.draw_seed(self, q.device) if p else None)
@@ -266,6 +263,30 @@ class FlashDisentangledSelfAttention(DisentangledSelfAttention):
                                                        max_rel, pos_key_layer=pos_key, pos_query_layer=pos_query,
                                                        zero_output=False)      # the packing comes from the verified mask
         return out.reshape(T, H * D)
+
+    def _by_probabilities(self, q, k, v, pos_key, pos_query, sm_scale, buckets, max_rel, seqlens):
+        """What ``ops.trainable_attention`` computes, with the module ``dropout`` called on the ``[B, H, L, L]`` probabilities, in q's type.  Products are float32 (as batched
+        ones of bfloat16 with a transposed operand are not to be relied on everywhere)."""
+        L, wide = q.shape[2], torch.autocast(q.device.type, enabled=False)
+        place = torch.arange(L, device=q.device)
+        valid = None if seqlens is None else place < seqlens[:, None]                    # [B, L]
+        with wide:
+            scores = q.float() @ k.float().transpose(-1, -2)
+            if pos_key is not None or pos_query is not None:
+                lut, half = delta_lut(q.device, L, buckets, max_rel)
+                rows = lut[place[:, None] - place + half].long().expand(*q.shape[:2], L, L)         # of query, key
+            if pos_key is not None:
+                scores = scores + (q.float() @ pos_key.float().transpose(-1, -2)).gather(-1, rows)
+            if pos_query is not None:
+                scores = scores + (k.float() @ pos_query.float().transpose(-1, -2)).gather(-1, rows.transpose(-1, -2)).transpose(-1, -2)
+            scores = scores * sm_scale
+            if valid is not None:
+                scores = scores.masked_fill(~valid[:, None, None], torch.finfo(torch.float32).min)
+            probs = scores.softmax(-1).to(q.dtype)
+        probs = self.dropout(probs)
+        with wide:
+            out = (probs.float() @ v.float()).to(q.dtype)
+        return out if valid is None else out.masked_fill(~valid[:, None, :, None], 0)
 
     def _position_terms(self, rel_embeddings, dtype, frozen):
         """``(pos_key, pos_query, sm_scale, position_buckets, max_relative_positions)`` of one call."""
