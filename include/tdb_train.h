@@ -1,6 +1,6 @@
 /*
  * tdb_train.h -- C ABI of the operators that training a DeBERTa-v2/v3 encoder needs beside tdb_attn.h's forward ones: dropout,
- * LayerNorm (with dropout and residual in front of it) and attention with its gradient.
+ * LayerNorm (with dropout and residual in front of it), attention, the loss over a vocabulary, each with its gradient, and the norm of all gradients with clipping.
  *
  * Conventions are those of tdb_attn.h: plain pointers and sizes, element strides, buffers (workspaces too) of the caller, TDB_OK or a
  * negative TDB_ERR_* code, nothing allocated, freed or synchronised, launches on the stream passed in.
@@ -99,6 +99,63 @@ typedef struct tdb_train_attn_args {
 int tdb_attn_train_fwd(const tdb_train_attn_args* args, void* stream);
 int tdb_attn_train_bwd(const tdb_train_attn_args* args, void* stream);
 int64_t tdb_attn_train_workspace(const tdb_train_attn_args* args);
+
+/*
+ * Softmax cross entropy over a vocabulary, from hidden states x [rows, hidden] and an output layer weight [vocab, hidden], bias [vocab] or NULL (bias_dtype: that of x, or
+ * TDB_F32): of each row whose label (64 bits) is not ignore_index the logarithm of the sum of the exponentials of its logits less the label's logit, in natural units.  The logits are
+ * never in memory.  reduction 0: loss [rows], 0 where a row does not count; 1: their sum; 2: their mean over the rows that count (none: NaN).  loss is float32.
+ * A label that is neither ignore_index nor in [0, vocab) makes its row's loss NaN, and every gradient that the row goes into.  Rows that do not count are not read.
+ * weight: rows 16-byte aligned and a multiple of 16 bytes apart (at most 4 MiB); where hidden is no multiple of 16 bytes, zeros follow up to one.  x: rows of any stride and alignment.
+ * Forward fills `state` (tdb_loss_state() bytes), which the backward call reads; x is not read again.  Both take a workspace of tdb_loss_workspace() bytes, 16-byte aligned like
+ * the state.  The backward one holds the gradient of the logits in the type of x, up to 2 GiB at a time or 256 columns of it, partial sums of dx of 1 KiB hidden for each CU or 4
+ * bytes for each value of x, and without a reduction one more x.
+ * Backward: dx, dweight, dbias (of bias_dtype); NULL: not wanted.  dloss: of the sum or mean one float32, without reduction one for each row, dloss_stride apart.
+ * Rows of dx that do not count are zeros.  Everything is added up in a fixed order.
+ */
+typedef struct tdb_loss_args {
+    int32_t dtype, bias_dtype, hidden, reduction;
+    int64_t rows, vocab, ignore_index;
+    const void *x, *weight, *bias;
+    const int64_t* labels;
+    float*  loss;
+    void*   state;
+    int64_t state_bytes;
+    void*   workspace;
+    int64_t workspace_bytes;
+    const float* dloss;
+    void *dx, *dweight, *dbias;
+    int64_t x_stride, weight_stride, dloss_stride, dx_stride, dweight_stride;
+} tdb_loss_args;
+
+int tdb_loss_fwd(const tdb_loss_args* args, void* stream);
+int tdb_loss_bwd(const tdb_loss_args* args, void* stream);
+/* bytes for these sizes, types and reduction (host only) */
+int64_t tdb_loss_state(const tdb_loss_args* args);
+int64_t tdb_loss_workspace(const tdb_loss_args* args, int32_t backward);
+
+/*
+ * The norm of many tensors together, and clipping.  from, to, numel, from_dtype, to_dtype: host arrays with an entry for each tensor, read before the call returns; a tensor's values lie
+ * back to back and are aligned to their own size.  norm: 2 (square root of the sum of squares), 1 (sum of magnitudes) or 0 (largest magnitude).  Sums are held in 64 bits and
+ * added up in a fixed order; a NaN makes every norm NaN.
+ * tdb_grads_norm writes the norm to `total` (float32, device) and leaves it in the workspace, tdb_grads_workspace() bytes for these sizes, 8-byte aligned.
+ * tdb_grads_clip, behind it with the same sizes and workspace: to = from * min(1, max_norm / (norm + 1e-6)), in float32, rounded to to_dtype.  A result may be its own input (same
+ * address and type), which is not written where that factor is 1; any other overlap of a result with an input or a result is refused.
+ */
+typedef struct tdb_grads_args {
+    int32_t tensors, norm;
+    double  max_norm;
+    const void* const* from;
+    void* const* to;
+    const int64_t* numel;
+    const int32_t *from_dtype, *to_dtype;
+    float*  total;
+    void*   workspace;
+    int64_t workspace_bytes;
+} tdb_grads_args;
+
+int tdb_grads_norm(const tdb_grads_args* args, void* stream);
+int tdb_grads_clip(const tdb_grads_args* args, void* stream);
+int64_t tdb_grads_workspace(const tdb_grads_args* args);
 
 #ifdef __cplusplus
 }

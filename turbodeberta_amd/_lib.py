@@ -30,7 +30,8 @@ _VALUE_ERRORS = {-1, -2, -3, -4, -5, -6, -7, -8, -9}
 EXPORTS = ("tdb_version", "tdb_last_error", "tdb_attn_fwd_fixed", "tdb_attn_fwd_varlen", "tdb_bucket_table",
            "tdb_delta_table", "tdb_check_cu_seqlens", "tdb_set_workgroup_limit")
 TRAIN_EXPORTS = ("tdb_dropout", "tdb_norm_fwd", "tdb_norm_bwd", "tdb_norm_workspace", "tdb_attn_train_fwd", "tdb_attn_train_bwd",
-                 "tdb_attn_train_workspace")       # declared in include/tdb_train.h
+                 "tdb_attn_train_workspace", "tdb_loss_fwd", "tdb_loss_bwd", "tdb_loss_state", "tdb_loss_workspace",
+                 "tdb_grads_norm", "tdb_grads_clip", "tdb_grads_workspace")       # declared in include/tdb_train.h
 
 
 class PosArgs(C.Structure):
@@ -100,6 +101,25 @@ class TrainAttnArgs(C.Structure):
     ]
 
 
+class LossArgs(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("bias_dtype", C.c_int32), ("hidden", C.c_int32), ("reduction", C.c_int32),
+        ("rows", C.c_int64), ("vocab", C.c_int64), ("ignore_index", C.c_int64),
+        ("x", C.c_void_p), ("weight", C.c_void_p), ("bias", C.c_void_p), ("labels", C.c_void_p), ("loss", C.c_void_p),
+        ("state", C.c_void_p), ("state_bytes", C.c_int64), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
+        ("dloss", C.c_void_p), ("dx", C.c_void_p), ("dweight", C.c_void_p), ("dbias", C.c_void_p),
+        ("x_stride", C.c_int64), ("weight_stride", C.c_int64), ("dloss_stride", C.c_int64), ("dx_stride", C.c_int64), ("dweight_stride", C.c_int64),
+    ]
+
+
+class GradsArgs(C.Structure):
+    _fields_ = [
+        ("tensors", C.c_int32), ("norm", C.c_int32), ("max_norm", C.c_double),
+        ("from", C.c_void_p), ("to", C.c_void_p), ("numel", C.c_void_p), ("from_dtype", C.c_void_p), ("to_dtype", C.c_void_p),
+        ("total", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
+    ]
+
+
 _lock = threading.Lock()
 _lib = None
 _host = None
@@ -139,6 +159,15 @@ def load() -> C.CDLL:
             getattr(lib, name).argtypes = [C.POINTER(TrainAttnArgs), C.c_void_p]
         lib.tdb_attn_train_workspace.argtypes = [C.POINTER(TrainAttnArgs)]
         lib.tdb_attn_train_workspace.restype = C.c_int64
+        for name in ("tdb_loss_fwd", "tdb_loss_bwd"):
+            getattr(lib, name).argtypes = [C.POINTER(LossArgs), C.c_void_p]
+        for name in ("tdb_grads_norm", "tdb_grads_clip"):
+            getattr(lib, name).argtypes = [C.POINTER(GradsArgs), C.c_void_p]
+        lib.tdb_grads_workspace.argtypes = [C.POINTER(GradsArgs)]
+        lib.tdb_grads_workspace.restype = C.c_int64
+        lib.tdb_loss_state.argtypes = [C.POINTER(LossArgs)]
+        lib.tdb_loss_workspace.argtypes = [C.POINTER(LossArgs), C.c_int32]
+        lib.tdb_loss_state.restype = lib.tdb_loss_workspace.restype = C.c_int64
         lib.tdb_norm_workspace.argtypes = [C.c_int64, C.c_int32]
         lib.tdb_norm_workspace.restype = C.c_int64
         if lib.tdb_version() != ABI_VERSION:
@@ -163,7 +192,8 @@ def host():
         module.bind_encoder(*(address("tdb_enc_" + n) for n in ("scan_mask", "embed", "add_norm", "small_gemm", "small_tiles", "small_splits", "unpack", "gemm", "gemm_splits",
                                                                                 "rows_fused", "embed_rows", "norm_gemm", "gemm_add", "norm_rows")))
         module.bind_train(*(address(n) for n in ("tdb_dropout", "tdb_norm_fwd", "tdb_norm_bwd", "tdb_norm_workspace", "tdb_attn_train_fwd", "tdb_attn_train_bwd",
-                                                 "tdb_attn_train_workspace", "tdb_last_error")))
+                                                 "tdb_attn_train_workspace", "tdb_loss_fwd", "tdb_loss_bwd", "tdb_loss_state", "tdb_loss_workspace",
+                                                 "tdb_grads_norm", "tdb_grads_clip", "tdb_grads_workspace", "tdb_last_error")))
         module.bind(address("tdb_attn_fwd_fixed"), address("tdb_attn_fwd_varlen"))
         _host = module
     return _host

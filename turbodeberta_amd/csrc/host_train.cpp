@@ -36,6 +36,13 @@ struct {
     decltype(&tdb_attn_train_fwd) attn_fwd;
     decltype(&tdb_attn_train_bwd) attn_bwd;
     decltype(&tdb_attn_train_workspace) attn_workspace;
+    decltype(&tdb_loss_fwd) loss_fwd;
+    decltype(&tdb_loss_bwd) loss_bwd;
+    decltype(&tdb_loss_state) loss_state;
+    decltype(&tdb_loss_workspace) loss_workspace;
+    decltype(&tdb_grads_norm) grads_norm;
+    decltype(&tdb_grads_clip) grads_clip;
+    decltype(&tdb_grads_workspace) grads_workspace;
     decltype(&tdb_last_error) last_error;
 } g;
 
@@ -281,6 +288,89 @@ struct Attention : torch::autograd::Function<Attention> {
     }
 };
 
+// -------------------------------------------------------------------------------------------------------------------- loss
+
+struct Loss : torch::autograd::Function<Loss> {
+    static tdb_loss_args args(const Tensor& weight, const Tensor& bias, int64_t rows, int64_t ignore, int64_t reduction) {
+        tdb_loss_args a;
+        memset(&a, 0, sizeof(a));
+        a.dtype = dtype_code(weight), a.bias_dtype = bias.defined() ? dtype_code(bias) : a.dtype, a.hidden = int32_t(weight.size(1)), a.reduction = int32_t(reduction);
+        a.rows = rows, a.vocab = weight.size(0), a.ignore_index = ignore, a.weight = weight.data_ptr(), a.weight_stride = weight.stride(0), a.bias = ptr(bias);
+        return a;
+    }
+    static int call(decltype(&tdb_loss_fwd) f, tdb_loss_args& a, const Tensor& state, bool backward) {
+        a.state = state.data_ptr(), a.state_bytes = state.numel();
+        const Tensor work = empty({g.loss_workspace(&a, backward)}, at::kByte, state);
+        a.workspace = work.data_ptr(), a.workspace_bytes = work.numel();
+        return f(&a, stream_of(state));
+    }
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Optional& of_bias, const Tensor& labels, int64_t ignore, int64_t reduction) {
+        const Tensor bias = plain(of_bias);
+        tdb_loss_args a = args(weight, bias, labels.numel(), ignore, reduction);
+        const Tensor rows = as_rows(x, x.size(-1), a.x_stride), loss = empty(reduction == 0 ? labels.sizes() : at::IntArrayRef{}, at::kFloat, x);
+        a.x = rows.data_ptr(), a.labels = static_cast<const int64_t*>(labels.data_ptr()), a.loss = static_cast<float*>(loss.data_ptr());
+        const Tensor state = empty({g.loss_state(&a)}, at::kByte, x);
+        forward_ok(call(g.loss_fwd, a, state, false));
+        ctx->save_for_backward({weight, bias, state});
+        ctx->saved_data["sizes"] = x.sizes(), ctx->saved_data["rows"] = labels.numel(), ctx->saved_data["ignore"] = ignore, ctx->saved_data["reduction"] = reduction;
+        return loss;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const variable_list saved = ctx->get_saved_variables();
+        const Tensor &weight = saved[0], &bias = saved[1], &state = saved[2];
+        arrived(grads[0], weight);
+        variable_list out(6);
+        {
+            const at::NoGradGuard off;
+            const int64_t reduction = ctx->saved_data["reduction"].toInt();
+            tdb_loss_args a = args(weight, bias, ctx->saved_data["rows"].toInt(), ctx->saved_data["ignore"].toInt(), reduction);
+            const Tensor dloss = reduction == 0 ? grads[0].reshape({-1}) : grads[0];
+            a.dloss = static_cast<const float*>(dloss.data_ptr()), a.dloss_stride = reduction == 0 ? dloss.stride(0) : 0;
+            const std::vector<int64_t> sizes = ctx->saved_data["sizes"].toIntVector();
+            if (ctx->needs_input_grad(0)) out[0] = empty(sizes, weight), a.dx = out[0].data_ptr(), a.dx_stride = a.hidden;
+            if (ctx->needs_input_grad(1)) out[1] = empty(weight.sizes(), weight), a.dweight = out[1].data_ptr(), a.dweight_stride = a.hidden;
+            if (bias.defined() && ctx->needs_input_grad(2)) out[2] = empty(bias.sizes(), bias), a.dbias = out[2].data_ptr();
+            backward_ok(call(g.loss_bwd, a, state, true));
+        }
+        return once(std::move(out));
+    }
+};
+
+// ------------------------------------------------------------------------------------------------------------------- norms
+
+// Tensors as the C ABI takes them; false for anything but ordinary ones whose values lie back to back, on the device of `like` (the first one, if there is none yet).
+struct Tensors {
+    std::vector<Tensor> t;
+    std::vector<const void*> at;
+    std::vector<int64_t> numel;
+    std::vector<int32_t> dtype;
+    bool take(PyObject* list, const Tensor* like) {
+        if (!PyList_CheckExact(list)) return false;
+        const Py_ssize_t n = PyList_GET_SIZE(list);
+        t.reserve(n), at.reserve(n), numel.reserve(n), dtype.reserve(n);
+        for (Py_ssize_t i = 0; i < n; ++i) {
+            PyObject* const o = PyList_GET_ITEM(list, i);
+            if (!THPVariable_CheckExact(o)) return false;
+            const Tensor& x = THPVariable_Unpack(o);
+            if (!tdb_host_plain(x, like ? *like : i ? t[0] : x, false) || dtype_code(x) < 0 || !x.is_non_overlapping_and_dense()) return false;
+            t.push_back(x), at.push_back(x.data_ptr()), numel.push_back(x.numel()), dtype.push_back(dtype_code(x));
+        }
+        return n > 0 && t[0].is_cuda() && t[0].device().index() == c10::hip::current_device();
+    }
+};
+
+struct Grads {
+    Tensors from, to;
+    Tensor total, work;
+    tdb_grads_args a;
+    void fill(int64_t norm) {
+        memset(&a, 0, sizeof(a));
+        a.tensors = int32_t(from.t.size()), a.norm = int32_t(norm), a.from = from.at.data(), a.numel = from.numel.data(), a.from_dtype = from.dtype.data();
+        total = empty({}, at::kFloat, from.t[0]), work = empty({g.grads_workspace(&a) / 8}, at::kDouble, from.t[0]);
+        a.total = static_cast<float*>(total.data_ptr()), a.workspace = work.data_ptr(), a.workspace_bytes = 8 * work.numel();
+    }
+};
+
 // ----------------------------------------------------------------------------------------------------------------- CPython
 
 // One tensor argument, undefined for None; `ok` is cleared for anything but a plain tensor on x's device.
@@ -425,11 +515,74 @@ PyObject* py_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     });
 }
 
+// train_loss(x, weight, labels, bias, ignore_index, reduction)
+PyObject* py_loss(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    if (nargs != 6) Py_RETURN_NONE;
+    return native([&]() -> Tensor {
+        bool ok = true;
+        int64_t reduction;
+        const Tensor x = first(args[0], ok);
+        if (!ok || x.dim() < 1 || x.size(-1) > 32768 || !PyLong_CheckExact(args[4]) || !as_int(args[5], reduction)) return Tensor();
+        const int64_t ignore = PyLong_AsLongLong(args[4]);
+        if (ignore == -1 && PyErr_Occurred()) {
+            PyErr_Clear();
+            return Tensor();
+        }
+        const Tensor weight = take(args[1], &x, ok), labels = take(args[2], &x, ok), bias = take(args[3], &x, ok);
+        if (!ok || !weight.defined() || !labels.defined() || weight.dim() != 2 || weight.size(0) < 2 || weight.size(1) != x.size(-1) || weight.scalar_type() != x.scalar_type() ||
+            weight.stride(0) < weight.size(1) || !tdb_host_rows_ok(weight) || weight.size(1) * weight.element_size() % 16)
+            return Tensor();
+        if (labels.scalar_type() != at::kLong || labels.sizes() != x.sizes().slice(0, x.dim() - 1) || !labels.is_contiguous()) return Tensor();
+        if (bias.defined() && (bias.dim() != 1 || bias.size(0) != weight.size(0) || !bias.is_contiguous() || (bias.scalar_type() != x.scalar_type() && bias.scalar_type() != at::kFloat)))
+            return Tensor();
+        return Loss::apply(x, weight, optional(bias), labels, ignore, reduction);
+    });
+}
+
+// train_grads_norm(tensors, norm)
+PyObject* py_grads_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    if (nargs != 2) Py_RETURN_NONE;
+    return native([&]() -> Tensor {
+        int64_t norm;
+        Grads c;
+        if (!as_int(args[1], norm) || !c.from.take(args[0], nullptr)) return Tensor();
+        c.fill(norm);
+        forward_ok(g.grads_norm(&c.a, stream_of(c.total)));
+        return c.total;
+    });
+}
+
+// train_grads_clip(grads, out, norm, max_norm): the norm
+PyObject* py_grads_clip(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    if (nargs != 4) Py_RETURN_NONE;
+    return native([&]() -> Tensor {
+        int64_t norm;
+        Grads c;
+        double max_norm;
+        if (!as_int(args[2], norm) || !as_double(args[3], max_norm) || !c.from.take(args[0], nullptr) || !c.to.take(args[1], &c.from.t[0]) || c.to.t.size() != c.from.t.size()) return Tensor();
+        for (size_t i = 0; i < c.to.t.size(); ++i)
+            if (c.to.t[i].sizes() != c.from.t[i].sizes() || c.to.t[i].strides() != c.from.t[i].strides() || c.to.t[i].is_inference()) return Tensor();
+        c.fill(norm);
+        c.a.to = const_cast<void* const*>(c.to.at.data()), c.a.to_dtype = c.to.dtype.data(), c.a.max_norm = max_norm;
+        forward_ok(g.grads_norm(&c.a, stream_of(c.total)));
+        forward_ok(g.grads_clip(&c.a, stream_of(c.total)));     // (what it refuses it refuses before it launches anything: the Python path repeats both and raises)
+        for (const Tensor& t : c.to.t) t.unsafeGetTensorImpl()->bump_version();
+        return c.total;
+    });
+}
+
 // bind_train(addresses of the entry points of tdb_train.h in its order, address of tdb_last_error)
 PyObject* py_bind_train(PyObject*, PyObject* args) {
-    unsigned long long at[8];
-    if (!PyArg_ParseTuple(args, "KKKKKKKK", at, at + 1, at + 2, at + 3, at + 4, at + 5, at + 6, at + 7)) return nullptr;
-    static_assert(sizeof(g) == sizeof(at), "");
+    constexpr int N = sizeof(g) / sizeof(void*);
+    unsigned long long at[N];
+    if (PyTuple_GET_SIZE(args) != N) {
+        PyErr_SetString(PyExc_TypeError, "bind_train: wrong number of addresses");
+        return nullptr;
+    }
+    for (int i = 0; i < N; ++i) {
+        at[i] = PyLong_AsUnsignedLongLong(PyTuple_GET_ITEM(args, i));
+        if (PyErr_Occurred()) return nullptr;
+    }
     memcpy(&g, at, sizeof(g));
     Py_RETURN_NONE;
 }
@@ -447,6 +600,9 @@ PyMethodDef kTrain[] = {
     {"bind_train", py_bind_train, METH_VARARGS, nullptr},
     {"train_dropout", reinterpret_cast<PyCFunction>(py_dropout), METH_FASTCALL, nullptr},
     {"train_norm", reinterpret_cast<PyCFunction>(py_norm), METH_FASTCALL, nullptr},
+    {"train_loss", reinterpret_cast<PyCFunction>(py_loss), METH_FASTCALL, nullptr},
+    {"train_grads_norm", reinterpret_cast<PyCFunction>(py_grads_norm), METH_FASTCALL, nullptr},
+    {"train_grads_clip", reinterpret_cast<PyCFunction>(py_grads_clip), METH_FASTCALL, nullptr},
     {"train_attention", reinterpret_cast<PyCFunction>(py_attention), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
