@@ -129,7 +129,7 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float 
     _checked(grads, "gradients")
     if out is None:
         out = [torch.empty_like(t) for t in grads]
-    _checked(list(out) + grads[:1], "out")
+    _checked(grads[:1] + list(out), "out")
     for o, t in zip(out, grads):
         if o.shape != t.shape:
             raise ValueError(f"out must have the gradients' shapes: {tuple(o.shape)}, {tuple(t.shape)}")
