@@ -18,8 +18,21 @@
 namespace tdb_train {
 
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.693147180559945309417f;
-constexpr int TILE = 256;           // rows that the gathered ones are filled up to with zeros, columns of D
-constexpr int FINISH_ROWS = 64;     // rows of a workgroup of the last forward kernel
+constexpr int TILE = 256;           // what rows and columns of the buffers are rounded up to
+constexpr int FINISH_ROWS = 32;     // rows of a workgroup of the last forward kernel
+constexpr int FEW = 1024;           // rows up to which tiles may be lower than 256
+
+// Rows of a tile where n count: what leaves the least of them empty, with lower tiles' smaller share of products in what they load counted in.
+__host__ __device__ constexpr int tile_rows(int n, int least) {
+    int best = 256, cost = (n + 255) / 256 * 256 * 16;
+    if (n > FEW) return best;
+    const int heights[] = {128, 64, 32}, dear[] = {18, 21, 26};
+    for (int i = 0; i < 3; ++i) {
+        const int h = heights[i], c = (n + h - 1) / h * h * dear[i];
+        if (h >= least && c < cost) best = h, cost = c;
+    }
+    return best;
+}
 
 // float16: D lies in [-2^14, 2^14], so that probabilities down to 2^-38 are told from 0 (2^-24 without).
 template <int DT>
@@ -34,47 +47,69 @@ struct Loss {
     float* loss;
     // state: count[0] rows that count, count[1] workgroups that are done
     int32_t *count, *index, *place, *label;     // of the gathered rows: row, label; of the rows: their place among the gathered ones
-    float *top, *inverse;                       // largest logit (base 2), 1 / sum of exponentials
+    float *top, *inverse, *right;               // largest logit, 1 / sum of exponentials relative to it, the label's logit
     char* gathered;
     int64_t pitch;                              // of a gathered row, bytes
     // workspace
-    float *right, *maxima, *sums;               // the label's logit; [groups of column tiles][rows]
+    float *maxima, *sums;                       // [groups of column tiles][rows]
     double* block_sums;
     int64_t padded;                             // rows, rounded up
-    int32_t column_tiles, group;                // of the vocabulary, those that one workgroup takes together
+    int32_t group;                              // column tiles that a workgroup of the kernel for many rows takes together
 };
 
+// How the logits' maxima and sums lie: groups of column tiles, rows `pitch` to each.  Tiles of fewer than 256 rows are 128 classes wide, the others 256.
+struct Partials {
+    int64_t groups, tiles, group, pitch;
+    __device__ __forceinline__ Partials(const Loss& p, bool many)
+        : tiles((p.vocab + (many ? 255 : 127)) / (many ? 256 : 128)), group(many ? p.group : 1), pitch(many ? p.padded : min(p.padded, int64_t(FEW))) {
+        groups = (tiles + group - 1) / group;
+    }
+};
+
+// The bias of a class, -inf past the vocabulary.  Values beyond 2^126 become that: a mask of the type's lowest value stays a number when logits are subtracted and scaled.
 template <int DT>
 __device__ __forceinline__ float bias_of(const Loss& p, int64_t v) {
     if (v >= p.vocab) return -INFINITY;
     if (!p.bias_kind) return 0.f;
     const float b = p.bias_kind == 2 ? static_cast<const float*>(p.bias)[v] : float(static_cast<const typename Matrix<DT>::T*>(p.bias)[v]);
-    const float t = b * LOG2E;
-    return fabsf(t) == INFINITY && fabsf(b) != INFINITY ? copysignf(FLT_MAX, b) : t;        // (a mask of the type's lowest value stays a number)
+    return fabsf(b) == INFINITY ? b : b > 0x1p126f ? 0x1p126f : b < -0x1p126f ? -0x1p126f : b;      // (NaN stays)
 }
 
+template <int WAVES>
 __device__ __forceinline__ int block_count(int x, int* scratch) {
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = x;
     __syncthreads();
-    return scratch[0] + scratch[1] + scratch[2] + scratch[3];
+    int all = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) all += scratch[w];
+    return all;
 }
 
-// Rows that count, in order: where they come from, their labels, and they themselves, dense, zeros behind them up to a multiple of TILE rows and of the steps' 128 bytes.
+constexpr int GATHER_WAVES = 8, GATHER_ROWS = 4;       // rows that a wave copies at once
+
+// Rows that count, in order: where they come from, their labels, and they themselves, dense, zeros behind them up to a multiple of the steps' 128 bytes.
 // A workgroup has `chunk` rows and counts for itself what lies in front of them.
 template <int DT>
-__global__ __launch_bounds__(256) void loss_gather_kernel(Loss p, int64_t chunk, bool wide) {
+__global__ __launch_bounds__(64 * GATHER_WAVES) void loss_gather_kernel(Loss p, int64_t chunk, bool wide) {
     using T = typename Matrix<DT>::T;
-    __shared__ int scratch[4];
+    constexpr int THREADS = 64 * GATHER_WAVES, U = 8;
+    __shared__ int scratch[GATHER_WAVES];
     const int wave = threadIdx.x >> 6, l = threadIdx.x & 63;
     const int64_t first = blockIdx.x * chunk, end = min(p.rows, first + chunk);
     int seen = 0;
-    for (int64_t i = threadIdx.x; i < first; i += 256) seen += p.labels[i] != p.ignore;
-    const int before = block_count(seen, scratch);
+    for (int64_t i = threadIdx.x; i < first; i += THREADS * U) {
+        int64_t label[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) label[u] = p.labels[min(i + THREADS * u, first - 1)];
+#pragma unroll
+        for (int u = 0; u < U; ++u) seen += i + THREADS * u < first && label[u] != p.ignore;
+    }
+    const int before = block_count<GATHER_WAVES>(seen, scratch);
     int at = before;
-    for (int64_t i0 = first; i0 < end; i0 += 256) {
+    for (int64_t i0 = first; i0 < end; i0 += THREADS) {
         const int64_t i = i0 + threadIdx.x;
         const int64_t label = i < end ? p.labels[i] : p.ignore;
         const bool counts = label != p.ignore;
@@ -84,7 +119,7 @@ __global__ __launch_bounds__(256) void loss_gather_kernel(Loss p, int64_t chunk,
         __syncthreads();
         int place = at + __popcll(who & ((uint64_t(1) << l) - 1)), all = 0;
 #pragma unroll
-        for (int v = 0; v < 4; ++v) place += v < wave ? scratch[v] : 0, all += scratch[v];
+        for (int v = 0; v < GATHER_WAVES; ++v) place += v < wave ? scratch[v] : 0, all += scratch[v];
         at += all;
         if (i < end) {
             p.place[i] = counts ? place : -1;
@@ -98,173 +133,209 @@ __global__ __launch_bounds__(256) void loss_gather_kernel(Loss p, int64_t chunk,
         }
     }
     if (blockIdx.x == 0 && threadIdx.x == 0) p.count[1] = 0;
-    int fill = at;
-    if (blockIdx.x == gridDim.x - 1) {
-        if (threadIdx.x == 0) p.count[0] = at;
-        fill = (at + TILE - 1) / TILE * TILE;
-    }
+    if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) p.count[0] = at;
     __syncthreads();
     const int columns = int(p.pitch / sizeof(T));
-    for (int r = before + wave; r < fill; r += 4) {
-        char* const to = p.gathered + r * p.pitch;
-        const T* const from = reinterpret_cast<const T*>(p.x) + (r < at ? p.index[r] : 0) * p.x_stride;
+    for (int r0 = before + wave * GATHER_ROWS; r0 < at; r0 += GATHER_WAVES * GATHER_ROWS) {
+        const T* from[GATHER_ROWS];
+#pragma unroll
+        for (int u = 0; u < GATHER_ROWS; ++u) from[u] = reinterpret_cast<const T*>(p.x) + p.index[min(r0 + u, at - 1)] * p.x_stride;
         if (wide) {
             constexpr int PER = 16 / sizeof(T);
             for (int c = l; c < columns / PER; c += 64) {
-                uint4 v = {0, 0, 0, 0};
-                if (r < at && c * PER < p.hidden) v = reinterpret_cast<const uint4*>(from)[c];
-                reinterpret_cast<uint4*>(to)[c] = v;
+                uint4 v[GATHER_ROWS];
+#pragma unroll
+                for (int u = 0; u < GATHER_ROWS; ++u) v[u] = c * PER < p.hidden ? reinterpret_cast<const uint4*>(from[u])[c] : uint4{0, 0, 0, 0};
+#pragma unroll
+                for (int u = 0; u < GATHER_ROWS; ++u)
+                    if (r0 + u < at) reinterpret_cast<uint4*>(p.gathered + (r0 + u) * p.pitch)[c] = v[u];
             }
         } else {
-            for (int c = l; c < columns; c += 64) reinterpret_cast<T*>(to)[c] = r < at && c < p.hidden ? from[c] : T(0.f);
+            for (int c = l; c < columns; c += 64) {
+                T v[GATHER_ROWS];
+#pragma unroll
+                for (int u = 0; u < GATHER_ROWS; ++u) v[u] = c < p.hidden ? from[u][c] : T(0.f);
+#pragma unroll
+                for (int u = 0; u < GATHER_ROWS; ++u)
+                    if (r0 + u < at) reinterpret_cast<T*>(p.gathered + (r0 + u) * p.pitch)[c] = v[u];
+            }
         }
     }
 }
 
-// The biases of a tile's columns, in base 2; -inf past the vocabulary.
-template <int DT, int BN>
-__device__ __forceinline__ void stage_bias(const Loss& p, int64_t n0, float* s_bias) {
-    if (threadIdx.x < BN) s_bias[threadIdx.x] = bias_of<DT>(p, n0 + threadIdx.x);
+// The operands of a tile's logits.
+template <int DT>
+__device__ __forceinline__ Rows hidden_rows(const Loss& p, int n) { return {p.gathered, p.pitch, n, uint32_t(p.pitch)}; }
+template <int DT>
+__device__ __forceinline__ Rows weight_rows(const Loss& p) { return {p.w, p.w_pitch, p.vocab, uint32_t((p.hidden * sizeof(typename Matrix<DT>::T) + 15) / 16 * 16)}; }
+
+// A tile's logits: the sums start from the biases.
+template <int DT, class P>
+__device__ __forceinline__ void logits_of(const Loss& p, int n, char* smem, float* s_bias, int64_t m0, int64_t n0, typename P::Acc& acc) {
+    __syncthreads();                        // (the biases of the tile before have been read)
+    if (threadIdx.x < P::BN) s_bias[threadIdx.x] = bias_of<DT>(p, n0 + threadIdx.x);
+    __syncthreads();
+    P::run(smem, hidden_rows<DT>(p, n), weight_rows<DT>(p), m0, n0, 0, p.pitch / P::LINE_BYTES, acc,
+           [&](int j, int q) { return *reinterpret_cast<const f32x4*>(s_bias + P::wave_n() + j * Matrix<DT>::SIDE + quad_n<DT>(q)); });
 }
 
 // Forward: of each gathered row and group of column tiles the largest logit and the sum of exponentials relative to it.
-template <int DT, class P, int BM, int BN, int WN>
-__global__ __launch_bounds__(P::WAVES * 64, 2) void loss_logits_kernel(Loss p) {
-    extern __shared__ __attribute__((aligned(1024))) char smem[];
-    __shared__ float s_bias[BN], s_top[WN][BM], s_sum[WN][BM];
+template <int DT, class P>
+__device__ __forceinline__ void logits_body(const Loss& p, int n, char* smem, float* s_bias, float* s_top, float* s_sum) {
     using M = Matrix<DT>;
-    const int n = p.count[0];
-    const int64_t row_tiles = (n + BM - 1) / BM, groups = (p.column_tiles + p.group - 1) / p.group, all = row_tiles * groups;
-    const Rows a{p.gathered, p.pitch, p.padded, uint32_t(p.pitch)}, b{p.w, p.w_pitch, p.vocab, uint32_t((p.hidden * sizeof(typename M::T) + 15) / 16 * 16)};
+    const Partials parts(p, P::BM == 256);
+    const int64_t row_tiles = (n + P::BM - 1) / P::BM, all = row_tiles * parts.groups;
     for (int64_t block = blockIdx.x; block < all; block += gridDim.x) {
         int64_t row, g, split;
-        tile_of(block, row_tiles, groups, 1, row, g, split);
-        const int64_t m0 = row * BM;
+        tile_of(block, row_tiles, parts.groups, 1, row, g, split);
+        const int64_t m0 = row * P::BM;
         float top[P::TM], sum[P::TM];
 #pragma unroll
         for (int i = 0; i < P::TM; ++i) top[i] = -FLT_MAX, sum[i] = 0.f;
-        for (int64_t t = g * p.group; t < min(int64_t(p.column_tiles), (g + 1) * p.group); ++t) {
-            const int64_t n0 = t * BN;
+        for (int64_t t = g * parts.group; t < min(parts.tiles, (g + 1) * parts.group); ++t) {
+            const int64_t n0 = t * P::BN;
             typename P::Acc acc;
-            P::run(smem, a, b, m0, n0, 0, p.pitch / 128, acc);
-            stage_bias<DT, BN>(p, n0, s_bias);
-            __syncthreads();
+            logits_of<DT, P>(p, n, smem, s_bias, m0, n0, acc);
 #pragma unroll
             for (int i = 0; i < P::TM; ++i) {
-                const int64_t m = m0 + P::wave_m() + i * M::SIDE + lane_m<DT>();
                 float most = top[i];
-                f32x4 s[P::TN][M::QUADS];
 #pragma unroll
                 for (int j = 0; j < P::TN; ++j)
 #pragma unroll
-                    for (int q = 0; q < M::QUADS; ++q) {
-                        const f32x4 v = P::quad(acc, i, j, q), bias = *reinterpret_cast<const f32x4*>(s_bias + P::wave_n() + j * M::SIDE + quad_n<DT>(q));
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            s[j][q][e] = fmaf(v[e], LOG2E, bias[e]);
-                            most = fmaxf(most, s[j][q][e]);
-                        }
-                    }
-                float more = 0.f;
+                    for (int e = 0; e < 4 * M::QUADS; ++e) most = fmaxf(most, acc[i][j][e]);
+                float more[2] = {0.f, 0.f};
 #pragma unroll
                 for (int j = 0; j < P::TN; ++j)
 #pragma unroll
-                    for (int q = 0; q < M::QUADS; ++q)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) more += __builtin_amdgcn_exp2f(s[j][q][e] - most);
-                sum[i] = sum[i] * __builtin_amdgcn_exp2f(top[i] - most) + more;
+                    for (int e = 0; e < 4 * M::QUADS; ++e) more[e & 1] += __builtin_amdgcn_exp2f((acc[i][j][e] - most) * LOG2E);
+                sum[i] = sum[i] * __builtin_amdgcn_exp2f((top[i] - most) * LOG2E) + (more[0] + more[1]);
                 top[i] = most;
-                // The label's own logit, in the one tile that has it.
+                // The label's own logit, in the one tile that has it: row after row, the value's place is the same for all lanes.
+                const int64_t m = m0 + P::wave_m() + i * M::SIDE + lane_m<DT>();
                 const int64_t label = m < n ? p.label[m] : -1, rel = label - n0 - P::wave_n();
-                const bool here = label >= 0 && rel >= 0 && rel < P::TN * M::SIDE;
-                if (__builtin_amdgcn_ballot_w64(here)) {
+                const bool here = label >= 0 && rel >= 0 && rel < P::COLUMNS;
+                for (uint64_t who = __builtin_amdgcn_ballot_w64(here) & (~uint64_t(0) >> (64 - M::SIDE)); who; who &= who - 1) {
+                    const int lane = __builtin_ctzll(who), c = __builtin_amdgcn_readlane(int(rel), lane);
 #pragma unroll
                     for (int j = 0; j < P::TN; ++j)
 #pragma unroll
-                        for (int q = 0; q < M::QUADS; ++q)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                if (here && rel == j * M::SIDE + quad_n<DT>(q) + e) p.right[m] = s[j][q][e];
+                        for (int e = 0; e < 4 * M::QUADS; ++e)
+                            if ((threadIdx.x & (M::SIDE - 1)) == lane && c == j * M::SIDE + quad_n<DT>(e / 4) + e % 4) p.right[m] = acc[i][j][e];
                 }
             }
         }
 #pragma unroll
         for (int i = 0; i < P::TM; ++i) {
             const float most = over_quads<DT>(top[i], [](float x, float y) { return fmaxf(x, y); });
-            const float s = over_quads<DT>(sum[i] * __builtin_amdgcn_exp2f(top[i] - most), [](float x, float y) { return x + y; });
-            const int at = P::wave_m() + i * M::SIDE + lane_m<DT>(), w = P::wave_n() / (P::TN * M::SIDE);
-            s_top[w][at] = most, s_sum[w][at] = s;
+            const float s = over_quads<DT>(sum[i] * __builtin_amdgcn_exp2f((top[i] - most) * LOG2E), [](float x, float y) { return x + y; });
+            const int at = P::wave_n() / P::COLUMNS * P::BM + P::wave_m() + i * M::SIDE + lane_m<DT>();
+            s_top[at] = most, s_sum[at] = s;
         }
         __syncthreads();
-        if (threadIdx.x < BM) {
-            float most = s_top[0][threadIdx.x], s = 0.f;
+        if (threadIdx.x < P::BM) {
+            float most = s_top[threadIdx.x], s = 0.f;
 #pragma unroll
-            for (int w = 1; w < WN; ++w) most = fmaxf(most, s_top[w][threadIdx.x]);
+            for (int w = 1; w < P::WN; ++w) most = fmaxf(most, s_top[w * P::BM + threadIdx.x]);
 #pragma unroll
-            for (int w = 0; w < WN; ++w) s += s_sum[w][threadIdx.x] * __builtin_amdgcn_exp2f(s_top[w][threadIdx.x] - most);
-            p.maxima[g * p.padded + m0 + threadIdx.x] = most;
-            p.sums[g * p.padded + m0 + threadIdx.x] = s;
+            for (int w = 0; w < P::WN; ++w) s += s_sum[w * P::BM + threadIdx.x] * __builtin_amdgcn_exp2f((s_top[w * P::BM + threadIdx.x] - most) * LOG2E);
+            p.maxima[g * parts.pitch + m0 + threadIdx.x] = most;
+            p.sums[g * parts.pitch + m0 + threadIdx.x] = s;
         }
     }
 }
 
-// The rows' losses and what the gradient needs of them; their sum by the workgroup that ends last.  A workgroup has 64 rows, its waves share the groups of columns out.
+// Many rows: a workgroup of eight waves to a CU.  Few: two of four waves, tiles of as many rows as there are.  (Two kernels, of which one ends at once: with all heights in one the compiler kept
+// some 100 scalar and a few vector registers in memory, and 8192 rows took 2520 us instead of LOGITS_MANY.)
 template <int DT>
-__global__ __launch_bounds__(256) void loss_finish_kernel(Loss p) {
-    __shared__ float s_top[4][64], s_sum[4][64];
-    __shared__ double s_all[256];
+using Logits256 = Product<DT, 256, 256, 2, 4, 2, false, false>;
+template <int DT>
+using Logits128 = Product<DT, 128, 128, 2, 2, 4, false, false, 64>;
+template <int DT>
+using Logits64 = Product<DT, 64, 128, 1, 4, 6, false, false, 64>;
+template <int DT>
+using Logits32 = Product<DT, 32, 128, 1, 4, 3, false, false, 128>;
+constexpr int MANY_SHARED = Logits256<TDB_BF16>::SHARED, FEW_SHARED = Logits64<TDB_BF16>::SHARED;
+static_assert(Logits128<TDB_BF16>::SHARED <= FEW_SHARED && Logits32<TDB_BF16>::SHARED <= FEW_SHARED, "");
+
+template <int DT>
+__global__ __launch_bounds__(512, 2) void loss_logits_many_kernel(Loss p) {
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    __shared__ __attribute__((aligned(16))) float s_bias[256];
+    __shared__ float s_top[1024], s_sum[1024];
+    const int n = p.count[0];
+    if (tile_rows(n, 32) == 256) logits_body<DT, Logits256<DT>>(p, n, smem, s_bias, s_top, s_sum);
+}
+template <int DT>
+__global__ __launch_bounds__(256, 2) void loss_logits_few_kernel(Loss p) {
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    __shared__ __attribute__((aligned(16))) float s_bias[128];
+    __shared__ float s_top[256], s_sum[256];
+    const int n = p.count[0];
+    switch (tile_rows(n, 32)) {
+        case 32: return logits_body<DT, Logits32<DT>>(p, n, smem, s_bias, s_top, s_sum);
+        case 64: return logits_body<DT, Logits64<DT>>(p, n, smem, s_bias, s_top, s_sum);
+        case 128: return logits_body<DT, Logits128<DT>>(p, n, smem, s_bias, s_top, s_sum);
+    }
+}
+
+// The rows' losses and what the gradient needs of them; their sum by the workgroup that ends last.  A workgroup has 32 rows, 32 groups of threads share the parts of each.
+template <int DT>
+__global__ __launch_bounds__(1024) void loss_finish_kernel(Loss p) {
+    __shared__ float s_top[32][33], s_sum[32][33];
+    __shared__ double s_all[1024];
     __shared__ bool s_last;
-    const int n = p.count[0], l = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int groups = (p.column_tiles + p.group - 1) / p.group, fill = (n + TILE - 1) / TILE * TILE;
+    const int n = p.count[0], l = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const Partials parts(p, tile_rows(n, 32) == 256);
+    const int groups = int(parts.groups);
     double mine = 0.0;
-    for (int64_t r0 = int64_t(blockIdx.x) * FINISH_ROWS; r0 < fill; r0 += int64_t(gridDim.x) * FINISH_ROWS) {
-        const int64_t r = r0 + l;
+    for (int64_t r0 = int64_t(blockIdx.x) * FINISH_ROWS; r0 < n; r0 += int64_t(gridDim.x) * FINISH_ROWS) {
+        const int64_t r = min(r0 + l, int64_t(n - 1));
         float top = -FLT_MAX, sum = 0.f;
-        if (r < n)
-            for (int g = w; g < groups; g += 16) {
-                float t[4], s[4];
+        for (int g = w; g < groups; g += 32 * 8) {
+            float t[8], s[8];
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const int at = min(g + 4 * u, groups - 1);
-                    t[u] = p.maxima[at * p.padded + r], s[u] = p.sums[at * p.padded + r];
-                }
-                float most = top;
-#pragma unroll
-                for (int u = 0; u < 4; ++u)
-                    if (g + 4 * u < groups) most = fmaxf(most, t[u]);
-                sum *= __builtin_amdgcn_exp2f(top - most);
-#pragma unroll
-                for (int u = 0; u < 4; ++u)
-                    if (g + 4 * u < groups) sum += s[u] * __builtin_amdgcn_exp2f(t[u] - most);
-                top = most;
+            for (int u = 0; u < 8; ++u) {
+                const int64_t at = min(g + 32 * u, groups - 1) * parts.pitch + r;
+                t[u] = g + 32 * u < groups ? p.maxima[at] : -FLT_MAX, s[u] = g + 32 * u < groups ? p.sums[at] : 0.f;
             }
-        __syncthreads();
-        s_top[w][l] = top, s_sum[w][l] = sum;
-        __syncthreads();
-        if (w == 0) {
+            float most = top;
 #pragma unroll
-            for (int v = 0; v < 4; ++v) top = fmaxf(top, s_top[v][l]);
-            sum = 0.f;
+            for (int u = 0; u < 8; ++u) most = fmaxf(most, t[u]);
+            sum *= __builtin_amdgcn_exp2f((top - most) * LOG2E);
 #pragma unroll
-            for (int v = 0; v < 4; ++v) sum += s_sum[v][l] * __builtin_amdgcn_exp2f(s_top[v][l] - top);
-            if (r < n) {
-                const float loss = ((top - p.right[r]) + log2f(sum)) * LN2;
-                p.top[r] = p.label[r] < 0 ? __builtin_nanf("") : top;
-                p.inverse[r] = D_SCALE<DT> / sum;
-                if (p.reduction == 0) p.loss[p.index[r]] = loss;
-                mine += loss;
-            } else if (r < fill) {
-                p.top[r] = 0.f, p.inverse[r] = 0.f;
-            }
+            for (int u = 0; u < 8; ++u) sum += s[u] * __builtin_amdgcn_exp2f((t[u] - most) * LOG2E);
+            top = most;
+        }
+        __syncthreads();
+        s_top[l][w] = top, s_sum[l][w] = sum;
+        __syncthreads();
+        // A row for each half wave.
+        top = s_top[w][l], sum = s_sum[w][l];
+        float most = top;
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
+        sum *= __builtin_amdgcn_exp2f((top - most) * LOG2E);
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
+        const int64_t row = r0 + w;
+        if (l == 0 && row < n) {
+            const float loss = (most - p.right[row]) + log2f(sum) * LN2;
+            p.top[row] = p.label[row] < 0 ? __builtin_nanf("") : most;
+            p.inverse[row] = D_SCALE<DT> / sum;
+            if (p.reduction == 0) p.loss[p.index[row]] = loss;
+            mine += loss;
         }
     }
     if (p.reduction == 0) return;
-    s_all[threadIdx.x] = mine;
-    __syncthreads();
-    for (int d = 32; d > 0; d >>= 1) {
-        if (threadIdx.x < d) s_all[threadIdx.x] += s_all[threadIdx.x + d];
+    auto total = [&](double x) {
         __syncthreads();
-    }
+        s_all[threadIdx.x] = x;
+        for (int d = 512; d > 0; d >>= 1) {
+            __syncthreads();
+            if (threadIdx.x < d) s_all[threadIdx.x] += s_all[threadIdx.x + d];
+        }
+    };
+    total(mine);
     if (threadIdx.x == 0) {
         __hip_atomic_store(p.block_sums + blockIdx.x, s_all[0], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         s_last = __hip_atomic_fetch_add(p.count + 1, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == int(gridDim.x) - 1;
@@ -272,13 +343,8 @@ __global__ __launch_bounds__(256) void loss_finish_kernel(Loss p) {
     __syncthreads();
     if (!s_last) return;
     double sum = 0.0;
-    for (unsigned i = threadIdx.x; i < gridDim.x; i += 256) sum += __hip_atomic_load(p.block_sums + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    s_all[threadIdx.x] = sum;
-    __syncthreads();
-    for (int d = 128; d > 0; d >>= 1) {
-        if (threadIdx.x < d) s_all[threadIdx.x] += s_all[threadIdx.x + d];
-        __syncthreads();
-    }
+    for (unsigned i = threadIdx.x; i < gridDim.x; i += 1024) sum += __hip_atomic_load(p.block_sums + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    total(sum);
     if (threadIdx.x == 0) p.loss[0] = float(p.reduction == 2 ? s_all[0] / double(n) : s_all[0]);
 }
 
@@ -301,85 +367,123 @@ struct Gradient {
     bool wide_dweight, later;   // later: a piece that is not the first
 };
 
-// D of a piece of the vocabulary.
-template <int DT, class P, int BM, int BN, int WM, bool WEIGHTED>
-__global__ __launch_bounds__(P::WAVES * 64, 2) void loss_difference_kernel(Loss p, Gradient g) {
-    extern __shared__ __attribute__((aligned(1024))) char smem[];
-    __shared__ float s_bias[BN], s_column[WM][BN];
+// D of a piece of the vocabulary, and its sums over the rows of a tile.
+template <int DT, class P, bool WEIGHTED>
+__device__ __forceinline__ void difference_body(const Loss& p, const Gradient& g, int n, char* smem, float* s_bias, float* s_column) {
     using M = Matrix<DT>;
-    const int n = p.count[0];
-    const int64_t row_tiles = (n + BM - 1) / BM, column_tiles = g.columns / BN, all = row_tiles * column_tiles;
-    const Rows a{p.gathered, p.pitch, p.padded, uint32_t(p.pitch)}, b{p.w, p.w_pitch, p.vocab, uint32_t((p.hidden * sizeof(typename M::T) + 15) / 16 * 16)};
+    using T = typename M::T;
+    constexpr int N = P::TN * M::QUADS * 4;     // values of a lane in a row
+    const int64_t row_tiles = (n + P::BM - 1) / P::BM, column_tiles = g.columns / P::BN, all = row_tiles * column_tiles;
     for (int64_t block = blockIdx.x; block < all; block += gridDim.x) {
         int64_t row, column, split;
         tile_of(block, row_tiles, column_tiles, 1, row, column, split);
-        const int64_t m0 = row * BM, n0 = g.first + column * BN;
+        const int64_t m0 = row * P::BM, n0 = g.first + column * P::BN;
         typename P::Acc acc;
-        P::run(smem, a, b, m0, n0, 0, p.pitch / 128, acc);
-        stage_bias<DT, BN>(p, n0, s_bias);
+        logits_of<DT, P>(p, n, smem, s_bias, m0, n0, acc);
         float top[P::TM], scale[P::TM], share[P::TM], shift[P::TM];
         int rel[P::TM];
 #pragma unroll
         for (int i = 0; i < P::TM; ++i) {
-            const int64_t m = m0 + P::wave_m() + i * M::SIDE + lane_m<DT>();
-            top[i] = p.top[m], scale[i] = WEIGHTED ? g.scale[m] : p.inverse[m];
-            share[i] = WEIGHTED ? g.share[m] : D_SCALE<DT>, shift[i] = WEIGHTED && DT == TDB_F16 ? g.shift[m] : 1.f;
-            rel[i] = m < n ? p.label[m] - int(n0) - P::wave_n() : -1;
+            const int64_t m = m0 + P::wave_m() + i * M::SIDE + lane_m<DT>(), at = min(m, int64_t(n - 1));
+            top[i] = m < n ? p.top[at] : INFINITY;      // (rows that are not there: zeros)
+            scale[i] = WEIGHTED ? g.scale[at] : p.inverse[at];
+            share[i] = WEIGHTED ? g.share[at] : D_SCALE<DT>, shift[i] = WEIGHTED && DT == TDB_F16 ? g.shift[at] : 1.f;
+            const int label = p.label[at];
+            rel[i] = m < n && label >= 0 ? label - int(n0) - P::wave_n() : -1;
         }
+        float sums[N];
+#pragma unroll
+        for (int c = 0; c < N; ++c) sums[c] = 0.f;
+        P::store(
+            smem, g.d + m0 * g.d_pitch + (n0 - g.first) * int64_t(sizeof(T)), g.d_pitch, P::BM, P::BN, true,
+            [&](int i, int j, int q) {
+                const f32x4 v = P::quad(acc, i, j, q);
+                f32x4 d;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    d[e] = __builtin_amdgcn_exp2f((v[e] - top[i]) * LOG2E) * scale[i];
+                    sums[(j * M::QUADS + q) * 4 + e] += d[e] * shift[i];
+                }
+                return d;
+            },
+            [&](int i, char* rows) {    // the label's own value
+                if (rel[i] >= 0 && rel[i] < P::COLUMNS && (threadIdx.x & 63) < M::SIDE) {
+                    const float right = p.right[m0 + P::wave_m() + i * M::SIDE + lane_m<DT>()];
+                    *reinterpret_cast<T*>(rows + lane_m<DT>() * P::PITCH + rel[i] * int(sizeof(T))) = T(__builtin_amdgcn_exp2f((right - top[i]) * LOG2E) * scale[i] - share[i]);
+                }
+            });
+        if (!g.dbias) continue;
+        float sum = over_m<DT>(sums);
+        const int c = lane_m<DT>() % N, mine = c / (4 * M::QUADS) * M::SIDE + quad_n<DT>(c / 4 % M::QUADS) + c % 4;     // the lane's column
+#pragma unroll
+        for (int i = 0; i < P::TM; ++i)
+            for (uint64_t who = __builtin_amdgcn_ballot_w64(rel[i] >= 0 && rel[i] < P::COLUMNS) & (~uint64_t(0) >> (64 - M::SIDE)); who; who &= who - 1) {
+                const int lane = __builtin_ctzll(who);
+                const float less = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, share[i] * shift[i]), lane));
+                sum -= __builtin_amdgcn_readlane(rel[i], lane) == mine ? less : 0.f;
+            }
+        if (lane_m<DT>() < N) s_column[P::wave_m() / (P::TM * M::SIDE) * P::BN + P::wave_n() + mine] = sum;
         __syncthreads();
-        float sums[P::TN * M::QUADS * 4];
+        if (threadIdx.x < P::BN) {
+            float all = 0.f;
 #pragma unroll
-        for (int c = 0; c < P::TN * M::QUADS * 4; ++c) sums[c] = 0.f;
-        P::store(smem, g.d, g.d_pitch, m0, p.padded, n0 - g.first, g.columns, true, [&](int i, int j, int q) {
-            const f32x4 v = P::quad(acc, i, j, q), bias = *reinterpret_cast<const f32x4*>(s_bias + P::wave_n() + j * M::SIDE + quad_n<DT>(q));
-            f32x4 d;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) d[e] = __builtin_amdgcn_exp2f(fmaf(v[e], LOG2E, bias[e]) - top[i]) * scale[i];
-            const int at = rel[i] - j * M::SIDE - quad_n<DT>(q);
-            if (__builtin_amdgcn_ballot_w64(at >= 0 && at < 4)) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) d[e] -= at == e ? share[i] : 0.f;
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sums[(j * M::QUADS + q) * 4 + e] += d[e] * shift[i];
-            return d;
-        });
-        if (g.dbias) {
-            const float sum = over_m<DT>(sums);
-            constexpr int N = P::TN * M::QUADS * 4;
-            const int c = lane_m<DT>() % N;     // the value that the lane has
-            if (lane_m<DT>() < N) s_column[P::wave_m() / (P::TM * M::SIDE)][P::wave_n() + c / (4 * M::QUADS) * M::SIDE + quad_n<DT>(c / 4 % M::QUADS) + c % 4] = sum;
-            __syncthreads();
-            if (threadIdx.x < BN) {
-                float all = 0.f;
-#pragma unroll
-                for (int w = 0; w < WM; ++w) all += s_column[w][threadIdx.x];
-                g.column_sums[row * g.columns + n0 - g.first + threadIdx.x] = all;
-            }
+            for (int w = 0; w < P::WM; ++w) all += s_column[w * P::BN + threadIdx.x];
+            g.column_sums[row * g.columns + n0 - g.first + threadIdx.x] = all;
         }
     }
 }
 
-// Parts of dx: D W over a share of the piece's columns.
-template <int DT, class P, int BM, int BN>
-__global__ __launch_bounds__(P::WAVES * 64, 2) void loss_dx_kernel(Loss p, Gradient g) {
+template <int DT, bool WEIGHTED>
+__global__ __launch_bounds__(512, 2) void loss_difference_many_kernel(Loss p, Gradient g) {
     extern __shared__ __attribute__((aligned(1024))) char smem[];
-    using M = Matrix<DT>;
+    __shared__ __attribute__((aligned(16))) float s_bias[256];
+    __shared__ float s_column[512];
     const int n = p.count[0];
-    const int64_t row_tiles = (n + BM - 1) / BM, column_tiles = (p.hidden + BN - 1) / BN, tiles = row_tiles * column_tiles, steps = g.columns / P::STEP;
-    const int64_t splits = tiles ? max(int64_t(1), min(int64_t(gridDim.x) / tiles, steps)) : 0, all = tiles * splits;
-    const Rows a{g.d, g.d_pitch, p.padded, uint32_t(g.d_pitch)};
-    const Rows b{p.w + g.first * p.w_pitch, p.w_pitch, min(g.columns, p.vocab - g.first), uint32_t((p.hidden * sizeof(typename M::T) + 15) / 16 * 16)};
+    if (tile_rows(n, 32) == 256) difference_body<DT, Logits256<DT>, WEIGHTED>(p, g, n, smem, s_bias, s_column);
+}
+template <int DT, bool WEIGHTED>
+__global__ __launch_bounds__(256, 2) void loss_difference_few_kernel(Loss p, Gradient g) {
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    __shared__ __attribute__((aligned(16))) float s_bias[128];
+    __shared__ float s_column[256];
+    const int n = p.count[0];
+    switch (tile_rows(n, 32)) {
+        case 32: return difference_body<DT, Logits32<DT>, WEIGHTED>(p, g, n, smem, s_bias, s_column);
+        case 64: return difference_body<DT, Logits64<DT>, WEIGHTED>(p, g, n, smem, s_bias, s_column);
+        case 128: return difference_body<DT, Logits128<DT>, WEIGHTED>(p, g, n, smem, s_bias, s_column);
+    }
+}
+
+// How the workgroups of a launch share out the product of dx: over the tiles of rows and columns, and where they are more than tiles, over the contraction.
+template <int DT>
+struct Shares {
+    int height;
+    int64_t row_tiles, column_tiles, splits;
+    __device__ __forceinline__ Shares(const Loss& p, const Gradient& g, int n, int64_t blocks) {
+        height = tile_rows(n, 64);
+        row_tiles = (n + height - 1) / height, column_tiles = (p.hidden + 255) / 256;
+        const int64_t tiles = row_tiles * column_tiles;
+        splits = tiles ? max(int64_t(1), min(blocks / tiles, g.columns * int64_t(sizeof(typename Matrix<DT>::T)) / 128)) : 0;
+    }
+};
+
+// Parts of dx: D W over a share of the piece's columns.
+template <int DT, class P>
+__device__ __forceinline__ void dx_body(const Loss& p, const Gradient& g, int n, const Shares<DT>& share, char* smem) {
+    using M = Matrix<DT>;
+    const int64_t all = share.row_tiles * share.column_tiles * share.splits, steps = g.columns / P::STEP;
+    const Rows a{g.d, g.d_pitch, n, uint32_t(g.d_pitch)};
+    const Rows b{p.w + g.first * p.w_pitch, p.w_pitch, min(g.columns, p.vocab - g.first), weight_rows<DT>(p).width};
     for (int64_t block = blockIdx.x; block < all; block += gridDim.x) {
         int64_t row, column, split;
-        tile_of(block, row_tiles, column_tiles, splits, row, column, split);
-        const int64_t m0 = row * BM, n0 = column * BN;
+        tile_of(block, share.row_tiles, share.column_tiles, share.splits, row, column, split);
+        const int64_t m0 = row * P::BM, n0 = column * P::BN;
         typename P::Acc acc;
-        P::run(smem, a, b, m0, n0, steps * split / splits, steps * (split + 1) / splits, acc);
+        P::run(smem, a, b, m0, n0, steps * split / share.splits, steps * (split + 1) / share.splits, acc);
 #pragma unroll
         for (int i = 0; i < P::TM; ++i) {
             const int64_t m = m0 + P::wave_m() + i * M::SIDE + lane_m<DT>();
-            float* const to = g.parts + (split * row_tiles * BM + m) * g.part_pitch;
+            float* const to = g.parts + (split * share.row_tiles * P::BM + m) * g.part_pitch;
 #pragma unroll
             for (int j = 0; j < P::TN; ++j)
 #pragma unroll
@@ -395,17 +499,37 @@ __global__ __launch_bounds__(P::WAVES * 64, 2) void loss_dx_kernel(Loss p, Gradi
     }
 }
 
+template <int DT>
+using Dx256 = Product<DT, 256, 256, 2, 4, 2, false, true>;
+template <int DT>
+using Dx128 = Product<DT, 128, 256, 2, 4, 3, false, true>;
+template <int DT>
+using Dx64 = Product<DT, 64, 256, 1, 8, 3, false, true>;
+constexpr int DX_SHARED = Dx128<TDB_BF16>::SHARED;
+static_assert(Dx256<TDB_BF16>::SHARED <= DX_SHARED && Dx64<TDB_BF16>::SHARED <= DX_SHARED, "");
+
+template <int DT>
+__global__ __launch_bounds__(512, 2) void loss_dx_kernel(Loss p, Gradient g) {
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    const int n = p.count[0];
+    const Shares<DT> share(p, g, n, gridDim.x);
+    switch (share.height) {
+        case 64: return dx_body<DT, Dx64<DT>>(p, g, n, share, smem);
+        case 128: return dx_body<DT, Dx128<DT>>(p, g, n, share, smem);
+        default: return dx_body<DT, Dx256<DT>>(p, g, n, share, smem);
+    }
+}
+
 // What the gradient of a sum or mean makes of every row.
 __device__ __forceinline__ float row_factor(const Loss& p, const Gradient& g, int n) { return p.reduction == 2 ? g.dloss[0] / float(n) : g.dloss[0]; }
 
-// dx: a workgroup for each row, zeros where it does not count.  blocks, tiles: of the launch before.
+// dx: a workgroup for each row, its four waves share out the parts; zeros where the row does not count.  blocks: workgroups of the launch before.
 template <int DT>
-__global__ __launch_bounds__(256) void loss_dx_sum_kernel(Loss p, Gradient g, int blocks, int bm, int bn) {
+__global__ __launch_bounds__(256) void loss_dx_sum_kernel(Loss p, Gradient g, int blocks) {
     using T = typename Matrix<DT>::T;
-    constexpr int STEP = 128 / sizeof(T);
-    const int n = p.count[0];
-    const int64_t high = int64_t((n + bm - 1) / bm), tiles = high * ((p.hidden + bn - 1) / bn);
-    const int64_t splits = tiles ? max(int64_t(1), min(int64_t(blocks) / tiles, g.columns / STEP)) : 0;
+    __shared__ float s_sum[4][256];
+    const int n = p.count[0], l = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const Shares<DT> share(p, g, n, blocks);
     for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
         const int place = p.place[row];
         T* const to = static_cast<T*>(g.dx) + row * g.dx_stride;
@@ -414,11 +538,24 @@ __global__ __launch_bounds__(256) void loss_dx_sum_kernel(Loss p, Gradient g, in
             continue;
         }
         const float factor = (p.reduction ? row_factor(p, g, n) : *g.common * g.shift[place]) * (1.f / D_SCALE<DT>);
-        for (int c = threadIdx.x; c < p.hidden; c += 256) {
-            float sum = 0.f;
-#pragma unroll 8
-            for (int64_t s = 0; s < splits; ++s) sum += g.parts[(s * high * bm + place) * g.part_pitch + c];
-            to[c] = T(sum * factor);
+        const float* const from = g.parts + place * g.part_pitch;
+        const int64_t apart = share.row_tiles * share.height * g.part_pitch;
+        for (int c0 = 0; c0 < p.hidden; c0 += 256) {
+            const int64_t c = min(int64_t(c0 + 4 * l), g.part_pitch - 4);
+            f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+            for (int64_t s = w; s < share.splits; s += 16) {
+                f32x4 x[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) x[u] = *reinterpret_cast<const f32x4*>(from + min(s + 4 * u, share.splits - 1) * apart + c);
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (s + 4 * u < share.splits) sum += x[u];
+            }
+            __syncthreads();
+            *reinterpret_cast<f32x4*>(&s_sum[w][4 * l]) = sum;
+            __syncthreads();
+            const int at = c0 + threadIdx.x;
+            if (at < p.hidden) to[at] = T((((s_sum[0][threadIdx.x] + s_sum[1][threadIdx.x]) + s_sum[2][threadIdx.x]) + s_sum[3][threadIdx.x]) * factor);
         }
     }
 }
@@ -428,7 +565,7 @@ template <int DT>
 __global__ __launch_bounds__(256) void loss_weigh_kernel(Loss p, Gradient g) {
     using T = typename Matrix<DT>::T;
     __shared__ float s_most[4];
-    const int n = p.count[0], l = threadIdx.x & 63, w = threadIdx.x >> 6, fill = (n + TILE - 1) / TILE * TILE;
+    const int n = p.count[0], l = threadIdx.x & 63, w = threadIdx.x >> 6;
     float most = 0.f;
     for (int r = threadIdx.x; r < n; r += 256) most = fmaxf(most, fabsf(g.dloss[p.index[r] * g.dloss_stride]));
 #pragma unroll
@@ -438,8 +575,8 @@ __global__ __launch_bounds__(256) void loss_weigh_kernel(Loss p, Gradient g) {
     most = fmaxf(fmaxf(s_most[0], s_most[1]), fmaxf(s_most[2], s_most[3]));
     const int common = most > 0.f && most < INFINITY ? ilogbf(most) : 0;
     if (blockIdx.x == 0 && threadIdx.x == 0) *g.common = ldexpf(1.f, common);
-    for (int r = blockIdx.x * 4 + w; r < fill; r += gridDim.x * 4) {
-        const float weight = r < n ? g.dloss[p.index[r] * g.dloss_stride] : 0.f;
+    for (int r = blockIdx.x * 4 + w; r < n; r += gridDim.x * 4) {
+        const float weight = g.dloss[p.index[r] * g.dloss_stride];
         const int own = DT == TDB_F16 && weight != 0.f && fabsf(weight) < INFINITY ? ilogbf(weight) : common;
         const float share = ldexpf(weight, -own), shift = ldexpf(1.f, own - common);
         if (l == 0) g.scale[r] = p.inverse[r] * share, g.share[r] = D_SCALE<DT> * share, g.shift[r] = shift;
@@ -452,15 +589,20 @@ __global__ __launch_bounds__(256) void loss_weigh_kernel(Loss p, Gradient g) {
 }
 
 // dW and dbias of a piece.
-template <int DT, class P, int BM, int BN>
-__global__ __launch_bounds__(P::WAVES * 64, 2) void loss_dweight_kernel(Loss p, Gradient g) {
+template <int DT>
+using Dweight = Product<DT, 256, 256, 2, 4, 2, true, true>;
+
+template <int DT>
+__global__ __launch_bounds__(512, 2) void loss_dweight_kernel(Loss p, Gradient g) {
     extern __shared__ __attribute__((aligned(1024))) char smem[];
-    using M = Matrix<DT>;
-    using T = typename M::T;
+    using P = Dweight<DT>;
+    using T = typename Matrix<DT>::T;
+    constexpr int BM = P::BM, BN = P::BN;
     const int n = p.count[0];
     const int64_t columns = min(g.columns, p.vocab - g.first), row_tiles = (columns + BM - 1) / BM, column_tiles = g.dweight ? (p.hidden + BN - 1) / BN : 1, all = row_tiles * column_tiles;
     const int64_t steps = (n + P::STEP - 1) / P::STEP;
-    const Rows a{g.d, g.d_pitch, p.padded, uint32_t(g.d_pitch)}, b{g.shifted, p.pitch, p.padded, uint32_t(p.pitch)};
+    const Rows a{g.d, g.d_pitch, n, uint32_t(g.d_pitch)}, b{g.shifted, p.pitch, n, uint32_t(p.pitch)};
+    const int heights = n ? (n + tile_rows(n, 32) - 1) / tile_rows(n, 32) : 0;
     const float factor = n == 0 ? 0.f : (p.reduction ? row_factor(p, g, n) : *g.common) * (1.f / D_SCALE<DT>);
     for (int64_t block = blockIdx.x; block < all; block += gridDim.x) {
         int64_t row, column, split;
@@ -468,19 +610,22 @@ __global__ __launch_bounds__(P::WAVES * 64, 2) void loss_dweight_kernel(Loss p, 
         const int64_t m0 = row * BM, n0 = column * BN, m = m0 + threadIdx.x;
         if (g.dbias && column == 0 && threadIdx.x < BM && m < columns) {
             float sum = 0.f;
-            for (int t = 0; t < (n + TILE - 1) / TILE; ++t) sum += g.column_sums[t * g.columns + m];
+            for (int t = 0; t < heights; ++t) sum += g.column_sums[t * g.columns + m];
             if (p.bias_kind == 2) static_cast<float*>(g.dbias)[g.first + m] = sum * factor;
             else static_cast<T*>(g.dbias)[g.first + m] = T(sum * factor);
         }
         if (!g.dweight) continue;
         typename P::Acc acc;
         P::run(smem, a, b, m0, n0, 0, steps, acc);
-        P::store(smem, g.dweight + g.first * g.dweight_pitch, g.dweight_pitch, m0, columns, n0, p.hidden, g.wide_dweight, [&](int i, int j, int q) {
-            f32x4 v = P::quad(acc, i, j, q);
+        P::store(
+            smem, g.dweight + (g.first + m0) * g.dweight_pitch + n0 * int64_t(sizeof(T)), g.dweight_pitch, columns - m0, p.hidden - n0, g.wide_dweight,
+            [&](int i, int j, int q) {
+                f32x4 v = P::quad(acc, i, j, q);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] *= factor;
-            return v;
-        });
+                for (int e = 0; e < 4; ++e) v[e] *= factor;
+                return v;
+            },
+            [](int, char*) {});
     }
 }
 
@@ -494,12 +639,13 @@ int64_t round_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 struct Plan {
     int size;                               // of a value
     int64_t padded, pitch, vocab;           // rows and bytes of the gathered rows, vocabulary, rounded up
-    int32_t column_tiles, group, groups;
+    int32_t group;
+    bool many, few;                         // whether there may be as many or as few rows as the kernels are for
     int64_t columns;                        // of a piece
     int blocks, finish_blocks;
     // offsets
-    int64_t index, place, label, top, inverse, gathered, state;
-    int64_t right, maxima, sums, block_sums, forward;
+    int64_t index, place, label, top, inverse, right, gathered, state;
+    int64_t maxima, sums, block_sums, forward;
     int64_t d, parts, part_pitch, column_sums, shifted, scale, share, shift, common, backward;
 };
 
@@ -509,31 +655,32 @@ Plan plan_of(const tdb_loss_args& a) {
     p.padded = round_up(std::max<int64_t>(a.rows, 1), TILE);
     p.pitch = round_up(int64_t(a.hidden) * p.size, 128);
     p.vocab = round_up(a.vocab, TILE);
-    p.column_tiles = int32_t(p.vocab / TILE);
-    p.group = int32_t((int64_t(p.column_tiles) * p.padded * 8 + PARTIAL_BYTES - 1) / PARTIAL_BYTES);
-    p.groups = (p.column_tiles + p.group - 1) / p.group;
-    const int64_t most = std::min<int64_t>(std::max<int64_t>(D_BYTES / (p.padded * p.size) / TILE, 1), (int64_t(1) << 22) / p.size / TILE), pieces = (p.column_tiles + most - 1) / most;
-    p.columns = (p.column_tiles + pieces - 1) / pieces * TILE;
+    const int64_t wide = p.vocab / TILE;
+    p.group = int32_t((wide * p.padded * 8 + PARTIAL_BYTES - 1) / PARTIAL_BYTES);
+    p.many = a.rows > 128, p.few = a.rows > 0;
+    const int64_t most = std::min<int64_t>(std::max<int64_t>(D_BYTES / (p.padded * p.size) / TILE, 1), (int64_t(1) << 22) / p.size / TILE), pieces = (wide + most - 1) / most;
+    p.columns = (wide + pieces - 1) / pieces * TILE;
     p.blocks = std::max(8, tdb_compute_units(-1) & -8);
-    p.finish_blocks = int(std::min<int64_t>(p.padded / FINISH_ROWS, 1024));
+    p.finish_blocks = int(std::min<int64_t>((std::max<int64_t>(a.rows, 1) + FINISH_ROWS - 1) / FINISH_ROWS, 512));
     int64_t at = 256;
     auto take = [&](int64_t bytes) {
         const int64_t here = at;
         at += round_up(bytes, 256);
         return here;
     };
-    p.index = take(p.padded * 4), p.place = take(p.padded * 4), p.label = take(p.padded * 4), p.top = take(p.padded * 4), p.inverse = take(p.padded * 4);
+    p.index = take(p.padded * 4), p.place = take(p.padded * 4), p.label = take(p.padded * 4), p.top = take(p.padded * 4), p.inverse = take(p.padded * 4), p.right = take(p.padded * 4);
     p.gathered = take(p.padded * p.pitch);
     p.state = at;
     at = 0;
-    p.right = take(p.padded * 4), p.maxima = take(p.groups * p.padded * 4), p.sums = take(p.groups * p.padded * 4), p.block_sums = take(p.finish_blocks * 8);
+    const int64_t partials = std::max((wide + p.group - 1) / p.group * p.padded, 2 * wide * std::min<int64_t>(p.padded, FEW)) * 4;
+    p.maxima = take(partials), p.sums = take(partials), p.block_sums = take(p.finish_blocks * 8);
     p.forward = at;
     at = 0;
     p.part_pitch = round_up(a.hidden, 4);
     // As many parts of dx as workgroups share its tiles, or one.
     p.d = take(p.padded * p.columns * p.size);
     p.parts = take(std::max(p.padded, int64_t(p.blocks) * TILE) * std::max<int64_t>(p.part_pitch, 1) * 4);
-    p.column_sums = take(p.padded / TILE * p.columns * 4);
+    p.column_sums = take(std::max<int64_t>(p.padded / TILE, std::min<int64_t>(p.padded, FEW) / 32) * p.columns * 4);
     const bool weighted = a.reduction == 0;
     p.shifted = take(weighted && a.dtype == TDB_F16 ? p.padded * p.pitch : 0);
     p.scale = take(weighted ? p.padded * 4 : 0), p.share = take(weighted ? p.padded * 4 : 0), p.shift = take(weighted ? p.padded * 4 : 0), p.common = take(4);
@@ -577,8 +724,8 @@ Loss loss_of(const tdb_loss_args& a, const Plan& p) {
     k.hidden = a.hidden, k.reduction = a.reduction, k.bias_kind = !a.bias ? 0 : a.bias_dtype == a.dtype ? 1 : 2, k.loss = a.loss;
     k.count = reinterpret_cast<int32_t*>(state), k.index = reinterpret_cast<int32_t*>(state + p.index), k.place = reinterpret_cast<int32_t*>(state + p.place);
     k.label = reinterpret_cast<int32_t*>(state + p.label), k.top = reinterpret_cast<float*>(state + p.top), k.inverse = reinterpret_cast<float*>(state + p.inverse);
-    k.gathered = state + p.gathered, k.pitch = p.pitch, k.padded = p.padded, k.column_tiles = p.column_tiles, k.group = p.group;
-    k.right = reinterpret_cast<float*>(work + p.right), k.maxima = reinterpret_cast<float*>(work + p.maxima), k.sums = reinterpret_cast<float*>(work + p.sums);
+    k.gathered = state + p.gathered, k.pitch = p.pitch, k.padded = p.padded, k.group = p.group;
+    k.right = reinterpret_cast<float*>(state + p.right), k.maxima = reinterpret_cast<float*>(work + p.maxima), k.sums = reinterpret_cast<float*>(work + p.sums);
     k.block_sums = reinterpret_cast<double*>(work + p.block_sums);
     return k;
 }
@@ -609,10 +756,10 @@ hipError_t forward(const tdb_loss_args& a, hipStream_t s) {
     const Loss k = loss_of(a, p);
     const int64_t chunk = round_up(std::max<int64_t>(64, (a.rows + 511) / 512), 64);
     const bool wide = reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.x_stride * p.size % 16 == 0 && int64_t(a.hidden) * p.size % 16 == 0;
-    TDB_TRY(launch<loss_gather_kernel<DT>>(std::max<int64_t>(1, (a.rows + chunk - 1) / chunk), 256, 0, s, k, chunk, wide));
-    using P = Product<DT, 256, 256, 2, 4, 2, false, false>;
-    if (a.rows) TDB_TRY(launch<loss_logits_kernel<DT, P, 256, 256, 4>>(p.blocks, P::WAVES * 64, P::SHARED, s, k));
-    return launch<loss_finish_kernel<DT>>(p.finish_blocks, 256, 0, s, k);
+    TDB_TRY(launch<loss_gather_kernel<DT>>(std::max<int64_t>(1, (a.rows + chunk - 1) / chunk), 64 * GATHER_WAVES, 0, s, k, chunk, wide));
+    if (p.few) TDB_TRY(launch<loss_logits_few_kernel<DT>>(2 * p.blocks, 256, FEW_SHARED, s, k));
+    if (p.many) TDB_TRY(launch<loss_logits_many_kernel<DT>>(p.blocks, 512, MANY_SHARED, s, k));
+    return launch<loss_finish_kernel<DT>>(p.finish_blocks, 1024, 0, s, k);
 }
 
 template <int DT>
@@ -630,19 +777,21 @@ hipError_t backward(const tdb_loss_args& a, hipStream_t s) {
     g.scale = floats(p.scale), g.share = floats(p.share), g.shift = floats(p.shift), g.common = floats(p.common), g.column_sums = floats(p.column_sums);
     g.wide_dweight = reinterpret_cast<uintptr_t>(a.dweight) % 16 == 0 && g.dweight_pitch % 16 == 0 && int64_t(a.hidden) * p.size % 16 == 0;
     if (weighted && a.rows) TDB_TRY(launch<loss_weigh_kernel<DT>>(std::min<int64_t>(p.padded / 16, 1024), 256, 0, s, k, g));
-    using Lined = Product<DT, 256, 256, 2, 4, 2, false, false>;
-    using Across = Product<DT, 256, 256, 2, 4, 2, false, true>;
-    using Turned = Product<DT, 256, 256, 2, 4, 2, true, true>;
     for (g.first = 0; g.first < a.vocab; g.first += p.columns) {
         g.columns = std::min(p.columns, p.vocab - g.first), g.later = g.first > 0;
-        if (a.rows && weighted) TDB_TRY(launch<loss_difference_kernel<DT, Lined, 256, 256, 2, true>>(p.blocks, Lined::WAVES * 64, Lined::SHARED, s, k, g));
-        else if (a.rows) TDB_TRY(launch<loss_difference_kernel<DT, Lined, 256, 256, 2, false>>(p.blocks, Lined::WAVES * 64, Lined::SHARED, s, k, g));
-        if (a.rows && a.dx) TDB_TRY(launch<loss_dx_kernel<DT, Across, 256, 256>>(p.blocks, Across::WAVES * 64, Across::SHARED, s, k, g));
-        if (a.dweight || a.dbias) TDB_TRY(launch<loss_dweight_kernel<DT, Turned, 256, 256>>(p.blocks, Turned::WAVES * 64, Turned::SHARED, s, k, g));
+        if (weighted) {
+            if (p.few) TDB_TRY(launch<loss_difference_few_kernel<DT, true>>(2 * p.blocks, 256, FEW_SHARED, s, k, g));
+            if (p.many) TDB_TRY(launch<loss_difference_many_kernel<DT, true>>(p.blocks, 512, MANY_SHARED, s, k, g));
+        } else {
+            if (p.few) TDB_TRY(launch<loss_difference_few_kernel<DT, false>>(2 * p.blocks, 256, FEW_SHARED, s, k, g));
+            if (p.many) TDB_TRY(launch<loss_difference_many_kernel<DT, false>>(p.blocks, 512, MANY_SHARED, s, k, g));
+        }
+        if (a.rows && a.dx) TDB_TRY(launch<loss_dx_kernel<DT>>(p.blocks, 512, DX_SHARED, s, k, g));
+        if (a.dweight || a.dbias) TDB_TRY(launch<loss_dweight_kernel<DT>>(p.blocks, 512, Dweight<DT>::SHARED, s, k, g));
     }
     if (a.rows && a.dx) {
         g.columns = p.columns;              // (what the parts of dx were shared out by: the first piece's)
-        TDB_TRY(launch<loss_dx_sum_kernel<DT>>(std::min<int64_t>(a.rows, 1 << 16), 256, 0, s, k, g, p.blocks, 256, 256));
+        TDB_TRY(launch<loss_dx_sum_kernel<DT>>(std::min<int64_t>(a.rows, 1 << 16), 256, 0, s, k, g, p.blocks));
     }
     return hipSuccess;
 }

@@ -96,20 +96,21 @@ __device__ __forceinline__ void step_barrier() { asm volatile("s_waitcnt lgkmcnt
 
 constexpr uint32_t PAST = 0x80000000u;      // past every buffer's end
 
-// One operand's share of a step: EXTENT rows of the tile (m or n).
-template <int DT, int EXTENT, bool TURNED, int WAVES>
+// One operand's share of a step: EXTENT rows of the tile (m or n), LINE bytes of each along the contraction (128 or 64).
+template <int DT, int EXTENT, bool TURNED, int WAVES, int LINE>
 struct Side {
     using M = Matrix<DT>;
     using T = typename M::T;
-    static constexpr int ES = sizeof(T), STEP = 128 / ES, BYTES = EXTENT * 128;
+    static constexpr int ES = sizeof(T), STEP = LINE / ES, BYTES = EXTENT * LINE;
     static constexpr int LOADS = BYTES / 1024 / WAVES;                 // of 1 KB, by each wave
-    static constexpr int ROW = TURNED ? EXTENT * ES : 128, CHUNKS = ROW / 16, BLOCKS = ROW / 64;
-    static_assert(LOADS * 1024 * WAVES == BYTES, "");
+    static constexpr int ROW = TURNED ? EXTENT * ES : LINE, CHUNKS = ROW / 16, BLOCKS = ROW / 64;
+    static_assert(LOADS * 1024 * WAVES == BYTES && (LINE == 128 || LINE == 64), "");
     uint32_t from[LOADS];       // of the lane, in the step's buffer
     uint32_t column[LOADS];     // lined: bytes into the row
 
-    // Lined: 16-byte chunk c of row r lies at c ^ (r / 2 % 8).  Turned: 64-byte block b of row k lies at b ^ turn(k), so that the four rows that a read of 16 bits takes
-    // together, or every fourth of float32, are on distinct banks.
+    // Lined: 16-byte chunk c of row r lies at c ^ swap(r), so that the 16 rows that LDS serves together (0..3, 12..15, 20..27 and the others) are on distinct banks.  Turned: 64-byte block b
+    // of row k lies at b ^ turn(k), so that the four rows that a read of 16 bits takes together, or every fourth of float32, are.
+    static __device__ __forceinline__ int swap(int r) { return LINE == 128 ? r >> 1 & 7 : r >> 2 & 3; }
     static __device__ __forceinline__ int turn(int k) { return (DT == TDB_F32 ? k >> 2 & 3 : (k & 3) | (k >> 1 & 4)) & (BLOCKS - 1); }
 
     // Tile of rows (lined) or columns (turned) first ..
@@ -122,7 +123,7 @@ struct Side {
                 const uint32_t c = ((((chunk >> 2) ^ turn(row)) << 2) | (chunk & 3)) * 16;
                 from[j] = c + uint32_t(first) * ES < a.width ? uint32_t(row) * uint32_t(a.pitch) + c : PAST;
             } else {
-                column[j] = (chunk ^ (row >> 1 & 7)) * 16;
+                column[j] = (chunk ^ swap(row)) * 16;
                 from[j] = uint32_t(row) * uint32_t(a.pitch) + column[j];
             }
         }
@@ -137,19 +138,19 @@ struct Side {
 #pragma unroll
             for (int j = 0; j < LOADS; ++j) load_shared(to + j * 1024, buffer, from[j]);
         } else {
-            const int64_t into = s * 128;
+            const int64_t into = s * LINE;
             const u32x4 buffer = buffer_of(a.p + first * a.pitch + into, (a.count - 1 - first) * a.pitch + a.width - into);
-            const bool whole = into + 128 <= a.width;
+            const bool whole = into + LINE <= a.width;
 #pragma unroll
             for (int j = 0; j < LOADS; ++j) load_shared(to + j * 1024, buffer, whole || into + column[j] < a.width ? from[j] : PAST);
         }
     }
-    // Frag of rows row .. (a multiple of SIDE), part kk of the step's 128 bytes (32 bytes, or 64 of float32)
+    // Frag of rows row .. (a multiple of SIDE), part kk of the step (32 bytes, or 64 of float32)
     __device__ __forceinline__ typename M::Frag frag(const char* lds, int row, int kk) const {
         const int l = threadIdx.x & 63;
         if constexpr (!TURNED) {
             const int r = row + lane_m<DT>(), chunk = DT == TDB_F32 ? 4 * kk + (l >> 4) : 2 * kk + (l >> 5);
-            return *reinterpret_cast<const typename M::Frag*>(lds + r * 128 + ((chunk ^ (r >> 1 & 7)) << 4));
+            return *reinterpret_cast<const typename M::Frag*>(lds + r * LINE + ((chunk ^ swap(r)) << 4));
         } else if constexpr (DT == TDB_F32) {
             f32x4 x;
 #pragma unroll
@@ -169,30 +170,28 @@ struct Side {
 };
 
 // BM x BN by WM x WN waves, NS stages in LDS.
-template <int DT, int BM, int BN, int WM, int WN, int NS, bool TURN_A, bool TURN_B>
+template <int DT, int BM_, int BN_, int WM_, int WN_, int NS, bool TURN_A, bool TURN_B, int LINE = 128>
 struct Product {
+    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, LINE_BYTES = LINE;
     using M = Matrix<DT>;
     using T = typename M::T;
-    static constexpr int WAVES = WM * WN, TM = BM / WM / M::SIDE, TN = BN / WN / M::SIDE, PARTS = DT == TDB_F32 ? 2 : 4;
-    using A = Side<DT, BM, TURN_A, WAVES>;
-    using B = Side<DT, BN, TURN_B, WAVES>;
+    static constexpr int WAVES = WM * WN, TM = BM / WM / M::SIDE, TN = BN / WN / M::SIDE, PARTS = LINE / (DT == TDB_F32 ? 64 : 32);
+    using A = Side<DT, BM, TURN_A, WAVES, LINE>;
+    using B = Side<DT, BN, TURN_B, WAVES, LINE>;
     static constexpr int STEP = A::STEP, STAGE = A::BYTES + B::BYTES, SHARED = NS * STAGE;
     using Acc = typename M::Acc[TM][TN];
 
     static __device__ __forceinline__ int wave_m() { return int(uniform(threadIdx.x >> 6)) / WN * (BM / WM); }
     static __device__ __forceinline__ int wave_n() { return int(uniform(threadIdx.x >> 6)) % WN * (BN / WN); }
 
-    // Steps [begin, end) of the tile at rows m0 of A and n0 of B.
-    static __device__ __forceinline__ void run(char* smem, const Rows& a, const Rows& b, int64_t m0, int64_t n0, int64_t begin, int64_t end, Acc& acc) {
+    // Steps [begin, end) of the tile at rows m0 of A and n0 of B.  The sums start from start(j, q), four neighbours along n, called behind the first step's barrier.
+    template <class START>
+    static __device__ __forceinline__ void run(char* smem, const Rows& a, const Rows& b, int64_t m0, int64_t n0, int64_t begin, int64_t end, Acc& acc, START start) {
         constexpr int LOADS = A::LOADS + B::LOADS;
         A side_a;
         B side_b;
         side_a.place(a, m0), side_b.place(b, n0);
         const uint32_t lds = uniform(uint32_t(reinterpret_cast<uintptr_t>(TDB_SHARED(char, smem))));
-#pragma unroll
-        for (int i = 0; i < TM; ++i)
-#pragma unroll
-            for (int j = 0; j < TN; ++j) acc[i][j] = typename M::Acc{};
         auto load = [&](int64_t s, int stage) {
             side_a.load(a, m0, s, lds + stage * STAGE);
             side_b.load(b, n0, s, lds + stage * STAGE + A::BYTES);
@@ -202,6 +201,16 @@ struct Product {
 #pragma unroll
         for (int s = 0; s < NS - 1; ++s)
             if (s < steps) load(begin + s, s);
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int q = 0; q < M::QUADS; ++q) {
+                const f32x4 v = start(j, q);
+#pragma unroll
+                for (int i = 0; i < TM; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] = v[e];
+            }
         int stage = 0, ahead = NS - 1;
         for (int s = 0; s < steps; ++s) {
             if (s + NS - 2 < steps) wait_loads<(NS - 2) * LOADS>();
@@ -226,16 +235,24 @@ struct Product {
         }
         step_barrier();                     // LDS is free for what follows
     }
-    // The tile's values, value(i, j, q) -> four neighbours, to rows of memory by way of LDS: whole 16-byte chunks where `wide`.
-    template <class OF>
-    static __device__ __forceinline__ void store(char* smem, char* to, int64_t pitch, int64_t m0, int64_t m_end, int64_t n0, int64_t n_end, bool wide, OF value) {
-        constexpr int ES = sizeof(T), COLS = TN * M::SIDE, PITCH = COLS * ES + 16, PER = COLS * ES / 16;
+    static __device__ __forceinline__ void run(char* smem, const Rows& a, const Rows& b, int64_t m0, int64_t n0, int64_t begin, int64_t end, Acc& acc) {
+        run(smem, a, b, m0, n0, begin, end, acc, [](int, int) { return f32x4{0.f, 0.f, 0.f, 0.f}; });
+    }
+
+    // The tile's values to rows of memory by way of LDS, SIDE rows at a time: value(i, j, q) gives four neighbours, then(i, the wave's rows in LDS) may change what lies there.
+    // to: value (m0, n0); rows and columns: how many of the tile's there are.  Whole 16-byte chunks where `wide`.
+    static constexpr int COLUMNS = TN * M::SIDE, PITCH = COLUMNS * int(sizeof(T)) + 16;
+    template <class OF, class THEN>
+    static __device__ __forceinline__ void store(char* smem, char* to, int64_t pitch, int64_t rows, int64_t columns, bool wide, OF value, THEN then) {
+        constexpr int ES = sizeof(T), PER = COLUMNS * ES / 16;
         typedef __attribute__((ext_vector_type(4))) T T4;
         const int l = threadIdx.x & 63;
-        char* const mine = smem + uniform(threadIdx.x >> 6) * (M::SIDE * PITCH);
-        static_assert(WAVES * M::SIDE * PITCH <= SHARED, "");
+        char* const own = smem + uniform(threadIdx.x >> 6) * (2 * M::SIDE * PITCH);
+        static_assert(WAVES * 2 * M::SIDE * PITCH <= SHARED, "");
+        to += wave_m() * pitch + wave_n() * ES, rows -= wave_m(), columns -= wave_n();
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
+            char* const mine = own + (i & 1) * (M::SIDE * PITCH);
 #pragma unroll
             for (int j = 0; j < TN; ++j)
 #pragma unroll
@@ -243,24 +260,23 @@ struct Product {
                     const f32x4 v = value(i, j, q);
                     *reinterpret_cast<T4*>(mine + lane_m<DT>() * PITCH + (j * M::SIDE + quad_n<DT>(q)) * ES) = T4{T(v[0]), T(v[1]), T(v[2]), T(v[3])};
                 }
+            then(i, mine);
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
-            const int64_t m = m0 + wave_m() + i * M::SIDE, n = n0 + wave_n();
             if (wide) {
+                const auto buffer = __builtin_amdgcn_make_buffer_rsrc(to + i * M::SIDE * pitch, 0, int(rows > i * M::SIDE && columns > 0 ? min((rows - 1 - i * M::SIDE) * pitch + columns * ES, int64_t(0x7fffffff)) : 0), 0x00020000);
 #pragma unroll
                 for (int r = 0; r < M::SIDE * PER / 64; ++r) {
                     const int at = r * 64 + l, row = at / PER, c = at % PER;
-                    const uint4 v = *reinterpret_cast<const uint4*>(mine + row * PITCH + c * 16);
-                    if (m + row < m_end && n + c * (16 / ES) < n_end) *reinterpret_cast<uint4*>(to + (m + row) * pitch + (n * ES + c * 16)) = v;
+                    const u32x4 v = *reinterpret_cast<const u32x4*>(mine + row * PITCH + c * 16);
+                    __builtin_amdgcn_raw_buffer_store_b128(v, buffer, c * 16 < columns * ES ? uint32_t(row) * uint32_t(pitch) + c * 16 : PAST, 0, 0);
                 }
             } else {
-                for (int at = l; at < M::SIDE * COLS; at += 64) {
-                    const int row = at / COLS, c = at % COLS;
-                    if (m + row < m_end && n + c < n_end) *reinterpret_cast<T*>(to + (m + row) * pitch + (n + c) * ES) = *reinterpret_cast<const T*>(mine + row * PITCH + c * ES);
+                for (int at = l; at < M::SIDE * COLUMNS; at += 64) {
+                    const int row = at / COLUMNS, c = at % COLUMNS;
+                    if (i * M::SIDE + row < rows && c < columns) *reinterpret_cast<T*>(to + (i * M::SIDE + row) * pitch + c * ES) = *reinterpret_cast<const T*>(mine + row * PITCH + c * ES);
                 }
             }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
         }
     }
     // Four neighbours of the sums.
@@ -281,8 +297,8 @@ __device__ __forceinline__ float over_m(float (&x)[N]) {
         const bool high = threadIdx.x & w;
 #pragma unroll
         for (int k = 0; k < w; ++k) {
-            const float other = __shfl_xor(high ? x[k] : x[k + w], w);
-            x[k] = (high ? x[k + w] : x[k]) + other;
+            const float a = x[k], b = x[k + w], pass = high ? a : b, keep = high ? b : a;     // (not high ? x[k] : x[k + w], which chooses an address)
+            x[k] = keep + __shfl_xor(pass, w);
         }
     }
     float sum = x[0];
