@@ -47,6 +47,7 @@ struct Loss {
     float* loss;
     // state: count[0] rows that count, count[1] workgroups that are done
     int32_t *count, *index, *place, *label;     // of the gathered rows: row, label; of the rows: their place among the gathered ones
+    float* biases;                              // of all classes, -inf behind them up to a multiple of TILE
     float *top, *inverse, *right;               // largest logit, 1 / sum of exponentials relative to it, the label's logit
     char* gathered;
     int64_t pitch;                              // of a gathered row, bytes
@@ -91,11 +92,16 @@ __device__ __forceinline__ int block_count(int x, int* scratch) {
 constexpr int GATHER_WAVES = 8, GATHER_ROWS = 4;       // rows that a wave copies at once
 
 // Rows that count, in order: where they come from, their labels, and they themselves, dense, zeros behind them up to a multiple of the steps' 128 bytes.
-// A workgroup has `chunk` rows and counts for itself what lies in front of them.
+// A workgroup has `chunk` rows and counts for itself what lies in front of them.  Workgroups from row_blocks on write the biases as the other kernels take them.
 template <int DT>
-__global__ __launch_bounds__(64 * GATHER_WAVES) void loss_gather_kernel(Loss p, int64_t chunk, bool wide) {
+__global__ __launch_bounds__(64 * GATHER_WAVES) void loss_gather_kernel(Loss p, int64_t chunk, int row_blocks, bool wide) {
     using T = typename Matrix<DT>::T;
     constexpr int THREADS = 64 * GATHER_WAVES, U = 8;
+    if (int(blockIdx.x) >= row_blocks) {
+        const int64_t v = (int64_t(blockIdx.x) - row_blocks) * (4 * THREADS) + 4 * threadIdx.x;
+        if (v < (p.vocab + TILE - 1) / TILE * TILE) *reinterpret_cast<f32x4*>(p.biases + v) = f32x4{bias_of<DT>(p, v), bias_of<DT>(p, v + 1), bias_of<DT>(p, v + 2), bias_of<DT>(p, v + 3)};
+        return;
+    }
     __shared__ int scratch[GATHER_WAVES];
     const int wave = threadIdx.x >> 6, l = threadIdx.x & 63;
     const int64_t first = blockIdx.x * chunk, end = min(p.rows, first + chunk);
@@ -133,7 +139,7 @@ __global__ __launch_bounds__(64 * GATHER_WAVES) void loss_gather_kernel(Loss p, 
         }
     }
     if (blockIdx.x == 0 && threadIdx.x == 0) p.count[1] = 0;
-    if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) p.count[0] = at;
+    if (int(blockIdx.x) == row_blocks - 1 && threadIdx.x == 0) p.count[0] = at;
     __syncthreads();
     const int columns = int(p.pitch / sizeof(T));
     for (int r0 = before + wave * GATHER_ROWS; r0 < at; r0 += GATHER_WAVES * GATHER_ROWS) {
@@ -171,59 +177,55 @@ __device__ __forceinline__ Rows weight_rows(const Loss& p) { return {p.w, p.w_pi
 
 // A tile's logits: the sums start from the biases.
 template <int DT, class P>
-__device__ __forceinline__ void logits_of(const Loss& p, int n, char* smem, float* s_bias, int64_t m0, int64_t n0, typename P::Acc& acc) {
+__device__ __forceinline__ void logits_of(const Loss& p, typename P::Flow& flow, float* s_bias, int64_t m0, int64_t n0, typename P::Acc& acc) {
     __syncthreads();                        // (the biases of the tile before have been read)
-    if (threadIdx.x < P::BN) s_bias[threadIdx.x] = bias_of<DT>(p, n0 + threadIdx.x);
+    if (threadIdx.x < P::BN) s_bias[threadIdx.x] = p.biases[n0 + threadIdx.x];
     __syncthreads();
-    P::run(smem, hidden_rows<DT>(p, n), weight_rows<DT>(p), m0, n0, 0, p.pitch / P::LINE_BYTES, acc,
+    P::run(flow, {m0, n0, 0, p.pitch / P::LINE_BYTES}, acc,
            [&](int j, int q) { return *reinterpret_cast<const f32x4*>(s_bias + P::wave_n() + j * Matrix<DT>::SIDE + quad_n<DT>(q)); });
 }
 
 // Forward: of each gathered row and group of column tiles the largest logit and the sum of exponentials relative to it.
 template <int DT, class P>
-__device__ __forceinline__ void logits_body(const Loss& p, int n, char* smem, float* s_bias, float* s_top, float* s_sum) {
+struct Running {
     using M = Matrix<DT>;
-    const Partials parts(p, P::BM == 256);
-    const int64_t row_tiles = (n + P::BM - 1) / P::BM, all = row_tiles * parts.groups;
-    for (int64_t block = blockIdx.x; block < all; block += gridDim.x) {
-        int64_t row, g, split;
-        tile_of(block, row_tiles, parts.groups, 1, row, g, split);
-        const int64_t m0 = row * P::BM;
-        float top[P::TM], sum[P::TM];
+    float top[P::TM], sum[P::TM];
+    __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int i = 0; i < P::TM; ++i) top[i] = -FLT_MAX, sum[i] = 0.f;
-        for (int64_t t = g * parts.group; t < min(parts.tiles, (g + 1) * parts.group); ++t) {
-            const int64_t n0 = t * P::BN;
-            typename P::Acc acc;
-            logits_of<DT, P>(p, n, smem, s_bias, m0, n0, acc);
+    }
+    // labels: of the tile's rows
+    __device__ __forceinline__ void add(const Loss& p, int n, const typename P::Acc& acc, int64_t m0, int64_t n0, const int32_t* labels) {
 #pragma unroll
-            for (int i = 0; i < P::TM; ++i) {
-                float most = top[i];
+        for (int i = 0; i < P::TM; ++i) {
+            float most = top[i];
+#pragma unroll
+            for (int j = 0; j < P::TN; ++j)
+#pragma unroll
+                for (int e = 0; e < 4 * M::QUADS; ++e) most = fmaxf(most, acc[i][j][e]);
+            float more[2] = {0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < P::TN; ++j)
+#pragma unroll
+                for (int e = 0; e < 4 * M::QUADS; ++e) more[e & 1] += __builtin_amdgcn_exp2f((acc[i][j][e] - most) * LOG2E);
+            sum[i] = sum[i] * __builtin_amdgcn_exp2f((top[i] - most) * LOG2E) + (more[0] + more[1]);
+            top[i] = most;
+            // The label's own logit, in the one tile that has it: row after row, the value's place is the same for all lanes.
+            const int at = P::wave_m() + i * M::SIDE + lane_m<DT>();
+            const int rel = m0 + at < n ? labels[at] - int(n0) - P::wave_n() : -1;
+            const bool here = rel >= 0 && rel < P::COLUMNS && n0 + P::wave_n() + rel < p.vocab;
+            for (uint64_t who = __builtin_amdgcn_ballot_w64(here) & (~uint64_t(0) >> (64 - M::SIDE)); who; who &= who - 1) {
+                const int lane = __builtin_ctzll(who), c = __builtin_amdgcn_readlane(rel, lane);
 #pragma unroll
                 for (int j = 0; j < P::TN; ++j)
 #pragma unroll
-                    for (int e = 0; e < 4 * M::QUADS; ++e) most = fmaxf(most, acc[i][j][e]);
-                float more[2] = {0.f, 0.f};
-#pragma unroll
-                for (int j = 0; j < P::TN; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4 * M::QUADS; ++e) more[e & 1] += __builtin_amdgcn_exp2f((acc[i][j][e] - most) * LOG2E);
-                sum[i] = sum[i] * __builtin_amdgcn_exp2f((top[i] - most) * LOG2E) + (more[0] + more[1]);
-                top[i] = most;
-                // The label's own logit, in the one tile that has it: row after row, the value's place is the same for all lanes.
-                const int64_t m = m0 + P::wave_m() + i * M::SIDE + lane_m<DT>();
-                const int64_t label = m < n ? p.label[m] : -1, rel = label - n0 - P::wave_n();
-                const bool here = label >= 0 && rel >= 0 && rel < P::COLUMNS;
-                for (uint64_t who = __builtin_amdgcn_ballot_w64(here) & (~uint64_t(0) >> (64 - M::SIDE)); who; who &= who - 1) {
-                    const int lane = __builtin_ctzll(who), c = __builtin_amdgcn_readlane(int(rel), lane);
-#pragma unroll
-                    for (int j = 0; j < P::TN; ++j)
-#pragma unroll
-                        for (int e = 0; e < 4 * M::QUADS; ++e)
-                            if ((threadIdx.x & (M::SIDE - 1)) == lane && c == j * M::SIDE + quad_n<DT>(e / 4) + e % 4) p.right[m] = acc[i][j][e];
-                }
+                    for (int e = 0; e < 4 * M::QUADS; ++e)
+                        if ((threadIdx.x & (M::SIDE - 1)) == lane && c == j * M::SIDE + quad_n<DT>(e / 4) + e % 4) p.right[m0 + at] = acc[i][j][e];
             }
         }
+    }
+    // All waves' together, to memory.  s_top, s_sum: WN * BM each.
+    __device__ __forceinline__ void finish(float* s_top, float* s_sum, float* maxima, float* sums) {
 #pragma unroll
         for (int i = 0; i < P::TM; ++i) {
             const float most = over_quads<DT>(top[i], [](float x, float y) { return fmaxf(x, y); });
@@ -231,21 +233,60 @@ __device__ __forceinline__ void logits_body(const Loss& p, int n, char* smem, fl
             const int at = P::wave_n() / P::COLUMNS * P::BM + P::wave_m() + i * M::SIDE + lane_m<DT>();
             s_top[at] = most, s_sum[at] = s;
         }
-        __syncthreads();
+        step_barrier();
         if (threadIdx.x < P::BM) {
             float most = s_top[threadIdx.x], s = 0.f;
 #pragma unroll
             for (int w = 1; w < P::WN; ++w) most = fmaxf(most, s_top[w * P::BM + threadIdx.x]);
 #pragma unroll
             for (int w = 0; w < P::WN; ++w) s += s_sum[w * P::BM + threadIdx.x] * __builtin_amdgcn_exp2f((s_top[w * P::BM + threadIdx.x] - most) * LOG2E);
-            p.maxima[g * parts.pitch + m0 + threadIdx.x] = most;
-            p.sums[g * parts.pitch + m0 + threadIdx.x] = s;
+            maxima[threadIdx.x] = most, sums[threadIdx.x] = s;
         }
+    }
+};
+
+template <int DT, class P>
+__device__ __forceinline__ void logits_body(const Loss& p, int n, char* smem, float* s_bias, int32_t* s_label, float* s_top, float* s_sum) {
+    const Partials parts(p, false);
+    typename P::Flow flow(smem, hidden_rows<DT>(p, n), weight_rows<DT>(p));
+    const int64_t row_tiles = (n + P::BM - 1) / P::BM, all = row_tiles * parts.groups;
+    for (int64_t block = blockIdx.x; block < all; block += gridDim.x) {
+        int64_t row, g, split;
+        tile_of(block, row_tiles, parts.groups, 1, row, g, split);
+        const int64_t m0 = row * P::BM, n0 = g * P::BN;
+        typename P::Acc acc;
+        if (threadIdx.x < P::BM) s_label[threadIdx.x] = m0 + threadIdx.x < n ? p.label[m0 + threadIdx.x] : -1;
+        logits_of<DT, P>(p, flow, s_bias, m0, n0, acc);
+        Running<DT, P> running;
+        running.clear();
+        running.add(p, n, acc, m0, n0, s_label);
+        running.finish(s_top, s_sum, p.maxima + g * parts.pitch + m0, p.sums + g * parts.pitch + m0);
     }
 }
 
+// What a tile needs beside its operands, 1 KB of each of several arrays: of float32 or labels, of the tile's columns (number 0) or rows (the others).  A wave brings one of them.
+template <class P, int ARRAYS>
+struct TileArrays {
+    static constexpr int BYTES = 2 * ARRAYS * 1024;
+    const char* from = nullptr;     // the wave's own
+    int64_t bytes = 0;
+    bool columns = false;
+    char* smem;
+    int set = 1;                    // of the two in LDS that holds the present tile's; the other one is filled
+    static __device__ __forceinline__ int own() { return int(uniform(threadIdx.x >> 6)) % ARRAYS; }
+    __device__ __forceinline__ void array(int k, const void* p, int64_t values) {
+        if (own() == k) from = static_cast<const char*>(p), bytes = 4 * values, columns = k == 0;
+    }
+    __device__ __forceinline__ void load(const typename P::Tile& t) {
+        const int64_t at = 4 * (columns ? t.n0 : t.m0);
+        const uint32_t lds = uniform(uint32_t(reinterpret_cast<uintptr_t>(TDB_SHARED(char, smem))));
+        load_shared(lds + ((set ^ 1) * ARRAYS + own()) * 1024, buffer_of(from + at, bytes - at), (threadIdx.x & 63) * 16);
+    }
+    __device__ __forceinline__ const char* of(int k) const { return smem + (set * ARRAYS + k) * 1024; }
+};
+
 // Many rows: a workgroup of eight waves to a CU.  Few: two of four waves, tiles of as many rows as there are.  (Two kernels, of which one ends at once: with all heights in one the compiler kept
-// some 100 scalar and a few vector registers in memory, and 8192 rows took 2520 us instead of LOGITS_MANY.)
+// some 100 scalar and a few vector registers in memory, and 8192 rows took 2520 us instead of LOGITS_MANY.)  The next tile's first step is on its way while a tile's exponentials are made.
 template <int DT>
 using Logits256 = Product<DT, 256, 256, 2, 4, 2, false, false>;
 template <int DT>
@@ -254,27 +295,65 @@ template <int DT>
 using Logits64 = Product<DT, 64, 128, 1, 4, 6, false, false, 64>;
 template <int DT>
 using Logits32 = Product<DT, 32, 128, 1, 4, 3, false, false, 128>;
-constexpr int MANY_SHARED = Logits256<TDB_BF16>::SHARED, FEW_SHARED = Logits64<TDB_BF16>::SHARED;
+constexpr int MANY_SHARED = Logits256<TDB_BF16>::SHARED,  FEW_SHARED = Logits64<TDB_BF16>::SHARED;
 static_assert(Logits128<TDB_BF16>::SHARED <= FEW_SHARED && Logits32<TDB_BF16>::SHARED <= FEW_SHARED, "");
 
 template <int DT>
 __global__ __launch_bounds__(512, 2) void loss_logits_many_kernel(Loss p) {
     extern __shared__ __attribute__((aligned(1024))) char smem[];
-    __shared__ __attribute__((aligned(16))) float s_bias[256];
     __shared__ float s_top[1024], s_sum[1024];
+    using P = Logits256<DT>;
     const int n = p.count[0];
-    if (tile_rows(n, 32) == 256) logits_body<DT, Logits256<DT>>(p, n, smem, s_bias, s_top, s_sum);
+    if (tile_rows(n, 32) != 256) return;
+    const Partials parts(p, true);
+    const int64_t row_tiles = (n + P::BM - 1) / P::BM, all = row_tiles * parts.groups;
+    typename P::Flow flow(smem, hidden_rows<DT>(p, n), weight_rows<DT>(p));
+    TileArrays<P, 2> arrays;
+    arrays.smem = smem + P::SHARED;
+    arrays.array(0, p.biases, (p.vocab + TILE - 1) / TILE * TILE), arrays.array(1, p.label, n);
+    // The tile after the t-th of a group: of the same group, or the first of the workgroup's next one.
+    int64_t row, g, split;
+    auto tile = [&](int64_t r, int64_t t) { return typename P::Tile{r * P::BM, t * P::BN, 0, p.pitch / P::LINE_BYTES}; };
+    int64_t block = blockIdx.x;
+    if (block >= all) return;
+    tile_of(block, row_tiles, parts.groups, 1, row, g, split);
+    int64_t t = g * parts.group;
+    typename P::Tile now = tile(row, t);
+    P::open(flow, now, arrays);
+    int stage = 0;
+    Running<DT, P> running;
+    running.clear();
+    while (true) {
+        const bool last = t + 1 == min(parts.tiles, (g + 1) * parts.group);
+        int64_t next_row = row, next_g = g;
+        if (last && block + gridDim.x < all) tile_of(block + gridDim.x, row_tiles, parts.groups, 1, next_row, next_g, split);
+        const int64_t next_t = last ? next_g * parts.group : t + 1;
+        const typename P::Tile next = tile(next_row, next_t);
+        const bool more = !last || block + gridDim.x < all;
+        arrays.set ^= 1;
+        typename P::Acc acc;
+        P::template run_on<0>(flow, now, next, more, stage, true, acc, [&](int j, int q) { return *reinterpret_cast<const f32x4*>(arrays.of(0) + 4 * (P::wave_n() + j * Matrix<DT>::SIDE + quad_n<DT>(q))); }, arrays);
+        running.add(p, n, acc, now.m0, now.n0, reinterpret_cast<const int32_t*>(arrays.of(1)));
+        if (last) {
+            running.finish(s_top, s_sum, p.maxima + g * parts.pitch + now.m0, p.sums + g * parts.pitch + now.m0);
+            running.clear();
+            block += gridDim.x;
+        }
+        if (!more) break;
+        row = next_row, g = next_g, t = next_t, now = next;
+    }
 }
 template <int DT>
 __global__ __launch_bounds__(256, 2) void loss_logits_few_kernel(Loss p) {
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     __shared__ __attribute__((aligned(16))) float s_bias[128];
+    __shared__ int32_t s_label[128];
     __shared__ float s_top[256], s_sum[256];
     const int n = p.count[0];
     switch (tile_rows(n, 32)) {
-        case 32: return logits_body<DT, Logits32<DT>>(p, n, smem, s_bias, s_top, s_sum);
-        case 64: return logits_body<DT, Logits64<DT>>(p, n, smem, s_bias, s_top, s_sum);
-        case 128: return logits_body<DT, Logits128<DT>>(p, n, smem, s_bias, s_top, s_sum);
+        case 32: return logits_body<DT, Logits32<DT>>(p, n, smem, s_bias, s_label, s_top, s_sum);
+        case 64: return logits_body<DT, Logits64<DT>>(p, n, smem, s_bias, s_label, s_top, s_sum);
+        case 128: return logits_body<DT, Logits128<DT>>(p, n, smem, s_bias, s_label, s_top, s_sum);
     }
 }
 
@@ -367,90 +446,142 @@ struct Gradient {
     bool wide_dweight, later;   // later: a piece that is not the first
 };
 
-// D of a piece of the vocabulary, and its sums over the rows of a tile.
+// What the gradient of a tile needs of its rows, in LDS.
+struct RowArrays {
+    const float *top, *scale, *right, *share, *shift;
+    const int32_t* label;
+};
+
+// D of a tile, to memory, and its sums over the tile's rows.  s_column: WM * BN.
 template <int DT, class P, bool WEIGHTED>
-__device__ __forceinline__ void difference_body(const Loss& p, const Gradient& g, int n, char* smem, float* s_bias, float* s_column) {
+__device__ __forceinline__ void difference_of(const Loss& p, const Gradient& g, int n, const typename P::Acc& acc, int64_t row, int64_t n0, const RowArrays& of, char* scratch, float* s_column) {
     using M = Matrix<DT>;
     using T = typename M::T;
     constexpr int N = P::TN * M::QUADS * 4;     // values of a lane in a row
+    const int64_t m0 = row * P::BM;
+    const int first = P::wave_m() + lane_m<DT>();
+    // (rows that are not there: zeros)
+    auto relative = [&](int i) { return m0 + first + i * M::SIDE < n ? of.label[first + i * M::SIDE] - int(n0) - P::wave_n() : -1; };
+    auto share_of = [&](int i) { return WEIGHTED ? of.share[first + i * M::SIDE] : D_SCALE<DT>; };
+    auto shift_of = [&](int i) { return WEIGHTED && DT == TDB_F16 ? of.shift[first + i * M::SIDE] : 1.f; };
+    float sums[N];
+#pragma unroll
+    for (int c = 0; c < N; ++c) sums[c] = 0.f;
+    float top = 0.f, scale = 0.f, shift = 1.f;
+    P::store(
+        scratch, g.d + m0 * g.d_pitch + (n0 - g.first) * int64_t(sizeof(T)), g.d_pitch, P::BM, P::BN, true,
+        [&](int i, int j, int q) {
+            if (j == 0 && q == 0) {
+                const bool there = m0 + first + i * M::SIDE < n;
+                top = there ? of.top[first + i * M::SIDE] : INFINITY, scale = there ? of.scale[first + i * M::SIDE] : 0.f, shift = there ? shift_of(i) : 0.f;
+            }
+            const f32x4 v = P::quad(acc, i, j, q);
+            f32x4 d;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                d[e] = __builtin_amdgcn_exp2f((v[e] - top) * LOG2E) * scale;
+                sums[(j * M::QUADS + q) * 4 + e] += WEIGHTED && DT == TDB_F16 ? d[e] * shift : d[e];
+            }
+            return d;
+        },
+        [&](int i, char* rows) {    // the label's own value
+            const int rel = relative(i);
+            if (rel >= 0 && rel < P::COLUMNS && (threadIdx.x & 63) < M::SIDE) {
+                const float right = of.right[first + i * M::SIDE];
+                *reinterpret_cast<T*>(rows + P::lies_at(lane_m<DT>(), rel * int(sizeof(T)))) = T(__builtin_amdgcn_exp2f((right - top) * LOG2E) * scale - share_of(i));
+            }
+        });
+    if (!g.dbias) return;
+    float sum = over_m<DT>(sums);
+    const int c = lane_m<DT>() % N, mine = c / (4 * M::QUADS) * M::SIDE + quad_n<DT>(c / 4 % M::QUADS) + c % 4;     // the lane's column
+#pragma unroll
+    for (int i = 0; i < P::TM; ++i) {
+        const int rel = relative(i);
+        for (uint64_t who = __builtin_amdgcn_ballot_w64(rel >= 0 && rel < P::COLUMNS) & (~uint64_t(0) >> (64 - M::SIDE)); who; who &= who - 1) {
+            const int lane = __builtin_ctzll(who);
+            const float less = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, share_of(i) * shift_of(i)), lane));
+            sum -= __builtin_amdgcn_readlane(rel, lane) == mine ? less : 0.f;
+        }
+    }
+    if (lane_m<DT>() < N) s_column[P::wave_m() / (P::TM * M::SIDE) * P::BN + P::wave_n() + mine] = sum;
+    step_barrier();
+    if (threadIdx.x < P::BN) {
+        float all = 0.f;
+#pragma unroll
+        for (int w = 0; w < P::WM; ++w) all += s_column[w * P::BN + threadIdx.x];
+        g.column_sums[row * g.columns + n0 - g.first + threadIdx.x] = all;
+    }
+}
+
+// D of a piece of the vocabulary.
+template <int DT, class P, bool WEIGHTED>
+__device__ __forceinline__ void difference_body(const Loss& p, const Gradient& g, int n, char* smem, float* s_bias, float (&s_rows)[6][128], float* s_column) {
+    typename P::Flow flow(smem, hidden_rows<DT>(p, n), weight_rows<DT>(p));
     const int64_t row_tiles = (n + P::BM - 1) / P::BM, column_tiles = g.columns / P::BN, all = row_tiles * column_tiles;
     for (int64_t block = blockIdx.x; block < all; block += gridDim.x) {
         int64_t row, column, split;
         tile_of(block, row_tiles, column_tiles, 1, row, column, split);
         const int64_t m0 = row * P::BM, n0 = g.first + column * P::BN;
         typename P::Acc acc;
-        logits_of<DT, P>(p, n, smem, s_bias, m0, n0, acc);
-        float top[P::TM], scale[P::TM], share[P::TM], shift[P::TM];
-        int rel[P::TM];
-#pragma unroll
-        for (int i = 0; i < P::TM; ++i) {
-            const int64_t m = m0 + P::wave_m() + i * M::SIDE + lane_m<DT>(), at = min(m, int64_t(n - 1));
-            top[i] = m < n ? p.top[at] : INFINITY;      // (rows that are not there: zeros)
-            scale[i] = WEIGHTED ? g.scale[at] : p.inverse[at];
-            share[i] = WEIGHTED ? g.share[at] : D_SCALE<DT>, shift[i] = WEIGHTED && DT == TDB_F16 ? g.shift[at] : 1.f;
-            const int label = p.label[at];
-            rel[i] = m < n && label >= 0 ? label - int(n0) - P::wave_n() : -1;
-        }
-        float sums[N];
-#pragma unroll
-        for (int c = 0; c < N; ++c) sums[c] = 0.f;
-        P::store(
-            smem, g.d + m0 * g.d_pitch + (n0 - g.first) * int64_t(sizeof(T)), g.d_pitch, P::BM, P::BN, true,
-            [&](int i, int j, int q) {
-                const f32x4 v = P::quad(acc, i, j, q);
-                f32x4 d;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    d[e] = __builtin_amdgcn_exp2f((v[e] - top[i]) * LOG2E) * scale[i];
-                    sums[(j * M::QUADS + q) * 4 + e] += d[e] * shift[i];
-                }
-                return d;
-            },
-            [&](int i, char* rows) {    // the label's own value
-                if (rel[i] >= 0 && rel[i] < P::COLUMNS && (threadIdx.x & 63) < M::SIDE) {
-                    const float right = p.right[m0 + P::wave_m() + i * M::SIDE + lane_m<DT>()];
-                    *reinterpret_cast<T*>(rows + lane_m<DT>() * P::PITCH + rel[i] * int(sizeof(T))) = T(__builtin_amdgcn_exp2f((right - top[i]) * LOG2E) * scale[i] - share[i]);
-                }
-            });
-        if (!g.dbias) continue;
-        float sum = over_m<DT>(sums);
-        const int c = lane_m<DT>() % N, mine = c / (4 * M::QUADS) * M::SIDE + quad_n<DT>(c / 4 % M::QUADS) + c % 4;     // the lane's column
-#pragma unroll
-        for (int i = 0; i < P::TM; ++i)
-            for (uint64_t who = __builtin_amdgcn_ballot_w64(rel[i] >= 0 && rel[i] < P::COLUMNS) & (~uint64_t(0) >> (64 - M::SIDE)); who; who &= who - 1) {
-                const int lane = __builtin_ctzll(who);
-                const float less = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, share[i] * shift[i]), lane));
-                sum -= __builtin_amdgcn_readlane(rel[i], lane) == mine ? less : 0.f;
-            }
-        if (lane_m<DT>() < N) s_column[P::wave_m() / (P::TM * M::SIDE) * P::BN + P::wave_n() + mine] = sum;
         __syncthreads();
-        if (threadIdx.x < P::BN) {
-            float all = 0.f;
-#pragma unroll
-            for (int w = 0; w < P::WM; ++w) all += s_column[w * P::BN + threadIdx.x];
-            g.column_sums[row * g.columns + n0 - g.first + threadIdx.x] = all;
+        if (const int64_t m = m0 + threadIdx.x; threadIdx.x < P::BM && m < n) {
+            s_rows[0][threadIdx.x] = p.top[m], s_rows[1][threadIdx.x] = WEIGHTED ? g.scale[m] : p.inverse[m], s_rows[2][threadIdx.x] = p.right[m];
+            s_rows[3][threadIdx.x] = __builtin_bit_cast(float, p.label[m]);
+            if (WEIGHTED) s_rows[4][threadIdx.x] = g.share[m], s_rows[5][threadIdx.x] = g.shift[m];
         }
+        logits_of<DT, P>(p, flow, s_bias, m0, n0, acc);
+        const RowArrays rows{s_rows[0], s_rows[1], s_rows[2], s_rows[4], s_rows[5], reinterpret_cast<const int32_t*>(s_rows[3])};
+        difference_of<DT, P, WEIGHTED>(p, g, n, acc, row, n0, rows, smem, s_column);
     }
 }
 
 template <int DT, bool WEIGHTED>
 __global__ __launch_bounds__(512, 2) void loss_difference_many_kernel(Loss p, Gradient g) {
     extern __shared__ __attribute__((aligned(1024))) char smem[];
-    __shared__ __attribute__((aligned(16))) float s_bias[256];
     __shared__ float s_column[512];
+    using P = Logits256<DT>;
     const int n = p.count[0];
-    if (tile_rows(n, 32) == 256) difference_body<DT, Logits256<DT>, WEIGHTED>(p, g, n, smem, s_bias, s_column);
+    if (tile_rows(n, 32) != 256) return;
+    const int64_t row_tiles = (n + P::BM - 1) / P::BM, column_tiles = g.columns / P::BN, all = row_tiles * column_tiles;
+    typename P::Flow flow(smem, hidden_rows<DT>(p, n), weight_rows<DT>(p));
+    constexpr int ARRAYS = WEIGHTED ? 7 : 5;
+    TileArrays<P, ARRAYS> arrays;
+    arrays.smem = smem + P::SHARED;
+    arrays.array(0, p.biases, (p.vocab + TILE - 1) / TILE * TILE), arrays.array(1, p.top, n), arrays.array(2, WEIGHTED ? g.scale : p.inverse, n), arrays.array(3, p.right, n);
+    arrays.array(4, p.label, n);
+    if constexpr (WEIGHTED) arrays.array(5, g.share, n), arrays.array(6, g.shift, n);
+    auto tile = [&](int64_t block, int64_t& row) {
+        int64_t column, split;
+        tile_of(block < all ? block : 0, row_tiles, column_tiles, 1, row, column, split);
+        return typename P::Tile{row * P::BM, g.first + column * P::BN, 0, p.pitch / P::LINE_BYTES};
+    };
+    if (blockIdx.x >= all) return;
+    int64_t row, next_row;
+    typename P::Tile now = tile(blockIdx.x, row);
+    P::open(flow, now, arrays);
+    int stage = 0;
+    for (int64_t block = blockIdx.x; block < all; block += gridDim.x) {
+        const typename P::Tile next = tile(block + gridDim.x, next_row);
+        arrays.set ^= 1;
+        typename P::Acc acc;
+        auto start = [&](int j, int q) { return *reinterpret_cast<const f32x4*>(arrays.of(0) + 4 * (P::wave_n() + j * Matrix<DT>::SIDE + quad_n<DT>(q))); };
+        P::template run_on<P::STORES>(flow, now, next, block + gridDim.x < all, stage, block == blockIdx.x, acc, start, arrays);
+        auto floats = [&](int k) { return reinterpret_cast<const float*>(arrays.of(k)); };
+        const RowArrays rows{floats(1), floats(2), floats(3), floats(ARRAYS - 2), floats(ARRAYS - 1), reinterpret_cast<const int32_t*>(arrays.of(4))};
+        difference_of<DT, P, WEIGHTED>(p, g, n, acc, row, now.n0, rows, P::scratch(smem, stage), s_column);
+        row = next_row, now = next;
+    }
 }
 template <int DT, bool WEIGHTED>
 __global__ __launch_bounds__(256, 2) void loss_difference_few_kernel(Loss p, Gradient g) {
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     __shared__ __attribute__((aligned(16))) float s_bias[128];
-    __shared__ float s_column[256];
+    __shared__ float s_column[256], s_rows[6][128];
     const int n = p.count[0];
     switch (tile_rows(n, 32)) {
-        case 32: return difference_body<DT, Logits32<DT>, WEIGHTED>(p, g, n, smem, s_bias, s_column);
-        case 64: return difference_body<DT, Logits64<DT>, WEIGHTED>(p, g, n, smem, s_bias, s_column);
-        case 128: return difference_body<DT, Logits128<DT>, WEIGHTED>(p, g, n, smem, s_bias, s_column);
+        case 32: return difference_body<DT, Logits32<DT>, WEIGHTED>(p, g, n, smem, s_bias, s_rows, s_column);
+        case 64: return difference_body<DT, Logits64<DT>, WEIGHTED>(p, g, n, smem, s_bias, s_rows, s_column);
+        case 128: return difference_body<DT, Logits128<DT>, WEIGHTED>(p, g, n, smem, s_bias, s_rows, s_column);
     }
 }
 
@@ -474,12 +605,13 @@ __device__ __forceinline__ void dx_body(const Loss& p, const Gradient& g, int n,
     const int64_t all = share.row_tiles * share.column_tiles * share.splits, steps = g.columns / P::STEP;
     const Rows a{g.d, g.d_pitch, n, uint32_t(g.d_pitch)};
     const Rows b{p.w + g.first * p.w_pitch, p.w_pitch, min(g.columns, p.vocab - g.first), weight_rows<DT>(p).width};
+    typename P::Flow flow(smem, a, b);
     for (int64_t block = blockIdx.x; block < all; block += gridDim.x) {
         int64_t row, column, split;
         tile_of(block, share.row_tiles, share.column_tiles, share.splits, row, column, split);
         const int64_t m0 = row * P::BM, n0 = column * P::BN;
         typename P::Acc acc;
-        P::run(smem, a, b, m0, n0, steps * split / share.splits, steps * (split + 1) / share.splits, acc);
+        P::run(flow, {m0, n0, steps * split / share.splits, steps * (split + 1) / share.splits}, acc, P::ZEROS);
 #pragma unroll
         for (int i = 0; i < P::TM; ++i) {
             const int64_t m = m0 + P::wave_m() + i * M::SIDE + lane_m<DT>();
@@ -602,8 +734,10 @@ __global__ __launch_bounds__(512, 2) void loss_dweight_kernel(Loss p, Gradient g
     const int64_t columns = min(g.columns, p.vocab - g.first), row_tiles = (columns + BM - 1) / BM, column_tiles = g.dweight ? (p.hidden + BN - 1) / BN : 1, all = row_tiles * column_tiles;
     const int64_t steps = (n + P::STEP - 1) / P::STEP;
     const Rows a{g.d, g.d_pitch, n, uint32_t(g.d_pitch)}, b{g.shifted, p.pitch, n, uint32_t(p.pitch)};
+    typename P::Flow flow(smem, a, b);
     const int heights = n ? (n + tile_rows(n, 32) - 1) / tile_rows(n, 32) : 0;
     const float factor = n == 0 ? 0.f : (p.reduction ? row_factor(p, g, n) : *g.common) * (1.f / D_SCALE<DT>);
+    // (Tiles by themselves: with the next one's first step asked for ahead, as the logits have it, 8192 rows took 2650 to 2830 us instead of 1890.)
     for (int64_t block = blockIdx.x; block < all; block += gridDim.x) {
         int64_t row, column, split;
         tile_of(block, row_tiles, column_tiles, 1, row, column, split);
@@ -616,7 +750,7 @@ __global__ __launch_bounds__(512, 2) void loss_dweight_kernel(Loss p, Gradient g
         }
         if (!g.dweight) continue;
         typename P::Acc acc;
-        P::run(smem, a, b, m0, n0, 0, steps, acc);
+        P::run(flow, {m0, n0, 0, steps}, acc, P::ZEROS);
         P::store(
             smem, g.dweight + (g.first + m0) * g.dweight_pitch + n0 * int64_t(sizeof(T)), g.dweight_pitch, columns - m0, p.hidden - n0, g.wide_dweight,
             [&](int i, int j, int q) {
@@ -644,7 +778,7 @@ struct Plan {
     int64_t columns;                        // of a piece
     int blocks, finish_blocks;
     // offsets
-    int64_t index, place, label, top, inverse, right, gathered, state;
+    int64_t index, place, label, top, inverse, right, biases, gathered, state;
     int64_t maxima, sums, block_sums, forward;
     int64_t d, parts, part_pitch, column_sums, shifted, scale, share, shift, common, backward;
 };
@@ -668,7 +802,7 @@ Plan plan_of(const tdb_loss_args& a) {
         at += round_up(bytes, 256);
         return here;
     };
-    p.index = take(p.padded * 4), p.place = take(p.padded * 4), p.label = take(p.padded * 4), p.top = take(p.padded * 4), p.inverse = take(p.padded * 4), p.right = take(p.padded * 4);
+    p.index = take(p.padded * 4), p.place = take(p.padded * 4), p.label = take(p.padded * 4), p.top = take(p.padded * 4), p.inverse = take(p.padded * 4), p.right = take(p.padded * 4), p.biases = take(p.vocab * 4);
     p.gathered = take(p.padded * p.pitch);
     p.state = at;
     at = 0;
@@ -724,7 +858,7 @@ Loss loss_of(const tdb_loss_args& a, const Plan& p) {
     k.hidden = a.hidden, k.reduction = a.reduction, k.bias_kind = !a.bias ? 0 : a.bias_dtype == a.dtype ? 1 : 2, k.loss = a.loss;
     k.count = reinterpret_cast<int32_t*>(state), k.index = reinterpret_cast<int32_t*>(state + p.index), k.place = reinterpret_cast<int32_t*>(state + p.place);
     k.label = reinterpret_cast<int32_t*>(state + p.label), k.top = reinterpret_cast<float*>(state + p.top), k.inverse = reinterpret_cast<float*>(state + p.inverse);
-    k.gathered = state + p.gathered, k.pitch = p.pitch, k.padded = p.padded, k.group = p.group;
+    k.biases = reinterpret_cast<float*>(state + p.biases), k.gathered = state + p.gathered, k.pitch = p.pitch, k.padded = p.padded, k.group = p.group;
     k.right = reinterpret_cast<float*>(state + p.right), k.maxima = reinterpret_cast<float*>(work + p.maxima), k.sums = reinterpret_cast<float*>(work + p.sums);
     k.block_sums = reinterpret_cast<double*>(work + p.block_sums);
     return k;
@@ -756,9 +890,10 @@ hipError_t forward(const tdb_loss_args& a, hipStream_t s) {
     const Loss k = loss_of(a, p);
     const int64_t chunk = round_up(std::max<int64_t>(64, (a.rows + 511) / 512), 64);
     const bool wide = reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.x_stride * p.size % 16 == 0 && int64_t(a.hidden) * p.size % 16 == 0;
-    TDB_TRY(launch<loss_gather_kernel<DT>>(std::max<int64_t>(1, (a.rows + chunk - 1) / chunk), 64 * GATHER_WAVES, 0, s, k, chunk, wide));
+    const int64_t row_blocks = std::max<int64_t>(1, (a.rows + chunk - 1) / chunk), bias_blocks = (p.vocab + 256 * GATHER_WAVES - 1) / (256 * GATHER_WAVES);
+    TDB_TRY(launch<loss_gather_kernel<DT>>(row_blocks + bias_blocks, 64 * GATHER_WAVES, 0, s, k, chunk, int(row_blocks), wide));
     if (p.few) TDB_TRY(launch<loss_logits_few_kernel<DT>>(2 * p.blocks, 256, FEW_SHARED, s, k));
-    if (p.many) TDB_TRY(launch<loss_logits_many_kernel<DT>>(p.blocks, 512, MANY_SHARED, s, k));
+    if (p.many) TDB_TRY(launch<loss_logits_many_kernel<DT>>(p.blocks, 512, MANY_SHARED + TileArrays<Logits256<DT>, 2>::BYTES, s, k));
     return launch<loss_finish_kernel<DT>>(p.finish_blocks, 1024, 0, s, k);
 }
 
@@ -781,10 +916,10 @@ hipError_t backward(const tdb_loss_args& a, hipStream_t s) {
         g.columns = std::min(p.columns, p.vocab - g.first), g.later = g.first > 0;
         if (weighted) {
             if (p.few) TDB_TRY(launch<loss_difference_few_kernel<DT, true>>(2 * p.blocks, 256, FEW_SHARED, s, k, g));
-            if (p.many) TDB_TRY(launch<loss_difference_many_kernel<DT, true>>(p.blocks, 512, MANY_SHARED, s, k, g));
+            if (p.many) TDB_TRY(launch<loss_difference_many_kernel<DT, true>>(p.blocks, 512, MANY_SHARED + TileArrays<Logits256<DT>, 7>::BYTES, s, k, g));
         } else {
             if (p.few) TDB_TRY(launch<loss_difference_few_kernel<DT, false>>(2 * p.blocks, 256, FEW_SHARED, s, k, g));
-            if (p.many) TDB_TRY(launch<loss_difference_many_kernel<DT, false>>(p.blocks, 512, MANY_SHARED, s, k, g));
+            if (p.many) TDB_TRY(launch<loss_difference_many_kernel<DT, false>>(p.blocks, 512, MANY_SHARED + TileArrays<Logits256<DT>, 5>::BYTES, s, k, g));
         }
         if (a.rows && a.dx) TDB_TRY(launch<loss_dx_kernel<DT>>(p.blocks, 512, DX_SHARED, s, k, g));
         if (a.dweight || a.dbias) TDB_TRY(launch<loss_dweight_kernel<DT>>(p.blocks, 512, Dweight<DT>::SHARED, s, k, g));

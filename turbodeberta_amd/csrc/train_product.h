@@ -11,6 +11,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "tdb_internal.h"
 #include "tdb_train.h"
 
@@ -113,37 +115,41 @@ struct Side {
     static __device__ __forceinline__ int swap(int r) { return LINE == 128 ? r >> 1 & 7 : r >> 2 & 3; }
     static __device__ __forceinline__ int turn(int k) { return (DT == TDB_F32 ? k >> 2 & 3 : (k & 3) | (k >> 1 & 4)) & (BLOCKS - 1); }
 
-    // Tile of rows (lined) or columns (turned) first ..
-    __device__ __forceinline__ void place(const Rows& a, int64_t first) {
+    // The same for every tile.  Columns of a turned operand past its width come from its next row, or as zeros: they are sums of their own, which nobody stores.
+    __device__ __forceinline__ void place(const Rows& a) {
         const int wave = threadIdx.x >> 6, l = threadIdx.x & 63;
 #pragma unroll
         for (int j = 0; j < LOADS; ++j) {
             const int at = (wave * LOADS + j) * 64 + l, row = at / CHUNKS, chunk = at % CHUNKS;
             if constexpr (TURNED) {
-                const uint32_t c = ((((chunk >> 2) ^ turn(row)) << 2) | (chunk & 3)) * 16;
-                from[j] = c + uint32_t(first) * ES < a.width ? uint32_t(row) * uint32_t(a.pitch) + c : PAST;
+                from[j] = uint32_t(row) * uint32_t(a.pitch) + ((((chunk >> 2) ^ turn(row)) << 2) | (chunk & 3)) * 16;
             } else {
                 column[j] = (chunk ^ swap(row)) * 16;
                 from[j] = uint32_t(row) * uint32_t(a.pitch) + column[j];
             }
         }
     }
-    // Step s of the contraction into LDS.
-    __device__ __forceinline__ void load(const Rows& a, int64_t first, int64_t s, uint32_t lds) const {
-        const uint32_t to = lds + uniform(threadIdx.x >> 6) * (LOADS * 1024);
-        if constexpr (TURNED) {
-            const int64_t k = s * STEP;
-            const char* p = a.p + k * a.pitch + first * ES;
-            const u32x4 buffer = buffer_of(p, (a.count - 1 - k) * a.pitch + a.width - first * ES);
-#pragma unroll
-            for (int j = 0; j < LOADS; ++j) load_shared(to + j * 1024, buffer, from[j]);
-        } else {
-            const int64_t into = s * LINE;
-            const u32x4 buffer = buffer_of(a.p + first * a.pitch + into, (a.count - 1 - first) * a.pitch + a.width - into);
-            const bool whole = into + LINE <= a.width;
-#pragma unroll
-            for (int j = 0; j < LOADS; ++j) load_shared(to + j * 1024, buffer, whole || into + column[j] < a.width ? from[j] : PAST);
+    // Where a step's buffer begins and how much there is of it from there on; lined: of its rows too.
+    struct Cursor {
+        const char* p;
+        int64_t left, line;
+        __device__ __forceinline__ void seek(const Rows& a, int64_t first, int64_t step) {
+            if constexpr (TURNED) p = a.p + step * STEP * a.pitch + first * ES, left = (a.count - 1 - step * STEP) * a.pitch + a.width - first * ES, line = 0;
+            else p = a.p + first * a.pitch + step * LINE, left = (a.count - 1 - first) * a.pitch + a.width - step * LINE, line = a.width - step * LINE;
         }
+        __device__ __forceinline__ void advance(const Rows& a) {
+            const int64_t by = TURNED ? STEP * a.pitch : int64_t(LINE);
+            p += by, left -= by, line -= by;
+        }
+    };
+    // Loads lo .. hi - 1 of a step into LDS.  TAIL: rows may end inside a step (what follows them is another row; the other operand's zeros do not take an infinity's or NaN's place).
+    template <bool TAIL>
+    __device__ __forceinline__ void load(const Cursor& c, uint32_t lds, int lo = 0, int hi = LOADS) const {
+        const uint32_t to = lds + uniform(threadIdx.x >> 6) * (LOADS * 1024);
+        const u32x4 buffer = buffer_of(c.p, c.left);
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j)
+            if (j >= lo && j < hi) load_shared(to + j * 1024, buffer, TURNED || !TAIL || column[j] < uint32_t(min(c.line, int64_t(LINE))) ? from[j] : PAST);
     }
     // Frag of rows row .. (a multiple of SIDE), part kk of the step (32 bytes, or 64 of float32)
     __device__ __forceinline__ typename M::Frag frag(const char* lds, int row, int kk) const {
@@ -184,23 +190,51 @@ struct Product {
     static __device__ __forceinline__ int wave_m() { return int(uniform(threadIdx.x >> 6)) / WN * (BM / WM); }
     static __device__ __forceinline__ int wave_n() { return int(uniform(threadIdx.x >> 6)) % WN * (BN / WN); }
 
-    // Steps [begin, end) of the tile at rows m0 of A and n0 of B.  The sums start from start(j, q), four neighbours along n, called behind the first step's barrier.
-    template <class START>
-    static __device__ __forceinline__ void run(char* smem, const Rows& a, const Rows& b, int64_t m0, int64_t n0, int64_t begin, int64_t end, Acc& acc, START start) {
-        constexpr int LOADS = A::LOADS + B::LOADS;
+    // A tile: rows m0 of A, n0 of B, steps [begin, end) of the contraction.
+    struct Tile {
+        int64_t m0, n0, begin, end;
+    };
+    // The loads of step after step, of one tile after another.
+    struct Flow {
         A side_a;
         B side_b;
-        side_a.place(a, m0), side_b.place(b, n0);
-        const uint32_t lds = uniform(uint32_t(reinterpret_cast<uintptr_t>(TDB_SHARED(char, smem))));
-        auto load = [&](int64_t s, int stage) {
-            side_a.load(a, m0, s, lds + stage * STAGE);
-            side_b.load(b, n0, s, lds + stage * STAGE + A::BYTES);
-        };
-        const int steps = int(end - begin);
-        step_barrier();                     // nobody has use for what LDS held
+        typename A::Cursor at_a;
+        typename B::Cursor at_b;
+        Rows a, b;
+        char* smem;
+        uint32_t lds;
+        static constexpr int LOADS = A::LOADS + B::LOADS;
+        __device__ __forceinline__ Flow(char* smem, const Rows& a, const Rows& b) : a(a), b(b), smem(smem) {
+            side_a.place(a), side_b.place(b);
+            lds = uniform(uint32_t(reinterpret_cast<uintptr_t>(TDB_SHARED(char, smem))));
+        }
+        __device__ __forceinline__ void seek(const Tile& t) { at_a.seek(a, t.m0, t.begin), at_b.seek(b, t.n0, t.begin); }
+        __device__ __forceinline__ void nothing() { at_a.left = at_b.left = 0; }        // (zeros)
+        __device__ __forceinline__ void load(int stage, int lo = 0, int hi = LOADS) {
+            side_a.template load<false>(at_a, lds + stage * STAGE, lo, hi);
+            side_b.template load<!TURN_A>(at_b, lds + stage * STAGE + A::BYTES, lo - A::LOADS, hi - A::LOADS);
+            if (hi == LOADS) at_a.advance(a), at_b.advance(b);
+        }
+        __device__ __forceinline__ void frag_a(typename M::Frag& f, int stage, int i, int kk) const { f = side_a.frag(smem + stage * STAGE, wave_m() + i * M::SIDE, kk); }
+        __device__ __forceinline__ void frag_b(typename M::Frag& f, int stage, int j, int kk) const { f = side_b.frag(smem + stage * STAGE + A::BYTES, wave_n() + j * M::SIDE, kk); }
+    };
+    static __device__ __forceinline__ void products(const Flow& flow, int stage, Acc& acc) {
 #pragma unroll
-        for (int s = 0; s < NS - 1; ++s)
-            if (s < steps) load(begin + s, s);
+        for (int kk = 0; kk < PARTS; ++kk) {
+            typename M::Frag fa[TM], fb[TN];
+#pragma unroll
+            for (int i = 0; i < TM; ++i) flow.frag_a(fa[i], stage, i, kk);
+#pragma unroll
+            for (int j = 0; j < TN; ++j) flow.frag_b(fb[j], stage, j, kk);
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) acc[i][j] = M::mma(fb[j], fa[i], acc[i][j]);
+        }
+    }
+    // The sums start from start(j, q), four neighbours along n, called behind a barrier.
+    template <class START>
+    static __device__ __forceinline__ void begin_sums(Acc& acc, START start) {
 #pragma unroll
         for (int j = 0; j < TN; ++j)
 #pragma unroll
@@ -211,54 +245,145 @@ struct Product {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] = v[e];
             }
+    }
+    static constexpr auto ZEROS = [](int, int) { return f32x4{0.f, 0.f, 0.f, 0.f}; };
+
+    // One tile by itself.
+    template <class START>
+    static __device__ __forceinline__ void run(Flow& flow, const Tile& t, Acc& acc, START start) {
+        const int steps = int(t.end - t.begin);
+        step_barrier();                     // nobody has use for what LDS held
+        flow.seek(t);
+#pragma unroll
+        for (int s = 0; s < NS - 1; ++s)
+            if (s < steps) flow.load(s);
+        begin_sums(acc, start);
         int stage = 0, ahead = NS - 1;
         for (int s = 0; s < steps; ++s) {
-            if (s + NS - 2 < steps) wait_loads<(NS - 2) * LOADS>();
+            if (s + NS - 2 < steps) wait_loads<(NS - 2) * Flow::LOADS>();
             else wait_loads<0>();
             step_barrier();                 // this stage is there, and nobody reads the one before it any more
-            if (s + NS - 1 < steps) load(begin + s + NS - 1, ahead);
-            const char* at = smem + stage * STAGE;
-#pragma unroll
-            for (int kk = 0; kk < PARTS; ++kk) {
-                typename M::Frag fa[TM], fb[TN];
-#pragma unroll
-                for (int i = 0; i < TM; ++i) fa[i] = side_a.frag(at, wave_m() + i * M::SIDE, kk);
-#pragma unroll
-                for (int j = 0; j < TN; ++j) fb[j] = side_b.frag(at + A::BYTES, wave_n() + j * M::SIDE, kk);
-#pragma unroll
-                for (int i = 0; i < TM; ++i)
-#pragma unroll
-                    for (int j = 0; j < TN; ++j) acc[i][j] = M::mma(fb[j], fa[i], acc[i][j]);
-            }
+            if (s + NS - 1 < steps) flow.load(ahead);
+            products(flow, stage, acc);
             stage = stage == NS - 1 ? 0 : stage + 1;
             ahead = ahead == NS - 1 ? 0 : ahead + 1;
         }
         step_barrier();                     // LDS is free for what follows
     }
-    static __device__ __forceinline__ void run(char* smem, const Rows& a, const Rows& b, int64_t m0, int64_t n0, int64_t begin, int64_t end, Acc& acc) {
-        run(smem, a, b, m0, n0, begin, end, acc, [](int, int) { return f32x4{0.f, 0.f, 0.f, 0.f}; });
-    }
 
-    // The tile's values to rows of memory by way of LDS, SIDE rows at a time: value(i, j, q) gives four neighbours, then(i, the wave's rows in LDS) may change what lies there.
-    // to: value (m0, n0); rows and columns: how many of the tile's there are.  Whole 16-byte chunks where `wide`.
-    static constexpr int COLUMNS = TN * M::SIDE, PITCH = COLUMNS * int(sizeof(T)) + 16;
+    // Tiles one after another with two stages: the first step of the next tile, and what beside.load asks for it, are on their way while this one's last steps are made.  `stage` holds the
+    // first step of this tile, which open or the call before has asked for; behind the call the next one's, and scratch(smem, stage) is free.  LATER: memory
+    // operations that every wave has issued since the last call asked for this tile's, unless it is the first one.
+    template <class BESIDE>
+    static __device__ __forceinline__ void open(Flow& flow, const Tile& t, BESIDE& beside) {
+        static_assert(NS == 2, "");
+        flow.seek(t);
+        beside.load(t);
+        if (t.begin < t.end) flow.load(0);
+    }
+    static __device__ __forceinline__ char* scratch(char* smem, int stage) { return smem + (stage ^ 1) * STAGE; }
+    template <int LATER, class START, class BESIDE>
+    static __device__ __forceinline__ void run_on(Flow& flow, const Tile& t, const Tile& next, bool more, int& stage, bool first, Acc& acc, START start, BESIDE& beside) {
+        const int steps = int(t.end - t.begin);
+        auto go_on = [&]() {
+            if (more) flow.seek(next), beside.load(next);
+            else flow.nothing();
+        };
+        if (LATER == 0 || first) wait_loads<0>();
+        else wait_loads<LATER>();
+        step_barrier();
+        if (steps == 1) go_on();
+        if (steps) flow.load(stage ^ 1);
+        begin_sums(acc, start);
+        if (steps == 0) {
+            if (more) beside.load(next);
+        } else if constexpr (DT == TDB_F32) {
+            for (int s = 0; s < steps; ++s) {
+                if (s) {
+                    wait_loads<0>();
+                    step_barrier();
+                    if (s + 1 == steps) go_on();
+                    flow.load(stage ^ 1);
+                }
+                products(flow, stage, acc);
+                stage ^= 1;
+            }
+        } else {
+            // The frags of a quarter of a step are read while the products of the one before it are made, each of which keeps the matrix pipe busy for 32 clk; the barrier lies in front of a
+            // step's last quarter, whose frags are in registers by then, and with that quarter the loads of the step after the next one are issued.
+            typename M::Frag fa[2][TM], fb[2][TN];
+            auto multiply = [&](auto KK, auto READ, int from, auto LOAD, int to) {
+                constexpr int kk = decltype(KK)::value, OPS = TM * TN, R = TM + TN, set = (kk + 1) & 1;
+#pragma unroll
+                for (int op = 0; op < OPS; ++op) {
+                    acc[op / TN][op % TN] = M::mma(fb[kk & 1][op % TN], fa[kk & 1][op / TN], acc[op / TN][op % TN]);
+                    __builtin_amdgcn_sched_barrier(0);
+                    if constexpr (decltype(READ)::value) {
+#pragma unroll
+                        for (int r = R * op / OPS; r < R * (op + 1) / OPS; ++r) {
+                            if (r < TN) flow.frag_b(fb[set][r < TN ? r : 0], from, r, (kk + 1) % PARTS);
+                            else flow.frag_a(fa[set][r < TN ? 0 : r - TN], from, r - TN, (kk + 1) % PARTS);
+                        }
+                    }
+                    if constexpr (decltype(LOAD)::value) flow.load(to, Flow::LOADS * op / OPS, Flow::LOADS * (op + 1) / OPS);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            };
+            static_assert(PARTS == 4, "");
+            constexpr std::true_type yes;
+            constexpr std::false_type no;
+            constexpr std::integral_constant<int, 0> q0;
+            constexpr std::integral_constant<int, 1> q1;
+            constexpr std::integral_constant<int, 2> q2;
+            constexpr std::integral_constant<int, 3> q3;
+#pragma unroll
+            for (int i = 0; i < TM; ++i) flow.frag_a(fa[0][i], stage, i, 0);
+#pragma unroll
+            for (int j = 0; j < TN; ++j) flow.frag_b(fb[0][j], stage, j, 0);
+            for (int s = 0; s + 1 < steps; ++s) {
+                multiply(q0, yes, stage, no, 0);
+                multiply(q1, yes, stage, no, 0);
+                multiply(q2, yes, stage, no, 0);
+                wait_loads<0>();
+                step_barrier();
+                if (s + 2 == steps) go_on();
+                multiply(q3, yes, stage ^ 1, yes, stage);
+                stage ^= 1;
+            }
+            multiply(q0, yes, stage, no, 0);
+            multiply(q1, yes, stage, no, 0);
+            multiply(q2, yes, stage, no, 0);
+            multiply(q3, no, 0, no, 0);
+            stage ^= 1;
+        }
+        step_barrier();
+    }
+    // Nothing beside the product's operands.
+    struct Alone {
+        __device__ __forceinline__ void load(const Tile&) {}
+    };
+
+    // The tile's values to rows of memory by way of LDS (SCRATCH bytes), SIDE rows at a time: value(i, j, q) gives four neighbours, then(i, the wave's rows in LDS) may change what
+    // lies there.  to: value (m0, n0); rows and columns: how many of the tile's there are.  Whole 16-byte chunks where `wide`: STORES memory operations of every wave.
+    static constexpr int COLUMNS = TN * M::SIDE, ROW = COLUMNS * int(sizeof(T)), PER = ROW / 16, SCRATCH = WAVES * 2 * M::SIDE * ROW, STORES = TM * M::SIDE * PER / 64;
+    // Where byte b of a wave's row lies: 16-byte chunks exchanged so that 16 rows' chunks are on distinct banks.
+    static __device__ __forceinline__ int lies_at(int row, int b) { return row * ROW + (b ^ ((row * ROW / 256 & (PER - 1)) << 4)); }
     template <class OF, class THEN>
-    static __device__ __forceinline__ void store(char* smem, char* to, int64_t pitch, int64_t rows, int64_t columns, bool wide, OF value, THEN then) {
-        constexpr int ES = sizeof(T), PER = COLUMNS * ES / 16;
+    static __device__ __forceinline__ void store(char* scratch, char* to, int64_t pitch, int64_t rows, int64_t columns, bool wide, OF value, THEN then) {
+        constexpr int ES = sizeof(T);
         typedef __attribute__((ext_vector_type(4))) T T4;
         const int l = threadIdx.x & 63;
-        char* const own = smem + uniform(threadIdx.x >> 6) * (2 * M::SIDE * PITCH);
-        static_assert(WAVES * 2 * M::SIDE * PITCH <= SHARED, "");
+        char* const own = scratch + uniform(threadIdx.x >> 6) * (2 * M::SIDE * ROW);
         to += wave_m() * pitch + wave_n() * ES, rows -= wave_m(), columns -= wave_n();
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
-            char* const mine = own + (i & 1) * (M::SIDE * PITCH);
+            char* const mine = own + (i & 1) * (M::SIDE * ROW);
 #pragma unroll
             for (int j = 0; j < TN; ++j)
 #pragma unroll
                 for (int q = 0; q < M::QUADS; ++q) {
                     const f32x4 v = value(i, j, q);
-                    *reinterpret_cast<T4*>(mine + lane_m<DT>() * PITCH + (j * M::SIDE + quad_n<DT>(q)) * ES) = T4{T(v[0]), T(v[1]), T(v[2]), T(v[3])};
+                    *reinterpret_cast<T4*>(mine + lies_at(lane_m<DT>(), (j * M::SIDE + quad_n<DT>(q)) * ES)) = T4{T(v[0]), T(v[1]), T(v[2]), T(v[3])};
                 }
             then(i, mine);
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -268,13 +393,13 @@ struct Product {
 #pragma unroll
                 for (int r = 0; r < M::SIDE * PER / 64; ++r) {
                     const int at = r * 64 + l, row = at / PER, c = at % PER;
-                    const u32x4 v = *reinterpret_cast<const u32x4*>(mine + row * PITCH + c * 16);
+                    const u32x4 v = *reinterpret_cast<const u32x4*>(mine + lies_at(row, c * 16));
                     __builtin_amdgcn_raw_buffer_store_b128(v, buffer, c * 16 < columns * ES ? uint32_t(row) * uint32_t(pitch) + c * 16 : PAST, 0, 0);
                 }
             } else {
                 for (int at = l; at < M::SIDE * COLUMNS; at += 64) {
                     const int row = at / COLUMNS, c = at % COLUMNS;
-                    if (i * M::SIDE + row < rows && c < columns) *reinterpret_cast<T*>(to + (i * M::SIDE + row) * pitch + c * ES) = *reinterpret_cast<const T*>(mine + row * PITCH + c * ES);
+                    if (i * M::SIDE + row < rows && c < columns) *reinterpret_cast<T*>(to + (i * M::SIDE + row) * pitch + c * ES) = *reinterpret_cast<const T*>(mine + lies_at(row, c * ES));
                 }
             }
         }
