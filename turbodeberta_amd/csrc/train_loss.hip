@@ -22,11 +22,14 @@ constexpr int TILE = 256;           // what rows and columns of the buffers are 
 constexpr int FINISH_ROWS = 32;     // rows of a workgroup of the last forward kernel
 constexpr int FEW = 1024;           // rows up to which tiles may be lower than 256
 
-// Rows of a tile where n count: what leaves the least of them empty, with lower tiles' smaller share of products in what they load counted in.
+// Rows of a tile where n count: the height with the least rows times what a row of such tiles costs.  16 bits, 128100 x 768: a tile's logits and their gradient took 125 us for 256 rows,
+// 70 to 77 for 128, 48 for 64, 31 for 32 (lower tiles load more for their products); float32, bound by products, 770, 390, 213, 116.  160 rows of float32: 610 us in tiles of
+// 32, 677 of 64, 770 of 256; of bfloat16 173, 163, 130.
+template <int DT>
 __host__ __device__ constexpr int tile_rows(int n, int least) {
     int best = 256, cost = (n + 255) / 256 * 256 * 16;
     if (n > FEW) return best;
-    const int heights[] = {128, 64, 32}, dear[] = {18, 21, 26};
+    const int heights[] = {128, 64, 32}, dear[] = {DT == TDB_F32 ? 16 : 20, DT == TDB_F32 ? 18 : 26, DT == TDB_F32 ? 19 : 32};
     for (int i = 0; i < 3; ++i) {
         const int h = heights[i], c = (n + h - 1) / h * h * dear[i];
         if (h >= least && c < cost) best = h, cost = c;
@@ -58,11 +61,10 @@ struct Loss {
     int32_t group;                              // column tiles that a workgroup of the kernel for many rows takes together
 };
 
-// How the logits' maxima and sums lie: groups of column tiles, rows `pitch` to each.  Tiles of fewer than 256 rows are 128 classes wide, the others 256.
+// How the logits' maxima and sums lie: groups of column tiles, rows `pitch` to each.
 struct Partials {
     int64_t groups, tiles, group, pitch;
-    __device__ __forceinline__ Partials(const Loss& p, bool many)
-        : tiles((p.vocab + (many ? 255 : 127)) / (many ? 256 : 128)), group(many ? p.group : 1), pitch(many ? p.padded : min(p.padded, int64_t(FEW))) {
+    __device__ __forceinline__ Partials(const Loss& p, bool many) : tiles((p.vocab + 255) / 256), group(many ? p.group : 1), pitch(many ? p.padded : min(p.padded, int64_t(FEW))) {
         groups = (tiles + group - 1) / group;
     }
 };
@@ -290,13 +292,13 @@ struct TileArrays {
 template <int DT>
 using Logits256 = Product<DT, 256, 256, 2, 4, 2, false, false>;
 template <int DT>
-using Logits128 = Product<DT, 128, 128, 2, 2, 4, false, false, 64>;
+using Logits128 = Product<DT, 128, 256, 1, 4, 3, false, false, 64>;
 template <int DT>
-using Logits64 = Product<DT, 64, 128, 1, 4, 6, false, false, 64>;
+using Logits64 = Product<DT, 64, 256, 1, 4, 3, false, false, 64>;
 template <int DT>
-using Logits32 = Product<DT, 32, 128, 1, 4, 3, false, false, 128>;
-constexpr int MANY_SHARED = Logits256<TDB_BF16>::SHARED,  FEW_SHARED = Logits64<TDB_BF16>::SHARED;
-static_assert(Logits128<TDB_BF16>::SHARED <= FEW_SHARED && Logits32<TDB_BF16>::SHARED <= FEW_SHARED, "");
+using Logits32 = Product<DT, 32, 256, 1, 4, 2, false, false, 128>;
+constexpr int MANY_SHARED = Logits256<TDB_BF16>::SHARED,  FEW_SHARED = Logits128<TDB_BF16>::SHARED;
+static_assert(Logits64<TDB_BF16>::SHARED <= FEW_SHARED && Logits32<TDB_BF16>::SHARED <= FEW_SHARED, "");
 
 template <int DT>
 __global__ __launch_bounds__(512, 2) void loss_logits_many_kernel(Loss p) {
@@ -304,7 +306,7 @@ __global__ __launch_bounds__(512, 2) void loss_logits_many_kernel(Loss p) {
     __shared__ float s_top[1024], s_sum[1024];
     using P = Logits256<DT>;
     const int n = p.count[0];
-    if (tile_rows(n, 32) != 256) return;
+    if (tile_rows<DT>(n, 32) != 256) return;
     const Partials parts(p, true);
     const int64_t row_tiles = (n + P::BM - 1) / P::BM, all = row_tiles * parts.groups;
     typename P::Flow flow(smem, hidden_rows<DT>(p, n), weight_rows<DT>(p));
@@ -346,11 +348,11 @@ __global__ __launch_bounds__(512, 2) void loss_logits_many_kernel(Loss p) {
 template <int DT>
 __global__ __launch_bounds__(256, 2) void loss_logits_few_kernel(Loss p) {
     extern __shared__ __attribute__((aligned(1024))) char smem[];
-    __shared__ __attribute__((aligned(16))) float s_bias[128];
+    __shared__ __attribute__((aligned(16))) float s_bias[256];
     __shared__ int32_t s_label[128];
-    __shared__ float s_top[256], s_sum[256];
+    __shared__ float s_top[512], s_sum[512];
     const int n = p.count[0];
-    switch (tile_rows(n, 32)) {
+    switch (tile_rows<DT>(n, 32)) {
         case 32: return logits_body<DT, Logits32<DT>>(p, n, smem, s_bias, s_label, s_top, s_sum);
         case 64: return logits_body<DT, Logits64<DT>>(p, n, smem, s_bias, s_label, s_top, s_sum);
         case 128: return logits_body<DT, Logits128<DT>>(p, n, smem, s_bias, s_label, s_top, s_sum);
@@ -364,7 +366,7 @@ __global__ __launch_bounds__(1024) void loss_finish_kernel(Loss p) {
     __shared__ double s_all[1024];
     __shared__ bool s_last;
     const int n = p.count[0], l = threadIdx.x & 31, w = threadIdx.x >> 5;
-    const Partials parts(p, tile_rows(n, 32) == 256);
+    const Partials parts(p, tile_rows<DT>(n, 32) == 256);
     const int groups = int(parts.groups);
     double mine = 0.0;
     for (int64_t r0 = int64_t(blockIdx.x) * FINISH_ROWS; r0 < n; r0 += int64_t(gridDim.x) * FINISH_ROWS) {
@@ -415,14 +417,17 @@ __global__ __launch_bounds__(1024) void loss_finish_kernel(Loss p) {
         }
     };
     total(mine);
+    // (only workgroups that have rows, or the first one, take part)
+    const int parts_done = max(1, min(int(gridDim.x), (n + FINISH_ROWS - 1) / FINISH_ROWS));
+    if (int(blockIdx.x) >= parts_done) return;
     if (threadIdx.x == 0) {
         __hip_atomic_store(p.block_sums + blockIdx.x, s_all[0], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        s_last = __hip_atomic_fetch_add(p.count + 1, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == int(gridDim.x) - 1;
+        s_last = __hip_atomic_fetch_add(p.count + 1, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == parts_done - 1;
     }
     __syncthreads();
     if (!s_last) return;
     double sum = 0.0;
-    for (unsigned i = threadIdx.x; i < gridDim.x; i += 1024) sum += __hip_atomic_load(p.block_sums + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (int i = threadIdx.x; i < parts_done; i += 1024) sum += __hip_atomic_load(p.block_sums + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     total(sum);
     if (threadIdx.x == 0) p.loss[0] = float(p.reduction == 2 ? s_all[0] / double(n) : s_all[0]);
 }
@@ -541,7 +546,7 @@ __global__ __launch_bounds__(512, 2) void loss_difference_many_kernel(Loss p, Gr
     __shared__ float s_column[512];
     using P = Logits256<DT>;
     const int n = p.count[0];
-    if (tile_rows(n, 32) != 256) return;
+    if (tile_rows<DT>(n, 32) != 256) return;
     const int64_t row_tiles = (n + P::BM - 1) / P::BM, column_tiles = g.columns / P::BN, all = row_tiles * column_tiles;
     typename P::Flow flow(smem, hidden_rows<DT>(p, n), weight_rows<DT>(p));
     constexpr int ARRAYS = WEIGHTED ? 7 : 5;
@@ -575,10 +580,10 @@ __global__ __launch_bounds__(512, 2) void loss_difference_many_kernel(Loss p, Gr
 template <int DT, bool WEIGHTED>
 __global__ __launch_bounds__(256, 2) void loss_difference_few_kernel(Loss p, Gradient g) {
     extern __shared__ __attribute__((aligned(1024))) char smem[];
-    __shared__ __attribute__((aligned(16))) float s_bias[128];
+    __shared__ __attribute__((aligned(16))) float s_bias[256];
     __shared__ float s_column[256], s_rows[6][128];
     const int n = p.count[0];
-    switch (tile_rows(n, 32)) {
+    switch (tile_rows<DT>(n, 32)) {
         case 32: return difference_body<DT, Logits32<DT>, WEIGHTED>(p, g, n, smem, s_bias, s_rows, s_column);
         case 64: return difference_body<DT, Logits64<DT>, WEIGHTED>(p, g, n, smem, s_bias, s_rows, s_column);
         case 128: return difference_body<DT, Logits128<DT>, WEIGHTED>(p, g, n, smem, s_bias, s_rows, s_column);
@@ -591,7 +596,8 @@ struct Shares {
     int height;
     int64_t row_tiles, column_tiles, splits;
     __device__ __forceinline__ Shares(const Loss& p, const Gradient& g, int n, int64_t blocks) {
-        height = tile_rows(n, 64);
+        // (Up to 192 rows the product waits for the weights whatever its tiles' height, and low ones make fewer parts to be added up: 154 x 768, tiles of 256 rows 56 + 27 us, of 64 57 + 10.)
+        height = n <= 192 ? 64 : tile_rows<DT>(n, 128);
         row_tiles = (n + height - 1) / height, column_tiles = (p.hidden + 255) / 256;
         const int64_t tiles = row_tiles * column_tiles;
         splits = tiles ? max(int64_t(1), min(blocks / tiles, g.columns * int64_t(sizeof(typename Matrix<DT>::T)) / 128)) : 0;
@@ -655,13 +661,51 @@ __global__ __launch_bounds__(512, 2) void loss_dx_kernel(Loss p, Gradient g) {
 // What the gradient of a sum or mean makes of every row.
 __device__ __forceinline__ float row_factor(const Loss& p, const Gradient& g, int n) { return p.reduction == 2 ? g.dloss[0] / float(n) : g.dloss[0]; }
 
-// dx: a workgroup for each row, its four waves share out the parts; zeros where the row does not count.  blocks: workgroups of the launch before.
+// dx, zeros where a row does not count.  Where few rows are split over many parts a workgroup has a row and its waves share out the parts, otherwise each wave has a row.
+// blocks: workgroups of the launch before.
 template <int DT>
 __global__ __launch_bounds__(256) void loss_dx_sum_kernel(Loss p, Gradient g, int blocks) {
     using T = typename Matrix<DT>::T;
     __shared__ float s_sum[4][256];
     const int n = p.count[0], l = threadIdx.x & 63, w = threadIdx.x >> 6;
     const Shares<DT> share(p, g, n, blocks);
+    const int64_t apart = share.row_tiles * share.height * g.part_pitch;
+    auto factor_of = [&](int place) { return (p.reduction ? row_factor(p, g, n) : *g.common * g.shift[place]) * (1.f / D_SCALE<DT>); };
+    // parts first, first + step, ... of columns c ..
+    auto sum_of = [&](int place, int64_t c, int64_t first, int64_t step) {
+        const float* const from = g.parts + place * g.part_pitch + min(c, g.part_pitch - 4);
+        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+        for (int64_t s = first; s < share.splits; s += 4 * step) {
+            f32x4 x[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) x[u] = *reinterpret_cast<const f32x4*>(from + min(s + u * step, share.splits - 1) * apart);
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (s + u * step < share.splits) sum += x[u];
+        }
+        return sum;
+    };
+    if (share.splits <= 16) {
+        const bool wide = reinterpret_cast<uintptr_t>(g.dx) % (4 * sizeof(T)) == 0 && g.dx_stride % 4 == 0 && p.hidden % 4 == 0;
+        for (int64_t row = int64_t(blockIdx.x) * 4 + w; row < p.rows; row += int64_t(gridDim.x) * 4) {
+            const int place = p.place[row];
+            T* const to = static_cast<T*>(g.dx) + row * g.dx_stride;
+            const float factor = place < 0 ? 0.f : factor_of(place);
+            for (int c = 4 * l; c < p.hidden; c += 256) {
+                f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+                if (place >= 0) sum = sum_of(place, c, 0, 1) * factor;
+                if (wide) {
+                    typedef __attribute__((ext_vector_type(4))) T T4;
+                    *reinterpret_cast<T4*>(to + c) = T4{T(sum[0]), T(sum[1]), T(sum[2]), T(sum[3])};
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (c + e < p.hidden) to[c + e] = T(sum[e]);
+                }
+            }
+        }
+        return;
+    }
     for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
         const int place = p.place[row];
         T* const to = static_cast<T*>(g.dx) + row * g.dx_stride;
@@ -669,20 +713,9 @@ __global__ __launch_bounds__(256) void loss_dx_sum_kernel(Loss p, Gradient g, in
             for (int c = threadIdx.x; c < p.hidden; c += 256) to[c] = T(0.f);
             continue;
         }
-        const float factor = (p.reduction ? row_factor(p, g, n) : *g.common * g.shift[place]) * (1.f / D_SCALE<DT>);
-        const float* const from = g.parts + place * g.part_pitch;
-        const int64_t apart = share.row_tiles * share.height * g.part_pitch;
+        const float factor = factor_of(place);
         for (int c0 = 0; c0 < p.hidden; c0 += 256) {
-            const int64_t c = min(int64_t(c0 + 4 * l), g.part_pitch - 4);
-            f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-            for (int64_t s = w; s < share.splits; s += 16) {
-                f32x4 x[4];
-#pragma unroll
-                for (int u = 0; u < 4; ++u) x[u] = *reinterpret_cast<const f32x4*>(from + min(s + 4 * u, share.splits - 1) * apart + c);
-#pragma unroll
-                for (int u = 0; u < 4; ++u)
-                    if (s + 4 * u < share.splits) sum += x[u];
-            }
+            const f32x4 sum = sum_of(place, c0 + 4 * l, w, 4);
             __syncthreads();
             *reinterpret_cast<f32x4*>(&s_sum[w][4 * l]) = sum;
             __syncthreads();
@@ -735,7 +768,7 @@ __global__ __launch_bounds__(512, 2) void loss_dweight_kernel(Loss p, Gradient g
     const int64_t steps = (n + P::STEP - 1) / P::STEP;
     const Rows a{g.d, g.d_pitch, n, uint32_t(g.d_pitch)}, b{g.shifted, p.pitch, n, uint32_t(p.pitch)};
     typename P::Flow flow(smem, a, b);
-    const int heights = n ? (n + tile_rows(n, 32) - 1) / tile_rows(n, 32) : 0;
+    const int heights = n ? (n + tile_rows<DT>(n, 32) - 1) / tile_rows<DT>(n, 32) : 0;
     const float factor = n == 0 ? 0.f : (p.reduction ? row_factor(p, g, n) : *g.common) * (1.f / D_SCALE<DT>);
     // (Tiles by themselves: with the next one's first step asked for ahead, as the logits have it, 8192 rows took 2650 to 2830 us instead of 1890.)
     for (int64_t block = blockIdx.x; block < all; block += gridDim.x) {
@@ -795,7 +828,7 @@ Plan plan_of(const tdb_loss_args& a) {
     const int64_t most = std::min<int64_t>(std::max<int64_t>(D_BYTES / (p.padded * p.size) / TILE, 1), (int64_t(1) << 22) / p.size / TILE), pieces = (wide + most - 1) / most;
     p.columns = (wide + pieces - 1) / pieces * TILE;
     p.blocks = std::max(8, tdb_compute_units(-1) & -8);
-    p.finish_blocks = int(std::min<int64_t>((std::max<int64_t>(a.rows, 1) + FINISH_ROWS - 1) / FINISH_ROWS, 512));
+    p.finish_blocks = int(std::min<int64_t>((std::max<int64_t>(a.rows, 1) + FINISH_ROWS - 1) / FINISH_ROWS, 256));
     int64_t at = 256;
     auto take = [&](int64_t bytes) {
         const int64_t here = at;
@@ -806,7 +839,7 @@ Plan plan_of(const tdb_loss_args& a) {
     p.gathered = take(p.padded * p.pitch);
     p.state = at;
     at = 0;
-    const int64_t partials = std::max((wide + p.group - 1) / p.group * p.padded, 2 * wide * std::min<int64_t>(p.padded, FEW)) * 4;
+    const int64_t partials = std::max((wide + p.group - 1) / p.group * p.padded, wide * std::min<int64_t>(p.padded, FEW)) * 4;
     p.maxima = take(partials), p.sums = take(partials), p.block_sums = take(p.finish_blocks * 8);
     p.forward = at;
     at = 0;
@@ -926,7 +959,7 @@ hipError_t backward(const tdb_loss_args& a, hipStream_t s) {
     }
     if (a.rows && a.dx) {
         g.columns = p.columns;              // (what the parts of dx were shared out by: the first piece's)
-        TDB_TRY(launch<loss_dx_sum_kernel<DT>>(std::min<int64_t>(a.rows, 1 << 16), 256, 0, s, k, g, p.blocks));
+        TDB_TRY(launch<loss_dx_sum_kernel<DT>>(std::min<int64_t>(a.rows, 2048), 256, 0, s, k, g, p.blocks));
     }
     return hipSuccess;
 }
