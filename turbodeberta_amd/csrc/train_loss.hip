@@ -595,10 +595,11 @@ template <int DT>
 struct Shares {
     int height;
     int64_t row_tiles, column_tiles, splits;
-    __device__ __forceinline__ Shares(const Loss& p, const Gradient& g, int n, int64_t blocks) {
+    __device__ __forceinline__ Shares(const Loss& p, const Gradient& g, int n, int64_t blocks, int width) {
         // (Up to 192 rows the product waits for the weights whatever its tiles' height, and low ones make fewer parts to be added up: 154 x 768, tiles of 256 rows 56 + 27 us, of 64 57 + 10.)
         height = n <= 192 ? 64 : tile_rows<DT>(n, 128);
-        row_tiles = (n + height - 1) / height, column_tiles = (p.hidden + 255) / 256;
+        if (height == 64 && width == 192) width = 256;
+        row_tiles = (n + height - 1) / height, column_tiles = (p.hidden + width - 1) / width;
         const int64_t tiles = row_tiles * column_tiles;
         splits = tiles ? max(int64_t(1), min(blocks / tiles, g.columns * int64_t(sizeof(typename Matrix<DT>::T)) / 128)) : 0;
     }
@@ -637,24 +638,25 @@ __device__ __forceinline__ void dx_body(const Loss& p, const Gradient& g, int n,
     }
 }
 
-template <int DT>
-using Dx256 = Product<DT, 256, 256, 2, 4, 2, false, true>;
-template <int DT>
-using Dx128 = Product<DT, 128, 256, 2, 4, 3, false, true>;
-template <int DT>
-using Dx64 = Product<DT, 64, 256, 1, 8, 3, false, true>;
-constexpr int DX_SHARED = Dx128<TDB_BF16>::SHARED;
-static_assert(Dx256<TDB_BF16>::SHARED <= DX_SHARED && Dx64<TDB_BF16>::SHARED <= DX_SHARED, "");
+// Tiles of dx and dW are 256, 192 or 128 columns wide.
+template <int DT, int BN>
+using Dx256 = Product<DT, 256, BN, BN == 256 ? 2 : 4, BN == 256 ? 4 : 2, 2, false, true>;
+template <int DT, int BN>
+using Dx128 = Product<DT, 128, BN, BN == 256 ? 2 : 4, BN == 256 ? 4 : 2, 3, false, true>;
+template <int DT, int BN>
+using Dx64 = Product<DT, 64, BN == 192 ? 256 : BN, BN == 128 ? 2 : 1, BN == 128 ? 4 : 8, 3, false, true>;
+constexpr int DX_SHARED = Dx128<TDB_BF16, 256>::SHARED;
+static_assert(Dx256<TDB_BF16, 256>::SHARED <= DX_SHARED && Dx64<TDB_BF16, 256>::SHARED <= DX_SHARED, "");
 
-template <int DT>
+template <int DT, int BN>
 __global__ __launch_bounds__(512, 2) void loss_dx_kernel(Loss p, Gradient g) {
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     const int n = p.count[0];
-    const Shares<DT> share(p, g, n, gridDim.x);
+    const Shares<DT> share(p, g, n, gridDim.x, BN);
     switch (share.height) {
-        case 64: return dx_body<DT, Dx64<DT>>(p, g, n, share, smem);
-        case 128: return dx_body<DT, Dx128<DT>>(p, g, n, share, smem);
-        default: return dx_body<DT, Dx256<DT>>(p, g, n, share, smem);
+        case 64: return dx_body<DT, Dx64<DT, BN>>(p, g, n, share, smem);
+        case 128: return dx_body<DT, Dx128<DT, BN>>(p, g, n, share, smem);
+        default: return dx_body<DT, Dx256<DT, BN>>(p, g, n, share, smem);
     }
 }
 
@@ -662,13 +664,13 @@ __global__ __launch_bounds__(512, 2) void loss_dx_kernel(Loss p, Gradient g) {
 __device__ __forceinline__ float row_factor(const Loss& p, const Gradient& g, int n) { return p.reduction == 2 ? g.dloss[0] / float(n) : g.dloss[0]; }
 
 // dx, zeros where a row does not count.  Where few rows are split over many parts a workgroup has a row and its waves share out the parts, otherwise each wave has a row.
-// blocks: workgroups of the launch before.
+// blocks, width: workgroups of the launch before and its tiles' columns.
 template <int DT>
-__global__ __launch_bounds__(256) void loss_dx_sum_kernel(Loss p, Gradient g, int blocks) {
+__global__ __launch_bounds__(256) void loss_dx_sum_kernel(Loss p, Gradient g, int blocks, int width) {
     using T = typename Matrix<DT>::T;
     __shared__ float s_sum[4][256];
     const int n = p.count[0], l = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const Shares<DT> share(p, g, n, blocks);
+    const Shares<DT> share(p, g, n, blocks, width);
     const int64_t apart = share.row_tiles * share.height * g.part_pitch;
     auto factor_of = [&](int place) { return (p.reduction ? row_factor(p, g, n) : *g.common * g.shift[place]) * (1.f / D_SCALE<DT>); };
     // parts first, first + step, ... of columns c ..
@@ -754,15 +756,15 @@ __global__ __launch_bounds__(256) void loss_weigh_kernel(Loss p, Gradient g) {
 }
 
 // dW and dbias of a piece.
-template <int DT>
-using Dweight = Product<DT, 256, 256, 2, 4, 2, true, true>;
+template <int DT, int BN>
+using Dweight = Product<DT, 256, BN, BN == 256 ? 2 : 4, BN == 256 ? 4 : 2, 2, true, true>;
 
-template <int DT>
+template <int DT, int BN>
 __global__ __launch_bounds__(512, 2) void loss_dweight_kernel(Loss p, Gradient g) {
     extern __shared__ __attribute__((aligned(1024))) char smem[];
-    using P = Dweight<DT>;
+    using P = Dweight<DT, BN>;
     using T = typename Matrix<DT>::T;
-    constexpr int BM = P::BM, BN = P::BN;
+    constexpr int BM = P::BM;
     const int n = p.count[0];
     const int64_t columns = min(g.columns, p.vocab - g.first), row_tiles = (columns + BM - 1) / BM, column_tiles = g.dweight ? (p.hidden + BN - 1) / BN : 1, all = row_tiles * column_tiles;
     const int64_t steps = (n + P::STEP - 1) / P::STEP;
@@ -803,10 +805,20 @@ constexpr int64_t PARTIAL_BYTES = int64_t(1) << 27;
 
 int64_t round_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 
+// The width with the fewest columns past the end, times what a column of such tiles costs.  dx and dW of 2500 x 768, 128100 classes, in tiles of 256, 192 and 128 columns: bfloat16 926, 1044 and
+// 1269 us, float32 7.37, 7.57 and 7.70 ms; 384 wide 649, 575 and 704 us, 4.92, 3.79 and 3.86 ms.
+int tile_columns(int hidden, int dtype) {
+    int best = 256, cost = (hidden + 255) / 256 * 256 * 64;
+    const int widths[] = {192, 128}, dear[] = {dtype == TDB_F32 ? 66 : 72, dtype == TDB_F32 ? 67 : 88};
+    for (int i = 0; i < 2; ++i)
+        if (const int c = (hidden + widths[i] - 1) / widths[i] * widths[i] * dear[i]; c < cost) best = widths[i], cost = c;
+    return best;
+}
+
 struct Plan {
     int size;                               // of a value
     int64_t padded, pitch, vocab;           // rows and bytes of the gathered rows, vocabulary, rounded up
-    int32_t group;
+    int32_t group, width;                   // width: columns of the tiles of dx and dW
     bool many, few;                         // whether there may be as many or as few rows as the kernels are for
     int64_t columns;                        // of a piece
     int blocks, finish_blocks;
@@ -824,6 +836,7 @@ Plan plan_of(const tdb_loss_args& a) {
     p.vocab = round_up(a.vocab, TILE);
     const int64_t wide = p.vocab / TILE;
     p.group = int32_t((wide * p.padded * 8 + PARTIAL_BYTES - 1) / PARTIAL_BYTES);
+    p.width = tile_columns(a.hidden, a.dtype);
     p.many = a.rows > 128, p.few = a.rows > 0;
     const int64_t most = std::min<int64_t>(std::max<int64_t>(D_BYTES / (p.padded * p.size) / TILE, 1), (int64_t(1) << 22) / p.size / TILE), pieces = (wide + most - 1) / most;
     p.columns = (wide + pieces - 1) / pieces * TILE;
@@ -954,12 +967,20 @@ hipError_t backward(const tdb_loss_args& a, hipStream_t s) {
             if (p.few) TDB_TRY(launch<loss_difference_few_kernel<DT, false>>(2 * p.blocks, 256, FEW_SHARED, s, k, g));
             if (p.many) TDB_TRY(launch<loss_difference_many_kernel<DT, false>>(p.blocks, 512, MANY_SHARED + TileArrays<Logits256<DT>, 5>::BYTES, s, k, g));
         }
-        if (a.rows && a.dx) TDB_TRY(launch<loss_dx_kernel<DT>>(p.blocks, 512, DX_SHARED, s, k, g));
-        if (a.dweight || a.dbias) TDB_TRY(launch<loss_dweight_kernel<DT>>(p.blocks, 512, Dweight<DT>::SHARED, s, k, g));
+        if (a.rows && a.dx) {
+            if (p.width == 256) TDB_TRY(launch<loss_dx_kernel<DT, 256>>(p.blocks, 512, DX_SHARED, s, k, g));
+            else if (p.width == 192) TDB_TRY(launch<loss_dx_kernel<DT, 192>>(p.blocks, 512, DX_SHARED, s, k, g));
+            else TDB_TRY(launch<loss_dx_kernel<DT, 128>>(p.blocks, 512, DX_SHARED, s, k, g));
+        }
+        if (a.dweight || a.dbias) {
+            if (p.width == 256) TDB_TRY(launch<loss_dweight_kernel<DT, 256>>(p.blocks, 512, Dweight<DT, 256>::SHARED, s, k, g));
+            else if (p.width == 192) TDB_TRY(launch<loss_dweight_kernel<DT, 192>>(p.blocks, 512, Dweight<DT, 192>::SHARED, s, k, g));
+            else TDB_TRY(launch<loss_dweight_kernel<DT, 128>>(p.blocks, 512, Dweight<DT, 128>::SHARED, s, k, g));
+        }
     }
     if (a.rows && a.dx) {
         g.columns = p.columns;              // (what the parts of dx were shared out by: the first piece's)
-        TDB_TRY(launch<loss_dx_sum_kernel<DT>>(std::min<int64_t>(a.rows, 2048), 256, 0, s, k, g, p.blocks));
+        TDB_TRY(launch<loss_dx_sum_kernel<DT>>(std::min<int64_t>(a.rows, 2048), 256, 0, s, k, g, p.blocks, int(p.width)));
     }
     return hipSuccess;
 }

@@ -113,7 +113,12 @@ struct Side {
     // Lined: 16-byte chunk c of row r lies at c ^ swap(r), so that the 16 rows that LDS serves together (0..3, 12..15, 20..27 and the others) are on distinct banks.  Turned: 64-byte block b
     // of row k lies at b ^ turn(k), so that the four rows that a read of 16 bits takes together, or every fourth of float32, are.
     static __device__ __forceinline__ int swap(int r) { return LINE == 128 ? r >> 1 & 7 : r >> 2 & 3; }
-    static __device__ __forceinline__ int turn(int k) { return (DT == TDB_F32 ? k >> 2 & 3 : (k & 3) | (k >> 1 & 4)) & (BLOCKS - 1); }
+    static __device__ __forceinline__ int turn(int k) {
+        if constexpr (DT == TDB_F32) return k >> 2 & 3;
+        else if constexpr (BLOCKS % 4) return k >> 1 & 1;       // (rows of an odd number of 128 bytes: neighbours are on distinct banks by themselves)
+        else return ((k & 3) | (k >> 1 & 4)) & (BLOCKS % 8 ? 3 : 7);
+    }
+    static_assert(!TURNED || (DT == TDB_F32 ? BLOCKS % 4 == 0 : BLOCKS % 2 == 0), "");
 
     // The same for every tile.  Columns of a turned operand past its width come from its next row, or as zeros: they are sums of their own, which nobody stores.
     __device__ __forceinline__ void place(const Rows& a) {
@@ -367,7 +372,7 @@ struct Product {
     // lies there.  to: value (m0, n0); rows and columns: how many of the tile's there are.  Whole 16-byte chunks where `wide`: STORES memory operations of every wave.
     static constexpr int COLUMNS = TN * M::SIDE, ROW = COLUMNS * int(sizeof(T)), PER = ROW / 16, SCRATCH = WAVES * 2 * M::SIDE * ROW, STORES = TM * M::SIDE * PER / 64;
     // Where byte b of a wave's row lies: 16-byte chunks exchanged so that 16 rows' chunks are on distinct banks.
-    static __device__ __forceinline__ int lies_at(int row, int b) { return row * ROW + (b ^ ((row * ROW / 256 & (PER - 1)) << 4)); }
+    static __device__ __forceinline__ int lies_at(int row, int b) { return row * ROW + (b ^ ((row * ROW / 256 & ((PER & -PER) - 1)) << 4)); }
     template <class OF, class THEN>
     static __device__ __forceinline__ void store(char* scratch, char* to, int64_t pitch, int64_t rows, int64_t columns, bool wide, OF value, THEN then) {
         constexpr int ES = sizeof(T);
