@@ -327,7 +327,9 @@ int norm_of(const tdb_grads_args& a, hipStream_t s) {
 extern "C" {
 
 int64_t tdb_grads_workspace(const tdb_grads_args* a) {
-    if (!a || a->tensors < 0 || (a->tensors && !a->numel)) return 0;
+    if (!a || a->tensors < 0 || a->tensors > (1 << 20) || (a->tensors && !a->numel)) return 0;
+    for (int i = 0; i < a->tensors; ++i)
+        if (a->numel[i] < 0 || a->numel[i] > int64_t(1) << 40) return 0;
     int64_t groups;
     tdb_train::run_of(*a, groups);
     return (tdb_train::HEAD + groups) * 8;

@@ -805,20 +805,24 @@ constexpr int64_t PARTIAL_BYTES = int64_t(1) << 27;
 
 int64_t round_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 
-// The width with the fewest columns past the end, times what a column of such tiles costs.  dx and dW of 2500 x 768, 128100 classes, in tiles of 256, 192 and 128 columns: bfloat16 926, 1044 and
-// 1269 us, float32 7.37, 7.57 and 7.70 ms; 384 wide 649, 575 and 704 us, 4.92, 3.79 and 3.86 ms.
-int tile_columns(int hidden, int dtype) {
-    int best = 256, cost = (hidden + 255) / 256 * 256 * 64;
-    const int widths[] = {192, 128}, dear[] = {dtype == TDB_F32 ? 66 : 72, dtype == TDB_F32 ? 67 : 88};
-    for (int i = 0; i < 2; ++i)
-        if (const int c = (hidden + widths[i] - 1) / widths[i] * widths[i] * dear[i]; c < cost) best = widths[i], cost = c;
+// The width of tiles of dx or dW: that of the least work of a workgroup, tiles at their price for each column.  tiles_high: of dW, whose tiles are dealt out whole; dx is split along its
+// contraction (0).  dx and dW of 2500 x 768, 128100 classes, in tiles of 256, 192 and 128 columns: bfloat16 926, 1044 and 1269 us, float32 7.37, 7.57 and 7.70 ms; 384 wide 649, 575 and
+// 704 us, 4.92, 3.79 and 3.86 ms.
+int tile_columns(int hidden, int dtype, int64_t tiles_high, int blocks) {
+    const int widths[] = {256, 192, 128}, dear[] = {64, dtype == TDB_F32 ? 66 : 72, dtype == TDB_F32 ? 67 : 88};
+    int best = 256;
+    int64_t least = INT64_MAX;
+    for (int i = 0; i < 3; ++i) {
+        const int64_t wide = (hidden + widths[i] - 1) / widths[i], rounds = tiles_high ? (tiles_high * wide + blocks - 1) / blocks : wide;
+        if (const int64_t c = rounds * widths[i] * dear[i]; c < least) best = widths[i], least = c;
+    }
     return best;
 }
 
 struct Plan {
     int size;                               // of a value
     int64_t padded, pitch, vocab;           // rows and bytes of the gathered rows, vocabulary, rounded up
-    int32_t group, width;                   // width: columns of the tiles of dx and dW
+    int32_t group, dx_width, dw_width;      // columns of the tiles of dx and dW
     bool many, few;                         // whether there may be as many or as few rows as the kernels are for
     int64_t columns;                        // of a piece
     int blocks, finish_blocks;
@@ -836,11 +840,11 @@ Plan plan_of(const tdb_loss_args& a) {
     p.vocab = round_up(a.vocab, TILE);
     const int64_t wide = p.vocab / TILE;
     p.group = int32_t((wide * p.padded * 8 + PARTIAL_BYTES - 1) / PARTIAL_BYTES);
-    p.width = tile_columns(a.hidden, a.dtype);
     p.many = a.rows > 128, p.few = a.rows > 0;
     const int64_t most = std::min<int64_t>(std::max<int64_t>(D_BYTES / (p.padded * p.size) / TILE, 1), (int64_t(1) << 22) / p.size / TILE), pieces = (wide + most - 1) / most;
     p.columns = (wide + pieces - 1) / pieces * TILE;
     p.blocks = std::max(8, tdb_compute_units(-1) & -8);
+    p.dx_width = tile_columns(a.hidden, a.dtype, 0, p.blocks), p.dw_width = tile_columns(a.hidden, a.dtype, p.columns / TILE, p.blocks);
     p.finish_blocks = int(std::min<int64_t>((std::max<int64_t>(a.rows, 1) + FINISH_ROWS - 1) / FINISH_ROWS, 256));
     int64_t at = 256;
     auto take = [&](int64_t bytes) {
@@ -868,13 +872,18 @@ Plan plan_of(const tdb_loss_args& a) {
     return p;
 }
 
-int check(const tdb_loss_args* a, bool backward) {
+int check_sizes(const tdb_loss_args* a) {
     if (!a) return tdb_fail(TDB_ERR_NULL, "args is NULL");
     if (a->dtype != TDB_F32 && a->dtype != TDB_BF16 && a->dtype != TDB_F16) return tdb_fail(TDB_ERR_DTYPE, "unknown dtype %d", a->dtype);
     if (a->bias && a->bias_dtype != a->dtype && a->bias_dtype != TDB_F32) return tdb_fail(TDB_ERR_DTYPE, "bias_dtype %d: need that of x, or float32", a->bias_dtype);
     if (a->rows < 0 || a->rows > (1 << 27) || a->vocab < 1 || a->vocab > (1 << 27) || a->hidden < 1 || a->hidden > 32768)
         return tdb_fail(TDB_ERR_SHAPE, "%lld rows, %d columns, %lld classes: need up to 2^27, 1 to 32768, 1 to 2^27", (long long)a->rows, a->hidden, (long long)a->vocab);
     if (a->reduction < 0 || a->reduction > 2) return tdb_fail(TDB_ERR_SHAPE, "reduction %d: need 0 (none), 1 (sum) or 2 (mean)", a->reduction);
+    return TDB_OK;
+}
+
+int check(const tdb_loss_args* a, bool backward) {
+    if (const int rc = check_sizes(a); rc != TDB_OK) return rc;
     const int size = a->dtype == TDB_F32 ? 4 : 2;
     if (!a->weight || !a->state || !a->workspace) return tdb_fail(TDB_ERR_NULL, "weight, state and workspace must be non-NULL");
     if (a->weight_stride * size % 16 || a->weight_stride * size < round_up(int64_t(a->hidden) * size, 16) || a->weight_stride * size > (1 << 22))
@@ -968,19 +977,19 @@ hipError_t backward(const tdb_loss_args& a, hipStream_t s) {
             if (p.many) TDB_TRY(launch<loss_difference_many_kernel<DT, false>>(p.blocks, 512, MANY_SHARED + TileArrays<Logits256<DT>, 5>::BYTES, s, k, g));
         }
         if (a.rows && a.dx) {
-            if (p.width == 256) TDB_TRY(launch<loss_dx_kernel<DT, 256>>(p.blocks, 512, DX_SHARED, s, k, g));
-            else if (p.width == 192) TDB_TRY(launch<loss_dx_kernel<DT, 192>>(p.blocks, 512, DX_SHARED, s, k, g));
+            if (p.dx_width == 256) TDB_TRY(launch<loss_dx_kernel<DT, 256>>(p.blocks, 512, DX_SHARED, s, k, g));
+            else if (p.dx_width == 192) TDB_TRY(launch<loss_dx_kernel<DT, 192>>(p.blocks, 512, DX_SHARED, s, k, g));
             else TDB_TRY(launch<loss_dx_kernel<DT, 128>>(p.blocks, 512, DX_SHARED, s, k, g));
         }
         if (a.dweight || a.dbias) {
-            if (p.width == 256) TDB_TRY(launch<loss_dweight_kernel<DT, 256>>(p.blocks, 512, Dweight<DT, 256>::SHARED, s, k, g));
-            else if (p.width == 192) TDB_TRY(launch<loss_dweight_kernel<DT, 192>>(p.blocks, 512, Dweight<DT, 192>::SHARED, s, k, g));
+            if (p.dw_width == 256) TDB_TRY(launch<loss_dweight_kernel<DT, 256>>(p.blocks, 512, Dweight<DT, 256>::SHARED, s, k, g));
+            else if (p.dw_width == 192) TDB_TRY(launch<loss_dweight_kernel<DT, 192>>(p.blocks, 512, Dweight<DT, 192>::SHARED, s, k, g));
             else TDB_TRY(launch<loss_dweight_kernel<DT, 128>>(p.blocks, 512, Dweight<DT, 128>::SHARED, s, k, g));
         }
     }
     if (a.rows && a.dx) {
         g.columns = p.columns;              // (what the parts of dx were shared out by: the first piece's)
-        TDB_TRY(launch<loss_dx_sum_kernel<DT>>(std::min<int64_t>(a.rows, 2048), 256, 0, s, k, g, p.blocks, int(p.width)));
+        TDB_TRY(launch<loss_dx_sum_kernel<DT>>(std::min<int64_t>(a.rows, 2048), 256, 0, s, k, g, p.blocks, int(p.dx_width)));
     }
     return hipSuccess;
 }
@@ -1000,9 +1009,9 @@ extern "C" {
 
 int tdb_loss_fwd(const tdb_loss_args* args, void* stream) { return tdb_train::run(args, false, stream); }
 int tdb_loss_bwd(const tdb_loss_args* args, void* stream) { return tdb_train::run(args, true, stream); }
-int64_t tdb_loss_state(const tdb_loss_args* args) { return args ? tdb_train::plan_of(*args).state : 0; }
+int64_t tdb_loss_state(const tdb_loss_args* args) { return tdb_train::check_sizes(args) == TDB_OK ? tdb_train::plan_of(*args).state : 0; }
 int64_t tdb_loss_workspace(const tdb_loss_args* args, int32_t backward) {
-    if (!args) return 0;
+    if (tdb_train::check_sizes(args) != TDB_OK) return 0;
     const tdb_train::Plan p = tdb_train::plan_of(*args);
     return backward ? p.backward : p.forward;
 }

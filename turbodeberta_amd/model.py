@@ -62,7 +62,7 @@ from .ops.flash_attention_varlen import flash_attention_with_disentangled_varlen
 from .ops.trainable_attention import trainable_attention_with_disentangled
 from .padding import index_first_axis, key_padding_mask, pad_input
 from . import training as _training
-from .training import FlashDebertaV2Output, FlashDebertaV2SelfOutput, FlashDropout, FlashLayerNorm
+from .training import FlashDebertaV2Output, FlashDebertaV2SelfOutput, FlashDropout, FlashLayerNorm, MaskedLMLoss
 
 
 def _versions(*tensors):
@@ -649,7 +649,7 @@ class _FusedHead:
         patch_model(self)
 
 
-class FlashDebertaV2ForMaskedLM(_FusedHead, DebertaV2ForMaskedLM):
+class FlashDebertaV2ForMaskedLM(MaskedLMLoss, _FusedHead, DebertaV2ForMaskedLM):
     pass
 
 
@@ -669,13 +669,16 @@ class FlashDebertaV2ForMultipleChoice(_FusedHead, DebertaV2ForMultipleChoice):
     pass
 
 
-def patch_model(model: nn.Module, training: bool = False) -> nn.Module:
+def patch_model(model: nn.Module, training: bool = False, fused_loss: bool = False) -> nn.Module:
     """Switch every ``DisentangledSelfAttention`` inside ``model`` (any DeBERTa-v2/v3 model or task head,
     e.g. one loaded with ``from_pretrained``) to the fused kernel, in place.  Parameters are untouched.
 
     ``training=True``: the model can be trained as well.  Attention, LayerNorms and dropouts of the DeBERTa modules run the training operators
     (``turbodeberta_amd.training``) in training mode and wherever autograd records; evaluation under ``torch.no_grad`` is not changed by it.  Head dimensions: multiples of 8
-    up to 64; no ``pos_att_type`` where ``relative_attention`` is off.  Masks come from PyTorch's generator but are not those that ``nn.Dropout`` would draw."""
+    up to 64; no ``pos_att_type`` where ``relative_attention`` is off.  Masks come from PyTorch's generator but are not those that ``nn.Dropout`` would draw.
+
+    ``fused_loss=True``: a masked language model that is called with labels, in training mode or where autograd records, computes its loss without the logits
+    (``turbodeberta_amd.training.MaskedLMLoss``): ``loss`` is float32, ``logits`` is None then."""
     swaps = {DisentangledSelfAttention: FlashDisentangledSelfAttention, DebertaV2Encoder: FlashDebertaV2Encoder,
              DebertaV2Model: FlashDebertaV2Model}        # none of them adds parameters or constructor state
     if training:
@@ -686,6 +689,12 @@ def patch_model(model: nn.Module, training: bool = False) -> nn.Module:
                 raise ValueError(f"head dimension {module.attention_head_size}: training needs a multiple of 8 up to 64")
             if module.pos_att_type and not module.relative_attention:        # Hugging Face counts them in the scale all the same (modeling_deberta_v2.py:237-243)
                 raise ValueError("pos_att_type names position terms and relative_attention is off: training needs one without the other")
+    if fused_loss:
+        heads = [module for module in model.modules() if type(module) in (DebertaV2ForMaskedLM, FlashDebertaV2ForMaskedLM)]
+        if not heads:
+            raise ValueError("fused_loss: there is no DebertaV2ForMaskedLM in the model")
+        for module in heads:
+            module.__class__, module.fused_loss = FlashDebertaV2ForMaskedLM, True
     inner = set()                       # of the DeBERTa modules: a task head's own dropout and norm stay as they are
     for module in model.modules():
         if type(module) in swaps:
