@@ -6,6 +6,7 @@
 // same bits every time, no overflow.
 #include <algorithm>
 #include <cmath>
+#include <new>
 #include <vector>
 
 #include "tdb_error.h"
@@ -342,7 +343,7 @@ int tdb_grads_norm(const tdb_grads_args* a, void* stream) {
     return a->norm == 0 ? norm_of<0>(*a, s) : a->norm == 1 ? norm_of<1>(*a, s) : norm_of<2>(*a, s);
 }
 
-int tdb_grads_clip(const tdb_grads_args* a, void* stream) {
+int tdb_grads_clip(const tdb_grads_args* a, void* stream) try {
     using namespace tdb_train;
     if (const int rc = check_grads(a, true); rc != TDB_OK) return rc;
     ClipTable t;
@@ -350,6 +351,8 @@ int tdb_grads_clip(const tdb_grads_args* a, void* stream) {
     in_tables<ClipTable, CLIP_TENSORS>(*a, t, [&](int i, int k) { t.from[k] = a->from[i], t.to[k] = a->to[i], t.kind[k] = uint16_t(a->to_dtype[i] * 4 + a->from_dtype[i]); },
                                        [&](int groups) { grads_scale_kernel<<<groups, 256, 0, static_cast<hipStream_t>(stream)>>>(t); });
     return launched();
+} catch (const std::bad_alloc&) {      // (of the list that overlaps are looked for in)
+    return tdb_fail(TDB_ERR_LAUNCH, "out of host memory");
 }
 
 }  // extern "C"

@@ -363,8 +363,7 @@ __global__ __launch_bounds__(256, 2) void loss_logits_few_kernel(Loss p) {
 template <int DT>
 __global__ __launch_bounds__(1024) void loss_finish_kernel(Loss p) {
     __shared__ float s_top[32][33], s_sum[32][33];
-    __shared__ double s_all[1024];
-    __shared__ bool s_last;
+    __shared__ double s_all[32];
     const int n = p.count[0], l = threadIdx.x & 31, w = threadIdx.x >> 5;
     const Partials parts(p, tile_rows<DT>(n, 32) == 256);
     const int groups = int(parts.groups);
@@ -408,28 +407,30 @@ __global__ __launch_bounds__(1024) void loss_finish_kernel(Loss p) {
         }
     }
     if (p.reduction == 0) return;
-    auto total = [&](double x) {
-        __syncthreads();
-        s_all[threadIdx.x] = x;
-        for (int d = 512; d > 0; d >>= 1) {
-            __syncthreads();
-            if (threadIdx.x < d) s_all[threadIdx.x] += s_all[threadIdx.x + d];
-        }
-    };
-    total(mine);
     // (only workgroups that have rows, or the first one, take part)
-    const int parts_done = max(1, min(int(gridDim.x), (n + FINISH_ROWS - 1) / FINISH_ROWS));
-    if (int(blockIdx.x) >= parts_done) return;
-    if (threadIdx.x == 0) {
-        __hip_atomic_store(p.block_sums + blockIdx.x, s_all[0], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        s_last = __hip_atomic_fetch_add(p.count + 1, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == parts_done - 1;
-    }
+    const int taking_part = max(1, min(int(gridDim.x), (n + FINISH_ROWS - 1) / FINISH_ROWS));
+    if (int(blockIdx.x) >= taking_part) return;
+    if (l == 0) s_all[w] = mine;
     __syncthreads();
-    if (!s_last) return;
-    double sum = 0.0;
-    for (int i = threadIdx.x; i < parts_done; i += 1024) sum += __hip_atomic_load(p.block_sums + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    total(sum);
-    if (threadIdx.x == 0) p.loss[0] = float(p.reduction == 2 ? s_all[0] / double(n) : s_all[0]);
+    if (threadIdx.x >= 64) return;
+    double sum = threadIdx.x < 32 ? s_all[threadIdx.x] : 0.0;
+    auto over_wave = [](double x) {
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) x += __shfl_xor(x, d);
+        return x;
+    };
+    sum = over_wave(sum);
+    bool last = false;
+    if (threadIdx.x == 0) {
+        __hip_atomic_store(p.block_sums + blockIdx.x, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        last = __hip_atomic_fetch_add(p.count + 1, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == taking_part - 1;
+    }
+    if (!__builtin_amdgcn_readfirstlane(int(last))) return;
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+    sum = 0.0;
+    for (int i = threadIdx.x; i < taking_part; i += 64) sum += __hip_atomic_load(p.block_sums + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    sum = over_wave(sum);
+    if (threadIdx.x == 0) p.loss[0] = float(p.reduction == 2 ? sum / double(n) : sum);
 }
 
 // What the gradient needs beside Loss.
@@ -663,7 +664,7 @@ __global__ __launch_bounds__(512, 2) void loss_dx_kernel(Loss p, Gradient g) {
 // What the gradient of a sum or mean makes of every row.
 __device__ __forceinline__ float row_factor(const Loss& p, const Gradient& g, int n) { return p.reduction == 2 ? g.dloss[0] / float(n) : g.dloss[0]; }
 
-// dx, zeros where a row does not count.  Where few rows are split over many parts a workgroup has a row and its waves share out the parts, otherwise each wave has a row.
+// dx, zeros where a row does not count.  Where few rows are split over many parts a workgroup has 256 columns of a row and its waves share out the parts, otherwise each wave has a row.
 // blocks, width: workgroups of the launch before and its tiles' columns.
 template <int DT>
 __global__ __launch_bounds__(256) void loss_dx_sum_kernel(Loss p, Gradient g, int blocks, int width) {
@@ -677,12 +678,12 @@ __global__ __launch_bounds__(256) void loss_dx_sum_kernel(Loss p, Gradient g, in
     auto sum_of = [&](int place, int64_t c, int64_t first, int64_t step) {
         const float* const from = g.parts + place * g.part_pitch + min(c, g.part_pitch - 4);
         f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-        for (int64_t s = first; s < share.splits; s += 4 * step) {
-            f32x4 x[4];
+        for (int64_t s = first; s < share.splits; s += 8 * step) {
+            f32x4 x[8];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) x[u] = *reinterpret_cast<const f32x4*>(from + min(s + u * step, share.splits - 1) * apart);
+            for (int u = 0; u < 8; ++u) x[u] = *reinterpret_cast<const f32x4*>(from + min(s + u * step, share.splits - 1) * apart);
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
+            for (int u = 0; u < 8; ++u)
                 if (s + u * step < share.splits) sum += x[u];
         }
         return sum;
@@ -708,22 +709,20 @@ __global__ __launch_bounds__(256) void loss_dx_sum_kernel(Loss p, Gradient g, in
         }
         return;
     }
-    for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
-        const int place = p.place[row];
+    const int chunks = (p.hidden + 255) / 256;
+    for (int64_t item = blockIdx.x; item < p.rows * chunks; item += gridDim.x) {
+        const int64_t row = item / chunks;
+        const int c0 = int(item - row * chunks) * 256, at = c0 + threadIdx.x, place = p.place[row];
         T* const to = static_cast<T*>(g.dx) + row * g.dx_stride;
         if (place < 0) {
-            for (int c = threadIdx.x; c < p.hidden; c += 256) to[c] = T(0.f);
+            if (at < p.hidden) to[at] = T(0.f);
             continue;
         }
-        const float factor = factor_of(place);
-        for (int c0 = 0; c0 < p.hidden; c0 += 256) {
-            const f32x4 sum = sum_of(place, c0 + 4 * l, w, 4);
-            __syncthreads();
-            *reinterpret_cast<f32x4*>(&s_sum[w][4 * l]) = sum;
-            __syncthreads();
-            const int at = c0 + threadIdx.x;
-            if (at < p.hidden) to[at] = T((((s_sum[0][threadIdx.x] + s_sum[1][threadIdx.x]) + s_sum[2][threadIdx.x]) + s_sum[3][threadIdx.x]) * factor);
-        }
+        const f32x4 sum = sum_of(place, c0 + 4 * l, w, 4);
+        __syncthreads();
+        *reinterpret_cast<f32x4*>(&s_sum[w][4 * l]) = sum;
+        __syncthreads();
+        if (at < p.hidden) to[at] = T((((s_sum[0][threadIdx.x] + s_sum[1][threadIdx.x]) + s_sum[2][threadIdx.x]) + s_sum[3][threadIdx.x]) * factor_of(place));
     }
 }
 
@@ -772,29 +771,38 @@ __global__ __launch_bounds__(512, 2) void loss_dweight_kernel(Loss p, Gradient g
     typename P::Flow flow(smem, a, b);
     const int heights = n ? (n + tile_rows<DT>(n, 32) - 1) / tile_rows<DT>(n, 32) : 0;
     const float factor = n == 0 ? 0.f : (p.reduction ? row_factor(p, g, n) : *g.common) * (1.f / D_SCALE<DT>);
-    // (Tiles by themselves: with the next one's first step asked for ahead, as the logits have it, 8192 rows took 2650 to 2830 us instead of 1890.)
-    for (int64_t block = blockIdx.x; block < all; block += gridDim.x) {
+    auto tile = [&](int64_t block) {
         int64_t row, column, split;
-        tile_of(block, row_tiles, column_tiles, 1, row, column, split);
-        const int64_t m0 = row * BM, n0 = column * BN, m = m0 + threadIdx.x;
-        if (g.dbias && column == 0 && threadIdx.x < BM && m < columns) {
+        tile_of(block < all ? block : 0, row_tiles, column_tiles, 1, row, column, split);
+        return typename P::Tile{row * BM, column * BN, 0, steps};
+    };
+    if (blockIdx.x >= all) return;
+    typename P::Tile now = tile(blockIdx.x);
+    typename P::Alone alone;
+    if (g.dweight) P::open(flow, now, alone);
+    int stage = 0;
+    for (int64_t block = blockIdx.x; block < all; block += gridDim.x) {
+        const typename P::Tile next = tile(block + gridDim.x);
+        if (const int64_t m = now.m0 + threadIdx.x; g.dbias && now.n0 == 0 && threadIdx.x < BM && m < columns) {
             float sum = 0.f;
             for (int t = 0; t < heights; ++t) sum += g.column_sums[t * g.columns + m];
             if (p.bias_kind == 2) static_cast<float*>(g.dbias)[g.first + m] = sum * factor;
             else static_cast<T*>(g.dbias)[g.first + m] = T(sum * factor);
         }
-        if (!g.dweight) continue;
-        typename P::Acc acc;
-        P::run(flow, {m0, n0, 0, steps}, acc, P::ZEROS);
-        P::store(
-            smem, g.dweight + (g.first + m0) * g.dweight_pitch + n0 * int64_t(sizeof(T)), g.dweight_pitch, columns - m0, p.hidden - n0, g.wide_dweight,
-            [&](int i, int j, int q) {
-                f32x4 v = P::quad(acc, i, j, q);
+        if (g.dweight) {
+            typename P::Acc acc;
+            P::template run_on<P::STORES>(flow, now, next, block + gridDim.x < all, stage, !g.wide_dweight || block == blockIdx.x, acc, P::ZEROS, alone);
+            P::store(
+                P::scratch(smem, stage), g.dweight + (g.first + now.m0) * g.dweight_pitch + now.n0 * int64_t(sizeof(T)), g.dweight_pitch, columns - now.m0, p.hidden - now.n0, g.wide_dweight,
+                [&](int i, int j, int q) {
+                    f32x4 v = P::quad(acc, i, j, q);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] *= factor;
-                return v;
-            },
-            [](int, char*) {});
+                    for (int e = 0; e < 4; ++e) v[e] *= factor;
+                    return v;
+                },
+                [](int, char*) {});
+        }
+        now = next;
     }
 }
 
@@ -989,7 +997,7 @@ hipError_t backward(const tdb_loss_args& a, hipStream_t s) {
     }
     if (a.rows && a.dx) {
         g.columns = p.columns;              // (what the parts of dx were shared out by: the first piece's)
-        TDB_TRY(launch<loss_dx_sum_kernel<DT>>(std::min<int64_t>(a.rows, 2048), 256, 0, s, k, g, p.blocks, int(p.dx_width)));
+        TDB_TRY(launch<loss_dx_sum_kernel<DT>>(std::min<int64_t>(a.rows * ((a.hidden + 255) / 256), 2048), 256, 0, s, k, g, p.blocks, int(p.dx_width)));
     }
     return hipSuccess;
 }

@@ -291,8 +291,8 @@ struct Product {
     static __device__ __forceinline__ void run_on(Flow& flow, const Tile& t, const Tile& next, bool more, int& stage, bool first, Acc& acc, START start, BESIDE& beside) {
         const int steps = int(t.end - t.begin);
         auto go_on = [&]() {
-            if (more) flow.seek(next), beside.load(next);
-            else flow.nothing();
+            flow.seek(next), beside.load(next);
+            flow.at_a.left = more ? flow.at_a.left : 0, flow.at_b.left = more ? flow.at_b.left : 0;
         };
         if (LATER == 0 || first) wait_loads<0>();
         else wait_loads<LATER>();
@@ -370,7 +370,9 @@ struct Product {
 
     // The tile's values to rows of memory by way of LDS (SCRATCH bytes), SIDE rows at a time: value(i, j, q) gives four neighbours, then(i, the wave's rows in LDS) may change what
     // lies there.  to: value (m0, n0); rows and columns: how many of the tile's there are.  Whole 16-byte chunks where `wide`: STORES memory operations of every wave.
-    static constexpr int COLUMNS = TN * M::SIDE, ROW = COLUMNS * int(sizeof(T)), PER = ROW / 16, SCRATCH = WAVES * 2 * M::SIDE * ROW, STORES = TM * M::SIDE * PER / 64;
+    static constexpr int COLUMNS = TN * M::SIDE, ROW = COLUMNS * int(sizeof(T)), PER = ROW / 16, STORES = TM * M::SIDE * PER / 64;
+    static constexpr int SETS = WAVES * 2 * M::SIDE * ROW <= STAGE ? 2 : 1, SCRATCH = WAVES * SETS * M::SIDE * ROW;       // (two where a stage holds them)
+    static_assert(SCRATCH <= (NS == 2 ? STAGE : SHARED), "");
     // Where byte b of a wave's row lies: 16-byte chunks exchanged so that 16 rows' chunks are on distinct banks.
     static __device__ __forceinline__ int lies_at(int row, int b) { return row * ROW + (b ^ ((row * ROW / 256 & ((PER & -PER) - 1)) << 4)); }
     template <class OF, class THEN>
@@ -378,11 +380,11 @@ struct Product {
         constexpr int ES = sizeof(T);
         typedef __attribute__((ext_vector_type(4))) T T4;
         const int l = threadIdx.x & 63;
-        char* const own = scratch + uniform(threadIdx.x >> 6) * (2 * M::SIDE * ROW);
+        char* const own = scratch + uniform(threadIdx.x >> 6) * (SETS * M::SIDE * ROW);
         to += wave_m() * pitch + wave_n() * ES, rows -= wave_m(), columns -= wave_n();
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
-            char* const mine = own + (i & 1) * (M::SIDE * ROW);
+            char* const mine = own + i % SETS * (M::SIDE * ROW);
 #pragma unroll
             for (int j = 0; j < TN; ++j)
 #pragma unroll
@@ -406,6 +408,10 @@ struct Product {
                     const int row = at / COLUMNS, c = at % COLUMNS;
                     if (i * M::SIDE + row < rows && c < columns) *reinterpret_cast<T*>(to + (i * M::SIDE + row) * pitch + c * ES) = *reinterpret_cast<const T*>(mine + lies_at(row, c * ES));
                 }
+            }
+            if constexpr (SETS == 1) {
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
             }
         }
     }
