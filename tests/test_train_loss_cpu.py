@@ -21,8 +21,8 @@ def _loss(**kw):
 @pytest.mark.parametrize("kw,err", [
     (dict(dtype=7), "TDB_ERR_DTYPE"), (dict(bias_dtype=_lib.TDB_F16), "TDB_ERR_DTYPE"), (dict(hidden=0), "TDB_ERR_SHAPE"), (dict(hidden=32769), "TDB_ERR_SHAPE"), (dict(rows=-1), "TDB_ERR_SHAPE"),
     (dict(rows=(1 << 27) + 1), "TDB_ERR_SHAPE"), (dict(vocab=0), "TDB_ERR_SHAPE"), (dict(vocab=(1 << 27) + 1), "TDB_ERR_SHAPE"), (dict(reduction=3), "TDB_ERR_SHAPE"), (dict(reduction=-1), "TDB_ERR_SHAPE"),
-    (dict(weight=None), "TDB_ERR_NULL"), (dict(state=None), "TDB_ERR_NULL"), (dict(workspace=None), "TDB_ERR_NULL"), (dict(weight=4104), "TDB_ERR_ALIGN"), (dict(state=4104), "TDB_ERR_ALIGN"),
-    (dict(workspace=4097), "TDB_ERR_ALIGN"), (dict(weight_stride=60), "TDB_ERR_STRIDE"), (dict(weight_stride=68), "TDB_ERR_STRIDE"), (dict(weight_stride=-64), "TDB_ERR_STRIDE"),
+    (dict(weight=None), "TDB_ERR_NULL"), (dict(state=None), "TDB_ERR_NULL"), (dict(workspace=None), "TDB_ERR_NULL"), (dict(weight=4098), "TDB_ERR_ALIGN"), (dict(state=4104), "TDB_ERR_ALIGN"),
+    (dict(workspace=4097), "TDB_ERR_ALIGN"), (dict(weight_stride=60), "TDB_ERR_STRIDE"), (dict(weight_stride=67), "TDB_ERR_STRIDE"), (dict(weight_stride=-64), "TDB_ERR_STRIDE"),
     (dict(weight_stride=(1 << 21) + 8), "TDB_ERR_STRIDE"), (dict(hidden=65), "TDB_ERR_STRIDE"), (dict(state_bytes=100), "TDB_ERR_SHAPE"), (dict(workspace_bytes=100), "TDB_ERR_SHAPE"),
 ])
 def test_refusals_of_both_directions(kw, err):

@@ -205,6 +205,27 @@ def test_layouts(hidden, dtype):
     assert torch.equal(loss, again)
 
 
+# few rows and many; rows that end 0, 2, 4 ... bytes into 16, one step and several
+@pytest.mark.parametrize("rows", [20, 600])
+@pytest.mark.parametrize("hidden", [8, 21, 66, 127, 130, 301])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_weights_among_other_values(dtype, hidden, rows):
+    """Rows at multiples of 4 bytes inside a wider matrix whose other values are NaN, and inside one whose rows are at odd places."""
+    x, w, labels, b = _inputs(rows, hidden, 700, dtype)
+    want = _check(x, w, labels, b)
+    for pad in (3, 4):
+        wide = torch.full((702, hidden + pad + (hidden + pad) % 2), torch.nan, dtype=dtype, device="cuda")
+        view = wide[1:701, 2:2 + hidden]
+        view.copy_(w)
+        got = _check(x, view, labels, b)
+        assert torch.equal(got[0], want[0]) and all(torch.equal(want[1][k], got[1][k]) for k in want[1])
+    wide = torch.full((700, hidden + 1 + hidden % 2), torch.nan, dtype=dtype, device="cuda")
+    view = wide[:, 1:1 + hidden]
+    view.copy_(w)
+    got = _check(x, view, labels, b)
+    assert torch.equal(got[0], want[0]) and all(torch.equal(want[1][k], got[1][k]) for k in want[1])
+
+
 def test_only_some_gradients():
     x, w, labels, b = _inputs(90, 96, 500, torch.bfloat16, 0.8)
     _, full = _step(x, w, labels, b, "mean")

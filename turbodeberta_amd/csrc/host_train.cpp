@@ -530,7 +530,8 @@ PyObject* py_loss(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         }
         const Tensor weight = take(args[1], &x, ok), labels = take(args[2], &x, ok), bias = take(args[3], &x, ok);
         if (!ok || !weight.defined() || !labels.defined() || weight.dim() != 2 || weight.size(0) < 2 || weight.size(1) != x.size(-1) || weight.scalar_type() != x.scalar_type() ||
-            weight.stride(0) < weight.size(1) || !tdb_host_rows_ok(weight) || weight.size(1) * weight.element_size() % 16)
+            weight.stride(0) < weight.size(1) || weight.stride(0) * weight.element_size() % 4 || weight.stride(0) * weight.element_size() > 1 << 22 || (weight.size(1) > 1 && weight.stride(1) != 1) ||
+            reinterpret_cast<uintptr_t>(weight.data_ptr()) % 4)
             return Tensor();
         if (labels.scalar_type() != at::kLong || labels.sizes() != x.sizes().slice(0, x.dim() - 1) || !labels.is_contiguous()) return Tensor();
         if (bias.defined() && (bias.dim() != 1 || bias.size(0) != weight.size(0) || !bias.is_contiguous() || (bias.scalar_type() != x.scalar_type() && bias.scalar_type() != at::kFloat)))

@@ -58,13 +58,13 @@ struct Loss {
     float *maxima, *sums;                       // [groups of column tiles][rows]
     double* block_sums;
     int64_t padded;                             // rows, rounded up
-    int32_t group;                              // column tiles that a workgroup of the kernel for many rows takes together
+    int32_t group, few_width;                   // column tiles that a workgroup of the kernel for many rows takes together; columns of the tiles of the one for few
 };
 
 // How the logits' maxima and sums lie: groups of column tiles, rows `pitch` to each.
 struct Partials {
     int64_t groups, tiles, group, pitch;
-    __device__ __forceinline__ Partials(const Loss& p, bool many) : tiles((p.vocab + 255) / 256), group(many ? p.group : 1), pitch(many ? p.padded : min(p.padded, int64_t(FEW))) {
+    __device__ __forceinline__ Partials(const Loss& p, bool many) : tiles(many ? (p.vocab + TILE - 1) / TILE : (p.vocab + p.few_width - 1) / p.few_width), group(many ? p.group : 1), pitch(many ? p.padded : min(p.padded, int64_t(FEW))) {
         groups = (tiles + group - 1) / group;
     }
 };
@@ -175,7 +175,7 @@ __global__ __launch_bounds__(64 * GATHER_WAVES) void loss_gather_kernel(Loss p, 
 template <int DT>
 __device__ __forceinline__ Rows hidden_rows(const Loss& p, int n) { return {p.gathered, p.pitch, n, uint32_t(p.pitch)}; }
 template <int DT>
-__device__ __forceinline__ Rows weight_rows(const Loss& p) { return {p.w, p.w_pitch, p.vocab, uint32_t((p.hidden * sizeof(typename Matrix<DT>::T) + 15) / 16 * 16)}; }
+__device__ __forceinline__ Rows weight_rows(const Loss& p) { return {p.w, p.w_pitch, p.vocab, uint32_t(p.hidden * sizeof(typename Matrix<DT>::T))}; }
 
 // A tile's logits: the sums start from the biases.
 template <int DT, class P>
@@ -287,18 +287,24 @@ struct TileArrays {
     __device__ __forceinline__ const char* of(int k) const { return smem + (set * ARRAYS + k) * 1024; }
 };
 
-// Many rows: a workgroup of eight waves to a CU.  Few: two of four waves, tiles of as many rows as there are.  (Two kernels, of which one ends at once: with all heights in one the compiler kept
-// some 100 scalar and a few vector registers in memory, and 8192 rows took 2520 us instead of LOGITS_MANY.)  The next tile's first step is on its way while a tile's exponentials are made.
+// Many rows: a workgroup of eight waves to a CU.  Few: tiles of as many rows as there are.  (Two kernels, of which one ends at once: with all heights in one the compiler kept
+// some 100 scalar and a few vector registers in memory, and 8192 rows took 2520 us instead of 2120.)  The next tile's first step is on its way while a tile's exponentials are made.
 template <int DT>
 using Logits256 = Product<DT, 256, 256, 2, 4, 2, false, false>;
-template <int DT>
-using Logits128 = Product<DT, 128, 256, 1, 4, 3, false, false, 64>;
-template <int DT>
-using Logits64 = Product<DT, 64, 256, 1, 4, 3, false, false, 64>;
-template <int DT>
-using Logits32 = Product<DT, 32, 256, 1, 4, 2, false, false, 128>;
-constexpr int MANY_SHARED = Logits256<TDB_BF16>::SHARED,  FEW_SHARED = Logits128<TDB_BF16>::SHARED;
-static_assert(Logits64<TDB_BF16>::SHARED <= FEW_SHARED && Logits32<TDB_BF16>::SHARED <= FEW_SHARED, "");
+constexpr int MANY_SHARED = Logits256<TDB_BF16>::SHARED;
+// Few rows: eight waves to a CU in 16 bits, steps as deep as LDS holds; of float32, which has the more to multiply, twice four, as of tiles of 128 columns.  (31 rows, 91214 classes, 1024 columns
+// of float32: 156 + 119 us with eight waves, 139 + 103 with twice four; 55, 128100, 1024 of float16: 76 + 49 and 81 + 51.)
+template <int DT, int BN>
+struct Few {
+    static constexpr bool DEEP = DT != TDB_F32 && BN == 256;
+    static constexpr int THREADS = DEEP ? 512 : 256, WM = DEEP ? 2 : 1, LINE = DEEP ? 128 : 64;
+    using Logits128 = Product<DT, 128, BN, WM, 4, 3, false, false, LINE>;
+    using Logits64 = Product<DT, 64, BN, WM, 4, 3, false, false, LINE>;
+    using Logits32 = Product<DT, 32, BN, 1, THREADS / 64, DEEP || BN == 128 ? 4 : 2, false, false>;
+    static constexpr int SHARED = Logits128::SHARED > Logits32::SHARED ? Logits128::SHARED : Logits32::SHARED;
+    static constexpr int PER_CU = DEEP ? 1 : 2;
+    static_assert(Logits64::SHARED <= SHARED, "");
+};
 
 template <int DT>
 __global__ __launch_bounds__(512, 2) void loss_logits_many_kernel(Loss p) {
@@ -345,17 +351,18 @@ __global__ __launch_bounds__(512, 2) void loss_logits_many_kernel(Loss p) {
         row = next_row, g = next_g, t = next_t, now = next;
     }
 }
-template <int DT>
-__global__ __launch_bounds__(256, 2) void loss_logits_few_kernel(Loss p) {
+template <int DT, int BN>
+__global__ __launch_bounds__((Few<DT, BN>::THREADS), 2) void loss_logits_few_kernel(Loss p) {
+    using F = Few<DT, BN>;
     extern __shared__ __attribute__((aligned(1024))) char smem[];
-    __shared__ __attribute__((aligned(16))) float s_bias[256];
+    __shared__ __attribute__((aligned(16))) float s_bias[BN];
     __shared__ int32_t s_label[128];
     __shared__ float s_top[512], s_sum[512];
     const int n = p.count[0];
     switch (tile_rows<DT>(n, 32)) {
-        case 32: return logits_body<DT, Logits32<DT>>(p, n, smem, s_bias, s_label, s_top, s_sum);
-        case 64: return logits_body<DT, Logits64<DT>>(p, n, smem, s_bias, s_label, s_top, s_sum);
-        case 128: return logits_body<DT, Logits128<DT>>(p, n, smem, s_bias, s_label, s_top, s_sum);
+        case 32: return logits_body<DT, typename F::Logits32>(p, n, smem, s_bias, s_label, s_top, s_sum);
+        case 64: return logits_body<DT, typename F::Logits64>(p, n, smem, s_bias, s_label, s_top, s_sum);
+        case 128: return logits_body<DT, typename F::Logits128>(p, n, smem, s_bias, s_label, s_top, s_sum);
     }
 }
 
@@ -578,16 +585,17 @@ __global__ __launch_bounds__(512, 2) void loss_difference_many_kernel(Loss p, Gr
         row = next_row, now = next;
     }
 }
-template <int DT, bool WEIGHTED>
-__global__ __launch_bounds__(256, 2) void loss_difference_few_kernel(Loss p, Gradient g) {
+template <int DT, bool WEIGHTED, int BN>
+__global__ __launch_bounds__((Few<DT, BN>::THREADS), 2) void loss_difference_few_kernel(Loss p, Gradient g) {
+    using F = Few<DT, BN>;
     extern __shared__ __attribute__((aligned(1024))) char smem[];
-    __shared__ __attribute__((aligned(16))) float s_bias[256];
-    __shared__ float s_column[256], s_rows[6][128];
+    __shared__ __attribute__((aligned(16))) float s_bias[BN];
+    __shared__ float s_column[2 * BN], s_rows[6][128];
     const int n = p.count[0];
     switch (tile_rows<DT>(n, 32)) {
-        case 32: return difference_body<DT, Logits32<DT>, WEIGHTED>(p, g, n, smem, s_bias, s_rows, s_column);
-        case 64: return difference_body<DT, Logits64<DT>, WEIGHTED>(p, g, n, smem, s_bias, s_rows, s_column);
-        case 128: return difference_body<DT, Logits128<DT>, WEIGHTED>(p, g, n, smem, s_bias, s_rows, s_column);
+        case 32: return difference_body<DT, typename F::Logits32, WEIGHTED>(p, g, n, smem, s_bias, s_rows, s_column);
+        case 64: return difference_body<DT, typename F::Logits64, WEIGHTED>(p, g, n, smem, s_bias, s_rows, s_column);
+        case 128: return difference_body<DT, typename F::Logits128, WEIGHTED>(p, g, n, smem, s_bias, s_rows, s_column);
     }
 }
 
@@ -830,7 +838,7 @@ int tile_columns(int hidden, int dtype, int64_t tiles_high, int blocks) {
 struct Plan {
     int size;                               // of a value
     int64_t padded, pitch, vocab;           // rows and bytes of the gathered rows, vocabulary, rounded up
-    int32_t group, dx_width, dw_width;      // columns of the tiles of dx and dW
+    int32_t group, few_width, dx_width, dw_width;       // columns of the tiles of few rows' logits, dx and dW
     bool many, few;                         // whether there may be as many or as few rows as the kernels are for
     int64_t columns;                        // of a piece
     int blocks, finish_blocks;
@@ -852,6 +860,10 @@ Plan plan_of(const tdb_loss_args& a) {
     const int64_t most = std::min<int64_t>(std::max<int64_t>(D_BYTES / (p.padded * p.size) / TILE, 1), (int64_t(1) << 22) / p.size / TILE), pieces = (wide + most - 1) / most;
     p.columns = (wide + pieces - 1) / pieces * TILE;
     p.blocks = std::max(8, tdb_compute_units(-1) & -8);
+    // Tiles of 128 columns where there are fewer of 256 than CUs to read the weights.  The two passes over them in tiles of 256 and 128 columns: one row, 32510 classes, 768 columns of float32
+    // 37 + 39 and 27 + 29 us; 3 rows, 3858 classes, 1024 columns of float16 14 + 15 and 11 + 12; 17, 36468, 416 of bfloat16 11 + 11 and 13 + 14; 269, 7913, 768 of float32, which multiplies
+    // for most of its time, 64 + 65 and 70 + 71.
+    p.few_width = a.rows <= 128 && wide * (p.size == 4 ? 1 : 2) < p.blocks ? 128 : 256;
     p.dx_width = tile_columns(a.hidden, a.dtype, 0, p.blocks), p.dw_width = tile_columns(a.hidden, a.dtype, p.columns / TILE, p.blocks);
     p.finish_blocks = int(std::min<int64_t>((std::max<int64_t>(a.rows, 1) + FINISH_ROWS - 1) / FINISH_ROWS, 256));
     int64_t at = 256;
@@ -864,7 +876,7 @@ Plan plan_of(const tdb_loss_args& a) {
     p.gathered = take(p.padded * p.pitch);
     p.state = at;
     at = 0;
-    const int64_t partials = std::max((wide + p.group - 1) / p.group * p.padded, wide * std::min<int64_t>(p.padded, FEW)) * 4;
+    const int64_t partials = std::max((wide + p.group - 1) / p.group * p.padded, p.vocab / p.few_width * std::min<int64_t>(p.padded, FEW)) * 4;
     p.maxima = take(partials), p.sums = take(partials), p.block_sums = take(p.finish_blocks * 8);
     p.forward = at;
     at = 0;
@@ -894,10 +906,11 @@ int check(const tdb_loss_args* a, bool backward) {
     if (const int rc = check_sizes(a); rc != TDB_OK) return rc;
     const int size = a->dtype == TDB_F32 ? 4 : 2;
     if (!a->weight || !a->state || !a->workspace) return tdb_fail(TDB_ERR_NULL, "weight, state and workspace must be non-NULL");
-    if (a->weight_stride * size % 16 || a->weight_stride * size < round_up(int64_t(a->hidden) * size, 16) || a->weight_stride * size > (1 << 22))
-        return tdb_fail(TDB_ERR_STRIDE, "weight_stride %lld: need whole 16 bytes, at least a row and at most 4 MiB", (long long)a->weight_stride);
-    for (const void* t : {a->weight, static_cast<const void*>(a->state), static_cast<const void*>(a->workspace)})
-        if (reinterpret_cast<uintptr_t>(t) % 16) return tdb_fail(TDB_ERR_ALIGN, "weight, state and workspace must be 16-byte aligned");
+    if (a->weight_stride * size % 4 || a->weight_stride < a->hidden || a->weight_stride * size > (1 << 22))
+        return tdb_fail(TDB_ERR_STRIDE, "weight_stride %lld: need a multiple of 4 bytes, at least a row and at most 4 MiB", (long long)a->weight_stride);
+    if (reinterpret_cast<uintptr_t>(a->weight) % 4) return tdb_fail(TDB_ERR_ALIGN, "weight must be 4-byte aligned");
+    for (const void* t : {static_cast<const void*>(a->state), static_cast<const void*>(a->workspace)})
+        if (reinterpret_cast<uintptr_t>(t) % 16) return tdb_fail(TDB_ERR_ALIGN, "state and workspace must be 16-byte aligned");
     if (!backward) {
         if (a->rows && (!a->x || !a->labels)) return tdb_fail(TDB_ERR_NULL, "x and labels must be non-NULL");
         if (a->x_stride < 0) return tdb_fail(TDB_ERR_STRIDE, "negative row stride");
@@ -921,7 +934,7 @@ Loss loss_of(const tdb_loss_args& a, const Plan& p) {
     k.hidden = a.hidden, k.reduction = a.reduction, k.bias_kind = !a.bias ? 0 : a.bias_dtype == a.dtype ? 1 : 2, k.loss = a.loss;
     k.count = reinterpret_cast<int32_t*>(state), k.index = reinterpret_cast<int32_t*>(state + p.index), k.place = reinterpret_cast<int32_t*>(state + p.place);
     k.label = reinterpret_cast<int32_t*>(state + p.label), k.top = reinterpret_cast<float*>(state + p.top), k.inverse = reinterpret_cast<float*>(state + p.inverse);
-    k.biases = reinterpret_cast<float*>(state + p.biases), k.gathered = state + p.gathered, k.pitch = p.pitch, k.padded = p.padded, k.group = p.group;
+    k.biases = reinterpret_cast<float*>(state + p.biases), k.gathered = state + p.gathered, k.pitch = p.pitch, k.padded = p.padded, k.group = p.group, k.few_width = p.few_width;
     k.right = reinterpret_cast<float*>(state + p.right), k.maxima = reinterpret_cast<float*>(work + p.maxima), k.sums = reinterpret_cast<float*>(work + p.sums);
     k.block_sums = reinterpret_cast<double*>(work + p.block_sums);
     return k;
@@ -942,6 +955,12 @@ hipError_t launch(int64_t grid, int threads, int shared, hipStream_t s, const AR
     return hipGetLastError();
 }
 
+// go(the width of the tiles of few rows' logits, a constant)
+template <class GO>
+hipError_t few_rows(const Plan& p, GO go) {
+    return p.few_width == 256 ? go(std::integral_constant<int, 256>()) : go(std::integral_constant<int, 128>());
+}
+
 #define TDB_TRY(...) \
     do { \
         if (const hipError_t e = (__VA_ARGS__); e != hipSuccess) return e; \
@@ -955,7 +974,7 @@ hipError_t forward(const tdb_loss_args& a, hipStream_t s) {
     const bool wide = reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.x_stride * p.size % 16 == 0 && int64_t(a.hidden) * p.size % 16 == 0;
     const int64_t row_blocks = std::max<int64_t>(1, (a.rows + chunk - 1) / chunk), bias_blocks = (p.vocab + 256 * GATHER_WAVES - 1) / (256 * GATHER_WAVES);
     TDB_TRY(launch<loss_gather_kernel<DT>>(row_blocks + bias_blocks, 64 * GATHER_WAVES, 0, s, k, chunk, int(row_blocks), wide));
-    if (p.few) TDB_TRY(launch<loss_logits_few_kernel<DT>>(2 * p.blocks, 256, FEW_SHARED, s, k));
+    if (p.few) TDB_TRY(few_rows(p, [&](auto f) { return launch<loss_logits_few_kernel<DT, f()>>(Few<DT, f()>::PER_CU * p.blocks, Few<DT, f()>::THREADS, Few<DT, f()>::SHARED, s, k); }));
     if (p.many) TDB_TRY(launch<loss_logits_many_kernel<DT>>(p.blocks, 512, MANY_SHARED + TileArrays<Logits256<DT>, 2>::BYTES, s, k));
     return launch<loss_finish_kernel<DT>>(p.finish_blocks, 1024, 0, s, k);
 }
@@ -973,15 +992,15 @@ hipError_t backward(const tdb_loss_args& a, hipStream_t s) {
     auto floats = [&](int64_t at) { return reinterpret_cast<float*>(work + at); };
     g.shifted = weighted && a.dtype == TDB_F16 ? work + p.shifted : k.gathered;
     g.scale = floats(p.scale), g.share = floats(p.share), g.shift = floats(p.shift), g.common = floats(p.common), g.column_sums = floats(p.column_sums);
-    g.wide_dweight = reinterpret_cast<uintptr_t>(a.dweight) % 16 == 0 && g.dweight_pitch % 16 == 0 && int64_t(a.hidden) * p.size % 16 == 0;
+    g.wide_dweight = reinterpret_cast<uintptr_t>(a.dweight) % 4 == 0 && g.dweight_pitch % 4 == 0;
     if (weighted && a.rows) TDB_TRY(launch<loss_weigh_kernel<DT>>(std::min<int64_t>(p.padded / 16, 1024), 256, 0, s, k, g));
     for (g.first = 0; g.first < a.vocab; g.first += p.columns) {
         g.columns = std::min(p.columns, p.vocab - g.first), g.later = g.first > 0;
         if (weighted) {
-            if (p.few) TDB_TRY(launch<loss_difference_few_kernel<DT, true>>(2 * p.blocks, 256, FEW_SHARED, s, k, g));
+            if (p.few) TDB_TRY(few_rows(p, [&](auto f) { return launch<loss_difference_few_kernel<DT, true, f()>>(Few<DT, f()>::PER_CU * p.blocks, Few<DT, f()>::THREADS, Few<DT, f()>::SHARED, s, k, g); }));
             if (p.many) TDB_TRY(launch<loss_difference_many_kernel<DT, true>>(p.blocks, 512, MANY_SHARED + TileArrays<Logits256<DT>, 7>::BYTES, s, k, g));
         } else {
-            if (p.few) TDB_TRY(launch<loss_difference_few_kernel<DT, false>>(2 * p.blocks, 256, FEW_SHARED, s, k, g));
+            if (p.few) TDB_TRY(few_rows(p, [&](auto f) { return launch<loss_difference_few_kernel<DT, false, f()>>(Few<DT, f()>::PER_CU * p.blocks, Few<DT, f()>::THREADS, Few<DT, f()>::SHARED, s, k, g); }));
             if (p.many) TDB_TRY(launch<loss_difference_many_kernel<DT, false>>(p.blocks, 512, MANY_SHARED + TileArrays<Logits256<DT>, 5>::BYTES, s, k, g));
         }
         if (a.rows && a.dx) {

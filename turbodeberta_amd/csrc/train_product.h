@@ -75,20 +75,20 @@ __device__ __forceinline__ float over_quads(float x, F f) {
 
 // A matrix in memory: rows `pitch` bytes apart, `width` bytes of each.
 struct Rows {
-    const char* p;
+    const char* p;          // at a multiple of 4 bytes, as is pitch
     int64_t pitch;
     int64_t count;
-    uint32_t width;         // a multiple of 16
+    uint32_t width;
 };
 
 __device__ __forceinline__ uint32_t uniform(uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ __forceinline__ void load_shared(uint32_t to, u32x4 buffer, uint32_t offset) {      // (nothing else in the kernels of this header uses m0)
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(offset), "s"(buffer) : "memory");
 }
-// `bytes` from p on, at most 2 GiB
+// `bytes` from p on, at most 2 GiB; an odd 16-bit value at their end has its four bytes read
 __device__ __forceinline__ u32x4 buffer_of(const char* p, int64_t bytes) {
     const uint64_t a = reinterpret_cast<uint64_t>(p);
-    return u32x4{uniform(uint32_t(a)), uniform(uint32_t(a >> 32) & 0xffff), uniform(uint32_t(bytes < 0 ? 0 : bytes > 0x7fffffff ? 0x7fffffff : bytes)), 0x00020000};
+    return u32x4{uniform(uint32_t(a)), uniform(uint32_t(a >> 32) & 0xffff), uniform(uint32_t(bytes < 0 ? 0 : bytes > 0x7ffffffc ? 0x7ffffffc : bytes + 3 & ~3)), 0x00020000};
 }
 template <int N>
 __device__ __forceinline__ void wait_loads() {
@@ -104,9 +104,10 @@ struct Side {
     using M = Matrix<DT>;
     using T = typename M::T;
     static constexpr int ES = sizeof(T), STEP = LINE / ES, BYTES = EXTENT * LINE;
-    static constexpr int LOADS = BYTES / 1024 / WAVES;                 // of 1 KB, by each wave
+    static constexpr int UNITS = BYTES / 1024, LOADS = UNITS < WAVES ? 1 : UNITS / WAVES;      // loads of 1 KB, by each wave (where there are fewer than waves, some bring the same)
     static constexpr int ROW = TURNED ? EXTENT * ES : LINE, CHUNKS = ROW / 16, BLOCKS = ROW / 64;
-    static_assert(LOADS * 1024 * WAVES == BYTES && (LINE == 128 || LINE == 64), "");
+    static_assert((UNITS % WAVES == 0 || WAVES % UNITS == 0) && UNITS * 1024 == BYTES && (LINE == 128 || LINE == 64), "");
+    static __device__ __forceinline__ uint32_t own() { return UNITS < WAVES ? uniform(threadIdx.x >> 6) % UNITS : uniform(threadIdx.x >> 6); }
     uint32_t from[LOADS];       // of the lane, in the step's buffer
     uint32_t column[LOADS];     // lined: bytes into the row
 
@@ -122,7 +123,7 @@ struct Side {
 
     // The same for every tile.  Columns of a turned operand past its width come from its next row, or as zeros: they are sums of their own, which nobody stores.
     __device__ __forceinline__ void place(const Rows& a) {
-        const int wave = threadIdx.x >> 6, l = threadIdx.x & 63;
+        const int wave = own(), l = threadIdx.x & 63;
 #pragma unroll
         for (int j = 0; j < LOADS; ++j) {
             const int at = (wave * LOADS + j) * 64 + l, row = at / CHUNKS, chunk = at % CHUNKS;
@@ -147,14 +148,20 @@ struct Side {
             p += by, left -= by, line -= by;
         }
     };
-    // Loads lo .. hi - 1 of a step into LDS.  TAIL: rows may end inside a step (what follows them is another row; the other operand's zeros do not take an infinity's or NaN's place).
+    // Loads lo .. hi - 1 of a step into LDS.  TAIL: rows may end inside a step; 16-byte chunks behind their ends are zeros, and clear() takes out what lies behind the
+    // end of a row in its last one.
     template <bool TAIL>
     __device__ __forceinline__ void load(const Cursor& c, uint32_t lds, int lo = 0, int hi = LOADS) const {
-        const uint32_t to = lds + uniform(threadIdx.x >> 6) * (LOADS * 1024);
+        const uint32_t to = lds + own() * (LOADS * 1024);
         const u32x4 buffer = buffer_of(c.p, c.left);
 #pragma unroll
         for (int j = 0; j < LOADS; ++j)
-            if (j >= lo && j < hi) load_shared(to + j * 1024, buffer, TURNED || !TAIL || column[j] < uint32_t(min(c.line, int64_t(LINE))) ? from[j] : PAST);
+            if (j >= lo && j < hi) load_shared(to + j * 1024, buffer, TURNED || !TAIL || int(column[j]) < int(max(int64_t(0), min(c.line, int64_t(LINE)))) ? from[j] : PAST);
+    }
+    // Zeros behind the first `rest` bytes of a lined step's rows, to the end of their 16.
+    static __device__ __forceinline__ void clear(char* lds, int rest) {
+        for (int r = threadIdx.x; r < EXTENT; r += WAVES * 64)
+            for (int b = rest & 15; b < 16; b += 2) *reinterpret_cast<uint16_t*>(lds + r * LINE + ((rest >> 4 ^ swap(r)) << 4) + b) = 0;
     }
     // Frag of rows row .. (a multiple of SIDE), part kk of the step (32 bytes, or 64 of float32)
     __device__ __forceinline__ typename M::Frag frag(const char* lds, int row, int kk) const {
@@ -223,6 +230,12 @@ struct Product {
         __device__ __forceinline__ void frag_a(typename M::Frag& f, int stage, int i, int kk) const { f = side_a.frag(smem + stage * STAGE, wave_m() + i * M::SIDE, kk); }
         __device__ __forceinline__ void frag_b(typename M::Frag& f, int stage, int j, int kk) const { f = side_b.frag(smem + stage * STAGE + A::BYTES, wave_n() + j * M::SIDE, kk); }
     };
+    // The step of a tile in which B's rows end inside 16 bytes (if there is none, one that never comes), and what lies behind their ends there taken out.
+    static __device__ __forceinline__ int ragged_step(const Flow& flow, const Tile& t) { return !TURN_B && flow.b.width % 16 ? int(flow.b.width / LINE - t.begin) : -1; }
+    static __device__ __forceinline__ void clear(const Flow& flow, int stage) {
+        if constexpr (!TURN_B) B::clear(flow.smem + stage * STAGE + A::BYTES, int(flow.b.width % LINE));
+        step_barrier();
+    }
     static __device__ __forceinline__ void products(const Flow& flow, int stage, Acc& acc) {
 #pragma unroll
         for (int kk = 0; kk < PARTS; ++kk) {
@@ -256,7 +269,7 @@ struct Product {
     // One tile by itself.
     template <class START>
     static __device__ __forceinline__ void run(Flow& flow, const Tile& t, Acc& acc, START start) {
-        const int steps = int(t.end - t.begin);
+        const int steps = int(t.end - t.begin), ragged = ragged_step(flow, t);
         step_barrier();                     // nobody has use for what LDS held
         flow.seek(t);
 #pragma unroll
@@ -269,6 +282,7 @@ struct Product {
             else wait_loads<0>();
             step_barrier();                 // this stage is there, and nobody reads the one before it any more
             if (s + NS - 1 < steps) flow.load(ahead);
+            if (s == ragged) clear(flow, stage);
             products(flow, stage, acc);
             stage = stage == NS - 1 ? 0 : stage + 1;
             ahead = ahead == NS - 1 ? 0 : ahead + 1;
@@ -289,7 +303,7 @@ struct Product {
     static __device__ __forceinline__ char* scratch(char* smem, int stage) { return smem + (stage ^ 1) * STAGE; }
     template <int LATER, class START, class BESIDE>
     static __device__ __forceinline__ void run_on(Flow& flow, const Tile& t, const Tile& next, bool more, int& stage, bool first, Acc& acc, START start, BESIDE& beside) {
-        const int steps = int(t.end - t.begin);
+        const int steps = int(t.end - t.begin), ragged = ragged_step(flow, t);
         auto go_on = [&]() {
             flow.seek(next), beside.load(next);
             flow.at_a.left = more ? flow.at_a.left : 0, flow.at_b.left = more ? flow.at_b.left : 0;
@@ -310,6 +324,7 @@ struct Product {
                     if (s + 1 == steps) go_on();
                     flow.load(stage ^ 1);
                 }
+                if (s == ragged) clear(flow, stage);
                 products(flow, stage, acc);
                 stage ^= 1;
             }
@@ -341,6 +356,7 @@ struct Product {
             constexpr std::integral_constant<int, 1> q1;
             constexpr std::integral_constant<int, 2> q2;
             constexpr std::integral_constant<int, 3> q3;
+            if (ragged == 0) clear(flow, stage);
 #pragma unroll
             for (int i = 0; i < TM; ++i) flow.frag_a(fa[0][i], stage, i, 0);
 #pragma unroll
@@ -351,6 +367,7 @@ struct Product {
                 multiply(q2, yes, stage, no, 0);
                 wait_loads<0>();
                 step_barrier();
+                if (s + 1 == ragged) clear(flow, stage ^ 1);
                 if (s + 2 == steps) go_on();
                 multiply(q3, yes, stage ^ 1, yes, stage);
                 stage ^= 1;
@@ -369,7 +386,8 @@ struct Product {
     };
 
     // The tile's values to rows of memory by way of LDS (SCRATCH bytes), SIDE rows at a time: value(i, j, q) gives four neighbours, then(i, the wave's rows in LDS) may change what
-    // lies there.  to: value (m0, n0); rows and columns: how many of the tile's there are.  Whole 16-byte chunks where `wide`: STORES memory operations of every wave.
+    // lies there.  to: value (m0, n0); rows and columns: how many of the tile's there are.  16 bytes at a time where `wide` (rows at multiples of 4 bytes), and what is less at
+    // a row's end value by value: STORES memory operations of every wave at least.
     static constexpr int COLUMNS = TN * M::SIDE, ROW = COLUMNS * int(sizeof(T)), PER = ROW / 16, STORES = TM * M::SIDE * PER / 64;
     static constexpr int SETS = WAVES * 2 * M::SIDE * ROW <= STAGE ? 2 : 1, SCRATCH = WAVES * SETS * M::SIDE * ROW;       // (two where a stage holds them)
     static_assert(SCRATCH <= (NS == 2 ? STAGE : SHARED), "");
@@ -401,8 +419,13 @@ struct Product {
                 for (int r = 0; r < M::SIDE * PER / 64; ++r) {
                     const int at = r * 64 + l, row = at / PER, c = at % PER;
                     const u32x4 v = *reinterpret_cast<const u32x4*>(mine + lies_at(row, c * 16));
-                    __builtin_amdgcn_raw_buffer_store_b128(v, buffer, c * 16 < columns * ES ? uint32_t(row) * uint32_t(pitch) + c * 16 : PAST, 0, 0);
+                    __builtin_amdgcn_raw_buffer_store_b128(v, buffer, c * 16 + 16 <= columns * ES ? uint32_t(row) * uint32_t(pitch) + c * 16 : PAST, 0, 0);
                 }
+                if (const int whole = int(columns * ES / 16 * (16 / ES)), rest = int(columns) - whole; rest > 0 && columns < COLUMNS)       // a row's end: fewer than 16 bytes
+                    for (int at = l; at < M::SIDE * rest; at += 64) {
+                        const int row = at / rest, c = whole + at % rest;
+                        if (i * M::SIDE + row < rows) *reinterpret_cast<T*>(to + (i * M::SIDE + row) * pitch + c * ES) = *reinterpret_cast<const T*>(mine + lies_at(row, c * ES));
+                    }
             } else {
                 for (int at = l; at < M::SIDE * COLUMNS; at += 64) {
                     const int row = at / COLUMNS, c = at % COLUMNS;

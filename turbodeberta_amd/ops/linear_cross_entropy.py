@@ -23,22 +23,21 @@ def _as_rows(x: torch.Tensor) -> torch.Tensor:
 
 
 def _weight_rows(w: torch.Tensor) -> torch.Tensor:
-    """Rows that the kernels can address: aligned, a multiple of 16 bytes apart, with zeros behind them up to one."""
+    """Rows that the kernels can address: values side by side, at multiples of 4 bytes; a copy where they are not."""
     es = w.element_size()
-    if (w.shape[1] * es) % 16:
-        to = torch.zeros(w.shape[0], -(-w.shape[1] * es // 16) * 16 // es, dtype=w.dtype, device=w.device)
-        to[:, :w.shape[1]] = w
-        return to
-    if w.shape[0] == 1:
-        return w if w.stride(1) == 1 and w.data_ptr() % 16 == 0 and w.stride(0) == w.shape[1] else L.copied(w)
-    return w if L.rows_ok(w) and w.shape[1] <= w.stride(0) and w.stride(0) * es <= 1 << 22 else L.copied(w)
+    apart = w.shape[1] if w.shape[0] == 1 else w.stride(0)
+    if (w.shape[1] == 1 or w.stride(1) == 1) and w.data_ptr() % 4 == 0 and w.shape[1] <= apart and (apart * es) % 4 == 0 and apart * es <= 1 << 22:
+        return w
+    if (w.shape[1] * es) % 4 == 0:
+        return L.copied(w)
+    return torch.empty(w.shape[0], w.shape[1] + 1, dtype=w.dtype, device=w.device)[:, :-1].copy_(w)
 
 
 def _arguments(weight, bias, rows, hidden, ignore_index, reduction) -> _lib.LossArgs:
     a = _lib.LossArgs()
     a.dtype, a.bias_dtype = L.dtype_code(weight), L.dtype_code(weight if bias is None else bias)
     a.hidden, a.reduction, a.rows, a.vocab, a.ignore_index = hidden, reduction, rows, weight.shape[0], ignore_index
-    a.weight, a.weight_stride, a.bias = weight.data_ptr(), weight.stride(0), None if bias is None else bias.data_ptr()
+    a.weight, a.weight_stride, a.bias = weight.data_ptr(), max(weight.stride(0), hidden), None if bias is None else bias.data_ptr()
     return a
 
 
