@@ -292,18 +292,15 @@ struct TileArrays {
 template <int DT>
 using Logits256 = Product<DT, 256, 256, 2, 4, 2, false, false>;
 constexpr int MANY_SHARED = Logits256<TDB_BF16>::SHARED;
-// Few rows: eight waves to a CU in 16 bits, steps as deep as LDS holds; of float32, which has the more to multiply, twice four, as of tiles of 128 columns.  (31 rows, 91214 classes, 1024 columns
-// of float32: 156 + 119 us with eight waves, 139 + 103 with twice four; 55, 128100, 1024 of float16: 76 + 49 and 81 + 51.)
+// Few rows: eight waves to a CU in 16 bits, with steps as deep as LDS holds; of float32, which has the more to multiply, twice four, or twice eight for tiles of 128 columns.  (31 rows, 91214 classes,
+// 1024 columns of float32: 156 + 119 us with eight waves, 139 + 103 with twice four; 55, 128100, 1024 of float16: 76 + 49 and 81 + 51.)
 template <int DT, int BN>
 struct Few {
-    static constexpr bool DEEP = DT != TDB_F32 && BN == 256;
-    static constexpr int THREADS = DEEP ? 512 : 256, WM = DEEP ? 2 : 1, LINE = DEEP ? 128 : 64;
-    using Logits128 = Product<DT, 128, BN, WM, 4, 3, false, false, LINE>;
+    static constexpr int THREADS = DT != TDB_F32 || BN == 128 ? 512 : 256, WAVES = THREADS / 64, WM = WAVES / 4, LINE = WM * 64, PER_CU = DT != TDB_F32 ? 1 : 2;
+    using Logits128 = Product<DT, 128, BN, WM, 4, BN == 128 ? 2 : 3, false, false, LINE>;
     using Logits64 = Product<DT, 64, BN, WM, 4, 3, false, false, LINE>;
-    using Logits32 = Product<DT, 32, BN, 1, THREADS / 64, DEEP || BN == 128 ? 4 : 2, false, false>;
-    static constexpr int SHARED = Logits128::SHARED > Logits32::SHARED ? Logits128::SHARED : Logits32::SHARED;
-    static constexpr int PER_CU = DEEP ? 1 : 2;
-    static_assert(Logits64::SHARED <= SHARED, "");
+    using Logits32 = Product<DT, 32, BN, 1, WAVES, DT != TDB_F32 ? 4 : BN == 128 ? 3 : 2, false, false>;
+    static constexpr int SHARED = std::max(std::max(Logits128::SHARED, Logits64::SHARED), Logits32::SHARED);
 };
 
 template <int DT>
@@ -860,10 +857,10 @@ Plan plan_of(const tdb_loss_args& a) {
     const int64_t most = std::min<int64_t>(std::max<int64_t>(D_BYTES / (p.padded * p.size) / TILE, 1), (int64_t(1) << 22) / p.size / TILE), pieces = (wide + most - 1) / most;
     p.columns = (wide + pieces - 1) / pieces * TILE;
     p.blocks = std::max(8, tdb_compute_units(-1) & -8);
-    // Tiles of 128 columns where there are fewer of 256 than CUs to read the weights.  The two passes over them in tiles of 256 and 128 columns: one row, 32510 classes, 768 columns of float32
-    // 37 + 39 and 27 + 29 us; 3 rows, 3858 classes, 1024 columns of float16 14 + 15 and 11 + 12; 17, 36468, 416 of bfloat16 11 + 11 and 13 + 14; 269, 7913, 768 of float32, which multiplies
-    // for most of its time, 64 + 65 and 70 + 71.
-    p.few_width = a.rows <= 128 && wide * (p.size == 4 ? 1 : 2) < p.blocks ? 128 : 256;
+    // Few rows of float32: tiles of 128 columns where those share out better over the CUs.  The two passes over the weights in tiles of 256 and 128 columns: one row, 32510 classes, 768 columns
+    // 37 + 39 and 27 + 29 us; 42, 73329, 928 148 + 145 and 125 + 125; 16, 128100, 1232 187 + 138 and 201 + 163.  (In 16 bits tiles of 128 are no faster: 20, 73329, 768 27 + 29 and 28 + 30.)
+    auto rounds = [&](int64_t tiles) { return (tiles + p.blocks - 1) / p.blocks; };
+    p.few_width = a.dtype == TDB_F32 && a.rows <= 128 && rounds(2 * wide) < 2 * rounds(wide) ? 128 : 256;
     p.dx_width = tile_columns(a.hidden, a.dtype, 0, p.blocks), p.dw_width = tile_columns(a.hidden, a.dtype, p.columns / TILE, p.blocks);
     p.finish_blocks = int(std::min<int64_t>((std::max<int64_t>(a.rows, 1) + FINISH_ROWS - 1) / FINISH_ROWS, 256));
     int64_t at = 256;
@@ -956,9 +953,11 @@ hipError_t launch(int64_t grid, int threads, int shared, hipStream_t s, const AR
 }
 
 // go(the width of the tiles of few rows' logits, a constant)
-template <class GO>
+template <int DT, class GO>
 hipError_t few_rows(const Plan& p, GO go) {
-    return p.few_width == 256 ? go(std::integral_constant<int, 256>()) : go(std::integral_constant<int, 128>());
+    if constexpr (DT == TDB_F32)
+        if (p.few_width == 128) return go(std::integral_constant<int, 128>());
+    return go(std::integral_constant<int, 256>());
 }
 
 #define TDB_TRY(...) \
@@ -974,7 +973,7 @@ hipError_t forward(const tdb_loss_args& a, hipStream_t s) {
     const bool wide = reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.x_stride * p.size % 16 == 0 && int64_t(a.hidden) * p.size % 16 == 0;
     const int64_t row_blocks = std::max<int64_t>(1, (a.rows + chunk - 1) / chunk), bias_blocks = (p.vocab + 256 * GATHER_WAVES - 1) / (256 * GATHER_WAVES);
     TDB_TRY(launch<loss_gather_kernel<DT>>(row_blocks + bias_blocks, 64 * GATHER_WAVES, 0, s, k, chunk, int(row_blocks), wide));
-    if (p.few) TDB_TRY(few_rows(p, [&](auto f) { return launch<loss_logits_few_kernel<DT, f()>>(Few<DT, f()>::PER_CU * p.blocks, Few<DT, f()>::THREADS, Few<DT, f()>::SHARED, s, k); }));
+    if (p.few) TDB_TRY(few_rows<DT>(p, [&](auto f) { return launch<loss_logits_few_kernel<DT, f()>>(Few<DT, f()>::PER_CU * p.blocks, Few<DT, f()>::THREADS, Few<DT, f()>::SHARED, s, k); }));
     if (p.many) TDB_TRY(launch<loss_logits_many_kernel<DT>>(p.blocks, 512, MANY_SHARED + TileArrays<Logits256<DT>, 2>::BYTES, s, k));
     return launch<loss_finish_kernel<DT>>(p.finish_blocks, 1024, 0, s, k);
 }
@@ -997,10 +996,10 @@ hipError_t backward(const tdb_loss_args& a, hipStream_t s) {
     for (g.first = 0; g.first < a.vocab; g.first += p.columns) {
         g.columns = std::min(p.columns, p.vocab - g.first), g.later = g.first > 0;
         if (weighted) {
-            if (p.few) TDB_TRY(few_rows(p, [&](auto f) { return launch<loss_difference_few_kernel<DT, true, f()>>(Few<DT, f()>::PER_CU * p.blocks, Few<DT, f()>::THREADS, Few<DT, f()>::SHARED, s, k, g); }));
+            if (p.few) TDB_TRY(few_rows<DT>(p, [&](auto f) { return launch<loss_difference_few_kernel<DT, true, f()>>(Few<DT, f()>::PER_CU * p.blocks, Few<DT, f()>::THREADS, Few<DT, f()>::SHARED, s, k, g); }));
             if (p.many) TDB_TRY(launch<loss_difference_many_kernel<DT, true>>(p.blocks, 512, MANY_SHARED + TileArrays<Logits256<DT>, 7>::BYTES, s, k, g));
         } else {
-            if (p.few) TDB_TRY(few_rows(p, [&](auto f) { return launch<loss_difference_few_kernel<DT, false, f()>>(Few<DT, f()>::PER_CU * p.blocks, Few<DT, f()>::THREADS, Few<DT, f()>::SHARED, s, k, g); }));
+            if (p.few) TDB_TRY(few_rows<DT>(p, [&](auto f) { return launch<loss_difference_few_kernel<DT, false, f()>>(Few<DT, f()>::PER_CU * p.blocks, Few<DT, f()>::THREADS, Few<DT, f()>::SHARED, s, k, g); }));
             if (p.many) TDB_TRY(launch<loss_difference_many_kernel<DT, false>>(p.blocks, 512, MANY_SHARED + TileArrays<Logits256<DT>, 5>::BYTES, s, k, g));
         }
         if (a.rows && a.dx) {
