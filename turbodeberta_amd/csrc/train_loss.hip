@@ -159,13 +159,17 @@ __global__ __launch_bounds__(64 * GATHER_WAVES) void loss_gather_kernel(Loss p, 
                     if (r0 + u < at) reinterpret_cast<uint4*>(p.gathered + (r0 + u) * p.pitch)[c] = v[u];
             }
         } else {
-            for (int c = l; c < columns; c += 64) {
-                T v[GATHER_ROWS];
+            for (int c0 = l; c0 < columns; c0 += 64 * U) {
+                T v[U][GATHER_ROWS];
 #pragma unroll
-                for (int u = 0; u < GATHER_ROWS; ++u) v[u] = c < p.hidden ? from[u][c] : T(0.f);
+                for (int k = 0; k < U; ++k)
 #pragma unroll
-                for (int u = 0; u < GATHER_ROWS; ++u)
-                    if (r0 + u < at) reinterpret_cast<T*>(p.gathered + (r0 + u) * p.pitch)[c] = v[u];
+                    for (int u = 0; u < GATHER_ROWS; ++u) v[k][u] = c0 + 64 * k < p.hidden ? from[u][c0 + 64 * k] : T(0.f);
+#pragma unroll
+                for (int k = 0; k < U; ++k)
+#pragma unroll
+                    for (int u = 0; u < GATHER_ROWS; ++u)
+                        if (r0 + u < at && c0 + 64 * k < columns) reinterpret_cast<T*>(p.gathered + (r0 + u) * p.pitch)[c0 + 64 * k] = v[k][u];
             }
         }
     }
