@@ -58,6 +58,15 @@ def test_sizes(rows, hidden, vocab, share, dtype):
     _check(x, w, labels, b, "mean", torch.tensor(0.7, device="cuda"))
 
 
+# every height of tiles, one and several of them, up to where the next one takes over
+@pytest.mark.parametrize("rows", [32, 60, 96, 97, 128, 160, 161, 192, 193, 257, 288, 320, 480, 481, 512, 760, 1024, 1025])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_heights_of_tiles(dtype, rows):
+    x, w, labels, b = _inputs(rows, 160, 900, dtype)
+    _check(x, w, labels, b, "mean")
+    _check(x, w, labels, b, "none", _rand(5, rows))
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
 @pytest.mark.parametrize("bias", [None, "same", "fp32"])

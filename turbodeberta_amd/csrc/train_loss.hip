@@ -22,17 +22,21 @@ constexpr int TILE = 256;           // what rows and columns of the buffers are 
 constexpr int FINISH_ROWS = 32;     // rows of a workgroup of the last forward kernel
 constexpr int FEW = 1024;           // rows up to which tiles may be lower than 256
 
-// Rows of a tile where n count: the height with the least rows times what a row of such tiles costs.  16 bits, 128100 x 768: a tile's logits and their gradient took 125 us for 256 rows,
-// 70 to 77 for 128, 48 for 64, 31 for 32 (lower tiles load more for their products); float32, bound by products, 770, 390, 213, 116.  160 rows of float32: 610 us in tiles of
-// 32, 677 of 64, 770 of 256; of bfloat16 173, 163, 130.
+// Rows of a tile where n count: the height by which the busiest of `blocks` workgroups has least to do, tiles at their price; `wide` tiles lie beside each other.  16 bits, 128100 x 768: a tile's
+// logits and their gradient took 125 us for 256 rows, 70 to 77 for 128, 48 for 64, 31 for 32 (lower tiles load more for their products).  float32, bound by products, 765 for 256, 514 for 160,
+// 414 for 128, 336 for 96, 240 for 64, 135 for 32: 96 rows 382 us in one tile and 529 in two of 64, 160 rows 524 in one and 667 in five of 32.  Where tiles are few, low ones share out better:
+// 141 rows, 18134 classes, 704 columns of bfloat16 take 51 us in 71 tiles of 256 rows and 31 in 213 of 64.  (No tiles past the rows' multiple of 256, which the buffers have.)
 template <int DT>
-__host__ __device__ constexpr int tile_rows(int n, int least) {
-    int best = 256, cost = (n + 255) / 256 * 256 * 16;
-    if (n > FEW) return best;
-    const int heights[] = {128, 64, 32}, dear[] = {DT == TDB_F32 ? 16 : 20, DT == TDB_F32 ? 18 : 26, DT == TDB_F32 ? 19 : 32};
-    for (int i = 0; i < 3; ++i) {
-        const int h = heights[i], c = (n + h - 1) / h * h * dear[i];
-        if (h >= least && c < cost) best = h, cost = c;
+__host__ __device__ constexpr int tile_rows(int n, int least, int64_t wide, int blocks) {
+    if (n > FEW) return TILE;
+    const int rows = (n + TILE - 1) / TILE;
+    int best = TILE;
+    int64_t cost = (rows * wide + blocks - 1) / blocks * (TILE * 32);
+    const int heights[] = {160, 128, 96, 64, 32}, dear[] = {DT == TDB_F32 ? 34 : 64, DT == TDB_F32 ? 35 : 40, DT == TDB_F32 ? 37 : 64, DT == TDB_F32 ? 40 : 52, DT == TDB_F32 ? 45 : 64};
+    for (int i = 0; i < 5; ++i) {
+        const int h = heights[i], high = (n + h - 1) / h;
+        const int64_t c = (high * wide + blocks - 1) / blocks * (h * dear[i]);
+        if (h >= least && high * h <= rows * TILE && c < cost && (DT == TDB_F32 || (h & (h - 1)) == 0)) best = h, cost = c;
     }
     return best;
 }
@@ -59,6 +63,9 @@ struct Loss {
     double* block_sums;
     int64_t padded;                             // rows, rounded up
     int32_t group, few_width;                   // column tiles that a workgroup of the kernel for many rows takes together; columns of the tiles of the one for few
+    int32_t blocks;                             // workgroups of the kernel for many rows
+    template <int DT>
+    __device__ __forceinline__ int rows_of(int n) const { return tile_rows<DT>(n, 32, (vocab + few_width - 1) / few_width, blocks); }       // of a tile of logits
 };
 
 // How the logits' maxima and sums lie: groups of column tiles, rows `pitch` to each.
@@ -304,7 +311,9 @@ struct Few {
     using Logits128 = Product<DT, 128, BN, WM, 4, BN == 128 ? 2 : 3, false, false, LINE>;
     using Logits64 = Product<DT, 64, BN, WM, 4, 3, false, false, LINE>;
     using Logits32 = Product<DT, 32, BN, 1, WAVES, DT != TDB_F32 ? 4 : BN == 128 ? 3 : 2, false, false>;
-    static constexpr int SHARED = std::max(std::max(Logits128::SHARED, Logits64::SHARED), Logits32::SHARED);
+    using Logits160 = Product<DT, 160, BN, WM, 4, 2, false, false, LINE>;       // (float32)
+    using Logits96 = Product<DT, 96, BN, WM, 4, BN == 128 ? 2 : 3, false, false, LINE>;
+    static constexpr int SHARED = std::max({Logits128::SHARED, Logits64::SHARED, Logits32::SHARED, DT == TDB_F32 ? Logits160::SHARED : 0, DT == TDB_F32 ? Logits96::SHARED : 0});
 };
 
 template <int DT>
@@ -313,7 +322,7 @@ __global__ __launch_bounds__(512, 2) void loss_logits_many_kernel(Loss p) {
     __shared__ float s_top[1024], s_sum[1024];
     using P = Logits256<DT>;
     const int n = p.count[0];
-    if (tile_rows<DT>(n, 32) != 256) return;
+    if (p.template rows_of<DT>(n) != 256) return;
     const Partials parts(p, true);
     const int64_t row_tiles = (n + P::BM - 1) / P::BM, all = row_tiles * parts.groups;
     typename P::Flow flow(smem, hidden_rows<DT>(p, n), weight_rows<DT>(p));
@@ -357,10 +366,16 @@ __global__ __launch_bounds__((Few<DT, BN>::THREADS), 2) void loss_logits_few_ker
     using F = Few<DT, BN>;
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     __shared__ __attribute__((aligned(16))) float s_bias[BN];
-    __shared__ int32_t s_label[128];
-    __shared__ float s_top[512], s_sum[512];
+    __shared__ int32_t s_label[192];
+    __shared__ float s_top[1024], s_sum[1024];
     const int n = p.count[0];
-    switch (tile_rows<DT>(n, 32)) {
+    const int height = p.template rows_of<DT>(n);
+    if constexpr (DT == TDB_F32) {
+        if (height == 96) return logits_body<DT, typename F::Logits96>(p, n, smem, s_bias, s_label, s_top, s_sum);
+        if constexpr (BN == 256)        // (the narrow tiles are for 128 rows at most)
+            if (height == 160) return logits_body<DT, typename F::Logits160>(p, n, smem, s_bias, s_label, s_top, s_sum);
+    }
+    switch (height) {
         case 32: return logits_body<DT, typename F::Logits32>(p, n, smem, s_bias, s_label, s_top, s_sum);
         case 64: return logits_body<DT, typename F::Logits64>(p, n, smem, s_bias, s_label, s_top, s_sum);
         case 128: return logits_body<DT, typename F::Logits128>(p, n, smem, s_bias, s_label, s_top, s_sum);
@@ -373,7 +388,7 @@ __global__ __launch_bounds__(1024) void loss_finish_kernel(Loss p) {
     __shared__ float s_top[32][33], s_sum[32][33];
     __shared__ double s_all[32];
     const int n = p.count[0], l = threadIdx.x & 31, w = threadIdx.x >> 5;
-    const Partials parts(p, tile_rows<DT>(n, 32) == 256);
+    const Partials parts(p, p.template rows_of<DT>(n) == 256);
     const int groups = int(parts.groups);
     double mine = 0.0;
     for (int64_t r0 = int64_t(blockIdx.x) * FINISH_ROWS; r0 < n; r0 += int64_t(gridDim.x) * FINISH_ROWS) {
@@ -529,7 +544,7 @@ __device__ __forceinline__ void difference_of(const Loss& p, const Gradient& g, 
 
 // D of a piece of the vocabulary.
 template <int DT, class P, bool WEIGHTED>
-__device__ __forceinline__ void difference_body(const Loss& p, const Gradient& g, int n, char* smem, float* s_bias, float (&s_rows)[6][128], float* s_column) {
+__device__ __forceinline__ void difference_body(const Loss& p, const Gradient& g, int n, char* smem, float* s_bias, float (&s_rows)[6][192], float* s_column) {
     typename P::Flow flow(smem, hidden_rows<DT>(p, n), weight_rows<DT>(p));
     const int64_t row_tiles = (n + P::BM - 1) / P::BM, column_tiles = g.columns / P::BN, all = row_tiles * column_tiles;
     for (int64_t block = blockIdx.x; block < all; block += gridDim.x) {
@@ -555,7 +570,7 @@ __global__ __launch_bounds__(512, 2) void loss_difference_many_kernel(Loss p, Gr
     __shared__ float s_column[512];
     using P = Logits256<DT>;
     const int n = p.count[0];
-    if (tile_rows<DT>(n, 32) != 256) return;
+    if (p.template rows_of<DT>(n) != 256) return;
     const int64_t row_tiles = (n + P::BM - 1) / P::BM, column_tiles = g.columns / P::BN, all = row_tiles * column_tiles;
     typename P::Flow flow(smem, hidden_rows<DT>(p, n), weight_rows<DT>(p));
     constexpr int ARRAYS = WEIGHTED ? 7 : 5;
@@ -591,9 +606,15 @@ __global__ __launch_bounds__((Few<DT, BN>::THREADS), 2) void loss_difference_few
     using F = Few<DT, BN>;
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     __shared__ __attribute__((aligned(16))) float s_bias[BN];
-    __shared__ float s_column[2 * BN], s_rows[6][128];
+    __shared__ float s_column[2 * BN], s_rows[6][192];
     const int n = p.count[0];
-    switch (tile_rows<DT>(n, 32)) {
+    const int height = p.template rows_of<DT>(n);
+    if constexpr (DT == TDB_F32) {
+        if (height == 96) return difference_body<DT, typename F::Logits96, WEIGHTED>(p, g, n, smem, s_bias, s_rows, s_column);
+        if constexpr (BN == 256)        // (the narrow tiles are for 128 rows at most)
+            if (height == 160) return difference_body<DT, typename F::Logits160, WEIGHTED>(p, g, n, smem, s_bias, s_rows, s_column);
+    }
+    switch (height) {
         case 32: return difference_body<DT, typename F::Logits32, WEIGHTED>(p, g, n, smem, s_bias, s_rows, s_column);
         case 64: return difference_body<DT, typename F::Logits64, WEIGHTED>(p, g, n, smem, s_bias, s_rows, s_column);
         case 128: return difference_body<DT, typename F::Logits128, WEIGHTED>(p, g, n, smem, s_bias, s_rows, s_column);
@@ -606,8 +627,9 @@ struct Shares {
     int height;
     int64_t row_tiles, column_tiles, splits;
     __device__ __forceinline__ Shares(const Loss& p, const Gradient& g, int n, int64_t blocks, int width) {
-        // (Up to 192 rows the product waits for the weights whatever its tiles' height, and low ones make fewer parts to be added up: 154 x 768, tiles of 256 rows 56 + 27 us, of 64 57 + 10.)
-        height = n <= 192 ? 64 : tile_rows<DT>(n, 128);
+        // (Up to 192 rows in 16 bits the product waits for the weights whatever its tiles' height, and low ones make fewer parts to be added up: 154 x 768, tiles of 256 rows 56 + 27 us, of
+        // 64 57 + 10.)
+        height = DT == TDB_F32 ? tile_rows<DT>(n, 64, 1, 1) : n <= 192 ? 64 : tile_rows<DT>(n, 128, 1, 1);
         if (height == 64 && width == 192) width = 256;
         row_tiles = (n + height - 1) / height, column_tiles = (p.hidden + width - 1) / width;
         const int64_t tiles = row_tiles * column_tiles;
@@ -655,14 +677,22 @@ template <int DT, int BN>
 using Dx128 = Product<DT, 128, BN, BN == 256 ? 2 : 4, BN == 256 ? 4 : 2, 3, false, true>;
 template <int DT, int BN>
 using Dx64 = Product<DT, 64, BN == 192 ? 256 : BN, BN == 128 ? 2 : 1, BN == 128 ? 4 : 8, 3, false, true>;
+template <int BN>
+using Dx160 = Product<TDB_F32, 160, BN, 2, 4, 2, false, true>;
+template <int BN>
+using Dx96 = Product<TDB_F32, 96, BN, 2, 4, 3, false, true>;
 constexpr int DX_SHARED = Dx128<TDB_BF16, 256>::SHARED;
-static_assert(Dx256<TDB_BF16, 256>::SHARED <= DX_SHARED && Dx64<TDB_BF16, 256>::SHARED <= DX_SHARED, "");
+static_assert(Dx256<TDB_BF16, 256>::SHARED <= DX_SHARED && Dx64<TDB_BF16, 256>::SHARED <= DX_SHARED && Dx160<256>::SHARED <= DX_SHARED && Dx96<256>::SHARED <= DX_SHARED, "");
 
 template <int DT, int BN>
 __global__ __launch_bounds__(512, 2) void loss_dx_kernel(Loss p, Gradient g) {
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     const int n = p.count[0];
     const Shares<DT> share(p, g, n, gridDim.x, BN);
+    if constexpr (DT == TDB_F32) {
+        if (share.height == 96) return dx_body<DT, Dx96<BN>>(p, g, n, share, smem);
+        if (share.height == 160) return dx_body<DT, Dx160<BN>>(p, g, n, share, smem);
+    }
     switch (share.height) {
         case 64: return dx_body<DT, Dx64<DT, BN>>(p, g, n, share, smem);
         case 128: return dx_body<DT, Dx128<DT, BN>>(p, g, n, share, smem);
@@ -778,7 +808,7 @@ __global__ __launch_bounds__(512, 2) void loss_dweight_kernel(Loss p, Gradient g
     const int64_t steps = (n + P::STEP - 1) / P::STEP;
     const Rows a{g.d, g.d_pitch, n, uint32_t(g.d_pitch)}, b{g.shifted, p.pitch, n, uint32_t(p.pitch)};
     typename P::Flow flow(smem, a, b);
-    const int heights = n ? (n + tile_rows<DT>(n, 32) - 1) / tile_rows<DT>(n, 32) : 0;
+    const int heights = n ? (n + p.template rows_of<DT>(n) - 1) / p.template rows_of<DT>(n) : 0;
     const float factor = n == 0 ? 0.f : (p.reduction ? row_factor(p, g, n) : *g.common) * (1.f / D_SCALE<DT>);
     auto tile = [&](int64_t block) {
         int64_t row, column, split;
@@ -935,7 +965,7 @@ Loss loss_of(const tdb_loss_args& a, const Plan& p) {
     k.hidden = a.hidden, k.reduction = a.reduction, k.bias_kind = !a.bias ? 0 : a.bias_dtype == a.dtype ? 1 : 2, k.loss = a.loss;
     k.count = reinterpret_cast<int32_t*>(state), k.index = reinterpret_cast<int32_t*>(state + p.index), k.place = reinterpret_cast<int32_t*>(state + p.place);
     k.label = reinterpret_cast<int32_t*>(state + p.label), k.top = reinterpret_cast<float*>(state + p.top), k.inverse = reinterpret_cast<float*>(state + p.inverse);
-    k.biases = reinterpret_cast<float*>(state + p.biases), k.gathered = state + p.gathered, k.pitch = p.pitch, k.padded = p.padded, k.group = p.group, k.few_width = p.few_width;
+    k.biases = reinterpret_cast<float*>(state + p.biases), k.gathered = state + p.gathered, k.pitch = p.pitch, k.padded = p.padded, k.group = p.group, k.few_width = p.few_width, k.blocks = p.blocks;
     k.right = reinterpret_cast<float*>(state + p.right), k.maxima = reinterpret_cast<float*>(work + p.maxima), k.sums = reinterpret_cast<float*>(work + p.sums);
     k.block_sums = reinterpret_cast<double*>(work + p.block_sums);
     return k;

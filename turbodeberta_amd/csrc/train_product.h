@@ -104,10 +104,13 @@ struct Side {
     using M = Matrix<DT>;
     using T = typename M::T;
     static constexpr int ES = sizeof(T), STEP = LINE / ES, BYTES = EXTENT * LINE;
-    static constexpr int UNITS = BYTES / 1024, LOADS = UNITS < WAVES ? 1 : UNITS / WAVES;      // loads of 1 KB, by each wave (where there are fewer than waves, some bring the same)
+    static constexpr int UNITS = BYTES / 1024, LOADS = (UNITS + WAVES - 1) / WAVES;        // loads of 1 KB, by each wave (where they do not share out evenly, some bring the same)
     static constexpr int ROW = TURNED ? EXTENT * ES : LINE, CHUNKS = ROW / 16, BLOCKS = ROW / 64;
-    static_assert((UNITS % WAVES == 0 || WAVES % UNITS == 0) && UNITS * 1024 == BYTES && (LINE == 128 || LINE == 64), "");
-    static __device__ __forceinline__ uint32_t own() { return UNITS < WAVES ? uniform(threadIdx.x >> 6) % UNITS : uniform(threadIdx.x >> 6); }
+    static_assert(UNITS * 1024 == BYTES && (LINE == 128 || LINE == 64), "");
+    static __device__ __forceinline__ uint32_t unit(int j) {
+        const uint32_t at = uniform(threadIdx.x >> 6) * LOADS + j;
+        return UNITS % WAVES ? at % UNITS : at;
+    }
     uint32_t from[LOADS];       // of the lane, in the step's buffer
     uint32_t column[LOADS];     // lined: bytes into the row
 
@@ -123,10 +126,10 @@ struct Side {
 
     // The same for every tile.  Columns of a turned operand past its width come from its next row, or as zeros: they are sums of their own, which nobody stores.
     __device__ __forceinline__ void place(const Rows& a) {
-        const int wave = own(), l = threadIdx.x & 63;
+        const int l = threadIdx.x & 63;
 #pragma unroll
         for (int j = 0; j < LOADS; ++j) {
-            const int at = (wave * LOADS + j) * 64 + l, row = at / CHUNKS, chunk = at % CHUNKS;
+            const int at = unit(j) * 64 + l, row = at / CHUNKS, chunk = at % CHUNKS;
             if constexpr (TURNED) {
                 from[j] = uint32_t(row) * uint32_t(a.pitch) + ((((chunk >> 2) ^ turn(row)) << 2) | (chunk & 3)) * 16;
             } else {
@@ -152,11 +155,10 @@ struct Side {
     // end of a row in its last one.
     template <bool TAIL>
     __device__ __forceinline__ void load(const Cursor& c, uint32_t lds, int lo = 0, int hi = LOADS) const {
-        const uint32_t to = lds + own() * (LOADS * 1024);
         const u32x4 buffer = buffer_of(c.p, c.left);
 #pragma unroll
         for (int j = 0; j < LOADS; ++j)
-            if (j >= lo && j < hi) load_shared(to + j * 1024, buffer, TURNED || !TAIL || int(column[j]) < int(max(int64_t(0), min(c.line, int64_t(LINE)))) ? from[j] : PAST);
+            if (j >= lo && j < hi) load_shared(lds + unit(j) * 1024, buffer, TURNED || !TAIL || int(column[j]) < int(max(int64_t(0), min(c.line, int64_t(LINE)))) ? from[j] : PAST);
     }
     // Zeros behind the first `rest` bytes of a lined step's rows, to the end of their 16.
     static __device__ __forceinline__ void clear(char* lds, int rest) {
