@@ -67,6 +67,21 @@ def test_heights_of_tiles(dtype, rows):
     _check(x, w, labels, b, "none", _rand(5, rows))
 
 
+# many rows of a small vocabulary: several workgroups share a tile of dweight, some of them without any row
+@pytest.mark.parametrize("rows,hidden,vocab,share", [(1025, 64, 100, 1.0), (1100, 130, 300, 0.01), (2100, 257, 515, 0.6), (4199, 96, 2010, 1.0), (6000, 33, 7, 0.9), (1600, 200, 9000, 1.0), (1500, 64, 300, 0.0)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_many_rows_of_few_classes(dtype, rows, hidden, vocab, share):
+    x, w, labels, b = _inputs(rows, hidden, vocab, dtype, share)
+    if share == 0.0:
+        loss, grads = _step(x, w, labels, b, "sum")
+        assert not loss.any() and all(not g.any() for g in grads.values())
+        return
+    first = _check(x, w, labels, b, "mean")
+    again = _step(x, w, labels, b, "mean")
+    assert torch.equal(first[0], again[0]) and all(torch.equal(first[1][k], again[1][k]) for k in first[1])
+    _check(x, w, labels, None, "none", _rand(5, rows))
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
 @pytest.mark.parametrize("bias", [None, "same", "fp32"])

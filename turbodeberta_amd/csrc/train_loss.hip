@@ -20,15 +20,15 @@ namespace tdb_train {
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.693147180559945309417f;
 constexpr int TILE = 256;           // what rows and columns of the buffers are rounded up to
 constexpr int FINISH_ROWS = 32;     // rows of a workgroup of the last forward kernel
-constexpr int FEW = 1024;           // rows up to which tiles may be lower than 256
+constexpr int FEW = 1024;           // rows up to which tiles may be lower than 256; all of them where there are few tiles
 
 // Rows of a tile where n count: the height by which the busiest of `blocks` workgroups has least to do, tiles at their price; `wide` tiles lie beside each other.  16 bits, 128100 x 768: a tile's
 // logits and their gradient took 125 us for 256 rows, 70 to 77 for 128, 48 for 64, 31 for 32 (lower tiles load more for their products).  float32, bound by products, 765 for 256, 514 for 160,
 // 414 for 128, 336 for 96, 240 for 64, 135 for 32: 96 rows 382 us in one tile and 529 in two of 64, 160 rows 524 in one and 667 in five of 32.  Where tiles are few, low ones share out better:
 // 141 rows, 18134 classes, 704 columns of bfloat16 take 51 us in 71 tiles of 256 rows and 31 in 213 of 64.  (No tiles past the rows' multiple of 256, which the buffers have.)
 template <int DT>
-__host__ __device__ constexpr int tile_rows(int n, int least, int64_t wide, int blocks) {
-    if (n > FEW) return TILE;
+__host__ __device__ constexpr int tile_rows(int n, int least, int64_t wide, int blocks, int64_t few) {
+    if (n > few) return TILE;
     const int rows = (n + TILE - 1) / TILE;
     int best = TILE;
     int64_t cost = (rows * wide + blocks - 1) / blocks * (TILE * 32);
@@ -64,14 +64,16 @@ struct Loss {
     int64_t padded;                             // rows, rounded up
     int32_t group, few_width;                   // column tiles that a workgroup of the kernel for many rows takes together; columns of the tiles of the one for few
     int32_t blocks;                             // workgroups of the kernel for many rows
+    int64_t few_rows;                           // rows up to which tiles may be lower than 256
+    __device__ __forceinline__ int64_t dw_rows() const { return (vocab + TILE - 1) / TILE * TILE; }
     template <int DT>
-    __device__ __forceinline__ int rows_of(int n) const { return tile_rows<DT>(n, 32, (vocab + few_width - 1) / few_width, blocks); }       // of a tile of logits
+    __device__ __forceinline__ int rows_of(int n) const { return tile_rows<DT>(n, 32, (vocab + few_width - 1) / few_width, blocks, few_rows); }       // of a tile of logits
 };
 
 // How the logits' maxima and sums lie: groups of column tiles, rows `pitch` to each.
 struct Partials {
     int64_t groups, tiles, group, pitch;
-    __device__ __forceinline__ Partials(const Loss& p, bool many) : tiles(many ? (p.vocab + TILE - 1) / TILE : (p.vocab + p.few_width - 1) / p.few_width), group(many ? p.group : 1), pitch(many ? p.padded : min(p.padded, int64_t(FEW))) {
+    __device__ __forceinline__ Partials(const Loss& p, bool many) : tiles(many ? (p.vocab + TILE - 1) / TILE : (p.vocab + p.few_width - 1) / p.few_width), group(many ? p.group : 1), pitch(many ? p.padded : p.few_rows) {
         groups = (tiles + group - 1) / group;
     }
 };
@@ -468,6 +470,8 @@ struct Gradient {
     int64_t first, columns;     // of the piece (columns a multiple of TILE)
     float* parts;               // of dx, [splits][rows that count, rounded up to tiles][part_pitch]
     int64_t part_pitch;
+    float* dw_parts;            // of dW, where its tiles' contraction is split: [dw_splits][vocabulary][part_pitch]
+    int64_t dw_splits;
     // Where every row has a gradient g of its own, it goes into D (g <- g / common), in float16 without its power of two, which the row itself takes (x <- x shift).
     char* shifted;              // gathered rows times shift; the gathered rows themselves otherwise
     float *scale, *share, *shift, *common;      // inverse times g; g; 1 but in float16; a power of two
@@ -629,13 +633,35 @@ struct Shares {
     __device__ __forceinline__ Shares(const Loss& p, const Gradient& g, int n, int64_t blocks, int width) {
         // (Up to 192 rows in 16 bits the product waits for the weights whatever its tiles' height, and low ones make fewer parts to be added up: 154 x 768, tiles of 256 rows 56 + 27 us, of
         // 64 57 + 10.)
-        height = DT == TDB_F32 ? tile_rows<DT>(n, 64, 1, 1) : n <= 192 ? 64 : tile_rows<DT>(n, 128, 1, 1);
+        height = DT == TDB_F32 ? tile_rows<DT>(n, 64, 1, 1, FEW) : n <= 192 ? 64 : tile_rows<DT>(n, 128, 1, 1, FEW);
         if (height == 64 && width == 192) width = 256;
         row_tiles = (n + height - 1) / height, column_tiles = (p.hidden + width - 1) / width;
         const int64_t tiles = row_tiles * column_tiles;
         splits = tiles ? max(int64_t(1), min(blocks / tiles, g.columns * int64_t(sizeof(typename Matrix<DT>::T)) / 128)) : 0;
     }
 };
+
+// A tile's part of a sum, in float32, to the rows that there are; more: added to what is there.
+template <int DT, class P>
+__device__ __forceinline__ void store_part(const typename P::Acc& acc, float* parts, int64_t pitch, int64_t m0, int64_t n0, int64_t rows, bool more) {
+    using M = Matrix<DT>;
+#pragma unroll
+    for (int i = 0; i < P::TM; ++i) {
+        const int64_t m = m0 + P::wave_m() + i * M::SIDE + lane_m<DT>();
+        float* const to = parts + m * pitch;
+#pragma unroll
+        for (int j = 0; j < P::TN; ++j)
+#pragma unroll
+            for (int q = 0; q < M::QUADS; ++q) {
+                const int64_t c = n0 + P::wave_n() + j * M::SIDE + quad_n<DT>(q);
+                if (m < rows && c < pitch) {
+                    f32x4 v = P::quad(acc, i, j, q);
+                    if (more) v += *reinterpret_cast<const f32x4*>(to + c);
+                    *reinterpret_cast<f32x4*>(to + c) = v;
+                }
+            }
+    }
+}
 
 // Parts of dx: D W over a share of the piece's columns.
 template <int DT, class P>
@@ -651,22 +677,7 @@ __device__ __forceinline__ void dx_body(const Loss& p, const Gradient& g, int n,
         const int64_t m0 = row * P::BM, n0 = column * P::BN;
         typename P::Acc acc;
         P::run(flow, {m0, n0, steps * split / share.splits, steps * (split + 1) / share.splits}, acc, P::ZEROS);
-#pragma unroll
-        for (int i = 0; i < P::TM; ++i) {
-            const int64_t m = m0 + P::wave_m() + i * M::SIDE + lane_m<DT>();
-            float* const to = g.parts + (split * share.row_tiles * P::BM + m) * g.part_pitch;
-#pragma unroll
-            for (int j = 0; j < P::TN; ++j)
-#pragma unroll
-                for (int q = 0; q < M::QUADS; ++q) {
-                    const int64_t c = n0 + P::wave_n() + j * M::SIDE + quad_n<DT>(q);
-                    if (m < n && c < g.part_pitch) {
-                        f32x4 v = P::quad(acc, i, j, q);
-                        if (g.later) v += *reinterpret_cast<const f32x4*>(to + c);
-                        *reinterpret_cast<f32x4*>(to + c) = v;
-                    }
-                }
-        }
+        store_part<DT, P>(acc, g.parts + split * share.row_tiles * P::BM * g.part_pitch, g.part_pitch, m0, n0, n, g.later);
     }
 }
 
@@ -804,25 +815,26 @@ __global__ __launch_bounds__(512, 2) void loss_dweight_kernel(Loss p, Gradient g
     using T = typename Matrix<DT>::T;
     constexpr int BM = P::BM;
     const int n = p.count[0];
-    const int64_t columns = min(g.columns, p.vocab - g.first), row_tiles = (columns + BM - 1) / BM, column_tiles = g.dweight ? (p.hidden + BN - 1) / BN : 1, all = row_tiles * column_tiles;
+    const int64_t columns = min(g.columns, p.vocab - g.first), row_tiles = (columns + BM - 1) / BM, column_tiles = g.dweight ? (p.hidden + BN - 1) / BN : 1, splits = g.dw_splits, all = row_tiles * column_tiles * splits;
     const int64_t steps = (n + P::STEP - 1) / P::STEP;
     const Rows a{g.d, g.d_pitch, n, uint32_t(g.d_pitch)}, b{g.shifted, p.pitch, n, uint32_t(p.pitch)};
     typename P::Flow flow(smem, a, b);
     const int heights = n ? (n + p.template rows_of<DT>(n) - 1) / p.template rows_of<DT>(n) : 0;
     const float factor = n == 0 ? 0.f : (p.reduction ? row_factor(p, g, n) : *g.common) * (1.f / D_SCALE<DT>);
-    auto tile = [&](int64_t block) {
-        int64_t row, column, split;
-        tile_of(block < all ? block : 0, row_tiles, column_tiles, 1, row, column, split);
-        return typename P::Tile{row * BM, column * BN, 0, steps};
+    int64_t split, next_split;
+    auto tile = [&](int64_t block, int64_t& part) {
+        int64_t row, column;
+        tile_of(block < all ? block : 0, row_tiles, column_tiles, splits, row, column, part);
+        return typename P::Tile{row * BM, column * BN, steps * part / splits, steps * (part + 1) / splits};
     };
     if (blockIdx.x >= all) return;
-    typename P::Tile now = tile(blockIdx.x);
+    typename P::Tile now = tile(blockIdx.x, split);
     typename P::Alone alone;
     if (g.dweight) P::open(flow, now, alone);
     int stage = 0;
     for (int64_t block = blockIdx.x; block < all; block += gridDim.x) {
-        const typename P::Tile next = tile(block + gridDim.x);
-        if (const int64_t m = now.m0 + threadIdx.x; g.dbias && now.n0 == 0 && threadIdx.x < BM && m < columns) {
+        const typename P::Tile next = tile(block + gridDim.x, next_split);
+        if (const int64_t m = now.m0 + threadIdx.x; g.dbias && now.n0 == 0 && split == 0 && threadIdx.x < BM && m < columns) {
             float sum = 0.f;
             for (int t = 0; t < heights; ++t) sum += g.column_sums[t * g.columns + m];
             if (p.bias_kind == 2) static_cast<float*>(g.dbias)[g.first + m] = sum * factor;
@@ -830,8 +842,9 @@ __global__ __launch_bounds__(512, 2) void loss_dweight_kernel(Loss p, Gradient g
         }
         if (g.dweight) {
             typename P::Acc acc;
-            P::template run_on<P::STORES>(flow, now, next, block + gridDim.x < all, stage, !g.wide_dweight || block == blockIdx.x, acc, P::ZEROS, alone);
-            P::store(
+            P::template run_on<P::STORES>(flow, now, next, block + gridDim.x < all, stage, !g.wide_dweight || splits > 1 || block == blockIdx.x, acc, P::ZEROS, alone);
+            if (splits > 1) store_part<DT, P>(acc, g.dw_parts + split * p.dw_rows() * g.part_pitch, g.part_pitch, now.m0, now.n0, columns, false);
+            else P::store(
                 P::scratch(smem, stage), g.dweight + (g.first + now.m0) * g.dweight_pitch + now.n0 * int64_t(sizeof(T)), g.dweight_pitch, columns - now.m0, p.hidden - now.n0, g.wide_dweight,
                 [&](int i, int j, int q) {
                     f32x4 v = P::quad(acc, i, j, q);
@@ -841,7 +854,25 @@ __global__ __launch_bounds__(512, 2) void loss_dweight_kernel(Loss p, Gradient g
                 },
                 [](int, char*) {});
         }
-        now = next;
+        now = next, split = next_split;
+    }
+}
+// dW of parts.
+template <int DT>
+__global__ __launch_bounds__(256) void loss_dweight_sum_kernel(Loss p, Gradient g) {
+    using T = typename Matrix<DT>::T;
+    const int n = p.count[0];
+    const float factor = n == 0 ? 0.f : (p.reduction ? row_factor(p, g, n) : *g.common) * (1.f / D_SCALE<DT>);
+    const int64_t quads = g.part_pitch / 4, apart = p.dw_rows() * g.part_pitch;
+    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < p.vocab * quads; i += int64_t(gridDim.x) * 256) {
+        const int64_t v = i / quads;
+        const int c = int(i - v * quads) * 4;
+        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+        for (int64_t s = 0; s < g.dw_splits; ++s) sum += *reinterpret_cast<const f32x4*>(g.dw_parts + s * apart + i * 4);
+        T* const to = reinterpret_cast<T*>(g.dweight + v * g.dweight_pitch) + c;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (c + e < p.hidden) to[e] = T(sum[e] * factor);
     }
 }
 
@@ -849,6 +880,7 @@ __global__ __launch_bounds__(512, 2) void loss_dweight_kernel(Loss p, Gradient g
 
 constexpr int64_t D_BYTES = int64_t(1) << 31;       // of the workspace that holds D, unless 256 columns take more
 constexpr int64_t PARTIAL_BYTES = int64_t(1) << 27;
+constexpr int64_t SPLIT_ROWS = 512;
 
 int64_t round_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 
@@ -870,13 +902,15 @@ struct Plan {
     int size;                               // of a value
     int64_t padded, pitch, vocab;           // rows and bytes of the gathered rows, vocabulary, rounded up
     int32_t group, few_width, dx_width, dw_width;       // columns of the tiles of few rows' logits, dx and dW
+    int32_t dw_splits;                      // workgroups that share the contraction of a tile of dW
+    int64_t few_rows;
     bool many, few;                         // whether there may be as many or as few rows as the kernels are for
     int64_t columns;                        // of a piece
     int blocks, finish_blocks;
     // offsets
     int64_t index, place, label, top, inverse, right, biases, gathered, state;
     int64_t maxima, sums, block_sums, forward;
-    int64_t d, parts, part_pitch, column_sums, shifted, scale, share, shift, common, backward;
+    int64_t d, parts, part_pitch, column_sums, dw_parts, shifted, scale, share, shift, common, backward;
 };
 
 Plan plan_of(const tdb_loss_args& a) {
@@ -895,7 +929,13 @@ Plan plan_of(const tdb_loss_args& a) {
     // 37 + 39 and 27 + 29 us; 42, 73329, 928 148 + 145 and 125 + 125; 16, 128100, 1232 187 + 138 and 201 + 163.  (In 16 bits tiles of 128 are no faster: 20, 73329, 768 27 + 29 and 28 + 30.)
     auto rounds = [&](int64_t tiles) { return (tiles + p.blocks - 1) / p.blocks; };
     p.few_width = a.dtype == TDB_F32 && a.rows <= 128 && rounds(2 * wide) < 2 * rounds(wide) ? 128 : 256;
+    p.few_rows = p.padded / TILE * wide <= 2 * p.blocks ? p.padded : std::min<int64_t>(p.padded, FEW);
     p.dx_width = tile_columns(a.hidden, a.dtype, 0, p.blocks), p.dw_width = tile_columns(a.hidden, a.dtype, p.columns / TILE, p.blocks);
+    // A small vocabulary's dW has few tiles: where half of the CUs would have none, several share a tile's rows, SPLIT_ROWS of them at least, and their parts are added up.  4199 rows, 2010 classes,
+    // 1024 columns of float32: 159 + 15 us instead of 537.
+    p.dw_splits = 1;
+    if (const int64_t tiles = p.columns / TILE * ((a.hidden + p.dx_width - 1) / p.dx_width), splits = std::min(p.blocks / tiles, a.rows / SPLIT_ROWS); p.columns == p.vocab && splits > 1)
+        p.dw_splits = int32_t(splits), p.dw_width = p.dx_width;
     p.finish_blocks = int(std::min<int64_t>((std::max<int64_t>(a.rows, 1) + FINISH_ROWS - 1) / FINISH_ROWS, 256));
     int64_t at = 256;
     auto take = [&](int64_t bytes) {
@@ -907,7 +947,7 @@ Plan plan_of(const tdb_loss_args& a) {
     p.gathered = take(p.padded * p.pitch);
     p.state = at;
     at = 0;
-    const int64_t partials = std::max((wide + p.group - 1) / p.group * p.padded, p.vocab / p.few_width * std::min<int64_t>(p.padded, FEW)) * 4;
+    const int64_t partials = std::max((wide + p.group - 1) / p.group * p.padded, p.vocab / p.few_width * p.few_rows) * 4;
     p.maxima = take(partials), p.sums = take(partials), p.block_sums = take(p.finish_blocks * 8);
     p.forward = at;
     at = 0;
@@ -915,7 +955,8 @@ Plan plan_of(const tdb_loss_args& a) {
     // As many parts of dx as workgroups share its tiles, or one.
     p.d = take(p.padded * p.columns * p.size);
     p.parts = take(std::max(p.padded, int64_t(p.blocks) * TILE) * std::max<int64_t>(p.part_pitch, 1) * 4);
-    p.column_sums = take(std::max<int64_t>(p.padded / TILE, std::min<int64_t>(p.padded, FEW) / 32) * p.columns * 4);
+    p.column_sums = take(std::max<int64_t>(p.padded / TILE, p.few_rows / 32) * p.columns * 4);
+    p.dw_parts = take(p.dw_splits > 1 ? p.dw_splits * p.vocab * p.part_pitch * 4 : 0);
     const bool weighted = a.reduction == 0;
     p.shifted = take(weighted && a.dtype == TDB_F16 ? p.padded * p.pitch : 0);
     p.scale = take(weighted ? p.padded * 4 : 0), p.share = take(weighted ? p.padded * 4 : 0), p.shift = take(weighted ? p.padded * 4 : 0), p.common = take(4);
@@ -965,7 +1006,7 @@ Loss loss_of(const tdb_loss_args& a, const Plan& p) {
     k.hidden = a.hidden, k.reduction = a.reduction, k.bias_kind = !a.bias ? 0 : a.bias_dtype == a.dtype ? 1 : 2, k.loss = a.loss;
     k.count = reinterpret_cast<int32_t*>(state), k.index = reinterpret_cast<int32_t*>(state + p.index), k.place = reinterpret_cast<int32_t*>(state + p.place);
     k.label = reinterpret_cast<int32_t*>(state + p.label), k.top = reinterpret_cast<float*>(state + p.top), k.inverse = reinterpret_cast<float*>(state + p.inverse);
-    k.biases = reinterpret_cast<float*>(state + p.biases), k.gathered = state + p.gathered, k.pitch = p.pitch, k.padded = p.padded, k.group = p.group, k.few_width = p.few_width, k.blocks = p.blocks;
+    k.biases = reinterpret_cast<float*>(state + p.biases), k.gathered = state + p.gathered, k.pitch = p.pitch, k.padded = p.padded, k.group = p.group, k.few_width = p.few_width, k.blocks = p.blocks, k.few_rows = p.few_rows;
     k.right = reinterpret_cast<float*>(state + p.right), k.maxima = reinterpret_cast<float*>(work + p.maxima), k.sums = reinterpret_cast<float*>(work + p.sums);
     k.block_sums = reinterpret_cast<double*>(work + p.block_sums);
     return k;
@@ -1024,7 +1065,7 @@ hipError_t backward(const tdb_loss_args& a, hipStream_t s) {
     const bool weighted = a.reduction == 0;
     auto floats = [&](int64_t at) { return reinterpret_cast<float*>(work + at); };
     g.shifted = weighted && a.dtype == TDB_F16 ? work + p.shifted : k.gathered;
-    g.scale = floats(p.scale), g.share = floats(p.share), g.shift = floats(p.shift), g.common = floats(p.common), g.column_sums = floats(p.column_sums);
+    g.scale = floats(p.scale), g.share = floats(p.share), g.shift = floats(p.shift), g.common = floats(p.common), g.column_sums = floats(p.column_sums), g.dw_parts = floats(p.dw_parts), g.dw_splits = a.dweight ? p.dw_splits : 1;
     g.wide_dweight = reinterpret_cast<uintptr_t>(a.dweight) % 4 == 0 && g.dweight_pitch % 4 == 0;
     if (weighted && a.rows) TDB_TRY(launch<loss_weigh_kernel<DT>>(std::min<int64_t>(p.padded / 16, 1024), 256, 0, s, k, g));
     for (g.first = 0; g.first < a.vocab; g.first += p.columns) {
@@ -1045,6 +1086,7 @@ hipError_t backward(const tdb_loss_args& a, hipStream_t s) {
             if (p.dw_width == 256) TDB_TRY(launch<loss_dweight_kernel<DT, 256>>(p.blocks, 512, Dweight<DT, 256>::SHARED, s, k, g));
             else if (p.dw_width == 192) TDB_TRY(launch<loss_dweight_kernel<DT, 192>>(p.blocks, 512, Dweight<DT, 192>::SHARED, s, k, g));
             else TDB_TRY(launch<loss_dweight_kernel<DT, 128>>(p.blocks, 512, Dweight<DT, 128>::SHARED, s, k, g));
+            if (g.dw_splits > 1) TDB_TRY(launch<loss_dweight_sum_kernel<DT>>(std::min<int64_t>((a.vocab * (p.part_pitch / 4) + 255) / 256, 4096), 256, 0, s, k, g));
         }
     }
     if (a.rows && a.dx) {

@@ -313,11 +313,11 @@ struct Product {
         if (LATER == 0 || first) wait_loads<0>();
         else wait_loads<LATER>();
         step_barrier();
-        if (steps == 1) go_on();
-        if (steps) flow.load(stage ^ 1);
+        if (steps <= 1) go_on();
+        flow.load(stage ^ 1);
         begin_sums(acc, start);
         if (steps == 0) {
-            if (more) beside.load(next);
+            stage ^= 1;
         } else if constexpr (DT == TDB_F32) {
             for (int s = 0; s < steps; ++s) {
                 if (s) {
