@@ -250,6 +250,15 @@ def test_weights_among_other_values(dtype, hidden, rows):
     assert torch.equal(got[0], want[0]) and all(torch.equal(want[1][k], got[1][k]) for k in want[1])
 
 
+@pytest.mark.parametrize("hidden", [6, 7])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_one_class_of_many(dtype, hidden):
+    """A single row of a matrix whose rows lie an odd number of values or very far apart."""
+    x, _, labels, _ = _inputs(20, hidden, 1, dtype)
+    for apart in (hidden + 2, hidden + 3, (1 << 22) + 1):
+        _check(x, torch.as_strided(_rand(2, hidden + 9, dtype=dtype), (1, hidden), (apart, 1)), labels, None, "sum")
+
+
 def test_only_some_gradients():
     x, w, labels, b = _inputs(90, 96, 500, torch.bfloat16, 0.8)
     _, full = _step(x, w, labels, b, "mean")

@@ -27,16 +27,17 @@ constexpr int FEW = 1024;           // rows up to which tiles may be lower than 
 // 414 for 128, 336 for 96, 240 for 64, 135 for 32: 96 rows 382 us in one tile and 529 in two of 64, 160 rows 524 in one and 667 in five of 32.  Where tiles are few, low ones share out better:
 // 141 rows, 18134 classes, 704 columns of bfloat16 take 51 us in 71 tiles of 256 rows and 31 in 213 of 64.  (No tiles past the rows' multiple of 256, which the buffers have.)
 template <int DT>
-__host__ __device__ constexpr int tile_rows(int n, int least, int64_t wide, int blocks, int64_t few) {
+__device__ __forceinline__ int tile_rows(int n, int least, uint32_t wide, uint32_t blocks, int64_t few) {
     if (n > few) return TILE;
-    const int rows = (n + TILE - 1) / TILE;
+    auto cost = [&](int h, int dear) { return float((uint32_t(n + h - 1) / uint32_t(h) * wide + blocks - 1) / blocks) * float(h * dear); };
+    constexpr int HEIGHTS[] = {160, 128, 96, 64, 32}, DEAR[] = {DT == TDB_F32 ? 34 : 0, DT == TDB_F32 ? 35 : 40, DT == TDB_F32 ? 37 : 0, DT == TDB_F32 ? 40 : 52, DT == TDB_F32 ? 45 : 64};
     int best = TILE;
-    int64_t cost = (rows * wide + blocks - 1) / blocks * (TILE * 32);
-    const int heights[] = {160, 128, 96, 64, 32}, dear[] = {DT == TDB_F32 ? 34 : 64, DT == TDB_F32 ? 35 : 40, DT == TDB_F32 ? 37 : 64, DT == TDB_F32 ? 40 : 52, DT == TDB_F32 ? 45 : 64};
+    float least_cost = cost(TILE, 32);
+#pragma unroll
     for (int i = 0; i < 5; ++i) {
-        const int h = heights[i], high = (n + h - 1) / h;
-        const int64_t c = (high * wide + blocks - 1) / blocks * (h * dear[i]);
-        if (h >= least && high * h <= rows * TILE && c < cost && (DT == TDB_F32 || (h & (h - 1)) == 0)) best = h, cost = c;
+        const int h = HEIGHTS[i];
+        const float c = cost(h, DEAR[i]);
+        if (DEAR[i] && h >= least && (n + h - 1) / h * h <= (n + TILE - 1) / TILE * TILE && c < least_cost) best = h, least_cost = c;
     }
     return best;
 }
@@ -67,7 +68,7 @@ struct Loss {
     int64_t few_rows;                           // rows up to which tiles may be lower than 256
     __device__ __forceinline__ int64_t dw_rows() const { return (vocab + TILE - 1) / TILE * TILE; }
     template <int DT>
-    __device__ __forceinline__ int rows_of(int n) const { return tile_rows<DT>(n, 32, (vocab + few_width - 1) / few_width, blocks, few_rows); }       // of a tile of logits
+    __device__ __forceinline__ int rows_of(int n) const { return tile_rows<DT>(n, 32, uint32_t(vocab + few_width - 1) / uint32_t(few_width), blocks, few_rows); }       // of a tile of logits
 };
 
 // How the logits' maxima and sums lie: groups of column tiles, rows `pitch` to each.
@@ -368,8 +369,8 @@ __global__ __launch_bounds__((Few<DT, BN>::THREADS), 2) void loss_logits_few_ker
     using F = Few<DT, BN>;
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     __shared__ __attribute__((aligned(16))) float s_bias[BN];
-    __shared__ int32_t s_label[192];
-    __shared__ float s_top[1024], s_sum[1024];
+    __shared__ int32_t s_label[160];
+    __shared__ float s_top[640], s_sum[640];
     const int n = p.count[0];
     const int height = p.template rows_of<DT>(n);
     if constexpr (DT == TDB_F32) {
@@ -548,7 +549,7 @@ __device__ __forceinline__ void difference_of(const Loss& p, const Gradient& g, 
 
 // D of a piece of the vocabulary.
 template <int DT, class P, bool WEIGHTED>
-__device__ __forceinline__ void difference_body(const Loss& p, const Gradient& g, int n, char* smem, float* s_bias, float (&s_rows)[6][192], float* s_column) {
+__device__ __forceinline__ void difference_body(const Loss& p, const Gradient& g, int n, char* smem, float* s_bias, float (&s_rows)[6][160], float* s_column) {
     typename P::Flow flow(smem, hidden_rows<DT>(p, n), weight_rows<DT>(p));
     const int64_t row_tiles = (n + P::BM - 1) / P::BM, column_tiles = g.columns / P::BN, all = row_tiles * column_tiles;
     for (int64_t block = blockIdx.x; block < all; block += gridDim.x) {
@@ -610,7 +611,7 @@ __global__ __launch_bounds__((Few<DT, BN>::THREADS), 2) void loss_difference_few
     using F = Few<DT, BN>;
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     __shared__ __attribute__((aligned(16))) float s_bias[BN];
-    __shared__ float s_column[2 * BN], s_rows[6][192];
+    __shared__ float s_column[2 * BN], s_rows[6][160];
     const int n = p.count[0];
     const int height = p.template rows_of<DT>(n);
     if constexpr (DT == TDB_F32) {

@@ -37,7 +37,7 @@ def _arguments(weight, bias, rows, hidden, ignore_index, reduction) -> _lib.Loss
     a = _lib.LossArgs()
     a.dtype, a.bias_dtype = L.dtype_code(weight), L.dtype_code(weight if bias is None else bias)
     a.hidden, a.reduction, a.rows, a.vocab, a.ignore_index = hidden, reduction, rows, weight.shape[0], ignore_index
-    a.weight, a.weight_stride, a.bias = weight.data_ptr(), max(weight.stride(0), hidden), None if bias is None else bias.data_ptr()
+    a.weight, a.weight_stride, a.bias = weight.data_ptr(), hidden + 3 & ~3 if weight.shape[0] == 1 else weight.stride(0), None if bias is None else bias.data_ptr()
     return a
 
 
