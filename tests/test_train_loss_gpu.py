@@ -259,6 +259,34 @@ def test_one_class_of_many(dtype, hidden):
         _check(x, torch.as_strided(_rand(2, hidden + 9, dtype=dtype), (1, hidden), (apart, 1)), labels, None, "sum")
 
 
+@pytest.mark.parametrize("rows,hidden,vocab", [(5, 32768, 300), (140, 32767, 70), (300, 20000, 300), (3, 4, 1 << 20), (1030, 2, 1 << 17)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_extreme_shapes(dtype, rows, hidden, vocab):
+    x, w, labels, b = _inputs(rows, hidden, vocab, dtype, 0.9)
+    if rows * vocab < 1 << 24:
+        _check(x, w, labels, b)
+        return
+    loss, grads = _step(x, w, labels, b, "sum")         # (64 bits of 10^8 logits: some of the rows by themselves, and what all of them add up to)
+    each, _ = _step(x, w, labels, b, "none", torch.ones(rows, device="cuda"))
+    few = R.loss(x[:50], w, labels[:50], b, IGNORED, "none", None, x.dtype)
+    R.check("loss", each[:50], *few["loss"])
+    R.check("dx", grads["dx"][:50], *few["dx"])
+    assert torch.isclose(loss.double(), each.double().sum(), rtol=1e-6)
+
+
+def test_backward_twice():
+    """What is kept for the backward pass is not used up by it."""
+    for dtype, reduction in ((torch.float16, "none"), (torch.bfloat16, "mean"), (torch.float32, "sum")):
+        x, w, labels, b = _inputs(150, 72, 700, dtype, 0.8)
+        leaves = [t.requires_grad_() for t in (x, w, b)]
+        loss = linear_cross_entropy(x, w, labels, b, reduction=reduction)
+        weight = torch.ones_like(loss)
+        first = torch.autograd.grad(loss, leaves, weight, retain_graph=True)
+        torch.autograd.grad(loss, leaves, 3 * weight, retain_graph=True)
+        again = torch.autograd.grad(loss, leaves, weight)
+        assert all(torch.equal(p, q) for p, q in zip(first, again))
+
+
 def test_only_some_gradients():
     x, w, labels, b = _inputs(90, 96, 500, torch.bfloat16, 0.8)
     _, full = _step(x, w, labels, b, "mean")
