@@ -108,7 +108,7 @@ int64_t tdb_attn_train_workspace(const tdb_train_attn_args* args);
  * weight: rows 4-byte aligned (so of an even stride in 16 bits) and at most 4 MiB apart.  x: rows of any stride, aligned to their values.
  * Forward fills `state` (tdb_loss_state() bytes), which the backward call reads; x is not read again.  Both take a workspace of tdb_loss_workspace() bytes, 16-byte aligned like
  * the state.  The backward one holds the gradient of the logits in the type of x, up to 2 GiB at a time or 256 columns of it, partial sums of dx of 1 KiB hidden for each CU or 4
- * bytes for each value of x, those of dweight of at most 256 KiB for each CU where a small vocabulary meets many rows, and without a reduction one more x.
+ * bytes for each value of x, those of dweight of at most 256 MiB where a small vocabulary meets many rows, and without a reduction one more x.
  * Backward: dx, dweight, dbias (of bias_dtype); NULL: not wanted.  dloss: of the sum or mean one float32, without reduction one for each row, dloss_stride apart.
  * Rows of dx that do not count are zeros.  Everything is added up in a fixed order.
  */

@@ -881,29 +881,44 @@ __global__ __launch_bounds__(256) void loss_dweight_sum_kernel(Loss p, Gradient 
 
 constexpr int64_t D_BYTES = int64_t(1) << 31;       // of the workspace that holds D, unless 256 columns take more
 constexpr int64_t PARTIAL_BYTES = int64_t(1) << 27;
-constexpr int64_t SPLIT_ROWS = 512;
+constexpr int64_t SPLIT_ROWS = 512, PART_BYTES = int64_t(1) << 28;
 
 int64_t round_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 
-// The width of tiles of dx or dW: that of the least work of a workgroup, tiles at their price for each column.  tiles_high: of dW, whose tiles are dealt out whole; dx is split along its
-// contraction (0).  dx and dW of 2500 x 768, 128100 classes, in tiles of 256, 192 and 128 columns: bfloat16 926, 1044 and 1269 us, float32 7.37, 7.57 and 7.70 ms; 384 wide 649, 575 and
-// 704 us, 4.92, 3.79 and 3.86 ms.
-int tile_columns(int hidden, int dtype, int64_t tiles_high, int blocks) {
-    const int widths[] = {256, 192, 128}, dear[] = {64, dtype == TDB_F32 ? 66 : 72, dtype == TDB_F32 ? 67 : 88};
-    int best = 256;
-    int64_t least = INT64_MAX;
+constexpr int WIDTHS[] = {256, 192, 128};
+constexpr int dear(int dtype, int i) { return i == 0 ? 64 : dtype == TDB_F32 ? i == 1 ? 66 : 67 : i == 1 ? 72 : 88; }        // what a column of such tiles costs
+
+// The width of tiles of dx, which is split along its contraction: that of the least work, tiles at their price for each column.  dx and dW of 2500 x 768, 128100 classes, in tiles of 256, 192 and
+// 128 columns: bfloat16 926, 1044 and 1269 us, float32 7.37, 7.57 and 7.70 ms; 384 wide 649, 575 and 704 us, 4.92, 3.79 and 3.86 ms.
+int dx_columns(int hidden, int dtype) {
+    int best = 0;
+    auto cost = [&](int i) { return (hidden + WIDTHS[i] - 1) / WIDTHS[i] * WIDTHS[i] * dear(dtype, i); };
+    for (int i = 1; i < 3; ++i)
+        if (cost(i) < cost(best)) best = i;
+    return WIDTHS[best];
+}
+
+// The width of tiles of dW, `high` of them below each other, and how many workgroups share the rows of each, SPLIT_ROWS of them at least: the least work of the busiest workgroup.  Parts are
+// written and read: of half of the rows' products 1 / 216 for each 1 / rows in float32, 1 / 1666 in 16 bits, and PART_BYTES hold them.  4199 rows, 2010 classes, 1024 columns of float32 whole and
+// by eight workgroups 537 and 159 + 15 us; 16055, 5157, 816 2030 and, by five, 1254 + 23.
+void dweight_tiles(int hidden, int dtype, int64_t high, int64_t rows, bool whole, int blocks, int32_t& width, int32_t& splits) {
+    double least = 0.0;
+    width = 0;
     for (int i = 0; i < 3; ++i) {
-        const int64_t wide = (hidden + widths[i] - 1) / widths[i], rounds = tiles_high ? (tiles_high * wide + blocks - 1) / blocks : wide;
-        if (const int64_t c = rounds * widths[i] * dear[i]; c < least) best = widths[i], least = c;
+        const int64_t tiles = high * ((hidden + WIDTHS[i] - 1) / WIDTHS[i]);
+        for (int64_t s = 1; s == 1 || (!whole && s <= 16 && s * SPLIT_ROWS <= rows && s * high * TILE * hidden * 4 <= PART_BYTES); ++s) {
+            const double part = s == 1 ? 0.0 : double(s) * (dtype == TDB_F32 ? 216 : 1666) / double(rows) * double(high * hidden * 64) / blocks;
+            const double cost = double((tiles * s + blocks - 1) / blocks) / double(s) * WIDTHS[i] * dear(dtype, i) + part;
+            if (!width || cost < least) least = cost, width = WIDTHS[i], splits = int32_t(s);
+        }
     }
-    return best;
 }
 
 struct Plan {
     int size;                               // of a value
     int64_t padded, pitch, vocab;           // rows and bytes of the gathered rows, vocabulary, rounded up
     int32_t group, few_width, dx_width, dw_width;       // columns of the tiles of few rows' logits, dx and dW
-    int32_t dw_splits;                      // workgroups that share the contraction of a tile of dW
+    int32_t dw_splits;                      // workgroups that share the rows of a tile of dW
     int64_t few_rows;
     bool many, few;                         // whether there may be as many or as few rows as the kernels are for
     int64_t columns;                        // of a piece
@@ -931,12 +946,8 @@ Plan plan_of(const tdb_loss_args& a) {
     auto rounds = [&](int64_t tiles) { return (tiles + p.blocks - 1) / p.blocks; };
     p.few_width = a.dtype == TDB_F32 && a.rows <= 128 && rounds(2 * wide) < 2 * rounds(wide) ? 128 : 256;
     p.few_rows = p.padded / TILE * wide <= 2 * p.blocks ? p.padded : std::min<int64_t>(p.padded, FEW);
-    p.dx_width = tile_columns(a.hidden, a.dtype, 0, p.blocks), p.dw_width = tile_columns(a.hidden, a.dtype, p.columns / TILE, p.blocks);
-    // A small vocabulary's dW has few tiles: where half of the CUs would have none, several share a tile's rows, SPLIT_ROWS of them at least, and their parts are added up.  4199 rows, 2010 classes,
-    // 1024 columns of float32: 159 + 15 us instead of 537.
-    p.dw_splits = 1;
-    if (const int64_t tiles = p.columns / TILE * ((a.hidden + p.dx_width - 1) / p.dx_width), splits = std::min(p.blocks / tiles, a.rows / SPLIT_ROWS); p.columns == p.vocab && splits > 1)
-        p.dw_splits = int32_t(splits), p.dw_width = p.dx_width;
+    p.dx_width = dx_columns(a.hidden, a.dtype);
+    dweight_tiles(a.hidden, a.dtype, p.columns / TILE, a.rows, p.columns != p.vocab, p.blocks, p.dw_width, p.dw_splits);
     p.finish_blocks = int(std::min<int64_t>((std::max<int64_t>(a.rows, 1) + FINISH_ROWS - 1) / FINISH_ROWS, 256));
     int64_t at = 256;
     auto take = [&](int64_t bytes) {
