@@ -59,7 +59,7 @@ def test_sizes(rows, hidden, vocab, share, dtype):
 
 
 # every height of tiles, one and several of them, up to where the next one takes over
-@pytest.mark.parametrize("rows", [32, 60, 96, 97, 128, 160, 161, 192, 193, 257, 288, 320, 480, 481, 512, 760, 1024, 1025])
+@pytest.mark.parametrize("rows", [1, 16, 17, 32, 60, 96, 97, 128, 160, 161, 192, 193, 257, 288, 320, 480, 481, 512, 760, 1024, 1025])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_heights_of_tiles(dtype, rows):
     x, w, labels, b = _inputs(rows, 160, 900, dtype)

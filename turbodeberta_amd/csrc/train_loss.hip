@@ -24,20 +24,21 @@ constexpr int FEW = 1024;           // rows up to which tiles may be lower than 
 
 // Rows of a tile where n count: the height by which the busiest of `blocks` workgroups has least to do, tiles at their price; `wide` tiles lie beside each other.  16 bits, 128100 x 768: a tile's
 // logits and their gradient took 125 us for 256 rows, 70 to 77 for 128, 48 for 64, 31 for 32 (lower tiles load more for their products).  float32, bound by products, 765 for 256, 514 for 160,
-// 414 for 128, 336 for 96, 240 for 64, 135 for 32: 96 rows 382 us in one tile and 529 in two of 64, 160 rows 524 in one and 667 in five of 32.  Where tiles are few, low ones share out better:
+// 414 for 128, 336 for 96, 240 for 64, 135 for 32: 96 rows 382 us in one tile and 529 in two of 64, 160 rows 524 in one and 667 in five of 32; up to 16 rows have a tile
+// of their own: 1, 43175 x 1060, 67 + 56 us in 32 rows, 67 + 43 in 16.  Where tiles are few, low ones share out better:
 // 141 rows, 18134 classes, 704 columns of bfloat16 take 51 us in 71 tiles of 256 rows and 31 in 213 of 64.  (No tiles past the rows' multiple of 256, which the buffers have.)
 template <int DT>
 __device__ __forceinline__ int tile_rows(int n, int least, uint32_t wide, uint32_t blocks, int64_t few) {
     if (n > few) return TILE;
     auto cost = [&](int h, int dear) { return float((uint32_t(n + h - 1) / uint32_t(h) * wide + blocks - 1) / blocks) * float(h * dear); };
-    constexpr int HEIGHTS[] = {160, 128, 96, 64, 32}, DEAR[] = {DT == TDB_F32 ? 34 : 0, DT == TDB_F32 ? 35 : 40, DT == TDB_F32 ? 37 : 0, DT == TDB_F32 ? 40 : 52, DT == TDB_F32 ? 45 : 64};
+    constexpr int HEIGHTS[] = {160, 128, 96, 64, 32, 16}, DEAR[] = {DT == TDB_F32 ? 34 : 0, DT == TDB_F32 ? 35 : 40, DT == TDB_F32 ? 37 : 0, DT == TDB_F32 ? 40 : 52, DT == TDB_F32 ? 45 : 64, DT == TDB_F32 ? 60 : 0};
     int best = TILE;
     float least_cost = cost(TILE, 32);
 #pragma unroll
-    for (int i = 0; i < 5; ++i) {
+    for (int i = 0; i < 6; ++i) {
         const int h = HEIGHTS[i];
         const float c = cost(h, DEAR[i]);
-        if (DEAR[i] && h >= least && (n + h - 1) / h * h <= (n + TILE - 1) / TILE * TILE && c < least_cost) best = h, least_cost = c;
+        if (DEAR[i] && h >= least && (h > 16 || n <= 16) && (n + h - 1) / h * h <= (n + TILE - 1) / TILE * TILE && c < least_cost) best = h, least_cost = c;
     }
     return best;
 }
@@ -68,7 +69,7 @@ struct Loss {
     int64_t few_rows;                           // rows up to which tiles may be lower than 256
     __device__ __forceinline__ int64_t dw_rows() const { return (vocab + TILE - 1) / TILE * TILE; }
     template <int DT>
-    __device__ __forceinline__ int rows_of(int n) const { return tile_rows<DT>(n, 32, uint32_t(vocab + few_width - 1) / uint32_t(few_width), blocks, few_rows); }       // of a tile of logits
+    __device__ __forceinline__ int rows_of(int n) const { return tile_rows<DT>(n, 16, uint32_t(vocab + few_width - 1) / uint32_t(few_width), blocks, few_rows); }       // of a tile of logits
 };
 
 // How the logits' maxima and sums lie: groups of column tiles, rows `pitch` to each.
@@ -314,6 +315,7 @@ struct Few {
     using Logits128 = Product<DT, 128, BN, WM, 4, BN == 128 ? 2 : 3, false, false, LINE>;
     using Logits64 = Product<DT, 64, BN, WM, 4, 3, false, false, LINE>;
     using Logits32 = Product<DT, 32, BN, 1, WAVES, DT != TDB_F32 ? 4 : BN == 128 ? 3 : 2, false, false>;
+    using Logits16 = Product<DT, 16, BN, 1, WAVES, BN == 128 ? 3 : 2, false, false>;
     using Logits160 = Product<DT, 160, BN, WM, 4, 2, false, false, LINE>;       // (float32)
     using Logits96 = Product<DT, 96, BN, WM, 4, BN == 128 ? 2 : 3, false, false, LINE>;
     static constexpr int SHARED = std::max({Logits128::SHARED, Logits64::SHARED, Logits32::SHARED, DT == TDB_F32 ? Logits160::SHARED : 0, DT == TDB_F32 ? Logits96::SHARED : 0});
@@ -374,6 +376,7 @@ __global__ __launch_bounds__((Few<DT, BN>::THREADS), 2) void loss_logits_few_ker
     const int n = p.count[0];
     const int height = p.template rows_of<DT>(n);
     if constexpr (DT == TDB_F32) {
+        if (height == 16) return logits_body<DT, typename F::Logits16>(p, n, smem, s_bias, s_label, s_top, s_sum);
         if (height == 96) return logits_body<DT, typename F::Logits96>(p, n, smem, s_bias, s_label, s_top, s_sum);
         if constexpr (BN == 256)        // (the narrow tiles are for 128 rows at most)
             if (height == 160) return logits_body<DT, typename F::Logits160>(p, n, smem, s_bias, s_label, s_top, s_sum);
@@ -615,6 +618,7 @@ __global__ __launch_bounds__((Few<DT, BN>::THREADS), 2) void loss_difference_few
     const int n = p.count[0];
     const int height = p.template rows_of<DT>(n);
     if constexpr (DT == TDB_F32) {
+        if (height == 16) return difference_body<DT, typename F::Logits16, WEIGHTED>(p, g, n, smem, s_bias, s_rows, s_column);
         if (height == 96) return difference_body<DT, typename F::Logits96, WEIGHTED>(p, g, n, smem, s_bias, s_rows, s_column);
         if constexpr (BN == 256)        // (the narrow tiles are for 128 rows at most)
             if (height == 160) return difference_body<DT, typename F::Logits160, WEIGHTED>(p, g, n, smem, s_bias, s_rows, s_column);
@@ -634,8 +638,9 @@ struct Shares {
     __device__ __forceinline__ Shares(const Loss& p, const Gradient& g, int n, int64_t blocks, int width) {
         // (Up to 192 rows in 16 bits the product waits for the weights whatever its tiles' height, and low ones make fewer parts to be added up: 154 x 768, tiles of 256 rows 56 + 27 us, of
         // 64 57 + 10.)
-        height = DT == TDB_F32 ? tile_rows<DT>(n, 64, 1, 1, FEW) : n <= 192 ? 64 : tile_rows<DT>(n, 128, 1, 1, FEW);
-        if (height == 64 && width == 192) width = 256;
+        // float32 is bound by products: 8 rows, 128100 x 768, 121 us in 64 rows, 75 in 32.
+        height = DT == TDB_F32 ? tile_rows<DT>(n, 32, 1, 1, FEW) : n <= 192 ? 64 : tile_rows<DT>(n, 128, 1, 1, FEW);
+        if (height <= 64 && width == 192) width = 256;
         row_tiles = (n + height - 1) / height, column_tiles = (p.hidden + width - 1) / width;
         const int64_t tiles = row_tiles * column_tiles;
         splits = tiles ? max(int64_t(1), min(blocks / tiles, g.columns * int64_t(sizeof(typename Matrix<DT>::T)) / 128)) : 0;
@@ -692,9 +697,11 @@ using Dx64 = Product<DT, 64, BN == 192 ? 256 : BN, BN == 128 ? 2 : 1, BN == 128 
 template <int BN>
 using Dx160 = Product<TDB_F32, 160, BN, 2, 4, 2, false, true>;
 template <int BN>
+using Dx32 = Product<TDB_F32, 32, BN == 192 ? 256 : BN, 1, 8, 4, false, true>;
+template <int BN>
 using Dx96 = Product<TDB_F32, 96, BN, 2, 4, 3, false, true>;
 constexpr int DX_SHARED = Dx128<TDB_BF16, 256>::SHARED;
-static_assert(Dx256<TDB_BF16, 256>::SHARED <= DX_SHARED && Dx64<TDB_BF16, 256>::SHARED <= DX_SHARED && Dx160<256>::SHARED <= DX_SHARED && Dx96<256>::SHARED <= DX_SHARED, "");
+static_assert(Dx256<TDB_BF16, 256>::SHARED <= DX_SHARED && Dx64<TDB_BF16, 256>::SHARED <= DX_SHARED && Dx32<256>::SHARED <= DX_SHARED && Dx160<256>::SHARED <= DX_SHARED && Dx96<256>::SHARED <= DX_SHARED, "");
 
 template <int DT, int BN>
 __global__ __launch_bounds__(512, 2) void loss_dx_kernel(Loss p, Gradient g) {
@@ -702,6 +709,7 @@ __global__ __launch_bounds__(512, 2) void loss_dx_kernel(Loss p, Gradient g) {
     const int n = p.count[0];
     const Shares<DT> share(p, g, n, gridDim.x, BN);
     if constexpr (DT == TDB_F32) {
+        if (share.height == 32) return dx_body<DT, Dx32<BN>>(p, g, n, share, smem);
         if (share.height == 96) return dx_body<DT, Dx96<BN>>(p, g, n, share, smem);
         if (share.height == 160) return dx_body<DT, Dx160<BN>>(p, g, n, share, smem);
     }
@@ -941,7 +949,7 @@ Plan plan_of(const tdb_loss_args& a) {
     const int64_t most = std::min<int64_t>(std::max<int64_t>(D_BYTES / (p.padded * p.size) / TILE, 1), (int64_t(1) << 22) / p.size / TILE), pieces = (wide + most - 1) / most;
     p.columns = (wide + pieces - 1) / pieces * TILE;
     p.blocks = std::max(8, tdb_compute_units(-1) & -8);
-    // Few rows of float32: tiles of 128 columns where those share out better over the CUs.  The two passes over the weights in tiles of 256 and 128 columns: one row, 32510 classes, 768 columns
+    // Few rows of float32: tiles of 128 columns where those share out better over the CUs.  The two passes over the weights in tiles of 256 and 128 columns: one row (of 32), 32510 classes, 768 columns
     // 37 + 39 and 27 + 29 us; 42, 73329, 928 148 + 145 and 125 + 125; 16, 128100, 1232 187 + 138 and 201 + 163.  (In 16 bits tiles of 128 are no faster: 20, 73329, 768 27 + 29 and 28 + 30.)
     auto rounds = [&](int64_t tiles) { return (tiles + p.blocks - 1) / p.blocks; };
     p.few_width = a.dtype == TDB_F32 && a.rows <= 128 && rounds(2 * wide) < 2 * rounds(wide) ? 128 : 256;
