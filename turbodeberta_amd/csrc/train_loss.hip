@@ -817,14 +817,15 @@ __global__ __launch_bounds__(256) void loss_weigh_kernel(Loss p, Gradient g) {
 template <int DT, int BN>
 using Dweight = Product<DT, 256, BN, BN == 256 ? 2 : 4, BN == 256 ? 4 : 2, 2, true, true>;
 
-template <int DT, int BN>
+// (SPLIT, several workgroups to a tile's rows, as a kernel of its own: as an argument it cost the others 2 of 41 us at 7 rows, 128100 x 768.)
+template <int DT, int BN, bool SPLIT>
 __global__ __launch_bounds__(512, 2) void loss_dweight_kernel(Loss p, Gradient g) {
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     using P = Dweight<DT, BN>;
     using T = typename Matrix<DT>::T;
     constexpr int BM = P::BM;
     const int n = p.count[0];
-    const int64_t columns = min(g.columns, p.vocab - g.first), row_tiles = (columns + BM - 1) / BM, column_tiles = g.dweight ? (p.hidden + BN - 1) / BN : 1, splits = g.dw_splits, all = row_tiles * column_tiles * splits;
+    const int64_t columns = min(g.columns, p.vocab - g.first), row_tiles = (columns + BM - 1) / BM, column_tiles = g.dweight ? (p.hidden + BN - 1) / BN : 1, splits = SPLIT ? g.dw_splits : 1, all = row_tiles * column_tiles * splits;
     const int64_t steps = (n + P::STEP - 1) / P::STEP;
     const Rows a{g.d, g.d_pitch, n, uint32_t(g.d_pitch)}, b{g.shifted, p.pitch, n, uint32_t(p.pitch)};
     typename P::Flow flow(smem, a, b);
@@ -851,8 +852,8 @@ __global__ __launch_bounds__(512, 2) void loss_dweight_kernel(Loss p, Gradient g
         }
         if (g.dweight) {
             typename P::Acc acc;
-            P::template run_on<P::STORES>(flow, now, next, block + gridDim.x < all, stage, !g.wide_dweight || splits > 1 || block == blockIdx.x, acc, P::ZEROS, alone);
-            if (splits > 1) store_part<DT, P>(acc, g.dw_parts + split * p.dw_rows() * g.part_pitch, g.part_pitch, now.m0, now.n0, columns, false);
+            P::template run_on<P::STORES>(flow, now, next, block + gridDim.x < all, stage, SPLIT || !g.wide_dweight || block == blockIdx.x, acc, P::ZEROS, alone);
+            if constexpr (SPLIT) store_part<DT, P>(acc, g.dw_parts + split * p.dw_rows() * g.part_pitch, g.part_pitch, now.m0, now.n0, columns, false);
             else P::store(
                 P::scratch(smem, stage), g.dweight + (g.first + now.m0) * g.dweight_pitch + now.n0 * int64_t(sizeof(T)), g.dweight_pitch, columns - now.m0, p.hidden - now.n0, g.wide_dweight,
                 [&](int i, int j, int q) {
@@ -1103,9 +1104,14 @@ hipError_t backward(const tdb_loss_args& a, hipStream_t s) {
             else TDB_TRY(launch<loss_dx_kernel<DT, 128>>(p.blocks, 512, DX_SHARED, s, k, g));
         }
         if (a.dweight || a.dbias) {
-            if (p.dw_width == 256) TDB_TRY(launch<loss_dweight_kernel<DT, 256>>(p.blocks, 512, Dweight<DT, 256>::SHARED, s, k, g));
-            else if (p.dw_width == 192) TDB_TRY(launch<loss_dweight_kernel<DT, 192>>(p.blocks, 512, Dweight<DT, 192>::SHARED, s, k, g));
-            else TDB_TRY(launch<loss_dweight_kernel<DT, 128>>(p.blocks, 512, Dweight<DT, 128>::SHARED, s, k, g));
+            auto dweight = [&](auto width) {
+                constexpr int BN = width();
+                return g.dw_splits > 1 ? launch<loss_dweight_kernel<DT, BN, true>>(p.blocks, 512, Dweight<DT, BN>::SHARED, s, k, g)
+                                       : launch<loss_dweight_kernel<DT, BN, false>>(p.blocks, 512, Dweight<DT, BN>::SHARED, s, k, g);
+            };
+            if (p.dw_width == 256) TDB_TRY(dweight(std::integral_constant<int, 256>()));
+            else if (p.dw_width == 192) TDB_TRY(dweight(std::integral_constant<int, 192>()));
+            else TDB_TRY(dweight(std::integral_constant<int, 128>()));
             if (g.dw_splits > 1) TDB_TRY(launch<loss_dweight_sum_kernel<DT>>(std::min<int64_t>((a.vocab * (p.part_pitch / 4) + 255) / 256, 4096), 256, 0, s, k, g));
         }
     }
