@@ -71,8 +71,12 @@ def _clip(a: _lib.GradsArgs, out, max_norm: float, dev) -> None:
 
 def _scaled(grads, out, max_norm: float, norm: int, error_if_nonfinite: bool) -> torch.Tensor:
     """The norm; out = grads * factor.  What does not lie back to back, or not in the same order on both sides, goes through copies."""
-    flat = [t if _dense(t) and _dense(o) and t.stride() == o.stride() else t.contiguous() for t, o in zip(grads, out)]
-    to = [o if t is f and _dense(o) else o if o is not t and o.is_contiguous() else torch.empty(o.shape, dtype=o.dtype, device=o.device) for t, f, o in zip(grads, flat, out)]
+    flat, to = [], []
+    for t, o in zip(grads, out):
+        if _dense(t) and _dense(o) and t.stride() == o.stride():        # the same place in memory is the same value on both sides
+            flat.append(t), to.append(o)
+        else:                                                           # by way of contiguous ones, on either side that is not
+            flat.append(t.contiguous()), to.append(o if o is not t and o.is_contiguous() else torch.empty(o.shape, dtype=o.dtype, device=o.device))
     a, total, keep = _norm(flat, norm)
     if error_if_nonfinite and not bool(torch.isfinite(total)):
         raise RuntimeError(f"the norm of the gradients is {total.item()}: nothing is clipped")
