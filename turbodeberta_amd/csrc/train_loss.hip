@@ -80,13 +80,13 @@ struct Partials {
     }
 };
 
-// The bias of a class, -inf past the vocabulary.  Values beyond 2^126 become that: a mask of the type's lowest value stays a number when logits are subtracted and scaled.
+// The bias of a class, -inf past the vocabulary.  As it is, a mask of float32's lowest value among them: logits are subtracted before they are scaled to base 2, so a difference of two of them is 0, one from an
+// ordinary logit the mask itself, whose exponential is 0, and a label's loss there the mask's size.
 template <int DT>
 __device__ __forceinline__ float bias_of(const Loss& p, int64_t v) {
     if (v >= p.vocab) return -INFINITY;
     if (!p.bias_kind) return 0.f;
-    const float b = p.bias_kind == 2 ? static_cast<const float*>(p.bias)[v] : float(static_cast<const typename Matrix<DT>::T*>(p.bias)[v]);
-    return fabsf(b) == INFINITY ? b : b > 0x1p126f ? 0x1p126f : b < -0x1p126f ? -0x1p126f : b;      // (NaN stays)
+    return p.bias_kind == 2 ? static_cast<const float*>(p.bias)[v] : float(static_cast<const typename Matrix<DT>::T*>(p.bias)[v]);
 }
 
 template <int WAVES>
