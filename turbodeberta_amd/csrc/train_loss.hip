@@ -477,8 +477,9 @@ struct Gradient {
     float* dw_parts;            // of dW, where its tiles' contraction is split: [dw_splits][vocabulary][part_pitch]
     int64_t dw_splits;
     // Where every row has a gradient g of its own, it goes into D (g <- g / common), in float16 without its power of two, which the row itself takes (x <- x shift).
+    int32_t* reach;             // float16: power of two of the row's g and of its largest value
     char* shifted;              // gathered rows times shift; the gathered rows themselves otherwise
-    float *scale, *share, *shift, *common;      // inverse times g; g; 1 but in float16; a power of two
+    float *scale, *share, *shift, *common;      // inverse times g; g; 1 but in float16, there the row's power of two relative to common; a power of two
     float* column_sums;         // of D, [tiles of rows][columns]
     bool wide_dweight, later;   // later: a piece that is not the first
 };
@@ -785,20 +786,49 @@ __global__ __launch_bounds__(256) void loss_dx_sum_kernel(Loss p, Gradient g, in
     }
 }
 
-// Rows with gradients of their own.  common is the power of two of the largest; float16: a row's own power of two, relative to that, goes to x, which takes it without rounding.
+// float16: of each row the power of two of its gradient and of its largest value together, or NO_REACH where the gradient is 0, infinite or NaN.  (Of a value: -24 for the smallest and for rows of
+// zeros, 15 for the largest and where one is infinite or NaN.)  A wave to a row.
+constexpr int NO_REACH = -(1 << 20);
+__global__ __launch_bounds__(256) void loss_reach_kernel(Loss p, Gradient g) {
+    const int n = p.count[0], l = threadIdx.x & 63, w = threadIdx.x >> 6;
+    for (int r = blockIdx.x * 4 + w; r < n; r += gridDim.x * 4) {
+        const float weight = g.dloss[p.index[r] * g.dloss_stride];
+        const uint4* const from = reinterpret_cast<const uint4*>(p.gathered + r * p.pitch);
+        uint32_t most = 0;
+        for (int c = l; c < int(p.pitch / 16); c += 64) {
+            const uint4 v = from[c];
+            for (const uint32_t pair : {v.x, v.y, v.z, v.w}) most = max(most, max(pair & 0x7fff, pair >> 16 & 0x7fff));
+        }
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) most = max(most, uint32_t(__shfl_xor(int(most), d)));
+        const int value = most >= 0x7c00 ? 15 : most ? ilogbf(float(__builtin_bit_cast(_Float16, uint16_t(most)))) : -24;
+        if (l == 0) g.reach[r] = weight != 0.f && fabsf(weight) < INFINITY ? ilogbf(weight) + value : NO_REACH;
+    }
+}
+
+// Rows with gradients of their own.  float32, bfloat16: common is the power of two of the largest.  float16: a row's own power of two goes to x instead of D, relative to a common one by which the largest of all
+// g x comes to lie in [2^15, 2^16).  Up to there a power of two takes no bits; what x loses at the other end is half of float16's smallest step, 2^-25, so 2^-40 of the largest g x, where dW, in float16
+// too, holds no more than 2^-41 of float16's largest value.  (With g alone made common, x of ordinary size lost bits from 2^-14 of the largest g on and was gone at 2^-24.)  The common one is not below 2^-100, where
+// all of dx and dW are float16's 0, so that float32 holds its products for dbias.
 template <int DT>
 __global__ __launch_bounds__(256) void loss_weigh_kernel(Loss p, Gradient g) {
     using T = typename Matrix<DT>::T;
-    __shared__ float s_most[4];
+    __shared__ int s_most[4];
     const int n = p.count[0], l = threadIdx.x & 63, w = threadIdx.x >> 6;
-    float most = 0.f;
-    for (int r = threadIdx.x; r < n; r += 256) most = fmaxf(most, fabsf(g.dloss[p.index[r] * g.dloss_stride]));
+    int most = NO_REACH;
+    float largest = 0.f;
+    for (int r = threadIdx.x; r < n; r += 256) {
+        if (DT == TDB_F16) most = max(most, g.reach[r]);
+        else largest = fmaxf(largest, fabsf(g.dloss[p.index[r] * g.dloss_stride]));
+    }
+    if (DT != TDB_F16) most = __builtin_bit_cast(int, largest);         // (of positive values the larger has the larger bits)
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) most = fmaxf(most, __shfl_xor(most, d));
+    for (int d = 1; d < 64; d <<= 1) most = max(most, __shfl_xor(most, d));
     if (l == 0) s_most[w] = most;
     __syncthreads();
-    most = fmaxf(fmaxf(s_most[0], s_most[1]), fmaxf(s_most[2], s_most[3]));
-    const int common = most > 0.f && most < INFINITY ? ilogbf(most) : 0;
+    most = max(max(s_most[0], s_most[1]), max(s_most[2], s_most[3]));
+    largest = __builtin_bit_cast(float, most);
+    const int common = DT == TDB_F16 ? (most == NO_REACH ? 0 : max(most - 15, -100)) : largest > 0.f && largest < INFINITY ? ilogbf(largest) : 0;
     if (blockIdx.x == 0 && threadIdx.x == 0) *g.common = ldexpf(1.f, common);
     for (int r = blockIdx.x * 4 + w; r < n; r += gridDim.x * 4) {
         const float weight = g.dloss[p.index[r] * g.dloss_stride];
@@ -935,7 +965,7 @@ struct Plan {
     // offsets
     int64_t index, place, label, top, inverse, right, biases, gathered, state;
     int64_t maxima, sums, block_sums, forward;
-    int64_t d, parts, part_pitch, column_sums, dw_parts, shifted, scale, share, shift, common, backward;
+    int64_t d, parts, part_pitch, column_sums, dw_parts, shifted, reach, scale, share, shift, common, backward;
 };
 
 Plan plan_of(const tdb_loss_args& a) {
@@ -980,6 +1010,7 @@ Plan plan_of(const tdb_loss_args& a) {
     p.dw_parts = take(p.dw_splits > 1 ? p.dw_splits * p.vocab * p.part_pitch * 4 : 0);
     const bool weighted = a.reduction == 0;
     p.shifted = take(weighted && a.dtype == TDB_F16 ? p.padded * p.pitch : 0);
+    p.reach = take(weighted && a.dtype == TDB_F16 ? p.padded * 4 : 0);
     p.scale = take(weighted ? p.padded * 4 : 0), p.share = take(weighted ? p.padded * 4 : 0), p.shift = take(weighted ? p.padded * 4 : 0), p.common = take(4);
     p.backward = at;
     return p;
@@ -1086,8 +1117,9 @@ hipError_t backward(const tdb_loss_args& a, hipStream_t s) {
     const bool weighted = a.reduction == 0;
     auto floats = [&](int64_t at) { return reinterpret_cast<float*>(work + at); };
     g.shifted = weighted && a.dtype == TDB_F16 ? work + p.shifted : k.gathered;
-    g.scale = floats(p.scale), g.share = floats(p.share), g.shift = floats(p.shift), g.common = floats(p.common), g.column_sums = floats(p.column_sums), g.dw_parts = floats(p.dw_parts), g.dw_splits = a.dweight ? p.dw_splits : 1;
+    g.reach = reinterpret_cast<int32_t*>(work + p.reach), g.scale = floats(p.scale), g.share = floats(p.share), g.shift = floats(p.shift), g.common = floats(p.common), g.column_sums = floats(p.column_sums), g.dw_parts = floats(p.dw_parts), g.dw_splits = a.dweight ? p.dw_splits : 1;
     g.wide_dweight = reinterpret_cast<uintptr_t>(a.dweight) % 4 == 0 && g.dweight_pitch % 4 == 0;
+    if (weighted && a.rows && a.dtype == TDB_F16) TDB_TRY(launch<loss_reach_kernel>(std::min<int64_t>(p.padded / 16, 1024), 256, 0, s, k, g));
     if (weighted && a.rows) TDB_TRY(launch<loss_weigh_kernel<DT>>(std::min<int64_t>(p.padded / 16, 1024), 256, 0, s, k, g));
     for (g.first = 0; g.first < a.vocab; g.first += p.columns) {
         g.columns = std::min(p.columns, p.vocab - g.first), g.later = g.first > 0;
