@@ -105,7 +105,7 @@ int64_t tdb_attn_train_workspace(const tdb_train_attn_args* args);
  * TDB_F32): of each row whose label (64 bits) is not ignore_index the logarithm of the sum of the exponentials of its logits less the label's logit, in natural units.  The logits are
  * never in memory.  reduction 0: loss [rows], 0 where a row does not count; 1: their sum; 2: their mean over the rows that count (none: NaN).  loss is float32.
  * A label that is neither ignore_index nor in [0, vocab) makes its row's loss NaN, and every gradient that the row goes into.  Rows that do not count are not read.
- * weight: rows 4-byte aligned (so of an even stride in 16 bits) and at most 4 MiB apart.  x: rows of any stride, aligned to their values.
+ * weight: rows 4-byte aligned (so of an even stride in 16 bits) and at most 4 MiB apart.  dweight: rows at most 4 MiB apart.  x: rows of any stride, aligned to their values.
  * Forward fills `state` (tdb_loss_state() bytes), which the backward call reads; x is not read again.  Both take a workspace of tdb_loss_workspace() bytes, 16-byte aligned like
  * the state.  The backward one holds the gradient of the logits in the type of x, up to 2 GiB at a time or 256 columns of it, partial sums of dx of 1 KiB hidden for each CU or 4
  * bytes for each value of x, those of dweight of at most 256 MiB where a small vocabulary meets many rows, and without a reduction one more x.

@@ -1044,6 +1044,8 @@ int check(const tdb_loss_args* a, bool backward) {
         if (a->dbias && !a->bias) return tdb_fail(TDB_ERR_NULL, "dbias needs a bias");
         if (a->dloss_stride < 0 || (a->dx && a->rows > 1 && a->dx_stride < a->hidden) || (a->dweight && a->dweight_stride < a->hidden))
             return tdb_fail(TDB_ERR_STRIDE, "rows of a result overlap");
+        if (a->dweight && a->dweight_stride > (1 << 22) / size)        // (a tile's rows are written through one buffer, whose offsets have 32 bits)
+            return tdb_fail(TDB_ERR_STRIDE, "dweight_stride %lld: need at most 4 MiB", (long long)a->dweight_stride);
     }
     const Plan p = plan_of(*a);
     if (a->state_bytes < p.state || a->workspace_bytes < (backward ? p.backward : p.forward)) return tdb_fail(TDB_ERR_SHAPE, "state or workspace is too small");
