@@ -1030,7 +1030,7 @@ int check(const tdb_loss_args* a, bool backward) {
     if (const int rc = check_sizes(a); rc != TDB_OK) return rc;
     const int size = a->dtype == TDB_F32 ? 4 : 2;
     if (!a->weight || !a->state || !a->workspace) return tdb_fail(TDB_ERR_NULL, "weight, state and workspace must be non-NULL");
-    if (a->weight_stride * size % 4 || a->weight_stride < a->hidden || a->weight_stride * size > (1 << 22))
+    if (a->weight_stride % (4 / size) || a->weight_stride < a->hidden || a->weight_stride > (1 << 22) / size)
         return tdb_fail(TDB_ERR_STRIDE, "weight_stride %lld: need a multiple of 4 bytes, at least a row and at most 4 MiB", (long long)a->weight_stride);
     if (reinterpret_cast<uintptr_t>(a->weight) % 4) return tdb_fail(TDB_ERR_ALIGN, "weight must be 4-byte aligned");
     for (const void* t : {static_cast<const void*>(a->state), static_cast<const void*>(a->workspace)})
