@@ -73,10 +73,11 @@ def _scaled(grads, out, max_norm: float, norm: int, error_if_nonfinite: bool) ->
     """The norm; out = grads * factor.  What does not lie back to back, or not in the same order on both sides, goes through copies."""
     flat, to = [], []
     for t, o in zip(grads, out):
-        if _dense(t) and _dense(o) and t.stride() == o.stride():        # the same place in memory is the same value on both sides
+        if _dense(t) and _dense(o) and t.stride() == o.stride() and t.is_neg() == o.is_neg():       # the same place in memory is the same value on both sides
             flat.append(t), to.append(o)
         else:                                                           # by way of contiguous ones, on either side that is not
-            flat.append(t.contiguous()), to.append(o if o is not t and o.is_contiguous() else torch.empty(o.shape, dtype=o.dtype, device=o.device))
+            flat.append(t.resolve_neg().contiguous())
+            to.append(o if o is not t and o.is_contiguous() and not o.is_neg() else torch.empty(o.shape, dtype=o.dtype, device=o.device))
     a, total, keep = _norm(flat, norm)
     if error_if_nonfinite and not bool(torch.isfinite(total)):
         raise RuntimeError(f"the norm of the gradients is {total.item()}: nothing is clipped")

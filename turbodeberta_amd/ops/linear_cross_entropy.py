@@ -18,13 +18,13 @@ _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 
 def _as_rows(x: torch.Tensor) -> torch.Tensor:
     """``[rows, hidden]``, columns side by side; a view where there is one."""
-    x = x.reshape(-1, x.shape[-1])
+    x = x.resolve_neg().reshape(-1, x.shape[-1])
     return x if (x.shape[1] == 1 or x.stride(1) == 1) and x.stride(0) >= 0 else x.contiguous()
 
 
 def _weight_rows(w: torch.Tensor) -> torch.Tensor:
     """Rows that the kernels can address: values side by side, at multiples of 4 bytes; a copy where they are not."""
-    es = w.element_size()
+    w, es = w.resolve_neg(), w.element_size()
     apart = w.shape[1] if w.shape[0] == 1 else w.stride(0)
     if (w.shape[1] == 1 or w.stride(1) == 1) and w.data_ptr() % 4 == 0 and w.shape[1] <= apart and (apart * es) % 4 == 0 and apart * es <= 1 << 22:
         return w
@@ -51,7 +51,7 @@ def _call(fn, a: _lib.LossArgs, state: torch.Tensor, backward: int) -> None:
 class _Loss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, labels, bias, ignore_index, reduction):
-        rows, w, b, y = _as_rows(x), _weight_rows(weight), None if bias is None else bias.contiguous(), labels.contiguous()
+        rows, w, b, y = _as_rows(x), _weight_rows(weight), None if bias is None else bias.resolve_neg().contiguous(), labels.resolve_neg().contiguous()
         loss = torch.empty(labels.shape if reduction == 0 else (), dtype=torch.float32, device=x.device)
         a = _arguments(w, b, labels.numel(), x.shape[-1], ignore_index, reduction)
         a.x, a.x_stride, a.labels, a.loss = rows.data_ptr(), rows.stride(0), y.data_ptr(), loss.data_ptr()
@@ -66,10 +66,10 @@ class _Loss(torch.autograd.Function):
     def backward(ctx, dloss):
         _lib.host().backward_begins()
         weight, bias, state = ctx.saved_tensors
-        w, b = _weight_rows(weight), None if bias is None else bias.contiguous()
+        w, b = _weight_rows(weight), None if bias is None else bias.resolve_neg().contiguous()
         hidden = ctx.shape[-1]
         a = _arguments(w, b, ctx.rows, hidden, ctx.ignore_index, ctx.reduction)
-        dloss = dloss.float()
+        dloss = dloss.float().resolve_neg()
         if ctx.reduction == 0:
             dloss = dloss.reshape(-1)
             if dloss.numel() > 1 and dloss.stride(0) < 0:
