@@ -94,6 +94,12 @@ template <int N>
 __device__ __forceinline__ void wait_loads() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
+// Behind the last products of a tile: all wait states that one of them may need (12; 16 of them), on every path.  Paths join here, and the compiler follows one of them back to the products (see tdb_settled).
+__device__ __forceinline__ void settle() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop 7\n\ts_nop 7" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
 __device__ __forceinline__ void step_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 constexpr uint32_t PAST = 0x80000000u;      // past every buffer's end
@@ -330,6 +336,7 @@ struct Product {
                 products(flow, stage, acc);
                 stage ^= 1;
             }
+            settle();
         } else {
             // The frags of a quarter of a step are read while the products of the one before it are made, each of which keeps the matrix pipe busy for 32 clk; the barrier lies in front of a
             // step's last quarter, whose frags are in registers by then, and with that quarter the loads of the step after the next one are issued.
