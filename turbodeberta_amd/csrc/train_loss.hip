@@ -43,7 +43,7 @@ __device__ __forceinline__ int tile_rows(int n, int least, uint32_t wide, uint32
     return best;
 }
 
-// float16: D lies in [-2^14, 2^14], so that probabilities down to 2^-38 are told from 0 (2^-24 without).
+// float16: D lies in [-2^14, 2^14] (twice that with gradients of the rows' own), so that probabilities down to 2^-38 are told from 0 (2^-24 without).
 template <int DT>
 constexpr float D_SCALE = DT == TDB_F16 ? 16384.f : 1.f;
 
@@ -472,7 +472,7 @@ struct Gradient {
     // D, [padded rows][columns of a piece], of x's type: a matrix instruction takes both operands in one.  So it is rounded, by half a step of the type at most, and that is the largest error of 16-bit gradients
     // beside their own rounding.  Against 64 bits, relative to the norm, bfloat16: 2458 rows x 768, 128100 classes, dx and dW 1.9e-3, from D in float32 1.7e-3; 512 rows with gradients of their own, 30011 classes,
     // 2.3e-3 and 1.7e-3; float16 2.5e-4 to 4.1e-4, and 2.0e-4 to 3.7e-4.  What that saves: D as a sum of two values takes both products twice (8192 x 1024, 128100 classes: 3.8 ms on 7.9) and twice the workspace, in
-    // float32 instructions an eighth of the rate.  Sums over D, of dx, dW and dbias, are of float32, dbias from D before it is rounded.
+    // float32 instructions a tenth of the rate.  Sums over D, of dx, dW and dbias, are of float32, dbias from D before it is rounded.
     char* d;
     int64_t d_pitch;
     int64_t first, columns;     // of the piece (columns a multiple of TILE)
